@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define MOE_HIP_ABI_VERSION 2   /* 2: router weight gradient, static-scratch sort, stage-timer selection, moe_combine with k = 0; fp16 on the matrix cores (dtype argument of moe_mlp_fwd / moe_mlp_bwd) */
+#define MOE_HIP_ABI_VERSION 3   /* 3: expert products in 8-bit integers; 2: router weight gradient, static-scratch sort, stage-timer selection, moe_combine with k = 0; fp16 on the matrix cores (dtype argument of moe_mlp_fwd / moe_mlp_bwd) */
 
 #define MOE_OK 0
 #define MOE_ERR_BAD_ARG (-1)      /* inconsistent sizes / null pointers */
@@ -249,6 +249,48 @@ int moe_mlp_bwd(const void* dy, int64_t lddy, int dy_grouped, int dy_fan_out, co
                 int64_t lddx, int dx_grouped, const void* pos, int pos64, const void* offsets, int off64, int E,
                 int64_t R, int64_t d, int64_t f, int fan_out, int dtype, const void* saved, void* workspace,
                 size_t workspace_bytes, void* stream);
+
+/* ---- expert products in 8-bit integers (no counterpart in the reference) --------------------------------------
+ * Codes are signed 8-bit integers with a fp32 scale: of a row for activations and gradients, of an expert's output column for weights.  A row v becomes
+ * codes[c] = rne(127 v[c] / a), a = max |v| (the exact quotient, ties to even), scale = a / 127; a row of zeros gets the scale 0, a row that holds an
+ * infinity or a NaN the scale NaN and codes 0, which makes every product of it NaN.  Sums of products are exact (K < 2^17, else MOE_ERR_UNSUPPORTED);
+ * their values do not depend on the order or number of launches.
+ *
+ * moe_quantize_rows: row m of the codes (pitch ldc >= ncols, a multiple of 16, 16-byte aligned; columns from ncols on are written as zeros) is row m of
+ * src, or with pos row pos[m] / fan_out; times coeff[pos[m]] (coeff[m] without pos) and, column by column, col_scale[e][c] of the expert e that grouped
+ * row m belongs to (offsets, E; a row behind the last group is left as it was).  fp32 rows are worked through in 64 bits.
+ * Products read the codes of a row up to the next multiple of 128 columns: ldc at least that. */
+int moe_quantize_rows(const void* src, int64_t lds, int dtype, const void* pos, int pos64, int fan_out, const void* coeff, int coeff_dtype,
+                      const float* col_scale, const void* offsets, int off64, int E, int8_t* codes, int64_t ldc, float* scale, int64_t nrows,
+                      int64_t ncols, void* stream);
+/* weights (E,K,N) of any strides -> codes (E,K,N) of any strides and scale (E,N), the maximum taken over K */
+size_t moe_quantize_weights_workspace_bytes(int E, int64_t N);
+int moe_quantize_weights(const void* W, int64_t swe, int64_t swk, int64_t swn, int dtype, int E, int64_t K, int64_t N, int8_t* codes, int64_t sce,
+                         int64_t sck, int64_t scn, float* scale, void* workspace, size_t workspace_bytes, void* stream);
+/* moe_scatter2scatter without adapters, of codes:  Y[out_row] = x_scale[in_row] * w_scale[e][n] * (X[in_row] @ W[e]).
+ * X: codes as moe_quantize_rows writes them, zeros from K to the next multiple of 128 (ldx at least that, a multiple of 16); W (E,K,N) of any strides -- read
+ * in place where contiguous along K or N with the other strides and the address multiples of 16, otherwise through a copy in the workspace;
+ * w_scale (E,N) or NULL (1); Y of `dtype` with unit column stride.  For a gradient X holds the codes of dY * w_scale, W its transposed view, w_scale NULL. */
+size_t moe_scatter2scatter_int8_workspace_bytes(const int8_t* W, int64_t swe, int64_t swk, int64_t swn, int64_t R, int E, int64_t K, int64_t N);
+int moe_scatter2scatter_int8(const int8_t* X, int64_t ldx, const float* x_scale, const int8_t* W, int64_t swe, int64_t swk, int64_t swn,
+                             const float* w_scale, void* Y, int64_t ldy, int dtype, const void* pos, int pos64, const void* offsets, int off64, int E,
+                             int64_t R, int64_t K, int64_t N, int fan_out, int x_grouped, int y_grouped, void* workspace, size_t workspace_bytes,
+                             void* stream);
+/* The expert MLP of moe_mlp_fwd / moe_mlp_bwd over 8-bit weights: w1, w3, w2 codes (E,f,d) contiguous, scales s1, s3 (E,f) and s2 (E,d); bf16 or fp16 x, y, dy, dx;
+ * d and f multiples of 64.  x has x_rows rows; row m of the order is row pos[m] / fan_out of them.
+ * Forward:  gate, up = codes(x) W1, codes(x) W3;  h = silu(gate) * up;  y[out_row] = codes(h) W2.  `saved` (or NULL): gate and up for the backward pass.
+ * Backward (weights frozen, the codes' rounding straight through), dy rows addressed and weighted as in moe_mlp_bwd, gates one weight per flat position or NULL:
+ *   dh = codes(gates dy s2) W2^T;  dgate, dup from SwiGLU;  dx_rows[pos[m]] = codes([dgate s1 | dup s3]) [W1; W3], one scale for the joint row. */
+size_t moe_mlp_int8_saved_bytes(int64_t R, int64_t f);
+size_t moe_mlp_int8_workspace_bytes(int64_t R, int64_t x_rows, int E, int64_t d, int64_t f, int backward);
+int moe_mlp_int8_fwd(const void* x, int64_t ldx, int64_t x_rows, int dtype, const int8_t* w1, const float* s1, const int8_t* w3, const float* s3,
+                     const int8_t* w2, const float* s2, void* y, int64_t ldy, const void* pos, int pos64, const void* offsets, int off64, int E,
+                     int64_t R, int64_t d, int64_t f, int fan_out, int y_grouped, void* saved, size_t saved_bytes, void* workspace,
+                     size_t workspace_bytes, void* stream);
+int moe_mlp_int8_bwd(const void* dy, int64_t lddy, int dtype, int dy_grouped, int dy_fan_out, const void* gates, int gates_dtype, const int8_t* w1,
+                     const float* s1, const int8_t* w3, const float* s3, const int8_t* w2, const float* s2, const void* saved, size_t saved_bytes,
+                     void* dx_rows, int64_t lddx, const void* pos, int pos64, const void* offsets, int off64, int E, int64_t R, int64_t d, int64_t f,
+                     void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

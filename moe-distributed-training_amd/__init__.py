@@ -9,17 +9,21 @@ machine without that library raises immediately -- there is no host fallback.
 from . import _lib  # noqa: F401
 from .scattermoe_utils.kernels.ops import (  # noqa: F401
     flatten_and_sort, padded_block_indices, scatter2scatter, scatter2scatter_lora, group, group_bwd_AB, group_bwd_W,
+    quantize_rows,
 )
 from .scattermoe_utils.parallel_linear_lora import ParallelLinearLora, parallel_linear_lora  # noqa: F401
 from .scattermoe_utils.parallel_experts import ParallelLinear, parallel_linear, ParallelExperts  # noqa: F401
+from .scattermoe_utils.parallel_linear_int8 import parallel_linear_int8, quantize_expert_weights  # noqa: F401
 from .megablocks_utils.router import forward_router, route_and_sort  # noqa: F401
 from .megablocks_utils.moe_mlp import (  # noqa: F401
     scattermoe_permute_and_compute, fused_expert_mlp, moe_layer_forward, ScatterMoEBlock,
+    Int8ExpertWeights, fused_expert_mlp_int8, moe_layer_forward_int8,
 )
 
 __all__ = [
     "flatten_and_sort", "padded_block_indices", "scatter2scatter", "scatter2scatter_lora", "group", "group_bwd_AB",
     "group_bwd_W", "ParallelLinearLora", "parallel_linear_lora", "ParallelLinear", "parallel_linear",
     "ParallelExperts", "forward_router", "route_and_sort", "scattermoe_permute_and_compute", "fused_expert_mlp",
-    "moe_layer_forward", "ScatterMoEBlock",
+    "moe_layer_forward", "ScatterMoEBlock", "quantize_rows", "quantize_expert_weights", "parallel_linear_int8",
+    "Int8ExpertWeights", "fused_expert_mlp_int8", "moe_layer_forward_int8",
 ]

@@ -10,7 +10,7 @@ import torch
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libmoe_hip.so")
 
-ABI_VERSION = 2   # MOE_HIP_ABI_VERSION of include/moe_hip.h this binding was written against
+ABI_VERSION = 3   # MOE_HIP_ABI_VERSION of include/moe_hip.h this binding was written against
 MOE_BF16, MOE_F16, MOE_F32 = 0, 1, 2
 _DTYPES = {torch.bfloat16: MOE_BF16, torch.float16: MOE_F16, torch.float32: MOE_F32}
 
@@ -62,6 +62,15 @@ _SIGNATURES = {
     "moe_mlp_saved_bytes": ("z", "li"),
     "moe_mlp_fwd": ("i", "pl" + "ppp" + "pp" + "if" + "pppp" + "l" + "pi" + "pi" + "i" + "lll" + "iii" + "p" + "pzp"),
     "moe_mlp_bwd": ("i", "plii" + "p" + "pl" + "ppp" + "pp" + "pp" + "if" + "ppp" + "pp" + "pli" + "pi" + "pi" + "i" + "lll" + "ii" + "p" + "pzp"),
+    "moe_quantize_rows": ("i", "pli" + "pii" + "pi" + "ppii" + "plp" + "ll" + "p"),
+    "moe_quantize_weights_workspace_bytes": ("z", "il"),
+    "moe_quantize_weights": ("i", "plll" + "iill" + "plll" + "p" + "pzp"),
+    "moe_scatter2scatter_int8_workspace_bytes": ("z", "plll" + "lill"),
+    "moe_scatter2scatter_int8": ("i", "plp" + "plll" + "p" + "pli" + "pi" + "pi" + "i" + "lll" + "iii" + "pzp"),
+    "moe_mlp_int8_saved_bytes": ("z", "ll"),
+    "moe_mlp_int8_workspace_bytes": ("z", "llilli"),
+    "moe_mlp_int8_fwd": ("i", "plli" + "pppppp" + "pl" + "pi" + "pi" + "i" + "lll" + "ii" + "pz" + "pzp"),
+    "moe_mlp_int8_bwd": ("i", "pliii" + "pi" + "pppppp" + "pz" + "pl" + "pi" + "pi" + "i" + "lll" + "pzp"),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

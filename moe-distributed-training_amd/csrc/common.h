@@ -5,6 +5,7 @@
 #include <hip/hip_fp16.h>
 #include <stdint.h>
 #include <atomic>
+#include <type_traits>
 
 // status codes returned by every C-ABI entry point (see include/moe_hip.h)
 #define MOE_OK 0

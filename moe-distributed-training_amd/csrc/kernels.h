@@ -211,3 +211,62 @@ int moe_launch_combine_dgates(const void* y, int64_t ldy, const void* dout, int6
 int moe_launch_swiglu_fwd(const void* g, const void* u, void* h, int64_t n, int dtype, hipStream_t stream);
 int moe_launch_swiglu_bwd(const void* g, const void* u, const void* dh, void* dg, void* du, int64_t n, int dtype,
                           hipStream_t stream);
+
+// ---- expert products in 8-bit integers (int8_rows.hip, int8_gemm.hip)
+constexpr int MOE_SEG_COLS = 32;        // columns that share a scale in the 16-bit interims
+constexpr int MOE_I8_KTILE = 128;       // codes of a row come in whole K tiles, zeros behind the last column
+constexpr int64_t MOE_I8_MAX_K = 131071;   // 128 * 128 * K < 2^31: the sums are exact in 32 bits
+inline int64_t moe_i8_pitch(int64_t cols) { return (cols + MOE_I8_KTILE - 1) / MOE_I8_KTILE * MOE_I8_KTILE; }
+
+// codes[m][c] and scale[m] of rows m: src row m, or with any of pos, coeff, col_scale: src row pos[m] / fan_out times coeff[pos[m]] (m without pos) and
+// col_scale[expert of m][c]; ldc: pitch of the codes, zeros from column cols on
+struct MoeQuantizeRows {
+    const void* src; int64_t lds;
+    const void* pos; int pos64; int fan_out;
+    const void* coeff; int coeff_dtype;
+    const float* col_scale; const void* offsets; int off64; int E;
+    int8_t* codes; int64_t ldc; float* scale;
+    int64_t cols;
+    int vec;                // (set by the launcher) rows of src are 16-byte aligned
+};
+int moe_launch_quantize_rows(const MoeQuantizeRows& p, int dtype, int64_t rows, hipStream_t stream);
+int moe_launch_requantize_rows(const int16_t* src, const float* seg, int64_t rows, int64_t cols, int8_t* codes, int64_t ldc, float* scale, hipStream_t stream);
+// codes [rows][2 * ldc] of the joint rows [dgate * s1 | dup * s3]; dh, gate, up: [rows][f] with their segments' scales [rows][f / MOE_SEG_COLS]
+struct MoeSwigluBwdCodes {
+    const int16_t *dh, *gate, *up;
+    const float *dh_seg, *gate_seg, *up_seg;
+    const float *s1, *s3;   // [E][f]
+    const void* offsets; int off64; int E;
+    int8_t* codes; int64_t ldc; float* scale;
+    int64_t f;
+};
+int moe_launch_swiglu_bwd_codes(const MoeSwigluBwdCodes& p, int64_t rows, hipStream_t stream);
+int moe_launch_pack_codes(const int8_t* W, int64_t swe, int64_t swk, int64_t swn, int E, int64_t K, int64_t N, int8_t* out, int64_t ldo, hipStream_t stream);
+int moe_launch_quantize_weights(const void* W, int64_t swe, int64_t swk, int64_t swn, int dtype, int E, int64_t K, int64_t N, int8_t* codes, int64_t sce,
+                                int64_t sck, int64_t scn, float* scale, uint32_t* top, hipStream_t stream);
+
+// epilogues of the 8-bit grouped product
+#define MOE_I8_STORE 0      // Y = acc * x_scale * w_scale in ydtype
+#define MOE_I8_SEG 1        // the same as 16-bit integers with segment scales (grouped rows)
+#define MOE_I8_SWIGLU 2     // weight pair (gate, up): S[0] = silu(gate) * up and, where given, S[1] = gate, S[2] = up, as segments
+
+struct MoeI8Gemm {
+    const int8_t* X; int64_t ldx;       // codes: rows of nseg times moe_i8_pitch(K), zeros behind every segment's K
+    const float* x_scale;               // per row of X
+    const int8_t* W[2];                 // nseg == 2: the second K segment's matrices; MOE_I8_SWIGLU: gate and up
+    int64_t swe, ldw;                   // expert stride; nn == 0: stride between n rows (k contiguous), nn == 1: between k rows (n contiguous)
+    int nn, nseg;
+    const float* w_scale[2];            // [E][N], or null (1); [1]: up
+    void* Y; int64_t ldy; int ydtype;
+    int16_t* S[3]; float* SS[3];        // segment outputs [R][N] and their scales [R][N / MOE_SEG_COLS]
+    const void* pos; int pos64; const void* offsets; int off64;
+    int E; int64_t K, N;                // K: of one segment
+    int fan_out, x_grouped, y_grouped, epi;
+    void* exchange;
+};
+// whether the kernel reads W in this orientation and alignment (otherwise: moe_launch_pack_codes first)
+bool moe_i8_weights_ok(const void* W, int64_t swe, int64_t ldw);
+// whether sizes stay inside the kernel's 32-bit offsets (x_rows: rows of X)
+bool moe_i8_gemm_supported(const MoeI8Gemm& p, int64_t R, int64_t x_rows);
+size_t moe_i8_exchange_bytes(int64_t R, int E, int64_t K, int64_t N, bool pair);   // K: all segments
+int moe_launch_i8_gemm(const MoeI8Gemm& p, int64_t R, hipStream_t stream);

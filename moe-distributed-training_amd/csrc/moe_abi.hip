@@ -1040,4 +1040,195 @@ int moe_mlp_bwd(const void* dy, int64_t lddy, int dy_grouped, int dy_fan_out, co
     return MOE_OK;
 }
 
+// ---- expert products in 8-bit integers -------------------------------------------------------------------------
+int moe_quantize_rows(const void* src, int64_t lds, int dtype, const void* pos, int pos64, int fan_out, const void* coeff, int coeff_dtype,
+                      const float* col_scale, const void* offsets, int off64, int E, int8_t* codes, int64_t ldc, float* scale, int64_t nrows,
+                      int64_t ncols, void* stream)
+{
+    if (dtype < 0 || dtype > 2 || nrows < 0 || ncols < 0 || ldc < ncols || ldc % 16 != 0) return MOE_ERR_BAD_ARG;
+    if (nrows == 0) return MOE_OK;
+    if (!src || !codes || !scale || !aligned16(codes) || (pos && fan_out < 1) || (coeff && (coeff_dtype < 0 || coeff_dtype > 2)) || (col_scale && (!offsets || E < 1))) return MOE_ERR_BAD_ARG;
+    if (nrows > 0x7fffffff) return MOE_ERR_UNSUPPORTED;
+    const MoeQuantizeRows q = {src, lds, pos, pos64, fan_out, coeff, coeff_dtype, col_scale, offsets, off64, E, codes, ldc, scale, ncols, 0};
+    return moe_launch_quantize_rows(q, dtype, nrows, S(stream));
+}
+
+size_t moe_quantize_weights_workspace_bytes(int E, int64_t N) { return E < 1 || N < 1 ? 0 : (size_t)E * (size_t)N * 4; }
+
+int moe_quantize_weights(const void* W, int64_t swe, int64_t swk, int64_t swn, int dtype, int E, int64_t K, int64_t N, int8_t* codes, int64_t sce,
+                         int64_t sck, int64_t scn, float* scale, void* workspace, size_t workspace_bytes, void* stream)
+{
+    if (dtype < 0 || dtype > 2 || E < 1 || K < 1 || N < 1 || !W || !codes || !scale) return MOE_ERR_BAD_ARG;
+    if (E > 65535 || K > 65535 * (int64_t)16 || N > 65535 * (int64_t)16) return MOE_ERR_UNSUPPORTED;
+    if (!workspace || workspace_bytes < moe_quantize_weights_workspace_bytes(E, N)) return MOE_ERR_WORKSPACE;
+    return moe_launch_quantize_weights(W, swe, swk, swn, dtype, E, K, N, codes, sce, sck, scn, scale, (uint32_t*)workspace, S(stream));
+}
+
+namespace {
+// the weights of a product as its kernel reads them: in place (contiguous along k or along n, 16-byte aligned rows), or a copy contiguous along k
+struct I8Weights { bool in_place; int nn; int64_t swe, ldw; size_t bytes; };
+I8Weights i8_weights(const void* W, int64_t swe, int64_t swk, int64_t swn, int E, int64_t K, int64_t N)
+{
+    if (swk == 1 && moe_i8_weights_ok(W, swe, swn)) return {true, 0, swe, swn, 0};
+    if (swn == 1 && moe_i8_weights_ok(W, swe, swk)) return {true, 1, swe, swk, 0};
+    const int64_t ld = (K + 15) / 16 * 16;
+    return {false, 0, N * ld, ld, al((size_t)E * (size_t)N * (size_t)ld)};
+}
+}  // namespace
+
+size_t moe_scatter2scatter_int8_workspace_bytes(const int8_t* W, int64_t swe, int64_t swk, int64_t swn, int64_t R, int E, int64_t K, int64_t N)
+{
+    if (R < 1 || E < 1 || K < 1 || N < 1) return 0;
+    return i8_weights(W, swe, swk, swn, E, K, N).bytes + moe_i8_exchange_bytes(R, E, K, N, false);
+}
+
+int moe_scatter2scatter_int8(const int8_t* X, int64_t ldx, const float* x_scale, const int8_t* W, int64_t swe, int64_t swk, int64_t swn,
+                             const float* w_scale, void* Y, int64_t ldy, int dtype, const void* pos, int pos64, const void* offsets, int off64, int E,
+                             int64_t R, int64_t K, int64_t N, int fan_out, int x_grouped, int y_grouped, void* workspace, size_t workspace_bytes,
+                             void* stream)
+{
+    hipStream_t st = S(stream);
+    if (dtype < 0 || dtype > 2 || E < 1 || R < 0 || K < 1 || N < 0 || fan_out < 1 || ldx < moe_i8_pitch(K) || ldx % 16 != 0 || ldy < N) return MOE_ERR_BAD_ARG;
+    if (R == 0 || N == 0) return MOE_OK;
+    if (!X || !x_scale || !W || !Y || !offsets || !aligned16(X) || ((!x_grouped || !y_grouped) && !pos)) return MOE_ERR_BAD_ARG;
+    if (K > MOE_I8_MAX_K || E > 65535) return MOE_ERR_UNSUPPORTED;
+    const I8Weights w = i8_weights(W, swe, swk, swn, E, K, N);
+    if (!workspace || workspace_bytes < moe_scatter2scatter_int8_workspace_bytes(W, swe, swk, swn, R, E, K, N)) return MOE_ERR_WORKSPACE;
+    Bump b(workspace, workspace_bytes);
+    MoeI8Gemm g = {};
+    g.X = X; g.ldx = ldx; g.x_scale = x_scale;
+    g.W[0] = W; g.swe = w.swe; g.ldw = w.ldw; g.nn = w.nn; g.nseg = 1; g.w_scale[0] = w_scale;
+    g.Y = Y; g.ldy = ldy; g.ydtype = dtype;
+    g.pos = pos; g.pos64 = pos64; g.offsets = offsets; g.off64 = off64; g.E = E; g.K = K; g.N = N;
+    g.fan_out = fan_out; g.x_grouped = x_grouped; g.y_grouped = y_grouped; g.epi = MOE_I8_STORE;
+    int8_t* packed = w.in_place ? nullptr : (int8_t*)b.take(w.bytes);
+    g.exchange = b.take(moe_i8_exchange_bytes(R, E, K, N, false));
+    if (packed) g.W[0] = packed;
+    if (!moe_i8_gemm_supported(g, R, (R + fan_out - 1) / fan_out)) return MOE_ERR_UNSUPPORTED;
+    if (packed) { TIMED("i8_pack"); TRY(moe_launch_pack_codes(W, swe, swk, swn, E, K, N, packed, w.ldw, st)); }
+    TIMED("i8_gemm");
+    return moe_launch_i8_gemm(g, R, st);
+}
+
+namespace {
+struct I8Seg { int16_t* v; float* s; };
+inline size_t i8_seg_bytes(int64_t R, int64_t N) { return al((size_t)R * N * 2) + al((size_t)R * (N / MOE_SEG_COLS) * 4); }
+inline I8Seg take_seg(Bump& b, int64_t R, int64_t N)
+{
+    I8Seg s;
+    s.v = (int16_t*)b.take((size_t)R * N * 2);
+    s.s = (float*)b.take((size_t)R * (N / MOE_SEG_COLS) * 4);
+    return s;
+}
+inline size_t i8_codes_bytes(int64_t rows, int64_t pitch) { return al((size_t)rows * pitch) + al((size_t)rows * 4); }
+inline bool i8_mlp_sizes_ok(int64_t d, int64_t f) { return d >= 64 && f >= 64 && d % 64 == 0 && f % 64 == 0; }
+}  // namespace
+
+size_t moe_mlp_int8_saved_bytes(int64_t R, int64_t f) { return R < 1 || f < 64 ? 0 : 2 * i8_seg_bytes(R, f); }
+
+size_t moe_mlp_int8_workspace_bytes(int64_t R, int64_t x_rows, int E, int64_t d, int64_t f, int backward)
+{
+    if (R < 1 || x_rows < 1 || E < 1 || !i8_mlp_sizes_ok(d, f)) return 0;
+    const size_t h = i8_seg_bytes(R, f);
+    if (!backward) {
+        const size_t xa = moe_i8_exchange_bytes(R, E, d, f, true), xb = moe_i8_exchange_bytes(R, E, f, d, false);
+        return i8_codes_bytes(x_rows, moe_i8_pitch(d)) + h + i8_codes_bytes(R, moe_i8_pitch(f)) + (xa > xb ? xa : xb);
+    }
+    const size_t xa = moe_i8_exchange_bytes(R, E, d, f, false), xb = moe_i8_exchange_bytes(R, E, 2 * moe_i8_pitch(f), d, false);
+    return i8_codes_bytes(R, moe_i8_pitch(d)) + h + i8_codes_bytes(R, 2 * moe_i8_pitch(f)) + (xa > xb ? xa : xb);
+}
+
+int moe_mlp_int8_fwd(const void* x, int64_t ldx, int64_t x_rows, int dtype, const int8_t* w1, const float* s1, const int8_t* w3, const float* s3,
+                     const int8_t* w2, const float* s2, void* y, int64_t ldy, const void* pos, int pos64, const void* offsets, int off64, int E,
+                     int64_t R, int64_t d, int64_t f, int fan_out, int y_grouped, void* saved, size_t saved_bytes, void* workspace,
+                     size_t workspace_bytes, void* stream)
+{
+    hipStream_t st = S(stream);
+    if (dtype < 0 || dtype > 2 || E < 1 || R < 0 || x_rows < 0 || d < 1 || f < 1 || fan_out < 1 || ldx < d || ldy < d) return MOE_ERR_BAD_ARG;
+    if (R == 0) return MOE_OK;
+    if (!x || x_rows < 1 || !w1 || !s1 || !w3 || !s3 || !w2 || !s2 || !y || !pos || !offsets) return MOE_ERR_BAD_ARG;
+    if (dtype == MOE_F32 || !i8_mlp_sizes_ok(d, f) || d > MOE_I8_MAX_K || f > MOE_I8_MAX_K || E > 65535 || x_rows > 0x7fffffff || R > 0x7fffffff) return MOE_ERR_UNSUPPORTED;
+    if (!aligned16(w1) || !aligned16(w3) || !aligned16(w2)) return MOE_ERR_UNSUPPORTED;
+    if (saved && saved_bytes < moe_mlp_int8_saved_bytes(R, f)) return MOE_ERR_WORKSPACE;
+    if (!workspace || workspace_bytes < moe_mlp_int8_workspace_bytes(R, x_rows, E, d, f, 0)) return MOE_ERR_WORKSPACE;
+    Bump b(workspace, workspace_bytes), sv(saved, saved ? saved_bytes : 0);
+    const int64_t dp = moe_i8_pitch(d), fp = moe_i8_pitch(f);
+    int8_t* xq = (int8_t*)b.take((size_t)x_rows * dp);
+    float* xs = (float*)b.take((size_t)x_rows * 4);
+    const I8Seg h = take_seg(b, R, f);
+    int8_t* hq = (int8_t*)b.take((size_t)R * fp);
+    float* hs = (float*)b.take((size_t)R * 4);
+    void* exchange = b.base + b.used;
+    I8Seg gate = {}, up = {};
+    if (saved) { gate = take_seg(sv, R, f); up = take_seg(sv, R, f); }
+
+    MoeI8Gemm g = {};
+    g.X = xq; g.ldx = dp; g.x_scale = xs;
+    g.W[0] = w1; g.W[1] = w3; g.swe = f * d; g.ldw = d; g.nn = 0; g.nseg = 1;
+    g.w_scale[0] = s1; g.w_scale[1] = s3;
+    g.S[0] = h.v; g.SS[0] = h.s; g.S[1] = gate.v; g.SS[1] = gate.s; g.S[2] = up.v; g.SS[2] = up.s;
+    g.pos = pos; g.pos64 = pos64; g.offsets = offsets; g.off64 = off64; g.E = E; g.K = d; g.N = f;
+    g.fan_out = fan_out; g.x_grouped = 0; g.y_grouped = 1; g.epi = MOE_I8_SWIGLU; g.exchange = exchange;
+    MoeI8Gemm g2 = {};
+    g2.X = hq; g2.ldx = fp; g2.x_scale = hs;
+    g2.W[0] = w2; g2.swe = f * d; g2.ldw = d; g2.nn = 1; g2.nseg = 1; g2.w_scale[0] = s2;
+    g2.Y = y; g2.ldy = ldy; g2.ydtype = dtype;
+    g2.pos = pos; g2.pos64 = pos64; g2.offsets = offsets; g2.off64 = off64; g2.E = E; g2.K = f; g2.N = d;
+    g2.fan_out = 1; g2.x_grouped = 1; g2.y_grouped = y_grouped; g2.epi = MOE_I8_STORE; g2.exchange = exchange;
+    if (!moe_i8_gemm_supported(g, R, x_rows) || !moe_i8_gemm_supported(g2, R, R)) return MOE_ERR_UNSUPPORTED;
+
+    const MoeQuantizeRows q = {x, ldx, nullptr, 0, 1, nullptr, 0, nullptr, nullptr, 0, 0, xq, dp, xs, d, 0};
+    { TIMED("i8_codes_x"); TRY(moe_launch_quantize_rows(q, dtype, x_rows, st)); }
+    { TIMED("i8_gemm_gate_up"); TRY(moe_launch_i8_gemm(g, R, st)); }
+    { TIMED("i8_codes_h"); TRY(moe_launch_requantize_rows(h.v, h.s, R, f, hq, fp, hs, st)); }
+    TIMED("i8_gemm_down");
+    return moe_launch_i8_gemm(g2, R, st);
+}
+
+int moe_mlp_int8_bwd(const void* dy, int64_t lddy, int dtype, int dy_grouped, int dy_fan_out, const void* gates, int gates_dtype, const int8_t* w1,
+                     const float* s1, const int8_t* w3, const float* s3, const int8_t* w2, const float* s2, const void* saved, size_t saved_bytes,
+                     void* dx_rows, int64_t lddx, const void* pos, int pos64, const void* offsets, int off64, int E, int64_t R, int64_t d, int64_t f,
+                     void* workspace, size_t workspace_bytes, void* stream)
+{
+    hipStream_t st = S(stream);
+    if (dtype < 0 || dtype > 2 || E < 1 || R < 0 || d < 1 || f < 1 || dy_fan_out < 1 || lddy < d || lddx < d || (gates && (gates_dtype < 0 || gates_dtype > 2 || dy_grouped))) return MOE_ERR_BAD_ARG;
+    if (R == 0) return MOE_OK;
+    if (!dy || !w1 || !s1 || !w3 || !s3 || !w2 || !s2 || !saved || !dx_rows || !pos || !offsets) return MOE_ERR_BAD_ARG;
+    if (dtype == MOE_F32 || !i8_mlp_sizes_ok(d, f) || d > MOE_I8_MAX_K || 2 * f > MOE_I8_MAX_K || E > 65535 || R > 0x7fffffff) return MOE_ERR_UNSUPPORTED;
+    if (!aligned16(w1) || !aligned16(w3) || !aligned16(w2)) return MOE_ERR_UNSUPPORTED;
+    if (saved_bytes < moe_mlp_int8_saved_bytes(R, f)) return MOE_ERR_WORKSPACE;
+    if (!workspace || workspace_bytes < moe_mlp_int8_workspace_bytes(R, R, E, d, f, 1)) return MOE_ERR_WORKSPACE;
+    Bump b(workspace, workspace_bytes), sv(const_cast<void*>(saved), saved_bytes);
+    const int64_t dp = moe_i8_pitch(d), fp = moe_i8_pitch(f);
+    int8_t* gq = (int8_t*)b.take((size_t)R * dp);
+    float* gs = (float*)b.take((size_t)R * 4);
+    const I8Seg dh = take_seg(b, R, f);
+    int8_t* aq = (int8_t*)b.take((size_t)R * 2 * fp);
+    float* as = (float*)b.take((size_t)R * 4);
+    void* exchange = b.base + b.used;
+    const I8Seg gate = take_seg(sv, R, f), up = take_seg(sv, R, f);
+
+    MoeI8Gemm g = {};   // dh = codes(gates dy s2) W2^T
+    g.X = gq; g.ldx = dp; g.x_scale = gs;
+    g.W[0] = w2; g.swe = f * d; g.ldw = d; g.nn = 0; g.nseg = 1;
+    g.S[0] = dh.v; g.SS[0] = dh.s;
+    g.pos = pos; g.pos64 = pos64; g.offsets = offsets; g.off64 = off64; g.E = E; g.K = d; g.N = f;
+    g.fan_out = 1; g.x_grouped = 1; g.y_grouped = 1; g.epi = MOE_I8_SEG; g.exchange = exchange;
+    MoeI8Gemm g2 = {};  // dx = codes(dgate s1 | dup s3) [W1; W3]
+    g2.X = aq; g2.ldx = 2 * fp; g2.x_scale = as;
+    g2.W[0] = w1; g2.W[1] = w3; g2.swe = f * d; g2.ldw = d; g2.nn = 1; g2.nseg = 2;
+    g2.Y = dx_rows; g2.ldy = lddx; g2.ydtype = dtype;
+    g2.pos = pos; g2.pos64 = pos64; g2.offsets = offsets; g2.off64 = off64; g2.E = E; g2.K = f; g2.N = d;
+    g2.fan_out = 1; g2.x_grouped = 1; g2.y_grouped = 0; g2.epi = MOE_I8_STORE; g2.exchange = exchange;
+    if (!moe_i8_gemm_supported(g, R, R) || !moe_i8_gemm_supported(g2, R, R)) return MOE_ERR_UNSUPPORTED;
+
+    const MoeQuantizeRows q = {dy, lddy, dy_grouped ? nullptr : pos, pos64, dy_fan_out, gates, gates_dtype, s2, offsets, off64, E, gq, dp, gs, d, 0};
+    const MoeSwigluBwdCodes a = {dh.v, gate.v, up.v, dh.s, gate.s, up.s, s1, s3, offsets, off64, E, aq, fp, as, f};
+    { TIMED("i8_codes_dy"); TRY(moe_launch_quantize_rows(q, dtype, R, st)); }
+    { TIMED("i8_gemm_dh"); TRY(moe_launch_i8_gemm(g, R, st)); }
+    { TIMED("i8_codes_dgate_dup"); TRY(moe_launch_swiglu_bwd_codes(a, R, st)); }
+    TIMED("i8_gemm_dx");
+    return moe_launch_i8_gemm(g2, R, st);
+}
+
 }  // extern "C"

@@ -830,6 +830,11 @@ variable_list layer(const Tensor& x, const Tensor& wg, const Tensor& w1_, const 
     return {out, rt[1], rt[2]};
 }
 
+// ---------------------------------------------------------------------------------------------------------------
+// the same products over 8-bit weights
+// ---------------------------------------------------------------------------------------------------------------
+#include "torch_int8.h"
+
 }  // namespace
 
 // Called from Python without the interpreter lock.  The wrapper carries a Python exception that is raised below (a saved-tensor
@@ -842,6 +847,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
     m.def("mlp_fast_path", torch::wrap_pybind_function(mlp_fast_path));
     m.def("expert_mlp", torch::wrap_pybind_function_no_gil(expert_mlp));
     m.def("layer", torch::wrap_pybind_function_no_gil(layer));
+    m.def("quantize_rows", torch::wrap_pybind_function_no_gil(quantize_rows));
+    m.def("quantize_weights", torch::wrap_pybind_function_no_gil(quantize_weights));
+    m.def("linear_int8", torch::wrap_pybind_function_no_gil(linear_int8));
+    m.def("expert_mlp_int8", torch::wrap_pybind_function_no_gil(expert_mlp_int8));
+    m.def("layer_int8", torch::wrap_pybind_function_no_gil(layer_int8));
 }
 
 // The same functions as dispatcher operators, for torch.jit.trace: a trace records operators, and of the functions above it
@@ -862,4 +872,16 @@ TORCH_LIBRARY(moe_hip, m)
                       at::TensorList lora, double lora_alpha, bool normalize, bool storage) {
         return layer(x, wg, w1, w2, w3, E, f, k, lora.vec(), lora_alpha, normalize, storage);
     });
+    m.def("quantize_rows", [](const Tensor& x) { return quantize_rows(x); });
+    m.def("quantize_weights", [](const Tensor& w) { return quantize_weights(w); });
+    m.def("linear_int8", [](const Tensor& x, const Tensor& W, const Tensor& scale, int64_t k, const Tensor& sei, const Tensor& ssi, const OptTensor& eo,
+                            const OptTensor& gates, bool grouped_in, bool grouped_out) {
+        return linear_int8(x, W, scale, k, sei, ssi, eo, gates, grouped_in, grouped_out);
+    });
+    m.def("expert_mlp_int8", [](const Tensor& x, const Tensor& w1, const Tensor& s1, const Tensor& w2, const Tensor& s2, const Tensor& w3, const Tensor& s3,
+                                int64_t fan_out, const Tensor& ssi, const Tensor& offsets, const OptTensor& gates, bool grouped_out) {
+        return expert_mlp_int8(x, w1, s1, w2, s2, w3, s3, fan_out, ssi, offsets, gates, grouped_out);
+    });
+    m.def("layer_int8", [](const Tensor& x, const Tensor& wg, const Tensor& w1, const Tensor& s1, const Tensor& w2, const Tensor& s2, const Tensor& w3,
+                           const Tensor& s3, int64_t k, bool normalize) { return layer_int8(x, wg, w1, s1, w2, s2, w3, s3, k, normalize); });
 }

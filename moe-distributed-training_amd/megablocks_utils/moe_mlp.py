@@ -17,6 +17,7 @@ import torch.nn as nn
 from .._lib import entry, native, require_gpu
 from ..scattermoe_utils.kernels import ops
 from ..scattermoe_utils.parallel_experts import parallel_linear
+from ..scattermoe_utils.parallel_linear_int8 import quantize_expert_weights
 from ..scattermoe_utils.parallel_linear_lora import parallel_linear_lora
 
 
@@ -65,6 +66,40 @@ def fused_expert_mlp(x, w1, w2, w3, k, sorted_scattered_idxs, expert_offsets, lo
     when ``grouped_out`` else at its flat position."""
     return entry("expert_mlp")(x, w1, w2, w3, k, sorted_scattered_idxs, expert_offsets, [] if lora is None else list(lora),
                                lora_alpha, gates, grouped_out)
+
+
+class Int8ExpertWeights(NamedTuple):
+    """Expert weights in 8 bits: codes (E, f, d) int8 in the reference's storage layout and, for each, the scales of its
+    output columns: w1 and w3 (E, f), w2 (E, d)."""
+    w1: torch.Tensor
+    w1_scale: torch.Tensor
+    w2: torch.Tensor
+    w2_scale: torch.Tensor
+    w3: torch.Tensor
+    w3_scale: torch.Tensor
+
+    @classmethod
+    def quantize(cls, w1, w2, w3, ffn_hidden_size=None, hidden_size=None):
+        """From bf16 / fp16 / fp32 weights (E, f, d), or in storage (E*f, d) with both sizes given."""
+        out = []
+        for name, w in (("w1", w1), ("w2", w2), ("w3", w3)):
+            w = resolve_dtensor(w)
+            if w.dim() == 2:
+                w = w.view(-1, ffn_hidden_size, hidden_size)
+            codes, scales = quantize_expert_weights(w if name == "w2" else w.transpose(1, 2))
+            out += [(codes if name == "w2" else codes.transpose(1, 2)).contiguous(), scales]
+        return cls(*out)
+
+
+def fused_expert_mlp_int8(x, weights: Int8ExpertWeights, k, sorted_scattered_idxs, expert_offsets,
+                          gates: Optional[torch.Tensor] = None, grouped_out: bool = False):
+    """``fused_expert_mlp`` over 8-bit weights (frozen; no adapters): x (rows, d) bf16 or fp16, d and f multiples of 64, the
+    other arguments and the result as there.  Both projections of a row work on one set of codes of it, the down projection
+    on codes of h = silu(gate) * up.  Gradients: of x and ``gates``, straight through the rounding to codes; the gradient
+    rows that meet weights are codes as well (dY times the gates and w2's scales; dgate and dup times their scales, one
+    joint row).  Every assignment has to belong to an expert."""
+    return entry("expert_mlp_int8")(x, weights.w1, weights.w1_scale, weights.w2, weights.w2_scale, weights.w3, weights.w3_scale, k,
+                                    sorted_scattered_idxs, expert_offsets, gates, grouped_out)
 
 
 def scattermoe_permute_and_compute(x, w1, w2, w3, ffn_hidden_size, hidden_size, top_k, bin_ids, indices, num_experts,
@@ -119,12 +154,26 @@ def moe_layer_forward(x, wg, w1, w2, w3, top_k=2, lora: Optional[LoraViews] = No
     return _layer(x, wg, w1, w2, w3, w1.size(0), w1.size(1), top_k, [] if lora is None else list(lora), lora_alpha, normalize, False)
 
 
+def _empty_layer(x, wg, weights, top_k):
+    """An empty batch routes nothing: empty outputs, and backward leaves every parameter's grad unset."""
+    require_gpu(x, wg, *weights)
+    return (x.clone(), torch.zeros((0, top_k), dtype=torch.float32, device=x.device),
+            torch.zeros((0, top_k), dtype=torch.int32, device=x.device))
+
+
 def _layer(x, wg, w1, w2, w3, E, f, top_k, lora, lora_alpha, normalize, storage):
-    if x.size(0) == 0:   # an empty batch routes nothing: empty outputs, and backward leaves every parameter's grad unset
-        require_gpu(x, wg, w1, w2, w3)
-        return (x.clone(), torch.zeros((0, top_k), dtype=torch.float32, device=x.device),
-                torch.zeros((0, top_k), dtype=torch.int32, device=x.device))
+    if x.size(0) == 0:
+        return _empty_layer(x, wg, (w1, w2, w3), top_k)
     return entry("layer")(x, wg, w1, w2, w3, E, f, top_k, lora, lora_alpha, bool(normalize), storage)
+
+
+def moe_layer_forward_int8(x, wg, weights: Int8ExpertWeights, top_k=2, normalize: bool = True):
+    """``moe_layer_forward`` over 8-bit expert weights: x (T, d) bf16 or fp16 -> (out (T, d), expert_weights (T, k) fp32,
+    expert_indices (T, k) int32).  Gradients: of x and the router weight wg."""
+    if x.size(0) == 0:
+        return _empty_layer(x, wg, weights, top_k)
+    return entry("layer_int8")(x, wg, weights.w1, weights.w1_scale, weights.w2, weights.w2_scale, weights.w3, weights.w3_scale, top_k,
+                               bool(normalize))
 
 
 class ScatterMoEBlock(nn.Module):
@@ -169,6 +218,26 @@ class ScatterMoEBlock(nn.Module):
             v["a" + n[1]], v["b" + n[1]] = a, b
         return LoraViews(v["a1"], v["b1"], v["a3"], v["b3"], v["a2"], v["b2"])
 
+    def quantize_experts(self) -> "ScatterMoEBlock":
+        """Puts 8-bit codes in the place of the expert weights, for serving and for training what lies before and around them:
+        w1, w2, w3 become int8 buffers (E, f, d) with fp32 buffers ``w1_scale``, ``w2_scale``, ``w3_scale`` of their output
+        columns, and ``forward`` takes the products over them (bf16 or fp16 hidden states, sizes that are multiples of 64).  The
+        router keeps its type.  Not for a block with adapters: its factors are trained against the weights as they are."""
+        if self.lora_r > 0:
+            raise ValueError("a block with adapters keeps its expert weights: quantize_experts() takes blocks with lora_r = 0")
+        if self.is_quantized:
+            return self
+        q = Int8ExpertWeights.quantize(self.w1, self.w2, self.w3, self.ffn_hidden_size, self.hidden_size)
+        for name, t in q._asdict().items():
+            if hasattr(self, name):
+                delattr(self, name)
+            self.register_buffer(name, t)
+        return self
+
+    @property
+    def is_quantized(self) -> bool:
+        return self.w1.dtype == torch.int8
+
     def forward(self, hidden_states: torch.Tensor):
         shape = hidden_states.shape
         x = hidden_states.reshape(-1, shape[-1])
@@ -176,8 +245,12 @@ class ScatterMoEBlock(nn.Module):
         lora = []
         if self.lora_r > 0:   # the factors in their storage, in the order a1, b1, a3, b3, a2, b2 (w2's are swapped, see lora_views)
             lora = [resolve_dtensor(t) for t in (self.lora_A_w1, self.lora_B_w1, self.lora_A_w3, self.lora_B_w3, self.lora_B_w2, self.lora_A_w2)]
-        out = _layer(x, resolve_dtensor(self.router), resolve_dtensor(self.w1), resolve_dtensor(self.w2), resolve_dtensor(self.w3), E, f,
-                     self.top_k, lora, self.lora_alpha, True, True)[0]
+        if self.is_quantized:
+            out = moe_layer_forward_int8(x, resolve_dtensor(self.router), Int8ExpertWeights(*(getattr(self, n) for n in Int8ExpertWeights._fields)),
+                                         self.top_k)[0]
+        else:
+            out = _layer(x, resolve_dtensor(self.router), resolve_dtensor(self.w1), resolve_dtensor(self.w2), resolve_dtensor(self.w3), E, f,
+                         self.top_k, lora, self.lora_alpha, True, True)[0]
         out = out.view(shape)
         if self.bias is not None:
             if self.return_bias:

@@ -15,7 +15,7 @@ from typing import Optional, Tuple
 import torch
 
 from ... import _lib
-from ..._lib import lib, check, dtype_code, is64, ptr, require_gpu, stream_ptr, workspace
+from ..._lib import lib, check, dtype_code, entry, is64, ptr, require_gpu, stream_ptr, workspace
 
 BLOCK_M = 128  # rows per padded block, as in the reference (ops.py:6)
 
@@ -237,3 +237,11 @@ def combine_dgates(y, dout, k, gates_dtype, inv=None):
     check(lib.moe_combine_dgates(ptr(y), y.stride(0), ptr(dout), dout.stride(0), ptr(dg), dtype_code(dg), ptr(inv), k, T,
                                  y.size(1), dtype_code(y), stream_ptr(dev)), "moe_combine_dgates")
     return dg
+
+
+def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(codes (rows, columns) int8, scales (rows,) fp32) of bf16, fp16 or fp32 rows: codes = x * 127 / max |x| of the row,
+    rounded to the nearest, ties to even (the exact quotient); scale = max |x| / 127.  A row of zeros has the scale 0, a row
+    that holds an infinity or a NaN the scale NaN and codes 0.  What ``parallel_linear_int8`` does to its inputs."""
+    codes, scales = entry("quantize_rows")(x)
+    return codes, scales
