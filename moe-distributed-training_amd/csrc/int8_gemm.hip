@@ -1,120 +1,76 @@
-// Grouped product of 8-bit codes over ragged expert groups:
-//   Y[out_row(m)][n] = x_scale[in_row(m)] * w_scale[e(m)][n] * sum_k X[in_row(m)][k] W[e(m)][k][n]
-// The sum of K < 2^17 products of 8-bit integers is exact in 32 bits.  One workgroup per 64 x 64 output tile, operands through LDS as dwords of four
-// codes along k, v_dot4 on 4 x 4 outputs per thread.
-#include "common.h"
-#include "kernels.h"
+// The grouped product of 8-bit codes with tiles of 256 x 256, one workgroup of 8 waves per compute unit, and what both tile sizes share.
+#define MOE_I8_TILE 256
+#include "int8_gemm_kernel.h"
 
 namespace {
 
-constexpr int TM = 64, TN = 64, TK = 64;
+constexpr int MAX_SPLIT = 8;   // K parts that a tile of the last, partial round of compute units may be cut into
 
-template <bool PAIR>
-__global__ void __launch_bounds__(256) i8_gemm_simple_kernel(const MoeI8Gemm p, int64_t kp)
+__global__ void zero_counters_kernel(int* p, int n)
 {
-    __shared__ uint32_t xs[TM][TK / 4 + 1];
-    __shared__ uint32_t ws[PAIR ? 2 : 1][TN][TK / 4 + 1];
-    __shared__ float ys[TM][TN + 1];
-    RowTile t;
-    if (!find_row_tile(p.offsets, p.off64, p.E, TM, blockIdx.y, &t)) return;
-    const int nrows = (int)(t.row1 - t.row0);
-    const int64_t n0 = (int64_t)blockIdx.x * TN;
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    int acc[PAIR ? 2 : 1][4][4] = {};
-    auto in_row = [&](int r) {
-        const int64_t m = t.row0 + (r < nrows ? r : nrows - 1);
-        return p.x_grouped ? m : load_idx(p.pos, m, p.pos64) / p.fan_out;
-    };
-    for (int seg = 0; seg < p.nseg; ++seg)
-        for (int64_t k0 = 0; k0 < p.K; k0 += TK) {
-            for (int i = threadIdx.x; i < TM * TK / 4; i += 256) {
-                const int r = i / (TK / 4), c = i % (TK / 4);
-                xs[r][c] = *(const uint32_t*)(p.X + in_row(r) * p.ldx + seg * kp + k0 + c * 4);
-                const int64_t n = n0 + r;
-#pragma unroll
-                for (int h = 0; h < (PAIR ? 2 : 1); ++h) {
-                    const int8_t* W = p.W[PAIR ? h : seg] + (int64_t)t.expert * p.swe;
-                    uint32_t v = 0;
-                    for (int b = 0; b < 4; ++b) {
-                        const int64_t k = k0 + c * 4 + b;
-                        if (k < p.K && n < p.N) v |= (uint32_t)(uint8_t)(p.nn ? W[k * p.ldw + n] : W[n * p.ldw + k]) << (8 * b);
-                    }
-                    ws[h][r][c] = v;
-                }
-            }
-            __syncthreads();
-            for (int c = 0; c < TK / 4; ++c)
-#pragma unroll
-                for (int h = 0; h < (PAIR ? 2 : 1); ++h)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            acc[h][i][j] = __builtin_amdgcn_sdot4((int)xs[ty * 4 + i][c], (int)ws[h][tx * 4 + j][c], acc[h][i][j], false);
-            __syncthreads();
-        }
-    float v[PAIR ? 2 : 1][4][4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float xs_ = p.x_scale[in_row(ty * 4 + i)];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int64_t n = n0 + tx * 4 + j < p.N ? n0 + tx * 4 + j : p.N - 1;
-#pragma unroll
-            for (int h = 0; h < (PAIR ? 2 : 1); ++h)
-                v[h][i][j] = (float)acc[h][i][j] * xs_ * (p.w_scale[h] ? p.w_scale[h][(int64_t)t.expert * p.N + n] : 1.f);
-        }
-    }
-    if (p.epi == MOE_I8_STORE) {
-        for (int i = 0; i < 4; ++i) {
-            const int r = ty * 4 + i;
-            if (r >= nrows) continue;
-            const int64_t m = t.row0 + r, o = p.y_grouped ? m : load_idx(p.pos, m, p.pos64);
-            for (int j = 0; j < 4; ++j) {
-                const int64_t n = n0 + tx * 4 + j;
-                if (n >= p.N) continue;
-                if (p.ydtype == MOE_F32) ((float*)p.Y)[o * p.ldy + n] = v[0][i][j];
-                else if (p.ydtype == MOE_BF16) ((uint16_t*)p.Y)[o * p.ldy + n] = NumBf16::from_f32(v[0][i][j]);
-                else ((uint16_t*)p.Y)[o * p.ldy + n] = NumF16::from_f32(v[0][i][j]);
-            }
-        }
-        return;
-    }
-    for (int s = 0; s < 3; ++s) {
-        if (!p.S[s]) continue;
-        for (int i = 0; i < 4; ++i)
-            for (int j = 0; j < 4; ++j) {
-                const float g = v[0][i][j], u = v[PAIR ? 1 : 0][i][j];
-                ys[ty * 4 + i][tx * 4 + j] = !PAIR || s == 1 ? g : s == 2 ? u : g / (1.f + __expf(-g)) * u;
-            }
-        __syncthreads();
-        for (int q = threadIdx.x; q < TM * (TN / MOE_SEG_COLS); q += 256) {
-            const int r = q / (TN / MOE_SEG_COLS), c0 = q % (TN / MOE_SEG_COLS) * MOE_SEG_COLS;
-            if (r >= nrows || n0 + c0 >= p.N) continue;
-            uint32_t top = 0;
-            for (int c = 0; c < MOE_SEG_COLS; ++c) top = max(top, __float_as_uint(ys[r][c0 + c]) & 0x7fffffffu);
-            const float amax = __uint_as_float(top), inv = top > 0 && top < 0x7f800000u ? 32767.f / amax : 0.f;
-            for (int c = 0; c < MOE_SEG_COLS; ++c) p.S[s][(t.row0 + r) * p.N + n0 + c0 + c] = inv > 0.f ? (int16_t)rintf(ys[r][c0 + c] * inv) : (int16_t)0;
-            p.SS[s][((t.row0 + r) * p.N + n0 + c0) / MOE_SEG_COLS] = top < 0x7f800000u ? amax / 32767.f : __uint_as_float(0x7fc00000u);
-        }
-        __syncthreads();
-    }
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i < n) p[i] = 0;
+}
+
+int64_t tiles_at_most(int tile, int64_t R, int E, int64_t N, bool pair)
+{
+    const int64_t cols = pair ? tile / 2 : tile;
+    return (R / tile + E) * ((N + cols - 1) / cols);
+}
+
+// K parts that a tile of `ktiles` K tiles can be cut into
+int parts_at_most(int64_t ktiles)
+{
+    int s = 1;
+    while (s * 2 <= MAX_SPLIT && ktiles / (s * 2) >= MIN_PART_KTILES) s *= 2;
+    return s;
 }
 
 }  // namespace
 
+// rows and columns of a launch's tiles
+int moe_i8_tile(int cus, int64_t R, int E, int64_t N, bool pair)
+{
+    const int64_t groups = R < E ? R : E;
+    const int64_t tiles = groups * (((R + groups - 1) / groups + BM - 1) / BM) * ((N + BN - 1) / BN * (pair ? 2 : 1));   // (as if the rows were dealt evenly)
+    return R <= groups * 128 || 2 * tiles <= cus ? 128 : 256;
+}
+
 bool moe_i8_weights_ok(const void* W, int64_t swe, int64_t ldw) { return (uintptr_t)W % 16 == 0 && swe % 16 == 0 && ldw % 16 == 0; }
+
+// 32-bit byte offsets: gathered rows of X from its start (grouped ones from the tile's first row), one expert's matrix (2 GiB where its last K tile is masked)
 bool moe_i8_gemm_supported(const MoeI8Gemm& p, int64_t R, int64_t x_rows)
 {
     (void)R;
-    return x_rows * p.ldx < ((int64_t)1 << 32) && (p.nn ? p.K : p.N) * p.ldw < ((int64_t)1 << 32);
+    const int64_t rows = p.x_grouped ? BM : x_rows, limit = p.K % BK ? (int64_t)1 << 31 : (int64_t)1 << 32;
+    return rows * p.ldx < ((int64_t)1 << 32) && (p.nn ? (p.K - 1) * p.ldw + p.N : (p.N - 1) * p.ldw + p.K) + 16 < limit;
 }
-size_t moe_i8_exchange_bytes(int64_t, int, int64_t, int64_t, bool) { return 256; }
-int moe_launch_i8_gemm(const MoeI8Gemm& p, int64_t R, hipStream_t stream)
+
+// counters of the split tiles (one per compute unit's workgroup) and their parts' sums, of the tile size that needs more
+size_t moe_i8_exchange_bytes(int64_t R, int E, int64_t K, int64_t N, bool pair)
 {
-    if (R == 0 || p.N == 0) return MOE_OK;
-    const dim3 grid((unsigned)((p.N + TN - 1) / TN), (unsigned)(R / TM + p.E));
-    if (p.epi == MOE_I8_SWIGLU) hipLaunchKernelGGL(i8_gemm_simple_kernel<true>, grid, dim3(256), 0, stream, p, moe_i8_pitch(p.K));
-    else hipLaunchKernelGGL(i8_gemm_simple_kernel<false>, grid, dim3(256), 0, stream, p, moe_i8_pitch(p.K));
-    return moe_launch_status();
+    const int cus = moe_device_cus();
+    const int64_t parts = parts_at_most((K + BK - 1) / BK);
+    size_t most = 0;
+    for (int tile = 256; tile >= 128; tile /= 2) {
+        const int64_t slots = (int64_t)(256 / tile) * cus, all = parts * tiles_at_most(tile, R, E, N, pair);
+        const size_t b = parts == 1 ? 0 : (size_t)(all < slots ? all : slots) * tile * tile * sizeof(int);
+        most = b > most ? b : most;
+    }
+    return 2 * (size_t)cus * sizeof(int) + 256 + most;
+}
+
+int moe_launch_i8_gemm(const MoeI8Gemm& p_, int64_t R, hipStream_t stream)
+{
+    if (R == 0 || p_.N == 0) return MOE_OK;
+    MoeI8Gemm p = p_;
+    const int cus = moe_device_cus() / NXCD * NXCD > 0 ? moe_device_cus() / NXCD * NXCD : NXCD;
+    p.num_cus = cus;
+    p.max_split = parts_at_most((p.K + BK - 1) / BK * p.nseg);
+    if (p.max_split > 1 && !p.exchange) return MOE_ERR_WORKSPACE;
+    p.sk_counters = (int*)p.exchange;
+    p.sk_partials = (int*)((uint8_t*)p.exchange + ((2 * (size_t)moe_device_cus() * sizeof(int) + 255) & ~(size_t)255));
+    p.y_vec = (uintptr_t)p.Y % 16 == 0 && (p.ydtype == MOE_F32 ? p.ldy % 4 == 0 && p.N % 4 == 0 : p.ldy % 8 == 0 && p.N % 8 == 0);
+    if (p.max_split > 1) hipLaunchKernelGGL(zero_counters_kernel, dim3((unsigned)((2 * cus + 255) / 256)), dim3(256), 0, stream, p.sk_counters, 2 * cus);
+    return moe_i8_tile(cus, R, p.E, p.N, p.epi == MOE_I8_SWIGLU) == 128 ? moe_launch_i8_gemm_small(p, R, stream) : launch_epilogue(p, R, stream);
 }

@@ -262,8 +262,15 @@ struct MoeI8Gemm {
     const void* pos; int pos64; const void* offsets; int off64;
     int E; int64_t K, N;                // K: of one segment
     int fan_out, x_grouped, y_grouped, epi;
-    void* exchange;
+    void* exchange;                     // moe_i8_exchange_bytes
+    // set by the launcher
+    int num_cus, max_split;             // workgroups of a round of the tile plan; K parts that a tile may be cut into
+    int *sk_counters, *sk_partials;
+    int y_vec;                          // rows of Y take 16-byte stores
 };
+constexpr int MOE_I8_MIN_PART = 4;
+int moe_i8_tile(int cus, int64_t R, int E, int64_t N, bool pair);
+int moe_launch_i8_gemm_small(const MoeI8Gemm& p, int64_t R, hipStream_t stream);
 // whether the kernel reads W in this orientation and alignment (otherwise: moe_launch_pack_codes first)
 bool moe_i8_weights_ok(const void* W, int64_t swe, int64_t ldw);
 // whether sizes stay inside the kernel's 32-bit offsets (x_rows: rows of X)
