@@ -9,7 +9,7 @@
 //     operand is contiguous along k, ds_read_b64_tr_b8 where W is contiguous along n.
 //   - Codes of X rows are padded with zeros to whole K tiles, so what stands in W's image behind K does not matter; only addresses do (KTAIL).
 //   - The sums are integers: K parts of a tile may be added in any order, with one result.
-//   - Epilogues: the scaled product in the output's type; the same as 16-bit integers with a scale per 32 columns (for the next product's codes);
+//   - Epilogues: the scaled product in the output's type; the same as 24-bit integers with a scale per 32 columns (for the next product's codes);
 //     or SwiGLU of a gate and an up product in that form.
 //
 // Included by one translation unit per tile size (MOE_I8_TILE: 256 or 128).
@@ -31,7 +31,7 @@ constexpr int B_REGION = 2 * A_STAGE_BYTES;
 constexpr int LDS_BYTES = B_REGION + 3 * B_STAGE_BYTES;   // 160 or 80 KiB
 // Row and scale tables borrow the third weight stage: it is empty before the main loop's first tile, and behind the epilogue's staging after the last.
 constexpr int TABLE_OFF = B_REGION + 2 * B_STAGE_BYTES;
-static_assert(TABLE_OFF >= NWAVES * WTM * WTN * 2, "epilogue staging must not reach the tables");
+static_assert(TABLE_OFF >= NWAVES * WTM * WTN * 2 && MOE_SEG_BYTES <= WTN * 2, "epilogue staging must not reach the tables");
 constexpr int MIN_PART_KTILES = MOE_I8_MIN_PART;    // K tiles of a split tile's part, at least
 static_assert(NTHREADS == BM + BN && WTN == 2 * MOE_SEG_COLS, "a thread brings one row's or one column's scale; a wave holds two segments per row");
 
@@ -342,29 +342,52 @@ __global__ void __launch_bounds__(NTHREADS, 2) i8_gemm_kernel(const MoeI8Gemm p)
         const float4 v = *(const float4*)(s_wscale + c);
         w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
     };
-    // 8 values of a lane, 32 of a row over the four lanes that share it -> 16-bit codes (staged) and the segment's scale
-    auto put_segment = [&](int sw, int mb, int block0, const float* v, float* scales, int64_t ncol) {
-        float top = 0.f;
+    // One output of 32 columns per wave in segments of 24-bit codes (value(mb, i): element i of this lane's 8 in row block mb): a row's 32 values lie
+    // with four lanes; their maximum gives the scale, the codes are staged as the segment's 96 bytes and go out 16 bytes per lane.
+    auto put_segments = [&](auto value, uint8_t* out, float* scales, int64_t ncol) {
+        const int64_t segs = p.N / MOE_SEG_COLS;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = __uint_as_float(max(__float_as_uint(top), __float_as_uint(v[i]) & 0x7fffffffu));   // (bits: NaN above infinity above every number)
-        top = __uint_as_float(max(__float_as_uint(top), (uint32_t)__shfl_xor((int)__float_as_uint(top), 16)));
-        top = __uint_as_float(max(__float_as_uint(top), (uint32_t)__shfl_xor((int)__float_as_uint(top), 32)));
-        const bool fine = __float_as_uint(top) < 0x7f800000u;
-        // (32767 / top is past fp32 for a segment below 2^-113: it is zero to the 8-bit codes of any row that is not)
-        const float inv = fine && top > 0x1p-110f ? 32767.f * __builtin_amdgcn_rcpf(top) : 0.f;
+        for (int mb = 0; mb < MB; ++mb) {
+            if (mb >= mb_cnt) continue;
+            float v[8];
+            uint32_t top = 0;
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            int q[4];
+            for (int i = 0; i < 8; ++i) {
+                v[i] = value(mb, i);
+                top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);   // (bits: NaN above infinity above every number)
+            }
+            top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+            top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+            const float amax = __uint_as_float(top);
+            const bool fine = top < 0x7f800000u;
+            // (a segment below 2^-100 is zero to the 8-bit codes of any row that is not as small as that)
+            const float inv = fine && amax > 0x1p-100f ? (float)MOE_SEG_LEVELS * __builtin_amdgcn_rcpf(amax) : 0.f;
+            const int m = mb * 16 + mrow;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) q[i] = fine ? (int)fminf(fmaxf(rintf(v[4 * b + i] * inv), -32767.f), 32767.f) : 0;
-            uint2 w;
-            w.x = (uint32_t)(q[0] & 0xffff) | (uint32_t)q[1] << 16;
-            w.y = (uint32_t)(q[2] & 0xffff) | (uint32_t)q[3] << 16;
-            stage_put(sw, mb * 16 + mrow, (block0 + b) * 16 + nq, w);
+            for (int b = 0; b < 2; ++b) {
+                int q[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) q[i] = fine ? (int)rintf(fminf(fmaxf(v[4 * b + i] * inv, -(float)MOE_SEG_LEVELS), (float)MOE_SEG_LEVELS)) : 0;
+                uint2 hi;
+                hi.x = __builtin_amdgcn_perm((uint32_t)q[1], (uint32_t)q[0], 0x06050201u);
+                hi.y = __builtin_amdgcn_perm((uint32_t)q[3], (uint32_t)q[2], 0x06050201u);
+                const uint32_t lo = (uint32_t)(q[0] & 0xff) | (uint32_t)(q[1] & 0xff) << 8 | (uint32_t)(q[2] & 0xff) << 16 | (uint32_t)q[3] << 24;
+                *(uint2*)(stg + m * MOE_SEG_BYTES + b * 32 + nq * 2) = hi;
+                *(uint32_t*)(stg + m * MOE_SEG_BYTES + 64 + b * 16 + nq) = lo;
+            }
+            if (lane < 16 && m < wrows && ncol < p.N)
+                scales[(row0 + wrow0 + m) * segs + ncol / MOE_SEG_COLS] = !fine ? __uint_as_float(0x7fc00000u) : inv > 0.f ? amax * (1.f / MOE_SEG_LEVELS) : 0.f;
         }
-        const int m = mb * 16 + mrow;
-        if (lane < 16 && m < wrows && ncol < p.N)
-            scales[(row0 + wrow0 + m) * (p.N / MOE_SEG_COLS) + ncol / MOE_SEG_COLS] = !fine ? __uint_as_float(0x7fc00000u) : inv > 0.f ? top * (1.f / 32767.f) : 0.f;
+        __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0): this wave's staging writes have landed
+        if (ncol < p.N) {
+            constexpr int PIECES = MOE_SEG_BYTES / 16;
+            uint8_t* to = out + ((row0 + wrow0) * segs + ncol / MOE_SEG_COLS) * MOE_SEG_BYTES;
+            for (int i = lane; i < wrows * PIECES; i += 64) {
+                const int m = i / PIECES, c = i - m * PIECES;
+                *(u32x4_t*)(to + m * segs * MOE_SEG_BYTES + c * 16) = *(const u32x4_t*)(stg + i * 16);
+            }
+        }
+        __builtin_amdgcn_s_waitcnt(0xC07F);   // reads done before the slice is reused
     };
 
     if (EPI == MOE_I8_STORE) {
@@ -417,18 +440,9 @@ __global__ void __launch_bounds__(NTHREADS, 2) i8_gemm_kernel(const MoeI8Gemm p)
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) column_scales(nb, w[nb]);
 #pragma unroll
-        for (int mb = 0; mb < MB; ++mb) {
-            if (mb >= mb_cnt) continue;
-            const float xs = s_xscale[wrow0 + mb * 16 + mrow];
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                float v[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = (float)acc[mb][2 * s + i / 4][i % 4] * xs * w[2 * s + i / 4][i % 4];
-                put_segment(WTN, mb, 2 * s, v, p.SS[0], n0 + wn * WTN + s * MOE_SEG_COLS);
-            }
-        }
-        stage_flush(WTN, (uint16_t*)p.S[0], p.N, false, n0 + wn * WTN, true);
+        for (int h = 0; h < 2; ++h)
+            put_segments([&](int mb, int i) { return (float)acc[mb][2 * h + i / 4][i % 4] * s_xscale[wrow0 + mb * 16 + mrow] * w[2 * h + i / 4][i % 4]; },
+                         p.S[0], p.SS[0], n0 + wn * WTN + h * MOE_SEG_COLS);
     } else {   // SwiGLU: gate = acc[mb][j], up = acc[mb][NBH + j] at the same row and column
         float w[NB][4];
 #pragma unroll
@@ -437,20 +451,12 @@ __global__ void __launch_bounds__(NTHREADS, 2) i8_gemm_kernel(const MoeI8Gemm p)
 #pragma unroll
         for (int out = 0; out < 3; ++out) {
             if (!p.S[out]) continue;
-#pragma unroll
-            for (int mb = 0; mb < MB; ++mb) {
-                if (mb >= mb_cnt) continue;
+            put_segments([&](int mb, int i) {
                 const float xs = s_xscale[wrow0 + mb * 16 + mrow];
-                float v[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float g = (float)acc[mb][i / 4][i % 4] * xs * w[i / 4][i % 4];
-                    const float u = (float)acc[mb][NBH + i / 4][i % 4] * xs * w[NBH + i / 4][i % 4];
-                    v[i] = out == 0 ? g * __builtin_amdgcn_rcpf(1.f + __expf(-g)) * u : out == 1 ? g : u;
-                }
-                put_segment(WTN / 2, mb, 0, v, p.SS[out], ncol0);
-            }
-            stage_flush(WTN / 2, (uint16_t*)p.S[out], p.N, false, ncol0, true);
+                const float g = (float)acc[mb][i / 4][i % 4] * xs * w[i / 4][i % 4];
+                const float u = (float)acc[mb][NBH + i / 4][i % 4] * xs * w[NBH + i / 4][i % 4];
+                return out == 0 ? g * __builtin_amdgcn_rcpf(1.f + __expf(-g)) * u : out == 1 ? g : u;
+            }, p.S[out], p.SS[out], ncol0);
         }
     }
 }

@@ -1,4 +1,4 @@
-// Rows of the 8-bit expert products: activations and gradients into codes with a scale per row, the 16-bit interims between two products, and
+// Rows of the 8-bit expert products: activations and gradients into codes with a scale per row, the interims between two products, and
 // weights in an order that the product kernel can read.
 //
 // A row v becomes codes q[c] = rne(127 v[c] / a) with a = max |v| and the scale a / 127: the quotient is rounded as it is, not as some fp32 value of
@@ -7,9 +7,10 @@
 // exactly for 2-byte types (at most 19 bits: values below a / 254 have q = 0) and fp64 for fp32 values.  A row that holds an infinity or a NaN gets the
 // scale NaN and codes 0, so that every product of it is NaN and no other row changes; a row of zeros the scale 0.
 //
-// Interims (h, the saved gate and up, dh) travel as 16-bit integers with a scale for each 32 columns of a row: 2 bytes per value as a bf16 tensor takes,
-// at 2^-16 of the segment's maximum instead of 2^-9 of the value.  A code of the next product's 8 bits is next to a border for 1 value in 500 then and
-// not for 1 in 4 (largest values, bf16), which is what keeps the MLP's error that of its last rounding.
+// Interims (h, the saved gate and up, dh) travel as 24-bit integers with a scale for each 32 columns of a row: 3 bytes per value, 2^-24 of the segment's maximum
+// off.  Every value that a rounding on the way carries over a border of the 8-bit codes costs a whole step, so this noise falls with the root of
+// the rounding only: with 16 bits 1 code in 700 changed and the MLP's error against 64 bits was 1.5e-3 of its result's norm (bf16 rows would be off by four
+// times that), with 24 it is that of fp32 arithmetic, at three quarters of an fp32 tensor's bytes.
 #include "common.h"
 #include "kernels.h"
 
@@ -126,11 +127,11 @@ template <> struct Loader<__half> {
 
 // One workgroup per row.  KEEP: a thread holds its KEEP pieces of 8 columns between the two passes (0: the row is read twice).  SCALED: row m is row
 // pos[m] / fan_out of src times coeff[pos[m]] and, column by column, col_scale[expert of m] (a gradient on its way through the weights' scales).
-// fp32 rows are worked through in fp64 throughout: the product of three fp32 numbers is rounded once, 29 bits behind what fp32 could tell.
+// Those products, and fp32 rows, are worked through in fp64 throughout: the quotient that is rounded is that of the exact values to 2^-50.
 template <typename T, bool SCALED, int KEEP>
 __global__ void __launch_bounds__(1024) quantize_rows_kernel(const MoeQuantizeRows p)
 {
-    typedef std::conditional_t<std::is_same_v<T, float>, double, float> C;
+    typedef std::conditional_t<SCALED || std::is_same_v<T, float>, double, float> C;
     const int64_t m = blockIdx.x;
     int64_t src_row = m;
     C coeff = 1;
@@ -205,18 +206,23 @@ __global__ void __launch_bounds__(1024) quantize_rows_kernel(const MoeQuantizeRo
     if (threadIdx.x == 0) p.scale[m] = rc.scale;
 }
 
-__device__ __forceinline__ void ld8_i16(const int16_t* p, float s, float* v)
+// columns c0 .. c0 + 7 of a row of segments, times s
+__device__ __forceinline__ void ld8_seg(const uint8_t* row, int64_t c0, float s, float* v)
 {
-    const u32x4_t w = *(const u32x4_t*)p;
+    const uint8_t* seg = row + c0 / MOE_SEG_COLS * MOE_SEG_BYTES;
+    const int c = (int)(c0 % MOE_SEG_COLS);
+    const u32x4_t hi = *(const u32x4_t*)(seg + c * 2);
+    const uint2 lo = *(const uint2*)(seg + 64 + c);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        v[2 * i] = (float)(int16_t)(w[i] & 0xffff) * s;
-        v[2 * i + 1] = (float)((int)w[i] >> 16) * s;
+        const uint32_t l = (i < 2 ? lo.x : lo.y) >> (16 * (i & 1));
+        v[2 * i] = (float)(((int)(hi[i] << 16) >> 8) | (int)(l & 0xff)) * s;
+        v[2 * i + 1] = (float)(((int)(hi[i] & 0xffff0000u) >> 8) | (int)((l >> 8) & 0xff)) * s;
     }
 }
 
-// 16-bit rows with segment scales -> codes: the maximum of a row is that of its segments, whose largest code is 32767.
-__global__ void __launch_bounds__(1024) requantize_rows_kernel(const int16_t* src, const float* seg, int64_t cols, int8_t* codes, int64_t ldc, float* scale)
+// Rows of segments -> codes: the maximum of a row is that of its segments, whose largest integer is MOE_SEG_LEVELS.
+__global__ void __launch_bounds__(1024) requantize_rows_kernel(const uint8_t* src, const float* seg, int64_t cols, int8_t* codes, int64_t ldc, float* scale)
 {
     const int64_t m = blockIdx.x;
     const int64_t nseg = cols / MOE_SEG_COLS;
@@ -228,7 +234,7 @@ __global__ void __launch_bounds__(1024) requantize_rows_kernel(const int16_t* sr
         top = fmaxf(top, s);
     }
     top = block_max(top, bad);
-    const float amax = top * 32767.f;
+    const float amax = top * (float)MOE_SEG_LEVELS;
     bad |= !finite(amax);
     const float f = row_factor(amax);
     const float inv = !bad && amax > 0.f ? 127.f / (amax * f) : 0.f;
@@ -236,7 +242,7 @@ __global__ void __launch_bounds__(1024) requantize_rows_kernel(const int16_t* sr
         uint2 w = {0u, 0u};
         if (c0 < cols && inv > 0.f) {
             float v[8];
-            ld8_i16(src + m * cols + c0, seg[m * nseg + c0 / MOE_SEG_COLS] * f * inv, v);
+            ld8_seg(src + m * nseg * MOE_SEG_BYTES, c0, seg[m * nseg + c0 / MOE_SEG_COLS] * f * inv, v);
             int q[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) q[i] = (int)rintf(fminf(fmaxf(v[i], -127.f), 127.f));
@@ -262,9 +268,9 @@ __global__ void __launch_bounds__(1024) swiglu_bwd_codes_kernel(const MoeSwigluB
     auto load = [&](int64_t c0, float* a, float* b) {
         float dh[8], g[8], u[8];
         const int64_t s = m * nseg + c0 / MOE_SEG_COLS;
-        ld8_i16(p.dh + m * p.f + c0, p.dh_seg[s], dh);
-        ld8_i16(p.gate + m * p.f + c0, p.gate_seg[s], g);
-        ld8_i16(p.up + m * p.f + c0, p.up_seg[s], u);
+        ld8_seg(p.dh + m * nseg * MOE_SEG_BYTES, c0, p.dh_seg[s], dh);
+        ld8_seg(p.gate + m * nseg * MOE_SEG_BYTES, c0, p.gate_seg[s], g);
+        ld8_seg(p.up + m * nseg * MOE_SEG_BYTES, c0, p.up_seg[s], u);
         float x1[8], x3[8];
         Loader<float>::ld8(c1 + c0, x1);
         Loader<float>::ld8(c3 + c0, x3);
@@ -421,7 +427,7 @@ int moe_launch_quantize_rows(const MoeQuantizeRows& p_, int dtype, int64_t rows,
     });
 }
 
-int moe_launch_requantize_rows(const int16_t* src, const float* seg, int64_t rows, int64_t cols, int8_t* codes, int64_t ldc, float* scale, hipStream_t stream)
+int moe_launch_requantize_rows(const uint8_t* src, const float* seg, int64_t rows, int64_t cols, int8_t* codes, int64_t ldc, float* scale, hipStream_t stream)
 {
     if (rows == 0) return MOE_OK;
     const int nt = ldc / 8 <= 64 ? 64 : ldc / 8 <= 128 ? 128 : 256;

@@ -213,7 +213,9 @@ int moe_launch_swiglu_bwd(const void* g, const void* u, const void* dh, void* dg
                           hipStream_t stream);
 
 // ---- expert products in 8-bit integers (int8_rows.hip, int8_gemm.hip)
-constexpr int MOE_SEG_COLS = 32;        // columns that share a scale in the 16-bit interims
+// interims between two products: segments of 32 columns of a row as 24-bit integers that share a scale, 96 bytes each: the upper 16 bits of the 32 values, then
+// their lower 8; [R][N / 32] of them
+constexpr int MOE_SEG_COLS = 32, MOE_SEG_BYTES = 96, MOE_SEG_LEVELS = 8388607;
 constexpr int MOE_I8_KTILE = 128;       // codes of a row come in whole K tiles, zeros behind the last column
 constexpr int64_t MOE_I8_MAX_K = 131071;   // 128 * 128 * K < 2^31: the sums are exact in 32 bits
 inline int64_t moe_i8_pitch(int64_t cols) { return (cols + MOE_I8_KTILE - 1) / MOE_I8_KTILE * MOE_I8_KTILE; }
@@ -230,10 +232,10 @@ struct MoeQuantizeRows {
     int vec;                // (set by the launcher) rows of src are 16-byte aligned
 };
 int moe_launch_quantize_rows(const MoeQuantizeRows& p, int dtype, int64_t rows, hipStream_t stream);
-int moe_launch_requantize_rows(const int16_t* src, const float* seg, int64_t rows, int64_t cols, int8_t* codes, int64_t ldc, float* scale, hipStream_t stream);
-// codes [rows][2 * ldc] of the joint rows [dgate * s1 | dup * s3]; dh, gate, up: [rows][f] with their segments' scales [rows][f / MOE_SEG_COLS]
+int moe_launch_requantize_rows(const uint8_t* src, const float* seg, int64_t rows, int64_t cols, int8_t* codes, int64_t ldc, float* scale, hipStream_t stream);
+// codes [rows][2 * ldc] of the joint rows [dgate * s1 | dup * s3]; dh, gate, up: segments with their scales [rows][f / MOE_SEG_COLS]
 struct MoeSwigluBwdCodes {
-    const int16_t *dh, *gate, *up;
+    const uint8_t *dh, *gate, *up;
     const float *dh_seg, *gate_seg, *up_seg;
     const float *s1, *s3;   // [E][f]
     const void* offsets; int off64; int E;
@@ -247,7 +249,7 @@ int moe_launch_quantize_weights(const void* W, int64_t swe, int64_t swk, int64_t
 
 // epilogues of the 8-bit grouped product
 #define MOE_I8_STORE 0      // Y = acc * x_scale * w_scale in ydtype
-#define MOE_I8_SEG 1        // the same as 16-bit integers with segment scales (grouped rows)
+#define MOE_I8_SEG 1        // the same as segments (grouped rows)
 #define MOE_I8_SWIGLU 2     // weight pair (gate, up): S[0] = silu(gate) * up and, where given, S[1] = gate, S[2] = up, as segments
 
 struct MoeI8Gemm {
@@ -258,7 +260,7 @@ struct MoeI8Gemm {
     int nn, nseg;
     const float* w_scale[2];            // [E][N], or null (1); [1]: up
     void* Y; int64_t ldy; int ydtype;
-    int16_t* S[3]; float* SS[3];        // segment outputs [R][N] and their scales [R][N / MOE_SEG_COLS]
+    uint8_t* S[3]; float* SS[3];        // segment outputs and their scales [R][N / MOE_SEG_COLS]
     const void* pos; int pos64; const void* offsets; int off64;
     int E; int64_t K, N;                // K: of one segment
     int fan_out, x_grouped, y_grouped, epi;

@@ -1111,12 +1111,12 @@ int moe_scatter2scatter_int8(const int8_t* X, int64_t ldx, const float* x_scale,
 }
 
 namespace {
-struct I8Seg { int16_t* v; float* s; };
-inline size_t i8_seg_bytes(int64_t R, int64_t N) { return al((size_t)R * N * 2) + al((size_t)R * (N / MOE_SEG_COLS) * 4); }
+struct I8Seg { uint8_t* v; float* s; };
+inline size_t i8_seg_bytes(int64_t R, int64_t N) { return al((size_t)R * (N / MOE_SEG_COLS) * MOE_SEG_BYTES) + al((size_t)R * (N / MOE_SEG_COLS) * 4); }
 inline I8Seg take_seg(Bump& b, int64_t R, int64_t N)
 {
     I8Seg s;
-    s.v = (int16_t*)b.take((size_t)R * N * 2);
+    s.v = (uint8_t*)b.take((size_t)R * (N / MOE_SEG_COLS) * MOE_SEG_BYTES);
     s.s = (float*)b.take((size_t)R * (N / MOE_SEG_COLS) * 4);
     return s;
 }

@@ -273,8 +273,8 @@ def mlp_case(dev, dtype, T, d, f, E, k, gates=True, grouped_out=False, train=Tru
     x = torch.randn(T, d, generator=g).to(dtype)
     gw = gw.to(dtype) if gates else None
     dout = torch.randn(T if gates else T * k, d, generator=g).to(dtype) if train else None
-    # h: 2^-16 of its segment's maximum (its 16-bit code), and the exponential's, the reciprocal's and five fp32 roundings (2^-21 together), times 127 steps
-    near = 127 * (2.0 ** -16 + 2.0 ** -20)
+    # h: 2^-24 of its segment's maximum (its 24-bit code), and the exponential's, the reciprocal's and eight fp32 roundings (2^-20 together), times 127 steps
+    near = 127 * (2.0 ** -24 + 2.0 ** -20)
     want = oracle.mlp(x, w, k, sei, ssi, gw, dout, grouped_out, near)
     xd = x.to(dev).requires_grad_(train)
     gd = gw.to(dev).requires_grad_(train) if gates else None
@@ -287,10 +287,10 @@ def mlp_case(dev, dtype, T, d, f, E, k, gates=True, grouped_out=False, train=Tru
     if not train:
         return
     y.backward(dout.to(dev))
-    # Gradients: rows rounded to the type (half a step) and summed (half a step), and of the codes of dgate and dup, whose values carry 2^-15 of their segments' maxima, at most
-    # 2 * 127 * 2^-14 round the other way: each moves its value by a step of at most 8 / 127 of the row's size (the largest of 2 f normal products
+    # Gradients: rows rounded to the type (half a step) and summed (half a step), and of the codes of dgate and dup, whose values are as exact as h, at most
+    # 2 * 127 * 2^-18 round the other way: each moves its value by a step of at most 8 / 127 of the row's size (the largest of 2 f normal products
     # is below 12 of it for f <= 2^12, and all but 2 % of rows below 8).
-    flips = (2 * 127 * 2.0 ** -14) ** 0.5 * 12 / 127
+    flips = (2 * 127 * 2.0 ** -18) ** 0.5 * 12 / 127
     assert norm_rel(xd.grad, want["dx"]) <= 2 * h + flips, norm_rel(xd.grad, want["dx"])
     if gates:
         assert norm_rel(gd.grad, want["d_gates"]) <= 2 * h + (2 * near) ** 0.5 * 12 / 127
