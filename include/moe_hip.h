@@ -256,26 +256,27 @@ int moe_mlp_bwd(const void* dy, int64_t lddy, int dy_grouped, int dy_fan_out, co
  * infinity or a NaN the scale NaN and codes 0, which makes every product of it NaN.  Sums of products are exact (K < 2^17, else MOE_ERR_UNSUPPORTED);
  * their values do not depend on the order or number of launches.
  *
- * moe_quantize_rows: row m of the codes (pitch ldc >= ncols, a multiple of 16, 16-byte aligned; columns from ncols on are written as zeros) is row m of
- * src, or with pos row pos[m] / fan_out; times coeff[pos[m]] (coeff[m] without pos) and, column by column, col_scale[e][c] of the expert e that grouped
- * row m belongs to (offsets, E; a row behind the last group is left as it was).  fp32 rows are worked through in 64 bits.
- * Products read the codes of a row up to the next multiple of 128 columns: ldc at least that. */
-int moe_quantize_rows(const void* src, int64_t lds, int dtype, const void* pos, int pos64, int fan_out, const void* coeff, int coeff_dtype,
-                      const float* col_scale, const void* offsets, int off64, int E, int8_t* codes, int64_t ldc, float* scale, int64_t nrows,
-                      int64_t ncols, void* stream);
+ * moe_quantize_rows: rows of src -> codes (pitch ldc >= ncols, a multiple of 16, 16-byte aligned; columns from ncols on are written as zeros) and scales. */
+int moe_quantize_rows(const void* src, int64_t lds, int dtype, int8_t* codes, int64_t ldc, float* scale, int64_t nrows, int64_t ncols, void* stream);
 /* weights (E,K,N) of any strides -> codes (E,K,N) of any strides and scale (E,N), the maximum taken over K */
 size_t moe_quantize_weights_workspace_bytes(int E, int64_t N);
 int moe_quantize_weights(const void* W, int64_t swe, int64_t swk, int64_t swn, int dtype, int E, int64_t K, int64_t N, int8_t* codes, int64_t sce,
                          int64_t sck, int64_t scn, float* scale, void* workspace, size_t workspace_bytes, void* stream);
-/* moe_scatter2scatter without adapters, of codes:  Y[out_row] = x_scale[in_row] * w_scale[e][n] * (X[in_row] @ W[e]).
- * X: codes as moe_quantize_rows writes them, zeros from K to the next multiple of 128 (ldx at least that, a multiple of 16); W (E,K,N) of any strides -- read
- * in place where contiguous along K or N with the other strides and the address multiples of 16, otherwise through a copy in the workspace;
- * w_scale (E,N) or NULL (1); Y of `dtype` with unit column stride.  For a gradient X holds the codes of dY * w_scale, W its transposed view, w_scale NULL. */
-size_t moe_scatter2scatter_int8_workspace_bytes(const int8_t* W, int64_t swe, int64_t swk, int64_t swn, int64_t R, int E, int64_t K, int64_t N);
-int moe_scatter2scatter_int8(const int8_t* X, int64_t ldx, const float* x_scale, const int8_t* W, int64_t swe, int64_t swk, int64_t swn,
-                             const float* w_scale, void* Y, int64_t ldy, int dtype, const void* pos, int pos64, const void* offsets, int off64, int E,
-                             int64_t R, int64_t K, int64_t N, int fan_out, int x_grouped, int y_grouped, void* workspace, size_t workspace_bytes,
-                             void* stream);
+/* moe_scatter2scatter without adapters over 8-bit weights: codes and scales sx of the x_rows rows of x, then
+ *   y[out_row] = sx[in_row] * w_scale[e][n] * (codes[in_row] @ W[e]),   rows addressed as there.
+ * W (E,K,N) of any strides: read in place where contiguous along K or N with the other strides and the address multiples of 16, otherwise through a copy in
+ * the workspace.  Backward (weights frozen, the codes' rounding straight through): row m of the order is dY's row m (dy_grouped) or pos[m] / dy_fan_out, times
+ * gates[pos[m]] (gates[m] with dy_grouped; NULL: 1) and, column by column, w_scale[e]; of its codes and scale sg
+ *   dx_rows[dx_grouped ? m : pos[m]] = sg[m] * (codes[m] @ W[e]^T).
+ * code_rows of the workspace query: x_rows, or R for the backward call (which asks with K and N, and their strides, swapped).  Rows that no group covers
+ * are not written. */
+size_t moe_linear_int8_workspace_bytes(const int8_t* W, int64_t swe, int64_t swk, int64_t swn, int64_t code_rows, int64_t R, int E, int64_t K, int64_t N);
+int moe_linear_int8_fwd(const void* x, int64_t ldx, int64_t x_rows, int dtype, const int8_t* W, int64_t swe, int64_t swk, int64_t swn,
+                        const float* w_scale, void* y, int64_t ldy, const void* pos, int pos64, const void* offsets, int off64, int E, int64_t R, int64_t K,
+                        int64_t N, int fan_out, int x_grouped, int y_grouped, void* workspace, size_t workspace_bytes, void* stream);
+int moe_linear_int8_bwd(const void* dy, int64_t lddy, int dtype, int dy_grouped, int dy_fan_out, const void* gates, int gates_dtype, const int8_t* W,
+                        int64_t swe, int64_t swk, int64_t swn, const float* w_scale, void* dx_rows, int64_t lddx, int dx_grouped, const void* pos, int pos64,
+                        const void* offsets, int off64, int E, int64_t R, int64_t K, int64_t N, void* workspace, size_t workspace_bytes, void* stream);
 /* The expert MLP of moe_mlp_fwd / moe_mlp_bwd over 8-bit weights: w1, w3, w2 codes (E,f,d) contiguous, scales s1, s3 (E,f) and s2 (E,d); bf16 or fp16 x, y, dy, dx;
  * d and f multiples of 64.  x has x_rows rows; row m of the order is row pos[m] / fan_out of them.
  * Forward:  gate, up = codes(x) W1, codes(x) W3;  h = silu(gate) * up;  y[out_row] = codes(h) W2.  `saved` (or NULL): gate and up for the backward pass.

@@ -62,11 +62,12 @@ _SIGNATURES = {
     "moe_mlp_saved_bytes": ("z", "li"),
     "moe_mlp_fwd": ("i", "pl" + "ppp" + "pp" + "if" + "pppp" + "l" + "pi" + "pi" + "i" + "lll" + "iii" + "p" + "pzp"),
     "moe_mlp_bwd": ("i", "plii" + "p" + "pl" + "ppp" + "pp" + "pp" + "if" + "ppp" + "pp" + "pli" + "pi" + "pi" + "i" + "lll" + "ii" + "p" + "pzp"),
-    "moe_quantize_rows": ("i", "pli" + "pii" + "pi" + "ppii" + "plp" + "ll" + "p"),
+    "moe_quantize_rows": ("i", "plipl" + "pll" + "p"),
     "moe_quantize_weights_workspace_bytes": ("z", "il"),
     "moe_quantize_weights": ("i", "plll" + "iill" + "plll" + "p" + "pzp"),
-    "moe_scatter2scatter_int8_workspace_bytes": ("z", "plll" + "lill"),
-    "moe_scatter2scatter_int8": ("i", "plp" + "plll" + "p" + "pli" + "pi" + "pi" + "i" + "lll" + "iii" + "pzp"),
+    "moe_linear_int8_workspace_bytes": ("z", "plll" + "llill"),
+    "moe_linear_int8_fwd": ("i", "plli" + "plll" + "p" + "pl" + "pi" + "pi" + "i" + "lll" + "iii" + "pzp"),
+    "moe_linear_int8_bwd": ("i", "pliii" + "pi" + "plll" + "p" + "pli" + "pi" + "pi" + "i" + "lll" + "pzp"),
     "moe_mlp_int8_saved_bytes": ("z", "ll"),
     "moe_mlp_int8_workspace_bytes": ("z", "llilli"),
     "moe_mlp_int8_fwd": ("i", "plli" + "pppppp" + "pl" + "pi" + "pi" + "i" + "lll" + "ii" + "pz" + "pzp"),

@@ -6,12 +6,6 @@ namespace {
 
 constexpr int MAX_SPLIT = 8;   // K parts that a tile of the last, partial round of compute units may be cut into
 
-__global__ void zero_counters_kernel(int* p, int n)
-{
-    const int i = blockIdx.x * 256 + threadIdx.x;
-    if (i < n) p[i] = 0;
-}
-
 int64_t tiles_at_most(int tile, int64_t R, int E, int64_t N, bool pair)
 {
     const int64_t cols = pair ? tile / 2 : tile;
@@ -46,10 +40,13 @@ bool moe_i8_gemm_supported(const MoeI8Gemm& p, int64_t R, int64_t x_rows)
     return rows * p.ldx < ((int64_t)1 << 32) && (p.nn ? (p.K - 1) * p.ldw + p.N : (p.N - 1) * p.ldw + p.K) + 16 < limit;
 }
 
+// counters of the split tiles: two per compute unit are enough for either tile size
+int moe_i8_counters() { return 2 * (moe_device_cus() / NXCD * NXCD > 0 ? moe_device_cus() / NXCD * NXCD : NXCD); }
+
 // counters of the split tiles (one per compute unit's workgroup) and their parts' sums, of the tile size that needs more
 size_t moe_i8_exchange_bytes(int64_t R, int E, int64_t K, int64_t N, bool pair)
 {
-    const int cus = moe_device_cus();
+    const int cus = moe_i8_counters() / 2;
     const int64_t parts = parts_at_most((K + BK - 1) / BK);
     size_t most = 0;
     for (int tile = 256; tile >= 128; tile /= 2) {
@@ -64,13 +61,12 @@ int moe_launch_i8_gemm(const MoeI8Gemm& p_, int64_t R, hipStream_t stream)
 {
     if (R == 0 || p_.N == 0) return MOE_OK;
     MoeI8Gemm p = p_;
-    const int cus = moe_device_cus() / NXCD * NXCD > 0 ? moe_device_cus() / NXCD * NXCD : NXCD;
+    const int cus = moe_i8_counters() / 2;
     p.num_cus = cus;
     p.max_split = parts_at_most((p.K + BK - 1) / BK * p.nseg);
     if (p.max_split > 1 && !p.exchange) return MOE_ERR_WORKSPACE;
     p.sk_counters = (int*)p.exchange;
-    p.sk_partials = (int*)((uint8_t*)p.exchange + ((2 * (size_t)moe_device_cus() * sizeof(int) + 255) & ~(size_t)255));
+    p.sk_partials = (int*)((uint8_t*)p.exchange + ((2 * (size_t)cus * sizeof(int) + 255) & ~(size_t)255));
     p.y_vec = (uintptr_t)p.Y % 16 == 0 && (p.ydtype == MOE_F32 ? p.ldy % 4 == 0 && p.N % 4 == 0 : p.ldy % 8 == 0 && p.N % 8 == 0);
-    if (p.max_split > 1) hipLaunchKernelGGL(zero_counters_kernel, dim3((unsigned)((2 * cus + 255) / 256)), dim3(256), 0, stream, p.sk_counters, 2 * cus);
     return moe_i8_tile(cus, R, p.E, p.N, p.epi == MOE_I8_SWIGLU) == 128 ? moe_launch_i8_gemm_small(p, R, stream) : launch_epilogue(p, R, stream);
 }

@@ -352,26 +352,30 @@ __global__ void __launch_bounds__(NTHREADS, 2) i8_gemm_kernel(const MoeI8Gemm p)
             float v[8];
             uint32_t top = 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < 8; i += 2) {
                 v[i] = value(mb, i);
-                top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);   // (bits: NaN above infinity above every number)
+                v[i + 1] = value(mb, i + 1);
+                top = max(max(__float_as_uint(v[i]) & 0x7fffffffu, __float_as_uint(v[i + 1]) & 0x7fffffffu), top);   // (bits: NaN above infinity above every number)
             }
             top = max(top, (uint32_t)__shfl_xor((int)top, 16));
             top = max(top, (uint32_t)__shfl_xor((int)top, 32));
             const float amax = __uint_as_float(top);
             const bool fine = top < 0x7f800000u;
             // (a segment below 2^-100 is zero to the 8-bit codes of any row that is not as small as that)
-            const float inv = fine && amax > 0x1p-100f ? (float)MOE_SEG_LEVELS * __builtin_amdgcn_rcpf(amax) : 0.f;
+            const float inv = fine && amax > 0x1p-100f ? MOE_SEG_LEVELS * __builtin_amdgcn_rcpf(amax) : 0.f;
+            if (__any(!fine))   // (its scale says NaN)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = fine ? v[i] : 0.f;
             const int m = mb * 16 + mrow;
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
                 int q[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) q[i] = fine ? (int)rintf(fminf(fmaxf(v[4 * b + i] * inv, -(float)MOE_SEG_LEVELS), (float)MOE_SEG_LEVELS)) : 0;
+                for (int i = 0; i < 4; ++i) q[i] = (int)(v[4 * b + i] * inv);
                 uint2 hi;
                 hi.x = __builtin_amdgcn_perm((uint32_t)q[1], (uint32_t)q[0], 0x06050201u);
                 hi.y = __builtin_amdgcn_perm((uint32_t)q[3], (uint32_t)q[2], 0x06050201u);
-                const uint32_t lo = (uint32_t)(q[0] & 0xff) | (uint32_t)(q[1] & 0xff) << 8 | (uint32_t)(q[2] & 0xff) << 16 | (uint32_t)q[3] << 24;
+                const uint32_t lo = __builtin_amdgcn_perm((uint32_t)q[1], (uint32_t)q[0], 0x0c0c0400u) | __builtin_amdgcn_perm((uint32_t)q[3], (uint32_t)q[2], 0x04000c0cu);
                 *(uint2*)(stg + m * MOE_SEG_BYTES + b * 32 + nq * 2) = hi;
                 *(uint32_t*)(stg + m * MOE_SEG_BYTES + 64 + b * 16 + nq) = lo;
             }

@@ -3,12 +3,14 @@
 //
 // A row v becomes codes q[c] = rne(127 v[c] / a) with a = max |v| and the scale a / 127: the quotient is rounded as it is, not as some fp32 value of
 // it comes out (ties are common: half the maximum is 63.5 for every row of a 2-byte type), so the codes are the same on every path and in any
-// precision that a checker takes.  q is guessed with one multiplication by 127 / a and put right from its remainder 127 v - q a, which fp32 holds
-// exactly for 2-byte types (at most 19 bits: values below a / 254 have q = 0) and fp64 for fp32 values.  A row that holds an infinity or a NaN gets the
-// scale NaN and codes 0, so that every product of it is NaN and no other row changes; a row of zeros the scale 0.
+// precision that a checker takes.  q is guessed with one multiplication by 127 / a and put right from its remainder 127 v - q a: 127 v is held as
+// an fp32 number and its rounding error, and the difference with q a is exact (it is a multiple of half a unit of a's last place and at most a / 2; below a / 254 q
+// is 0).  Gradient rows, products of two or three numbers, are held as an fp32 number and its error from the start.  (In fp64 instead, 8192 x 4096
+// gradient rows took 92 us.)  A row that holds an infinity or a NaN gets the scale NaN and codes 0, so that every product of it is NaN and
+// no other row changes; a row of zeros the scale 0.
 //
-// Interims (h, the saved gate and up, dh) travel as 24-bit integers with a scale for each 32 columns of a row: 3 bytes per value, 2^-24 of the segment's maximum
-// off.  Every value that a rounding on the way carries over a border of the 8-bit codes costs a whole step, so this noise falls with the root of
+// Interims (h, the saved gate and up, dh) travel as 24-bit integers with a scale for each 32 columns of a row: 3 bytes per value, at most 2^-23 of the segment's
+// maximum off.  Every value that a rounding on the way carries over a border of the 8-bit codes costs a whole step, so this noise falls with the root of
 // the rounding only: with 16 bits 1 code in 700 changed and the MLP's error against 64 bits was 1.5e-3 of its result's norm (bf16 rows would be off by four
 // times that), with 24 it is that of fp32 arithmetic, at three quarters of an fp32 tensor's bytes.
 #include "common.h"
@@ -18,74 +20,70 @@ namespace {
 
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 
-__device__ __forceinline__ float wave_max(float v)
+// Magnitudes are compared as bits: those of an infinity lie above every number's, and NaN's above those.
+constexpr uint32_t NOT_FINITE = 0x7f800000u;
+__device__ __forceinline__ uint32_t mag_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+template <typename U> __device__ __forceinline__ U block_max(U v)
 {
+    __shared__ U s_max[16];
 #pragma unroll
-    for (int m = 32; m > 0; m >>= 1) v = fmaxf(v, __shfl_xor(v, m));
-    return v;
-}
-__device__ __forceinline__ double wave_max(double v)
-{
-#pragma unroll
-    for (int m = 32; m > 0; m >>= 1) v = fmax(v, __shfl_xor(v, m));
-    return v;
-}
-
-// Largest value of a workgroup and whether any thread saw something that is not finite (both in every thread).
-template <typename C> __device__ __forceinline__ C block_max(C v, bool& bad)
-{
-    __shared__ C s_max[16];
-    __shared__ int s_bad[16];
-    v = wave_max(v);
-    const bool b = __any(bad);
-    const int wave = threadIdx.x >> 6, nw = blockDim.x >> 6;
-    if ((threadIdx.x & 63) == 0) { s_max[wave] = v; s_bad[wave] = b; }
+    for (int m = 32; m > 0; m >>= 1) { const U o = __shfl_xor(v, m); v = v > o ? v : o; }
+    if (blockDim.x == 64) return v;
+    if ((threadIdx.x & 63) == 0) s_max[threadIdx.x >> 6] = v;
     __syncthreads();
     v = s_max[0];
-    int any = s_bad[0];
-    for (int w = 1; w < nw; ++w) { v = v > s_max[w] ? v : s_max[w]; any |= s_bad[w]; }
-    bad = any != 0;
+    for (int w = 1; w < (int)(blockDim.x >> 6); ++w) v = v > s_max[w] ? v : s_max[w];
     return v;
 }
+// The order of magnitudes |v + lo| of numbers held with their errors, and the error of the magnitude at a place in that order.
+__device__ __forceinline__ unsigned long long mag_key(float v, float lo)
+{
+    const uint32_t b = __float_as_uint(v < 0.f ? -lo : lo);
+    return (unsigned long long)mag_bits(v) << 32 | (b >> 31 ? ~b : b | 0x80000000u);
+}
+__device__ __forceinline__ float key_error(unsigned long long key)
+{
+    const uint32_t b = (uint32_t)key;
+    return __uint_as_float(b >> 31 ? b & 0x7fffffffu : ~b);
+}
 
-__device__ __forceinline__ float mag(float v) { return fabsf(v); }
-__device__ __forceinline__ double mag(double v) { return fabs(v); }
-__device__ __forceinline__ bool finite(float v) { return fabsf(v) <= 3.402823466e38f; }
-__device__ __forceinline__ bool finite(double v) { return fabs(v) <= 1.7976931348623157e308; }
-__device__ __forceinline__ float near_int(float v) { return rintf(v); }
-__device__ __forceinline__ double near_int(double v) { return rint(v); }
-__device__ __forceinline__ float mul_add(float a, float b, float c) { return fmaf(a, b, c); }
-__device__ __forceinline__ double mul_add(double a, double b, double c) { return fma(a, b, c); }
-
-// What a row's values are multiplied by before they meet its maximum, so that 127 v and 127 / a stay inside fp32's range (fp64: 1; a value that the factor
-// makes subnormal is far below half a step).
-__device__ __forceinline__ float row_factor(float a) { return a > 0x1p64f ? 0x1p-64f : a < 0x1p-64f ? 0x1p64f : 1.f; }
-__device__ __forceinline__ double row_factor(double) { return 1.0; }
-
-template <typename C> struct RowCoder {
-    C f, a, inv;
-    float scale;
-    __device__ __forceinline__ RowCoder(C amax, bool bad)
+// What turns values of a row into its codes.  f: what the values are multiplied by first, so that 127 v and 127 / a stay inside fp32's range (a value that the
+// factor makes subnormal is far below half a step).
+struct RowCoder {
+    float f, a, a_lo, inv, scale;
+    __device__ __forceinline__ RowCoder(uint32_t top, float top_lo = 0.f)
     {
-        f = row_factor(amax);
-        a = amax * f;
-        inv = !bad && a > 0 ? (C)127 / a : (C)0;
-        if (inv == (C)0) f = 0;   // every code 0
-        scale = bad ? __uint_as_float(0x7fc00000u) : (float)(amax / (C)127);
+        const float amax = __uint_as_float(top);
+        const bool fine = top < NOT_FINITE;
+        f = amax > 0x1p64f ? 0x1p-64f : amax < 0x1p-64f ? 0x1p64f : 1.f;
+        a = fine ? amax * f : 0.f;
+        a_lo = fine ? top_lo * f : 0.f;
+        inv = a > 0.f ? 127.f / a : 0.f;
+        if (inv == 0.f) f = 0.f;   // every code 0
+        scale = fine ? amax / 127.f : __uint_as_float(0x7fc00000u);
     }
-    __device__ __forceinline__ int code(C v) const
+    // the code of v + lo, lo the rounding error of v
+    __device__ __forceinline__ float exact(float v, float lo) const
     {
-        const C x = f == (C)0 ? (C)0 : v * f;
-        C q = near_int(x * inv);
-        const C r = mul_add(-q, a, (C)127 * x), d = 2 * mag(r);
-        if (d > a || (d == a && ((int)q & 1))) q += r < 0 ? (C)-1 : (C)1;
-        return (int)q;
+        v = f == 0.f ? 0.f : v * f;
+        lo = f == 0.f ? 0.f : lo * f;
+        float q = rintf(v * inv);
+        const float t = 127.f * v, te = fmaf(127.f, v, -t) + 127.f * lo - q * a_lo, r = fmaf(-q, a, t);
+        const float side = copysignf(1.f, r), d = fmaf(2.f, fabsf(r), -a) + (2.f * side * te - a_lo);   // twice the distance to q, minus a step
+        if (d > 0.f || (d == 0.f && a > 0.f && ((int)q & 1))) q += side;
+        return q;
     }
+    // ... of a value that carries fp32 rounding anyway
+    __device__ __forceinline__ float nearest(float v) const { return f == 0.f ? 0.f : rintf(v * f * inv); }
 };
 
-__device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d)
+// four whole numbers of magnitude 127 at most as bytes: 1.5 * 2^23 more, and they stand in the lowest bits
+__device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d)
 {
-    return (uint32_t)(a & 0xff) | (uint32_t)(b & 0xff) << 8 | (uint32_t)(c & 0xff) << 16 | (uint32_t)d << 24;
+    constexpr float M = 12582912.f;
+    const uint32_t ab = __builtin_amdgcn_perm(__float_as_uint(b + M), __float_as_uint(a + M), 0x0c0c0400u);
+    const uint32_t cd = __builtin_amdgcn_perm(__float_as_uint(d + M), __float_as_uint(c + M), 0x04000c0cu);
+    return ab | cd;
 }
 
 // the expert that grouped row m belongs to (E or more: none)
@@ -127,14 +125,14 @@ template <> struct Loader<__half> {
 
 // One workgroup per row.  KEEP: a thread holds its KEEP pieces of 8 columns between the two passes (0: the row is read twice).  SCALED: row m is row
 // pos[m] / fan_out of src times coeff[pos[m]] and, column by column, col_scale[expert of m] (a gradient on its way through the weights' scales).
-// Those products, and fp32 rows, are worked through in fp64 throughout: the quotient that is rounded is that of the exact values to 2^-50.
 template <typename T, bool SCALED, int KEEP>
 __global__ void __launch_bounds__(1024) quantize_rows_kernel(const MoeQuantizeRows p)
 {
-    typedef std::conditional_t<SCALED || std::is_same_v<T, float>, double, float> C;
     const int64_t m = blockIdx.x;
+    if (m == 0)   // side job: the counters of the product behind this launch
+        for (int i = threadIdx.x; i < p.zero_n; i += blockDim.x) p.zero[i] = 0;
     int64_t src_row = m;
-    C coeff = 1;
+    float coeff = 1.f;
     const float* cs = nullptr;
     if (SCALED) {
         int64_t at = m;
@@ -142,7 +140,7 @@ __global__ void __launch_bounds__(1024) quantize_rows_kernel(const MoeQuantizeRo
             at = load_idx(p.pos, m, p.pos64);
             src_row = at / p.fan_out;
         }
-        if (p.coeff) coeff = (C)load_gate(p.coeff, at, p.coeff_dtype);
+        if (p.coeff) coeff = load_gate(p.coeff, at, p.coeff_dtype);
         if (p.col_scale) {
             const int e = expert_of_row(p.offsets, p.off64, p.E, m);
             if (e >= p.E) return;   // behind the last group: no product reads the row
@@ -151,144 +149,154 @@ __global__ void __launch_bounds__(1024) quantize_rows_kernel(const MoeQuantizeRo
     }
     const T* row = (const T*)p.src + src_row * p.lds;
     const int nt = blockDim.x;
-    auto load = [&](int64_t c0, C* v) {
-        float x[8];
-        if (p.vec && c0 + 8 <= p.cols) Loader<T>::ld8(row + c0, x);
+    // eight values and, of products, their rounding errors
+    auto load = [&](int64_t c0, float* v, float* lo) {
+        const bool whole = c0 + 8 <= p.cols;
+        float x[8], s[8];
+        if (p.vec && whole) Loader<T>::ld8(row + c0, x);
         else
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] = c0 + i < p.cols ? Elem<T>::ld(row + c0 + i) : 0.f;
+        if (SCALED && cs) {
+            if (p.vec_scale && whole) Loader<float>::ld8(cs + c0, s);
+            else
+#pragma unroll
+                for (int i = 0; i < 8; ++i) s[i] = c0 + i < p.cols ? cs[c0 + i] : 0.f;
+        }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            v[i] = (C)x[i];
+            v[i] = x[i];
+            lo[i] = 0.f;
             if (SCALED) {
-                v[i] *= coeff;
-                if (cs) v[i] *= c0 + i < p.cols ? (C)cs[c0 + i] : (C)0;
+                const float g = coeff * x[i], ge = fmaf(coeff, x[i], -g);
+                v[i] = g;
+                lo[i] = ge;
+                if (cs) {
+                    v[i] = g * s[i];
+                    lo[i] = fmaf(g, s[i], -v[i]) + ge * s[i];
+                }
             }
         }
     };
-    C keep[KEEP ? KEEP : 1][8];
-    C amax = 0;
-    bool bad = false;
-    auto look = [&](const C* v) {
+    // (the maximum of fp32 products is taken with its error too: left out, it moves borders by 127 * 2^-25 of a step, which would show in an fp32 result and
+    // does not in a 2-byte one)
+    constexpr bool WITH_ERROR = SCALED && std::is_same_v<T, float>;
+    float keep[KEEP ? KEEP : 1][8], low[KEEP ? KEEP : 1][8];
+    std::conditional_t<WITH_ERROR, unsigned long long, uint32_t> top = 0;
+    auto look = [&](const float* v, const float* lo) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            bad |= !finite(v[i]);
-            amax = mag(v[i]) > amax ? mag(v[i]) : amax;
+            if constexpr (WITH_ERROR) { const unsigned long long key = mag_key(v[i], lo[i]); top = key > top ? key : top; }
+            else top = max(top, mag_bits(v[i]));
         }
     };
     if constexpr (KEEP > 0) {
 #pragma unroll
         for (int j = 0; j < KEEP; ++j) {
             const int64_t c0 = ((int64_t)j * nt + threadIdx.x) * 8;
-            if (c0 < p.ldc) { load(c0, keep[j]); look(keep[j]); }
+            if (c0 < p.ldc) { load(c0, keep[j], low[j]); look(keep[j], low[j]); }
         }
     } else {
-        for (int64_t c0 = (int64_t)threadIdx.x * 8; c0 < p.ldc; c0 += (int64_t)nt * 8) { load(c0, keep[0]); look(keep[0]); }
+        for (int64_t c0 = (int64_t)threadIdx.x * 8; c0 < p.ldc; c0 += (int64_t)nt * 8) { load(c0, keep[0], low[0]); look(keep[0], low[0]); }
     }
-    amax = block_max(amax, bad);
-    const RowCoder<C> rc(amax, bad);
+    top = block_max(top);
+    RowCoder rc(0u);
+    if constexpr (WITH_ERROR) rc = RowCoder((uint32_t)(top >> 32), key_error(top));
+    else rc = RowCoder(top);
     int8_t* out = p.codes + m * p.ldc;
-    auto store = [&](int64_t c0, const C* v) {
+    auto store = [&](int64_t c0, const float* v, const float* lo) {
+        float q[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q[i] = rc.exact(v[i], lo[i]);
         uint2 w;
-        w.x = pack4(rc.code(v[0]), rc.code(v[1]), rc.code(v[2]), rc.code(v[3]));
-        w.y = pack4(rc.code(v[4]), rc.code(v[5]), rc.code(v[6]), rc.code(v[7]));
+        w.x = pack4(q[0], q[1], q[2], q[3]);
+        w.y = pack4(q[4], q[5], q[6], q[7]);
         *(uint2*)(out + c0) = w;
     };
     if constexpr (KEEP > 0) {
 #pragma unroll
         for (int j = 0; j < KEEP; ++j) {
             const int64_t c0 = ((int64_t)j * nt + threadIdx.x) * 8;
-            if (c0 < p.ldc) store(c0, keep[j]);
+            if (c0 < p.ldc) store(c0, keep[j], low[j]);
         }
     } else {
-        for (int64_t c0 = (int64_t)threadIdx.x * 8; c0 < p.ldc; c0 += (int64_t)nt * 8) { load(c0, keep[0]); store(c0, keep[0]); }
+        for (int64_t c0 = (int64_t)threadIdx.x * 8; c0 < p.ldc; c0 += (int64_t)nt * 8) { load(c0, keep[0], low[0]); store(c0, keep[0], low[0]); }
     }
     if (threadIdx.x == 0) p.scale[m] = rc.scale;
 }
 
-// columns c0 .. c0 + 7 of a row of segments, times s
+// Columns c0 .. c0 + 7 of a row of segments, times s.  A value's three bytes go to the upper three of a word, so that one conversion makes it a float (256 times
+// what it is: s carries the rest).
 __device__ __forceinline__ void ld8_seg(const uint8_t* row, int64_t c0, float s, float* v)
 {
     const uint8_t* seg = row + c0 / MOE_SEG_COLS * MOE_SEG_BYTES;
     const int c = (int)(c0 % MOE_SEG_COLS);
     const u32x4_t hi = *(const u32x4_t*)(seg + c * 2);
     const uint2 lo = *(const uint2*)(seg + 64 + c);
+    s *= 1.f / 256.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const uint32_t l = (i < 2 ? lo.x : lo.y) >> (16 * (i & 1));
-        v[2 * i] = (float)(((int)(hi[i] << 16) >> 8) | (int)(l & 0xff)) * s;
-        v[2 * i + 1] = (float)(((int)(hi[i] & 0xffff0000u) >> 8) | (int)((l >> 8) & 0xff)) * s;
+        const uint32_t l = i < 2 ? lo.x : lo.y;
+        v[2 * i] = (float)(int)__builtin_amdgcn_perm(hi[i], l, i & 1 ? 0x0504020cu : 0x0504000cu) * s;
+        v[2 * i + 1] = (float)(int)__builtin_amdgcn_perm(hi[i], l, i & 1 ? 0x0706030cu : 0x0706010cu) * s;
     }
 }
 
-// Rows of segments -> codes: the maximum of a row is that of its segments, whose largest integer is MOE_SEG_LEVELS.
+// Rows of segments -> codes: the maximum of a row is that of its segments, MOE_SEG_LEVELS times their scales.
 __global__ void __launch_bounds__(1024) requantize_rows_kernel(const uint8_t* src, const float* seg, int64_t cols, int8_t* codes, int64_t ldc, float* scale)
 {
     const int64_t m = blockIdx.x;
     const int64_t nseg = cols / MOE_SEG_COLS;
-    float top = 0.f;
-    bool bad = false;
-    for (int64_t i = threadIdx.x; i < nseg; i += blockDim.x) {
-        const float s = seg[m * nseg + i];
-        bad |= !finite(s);
-        top = fmaxf(top, s);
-    }
-    top = block_max(top, bad);
-    const float amax = top * (float)MOE_SEG_LEVELS;
-    bad |= !finite(amax);
-    const float f = row_factor(amax);
-    const float inv = !bad && amax > 0.f ? 127.f / (amax * f) : 0.f;
+    uint32_t top = 0;
+    for (int64_t i = threadIdx.x; i < nseg; i += blockDim.x) top = max(top, mag_bits(seg[m * nseg + i] * MOE_SEG_LEVELS));
+    const RowCoder rc(block_max(top));
     for (int64_t c0 = (int64_t)threadIdx.x * 8; c0 < ldc; c0 += (int64_t)blockDim.x * 8) {
         uint2 w = {0u, 0u};
-        if (c0 < cols && inv > 0.f) {
+        if (c0 < cols && rc.f != 0.f) {
             float v[8];
-            ld8_seg(src + m * nseg * MOE_SEG_BYTES, c0, seg[m * nseg + c0 / MOE_SEG_COLS] * f * inv, v);
-            int q[8];
+            ld8_seg(src + m * nseg * MOE_SEG_BYTES, c0, seg[m * nseg + c0 / MOE_SEG_COLS] * rc.f * rc.inv, v);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) q[i] = (int)rintf(fminf(fmaxf(v[i], -127.f), 127.f));
-            w.x = pack4(q[0], q[1], q[2], q[3]);
-            w.y = pack4(q[4], q[5], q[6], q[7]);
+            for (int i = 0; i < 8; ++i) v[i] = rintf(fminf(fmaxf(v[i], -127.f), 127.f));
+            w.x = pack4(v[0], v[1], v[2], v[3]);
+            w.y = pack4(v[4], v[5], v[6], v[7]);
         }
         *(uint2*)(codes + m * ldc + c0) = w;
     }
-    if (threadIdx.x == 0) scale[m] = bad ? __uint_as_float(0x7fc00000u) : amax / 127.f;
+    if (threadIdx.x == 0) scale[m] = rc.scale;
 }
 
 // SwiGLU's backward pass and the codes of the joint row [dgate * s1 | dup * s3] in one pass over dh, gate and up:
 //   dgate = dh up sig(g) (1 + g (1 - sig(g))),  dup = dh g sig(g).
 // One scale for both halves, so that the product behind it is one sum over 2 f codes.
 template <int KEEP>
-__global__ void __launch_bounds__(1024) swiglu_bwd_codes_kernel(const MoeSwigluBwdCodes p)
+__global__ void __launch_bounds__(KEEP == 1 ? 256 : 512) swiglu_bwd_codes_kernel(const MoeSwigluBwdCodes p)
 {
     const int64_t m = blockIdx.x;
     const int e = expert_of_row(p.offsets, p.off64, p.E, m);
     if (e >= p.E) return;
     const float *c1 = p.s1 + (int64_t)e * p.f, *c3 = p.s3 + (int64_t)e * p.f;
     const int64_t nseg = p.f / MOE_SEG_COLS;
+    const uint8_t *dh_row = p.dh + m * nseg * MOE_SEG_BYTES, *gate_row = p.gate + m * nseg * MOE_SEG_BYTES, *up_row = p.up + m * nseg * MOE_SEG_BYTES;
     auto load = [&](int64_t c0, float* a, float* b) {
-        float dh[8], g[8], u[8];
+        float dh[8], g[8], u[8], x1[8], x3[8];
         const int64_t s = m * nseg + c0 / MOE_SEG_COLS;
-        ld8_seg(p.dh + m * nseg * MOE_SEG_BYTES, c0, p.dh_seg[s], dh);
-        ld8_seg(p.gate + m * nseg * MOE_SEG_BYTES, c0, p.gate_seg[s], g);
-        ld8_seg(p.up + m * nseg * MOE_SEG_BYTES, c0, p.up_seg[s], u);
-        float x1[8], x3[8];
+        ld8_seg(dh_row, c0, p.dh_seg[s], dh);
+        ld8_seg(gate_row, c0, p.gate_seg[s], g);
+        ld8_seg(up_row, c0, p.up_seg[s], u);
         Loader<float>::ld8(c1 + c0, x1);
         Loader<float>::ld8(c3 + c0, x3);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float sg = __builtin_amdgcn_rcpf(1.f + __expf(-g[i]));
-            a[i] = dh[i] * u[i] * sg * (1.f + g[i] * (1.f - sg)) * x1[i];
-            b[i] = dh[i] * g[i] * sg * x3[i];
+            const float sg = __builtin_amdgcn_rcpf(1.f + __expf(-g[i])), t = dh[i] * sg;
+            a[i] = t * u[i] * fmaf(g[i], 1.f - sg, 1.f) * x1[i];
+            b[i] = t * g[i] * x3[i];
         }
     };
-    float a[KEEP ? KEEP : 1][8], b[KEEP ? KEEP : 1][8], amax = 0.f;
-    bool bad = false;
+    float a[KEEP ? KEEP : 1][8], b[KEEP ? KEEP : 1][8];
+    uint32_t top = 0;
     auto look = [&](const float* v) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            bad |= !finite(v[i]);
-            amax = fmaxf(amax, fabsf(v[i]));
-        }
+        for (int i = 0; i < 8; ++i) top = max(top, mag_bits(v[i]));
     };
     if constexpr (KEEP > 0) {
 #pragma unroll
@@ -299,13 +307,15 @@ __global__ void __launch_bounds__(1024) swiglu_bwd_codes_kernel(const MoeSwigluB
     } else {
         for (int64_t c0 = (int64_t)threadIdx.x * 8; c0 < p.f; c0 += (int64_t)blockDim.x * 8) { load(c0, a[0], b[0]); look(a[0]); look(b[0]); }
     }
-    amax = block_max(amax, bad);
-    const RowCoder<float> rc(amax, bad);
+    const RowCoder rc(block_max(top));
     int8_t* out = p.codes + m * 2 * p.ldc;
     auto store = [&](int8_t* at, const float* v) {
+        float q[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q[i] = rc.nearest(v[i]);
         uint2 w;
-        w.x = pack4(rc.code(v[0]), rc.code(v[1]), rc.code(v[2]), rc.code(v[3]));
-        w.y = pack4(rc.code(v[4]), rc.code(v[5]), rc.code(v[6]), rc.code(v[7]));
+        w.x = pack4(q[0], q[1], q[2], q[3]);
+        w.y = pack4(q[4], q[5], q[6], q[7]);
         *(uint2*)at = w;
     };
     if constexpr (KEEP > 0) {
@@ -328,8 +338,21 @@ __global__ void __launch_bounds__(1024) swiglu_bwd_codes_kernel(const MoeSwigluB
     if (threadIdx.x == 0) p.scale[m] = rc.scale;
 }
 
-// Expert matrices of any strides -> [E][N][ldo], contiguous along the contraction, zeros from K on.  64 x 64 tiles through LDS: the loads run along
-// whichever dimension is contiguous, the stores along the contraction.
+// Expert matrices whose rows are contiguous but not 16-byte aligned -> the same rows at a pitch of ldo, a multiple of 16.  16 bytes per lane, unaligned loads.
+__global__ void __launch_bounds__(256) repitch_codes_kernel(const int8_t* W, int64_t swe, int64_t ldw, int64_t rows, int64_t cols, int8_t* out, int64_t ldo)
+{
+    const int64_t pieces = ldo / 16, i = (int64_t)blockIdx.x * 256 + threadIdx.x, r = i / pieces, c = (i - r * pieces) * 16, e = blockIdx.y;
+    if (r >= rows) return;
+    const int8_t* src = W + e * swe + r * ldw + c;
+    union { u32x4_t v; int8_t b[16]; } w;
+    if (c + 16 <= cols) __builtin_memcpy(&w.v, src, 16);
+    else
+#pragma unroll
+        for (int j = 0; j < 16; ++j) w.b[j] = c + j < cols ? src[j] : (int8_t)0;
+    *(u32x4_t*)(out + (e * rows + r) * ldo + c) = w.v;
+}
+
+// Expert matrices contiguous along neither dimension -> [E][N][ldo], contiguous along the contraction, zeros from K on; 64 x 64 tiles through LDS.
 __global__ void __launch_bounds__(256) pack_codes_kernel(const int8_t* W, int64_t swe, int64_t swk, int64_t swn, int64_t K, int64_t N, int8_t* out, int64_t ldo)
 {
     __shared__ int8_t tile[64][68];
@@ -360,7 +383,7 @@ __global__ void __launch_bounds__(256) weight_max_kernel(const T* W, int64_t swe
         const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x, k0 = (int64_t)blockIdx.y * 256;
         if (n >= N) return;
         for (int64_t k = k0; k < k0 + 256 && k < K; ++k) {
-            const uint32_t b = __float_as_uint(Elem<T>::ld(W + e * swe + k * swk + n * swn)) & 0x7fffffffu;
+            const uint32_t b = mag_bits(Elem<T>::ld(W + e * swe + k * swk + n * swn));
             best = b > best ? b : best;
         }
         atomicMax(top + e * N + n, best);
@@ -368,7 +391,7 @@ __global__ void __launch_bounds__(256) weight_max_kernel(const T* W, int64_t swe
         const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
         if (n >= N) return;
         for (int64_t k = threadIdx.x & 63; k < K; k += 64) {
-            const uint32_t b = __float_as_uint(Elem<T>::ld(W + e * swe + k * swk + n * swn)) & 0x7fffffffu;
+            const uint32_t b = mag_bits(Elem<T>::ld(W + e * swe + k * swk + n * swn));
             best = b > best ? b : best;
         }
 #pragma unroll
@@ -381,16 +404,14 @@ template <typename T>
 __global__ void __launch_bounds__(256) weight_codes_kernel(const T* W, int64_t swe, int64_t swk, int64_t swn, int64_t K, int64_t N, const uint32_t* top,
                                                            int8_t* codes, int64_t sce, int64_t sck, int64_t scn, float* scale)
 {
-    typedef std::conditional_t<std::is_same_v<T, float>, double, float> C;
     const int64_t e = blockIdx.z;
     const bool along_n = swn <= swk;
     const int64_t inner = (int64_t)blockIdx.x * 256 + threadIdx.x;
     for (int64_t j = (int64_t)blockIdx.y * 16; j < (int64_t)blockIdx.y * 16 + 16; ++j) {
         const int64_t k = along_n ? j : inner, n = along_n ? inner : j;
         if (k >= K || n >= N) continue;
-        const float a = __uint_as_float(top[e * N + n]);
-        const RowCoder<C> rc((C)a, !finite(a));
-        codes[e * sce + k * sck + n * scn] = (int8_t)rc.code((C)Elem<T>::ld(W + e * swe + k * swk + n * swn));
+        const RowCoder rc(top[e * N + n]);
+        codes[e * sce + k * sck + n * scn] = (int8_t)(int)rc.exact(Elem<T>::ld(W + e * swe + k * swk + n * swn), 0.f);
         if (k == 0) scale[e * N + n] = rc.scale;
     }
 }
@@ -423,6 +444,7 @@ int moe_launch_quantize_rows(const MoeQuantizeRows& p_, int dtype, int64_t rows,
     const bool scaled = p.pos || p.coeff || p.col_scale;
     MOE_DISPATCH_DTYPE(dtype, {
         p.vec = (uintptr_t)p.src % 16 == 0 && (p.lds * sizeof(T)) % 16 == 0;
+        p.vec_scale = (uintptr_t)p.col_scale % 16 == 0 && p.cols % 4 == 0;
         return scaled ? launch_quantize_t<T, true>(p, rows, stream) : launch_quantize_t<T, false>(p, rows, stream);
     });
 }
@@ -439,11 +461,18 @@ int moe_launch_swiglu_bwd_codes(const MoeSwigluBwdCodes& p, int64_t rows, hipStr
 {
     if (rows == 0) return MOE_OK;
     const int64_t pieces = p.f / 8;
-    const int nt = pieces <= 64 ? 64 : pieces <= 128 ? 128 : pieces <= 512 ? 256 : pieces <= 1024 ? 512 : 1024;
+    const int nt = pieces <= 64 ? 64 : pieces <= 128 ? 128 : pieces <= 256 ? 256 : 512;
     const int64_t keep = (pieces + nt - 1) / nt;
-    if (keep <= 1) hipLaunchKernelGGL(swiglu_bwd_codes_kernel<1>, dim3((unsigned)rows), dim3(nt), 0, stream, p);
+    if (keep <= 1 && nt <= 256) hipLaunchKernelGGL(swiglu_bwd_codes_kernel<1>, dim3((unsigned)rows), dim3(nt), 0, stream, p);
     else if (keep <= 2) hipLaunchKernelGGL(swiglu_bwd_codes_kernel<2>, dim3((unsigned)rows), dim3(nt), 0, stream, p);
+    else if (keep <= 4) hipLaunchKernelGGL(swiglu_bwd_codes_kernel<4>, dim3((unsigned)rows), dim3(nt), 0, stream, p);
     else hipLaunchKernelGGL(swiglu_bwd_codes_kernel<0>, dim3((unsigned)rows), dim3(nt), 0, stream, p);
+    return moe_launch_status();
+}
+
+int moe_launch_repitch_codes(const int8_t* W, int64_t swe, int64_t ldw, int E, int64_t rows, int64_t cols, int8_t* out, int64_t ldo, hipStream_t stream)
+{
+    hipLaunchKernelGGL(repitch_codes_kernel, dim3((unsigned)((rows * (ldo / 16) + 255) / 256), (unsigned)E), dim3(256), 0, stream, W, swe, ldw, rows, cols, out, ldo);
     return moe_launch_status();
 }
 

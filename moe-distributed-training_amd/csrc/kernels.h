@@ -214,8 +214,9 @@ int moe_launch_swiglu_bwd(const void* g, const void* u, const void* dh, void* dg
 
 // ---- expert products in 8-bit integers (int8_rows.hip, int8_gemm.hip)
 // interims between two products: segments of 32 columns of a row as 24-bit integers that share a scale, 96 bytes each: the upper 16 bits of the 32 values, then
-// their lower 8; [R][N / 32] of them
-constexpr int MOE_SEG_COLS = 32, MOE_SEG_BYTES = 96, MOE_SEG_LEVELS = 8388607;
+// their lower 8; [R][N / 32] of them.  The maximum of a segment is MOE_SEG_LEVELS steps, far enough from 2^23 for a reciprocal that is off by its last bit.
+constexpr int MOE_SEG_COLS = 32, MOE_SEG_BYTES = 96;
+constexpr float MOE_SEG_LEVELS = 8388600.f;
 constexpr int MOE_I8_KTILE = 128;       // codes of a row come in whole K tiles, zeros behind the last column
 constexpr int64_t MOE_I8_MAX_K = 131071;   // 128 * 128 * K < 2^31: the sums are exact in 32 bits
 inline int64_t moe_i8_pitch(int64_t cols) { return (cols + MOE_I8_KTILE - 1) / MOE_I8_KTILE * MOE_I8_KTILE; }
@@ -229,7 +230,8 @@ struct MoeQuantizeRows {
     const float* col_scale; const void* offsets; int off64; int E;
     int8_t* codes; int64_t ldc; float* scale;
     int64_t cols;
-    int vec;                // (set by the launcher) rows of src are 16-byte aligned
+    int* zero; int zero_n;  // side job of the launch: cleared
+    int vec, vec_scale;     // (set by the launcher) rows of src, of col_scale, are 16-byte aligned
 };
 int moe_launch_quantize_rows(const MoeQuantizeRows& p, int dtype, int64_t rows, hipStream_t stream);
 int moe_launch_requantize_rows(const uint8_t* src, const float* seg, int64_t rows, int64_t cols, int8_t* codes, int64_t ldc, float* scale, hipStream_t stream);
@@ -243,6 +245,7 @@ struct MoeSwigluBwdCodes {
     int64_t f;
 };
 int moe_launch_swiglu_bwd_codes(const MoeSwigluBwdCodes& p, int64_t rows, hipStream_t stream);
+int moe_launch_repitch_codes(const int8_t* W, int64_t swe, int64_t ldw, int E, int64_t rows, int64_t cols, int8_t* out, int64_t ldo, hipStream_t stream);
 int moe_launch_pack_codes(const int8_t* W, int64_t swe, int64_t swk, int64_t swn, int E, int64_t K, int64_t N, int8_t* out, int64_t ldo, hipStream_t stream);
 int moe_launch_quantize_weights(const void* W, int64_t swe, int64_t swk, int64_t swn, int dtype, int E, int64_t K, int64_t N, int8_t* codes, int64_t sce,
                                 int64_t sck, int64_t scn, float* scale, uint32_t* top, hipStream_t stream);
@@ -264,13 +267,14 @@ struct MoeI8Gemm {
     const void* pos; int pos64; const void* offsets; int off64;
     int E; int64_t K, N;                // K: of one segment
     int fan_out, x_grouped, y_grouped, epi;
-    void* exchange;                     // moe_i8_exchange_bytes
+    void* exchange;                     // moe_i8_exchange_bytes; the first moe_i8_counters() ints of it zero at launch, and left so
     // set by the launcher
     int num_cus, max_split;             // workgroups of a round of the tile plan; K parts that a tile may be cut into
     int *sk_counters, *sk_partials;
     int y_vec;                          // rows of Y take 16-byte stores
 };
 constexpr int MOE_I8_MIN_PART = 4;
+int moe_i8_counters();                  // ints at the start of the exchange area
 int moe_i8_tile(int cus, int64_t R, int E, int64_t N, bool pair);
 int moe_launch_i8_gemm_small(const MoeI8Gemm& p, int64_t R, hipStream_t stream);
 // whether the kernel reads W in this orientation and alignment (otherwise: moe_launch_pack_codes first)

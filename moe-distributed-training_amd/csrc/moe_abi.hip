@@ -1041,15 +1041,14 @@ int moe_mlp_bwd(const void* dy, int64_t lddy, int dy_grouped, int dy_fan_out, co
 }
 
 // ---- expert products in 8-bit integers -------------------------------------------------------------------------
-int moe_quantize_rows(const void* src, int64_t lds, int dtype, const void* pos, int pos64, int fan_out, const void* coeff, int coeff_dtype,
-                      const float* col_scale, const void* offsets, int off64, int E, int8_t* codes, int64_t ldc, float* scale, int64_t nrows,
-                      int64_t ncols, void* stream)
+int moe_quantize_rows(const void* src, int64_t lds, int dtype, int8_t* codes, int64_t ldc, float* scale, int64_t nrows, int64_t ncols, void* stream)
 {
     if (dtype < 0 || dtype > 2 || nrows < 0 || ncols < 0 || ldc < ncols || ldc % 16 != 0) return MOE_ERR_BAD_ARG;
     if (nrows == 0) return MOE_OK;
-    if (!src || !codes || !scale || !aligned16(codes) || (pos && fan_out < 1) || (coeff && (coeff_dtype < 0 || coeff_dtype > 2)) || (col_scale && (!offsets || E < 1))) return MOE_ERR_BAD_ARG;
+    if (!src || !codes || !scale || !aligned16(codes)) return MOE_ERR_BAD_ARG;
     if (nrows > 0x7fffffff) return MOE_ERR_UNSUPPORTED;
-    const MoeQuantizeRows q = {src, lds, pos, pos64, fan_out, coeff, coeff_dtype, col_scale, offsets, off64, E, codes, ldc, scale, ncols, 0};
+    MoeQuantizeRows q = {};
+    q.src = src; q.lds = lds; q.codes = codes; q.ldc = ldc; q.scale = scale; q.cols = ncols;
     return moe_launch_quantize_rows(q, dtype, nrows, S(stream));
 }
 
@@ -1065,49 +1064,93 @@ int moe_quantize_weights(const void* W, int64_t swe, int64_t swk, int64_t swn, i
 }
 
 namespace {
-// the weights of a product as its kernel reads them: in place (contiguous along k or along n, 16-byte aligned rows), or a copy contiguous along k
-struct I8Weights { bool in_place; int nn; int64_t swe, ldw; size_t bytes; };
+inline size_t i8_codes_bytes(int64_t rows, int64_t pitch) { return al((size_t)rows * pitch) + al((size_t)rows * 4); }
+
+// the weights of a product as its kernel reads them: in place (contiguous along k or along n, 16-byte aligned rows), a copy of such rows that are aligned, or, of
+// matrices contiguous along neither, one contiguous along k
+struct I8Weights { int copy, nn; int64_t swe, ldw; size_t bytes; };   // copy: 0 none, 1 rows, 2 transposed
 I8Weights i8_weights(const void* W, int64_t swe, int64_t swk, int64_t swn, int E, int64_t K, int64_t N)
 {
-    if (swk == 1 && moe_i8_weights_ok(W, swe, swn)) return {true, 0, swe, swn, 0};
-    if (swn == 1 && moe_i8_weights_ok(W, swe, swk)) return {true, 1, swe, swk, 0};
-    const int64_t ld = (K + 15) / 16 * 16;
-    return {false, 0, N * ld, ld, al((size_t)E * (size_t)N * (size_t)ld)};
+    if (swk == 1 && moe_i8_weights_ok(W, swe, swn)) return {0, 0, swe, swn, 0};
+    if (swn == 1 && moe_i8_weights_ok(W, swe, swk)) return {0, 1, swe, swk, 0};
+    const int nn = swn == 1 && swk != 1;
+    const int64_t rows = nn ? K : N, ld = ((nn ? N : K) + 15) / 16 * 16;
+    return {swn == 1 || swk == 1 ? 1 : 2, nn, rows * ld, ld, al((size_t)E * (size_t)rows * (size_t)ld)};
+}
+
+size_t i8_linear_bytes(const I8Weights& w, int64_t code_rows, int64_t R, int E, int64_t K, int64_t N)
+{
+    return i8_codes_bytes(code_rows, moe_i8_pitch(K)) + w.bytes + moe_i8_exchange_bytes(R, E, K, N, false);
+}
+
+// codes of the rows that q describes, and their product; g: what the caller knows of it
+int i8_linear(MoeQuantizeRows q, MoeI8Gemm g, int dtype, const I8Weights& w, const int8_t* W, int64_t swe, int64_t swk, int64_t swn, int64_t code_rows, int64_t R,
+              void* workspace, hipStream_t st)
+{
+    Bump b(workspace, i8_linear_bytes(w, code_rows, R, g.E, g.K, g.N));
+    const int64_t pitch = moe_i8_pitch(g.K);
+    q.codes = (int8_t*)b.take((size_t)code_rows * pitch); q.ldc = pitch; q.scale = (float*)b.take((size_t)code_rows * 4); q.cols = g.K;
+    g.X = q.codes; g.ldx = pitch; g.x_scale = q.scale;
+    int8_t* copy = w.copy ? (int8_t*)b.take(w.bytes) : nullptr;
+    g.W[0] = copy ? copy : W; g.swe = w.swe; g.ldw = w.ldw; g.nn = w.nn; g.nseg = 1;
+    g.exchange = b.take(moe_i8_exchange_bytes(R, g.E, g.K, g.N, false));
+    q.zero = (int*)g.exchange; q.zero_n = moe_i8_counters();
+    g.epi = MOE_I8_STORE;
+    if (!moe_i8_gemm_supported(g, R, code_rows)) return MOE_ERR_UNSUPPORTED;
+    { TIMED("i8_codes"); TRY(moe_launch_quantize_rows(q, dtype, code_rows, st)); }
+    if (w.copy) {
+        TIMED("i8_weights_copy");
+        if (w.copy == 1) TRY(moe_launch_repitch_codes(W, swe, w.nn ? swk : swn, g.E, w.nn ? g.K : g.N, w.nn ? g.N : g.K, copy, w.ldw, st));
+        else TRY(moe_launch_pack_codes(W, swe, swk, swn, g.E, g.K, g.N, copy, w.ldw, st));
+    }
+    TIMED("i8_gemm");
+    return moe_launch_i8_gemm(g, R, st);
 }
 }  // namespace
 
-size_t moe_scatter2scatter_int8_workspace_bytes(const int8_t* W, int64_t swe, int64_t swk, int64_t swn, int64_t R, int E, int64_t K, int64_t N)
+size_t moe_linear_int8_workspace_bytes(const int8_t* W, int64_t swe, int64_t swk, int64_t swn, int64_t code_rows, int64_t R, int E, int64_t K, int64_t N)
 {
-    if (R < 1 || E < 1 || K < 1 || N < 1) return 0;
-    return i8_weights(W, swe, swk, swn, E, K, N).bytes + moe_i8_exchange_bytes(R, E, K, N, false);
+    if (code_rows < 1 || R < 1 || E < 1 || K < 1 || N < 1) return 0;
+    return i8_linear_bytes(i8_weights(W, swe, swk, swn, E, K, N), code_rows, R, E, K, N);
 }
 
-int moe_scatter2scatter_int8(const int8_t* X, int64_t ldx, const float* x_scale, const int8_t* W, int64_t swe, int64_t swk, int64_t swn,
-                             const float* w_scale, void* Y, int64_t ldy, int dtype, const void* pos, int pos64, const void* offsets, int off64, int E,
-                             int64_t R, int64_t K, int64_t N, int fan_out, int x_grouped, int y_grouped, void* workspace, size_t workspace_bytes,
-                             void* stream)
+int moe_linear_int8_fwd(const void* x, int64_t ldx, int64_t x_rows, int dtype, const int8_t* W, int64_t swe, int64_t swk, int64_t swn,
+                        const float* w_scale, void* y, int64_t ldy, const void* pos, int pos64, const void* offsets, int off64, int E, int64_t R, int64_t K,
+                        int64_t N, int fan_out, int x_grouped, int y_grouped, void* workspace, size_t workspace_bytes, void* stream)
 {
-    hipStream_t st = S(stream);
-    if (dtype < 0 || dtype > 2 || E < 1 || R < 0 || K < 1 || N < 0 || fan_out < 1 || ldx < moe_i8_pitch(K) || ldx % 16 != 0 || ldy < N) return MOE_ERR_BAD_ARG;
+    if (dtype < 0 || dtype > 2 || E < 1 || R < 0 || x_rows < 0 || K < 1 || N < 0 || fan_out < 1 || ldx < K || ldy < N) return MOE_ERR_BAD_ARG;
     if (R == 0 || N == 0) return MOE_OK;
-    if (!X || !x_scale || !W || !Y || !offsets || !aligned16(X) || ((!x_grouped || !y_grouped) && !pos)) return MOE_ERR_BAD_ARG;
-    if (K > MOE_I8_MAX_K || E > 65535) return MOE_ERR_UNSUPPORTED;
+    if (!x || x_rows < 1 || !W || !w_scale || !y || !offsets || ((!x_grouped || !y_grouped) && !pos) || (x_grouped && x_rows < R)) return MOE_ERR_BAD_ARG;
+    if (K > MOE_I8_MAX_K || E > 65535 || x_rows > 0x7fffffff) return MOE_ERR_UNSUPPORTED;
     const I8Weights w = i8_weights(W, swe, swk, swn, E, K, N);
-    if (!workspace || workspace_bytes < moe_scatter2scatter_int8_workspace_bytes(W, swe, swk, swn, R, E, K, N)) return MOE_ERR_WORKSPACE;
-    Bump b(workspace, workspace_bytes);
+    if (!workspace || workspace_bytes < i8_linear_bytes(w, x_rows, R, E, K, N)) return MOE_ERR_WORKSPACE;
+    MoeQuantizeRows q = {};
+    q.src = x; q.lds = ldx;
     MoeI8Gemm g = {};
-    g.X = X; g.ldx = ldx; g.x_scale = x_scale;
-    g.W[0] = W; g.swe = w.swe; g.ldw = w.ldw; g.nn = w.nn; g.nseg = 1; g.w_scale[0] = w_scale;
-    g.Y = Y; g.ldy = ldy; g.ydtype = dtype;
+    g.w_scale[0] = w_scale; g.Y = y; g.ldy = ldy; g.ydtype = dtype;
     g.pos = pos; g.pos64 = pos64; g.offsets = offsets; g.off64 = off64; g.E = E; g.K = K; g.N = N;
-    g.fan_out = fan_out; g.x_grouped = x_grouped; g.y_grouped = y_grouped; g.epi = MOE_I8_STORE;
-    int8_t* packed = w.in_place ? nullptr : (int8_t*)b.take(w.bytes);
-    g.exchange = b.take(moe_i8_exchange_bytes(R, E, K, N, false));
-    if (packed) g.W[0] = packed;
-    if (!moe_i8_gemm_supported(g, R, (R + fan_out - 1) / fan_out)) return MOE_ERR_UNSUPPORTED;
-    if (packed) { TIMED("i8_pack"); TRY(moe_launch_pack_codes(W, swe, swk, swn, E, K, N, packed, w.ldw, st)); }
-    TIMED("i8_gemm");
-    return moe_launch_i8_gemm(g, R, st);
+    g.fan_out = fan_out; g.x_grouped = x_grouped; g.y_grouped = y_grouped;
+    return i8_linear(q, g, dtype, w, W, swe, swk, swn, x_rows, R, workspace, S(stream));
+}
+
+int moe_linear_int8_bwd(const void* dy, int64_t lddy, int dtype, int dy_grouped, int dy_fan_out, const void* gates, int gates_dtype, const int8_t* W,
+                        int64_t swe, int64_t swk, int64_t swn, const float* w_scale, void* dx_rows, int64_t lddx, int dx_grouped, const void* pos, int pos64,
+                        const void* offsets, int off64, int E, int64_t R, int64_t K, int64_t N, void* workspace, size_t workspace_bytes, void* stream)
+{
+    if (dtype < 0 || dtype > 2 || E < 1 || R < 0 || K < 0 || N < 1 || dy_fan_out < 1 || lddy < N || lddx < K || (gates && (gates_dtype < 0 || gates_dtype > 2))) return MOE_ERR_BAD_ARG;
+    if (R == 0 || K == 0) return MOE_OK;
+    if (!dy || !W || !w_scale || !dx_rows || !offsets || ((!dy_grouped || !dx_grouped) && !pos)) return MOE_ERR_BAD_ARG;
+    if (N > MOE_I8_MAX_K || E > 65535 || R > 0x7fffffff) return MOE_ERR_UNSUPPORTED;
+    const I8Weights w = i8_weights(W, swe, swn, swk, E, N, K);   // W^T: the contraction runs over N
+    if (!workspace || workspace_bytes < i8_linear_bytes(w, R, R, E, N, K)) return MOE_ERR_WORKSPACE;
+    MoeQuantizeRows q = {};
+    q.src = dy; q.lds = lddy; q.pos = dy_grouped ? nullptr : pos; q.pos64 = pos64; q.fan_out = dy_fan_out; q.coeff = gates; q.coeff_dtype = gates_dtype;
+    q.col_scale = w_scale; q.offsets = offsets; q.off64 = off64; q.E = E;
+    MoeI8Gemm g = {};
+    g.Y = dx_rows; g.ldy = lddx; g.ydtype = dtype;
+    g.pos = pos; g.pos64 = pos64; g.offsets = offsets; g.off64 = off64; g.E = E; g.K = N; g.N = K;
+    g.fan_out = 1; g.x_grouped = 1; g.y_grouped = dx_grouped;
+    return i8_linear(q, g, dtype, w, W, swe, swn, swk, R, R, workspace, S(stream));
 }
 
 namespace {
@@ -1120,7 +1163,6 @@ inline I8Seg take_seg(Bump& b, int64_t R, int64_t N)
     s.s = (float*)b.take((size_t)R * (N / MOE_SEG_COLS) * 4);
     return s;
 }
-inline size_t i8_codes_bytes(int64_t rows, int64_t pitch) { return al((size_t)rows * pitch) + al((size_t)rows * 4); }
 inline bool i8_mlp_sizes_ok(int64_t d, int64_t f) { return d >= 64 && f >= 64 && d % 64 == 0 && f % 64 == 0; }
 }  // namespace
 
@@ -1177,7 +1219,8 @@ int moe_mlp_int8_fwd(const void* x, int64_t ldx, int64_t x_rows, int dtype, cons
     g2.fan_out = 1; g2.x_grouped = 1; g2.y_grouped = y_grouped; g2.epi = MOE_I8_STORE; g2.exchange = exchange;
     if (!moe_i8_gemm_supported(g, R, x_rows) || !moe_i8_gemm_supported(g2, R, R)) return MOE_ERR_UNSUPPORTED;
 
-    const MoeQuantizeRows q = {x, ldx, nullptr, 0, 1, nullptr, 0, nullptr, nullptr, 0, 0, xq, dp, xs, d, 0};
+    MoeQuantizeRows q = {};
+    q.src = x; q.lds = ldx; q.codes = xq; q.ldc = dp; q.scale = xs; q.cols = d; q.zero = (int*)exchange; q.zero_n = moe_i8_counters();
     { TIMED("i8_codes_x"); TRY(moe_launch_quantize_rows(q, dtype, x_rows, st)); }
     { TIMED("i8_gemm_gate_up"); TRY(moe_launch_i8_gemm(g, R, st)); }
     { TIMED("i8_codes_h"); TRY(moe_launch_requantize_rows(h.v, h.s, R, f, hq, fp, hs, st)); }
@@ -1222,7 +1265,10 @@ int moe_mlp_int8_bwd(const void* dy, int64_t lddy, int dtype, int dy_grouped, in
     g2.fan_out = 1; g2.x_grouped = 1; g2.y_grouped = 0; g2.epi = MOE_I8_STORE; g2.exchange = exchange;
     if (!moe_i8_gemm_supported(g, R, R) || !moe_i8_gemm_supported(g2, R, R)) return MOE_ERR_UNSUPPORTED;
 
-    const MoeQuantizeRows q = {dy, lddy, dy_grouped ? nullptr : pos, pos64, dy_fan_out, gates, gates_dtype, s2, offsets, off64, E, gq, dp, gs, d, 0};
+    MoeQuantizeRows q = {};
+    q.src = dy; q.lds = lddy; q.pos = dy_grouped ? nullptr : pos; q.pos64 = pos64; q.fan_out = dy_fan_out; q.coeff = gates; q.coeff_dtype = gates_dtype;
+    q.col_scale = s2; q.offsets = offsets; q.off64 = off64; q.E = E; q.codes = gq; q.ldc = dp; q.scale = gs; q.cols = d;
+    q.zero = (int*)exchange; q.zero_n = moe_i8_counters();
     const MoeSwigluBwdCodes a = {dh.v, gate.v, up.v, dh.s, gate.s, up.s, s1, s3, offsets, off64, E, aq, fp, as, f};
     { TIMED("i8_codes_dy"); TRY(moe_launch_quantize_rows(q, dtype, R, st)); }
     { TIMED("i8_gemm_dh"); TRY(moe_launch_i8_gemm(g, R, st)); }

@@ -3,21 +3,6 @@
 
 inline int64_t code_pitch(int64_t cols) { return (cols + 127) / 128 * 128; }
 
-struct Codes { Tensor q, scale; };   // q: (rows, pitch)
-
-Codes empty_codes(const Tensor& like, int64_t rows, int64_t cols)
-{
-    return {at::empty({rows, code_pitch(cols)}, like.options().dtype(at::kChar)), at::empty({rows}, like.options().dtype(at::kFloat))};
-}
-
-Codes row_codes(const Tensor& x)
-{
-    Codes c = empty_codes(x, x.size(0), x.size(1));
-    check(moe_quantize_rows(ptr(x), x.stride(0), dtype_code(x), nullptr, 0, 1, nullptr, 0, nullptr, nullptr, 0, 0, (int8_t*)ptr(c.q), c.q.stride(0),
-                            (float*)ptr(c.scale), x.size(0), x.size(1), stream_of(x)), "moe_quantize_rows");
-    return c;
-}
-
 // (codes (rows, cols), scale (rows)); the codes are a view of whole 128-column pieces
 variable_list quantize_rows(const Tensor& x_)
 {
@@ -26,8 +11,9 @@ variable_list quantize_rows(const Tensor& x_)
     dtype_code(x_);
     const c10::DeviceGuard guard(x_.device());
     const Tensor x = unit_inner(x_.detach());
-    const Codes c = row_codes(x);
-    return {c.q.narrow(1, 0, x.size(1)), c.scale};
+    Tensor q = at::empty({x.size(0), code_pitch(x.size(1))}, x.options().dtype(at::kChar)), scale = at::empty({x.size(0)}, x.options().dtype(at::kFloat));
+    check(moe_quantize_rows(ptr(x), x.stride(0), dtype_code(x), (int8_t*)ptr(q), q.stride(0), (float*)ptr(scale), x.size(0), x.size(1), stream_of(x)), "moe_quantize_rows");
+    return {q.narrow(1, 0, x.size(1)), scale};
 }
 
 // (E, K, N) -> codes (E, K, N) in w's orientation, rows padded to 16 bytes, and scale (E, N)
@@ -60,30 +46,33 @@ void check_codes(const Tensor& q, const Tensor& scale, int64_t E, int64_t N)
                 N, " output columns");
 }
 
-// rows of codes through W, strides those of (E, K, N); scale may be undefined
-Tensor product_int8(const Codes& x, const Tensor& W, const Tensor& scale, at::ScalarType dt, const Tensor& ssi, const Tensor& eo, int64_t k, bool x_grouped,
-                    bool y_grouped)
+Tensor linear_int8_rows(const Tensor& x, const Tensor& W, const Tensor& scale, const Tensor& ssi, const Tensor& eo, const LinearCfg& c)
 {
-    const int64_t L = ssi.size(0), E = W.size(0), K = W.size(1), N = W.size(2);
-    Tensor out = at::empty({L, N}, x.q.options().dtype(dt));
-    if (L == 0 || N == 0) return out;
+    const int64_t R = ssi.size(0), E = W.size(0), K = W.size(1), N = W.size(2);
+    Tensor y = at::empty({R, N}, x.options());
+    if (R == 0 || N == 0) return y;
     const int8_t* w = (const int8_t*)ptr(W);
-    Tensor ws = bytes_on(x.q, moe_scatter2scatter_int8_workspace_bytes(w, W.stride(0), W.stride(1), W.stride(2), L, (int)E, K, N));
-    check(moe_scatter2scatter_int8((const int8_t*)ptr(x.q), x.q.stride(0), (const float*)ptr(x.scale), w, W.stride(0), W.stride(1), W.stride(2),
-                                   (const float*)ptr(scale), ptr(out), out.stride(0), dtype_code(out), ptr(ssi), is64(ssi), ptr(eo), is64(eo), (int)E, L, K, N,
-                                   (int)k, x_grouped, y_grouped, ptr(ws), (size_t)ws.numel(), stream_of(out)), "moe_scatter2scatter_int8");
-    return out;
+    Tensor ws = bytes_on(x, moe_linear_int8_workspace_bytes(w, W.stride(0), W.stride(1), W.stride(2), x.size(0), R, (int)E, K, N));
+    check(moe_linear_int8_fwd(ptr(x), x.stride(0), x.size(0), dtype_code(x), w, W.stride(0), W.stride(1), W.stride(2), (const float*)ptr(scale), ptr(y), y.stride(0),
+                              ptr(ssi), is64(ssi), ptr(eo), is64(eo), (int)E, R, K, N, (int)c.k, c.grouped_in, c.grouped_out, ptr(ws), (size_t)ws.numel(), stream_of(x)),
+          "moe_linear_int8_fwd");
+    return y;
 }
 
-// codes of the gradient rows in grouped order, weighted by their gates and, column by column, by their expert's scales
-Codes gradient_codes(const Tensor& dout, const Tensor& gates, int64_t gate_fan, const Tensor& scale, const Tensor& ssi, const Tensor& eo, bool grouped)
+// rows of dx, at their flat positions or grouped
+Tensor linear_int8_dx_rows(const Tensor& dout, const Tensor& gates, int64_t gate_fan, const Tensor& W, const Tensor& scale, const Tensor& ssi, const Tensor& eo,
+                           bool dy_grouped, bool dx_grouped)
 {
-    const int64_t L = ssi.size(0), N = dout.size(1);
-    Codes c = empty_codes(dout, L, N);
-    check(moe_quantize_rows(ptr(dout), dout.stride(0), dtype_code(dout), grouped ? nullptr : ptr(ssi), is64(ssi), (int)gate_fan, ptr(gates),
-                            gates.defined() ? dtype_code(gates) : 0, (const float*)ptr(scale), ptr(eo), is64(eo), (int)scale.size(0), (int8_t*)ptr(c.q),
-                            c.q.stride(0), (float*)ptr(c.scale), L, N, stream_of(dout)), "moe_quantize_rows (gradient)");
-    return c;
+    const int64_t R = ssi.size(0), E = W.size(0), K = W.size(1), N = W.size(2);
+    Tensor dx = at::empty({R, K}, dout.options());
+    if (R == 0) return dx;
+    if (N == 0) return dx.zero_();
+    const int8_t* w = (const int8_t*)ptr(W);
+    Tensor ws = bytes_on(dout, moe_linear_int8_workspace_bytes(w, W.stride(0), W.stride(2), W.stride(1), R, R, (int)E, N, K));
+    check(moe_linear_int8_bwd(ptr(dout), dout.stride(0), dtype_code(dout), dy_grouped, (int)gate_fan, ptr(gates), gates.defined() ? dtype_code(gates) : 0, w,
+                              W.stride(0), W.stride(1), W.stride(2), (const float*)ptr(scale), ptr(dx), dx.stride(0), dx_grouped, ptr(ssi), is64(ssi), ptr(eo), is64(eo),
+                              (int)E, R, K, N, ptr(ws), (size_t)ws.numel(), stream_of(dout)), "moe_linear_int8_bwd");
+    return dx;
 }
 
 struct LinearI8Fn : Function<LinearI8Fn> {
@@ -91,7 +80,7 @@ struct LinearI8Fn : Function<LinearI8Fn> {
                           const LinearCfg& c)
     {
         const Tensor gates = val(gates_);
-        Tensor y = product_int8(row_codes(x), W, scale, x.scalar_type(), ssi, eo, c.k, c.grouped_in, c.grouped_out), y_rows;
+        Tensor y = linear_int8_rows(x, W, scale, ssi, eo, c), y_rows;
         if (gates.defined()) {
             y_rows = y;
             y = combine(y_rows, gates, nullptr, gates.size(1), gates.size(0));
@@ -116,8 +105,7 @@ struct LinearI8Fn : Function<LinearI8Fn> {
             if (ctx->needs_input_grad(1)) d_gates = combine_dgates(y_rows, dout, gate_fan, gates.scalar_type(), nullptr);
         }
         if (ctx->needs_input_grad(0)) {
-            const Codes c = gradient_codes(dout, flat_gates(gates), gate_fan, scale, ssi, eo, grouped_out);
-            dx = product_int8(c, W.transpose(1, 2), Tensor(), dout.scalar_type(), ssi, eo, 1, true, grouped_in);
+            dx = linear_int8_dx_rows(dout, flat_gates(gates), gate_fan, W, scale, ssi, eo, grouped_out, grouped_in);
             if (k != 1) dx = combine(dx, Tensor(), nullptr, k, dx.size(0) / k);
         }
         return {dx, d_gates, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
@@ -147,7 +135,7 @@ Tensor linear_int8(const Tensor& x_, const Tensor& W, const Tensor& scale_, int6
     const Tensor gates = gates_.defined() ? gates_.contiguous() : Tensor();
     const LinearCfg c{0.0, 0.0, k, grouped_in, grouped_out};
     if (needs_node({&x, &gates})) return LinearI8Fn::apply(x, opt(gates), W, scale, ssi, eo, c);
-    Tensor y = product_int8(row_codes(x), W, scale, x.scalar_type(), ssi, eo, k, grouped_in, grouped_out);
+    Tensor y = linear_int8_rows(x, W, scale, ssi, eo, c);
     return gates.defined() ? combine(y, gates, nullptr, gates.size(1), gates.size(0)) : y;
 }
 
