@@ -31,7 +31,7 @@ constexpr int B_REGION = 2 * A_STAGE_BYTES;
 constexpr int LDS_BYTES = B_REGION + 3 * B_STAGE_BYTES;   // 160 or 80 KiB
 // Row and scale tables borrow the third weight stage: it is empty before the main loop's first tile, and behind the epilogue's staging after the last.
 constexpr int TABLE_OFF = B_REGION + 2 * B_STAGE_BYTES;
-static_assert(TABLE_OFF >= NWAVES * WTM * WTN * 2 && MOE_SEG_BYTES <= WTN * 2, "epilogue staging must not reach the tables");
+static_assert(TABLE_OFF >= NWAVES * WTM * WTN * 2, "epilogue staging must not reach the tables");
 constexpr int MIN_PART_KTILES = MOE_I8_MIN_PART;    // K tiles of a split tile's part, at least
 static_assert(NTHREADS == BM + BN && WTN == 2 * MOE_SEG_COLS, "a thread brings one row's or one column's scale; a wave holds two segments per row");
 
@@ -81,7 +81,12 @@ __global__ void __launch_bounds__(NTHREADS, 2) i8_gemm_kernel(const MoeI8Gemm p)
     __syncthreads();
 
     // ---- per-lane offsets of the direct-to-LDS loads (the K tile's offset is added per tile).  Image of a K-contiguous operand: row r at r*128 bytes, its
-    // 16-byte chunk c at slot c ^ ((r >> 1) & 7).  Wave w's instruction j fills rows [(j*NWAVES + w)*8, +8).
+    // 16-byte chunk c at slot c ^ ((r >> 1) & 7): the 16 rows of a fragment read meet 16 different bank groups.  Wave w's instruction j fills rows [(j*NWAVES + w)*8, +8).
+    // SEGMENTS: the columns of a wave's blocks 2 s and 2 s + 1 are dealt to their MFMA rows so that a lane ends up with 8 consecutive columns of a
+    // 32-column segment: row i of block b is column 8 (i >> 2) + 4 b + (i & 3).  W's image is swizzled for that set of rows instead.
+    constexpr bool SEGMENTS = EPI != MOE_I8_STORE;
+    static_assert(!NN || !SEGMENTS, "segments are written for K-contiguous weights");
+    auto b_swizzle = [](int r) { return SEGMENTS ? ((r >> 1) & 1) | (((r >> 3) & 3) << 1) : (r >> 1) & 7; };
     const int64_t a_row_base = p.x_grouped ? row0 : 0;
     uint32_t a_off[LPT], b_off[LPT];
 #pragma unroll
@@ -104,7 +109,7 @@ __global__ void __launch_bounds__(NTHREADS, 2) i8_gemm_kernel(const MoeI8Gemm p)
             const int r = (j * NWAVES + wave) * 8 + (lane >> 3);
             int64_t n = PAIR ? n0 + (r & (BN / 2 - 1)) : n0 + r;
             if (n >= p.N) n = p.N - 1;
-            b_off[j] = (uint32_t)(n * p.ldw + ((lane & 7) ^ ((r >> 1) & 7)) * 16);
+            b_off[j] = (uint32_t)(n * p.ldw + ((lane & 7) ^ b_swizzle(r)) * 16);
         } else {
             const int k = (j * NWAVES + wave) * KROWS + lane / NCH;
             int64_t n = n0 + ((lane & (NCH - 1)) ^ nn_swizzle(k)) * 16;
@@ -119,7 +124,10 @@ __global__ void __launch_bounds__(NTHREADS, 2) i8_gemm_kernel(const MoeI8Gemm p)
     for (int ks = 0; ks < 2; ++ks) a_frag_off[ks] = (wrow0 + (lane & 15)) * 128 + (((ks * 4 + (lane >> 4)) ^ ((lane >> 1) & 7)) << 4);
     if (!NN) {
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) b_frag_off[ks] = (lane & 15) * 128 + (((ks * 4 + (lane >> 4)) ^ ((lane >> 1) & 7)) << 4);
+        for (int ks = 0; ks < 2; ++ks) {
+            const int r = SEGMENTS ? 8 * ((lane & 15) >> 2) + (lane & 3) : lane & 15;
+            b_frag_off[ks] = r * 128 + (((ks * 4 + (lane >> 4)) ^ b_swizzle(r)) << 4);
+        }
     } else {
         // transposing reads: of a group g of 16 lanes, lane i fetches 8 columns (half i & 1 of the block's 16) at k row 16 g + (i >> 1), a second read 8 rows further
         // down; the hardware hands lane i the 8 codes of column i
@@ -138,7 +146,7 @@ __global__ void __launch_bounds__(NTHREADS, 2) i8_gemm_kernel(const MoeI8Gemm p)
 
     const uint32_t smem_u = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)LDS_PTR(smem) + wave * 1024);   // this wave's 1 KiB of the image that a round of load instructions fills
     const int live_rows = (nrows + 31) / 32 * 32;
-    const uint32_t tail_k = (uint32_t)(((lane & 7) ^ (((lane >> 4) + 4 * (wave & 1)) & 7)) * 16);   // k of this lane's chunk within a K-contiguous image
+    const uint32_t tail_k = (uint32_t)(((lane & 7) ^ b_swizzle(wave * 8 + (lane >> 3))) * 16);   // k of this lane's chunk within W's K-contiguous image (the same for every instruction)
     // Only tile of its group: K tiles are walked from a start that differs between output tiles, so that all workgroups' pieces do not lie on a few memory
     // channels; and the weight loads are non-temporal (nobody else reads them).
     const int krot = __builtin_amdgcn_readfirstlane((int)((uint32_t)(nt + expert * 8) % (uint32_t)(ke - kb)));
@@ -174,7 +182,8 @@ __global__ void __launch_bounds__(NTHREADS, 2) i8_gemm_kernel(const MoeI8Gemm p)
     // The weight fragment is the MFMA's first operand: a lane ends up with 4 consecutive output columns of one row.
     auto read_b1 = [&](const uint8_t* b_lds, int ks, int nb, i8frag_t* bfrag) {
         if (!NN) {
-            const int brow = PAIR ? (nb / NBH) * (BN / 2) + wn * (WTN / 2) + (nb % NBH) * 16 : wn * WTN + nb * 16;
+            const int b = SEGMENTS ? (nb % NBH) * 4 : (nb % NBH) * 16;
+            const int brow = (PAIR ? (nb / NBH) * (BN / 2) + wn * (WTN / 2) : wn * WTN + (nb / NBH) * (WTN / 2)) + b;
             bfrag[nb] = *(const i8frag_t*)(b_lds + brow * 128 + b_frag_off[ks]);
         } else {
             const uint8_t* bp = b_lds + b_frag_off[nb] + ks * 64 * BN;
@@ -261,12 +270,14 @@ __global__ void __launch_bounds__(NTHREADS, 2) i8_gemm_kernel(const MoeI8Gemm p)
     };
     using T_ = std::true_type;
     using F_ = std::false_type;
-    if (nblocks > MB || !item.only_tile) {   // more than half a tile, or a group of several tiles: their two rows of waves have at least MBH blocks each, or nearly
+    if (nblocks > MB || !item.only_tile) {   // more than half a tile, or one of several tiles of a group, whose rows are dealt evenly
         if (item.only_tile) {
             if (MB == 8 && mb_cnt <= 6) mainloop(std::integral_constant<int, MB * 3 / 4>{}, T_{}, T_{});
             else mainloop(std::integral_constant<int, MB>{}, T_{}, T_{});
-        } else if (mb_cnt > MB * 3 / 4) mainloop(std::integral_constant<int, MB>{}, T_{}, F_{});
-        else if (mb_cnt > MBH) mainloop(std::integral_constant<int, MB * 3 / 4>{}, T_{}, F_{});
+        } else if (mb_cnt == MB) mainloop(std::integral_constant<int, MB>{}, T_{}, F_{});
+        else if (mb_cnt == MB - 1) mainloop(std::integral_constant<int, MB - 1>{}, T_{}, F_{});
+        else if (MB == 8 && mb_cnt == 6) mainloop(std::integral_constant<int, MB * 3 / 4>{}, T_{}, F_{});
+        else if (MB == 8 && mb_cnt == 5) mainloop(std::integral_constant<int, MB / 2 + 1>{}, T_{}, F_{});
         else mainloop(std::integral_constant<int, MBH>{}, T_{}, F_{});
     } else if (mb_cnt > 2) mainloop(std::integral_constant<int, MBH>{}, F_{}, T_{});
     else if (mb_cnt == 2) mainloop(std::integral_constant<int, 2>{}, F_{}, T_{});
@@ -308,12 +319,86 @@ __global__ void __launch_bounds__(NTHREADS, 2) i8_gemm_kernel(const MoeI8Gemm p)
         }
     }
 
-    // ---- epilogue: acc[mb][nb][r] is (row mb*16 + lane%16, column nb*16 + (lane/16)*4 + r) of the wave's sub-tile
+    // ---- epilogue: acc[mb][nb][r] is (row mb*16 + lane%16, column nb*16 + (lane/16)*4 + r) of the wave's sub-tile; SEGMENTS: column (lane/16)*8 + (nb%2)*4 + r of
+    // segment nb/2
     if (tid < BM) {
         s_xscale[tid] = my_scale;
         if (!p.y_grouped) s_row[tid] = load_idx(p.pos, row0 + (tid < nrows ? tid : nrows - 1), p.pos64);
     } else s_wscale[tid - BM] = my_scale;
     __syncthreads();
+    if constexpr (SEGMENTS) {
+        const int64_t segs = p.N / MOE_SEG_COLS;
+        const int g = lane >> 4;
+        // One segment of the wave's rows (value(mb, i): element i of this lane's 8 in row block mb, times row_scale(mb)): four lanes hold a row's 32 values, whose
+        // maximum gives the scale; a lane stores the upper 16 bits of its 8 codes and then their lower 8, the four lanes of a row side by side.
+        auto put_segments = [&](auto value, auto row_scale, uint8_t* out, float* scales, int64_t ncol) {
+            if (ncol >= p.N) return;
+#pragma unroll
+            for (int mb = 0; mb < MB; ++mb) {
+                if (mb >= mb_cnt) continue;
+                float v[8];
+                uint32_t top = 0;
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) {
+                    v[i] = value(mb, i);
+                    v[i + 1] = value(mb, i + 1);
+                    top = max(max(__float_as_uint(v[i]) & 0x7fffffffu, __float_as_uint(v[i + 1]) & 0x7fffffffu), top);   // (bits: NaN above infinity above every number)
+                }
+                auto pair = __builtin_amdgcn_permlane16_swap(top, top, false, false);
+                top = max(pair[0], pair[1]);
+                pair = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+                top = max(pair[0], pair[1]);
+                const float amax = __uint_as_float(top);
+                const bool fine = top < 0x7f800000u;
+                // (a segment below 2^-100 is zero to the 8-bit codes of any row that is not as small as that)
+                const float inv = fine && amax > 0x1p-100f ? MOE_SEG_LEVELS * __builtin_amdgcn_rcpf(amax) : 0.f;
+                if (__any(!fine))   // (its scale says NaN)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = fine ? v[i] : 0.f;
+                int q[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) q[i] = (int)(v[i] * inv);
+                u32x4_t hi;
+                uint2 lo;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) hi[i] = __builtin_amdgcn_perm((uint32_t)q[2 * i + 1], (uint32_t)q[2 * i], 0x06050201u);
+                lo.x = __builtin_amdgcn_perm((uint32_t)q[1], (uint32_t)q[0], 0x0c0c0400u) | __builtin_amdgcn_perm((uint32_t)q[3], (uint32_t)q[2], 0x04000c0cu);
+                lo.y = __builtin_amdgcn_perm((uint32_t)q[5], (uint32_t)q[4], 0x0c0c0400u) | __builtin_amdgcn_perm((uint32_t)q[7], (uint32_t)q[6], 0x04000c0cu);
+                const int m = mb * 16 + (lane & 15);
+                if (m < wrows) {
+                    const int64_t at = (row0 + wrow0 + m) * segs + ncol / MOE_SEG_COLS;
+                    uint8_t* to = out + at * MOE_SEG_BYTES;
+                    *(u32x4_t*)(to + g * 16) = hi;
+                    *(uint2*)(to + 64 + g * 8) = lo;
+                    if (g == 0) scales[at] = !fine ? __uint_as_float(0x7fc00000u) : inv > 0.f ? amax * (1.f / MOE_SEG_LEVELS) * row_scale(mb) : 0.f;
+                }
+            }
+        };
+        auto xs = [&](int mb) { return s_xscale[wrow0 + mb * 16 + (lane & 15)]; };
+        auto one = [](int) { return 1.f; };
+        if (EPI == MOE_I8_SEG) {   // (without column scales: the maximum of the sums themselves)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                put_segments([&](int mb, int i) { return (float)acc[mb][2 * h + i / 4][i % 4]; }, xs, p.S[0], p.SS[0], n0 + wn * WTN + h * MOE_SEG_COLS);
+        } else {   // SwiGLU: gate = acc[mb][b], up = acc[mb][NBH + b] at the same row and column
+            float wg[8], wu[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                wg[i] = s_wscale[wn * (WTN / 2) + g * 8 + i];
+                wu[i] = s_wscale[BN / 2 + wn * (WTN / 2) + g * 8 + i];
+            }
+            const int64_t ncol = n0 + wn * (WTN / 2);
+            put_segments([&](int mb, int i) {
+                const float x = xs(mb), a = (float)acc[mb][i / 4][i % 4] * x * wg[i], u = (float)acc[mb][NBH + i / 4][i % 4] * x * wu[i];
+                return a * __builtin_amdgcn_rcpf(1.f + __expf(-a)) * u;
+            }, one, p.S[0], p.SS[0], ncol);
+            if (p.S[1]) {
+                put_segments([&](int mb, int i) { return (float)acc[mb][i / 4][i % 4] * wg[i]; }, xs, p.S[1], p.SS[1], ncol);
+                put_segments([&](int mb, int i) { return (float)acc[mb][NBH + i / 4][i % 4] * wu[i]; }, xs, p.S[2], p.SS[2], ncol);
+            }
+        }
+        return;
+    }
     const int mrow = lane & 15, nq = (lane >> 4) * 4;
     uint8_t* stg = smem + wave * (WTM * WTN * 2);   // 16-bit values of the wave's sub-tile
     auto swz = [](int sw, int m, int c) { return c ^ ((m / (sw >= 128 ? 1 : 128 / sw)) & (sw / 8 - 1)); };
@@ -338,63 +423,10 @@ __global__ void __launch_bounds__(NTHREADS, 2) i8_gemm_kernel(const MoeI8Gemm p)
         __builtin_amdgcn_s_waitcnt(0xC07F);   // reads done before the slice is reused
     };
     auto column_scales = [&](int nb, float* w) {   // of this lane's four columns of block nb
-        const int c = PAIR ? (nb / NBH) * (BN / 2) + wn * (WTN / 2) + (nb % NBH) * 16 + nq : wn * WTN + nb * 16 + nq;
-        const float4 v = *(const float4*)(s_wscale + c);
+        const float4 v = *(const float4*)(s_wscale + wn * WTN + nb * 16 + nq);
         w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
     };
-    // One output of 32 columns per wave in segments of 24-bit codes (value(mb, i): element i of this lane's 8 in row block mb): a row's 32 values lie
-    // with four lanes; their maximum gives the scale, the codes are staged as the segment's 96 bytes and go out 16 bytes per lane.
-    auto put_segments = [&](auto value, uint8_t* out, float* scales, int64_t ncol) {
-        const int64_t segs = p.N / MOE_SEG_COLS;
-#pragma unroll
-        for (int mb = 0; mb < MB; ++mb) {
-            if (mb >= mb_cnt) continue;
-            float v[8];
-            uint32_t top = 0;
-#pragma unroll
-            for (int i = 0; i < 8; i += 2) {
-                v[i] = value(mb, i);
-                v[i + 1] = value(mb, i + 1);
-                top = max(max(__float_as_uint(v[i]) & 0x7fffffffu, __float_as_uint(v[i + 1]) & 0x7fffffffu), top);   // (bits: NaN above infinity above every number)
-            }
-            top = max(top, (uint32_t)__shfl_xor((int)top, 16));
-            top = max(top, (uint32_t)__shfl_xor((int)top, 32));
-            const float amax = __uint_as_float(top);
-            const bool fine = top < 0x7f800000u;
-            // (a segment below 2^-100 is zero to the 8-bit codes of any row that is not as small as that)
-            const float inv = fine && amax > 0x1p-100f ? MOE_SEG_LEVELS * __builtin_amdgcn_rcpf(amax) : 0.f;
-            if (__any(!fine))   // (its scale says NaN)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = fine ? v[i] : 0.f;
-            const int m = mb * 16 + mrow;
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                int q[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) q[i] = (int)(v[4 * b + i] * inv);
-                uint2 hi;
-                hi.x = __builtin_amdgcn_perm((uint32_t)q[1], (uint32_t)q[0], 0x06050201u);
-                hi.y = __builtin_amdgcn_perm((uint32_t)q[3], (uint32_t)q[2], 0x06050201u);
-                const uint32_t lo = __builtin_amdgcn_perm((uint32_t)q[1], (uint32_t)q[0], 0x0c0c0400u) | __builtin_amdgcn_perm((uint32_t)q[3], (uint32_t)q[2], 0x04000c0cu);
-                *(uint2*)(stg + m * MOE_SEG_BYTES + b * 32 + nq * 2) = hi;
-                *(uint32_t*)(stg + m * MOE_SEG_BYTES + 64 + b * 16 + nq) = lo;
-            }
-            if (lane < 16 && m < wrows && ncol < p.N)
-                scales[(row0 + wrow0 + m) * segs + ncol / MOE_SEG_COLS] = !fine ? __uint_as_float(0x7fc00000u) : inv > 0.f ? amax * (1.f / MOE_SEG_LEVELS) : 0.f;
-        }
-        __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0): this wave's staging writes have landed
-        if (ncol < p.N) {
-            constexpr int PIECES = MOE_SEG_BYTES / 16;
-            uint8_t* to = out + ((row0 + wrow0) * segs + ncol / MOE_SEG_COLS) * MOE_SEG_BYTES;
-            for (int i = lane; i < wrows * PIECES; i += 64) {
-                const int m = i / PIECES, c = i - m * PIECES;
-                *(u32x4_t*)(to + m * segs * MOE_SEG_BYTES + c * 16) = *(const u32x4_t*)(stg + i * 16);
-            }
-        }
-        __builtin_amdgcn_s_waitcnt(0xC07F);   // reads done before the slice is reused
-    };
-
-    if (EPI == MOE_I8_STORE) {
+    {
         float w[NB][4];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) column_scales(nb, w[nb]);
@@ -439,29 +471,6 @@ __global__ void __launch_bounds__(NTHREADS, 2) i8_gemm_kernel(const MoeI8Gemm p)
             }
         }
         stage_flush(WTN, (uint16_t*)p.Y, p.ldy, !p.y_grouped, ncol0, p.y_vec);
-    } else if (EPI == MOE_I8_SEG) {
-        float w[NB][4];
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) column_scales(nb, w[nb]);
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-            put_segments([&](int mb, int i) { return (float)acc[mb][2 * h + i / 4][i % 4] * s_xscale[wrow0 + mb * 16 + mrow] * w[2 * h + i / 4][i % 4]; },
-                         p.S[0], p.SS[0], n0 + wn * WTN + h * MOE_SEG_COLS);
-    } else {   // SwiGLU: gate = acc[mb][j], up = acc[mb][NBH + j] at the same row and column
-        float w[NB][4];
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) column_scales(nb, w[nb]);
-        const int64_t ncol0 = n0 + wn * (WTN / 2);
-#pragma unroll
-        for (int out = 0; out < 3; ++out) {
-            if (!p.S[out]) continue;
-            put_segments([&](int mb, int i) {
-                const float xs = s_xscale[wrow0 + mb * 16 + mrow];
-                const float g = (float)acc[mb][i / 4][i % 4] * xs * w[i / 4][i % 4];
-                const float u = (float)acc[mb][NBH + i / 4][i % 4] * xs * w[NBH + i / 4][i % 4];
-                return out == 0 ? g * __builtin_amdgcn_rcpf(1.f + __expf(-g)) * u : out == 1 ? g : u;
-            }, p.S[out], p.SS[out], ncol0);
-        }
     }
 }
 
