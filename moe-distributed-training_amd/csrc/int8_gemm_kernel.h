@@ -329,57 +329,61 @@ __global__ void __launch_bounds__(NTHREADS, 2) i8_gemm_kernel(const MoeI8Gemm p)
     if constexpr (SEGMENTS) {
         const int64_t segs = p.N / MOE_SEG_COLS;
         const int g = lane >> 4;
-        // One segment of the wave's rows (value(mb, i): element i of this lane's 8 in row block mb, times row_scale(mb)): four lanes hold a row's 32 values, whose
+        // The tile's scales are gathered in LDS and written behind the codes, whole pieces of a row: one by one they made a third of the launch's store requests.
+        constexpr int SEGS = (PAIR ? BN / 2 : BN) / MOE_SEG_COLS;   // per row and output
+        float* s_seg = (float*)smem;
+        static_assert(3 * BM * SEGS * 4 <= TABLE_OFF, "segment scales lie in front of the tables");
+        // Segment h of the wave's rows in block mb (value(i): element i of this lane's 8, times row_scale): four lanes hold a row's 32 values, whose
         // maximum gives the scale; a lane stores the upper 16 bits of its 8 codes and then their lower 8, the four lanes of a row side by side.
-        auto put_segments = [&](auto value, auto row_scale, uint8_t* out, float* scales, int64_t ncol) {
+        auto put_segment = [&](int mb, auto value, float row_scale, uint8_t* out, float* scales, int seg) {
+            const int64_t ncol = n0 + seg * MOE_SEG_COLS;
             if (ncol >= p.N) return;
+            float v[8];
+            uint32_t top = 0;
 #pragma unroll
-            for (int mb = 0; mb < MB; ++mb) {
-                if (mb >= mb_cnt) continue;
-                float v[8];
-                uint32_t top = 0;
+            for (int i = 0; i < 8; i += 2) {
+                v[i] = value(i);
+                v[i + 1] = value(i + 1);
+                top = max(max(__float_as_uint(v[i]) & 0x7fffffffu, __float_as_uint(v[i + 1]) & 0x7fffffffu), top);   // (bits: NaN above infinity above every number)
+            }
+            auto pair = __builtin_amdgcn_permlane16_swap(top, top, false, false);
+            top = max(pair[0], pair[1]);
+            pair = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+            top = max(pair[0], pair[1]);
+            const float amax = __uint_as_float(top);
+            const bool fine = top < 0x7f800000u;
+            // (a segment below 2^-100 is zero to the 8-bit codes of any row that is not as small as that)
+            const float inv = fine && amax > 0x1p-100f ? MOE_SEG_LEVELS * __builtin_amdgcn_rcpf(amax) : 0.f;
+            if (__any(!fine))   // (its scale says NaN)
 #pragma unroll
-                for (int i = 0; i < 8; i += 2) {
-                    v[i] = value(mb, i);
-                    v[i + 1] = value(mb, i + 1);
-                    top = max(max(__float_as_uint(v[i]) & 0x7fffffffu, __float_as_uint(v[i + 1]) & 0x7fffffffu), top);   // (bits: NaN above infinity above every number)
-                }
-                auto pair = __builtin_amdgcn_permlane16_swap(top, top, false, false);
-                top = max(pair[0], pair[1]);
-                pair = __builtin_amdgcn_permlane32_swap(top, top, false, false);
-                top = max(pair[0], pair[1]);
-                const float amax = __uint_as_float(top);
-                const bool fine = top < 0x7f800000u;
-                // (a segment below 2^-100 is zero to the 8-bit codes of any row that is not as small as that)
-                const float inv = fine && amax > 0x1p-100f ? MOE_SEG_LEVELS * __builtin_amdgcn_rcpf(amax) : 0.f;
-                if (__any(!fine))   // (its scale says NaN)
+                for (int i = 0; i < 8; ++i) v[i] = fine ? v[i] : 0.f;
+            int q[8];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] = fine ? v[i] : 0.f;
-                int q[8];
+            for (int i = 0; i < 8; ++i) q[i] = (int)(v[i] * inv);
+            u32x4_t hi;
+            uint2 lo;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) q[i] = (int)(v[i] * inv);
-                u32x4_t hi;
-                uint2 lo;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) hi[i] = __builtin_amdgcn_perm((uint32_t)q[2 * i + 1], (uint32_t)q[2 * i], 0x06050201u);
-                lo.x = __builtin_amdgcn_perm((uint32_t)q[1], (uint32_t)q[0], 0x0c0c0400u) | __builtin_amdgcn_perm((uint32_t)q[3], (uint32_t)q[2], 0x04000c0cu);
-                lo.y = __builtin_amdgcn_perm((uint32_t)q[5], (uint32_t)q[4], 0x0c0c0400u) | __builtin_amdgcn_perm((uint32_t)q[7], (uint32_t)q[6], 0x04000c0cu);
-                const int m = mb * 16 + (lane & 15);
-                if (m < wrows) {
-                    const int64_t at = (row0 + wrow0 + m) * segs + ncol / MOE_SEG_COLS;
-                    uint8_t* to = out + at * MOE_SEG_BYTES;
-                    *(u32x4_t*)(to + g * 16) = hi;
-                    *(uint2*)(to + 64 + g * 8) = lo;
-                    if (g == 0) scales[at] = !fine ? __uint_as_float(0x7fc00000u) : inv > 0.f ? amax * (1.f / MOE_SEG_LEVELS) * row_scale(mb) : 0.f;
-                }
+            for (int i = 0; i < 4; ++i) hi[i] = __builtin_amdgcn_perm((uint32_t)q[2 * i + 1], (uint32_t)q[2 * i], 0x06050201u);
+            lo.x = __builtin_amdgcn_perm((uint32_t)q[1], (uint32_t)q[0], 0x0c0c0400u) | __builtin_amdgcn_perm((uint32_t)q[3], (uint32_t)q[2], 0x04000c0cu);
+            lo.y = __builtin_amdgcn_perm((uint32_t)q[5], (uint32_t)q[4], 0x0c0c0400u) | __builtin_amdgcn_perm((uint32_t)q[7], (uint32_t)q[6], 0x04000c0cu);
+            const int m = mb * 16 + (lane & 15);
+            if (m < wrows) {
+                const int64_t at = (row0 + wrow0 + m) * segs + ncol / MOE_SEG_COLS;
+                uint8_t* to = out + at * MOE_SEG_BYTES;
+                *(u32x4_t*)(to + g * 16) = hi;
+                *(uint2*)(to + 64 + g * 8) = lo;
+                if (g == 0) scales[(wrow0 + m) * SEGS + seg] = !fine ? __uint_as_float(0x7fc00000u) : inv > 0.f ? amax * (1.f / MOE_SEG_LEVELS) * row_scale : 0.f;
             }
         };
         auto xs = [&](int mb) { return s_xscale[wrow0 + mb * 16 + (lane & 15)]; };
-        auto one = [](int) { return 1.f; };
         if (EPI == MOE_I8_SEG) {   // (without column scales: the maximum of the sums themselves)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-                put_segments([&](int mb, int i) { return (float)acc[mb][2 * h + i / 4][i % 4]; }, xs, p.S[0], p.SS[0], n0 + wn * WTN + h * MOE_SEG_COLS);
+            for (int mb = 0; mb < MB; ++mb) {
+                if (mb >= mb_cnt) continue;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)   // (both segments of a row block together: their 192 bytes meet in the cache)
+                    put_segment(mb, [&](int i) { return (float)acc[mb][2 * h + i / 4][i % 4]; }, xs(mb), p.S[0], s_seg, wn * 2 + h);
+            }
         } else {   // SwiGLU: gate = acc[mb][b], up = acc[mb][NBH + b] at the same row and column
             float wg[8], wu[8];
 #pragma unroll
@@ -387,14 +391,28 @@ __global__ void __launch_bounds__(NTHREADS, 2) i8_gemm_kernel(const MoeI8Gemm p)
                 wg[i] = s_wscale[wn * (WTN / 2) + g * 8 + i];
                 wu[i] = s_wscale[BN / 2 + wn * (WTN / 2) + g * 8 + i];
             }
-            const int64_t ncol = n0 + wn * (WTN / 2);
-            put_segments([&](int mb, int i) {
-                const float x = xs(mb), a = (float)acc[mb][i / 4][i % 4] * x * wg[i], u = (float)acc[mb][NBH + i / 4][i % 4] * x * wu[i];
-                return a * __builtin_amdgcn_rcpf(1.f + __expf(-a)) * u;
-            }, one, p.S[0], p.SS[0], ncol);
-            if (p.S[1]) {
-                put_segments([&](int mb, int i) { return (float)acc[mb][i / 4][i % 4] * wg[i]; }, xs, p.S[1], p.SS[1], ncol);
-                put_segments([&](int mb, int i) { return (float)acc[mb][NBH + i / 4][i % 4] * wu[i]; }, xs, p.S[2], p.SS[2], ncol);
+#pragma unroll
+            for (int mb = 0; mb < MB; ++mb) {
+                if (mb >= mb_cnt) continue;
+                const float x = xs(mb);
+                put_segment(mb, [&](int i) {
+                    const float a = (float)acc[mb][i / 4][i % 4] * x * wg[i], u = (float)acc[mb][NBH + i / 4][i % 4] * x * wu[i];
+                    return a * __builtin_amdgcn_rcpf(1.f + __expf(-a)) * u;
+                }, 1.f, p.S[0], s_seg, wn);
+                if (p.S[1]) {
+                    put_segment(mb, [&](int i) { return (float)acc[mb][i / 4][i % 4] * wg[i]; }, x, p.S[1], s_seg + BM * SEGS, wn);
+                    put_segment(mb, [&](int i) { return (float)acc[mb][NBH + i / 4][i % 4] * wu[i]; }, x, p.S[2], s_seg + 2 * BM * SEGS, wn);
+                }
+            }
+        }
+        __syncthreads();
+        const int64_t seg0 = n0 / MOE_SEG_COLS;
+#pragma unroll
+        for (int out = 0; out < (PAIR ? 3 : 1); ++out) {
+            if (!p.SS[out]) continue;
+            for (int i = tid; i < nrows * (SEGS / 2); i += NTHREADS) {   // (segments come in pairs: N is a multiple of 64)
+                const int r = i / (SEGS / 2), c = i % (SEGS / 2) * 2;
+                if (seg0 + c < segs) *(float2*)(p.SS[out] + (row0 + r) * segs + seg0 + c) = *(const float2*)(s_seg + (out * BM + r) * SEGS + c);
             }
         }
         return;
