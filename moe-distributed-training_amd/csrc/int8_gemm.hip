@@ -6,29 +6,56 @@ namespace {
 
 constexpr int MAX_SPLIT = 8;   // K parts that a tile of the last, partial round of compute units may be cut into
 
+// compute units that the plan fills, whole rounds of the 8 XCDs
+int plan_cus()
+{
+    const int n = moe_device_cus() / NXCD * NXCD;
+    return n < NXCD ? NXCD : n;
+}
+int64_t counters(int cus) { return 2 * (int64_t)cus + 64; }   // ints in front of the sums or slots (whole 256 bytes)
+
 int64_t tiles_at_most(int tile, int64_t R, int E, int64_t N, bool pair)
 {
     const int64_t cols = pair ? tile / 2 : tile;
     return (R / tile + E) * ((N + cols - 1) / cols);
 }
 
-// K parts that a tile of `ktiles` K tiles can be cut into
-int parts_at_most(int64_t ktiles)
+// A launch's tile size and the K parts that its tiles may be cut into, by what a launch of evenly dealt rows would take (ns):
+//   - a chain of K tiles per workgroup, 550 + 1.2 per row of the tile for tiles of 128 (two workgroups per compute unit) and 750 + 1.8 for 256, times the rounds;
+//   - at least the weights at 6 TB/s;
+//   - where tiles are cut, the meeting of the parts: sums by atomics at 80 per ns (128), or slots written and read at 2.5 TB/s behind fences of 8 us (256).
+// Measured (d=4096, f=14336; us, [tile, parts] and the estimate in brackets): h W2 of 4 rows of one expert [128, 8] 19 (20), [128, 1] 61 (68), [256, 8] 29 (26); of 64 rows
+// [128, 8] 43 (46), [256, 8] 40 (33), [128, 1] 71 (76); of 500 [128, 1] 61 (78), [256, 8] 85 (80); 48 rows of 8 experts [128, 1] 83 (87), [256, 4] 92; gate/up of
+// 666 rows of 8 [128, 1] 200 (163), [256, 1] 187.  Where the chip is full anyway (a round of tiles or more) only tiles of 256 are cut, into parts of 16 K tiles at least: those of
+// the last round (dX of 8192 rows of 2 experts 903 us uncut, 752 cut; dh, whose K is 32 tiles, 485 uncut, 510 in parts of 4).
+struct Plan { int tile, split; };
+Plan plan(int cus, int64_t R, int E, int64_t ktiles, int64_t N, bool pair)
 {
-    int s = 1;
-    while (s * 2 <= MAX_SPLIT && ktiles / (s * 2) >= MIN_PART_KTILES) s *= 2;
-    return s;
+    const int64_t groups = R < E ? R : E, rows = (R + groups - 1) / groups;
+    const double weights = (double)groups * (double)ktiles * BK * (double)N * (pair ? 2 : 1) / 6000.0;
+    Plan best = {128, 1};
+    double best_ns = -1.0;
+    for (int tile = 128; tile <= 256; tile *= 2) {
+        const int64_t cols = pair ? tile / 2 : tile, tiles = groups * ((rows + tile - 1) / tile) * ((N + cols - 1) / cols), slots = tile == 128 ? 2 * (int64_t)cus : cus;
+        const double ktile_ns = tile == 128 ? 550.0 + 1.2 * (double)(rows < 128 ? rows : 128) : 750.0 + 1.8 * (double)(rows < 256 ? rows : 256);
+        for (int split = 1; split <= MAX_SPLIT; split *= 2) {
+            if (split > 1 && (ktiles / split < MIN_PART_KTILES || tiles * split > slots)) break;
+            const int64_t rounds = (tiles * split + slots - 1) / slots;
+            const double chain = (double)((ktiles + split - 1) / split) * ktile_ns * (double)rounds;
+            const double sums = (double)R * (double)N * (pair ? 2 : 1) * split;
+            const double meet = split == 1 ? 0.0 : tile == 128 ? 3000.0 + sums / 80.0 : 8000.0 + sums * 8.0 / 2500.0;
+            const double ns = (chain > weights ? chain : weights) + meet;
+            if (best_ns < 0.0 || ns < best_ns) { best = {tile, split}; best_ns = ns; }
+        }
+        if (tile == 256 && best.tile == 256 && tiles >= cus) {
+            best.split = 1;
+            while (best.split * 2 <= 4 && ktiles / (best.split * 2) >= 16) best.split *= 2;
+        }
+    }
+    return best;
 }
 
 }  // namespace
-
-// rows and columns of a launch's tiles
-int moe_i8_tile(int cus, int64_t R, int E, int64_t N, bool pair)
-{
-    const int64_t groups = R < E ? R : E;
-    const int64_t tiles = groups * (((R + groups - 1) / groups + BM - 1) / BM) * ((N + BN - 1) / BN * (pair ? 2 : 1));   // (as if the rows were dealt evenly)
-    return R <= groups * 128 || 2 * tiles <= cus ? 128 : 256;
-}
 
 bool moe_i8_weights_ok(const void* W, int64_t swe, int64_t ldw) { return (uintptr_t)W % 16 == 0 && swe % 16 == 0 && ldw % 16 == 0; }
 
@@ -40,33 +67,31 @@ bool moe_i8_gemm_supported(const MoeI8Gemm& p, int64_t R, int64_t x_rows)
     return rows * p.ldx < ((int64_t)1 << 32) && (p.nn ? (p.K - 1) * p.ldw + p.N : (p.N - 1) * p.ldw + p.K) + 16 < limit;
 }
 
-// counters of the split tiles: two per compute unit are enough for either tile size
-int moe_i8_counters() { return 2 * (moe_device_cus() / NXCD * NXCD > 0 ? moe_device_cus() / NXCD * NXCD : NXCD); }
-
-// counters of the split tiles (one per compute unit's workgroup) and their parts' sums, of the tile size that needs more
-size_t moe_i8_exchange_bytes(int64_t R, int E, int64_t K, int64_t N, bool pair)
+// Where a launch's split tiles meet: `zeros` ints, a counter per workgroup of a round (tiles of 128 have twice those of 256) and, for tiles of 128, the matrix of
+// sums; and for tiles of 256 `slots` ints, a tile of them per part.
+MoeI8Exchange moe_i8_exchange(int64_t R, int E, int64_t K, int64_t N, bool pair)
 {
-    const int cus = moe_i8_counters() / 2;
-    const int64_t parts = parts_at_most((K + BK - 1) / BK);
-    size_t most = 0;
-    for (int tile = 256; tile >= 128; tile /= 2) {
-        const int64_t slots = (int64_t)(256 / tile) * cus, all = parts * tiles_at_most(tile, R, E, N, pair);
-        const size_t b = parts == 1 ? 0 : (size_t)(all < slots ? all : slots) * tile * tile * sizeof(int);
-        most = b > most ? b : most;
-    }
-    return 2 * (size_t)cus * sizeof(int) + 256 + most;
+    if (R < 1) return {0, 0};
+    const int cus = plan_cus();
+    const Plan pl = plan(cus, R, E, (K + BK - 1) / BK, N, pair);
+    if (pl.split == 1) return {0, 0};
+    if (pl.tile == 128) return {counters(cus) + (pair ? 2 : 1) * R * N, 0};
+    const int64_t all = pl.split * tiles_at_most(pl.tile, R, E, N, pair);
+    return {counters(cus), (all < cus ? all : cus) * BM * BN};
 }
 
 int moe_launch_i8_gemm(const MoeI8Gemm& p_, int64_t R, hipStream_t stream)
 {
     if (R == 0 || p_.N == 0) return MOE_OK;
     MoeI8Gemm p = p_;
-    const int cus = moe_i8_counters() / 2;
+    const int cus = plan_cus();
+    const Plan pl = plan(cus, R, p.E, (p.K + BK - 1) / BK * p.nseg, p.N, p.epi == MOE_I8_SWIGLU);
     p.num_cus = cus;
-    p.max_split = parts_at_most((p.K + BK - 1) / BK * p.nseg);
-    if (p.max_split > 1 && !p.exchange) return MOE_ERR_WORKSPACE;
-    p.sk_counters = (int*)p.exchange;
-    p.sk_partials = (int*)((uint8_t*)p.exchange + ((2 * (size_t)cus * sizeof(int) + 255) & ~(size_t)255));
+    p.rows = R;
+    p.max_split = pl.split;
+    if (p.max_split > 1 && (!p.zeros || (pl.tile == 256 && !p.slots))) return MOE_ERR_WORKSPACE;
+    p.sk_counters = p.zeros;
+    p.sk_partials = pl.tile == 256 ? p.slots : p.zeros + counters(cus);
     p.y_vec = (uintptr_t)p.Y % 16 == 0 && (p.ydtype == MOE_F32 ? p.ldy % 4 == 0 && p.N % 4 == 0 : p.ldy % 8 == 0 && p.N % 8 == 0);
-    return moe_i8_tile(cus, R, p.E, p.N, p.epi == MOE_I8_SWIGLU) == 128 ? moe_launch_i8_gemm_small(p, R, stream) : launch_epilogue(p, R, stream);
+    return pl.tile == 128 ? moe_launch_i8_gemm_small(p, R, stream) : launch_epilogue(p, R, stream);
 }

@@ -284,9 +284,40 @@ __global__ void __launch_bounds__(NTHREADS, 2) i8_gemm_kernel(const MoeI8Gemm p)
     else if (mb_cnt == 1) mainloop(std::integral_constant<int, 1>{}, F_{}, T_{});
     else mainloop(std::integral_constant<int, 0>{}, F_{}, T_{});
 
-    // ---- K parts of a split tile: every part publishes its sums and then bumps the tile's counter; the part that finds all others counted adds theirs to its
-    // own and finishes the tile.  Nobody waits for anybody; device-scope stores and loads, visible across the XCDs' L2 caches.
+    // ---- K parts of a split tile; nobody waits for anybody.
+    // Tiles of 128: every part adds its sums to the launch's (zeroed) matrix of sums by device-scope atomics and then bumps the tile's counter; the part that finds
+    // all others counted takes the complete sums out, leaving zeros for the next launch.  Integers: the order does not matter.  Data and counter move by
+    // relaxed atomics alone, each awaited before the next: no fence, which writes back and empties whole L2 caches (with the parts in slots and fences as below, h W2 of
+    // one token, 512 parts: 46 us).  Only rows that exist are moved.
+    // Tiles of 256: a part's sums are too many for atomics; they go to a slot of their own by device-scope stores, and the last part adds the others' to its own.
     if (nparts > 1) {
+        if constexpr (BM == 128) {
+            const int g = lane >> 4;
+            const int64_t m0 = row0 + wrow0 + (lane & 15);
+            auto each = [&](auto fn) {   // (sum, where it lies) of every element of this lane that exists
+#pragma unroll
+                for (int mb = 0; mb < MB; ++mb)
+                    if (mb * 16 + (lane & 15) < wrows)
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb) {
+                            const int half = nb / NBH, b = nb % NBH;
+                            const int64_t n = n0 + (PAIR ? wn * (WTN / 2) : wn * WTN + half * (WTN / 2)) + (EPI != MOE_I8_STORE ? g * 8 + b * 4 : b * 16 + g * 4);
+                            int* at = p.sk_partials + ((PAIR && half ? p.rows : 0) + m0 + mb * 16) * p.N + n;
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                if (n + r < p.N) fn(mb, nb, r, at + r);
+                        }
+            };
+            each([&](int mb, int nb, int r, int* at) { (void)__hip_atomic_fetch_add(at, acc[mb][nb][r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); });
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wave's sums have been added
+            __syncthreads();                                   // ... and every wave's
+            if (tid == 0) *s_arrival = __hip_atomic_fetch_add(&p.sk_counters[item.split_tile], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __syncthreads();
+            if (*s_arrival != nparts - 1) return;
+            if (tid == 0) __hip_atomic_store(&p.sk_counters[item.split_tile], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            asm volatile("" ::: "memory");
+            each([&](int mb, int nb, int r, int* at) { acc[mb][nb][r] = __hip_atomic_exchange(at, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); });
+        } else {
         constexpr int DEVICE_SCOPE = 16;
         const __amdgpu_buffer_rsrc_t xbuf = __builtin_amdgcn_make_buffer_rsrc(p.sk_partials, 0, (int)0x80000000u, 0x00020000);
         auto slot = [&](int x) { return (uint32_t)(item.split_item - part + x) * (uint32_t)(BM * BN * sizeof(int)); };
@@ -316,6 +347,7 @@ __global__ void __launch_bounds__(NTHREADS, 2) i8_gemm_kernel(const MoeI8Gemm p)
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
+        }
         }
     }
 

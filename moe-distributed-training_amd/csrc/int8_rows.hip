@@ -125,12 +125,16 @@ template <> struct Loader<__half> {
 
 // One workgroup per row.  KEEP: a thread holds its KEEP pieces of 8 columns between the two passes (0: the row is read twice).  SCALED: row m is row
 // pos[m] / fan_out of src times coeff[pos[m]] and, column by column, col_scale[expert of m] (a gradient on its way through the weights' scales).
+constexpr int64_t ZERO_PIECE = 4096;   // ints that a workgroup clears
 template <typename T, bool SCALED, int KEEP>
 __global__ void __launch_bounds__(1024) quantize_rows_kernel(const MoeQuantizeRows p)
 {
     const int64_t m = blockIdx.x;
-    if (m == 0)   // side job: the counters of the product behind this launch
-        for (int i = threadIdx.x; i < p.zero_n; i += blockDim.x) p.zero[i] = 0;
+    if (m >= p.rows) {   // side job: the counters and sums of the products behind this launch
+        const int64_t i0 = (m - p.rows) * ZERO_PIECE;
+        for (int64_t i = i0 + threadIdx.x; i < i0 + ZERO_PIECE && i < p.zero_n; i += blockDim.x) p.zero[i] = 0;
+        return;
+    }
     int64_t src_row = m;
     float coeff = 1.f;
     const float* cs = nullptr;
@@ -425,13 +429,13 @@ __global__ void zero_u32_kernel(uint32_t* p, int64_t n)
 template <typename T, bool SCALED> int launch_quantize_t(const MoeQuantizeRows& p, int64_t rows, hipStream_t stream)
 {
     // pieces of 8 columns: one to four of them a thread
-    const int64_t pieces = (p.ldc + 7) / 8;
+    const int64_t pieces = (p.ldc + 7) / 8, grid = rows + (p.zero_n + ZERO_PIECE - 1) / ZERO_PIECE;
     const int nt = pieces <= 64 ? 64 : pieces <= 128 ? 128 : pieces <= 1024 ? 256 : pieces <= 2048 ? 512 : 1024;
     const int64_t keep = (pieces + nt - 1) / nt;
-    if (keep <= 1) hipLaunchKernelGGL((quantize_rows_kernel<T, SCALED, 1>), dim3((unsigned)rows), dim3(nt), 0, stream, p);
-    else if (keep <= 2) hipLaunchKernelGGL((quantize_rows_kernel<T, SCALED, 2>), dim3((unsigned)rows), dim3(nt), 0, stream, p);
-    else if (keep <= 4) hipLaunchKernelGGL((quantize_rows_kernel<T, SCALED, 4>), dim3((unsigned)rows), dim3(nt), 0, stream, p);
-    else hipLaunchKernelGGL((quantize_rows_kernel<T, SCALED, 0>), dim3((unsigned)rows), dim3(nt), 0, stream, p);
+    if (keep <= 1) hipLaunchKernelGGL((quantize_rows_kernel<T, SCALED, 1>), dim3((unsigned)grid), dim3(nt), 0, stream, p);
+    else if (keep <= 2) hipLaunchKernelGGL((quantize_rows_kernel<T, SCALED, 2>), dim3((unsigned)grid), dim3(nt), 0, stream, p);
+    else if (keep <= 4) hipLaunchKernelGGL((quantize_rows_kernel<T, SCALED, 4>), dim3((unsigned)grid), dim3(nt), 0, stream, p);
+    else hipLaunchKernelGGL((quantize_rows_kernel<T, SCALED, 0>), dim3((unsigned)grid), dim3(nt), 0, stream, p);
     return moe_launch_status();
 }
 
@@ -441,6 +445,7 @@ int moe_launch_quantize_rows(const MoeQuantizeRows& p_, int dtype, int64_t rows,
 {
     if (rows == 0) return MOE_OK;
     MoeQuantizeRows p = p_;
+    p.rows = rows;
     const bool scaled = p.pos || p.coeff || p.col_scale;
     MOE_DISPATCH_DTYPE(dtype, {
         p.vec = (uintptr_t)p.src % 16 == 0 && (p.lds * sizeof(T)) % 16 == 0;

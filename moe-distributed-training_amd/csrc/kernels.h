@@ -230,7 +230,8 @@ struct MoeQuantizeRows {
     const float* col_scale; const void* offsets; int off64; int E;
     int8_t* codes; int64_t ldc; float* scale;
     int64_t cols;
-    int* zero; int zero_n;  // side job of the launch: cleared
+    int* zero; int64_t zero_n;   // side job of the launch: cleared
+    int64_t rows;           // (set by the launcher) workgroups behind these only clear
     int vec, vec_scale;     // (set by the launcher) rows of src, of col_scale, are 16-byte aligned
 };
 int moe_launch_quantize_rows(const MoeQuantizeRows& p, int dtype, int64_t rows, hipStream_t stream);
@@ -267,19 +268,19 @@ struct MoeI8Gemm {
     const void* pos; int pos64; const void* offsets; int off64;
     int E; int64_t K, N;                // K: of one segment
     int fan_out, x_grouped, y_grouped, epi;
-    void* exchange;                     // moe_i8_exchange_bytes; the first moe_i8_counters() ints of it zero at launch, and left so
+    int *zeros, *slots;                 // where split tiles meet (moe_i8_exchange); zeros: zero at launch, and left so
     // set by the launcher
+    int64_t rows;                       // R
     int num_cus, max_split;             // workgroups of a round of the tile plan; K parts that a tile may be cut into
     int *sk_counters, *sk_partials;
     int y_vec;                          // rows of Y take 16-byte stores
 };
 constexpr int MOE_I8_MIN_PART = 4;
-int moe_i8_counters();                  // ints at the start of the exchange area
-int moe_i8_tile(int cus, int64_t R, int E, int64_t N, bool pair);
 int moe_launch_i8_gemm_small(const MoeI8Gemm& p, int64_t R, hipStream_t stream);
 // whether the kernel reads W in this orientation and alignment (otherwise: moe_launch_pack_codes first)
 bool moe_i8_weights_ok(const void* W, int64_t swe, int64_t ldw);
 // whether sizes stay inside the kernel's 32-bit offsets (x_rows: rows of X)
 bool moe_i8_gemm_supported(const MoeI8Gemm& p, int64_t R, int64_t x_rows);
-size_t moe_i8_exchange_bytes(int64_t R, int E, int64_t K, int64_t N, bool pair);   // K: all segments
+struct MoeI8Exchange { int64_t zeros, slots; };   // ints
+MoeI8Exchange moe_i8_exchange(int64_t R, int E, int64_t K, int64_t N, bool pair);   // K: all segments
 int moe_launch_i8_gemm(const MoeI8Gemm& p, int64_t R, hipStream_t stream);

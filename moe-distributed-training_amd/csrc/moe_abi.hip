@@ -67,6 +67,25 @@ inline bool aligned16(const void* p) { return ((uintptr_t)p % 16) == 0; }
 inline size_t pack_bytes(int E, int64_t K) { return al((size_t)E * 16 * (size_t)((K + 31) / 32 * 32) * 2); }   // fragment-order images cover K rounded up to 32
 inline size_t q_bytes(int64_t R) { return al((size_t)pad_rows(R) * 16 * 2); }
 
+// 8-bit expert products: the areas where split tiles meet, of one launch, or of two one behind the other (each leaves the zeros as it found them)
+struct I8Exchange {
+    MoeI8Exchange x;
+    explicit I8Exchange(MoeI8Exchange a, MoeI8Exchange b = {}) : x{a.zeros > b.zeros ? a.zeros : b.zeros, a.slots > b.slots ? a.slots : b.slots} {}
+    size_t bytes() const { return al((size_t)x.zeros * 4) + al((size_t)x.slots * 4); }
+    template <typename... G> void take(Bump& b, MoeQuantizeRows& q, G&... gs) const
+    {
+        q.zero = (int*)b.take((size_t)x.zeros * 4);
+        q.zero_n = x.zeros;
+        int* slots = (int*)b.take((size_t)x.slots * 4);
+        ((gs.zeros = q.zero, gs.slots = slots), ...);
+    }
+};
+inline I8Exchange i8_mlp_exchange(int64_t R, int E, int64_t d, int64_t f, bool backward)
+{
+    return backward ? I8Exchange(moe_i8_exchange(R, E, d, f, false), moe_i8_exchange(R, E, 2 * moe_i8_pitch(f), d, false))
+                    : I8Exchange(moe_i8_exchange(R, E, d, f, true), moe_i8_exchange(R, E, f, d, false));
+}
+
 }  // namespace
 
 extern "C" {
@@ -1080,7 +1099,7 @@ I8Weights i8_weights(const void* W, int64_t swe, int64_t swk, int64_t swn, int E
 
 size_t i8_linear_bytes(const I8Weights& w, int64_t code_rows, int64_t R, int E, int64_t K, int64_t N)
 {
-    return i8_codes_bytes(code_rows, moe_i8_pitch(K)) + w.bytes + moe_i8_exchange_bytes(R, E, K, N, false);
+    return i8_codes_bytes(code_rows, moe_i8_pitch(K)) + w.bytes + I8Exchange(moe_i8_exchange(R, E, K, N, false)).bytes();
 }
 
 // codes of the rows that q describes, and their product; g: what the caller knows of it
@@ -1093,8 +1112,7 @@ int i8_linear(MoeQuantizeRows q, MoeI8Gemm g, int dtype, const I8Weights& w, con
     g.X = q.codes; g.ldx = pitch; g.x_scale = q.scale;
     int8_t* copy = w.copy ? (int8_t*)b.take(w.bytes) : nullptr;
     g.W[0] = copy ? copy : W; g.swe = w.swe; g.ldw = w.ldw; g.nn = w.nn; g.nseg = 1;
-    g.exchange = b.take(moe_i8_exchange_bytes(R, g.E, g.K, g.N, false));
-    q.zero = (int*)g.exchange; q.zero_n = moe_i8_counters();
+    I8Exchange(moe_i8_exchange(R, g.E, g.K, g.N, false)).take(b, q, g);
     g.epi = MOE_I8_STORE;
     if (!moe_i8_gemm_supported(g, R, code_rows)) return MOE_ERR_UNSUPPORTED;
     { TIMED("i8_codes"); TRY(moe_launch_quantize_rows(q, dtype, code_rows, st)); }
@@ -1173,11 +1191,9 @@ size_t moe_mlp_int8_workspace_bytes(int64_t R, int64_t x_rows, int E, int64_t d,
     if (R < 1 || x_rows < 1 || E < 1 || !i8_mlp_sizes_ok(d, f)) return 0;
     const size_t h = i8_seg_bytes(R, f);
     if (!backward) {
-        const size_t xa = moe_i8_exchange_bytes(R, E, d, f, true), xb = moe_i8_exchange_bytes(R, E, f, d, false);
-        return i8_codes_bytes(x_rows, moe_i8_pitch(d)) + h + i8_codes_bytes(R, moe_i8_pitch(f)) + (xa > xb ? xa : xb);
+        return i8_codes_bytes(x_rows, moe_i8_pitch(d)) + h + i8_codes_bytes(R, moe_i8_pitch(f)) + i8_mlp_exchange(R, E, d, f, false).bytes();
     }
-    const size_t xa = moe_i8_exchange_bytes(R, E, d, f, false), xb = moe_i8_exchange_bytes(R, E, 2 * moe_i8_pitch(f), d, false);
-    return i8_codes_bytes(R, moe_i8_pitch(d)) + h + i8_codes_bytes(R, 2 * moe_i8_pitch(f)) + (xa > xb ? xa : xb);
+    return i8_codes_bytes(R, moe_i8_pitch(d)) + h + i8_codes_bytes(R, 2 * moe_i8_pitch(f)) + i8_mlp_exchange(R, E, d, f, true).bytes();
 }
 
 int moe_mlp_int8_fwd(const void* x, int64_t ldx, int64_t x_rows, int dtype, const int8_t* w1, const float* s1, const int8_t* w3, const float* s3,
@@ -1200,7 +1216,6 @@ int moe_mlp_int8_fwd(const void* x, int64_t ldx, int64_t x_rows, int dtype, cons
     const I8Seg h = take_seg(b, R, f);
     int8_t* hq = (int8_t*)b.take((size_t)R * fp);
     float* hs = (float*)b.take((size_t)R * 4);
-    void* exchange = b.base + b.used;
     I8Seg gate = {}, up = {};
     if (saved) { gate = take_seg(sv, R, f); up = take_seg(sv, R, f); }
 
@@ -1210,17 +1225,18 @@ int moe_mlp_int8_fwd(const void* x, int64_t ldx, int64_t x_rows, int dtype, cons
     g.w_scale[0] = s1; g.w_scale[1] = s3;
     g.S[0] = h.v; g.SS[0] = h.s; g.S[1] = gate.v; g.SS[1] = gate.s; g.S[2] = up.v; g.SS[2] = up.s;
     g.pos = pos; g.pos64 = pos64; g.offsets = offsets; g.off64 = off64; g.E = E; g.K = d; g.N = f;
-    g.fan_out = fan_out; g.x_grouped = 0; g.y_grouped = 1; g.epi = MOE_I8_SWIGLU; g.exchange = exchange;
+    g.fan_out = fan_out; g.x_grouped = 0; g.y_grouped = 1; g.epi = MOE_I8_SWIGLU;
     MoeI8Gemm g2 = {};
     g2.X = hq; g2.ldx = fp; g2.x_scale = hs;
     g2.W[0] = w2; g2.swe = f * d; g2.ldw = d; g2.nn = 1; g2.nseg = 1; g2.w_scale[0] = s2;
     g2.Y = y; g2.ldy = ldy; g2.ydtype = dtype;
     g2.pos = pos; g2.pos64 = pos64; g2.offsets = offsets; g2.off64 = off64; g2.E = E; g2.K = f; g2.N = d;
-    g2.fan_out = 1; g2.x_grouped = 1; g2.y_grouped = y_grouped; g2.epi = MOE_I8_STORE; g2.exchange = exchange;
+    g2.fan_out = 1; g2.x_grouped = 1; g2.y_grouped = y_grouped; g2.epi = MOE_I8_STORE;
     if (!moe_i8_gemm_supported(g, R, x_rows) || !moe_i8_gemm_supported(g2, R, R)) return MOE_ERR_UNSUPPORTED;
 
     MoeQuantizeRows q = {};
-    q.src = x; q.lds = ldx; q.codes = xq; q.ldc = dp; q.scale = xs; q.cols = d; q.zero = (int*)exchange; q.zero_n = moe_i8_counters();
+    q.src = x; q.lds = ldx; q.codes = xq; q.ldc = dp; q.scale = xs; q.cols = d;
+    i8_mlp_exchange(R, E, d, f, false).take(b, q, g, g2);
     { TIMED("i8_codes_x"); TRY(moe_launch_quantize_rows(q, dtype, x_rows, st)); }
     { TIMED("i8_gemm_gate_up"); TRY(moe_launch_i8_gemm(g, R, st)); }
     { TIMED("i8_codes_h"); TRY(moe_launch_requantize_rows(h.v, h.s, R, f, hq, fp, hs, st)); }
@@ -1248,7 +1264,6 @@ int moe_mlp_int8_bwd(const void* dy, int64_t lddy, int dtype, int dy_grouped, in
     const I8Seg dh = take_seg(b, R, f);
     int8_t* aq = (int8_t*)b.take((size_t)R * 2 * fp);
     float* as = (float*)b.take((size_t)R * 4);
-    void* exchange = b.base + b.used;
     const I8Seg gate = take_seg(sv, R, f), up = take_seg(sv, R, f);
 
     MoeI8Gemm g = {};   // dh = codes(gates dy s2) W2^T
@@ -1256,19 +1271,19 @@ int moe_mlp_int8_bwd(const void* dy, int64_t lddy, int dtype, int dy_grouped, in
     g.W[0] = w2; g.swe = f * d; g.ldw = d; g.nn = 0; g.nseg = 1;
     g.S[0] = dh.v; g.SS[0] = dh.s;
     g.pos = pos; g.pos64 = pos64; g.offsets = offsets; g.off64 = off64; g.E = E; g.K = d; g.N = f;
-    g.fan_out = 1; g.x_grouped = 1; g.y_grouped = 1; g.epi = MOE_I8_SEG; g.exchange = exchange;
+    g.fan_out = 1; g.x_grouped = 1; g.y_grouped = 1; g.epi = MOE_I8_SEG;
     MoeI8Gemm g2 = {};  // dx = codes(dgate s1 | dup s3) [W1; W3]
     g2.X = aq; g2.ldx = 2 * fp; g2.x_scale = as;
     g2.W[0] = w1; g2.W[1] = w3; g2.swe = f * d; g2.ldw = d; g2.nn = 1; g2.nseg = 2;
     g2.Y = dx_rows; g2.ldy = lddx; g2.ydtype = dtype;
     g2.pos = pos; g2.pos64 = pos64; g2.offsets = offsets; g2.off64 = off64; g2.E = E; g2.K = f; g2.N = d;
-    g2.fan_out = 1; g2.x_grouped = 1; g2.y_grouped = 0; g2.epi = MOE_I8_STORE; g2.exchange = exchange;
+    g2.fan_out = 1; g2.x_grouped = 1; g2.y_grouped = 0; g2.epi = MOE_I8_STORE;
     if (!moe_i8_gemm_supported(g, R, R) || !moe_i8_gemm_supported(g2, R, R)) return MOE_ERR_UNSUPPORTED;
 
     MoeQuantizeRows q = {};
     q.src = dy; q.lds = lddy; q.pos = dy_grouped ? nullptr : pos; q.pos64 = pos64; q.fan_out = dy_fan_out; q.coeff = gates; q.coeff_dtype = gates_dtype;
     q.col_scale = s2; q.offsets = offsets; q.off64 = off64; q.E = E; q.codes = gq; q.ldc = dp; q.scale = gs; q.cols = d;
-    q.zero = (int*)exchange; q.zero_n = moe_i8_counters();
+    i8_mlp_exchange(R, E, d, f, true).take(b, q, g, g2);
     const MoeSwigluBwdCodes a = {dh.v, gate.v, up.v, dh.s, gate.s, up.s, s1, s3, offsets, off64, E, aq, fp, as, f};
     { TIMED("i8_codes_dy"); TRY(moe_launch_quantize_rows(q, dtype, R, st)); }
     { TIMED("i8_gemm_dh"); TRY(moe_launch_i8_gemm(g, R, st)); }
