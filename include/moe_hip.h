@@ -258,13 +258,19 @@ int moe_mlp_bwd(const void* dy, int64_t lddy, int dy_grouped, int dy_fan_out, co
  *
  * moe_quantize_rows: rows of src -> codes (pitch ldc >= ncols, a multiple of 16, 16-byte aligned; columns from ncols on are written as zeros) and scales. */
 int moe_quantize_rows(const void* src, int64_t lds, int dtype, int8_t* codes, int64_t ldc, float* scale, int64_t nrows, int64_t ncols, void* stream);
+/* moe_combine and moe_combine_dgates of fp32 rows in token order and an output, or dout, of `dtype`: out[t] = sum_j gates[t*k+j] * y[t*k+j] (gates NULL: 1),
+ * d_gates[t*k+j] = <y[t*k+j], dout[t]>. */
+int moe_combine_f32(const float* y, int64_t ldy, void* out, int64_t ldo, int dtype, const void* gates, int gates_dtype, int k, int64_t ntok,
+                    int64_t ncols, void* stream);
+int moe_combine_f32_dgates(const float* y, int64_t ldy, const void* dout, int64_t ldd, int dtype, void* dgates, int gates_dtype, int k, int64_t ntok,
+                           int64_t ncols, void* stream);
 /* weights (E,K,N) of any strides -> codes (E,K,N) of any strides and scale (E,N), the maximum taken over K */
 size_t moe_quantize_weights_workspace_bytes(int E, int64_t N);
 int moe_quantize_weights(const void* W, int64_t swe, int64_t swk, int64_t swn, int dtype, int E, int64_t K, int64_t N, int8_t* codes, int64_t sce,
                          int64_t sck, int64_t scn, float* scale, void* workspace, size_t workspace_bytes, void* stream);
 /* moe_scatter2scatter without adapters over 8-bit weights: codes and scales sx of the x_rows rows of x, then
  *   y[out_row] = sx[in_row] * w_scale[e][n] * (codes[in_row] @ W[e]),   rows addressed as there.
- * W (E,K,N) of any strides: read in place where contiguous along K or N with the other strides and the address multiples of 16, otherwise through a copy in
+ * x of `dtype`, y of y_dtype, dx of dx_dtype.  W (E,K,N) of any strides: read in place where contiguous along K or N with the other strides and the address multiples of 16, otherwise through a copy in
  * the workspace.  Backward (weights frozen, the codes' rounding straight through): row m of the order is dY's row m (dy_grouped) or pos[m] / dy_fan_out, times
  * gates[pos[m]] (gates[m] with dy_grouped; NULL: 1) and, column by column, w_scale[e]; of its codes and scale sg
  *   dx_rows[dx_grouped ? m : pos[m]] = sg[m] * (codes[m] @ W[e]^T).
@@ -272,12 +278,12 @@ int moe_quantize_weights(const void* W, int64_t swe, int64_t swk, int64_t swn, i
  * are not written. */
 size_t moe_linear_int8_workspace_bytes(const int8_t* W, int64_t swe, int64_t swk, int64_t swn, int64_t code_rows, int64_t R, int E, int64_t K, int64_t N);
 int moe_linear_int8_fwd(const void* x, int64_t ldx, int64_t x_rows, int dtype, const int8_t* W, int64_t swe, int64_t swk, int64_t swn,
-                        const float* w_scale, void* y, int64_t ldy, const void* pos, int pos64, const void* offsets, int off64, int E, int64_t R, int64_t K,
+                        const float* w_scale, void* y, int64_t ldy, int y_dtype, const void* pos, int pos64, const void* offsets, int off64, int E, int64_t R, int64_t K,
                         int64_t N, int fan_out, int x_grouped, int y_grouped, void* workspace, size_t workspace_bytes, void* stream);
 int moe_linear_int8_bwd(const void* dy, int64_t lddy, int dtype, int dy_grouped, int dy_fan_out, const void* gates, int gates_dtype, const int8_t* W,
-                        int64_t swe, int64_t swk, int64_t swn, const float* w_scale, void* dx_rows, int64_t lddx, int dx_grouped, const void* pos, int pos64,
+                        int64_t swe, int64_t swk, int64_t swn, const float* w_scale, void* dx_rows, int64_t lddx, int dx_dtype, int dx_grouped, const void* pos, int pos64,
                         const void* offsets, int off64, int E, int64_t R, int64_t K, int64_t N, void* workspace, size_t workspace_bytes, void* stream);
-/* The expert MLP of moe_mlp_fwd / moe_mlp_bwd over 8-bit weights: w1, w3, w2 codes (E,f,d) contiguous, scales s1, s3 (E,f) and s2 (E,d); bf16 or fp16 x, y, dy, dx;
+/* The expert MLP of moe_mlp_fwd / moe_mlp_bwd over 8-bit weights: w1, w3, w2 codes (E,f,d) contiguous, scales s1, s3 (E,f) and s2 (E,d); bf16 or fp16 x and dy (`dtype`), y of y_dtype, dx of dx_dtype;
  * d and f multiples of 64.  x has x_rows rows; row m of the order is row pos[m] / fan_out of them.
  * Forward:  gate, up = codes(x) W1, codes(x) W3;  h = silu(gate) * up;  y[out_row] = codes(h) W2.  `saved` (or NULL): gate and up for the backward pass.
  * Backward (weights frozen, the codes' rounding straight through), dy rows addressed and weighted as in moe_mlp_bwd, gates one weight per flat position or NULL:
@@ -285,12 +291,12 @@ int moe_linear_int8_bwd(const void* dy, int64_t lddy, int dtype, int dy_grouped,
 size_t moe_mlp_int8_saved_bytes(int64_t R, int64_t f);
 size_t moe_mlp_int8_workspace_bytes(int64_t R, int64_t x_rows, int E, int64_t d, int64_t f, int backward);
 int moe_mlp_int8_fwd(const void* x, int64_t ldx, int64_t x_rows, int dtype, const int8_t* w1, const float* s1, const int8_t* w3, const float* s3,
-                     const int8_t* w2, const float* s2, void* y, int64_t ldy, const void* pos, int pos64, const void* offsets, int off64, int E,
+                     const int8_t* w2, const float* s2, void* y, int64_t ldy, int y_dtype, const void* pos, int pos64, const void* offsets, int off64, int E,
                      int64_t R, int64_t d, int64_t f, int fan_out, int y_grouped, void* saved, size_t saved_bytes, void* workspace,
                      size_t workspace_bytes, void* stream);
 int moe_mlp_int8_bwd(const void* dy, int64_t lddy, int dtype, int dy_grouped, int dy_fan_out, const void* gates, int gates_dtype, const int8_t* w1,
                      const float* s1, const int8_t* w3, const float* s3, const int8_t* w2, const float* s2, const void* saved, size_t saved_bytes,
-                     void* dx_rows, int64_t lddx, const void* pos, int pos64, const void* offsets, int off64, int E, int64_t R, int64_t d, int64_t f,
+                     void* dx_rows, int64_t lddx, int dx_dtype, const void* pos, int pos64, const void* offsets, int off64, int E, int64_t R, int64_t d, int64_t f,
                      void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus

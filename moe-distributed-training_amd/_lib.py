@@ -66,12 +66,14 @@ _SIGNATURES = {
     "moe_quantize_weights_workspace_bytes": ("z", "il"),
     "moe_quantize_weights": ("i", "plll" + "iill" + "plll" + "p" + "pzp"),
     "moe_linear_int8_workspace_bytes": ("z", "plll" + "llill"),
-    "moe_linear_int8_fwd": ("i", "plli" + "plll" + "p" + "pl" + "pi" + "pi" + "i" + "lll" + "iii" + "pzp"),
-    "moe_linear_int8_bwd": ("i", "pliii" + "pi" + "plll" + "p" + "pli" + "pi" + "pi" + "i" + "lll" + "pzp"),
+    "moe_combine_f32": ("i", "plpli" + "piill" + "p"),
+    "moe_combine_f32_dgates": ("i", "plpli" + "piill" + "p"),
+    "moe_linear_int8_fwd": ("i", "plli" + "plll" + "p" + "pli" + "pi" + "pi" + "i" + "lll" + "iii" + "pzp"),
+    "moe_linear_int8_bwd": ("i", "pliii" + "pi" + "plll" + "p" + "plii" + "pi" + "pi" + "i" + "lll" + "pzp"),
     "moe_mlp_int8_saved_bytes": ("z", "ll"),
     "moe_mlp_int8_workspace_bytes": ("z", "llilli"),
-    "moe_mlp_int8_fwd": ("i", "plli" + "pppppp" + "pl" + "pi" + "pi" + "i" + "lll" + "ii" + "pz" + "pzp"),
-    "moe_mlp_int8_bwd": ("i", "pliii" + "pi" + "pppppp" + "pz" + "pl" + "pi" + "pi" + "i" + "lll" + "pzp"),
+    "moe_mlp_int8_fwd": ("i", "plli" + "pppppp" + "pli" + "pi" + "pi" + "i" + "lll" + "ii" + "pz" + "pzp"),
+    "moe_mlp_int8_bwd": ("i", "pliii" + "pi" + "pppppp" + "pz" + "pli" + "pi" + "pi" + "i" + "lll" + "pzp"),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

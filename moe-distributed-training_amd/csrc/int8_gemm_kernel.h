@@ -391,7 +391,7 @@ __global__ void __launch_bounds__(NTHREADS, 2) i8_gemm_kernel(const MoeI8Gemm p)
                 for (int i = 0; i < 8; ++i) v[i] = fine ? v[i] : 0.f;
             int q[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) q[i] = (int)(v[i] * inv);
+            for (int i = 0; i < 8; ++i) q[i] = (int)rintf(v[i] * inv);
             u32x4_t hi;
             uint2 lo;
 #pragma unroll

@@ -9,7 +9,7 @@
 // gradient rows took 92 us.)  A row that holds an infinity or a NaN gets the scale NaN and codes 0, so that every product of it is NaN and
 // no other row changes; a row of zeros the scale 0.
 //
-// Interims (h, the saved gate and up, dh) travel as 24-bit integers with a scale for each 32 columns of a row: 3 bytes per value, at most 2^-23 of the segment's
+// Interims (h, the saved gate and up, dh) travel as 24-bit integers with a scale for each 32 columns of a row: 3 bytes per value, at most 2^-24 of the segment's
 // maximum off.  Every value that a rounding on the way carries over a border of the 8-bit codes costs a whole step, so this noise falls with the root of
 // the rounding only: with 16 bits 1 code in 700 changed and the MLP's error against 64 bits was 1.5e-3 of its result's norm (bf16 rows would be off by four
 // times that), with 24 it is that of fp32 arithmetic, at three quarters of an fp32 tensor's bytes.
@@ -342,6 +342,63 @@ __global__ void __launch_bounds__(KEEP == 1 ? 256 : 512) swiglu_bwd_codes_kernel
     if (threadIdx.x == 0) p.scale[m] = rc.scale;
 }
 
+// Weighted sums of fp32 rows, out[t] = sum_j gates[t*k+j] y[t*k+j] (no gates: 1), in the output's type: the rows of a token's experts, or of its gradient, meet before
+// they are rounded.  (Rounded to bf16 first, a result is off by 1.4 times its own rounding; the fp32 rows cost 1 % of a step of 4096 tokens.)  Four columns a thread.
+template <typename T> __device__ __forceinline__ void store4(T* p, const float* v);
+template <> __device__ __forceinline__ void store4(float* p, const float* v) { *(float4*)p = make_float4(v[0], v[1], v[2], v[3]); }
+template <> __device__ __forceinline__ void store4(__hip_bfloat16* p, const float* v) { *(uint2*)p = make_uint2(NumBf16::pack2(v[0], v[1]), NumBf16::pack2(v[2], v[3])); }
+template <> __device__ __forceinline__ void store4(__half* p, const float* v) { *(uint2*)p = make_uint2(NumF16::pack2(v[0], v[1]), NumF16::pack2(v[2], v[3])); }
+
+template <typename T>
+__global__ void __launch_bounds__(256) combine_f32_kernel(const float* y, int64_t ldy, T* out, int64_t ldo, const void* gates, int gdtype, int k, int64_t cols, int vec)
+{
+    const int64_t t = blockIdx.x;
+    for (int64_t c = ((int64_t)blockIdx.y * 256 + threadIdx.x) * 4; c < cols; c += (int64_t)gridDim.y * 1024) {
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < k; ++j) {
+            const float g = gates ? load_gate(gates, t * k + j, gdtype) : 1.f;
+            const float* row = y + (t * k + j) * ldy + c;
+            float4 x;
+            if (vec) x = *(const float4*)row;
+            else x = make_float4(row[0], c + 1 < cols ? row[1] : 0.f, c + 2 < cols ? row[2] : 0.f, c + 3 < cols ? row[3] : 0.f);
+            v[0] = fmaf(g, x.x, v[0]); v[1] = fmaf(g, x.y, v[1]); v[2] = fmaf(g, x.z, v[2]); v[3] = fmaf(g, x.w, v[3]);
+        }
+        if (vec) store4(out + t * ldo + c, v);
+        else
+            for (int i = 0; i < 4; ++i)
+                if (c + i < cols) Elem<T>::st(out + t * ldo + c + i, v[i]);
+    }
+}
+
+// d_gates[p] = <y[p], dout[p / k]> of fp32 rows y; a workgroup per flat position
+template <typename T>
+__global__ void __launch_bounds__(256) dgates_f32_kernel(const float* y, int64_t ldy, const T* dout, int64_t ldd, void* dgates, int gdtype, int k, int64_t cols, int vec)
+{
+    const int64_t p = blockIdx.x;
+    const float* row = y + p * ldy;
+    const T* d = dout + p / k * ldd;
+    float s = 0.f;
+    for (int64_t c = (int64_t)threadIdx.x * 8; c < cols; c += 2048) {
+        float a[8], b[8];
+        if (vec) { Loader<float>::ld8(row + c, a); Loader<T>::ld8(d + c, b); }
+        else
+#pragma unroll
+            for (int i = 0; i < 8; ++i) { a[i] = c + i < cols ? row[c + i] : 0.f; b[i] = c + i < cols ? Elem<T>::ld(d + c + i) : 0.f; }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s = fmaf(a[i], b[i], s);
+    }
+    __shared__ float part[4];
+#pragma unroll
+    for (int m = 32; m > 0; m >>= 1) s += __shfl_xor(s, m);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    s = (part[0] + part[1]) + (part[2] + part[3]);
+    if (gdtype == MOE_F32) ((float*)dgates)[p] = s;
+    else if (gdtype == MOE_BF16) ((uint16_t*)dgates)[p] = NumBf16::from_f32(s);
+    else ((uint16_t*)dgates)[p] = NumF16::from_f32(s);
+}
+
 // Expert matrices whose rows are contiguous but not 16-byte aligned -> the same rows at a pitch of ldo, a multiple of 16.  16 bytes per lane, unaligned loads.
 __global__ void __launch_bounds__(256) repitch_codes_kernel(const int8_t* W, int64_t swe, int64_t ldw, int64_t rows, int64_t cols, int8_t* out, int64_t ldo)
 {
@@ -430,7 +487,7 @@ template <typename T, bool SCALED> int launch_quantize_t(const MoeQuantizeRows& 
 {
     // pieces of 8 columns: one to four of them a thread
     const int64_t pieces = (p.ldc + 7) / 8, grid = rows + (p.zero_n + ZERO_PIECE - 1) / ZERO_PIECE;
-    const int nt = pieces <= 64 ? 64 : pieces <= 128 ? 128 : pieces <= 1024 ? 256 : pieces <= 2048 ? 512 : 1024;
+    const int nt = pieces <= 64 ? 64 : pieces <= 128 ? 128 : pieces <= 256 || (pieces <= 1024 && rows > 256) ? 256 : pieces <= 512 || (pieces <= 2048 && rows > 256) ? 512 : 1024;
     const int64_t keep = (pieces + nt - 1) / nt;
     if (keep <= 1) hipLaunchKernelGGL((quantize_rows_kernel<T, SCALED, 1>), dim3((unsigned)grid), dim3(nt), 0, stream, p);
     else if (keep <= 2) hipLaunchKernelGGL((quantize_rows_kernel<T, SCALED, 2>), dim3((unsigned)grid), dim3(nt), 0, stream, p);
@@ -457,7 +514,8 @@ int moe_launch_quantize_rows(const MoeQuantizeRows& p_, int dtype, int64_t rows,
 int moe_launch_requantize_rows(const uint8_t* src, const float* seg, int64_t rows, int64_t cols, int8_t* codes, int64_t ldc, float* scale, hipStream_t stream)
 {
     if (rows == 0) return MOE_OK;
-    const int nt = ldc / 8 <= 64 ? 64 : ldc / 8 <= 128 ? 128 : 256;
+    // (few rows: latency is all of it, and more threads have less each)
+    const int nt = ldc / 8 <= 64 ? 64 : ldc / 8 <= 128 ? 128 : rows > 256 || ldc / 8 <= 256 ? 256 : ldc / 8 <= 512 ? 512 : 1024;
     hipLaunchKernelGGL(requantize_rows_kernel, dim3((unsigned)rows), dim3(nt), 0, stream, src, seg, cols, codes, ldc, scale);
     return moe_launch_status();
 }
@@ -498,6 +556,29 @@ int moe_launch_quantize_weights(const void* W, int64_t swe, int64_t swk, int64_t
     MOE_DISPATCH_DTYPE(dtype, {
         hipLaunchKernelGGL(weight_max_kernel<T>, g1, dim3(256), 0, stream, (const T*)W, swe, swk, swn, K, N, top);
         hipLaunchKernelGGL(weight_codes_kernel<T>, g2, dim3(256), 0, stream, (const T*)W, swe, swk, swn, K, N, top, codes, sce, sck, scn, scale);
+        return moe_launch_status();
+    });
+}
+
+int moe_launch_combine_f32(const float* y, int64_t ldy, void* out, int64_t ldo, int dtype, const void* gates, int gdtype, int k, int64_t ntok, int64_t ncols, hipStream_t stream)
+{
+    if (ntok == 0 || ncols == 0) return MOE_OK;
+    // (few tokens: the columns of one are dealt to several workgroups)
+    const int64_t pieces = (ncols + 1023) / 1024;
+    const dim3 grid((unsigned)ntok, (unsigned)(ntok < 1024 ? pieces : (pieces + 3) / 4));
+    MOE_DISPATCH_DTYPE(dtype, {
+        const int vec = ncols % 4 == 0 && ldy % 4 == 0 && ldo % 4 == 0 && (uintptr_t)y % 16 == 0 && (uintptr_t)out % (4 * sizeof(T)) == 0;
+        hipLaunchKernelGGL(combine_f32_kernel<T>, grid, dim3(256), 0, stream, y, ldy, (T*)out, ldo, gates, gdtype, k, ncols, vec);
+        return moe_launch_status();
+    });
+}
+
+int moe_launch_dgates_f32(const float* y, int64_t ldy, const void* dout, int64_t ldd, int dtype, void* dgates, int gdtype, int k, int64_t ntok, int64_t ncols, hipStream_t stream)
+{
+    if (ntok == 0 || k == 0) return MOE_OK;
+    MOE_DISPATCH_DTYPE(dtype, {
+        const int vec = ncols % 8 == 0 && ldy % 4 == 0 && (uintptr_t)y % 16 == 0 && (uintptr_t)dout % 16 == 0 && ldd * sizeof(T) % 16 == 0;
+        hipLaunchKernelGGL(dgates_f32_kernel<T>, dim3((unsigned)(ntok * k)), dim3(256), 0, stream, y, ldy, (const T*)dout, ldd, dgates, gdtype, k, ncols, vec);
         return moe_launch_status();
     });
 }

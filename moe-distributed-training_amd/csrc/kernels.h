@@ -251,6 +251,9 @@ int moe_launch_pack_codes(const int8_t* W, int64_t swe, int64_t swk, int64_t swn
 int moe_launch_quantize_weights(const void* W, int64_t swe, int64_t swk, int64_t swn, int dtype, int E, int64_t K, int64_t N, int8_t* codes, int64_t sce,
                                 int64_t sck, int64_t scn, float* scale, uint32_t* top, hipStream_t stream);
 
+int moe_launch_combine_f32(const float* y, int64_t ldy, void* out, int64_t ldo, int dtype, const void* gates, int gdtype, int k, int64_t ntok, int64_t ncols, hipStream_t stream);
+int moe_launch_dgates_f32(const float* y, int64_t ldy, const void* dout, int64_t ldd, int dtype, void* dgates, int gdtype, int k, int64_t ntok, int64_t ncols, hipStream_t stream);
+
 // epilogues of the 8-bit grouped product
 #define MOE_I8_STORE 0      // Y = acc * x_scale * w_scale in ydtype
 #define MOE_I8_SEG 1        // the same as segments (grouped rows)

@@ -1071,6 +1071,28 @@ int moe_quantize_rows(const void* src, int64_t lds, int dtype, int8_t* codes, in
     return moe_launch_quantize_rows(q, dtype, nrows, S(stream));
 }
 
+int moe_combine_f32(const float* y, int64_t ldy, void* out, int64_t ldo, int dtype, const void* gates, int gates_dtype, int k, int64_t ntok, int64_t ncols, void* stream)
+{
+    hipStream_t st = S(stream);
+    if (dtype < 0 || dtype > 2 || k < 1 || ntok < 0 || ncols < 0 || ldy < ncols || ldo < ncols || (gates && (gates_dtype < 0 || gates_dtype > 2))) return MOE_ERR_BAD_ARG;
+    if (ntok == 0 || ncols == 0) return MOE_OK;
+    if (!y || !out) return MOE_ERR_BAD_ARG;
+    if (ntok > 0x7fffffff) return MOE_ERR_UNSUPPORTED;
+    TIMED("rows.combine_f32");
+    return moe_launch_combine_f32(y, ldy, out, ldo, dtype, gates, gates_dtype, k, ntok, ncols, st);
+}
+
+int moe_combine_f32_dgates(const float* y, int64_t ldy, const void* dout, int64_t ldd, int dtype, void* dgates, int gates_dtype, int k, int64_t ntok, int64_t ncols, void* stream)
+{
+    hipStream_t st = S(stream);
+    if (dtype < 0 || dtype > 2 || gates_dtype < 0 || gates_dtype > 2 || k < 1 || ntok < 0 || ncols < 0 || ldy < ncols || ldd < ncols) return MOE_ERR_BAD_ARG;
+    if (ntok == 0) return MOE_OK;
+    if (!y || !dout || !dgates) return MOE_ERR_BAD_ARG;
+    if (ntok * k > 0x7fffffff) return MOE_ERR_UNSUPPORTED;
+    TIMED("rows.combine_f32_dgates");
+    return moe_launch_dgates_f32(y, ldy, dout, ldd, dtype, dgates, gates_dtype, k, ntok, ncols, st);
+}
+
 size_t moe_quantize_weights_workspace_bytes(int E, int64_t N) { return E < 1 || N < 1 ? 0 : (size_t)E * (size_t)N * 4; }
 
 int moe_quantize_weights(const void* W, int64_t swe, int64_t swk, int64_t swn, int dtype, int E, int64_t K, int64_t N, int8_t* codes, int64_t sce,
@@ -1133,10 +1155,10 @@ size_t moe_linear_int8_workspace_bytes(const int8_t* W, int64_t swe, int64_t swk
 }
 
 int moe_linear_int8_fwd(const void* x, int64_t ldx, int64_t x_rows, int dtype, const int8_t* W, int64_t swe, int64_t swk, int64_t swn,
-                        const float* w_scale, void* y, int64_t ldy, const void* pos, int pos64, const void* offsets, int off64, int E, int64_t R, int64_t K,
+                        const float* w_scale, void* y, int64_t ldy, int y_dtype, const void* pos, int pos64, const void* offsets, int off64, int E, int64_t R, int64_t K,
                         int64_t N, int fan_out, int x_grouped, int y_grouped, void* workspace, size_t workspace_bytes, void* stream)
 {
-    if (dtype < 0 || dtype > 2 || E < 1 || R < 0 || x_rows < 0 || K < 1 || N < 0 || fan_out < 1 || ldx < K || ldy < N) return MOE_ERR_BAD_ARG;
+    if (dtype < 0 || dtype > 2 || y_dtype < 0 || y_dtype > 2 || E < 1 || R < 0 || x_rows < 0 || K < 1 || N < 0 || fan_out < 1 || ldx < K || ldy < N) return MOE_ERR_BAD_ARG;
     if (R == 0 || N == 0) return MOE_OK;
     if (!x || x_rows < 1 || !W || !w_scale || !y || !offsets || ((!x_grouped || !y_grouped) && !pos) || (x_grouped && x_rows < R)) return MOE_ERR_BAD_ARG;
     if (K > MOE_I8_MAX_K || E > 65535 || x_rows > 0x7fffffff) return MOE_ERR_UNSUPPORTED;
@@ -1145,17 +1167,17 @@ int moe_linear_int8_fwd(const void* x, int64_t ldx, int64_t x_rows, int dtype, c
     MoeQuantizeRows q = {};
     q.src = x; q.lds = ldx;
     MoeI8Gemm g = {};
-    g.w_scale[0] = w_scale; g.Y = y; g.ldy = ldy; g.ydtype = dtype;
+    g.w_scale[0] = w_scale; g.Y = y; g.ldy = ldy; g.ydtype = y_dtype;
     g.pos = pos; g.pos64 = pos64; g.offsets = offsets; g.off64 = off64; g.E = E; g.K = K; g.N = N;
     g.fan_out = fan_out; g.x_grouped = x_grouped; g.y_grouped = y_grouped;
     return i8_linear(q, g, dtype, w, W, swe, swk, swn, x_rows, R, workspace, S(stream));
 }
 
 int moe_linear_int8_bwd(const void* dy, int64_t lddy, int dtype, int dy_grouped, int dy_fan_out, const void* gates, int gates_dtype, const int8_t* W,
-                        int64_t swe, int64_t swk, int64_t swn, const float* w_scale, void* dx_rows, int64_t lddx, int dx_grouped, const void* pos, int pos64,
+                        int64_t swe, int64_t swk, int64_t swn, const float* w_scale, void* dx_rows, int64_t lddx, int dx_dtype, int dx_grouped, const void* pos, int pos64,
                         const void* offsets, int off64, int E, int64_t R, int64_t K, int64_t N, void* workspace, size_t workspace_bytes, void* stream)
 {
-    if (dtype < 0 || dtype > 2 || E < 1 || R < 0 || K < 0 || N < 1 || dy_fan_out < 1 || lddy < N || lddx < K || (gates && (gates_dtype < 0 || gates_dtype > 2))) return MOE_ERR_BAD_ARG;
+    if (dtype < 0 || dtype > 2 || dx_dtype < 0 || dx_dtype > 2 || E < 1 || R < 0 || K < 0 || N < 1 || dy_fan_out < 1 || lddy < N || lddx < K || (gates && (gates_dtype < 0 || gates_dtype > 2))) return MOE_ERR_BAD_ARG;
     if (R == 0 || K == 0) return MOE_OK;
     if (!dy || !W || !w_scale || !dx_rows || !offsets || ((!dy_grouped || !dx_grouped) && !pos)) return MOE_ERR_BAD_ARG;
     if (N > MOE_I8_MAX_K || E > 65535 || R > 0x7fffffff) return MOE_ERR_UNSUPPORTED;
@@ -1165,7 +1187,7 @@ int moe_linear_int8_bwd(const void* dy, int64_t lddy, int dtype, int dy_grouped,
     q.src = dy; q.lds = lddy; q.pos = dy_grouped ? nullptr : pos; q.pos64 = pos64; q.fan_out = dy_fan_out; q.coeff = gates; q.coeff_dtype = gates_dtype;
     q.col_scale = w_scale; q.offsets = offsets; q.off64 = off64; q.E = E;
     MoeI8Gemm g = {};
-    g.Y = dx_rows; g.ldy = lddx; g.ydtype = dtype;
+    g.Y = dx_rows; g.ldy = lddx; g.ydtype = dx_dtype;
     g.pos = pos; g.pos64 = pos64; g.offsets = offsets; g.off64 = off64; g.E = E; g.K = N; g.N = K;
     g.fan_out = 1; g.x_grouped = 1; g.y_grouped = dx_grouped;
     return i8_linear(q, g, dtype, w, W, swe, swn, swk, R, R, workspace, S(stream));
@@ -1197,12 +1219,12 @@ size_t moe_mlp_int8_workspace_bytes(int64_t R, int64_t x_rows, int E, int64_t d,
 }
 
 int moe_mlp_int8_fwd(const void* x, int64_t ldx, int64_t x_rows, int dtype, const int8_t* w1, const float* s1, const int8_t* w3, const float* s3,
-                     const int8_t* w2, const float* s2, void* y, int64_t ldy, const void* pos, int pos64, const void* offsets, int off64, int E,
+                     const int8_t* w2, const float* s2, void* y, int64_t ldy, int y_dtype, const void* pos, int pos64, const void* offsets, int off64, int E,
                      int64_t R, int64_t d, int64_t f, int fan_out, int y_grouped, void* saved, size_t saved_bytes, void* workspace,
                      size_t workspace_bytes, void* stream)
 {
     hipStream_t st = S(stream);
-    if (dtype < 0 || dtype > 2 || E < 1 || R < 0 || x_rows < 0 || d < 1 || f < 1 || fan_out < 1 || ldx < d || ldy < d) return MOE_ERR_BAD_ARG;
+    if (dtype < 0 || dtype > 2 || y_dtype < 0 || y_dtype > 2 || E < 1 || R < 0 || x_rows < 0 || d < 1 || f < 1 || fan_out < 1 || ldx < d || ldy < d) return MOE_ERR_BAD_ARG;
     if (R == 0) return MOE_OK;
     if (!x || x_rows < 1 || !w1 || !s1 || !w3 || !s3 || !w2 || !s2 || !y || !pos || !offsets) return MOE_ERR_BAD_ARG;
     if (dtype == MOE_F32 || !i8_mlp_sizes_ok(d, f) || d > MOE_I8_MAX_K || f > MOE_I8_MAX_K || E > 65535 || x_rows > 0x7fffffff || R > 0x7fffffff) return MOE_ERR_UNSUPPORTED;
@@ -1229,7 +1251,7 @@ int moe_mlp_int8_fwd(const void* x, int64_t ldx, int64_t x_rows, int dtype, cons
     MoeI8Gemm g2 = {};
     g2.X = hq; g2.ldx = fp; g2.x_scale = hs;
     g2.W[0] = w2; g2.swe = f * d; g2.ldw = d; g2.nn = 1; g2.nseg = 1; g2.w_scale[0] = s2;
-    g2.Y = y; g2.ldy = ldy; g2.ydtype = dtype;
+    g2.Y = y; g2.ldy = ldy; g2.ydtype = y_dtype;
     g2.pos = pos; g2.pos64 = pos64; g2.offsets = offsets; g2.off64 = off64; g2.E = E; g2.K = f; g2.N = d;
     g2.fan_out = 1; g2.x_grouped = 1; g2.y_grouped = y_grouped; g2.epi = MOE_I8_STORE;
     if (!moe_i8_gemm_supported(g, R, x_rows) || !moe_i8_gemm_supported(g2, R, R)) return MOE_ERR_UNSUPPORTED;
@@ -1246,11 +1268,11 @@ int moe_mlp_int8_fwd(const void* x, int64_t ldx, int64_t x_rows, int dtype, cons
 
 int moe_mlp_int8_bwd(const void* dy, int64_t lddy, int dtype, int dy_grouped, int dy_fan_out, const void* gates, int gates_dtype, const int8_t* w1,
                      const float* s1, const int8_t* w3, const float* s3, const int8_t* w2, const float* s2, const void* saved, size_t saved_bytes,
-                     void* dx_rows, int64_t lddx, const void* pos, int pos64, const void* offsets, int off64, int E, int64_t R, int64_t d, int64_t f,
+                     void* dx_rows, int64_t lddx, int dx_dtype, const void* pos, int pos64, const void* offsets, int off64, int E, int64_t R, int64_t d, int64_t f,
                      void* workspace, size_t workspace_bytes, void* stream)
 {
     hipStream_t st = S(stream);
-    if (dtype < 0 || dtype > 2 || E < 1 || R < 0 || d < 1 || f < 1 || dy_fan_out < 1 || lddy < d || lddx < d || (gates && (gates_dtype < 0 || gates_dtype > 2 || dy_grouped))) return MOE_ERR_BAD_ARG;
+    if (dtype < 0 || dtype > 2 || dx_dtype < 0 || dx_dtype > 2 || E < 1 || R < 0 || d < 1 || f < 1 || dy_fan_out < 1 || lddy < d || lddx < d || (gates && (gates_dtype < 0 || gates_dtype > 2 || dy_grouped))) return MOE_ERR_BAD_ARG;
     if (R == 0) return MOE_OK;
     if (!dy || !w1 || !s1 || !w3 || !s3 || !w2 || !s2 || !saved || !dx_rows || !pos || !offsets) return MOE_ERR_BAD_ARG;
     if (dtype == MOE_F32 || !i8_mlp_sizes_ok(d, f) || d > MOE_I8_MAX_K || 2 * f > MOE_I8_MAX_K || E > 65535 || R > 0x7fffffff) return MOE_ERR_UNSUPPORTED;
@@ -1275,7 +1297,7 @@ int moe_mlp_int8_bwd(const void* dy, int64_t lddy, int dtype, int dy_grouped, in
     MoeI8Gemm g2 = {};  // dx = codes(dgate s1 | dup s3) [W1; W3]
     g2.X = aq; g2.ldx = 2 * fp; g2.x_scale = as;
     g2.W[0] = w1; g2.W[1] = w3; g2.swe = f * d; g2.ldw = d; g2.nn = 1; g2.nseg = 2;
-    g2.Y = dx_rows; g2.ldy = lddx; g2.ydtype = dtype;
+    g2.Y = dx_rows; g2.ldy = lddx; g2.ydtype = dx_dtype;
     g2.pos = pos; g2.pos64 = pos64; g2.offsets = offsets; g2.off64 = off64; g2.E = E; g2.K = f; g2.N = d;
     g2.fan_out = 1; g2.x_grouped = 1; g2.y_grouped = 0; g2.epi = MOE_I8_STORE;
     if (!moe_i8_gemm_supported(g, R, R) || !moe_i8_gemm_supported(g2, R, R)) return MOE_ERR_UNSUPPORTED;

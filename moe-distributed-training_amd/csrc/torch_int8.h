@@ -3,6 +3,25 @@
 
 inline int64_t code_pitch(int64_t cols) { return (cols + 127) / 128 * 128; }
 
+// Rows that are summed per token stay fp32 until then (sums: whether they are).
+inline at::ScalarType rows_type(at::ScalarType dt, bool sums) { return sums ? at::kFloat : dt; }
+
+Tensor combine_rows(const Tensor& y, const Tensor& gates, int64_t k, int64_t T, at::ScalarType dt)
+{
+    Tensor out = at::empty({T, y.size(1)}, y.options().dtype(dt));
+    check(moe_combine_f32((const float*)ptr(y), y.stride(0), ptr(out), out.stride(0), dtype_code(out), ptr(gates), gates.defined() ? dtype_code(gates) : 0, (int)k, T,
+                          y.size(1), stream_of(y)), "moe_combine_f32");
+    return out;
+}
+
+Tensor combine_rows_dgates(const Tensor& y, const Tensor& dout, int64_t k, at::ScalarType dt)
+{
+    Tensor dg = at::empty({dout.size(0), k}, y.options().dtype(dt));
+    check(moe_combine_f32_dgates((const float*)ptr(y), y.stride(0), ptr(dout), dout.stride(0), dtype_code(dout), ptr(dg), dtype_code(dg), (int)k, dout.size(0), y.size(1),
+                                 stream_of(y)), "moe_combine_f32_dgates");
+    return dg;
+}
+
 // (codes (rows, cols), scale (rows)); the codes are a view of whole 128-column pieces
 variable_list quantize_rows(const Tensor& x_)
 {
@@ -46,14 +65,14 @@ void check_codes(const Tensor& q, const Tensor& scale, int64_t E, int64_t N)
                 N, " output columns");
 }
 
-Tensor linear_int8_rows(const Tensor& x, const Tensor& W, const Tensor& scale, const Tensor& ssi, const Tensor& eo, const LinearCfg& c)
+Tensor linear_int8_rows(const Tensor& x, const Tensor& W, const Tensor& scale, const Tensor& ssi, const Tensor& eo, const LinearCfg& c, bool sums)
 {
     const int64_t R = ssi.size(0), E = W.size(0), K = W.size(1), N = W.size(2);
-    Tensor y = at::empty({R, N}, x.options());
+    Tensor y = at::empty({R, N}, x.options().dtype(rows_type(x.scalar_type(), sums)));
     if (R == 0 || N == 0) return y;
     const int8_t* w = (const int8_t*)ptr(W);
     Tensor ws = bytes_on(x, moe_linear_int8_workspace_bytes(w, W.stride(0), W.stride(1), W.stride(2), x.size(0), R, (int)E, K, N));
-    check(moe_linear_int8_fwd(ptr(x), x.stride(0), x.size(0), dtype_code(x), w, W.stride(0), W.stride(1), W.stride(2), (const float*)ptr(scale), ptr(y), y.stride(0),
+    check(moe_linear_int8_fwd(ptr(x), x.stride(0), x.size(0), dtype_code(x), w, W.stride(0), W.stride(1), W.stride(2), (const float*)ptr(scale), ptr(y), y.stride(0), dtype_code(y),
                               ptr(ssi), is64(ssi), ptr(eo), is64(eo), (int)E, R, K, N, (int)c.k, c.grouped_in, c.grouped_out, ptr(ws), (size_t)ws.numel(), stream_of(x)),
           "moe_linear_int8_fwd");
     return y;
@@ -61,16 +80,16 @@ Tensor linear_int8_rows(const Tensor& x, const Tensor& W, const Tensor& scale, c
 
 // rows of dx, at their flat positions or grouped
 Tensor linear_int8_dx_rows(const Tensor& dout, const Tensor& gates, int64_t gate_fan, const Tensor& W, const Tensor& scale, const Tensor& ssi, const Tensor& eo,
-                           bool dy_grouped, bool dx_grouped)
+                           bool dy_grouped, bool dx_grouped, bool sums)
 {
     const int64_t R = ssi.size(0), E = W.size(0), K = W.size(1), N = W.size(2);
-    Tensor dx = at::empty({R, K}, dout.options());
+    Tensor dx = at::empty({R, K}, dout.options().dtype(rows_type(dout.scalar_type(), sums)));
     if (R == 0) return dx;
     if (N == 0) return dx.zero_();
     const int8_t* w = (const int8_t*)ptr(W);
     Tensor ws = bytes_on(dout, moe_linear_int8_workspace_bytes(w, W.stride(0), W.stride(2), W.stride(1), R, R, (int)E, N, K));
     check(moe_linear_int8_bwd(ptr(dout), dout.stride(0), dtype_code(dout), dy_grouped, (int)gate_fan, ptr(gates), gates.defined() ? dtype_code(gates) : 0, w,
-                              W.stride(0), W.stride(1), W.stride(2), (const float*)ptr(scale), ptr(dx), dx.stride(0), dx_grouped, ptr(ssi), is64(ssi), ptr(eo), is64(eo),
+                              W.stride(0), W.stride(1), W.stride(2), (const float*)ptr(scale), ptr(dx), dx.stride(0), dtype_code(dx), dx_grouped, ptr(ssi), is64(ssi), ptr(eo), is64(eo),
                               (int)E, R, K, N, ptr(ws), (size_t)ws.numel(), stream_of(dout)), "moe_linear_int8_bwd");
     return dx;
 }
@@ -80,10 +99,10 @@ struct LinearI8Fn : Function<LinearI8Fn> {
                           const LinearCfg& c)
     {
         const Tensor gates = val(gates_);
-        Tensor y = linear_int8_rows(x, W, scale, ssi, eo, c), y_rows;
+        Tensor y = linear_int8_rows(x, W, scale, ssi, eo, c, gates.defined()), y_rows;
         if (gates.defined()) {
             y_rows = y;
-            y = combine(y_rows, gates, nullptr, gates.size(1), gates.size(0));
+            y = combine_rows(y_rows, gates, gates.size(1), gates.size(0), x.scalar_type());
         }
         ctx->save_for_backward({W, scale, gates, ssi, eo, gates.defined() && gates.requires_grad() ? y_rows : Tensor()});
         ctx->saved_data["k"] = c.k;
@@ -102,11 +121,11 @@ struct LinearI8Fn : Function<LinearI8Fn> {
         int64_t gate_fan = 1;
         if (gates.defined()) {
             gate_fan = gates.size(1);
-            if (ctx->needs_input_grad(1)) d_gates = combine_dgates(y_rows, dout, gate_fan, gates.scalar_type(), nullptr);
+            if (ctx->needs_input_grad(1)) d_gates = combine_rows_dgates(y_rows, dout, gate_fan, gates.scalar_type());
         }
         if (ctx->needs_input_grad(0)) {
-            dx = linear_int8_dx_rows(dout, flat_gates(gates), gate_fan, W, scale, ssi, eo, grouped_out, grouped_in);
-            if (k != 1) dx = combine(dx, Tensor(), nullptr, k, dx.size(0) / k);
+            dx = linear_int8_dx_rows(dout, flat_gates(gates), gate_fan, W, scale, ssi, eo, grouped_out, grouped_in, k != 1);
+            if (k != 1) dx = combine_rows(dx, Tensor(), k, dx.size(0) / k, dout.scalar_type());
         }
         return {dx, d_gates, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
     }
@@ -135,23 +154,23 @@ Tensor linear_int8(const Tensor& x_, const Tensor& W, const Tensor& scale_, int6
     const Tensor gates = gates_.defined() ? gates_.contiguous() : Tensor();
     const LinearCfg c{0.0, 0.0, k, grouped_in, grouped_out};
     if (needs_node({&x, &gates})) return LinearI8Fn::apply(x, opt(gates), W, scale, ssi, eo, c);
-    Tensor y = linear_int8_rows(x, W, scale, ssi, eo, c);
-    return gates.defined() ? combine(y, gates, nullptr, gates.size(1), gates.size(0)) : y;
+    Tensor y = linear_int8_rows(x, W, scale, ssi, eo, c, gates.defined());
+    return gates.defined() ? combine_rows(y, gates, gates.size(1), gates.size(0), x.scalar_type()) : y;
 }
 
 // ---- expert MLP: codes (E, f, d) and scales in the order w1, w2, w3
 struct I8Mlp { Tensor w[3], s[3]; };
 
-Tensor mlp_int8_rows(const Tensor& x, const I8Mlp& m, const MlpCfg& c, const Tensor& ssi, const Tensor& offsets, Tensor* saved)
+Tensor mlp_int8_rows(const Tensor& x, const I8Mlp& m, const MlpCfg& c, const Tensor& ssi, const Tensor& offsets, Tensor* saved, bool sums)
 {
     const int64_t E = m.w[0].size(0), f = m.w[0].size(1), d = m.w[0].size(2), R = ssi.numel();
-    Tensor y = at::empty({R, d}, x.options());
+    Tensor y = at::empty({R, d}, x.options().dtype(rows_type(x.scalar_type(), sums)));
     if (R == 0) return y;
     if (saved) *saved = bytes_on(x, moe_mlp_int8_saved_bytes(R, f));
     Tensor ws = bytes_on(x, moe_mlp_int8_workspace_bytes(R, x.size(0), (int)E, d, f, 0));
     auto q = [&](int i) { return (const int8_t*)ptr(m.w[i]); };
     auto s = [&](int i) { return (const float*)ptr(m.s[i]); };
-    check(moe_mlp_int8_fwd(ptr(x), x.stride(0), x.size(0), dtype_code(x), q(0), s(0), q(2), s(2), q(1), s(1), ptr(y), y.stride(0), ptr(ssi), is64(ssi),
+    check(moe_mlp_int8_fwd(ptr(x), x.stride(0), x.size(0), dtype_code(x), q(0), s(0), q(2), s(2), q(1), s(1), ptr(y), y.stride(0), dtype_code(y), ptr(ssi), is64(ssi),
                            ptr(offsets), is64(offsets), (int)E, R, d, f, (int)c.fan_out, c.y_grouped, saved ? ptr(*saved) : nullptr,
                            saved ? (size_t)saved->numel() : 0, ptr(ws), (size_t)ws.numel(), stream_of(x)), "moe_mlp_int8_fwd");
     return y;
@@ -161,8 +180,8 @@ struct MlpI8Fn : Function<MlpI8Fn> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& gates_, const I8Mlp& m, const Tensor& ssi, const Tensor& offsets, const MlpCfg& c)
     {
         const Tensor gates = val(gates_);
-        Tensor saved, y = mlp_int8_rows(x, m, c, ssi, offsets, &saved);
-        Tensor out = gates.defined() ? combine(y, gates, nullptr, gates.size(1), gates.size(0)) : y;
+        Tensor saved, y = mlp_int8_rows(x, m, c, ssi, offsets, &saved, gates.defined());
+        Tensor out = gates.defined() ? combine_rows(y, gates, gates.size(1), gates.size(0), x.scalar_type()) : y;
         ctx->save_for_backward({m.w[0], m.w[1], m.w[2], m.s[0], m.s[1], m.s[2], gates, ssi, offsets, saved, gates.defined() && gates.requires_grad() ? y : Tensor()});
         ctx->saved_data["fan_out"] = c.fan_out;
         ctx->saved_data["y_grouped"] = c.y_grouped;
@@ -179,19 +198,19 @@ struct MlpI8Fn : Function<MlpI8Fn> {
         int64_t dy_fan = 1;
         if (gates.defined()) {
             dy_fan = gates.size(1);
-            if (ctx->needs_input_grad(1)) d_gates = combine_dgates(y, dout, dy_fan, gates.scalar_type(), nullptr);
+            if (ctx->needs_input_grad(1)) d_gates = combine_rows_dgates(y, dout, dy_fan, gates.scalar_type());
         }
         if (ctx->needs_input_grad(0)) {
-            Tensor rows = at::empty({R, d}, dout.options());
+            Tensor rows = at::empty({R, d}, dout.options().dtype(rows_type(dout.scalar_type(), fan_out != 1)));
             const Tensor coeff = flat_gates(gates);
             Tensor ws = bytes_on(dout, moe_mlp_int8_workspace_bytes(R, R, (int)E, d, f, 1));
             auto q = [&](int i) { return (const int8_t*)ptr(sv[i]); };
             auto s = [&](int i) { return (const float*)ptr(sv[3 + i]); };
             check(moe_mlp_int8_bwd(ptr(dout), dout.stride(0), dtype_code(dout), ctx->saved_data["y_grouped"].toBool(), (int)dy_fan, ptr(coeff),
-                                   gates.defined() ? dtype_code(gates) : 0, q(0), s(0), q(2), s(2), q(1), s(1), ptr(saved), saved.defined() ? (size_t)saved.numel() : 0, ptr(rows), rows.stride(0),
+                                   gates.defined() ? dtype_code(gates) : 0, q(0), s(0), q(2), s(2), q(1), s(1), ptr(saved), saved.defined() ? (size_t)saved.numel() : 0, ptr(rows), rows.stride(0), dtype_code(rows),
                                    ptr(ssi), is64(ssi), ptr(offsets), is64(offsets), (int)E, R, d, f, ptr(ws), (size_t)ws.numel(), stream_of(dout)),
                   "moe_mlp_int8_bwd");
-            dx = fan_out == 1 ? rows : combine(rows, Tensor(), nullptr, fan_out, R / fan_out);
+            dx = fan_out == 1 ? rows : combine_rows(rows, Tensor(), fan_out, R / fan_out, dout.scalar_type());
         }
         return {dx, d_gates, Tensor(), Tensor(), Tensor(), Tensor()};
     }
@@ -235,8 +254,8 @@ Tensor expert_mlp_int8(const Tensor& x_, const Tensor& w1, const Tensor& s1, con
         TORCH_CHECK(ssi.numel() == x.size(0) * fan_out, "gradients need one position for each of the ", x.size(0) * fan_out, " assignments, got ", ssi.numel());
         return MlpI8Fn::apply(x, opt(gates), m, ssi, offsets, c);
     }
-    Tensor y = mlp_int8_rows(x, m, c, ssi, offsets, nullptr);
-    return gates.defined() ? combine(y, gates, nullptr, gates.size(1), gates.size(0)) : y;
+    Tensor y = mlp_int8_rows(x, m, c, ssi, offsets, nullptr, gates.defined());
+    return gates.defined() ? combine_rows(y, gates, gates.size(1), gates.size(0), x.scalar_type()) : y;
 }
 
 // router -> sort -> expert MLP over 8-bit weights -> weighted combine; returns as layer()
