@@ -112,8 +112,9 @@ struct LinearI8Fn : Function<LinearI8Fn> {
     static variable_list backward(AutogradContext* ctx, variable_list g)
     {
         const auto sv = ctx->get_saved_variables();
-        const Tensor &W = sv[0], &scale = sv[1], &gates = sv[2], &ssi = sv[3], &eo = sv[4], &y_rows = sv[5];
+        const Tensor &W = sv[0], &gates = sv[2];
         const c10::DeviceGuard guard(W.device());
+        const Tensor scale = sv[1].contiguous(), ssi = sv[3].contiguous(), eo = sv[4].contiguous();   // (a saved-tensor hook may hand back other strides)
         const int64_t k = ctx->saved_data["k"].toInt(), flags = ctx->saved_data["flags"].toInt();
         const bool grouped_in = flags & 1, grouped_out = flags & 2;
         const Tensor dout = g[0].contiguous();
@@ -121,7 +122,7 @@ struct LinearI8Fn : Function<LinearI8Fn> {
         int64_t gate_fan = 1;
         if (gates.defined()) {
             gate_fan = gates.size(1);
-            if (ctx->needs_input_grad(1)) d_gates = combine_rows_dgates(y_rows, dout, gate_fan, gates.scalar_type());
+            if (ctx->needs_input_grad(1)) d_gates = combine_rows_dgates(sv[5].contiguous(), dout, gate_fan, gates.scalar_type());
         }
         if (ctx->needs_input_grad(0)) {
             dx = linear_int8_dx_rows(dout, flat_gates(gates), gate_fan, W, scale, ssi, eo, grouped_out, grouped_in, k != 1);
@@ -190,22 +191,25 @@ struct MlpI8Fn : Function<MlpI8Fn> {
     static variable_list backward(AutogradContext* ctx, variable_list g)
     {
         const auto sv = ctx->get_saved_variables();
-        const Tensor &gates = sv[6], &ssi = sv[7], &offsets = sv[8], &saved = sv[9], &y = sv[10];
+        const Tensor& gates = sv[6];
         const c10::DeviceGuard guard(sv[0].device());
+        Tensor m[6];   // (a saved-tensor hook may hand back other strides)
+        for (int i = 0; i < 6; ++i) m[i] = sv[i].contiguous();
+        const Tensor ssi = sv[7].contiguous(), offsets = sv[8].contiguous(), saved = sv[9].defined() ? sv[9].contiguous() : Tensor();
         const int64_t fan_out = ctx->saved_data["fan_out"].toInt(), E = sv[0].size(0), f = sv[0].size(1), d = sv[0].size(2), R = ssi.numel();
         const Tensor dout = g[0].contiguous();
         Tensor dx, d_gates;
         int64_t dy_fan = 1;
         if (gates.defined()) {
             dy_fan = gates.size(1);
-            if (ctx->needs_input_grad(1)) d_gates = combine_rows_dgates(y, dout, dy_fan, gates.scalar_type());
+            if (ctx->needs_input_grad(1)) d_gates = combine_rows_dgates(sv[10].contiguous(), dout, dy_fan, gates.scalar_type());
         }
         if (ctx->needs_input_grad(0)) {
             Tensor rows = at::empty({R, d}, dout.options().dtype(rows_type(dout.scalar_type(), fan_out != 1)));
             const Tensor coeff = flat_gates(gates);
             Tensor ws = bytes_on(dout, moe_mlp_int8_workspace_bytes(R, R, (int)E, d, f, 1));
-            auto q = [&](int i) { return (const int8_t*)ptr(sv[i]); };
-            auto s = [&](int i) { return (const float*)ptr(sv[3 + i]); };
+            auto q = [&](int i) { return (const int8_t*)ptr(m[i]); };
+            auto s = [&](int i) { return (const float*)ptr(m[3 + i]); };
             check(moe_mlp_int8_bwd(ptr(dout), dout.stride(0), dtype_code(dout), ctx->saved_data["y_grouped"].toBool(), (int)dy_fan, ptr(coeff),
                                    gates.defined() ? dtype_code(gates) : 0, q(0), s(0), q(2), s(2), q(1), s(1), ptr(saved), saved.defined() ? (size_t)saved.numel() : 0, ptr(rows), rows.stride(0), dtype_code(rows),
                                    ptr(ssi), is64(ssi), ptr(offsets), is64(offsets), (int)E, R, d, f, ptr(ws), (size_t)ws.numel(), stream_of(dout)),

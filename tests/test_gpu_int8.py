@@ -138,19 +138,19 @@ def linear_case(dev, dtype, T, K, N, E, k, layout="nk", gates=False, grouped_in=
     assert y.dtype == dtype
     h, tiny = half_step(dtype), torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
     if gates:
-        # rows rounded to the type, then (k products and k - 1 sums in fp32) and rounded again
-        close(y, want["y"], want["y_terms"] * (h + F32_STEPS + 2 * k * 2.0 ** -24) * 1.01 + want["y"].abs() * h * 1.01 + k * tiny, "y")
+        # fp32 rows, k products and k - 1 sums in fp32, one rounding
+        close(y, want["y"], want["y_terms"] * (F32_STEPS + 2 * k * 2.0 ** -24) * 1.01 + want["y"].abs() * h * 1.01 + k * tiny, "y")
     else:
         close(y, want["y"], want["y"].abs() * (h + F32_STEPS) * 1.01 + tiny, "y")
     if not train:
         return
     y.backward(dout.to(dev))
-    slack = want["dx_slack"] + want["dx_terms"] * ((h if k > 1 else 0.0) + F32_STEPS + k * 2.0 ** -24) * 1.01 + (want["dx"].abs() + want["dx_slack"]) * h * 1.01 + k * tiny
+    slack = want["dx_slack"] + want["dx_terms"] * (F32_STEPS + k * 2.0 ** -24) * 1.01 + (want["dx"].abs() + want["dx_slack"]) * h * 1.01 + k * tiny
     close(xd.grad, want["dx"], slack, "dx")
     if gates:
         assert gd.grad.dtype == dtype
         # fp32 products and sums of N terms (in any order: at most N + 1 roundings of what they come to)
-        close(gd.grad, want["d_gates"], want["d_gates_terms"] * (h + F32_STEPS + (N + 1) * 2.0 ** -24) * 1.01 + want["d_gates"].abs() * h * 1.01 + tiny, "d_gates")
+        close(gd.grad, want["d_gates"], want["d_gates_terms"] * (F32_STEPS + (N + 1) * 2.0 ** -24) * 1.01 + want["d_gates"].abs() * h * 1.01 + tiny, "d_gates")
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
@@ -282,18 +282,18 @@ def mlp_case(dev, dtype, T, d, f, E, k, gates=True, grouped_out=False, train=Tru
     assert y.dtype == dtype
     h, tiny = half_step(dtype), torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
     terms = want.get("y_terms", want["y"].abs())
-    rounding = terms * ((h if gates else 0.0) + F32_STEPS + 2.0 ** -20 + 2 * k * 2.0 ** -24) + want["y"].abs() * h
+    rounding = terms * (F32_STEPS + 2.0 ** -20 + 2 * k * 2.0 ** -24) + want["y"].abs() * h
     close(y, want["y"], want["y_slack"] * 1.01 + (rounding + want["y_slack"] * h) * 1.02 + (k + 1) * tiny, "y")
     if not train:
         return
     y.backward(dout.to(dev))
-    # Gradients: rows rounded to the type (half a step) and summed (half a step), and of the codes of dgate and dup, whose values are as exact as h, at most
+    # Gradients: one rounding to the type (half a step), and of the codes of dgate and dup, whose values are as exact as h, at most
     # 2 * 127 * 2^-18 round the other way: each moves its value by a step of at most 8 / 127 of the row's size (the largest of 2 f normal products
     # is below 12 of it for f <= 2^12, and all but 2 % of rows below 8).
     flips = (2 * 127 * 2.0 ** -18) ** 0.5 * 12 / 127
-    assert norm_rel(xd.grad, want["dx"]) <= 2 * h + flips, norm_rel(xd.grad, want["dx"])
+    assert norm_rel(xd.grad, want["dx"]) <= h + flips, norm_rel(xd.grad, want["dx"])
     if gates:
-        assert norm_rel(gd.grad, want["d_gates"]) <= 2 * h + (2 * near) ** 0.5 * 12 / 127
+        assert norm_rel(gd.grad, want["d_gates"]) <= h + (2 * near) ** 0.5 * 12 / 127
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
@@ -311,3 +311,275 @@ def test_mlp_rows_without_gates(dev, grouped_out):
 @pytest.mark.parametrize("T,E,absent", [(300, 16, tuple(range(2, 16))), (64, 80, ()), (7, 3, (1,)), (1000, 1, ())])
 def test_mlp_of_uneven_groups(dev, T, E, absent):
     mlp_case(dev, BF16, T, 128, 256, E, min(2, E - len(absent)), absent=absent)
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# sizes that take the large tiles, parts of tiles, and addresses past 32 bits
+# ---------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("layout", ["nk", "kn"])
+@pytest.mark.parametrize("dtype,T,K,N,E,k,gates", [(BF16, 3000, 1088, 2304, 4, 2, True), (F32, 2100, 512, 2048, 2, 2, False), (F16, 1300, 2000, 1000, 1, 1, False),
+                                                   (BF16, 40, 4096, 300, 2, 2, True), (BF16, 3, 8192, 512, 4, 1, False), (F32, 20, 5000, 130, 1, 1, False)])
+def test_linear_of_many_rows_and_of_long_sums(dev, dtype, T, K, N, E, k, gates, layout):
+    linear_case(dev, dtype, T, K, N, E, k, layout, gates=gates)
+
+
+@pytest.mark.parametrize("T,d,f,E,k", [(2500, 512, 2048, 4, 2), (1400, 1088, 1216, 2, 1), (2, 4096, 1024, 4, 2), (30, 2048, 2112, 2, 1)])
+def test_mlp_of_many_rows_and_of_long_sums(dev, T, d, f, E, k):
+    mlp_case(dev, BF16, T, d, f, E, k)
+
+
+def test_outputs_past_two_to_the_31_elements(dev):
+    """Rows of an output of 2.3e9 elements lie where they should, at both ends."""
+    T, K, N, E = 160000, 64, 14336, 2
+    g = torch.Generator(device=dev).manual_seed(0)
+    x = torch.randn(T, K, generator=g, device=dev).to(BF16)
+    w = torch.randint(-127, 128, (E, N, K), generator=g, device=dev, dtype=torch.int8).transpose(1, 2)
+    ws = torch.rand(E, N, generator=g, device=dev) * 1e-3
+    idx = torch.randint(0, E, (T,), generator=g, device=dev)
+    sei, ssi = idx.sort(stable=True)
+    y = moe.parallel_linear_int8(x, w, ws, 1, sei, ssi, None, None)
+    for t in (0, 1, 74898, 74899, 149796, T - 2, T - 1):
+        c, s, _ = oracle.codes(x[t:t + 1].cpu())
+        e = int(idx[t])
+        want = (c @ w[e].cpu().double()) * s.float().double() * ws[e].cpu().double()
+        close(y[t:t + 1], want, want.abs() * (half_step(BF16) + F32_STEPS) * 1.01 + 1e-30, f"row {t}")
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# what does not depend on the rest of a batch, on the stream, on the call
+# ---------------------------------------------------------------------------------------------------------------
+def setup_mlp(dev, T, d=512, f=1024, E=8, k=2, dtype=BF16, seed=0):
+    sei, ssi, eo, gw = oracle.route(T, E, k, seed)
+    w = moe.Int8ExpertWeights(*(t.to(dev) for t in mlp_weights(E, d, f, seed)))
+    x = torch.randn(T, d, generator=torch.Generator().manual_seed(seed)).to(dtype)
+    return x.to(dev), w, ssi.to(dev), eo.to(dev), gw.to(dtype).to(dev)
+
+
+def test_a_token_has_the_same_result_in_any_batch(dev):
+    """Sums are exact and everything else is per row, so tiles, K parts and the other tokens change no bit."""
+    T, E, k = 900, 8, 2
+    x, w, ssi, eo, gates = setup_mlp(dev, T, d=1024, f=2048)
+    idx = torch.empty(T * k, dtype=torch.int64, device=dev)
+    idx[ssi] = torch.repeat_interleave(torch.arange(E, device=dev), torch.diff(eo, prepend=eo.new_zeros(1)))
+    whole = moe.fused_expert_mlp_int8(x, w, k, ssi, eo, gates)
+    for lo, hi in ((0, 1), (17, 20), (300, 364), (100, 700)):
+        part = idx.view(T, k)[lo:hi].reshape(-1)
+        sei, pos = part.sort(stable=True)
+        offs = torch.bincount(sei, minlength=E).cumsum(0)
+        got = moe.fused_expert_mlp_int8(x[lo:hi], w, k, pos, offs, gates[lo:hi])
+        assert torch.equal(got, whole[lo:hi]), (lo, hi)
+
+
+def mlp_step(x, w, k, ssi, eo, gates, dout):
+    x, gates = x.detach().requires_grad_(True), gates.detach().requires_grad_(True)
+    y = moe.fused_expert_mlp_int8(x, w, k, ssi, eo, gates)
+    return [y.detach(), *torch.autograd.grad(y, (x, gates), dout)]
+
+
+def test_two_streams_at_once_and_again(dev):
+    cases = [setup_mlp(dev, T, seed=T) for T in (700, 3, 64, 257)]
+    douts = [torch.randn_like(c[0]) for c in cases]
+    want = [mlp_step(c[0], c[1], 2, *c[2:], d) for c, d in zip(cases, douts)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(2):
+        got = []
+        for st, c, d in zip(streams, cases, douts):
+            with torch.cuda.stream(st):
+                got.append(mlp_step(c[0], c[1], 2, *c[2:], d))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+@pytest.mark.parametrize("T", [1, 48, 700])
+def test_calls_capture_into_graphs_that_share_the_device(dev, T):
+    """Two captured calls, replayed in turn between eager ones, give the eager results bit for bit, with new inputs too."""
+    x, w, ssi, eo, gates = setup_mlp(dev, T, d=1024)
+    lw, ls = (t.to(dev) for t in weights(8, 1024, 520, 1, "nk"))
+    sei = torch.repeat_interleave(torch.arange(8, device=dev), torch.diff(eo, prepend=eo.new_zeros(1)), output_size=ssi.numel())
+    calls = [lambda: moe.fused_expert_mlp_int8(x, w, 2, ssi, eo, gates), lambda: moe.parallel_linear_int8(x, lw, ls, 2, sei, ssi, None, eo, gates)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for c in calls:
+            c()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for c in calls:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(c())
+    for trial in range(4):
+        x.copy_(torch.randn(x.shape, generator=torch.Generator().manual_seed(trial)).to(x.dtype))
+        for i in ((0, 1), (1, 0), (0, 0))[trial % 3]:
+            graphs[i].replay()
+            torch.cuda.synchronize()
+            got = outs[i].clone()
+            assert torch.equal(got, calls[i]()), (trial, i)
+
+
+def test_a_training_step_captures_into_a_graph(dev):
+    x, w, ssi, eo, gates = setup_mlp(dev, 600)
+    dout = torch.randn_like(x)
+    leaves = [x.requires_grad_(True), gates.requires_grad_(True)]
+
+    def step():
+        for t in leaves:
+            t.grad = None
+        moe.fused_expert_mlp_int8(x, w, 2, ssi, eo, gates).backward(dout)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    captured = [t.grad for t in leaves]
+    for trial in range(3):
+        with torch.no_grad():
+            x.copy_(torch.randn(x.shape, generator=torch.Generator().manual_seed(trial)).to(x.dtype))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [g.clone() for g in captured]
+        step()
+        assert all(torch.equal(a, t.grad) for a, t in zip(got, leaves)), trial
+
+
+def test_backward_runs_again_and_for_either_input_alone(dev):
+    x, w, ssi, eo, gates = setup_mlp(dev, 130)
+    sei = torch.repeat_interleave(torch.arange(8, device=dev), torch.diff(eo, prepend=eo.new_zeros(1)))
+    lw, ls = (t.to(dev) for t in weights(8, 512, 200, 1, "kn"))
+    for call in (lambda a, b: moe.fused_expert_mlp_int8(a, w, 2, ssi, eo, b), lambda a, b: moe.parallel_linear_int8(a, lw, ls, 2, sei, ssi, None, eo, b)):
+        a, b = x.detach().requires_grad_(True), gates.detach().requires_grad_(True)
+        y = call(a, b)
+        dout = torch.randn_like(y)
+        want = torch.autograd.grad(y, (a, b), dout, retain_graph=True)
+        again = torch.autograd.grad(y, (a, b), dout)
+        assert all(torch.equal(u, v) for u, v in zip(want, again))
+        assert torch.equal(torch.autograd.grad(call(a, gates), a, dout)[0], want[0])
+        assert torch.equal(torch.autograd.grad(call(x, b), b, dout)[0], want[1])
+        assert torch.equal(call(x, gates), y) and not call(x, gates).requires_grad
+        # gradients that are not contiguous, or broadcast
+        odd = dout.t().contiguous().t()
+        assert torch.equal(torch.autograd.grad(call(a, b), a, odd)[0], want[0])
+        ones = torch.autograd.grad(call(a, b).sum(), a)[0]
+        assert torch.equal(ones, torch.autograd.grad(call(a, b), a, torch.ones_like(dout))[0])
+
+
+def test_among_the_tools_of_autograd(dev):
+    import torch.autograd.forward_ad as fwad
+    from torch.utils.checkpoint import checkpoint
+    x, w, ssi, eo, gates = setup_mlp(dev, 90)
+    call = lambda v: moe.fused_expert_mlp_int8(v, w, 2, ssi, eo, gates)   # noqa: E731
+    dout = torch.randn_like(x)
+
+    def grad_of(f):
+        v = x.detach().requires_grad_(True)
+        return torch.autograd.grad(f(v), v, dout)[0] if f is call else (f(v).backward(dout), v.grad)[1]
+    want = grad_of(call)
+    for reentrant in (False, True):
+        assert torch.equal(grad_of(lambda v: checkpoint(call, v, use_reentrant=reentrant)), want)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.to(dev)):
+        assert torch.equal(grad_of(lambda v: call(v)), want)
+    traced = torch.jit.trace(call, (x,), check_trace=False)
+    other = torch.randn_like(x)
+    assert torch.equal(traced(other), call(other))
+    with fwad.dual_level(), pytest.raises(RuntimeError, match="(?i)jvp|forward"):
+        call(fwad.make_dual(x, torch.randn_like(x)))
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# the block and the layer
+# ---------------------------------------------------------------------------------------------------------------
+def make_block(dev, dtype=BF16, d=256, f=512, E=8, **kw):
+    torch.manual_seed(0)
+    return moe.ScatterMoEBlock(d, f, E, dtype=dtype, device=dev, **kw)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_a_quantised_block_is_the_operators_one_after_the_other(dev, dtype):
+    block = make_block(dev, dtype)
+    stored = {n: getattr(block, n).detach().clone().view(8, 512, 256) for n in ("w1", "w2", "w3")}
+    assert block.quantize_experts() is block and block.is_quantized and block.quantize_experts() is block
+    assert sorted(n for n, _ in block.named_parameters()) == ["router"]
+    weights_ = moe.Int8ExpertWeights.quantize(stored["w1"], stored["w2"], stored["w3"])
+    for n, t in weights_._asdict().items():
+        assert torch.equal(getattr(block, n), t), n
+    x = torch.randn(3, 50, 256, device=dev).to(dtype)
+    with torch.no_grad():
+        hidden, none = block(x)
+        flat = x.view(-1, 256)
+        out, ew, ei = moe.moe_layer_forward_int8(flat, block.router, weights_)
+        assert none is None and torch.equal(hidden.view(-1, 256), out)
+        _, rw, ri = moe.forward_router(flat, block.router, 2)
+        assert torch.equal(ei.long(), ri) and torch.equal(ew, rw)
+        sei, ssi = moe.flatten_and_sort(ri, 8)
+        eo = torch.bincount(sei, minlength=8).cumsum(0)
+        assert torch.equal(moe.fused_expert_mlp_int8(flat, weights_, 2, ssi, eo, rw), out)
+        # three projections and torch's SwiGLU: the same up to the fp32 roundings of h, which a code or two may show
+        g1, u1 = (moe.parallel_linear_int8(flat.float(), getattr(weights_, n).transpose(1, 2), getattr(weights_, n + "_scale"), 2, sei, ssi, None, eo, grouped_out=True)
+                  for n in ("w1", "w3"))
+        h = torch.nn.functional.silu(g1) * u1
+        y = moe.parallel_linear_int8(h, weights_.w2, weights_.w2_scale, 1, sei, ssi, None, eo, gates=None, grouped_in=True)
+        ref = (y.view(-1, 2, 256) * rw.unsqueeze(-1)).sum(1)
+        assert norm_rel(out, ref.double().cpu()) <= half_step(dtype) + (2 * 127 * 2.0 ** -19) ** 0.5 * 12 / 127
+
+
+def test_a_quantised_block_learns_what_lies_around_it(dev):
+    """Gradients of the hidden states and the router against those of the definition's parts: experts by the oracle, the router by autograd."""
+    block = make_block(dev).quantize_experts()
+    x = torch.randn(70, 256, device=dev).to(BF16).requires_grad_(True)
+    dout = torch.randn(70, 256, device=dev).to(BF16)
+    block(x)[0].backward(dout)
+    xr = x.detach().cpu().double().requires_grad_(True)
+    wr = block.router.detach().cpu().double().requires_grad_(True)
+    w, idx = torch.softmax(xr @ wr.t(), -1).topk(2, -1)
+    w = w / w.sum(-1, keepdim=True)
+    sei, ssi = idx.reshape(-1).sort(stable=True)
+    parts = [getattr(block, n).cpu() for n in moe.Int8ExpertWeights._fields]
+    want = oracle.mlp(x.detach().cpu(), parts, 2, sei, ssi, w.detach(), dout.cpu())
+    (w * want["d_gates"]).sum().backward()
+    flips = (2 * 127 * 2.0 ** -18) ** 0.5 * 12 / 127
+    assert norm_rel(x.grad, want["dx"] + xr.grad) <= 2 * half_step(BF16) + flips     # (two gradients, each rounded, and their sum)
+    # weights of the router come from fp32 logits of bf16 values: 2^-20 of the largest; d_gates carries the flips of h
+    assert norm_rel(block.router.grad, wr.grad) <= half_step(BF16) + 2 * flips
+
+
+def test_a_quantised_block_loads_what_it_saved(dev):
+    a, b = make_block(dev).quantize_experts(), make_block(dev, E=8).quantize_experts()
+    with torch.no_grad():
+        b.router.zero_()
+        b.w1.zero_()
+    b.load_state_dict(a.state_dict())
+    x = torch.randn(9, 256, device=dev).to(BF16)
+    with torch.no_grad():
+        assert torch.equal(a(x)[0], b(x)[0])
+        empty, _ = a(x[:0])
+        assert empty.shape == (0, 256)
+        biased = make_block(dev, bias=True, return_bias=True).quantize_experts()
+        out, bias = biased(x)
+        assert bias is biased.bias and out.shape == x.shape
+    with pytest.raises(ValueError, match="adapters"):
+        make_block(dev, lora_r=16).quantize_experts()
+    with pytest.raises((RuntimeError, TypeError), match="float32"):
+        a.to(BF16)(x)                                          # its scales would be bf16
+
+
+def test_adapters_beside_quantised_weights(dev):
+    """A frozen projection in 8 bits and a trained low-rank one beside it: the sum of two calls, with the gradients of both."""
+    T, K, N, E, k, r = 300, 256, 384, 4, 2, 16
+    sei, ssi, eo, gates = (t.to(dev) for t in oracle.route(T, E, k, 1))
+    w, ws = (t.to(dev) for t in weights(E, K, N, 3, "nk"))
+    g = torch.Generator().manual_seed(4)
+    mk = lambda *s: (torch.randn(*s, generator=g) * 0.1).to(BF16).to(dev).requires_grad_(True)   # noqa: E731
+    x, a, b, dout = mk(T, K), mk(E, K, r), mk(E, r, N), mk(T * k, N).detach()
+    base = moe.parallel_linear_int8(x, w, ws, k, sei, ssi, None, eo)
+    low = moe.parallel_linear(moe.parallel_linear(x, a, k, sei, ssi, None, eo, grouped_out=True), b, 1, sei, ssi, None, eo, grouped_in=True)
+    (base + low).backward(dout)
+    parts = [torch.autograd.grad(moe.parallel_linear_int8(x, w, ws, k, sei, ssi, None, eo), x, dout)[0]]
+    low = moe.parallel_linear(moe.parallel_linear(x, a, k, sei, ssi, None, eo, grouped_out=True), b, 1, sei, ssi, None, eo, grouped_in=True)
+    parts += torch.autograd.grad(low, (x, a, b), dout)
+    assert torch.equal(x.grad, parts[0] + parts[1]) and torch.equal(a.grad, parts[2]) and torch.equal(b.grad, parts[3])
