@@ -239,12 +239,12 @@ Tensor expert_mlp_int8(const Tensor& x_, const Tensor& w1, const Tensor& s1, con
     const Tensor gates_ = val(gates_in);
     require_gpu({&x_, &w1, &s1, &w2, &s2, &w3, &s3, &ssi_, &offsets_, &gates_});
     const c10::DeviceGuard guard(x_.device());
+    const I8Mlp m = take_mlp_int8(w1, s1, w2, s2, w3, s3);
     check_gates(gates_, ssi_.numel());
     if (gates_.defined()) dtype_code(gates_);
-    check_offsets(offsets_, w1.dim() ? w1.size(0) : 0);
+    check_offsets(offsets_, w1.size(0));
     is64(ssi_);
     is64(offsets_);
-    const I8Mlp m = take_mlp_int8(w1, s1, w2, s2, w3, s3);
     TORCH_CHECK(x_.dim() == 2 && x_.size(1) == w1.size(2), "rows of ", x_.sizes(), " do not fit expert weights of ", w1.sizes());
     TORCH_CHECK_TYPE(x_.scalar_type() == at::kBFloat16 || x_.scalar_type() == at::kHalf, "fused_expert_mlp_int8 takes bf16 or fp16 rows, got ", x_.scalar_type(),
                      "; use parallel_linear_int8 for others");

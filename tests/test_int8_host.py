@@ -1,0 +1,202 @@
+"""The expert products over 8-bit weights on the host: what their entry points refuse before anything is enqueued (tensors are fakes that only claim to
+lie on a GPU), what the C entries refuse, and the 64-bit oracle against closed forms."""
+import warnings
+
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+from oracle import int8_oracle as oracle
+
+T, K, N, E, k = 24, 64, 128, 4, 2
+BF16, F32, I8, I32 = torch.bfloat16, torch.float32, torch.int8, torch.int32
+_MODE = FakeTensorMode(allow_non_fake_inputs=True)
+on_host = pytest.mark.skipif(torch.cuda.is_available(), reason="a fake's pointer must not reach a kernel")
+
+
+def _fake(*shape, dtype=BF16, device="cuda:0"):
+    with _MODE:
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
+def _refused(match, fn, *args, **kw):
+    with warnings.catch_warnings():
+        warnings.simplefilter("ignore")   # (a fake's data pointer)
+        with pytest.raises((RuntimeError, AssertionError, TypeError), match=match):
+            fn(*args, **kw)
+
+
+def _linear(**changed):
+    import moe_distributed_training_amd as moe
+    args = dict(inputs=_fake(T, K), expert_weights=_fake(E, K, N, dtype=I8), weight_scales=_fake(E, N, dtype=F32), k=k, sorted_expert_idxs=_fake(T * k, dtype=I32),
+                sorted_scattered_idxs=_fake(T * k, dtype=I32), padded_block_idxs=None, expert_offsets=_fake(E, dtype=I32))
+    return moe.parallel_linear_int8, {**args, **changed}
+
+
+def _weights(**changed):
+    import moe_distributed_training_amd as moe
+    d, f = K, N
+    w = dict(w1=_fake(E, f, d, dtype=I8), w1_scale=_fake(E, f, dtype=F32), w2=_fake(E, f, d, dtype=I8), w2_scale=_fake(E, d, dtype=F32),
+             w3=_fake(E, f, d, dtype=I8), w3_scale=_fake(E, f, dtype=F32))
+    return moe.Int8ExpertWeights(**{**w, **changed})
+
+
+def _mlp(weights=None, **changed):
+    import moe_distributed_training_amd as moe
+    args = dict(x=_fake(T, K), weights=weights or _weights(), k=k, sorted_scattered_idxs=_fake(T * k, dtype=I32), expert_offsets=_fake(E, dtype=I32))
+    return moe.fused_expert_mlp_int8, {**args, **changed}
+
+
+ELSEWHERE = [("GPU only", "cpu"), ("same device", "cuda:1")]
+
+
+@on_host
+@pytest.mark.parametrize("match,device", ELSEWHERE)
+@pytest.mark.parametrize("name,shape,dtype", [("expert_weights", (E, K, N), I8), ("weight_scales", (E, N), F32), ("sorted_expert_idxs", (T * k,), I32),
+                                              ("sorted_scattered_idxs", (T * k,), I32), ("expert_offsets", (E,), I32), ("gates", (T, k), F32)])
+def test_projection_tensors_elsewhere(match, device, name, shape, dtype):
+    fn, args = _linear(**{name: _fake(*shape, dtype=dtype, device=device)})
+    _refused(match, fn, **args)
+
+
+@on_host
+@pytest.mark.parametrize("match,changed", [
+    ("inner dims", dict(inputs=_fake(T, K + 1))), ("inner dims", dict(inputs=_fake(T, K, 1))), ("inner dims", dict(expert_weights=_fake(K, N, dtype=I8))),
+    ("int8", dict(expert_weights=_fake(E, K, N))), ("float32", dict(weight_scales=_fake(E, N))), ("output columns", dict(weight_scales=_fake(E, K, dtype=F32))),
+    ("output columns", dict(weight_scales=_fake(E * N, dtype=F32))), ("unsupported dtype", dict(inputs=_fake(T, K, dtype=torch.float64))),
+    ("unsupported dtype", dict(inputs=_fake(T, K, dtype=I8))), ("assignments", dict(k=3)), ("assignments", dict(k=0)), ("length", dict(sorted_expert_idxs=_fake(T, dtype=I32))),
+    ("k is 1", dict(grouped_in=True)), ("cover", dict(expert_offsets=_fake(E - 1, dtype=I32))), ("int32 or int64", dict(expert_offsets=_fake(E, dtype=F32))),
+    ("int32 or int64", dict(sorted_scattered_idxs=_fake(T * k, dtype=torch.int16))), ("gates of", dict(gates=_fake(T * k, dtype=F32))),
+    ("gates of", dict(gates=_fake(T, k + 1, dtype=F32))), ("grouped output", dict(gates=_fake(T, k, dtype=F32), grouped_out=True)),
+    ("unsupported dtype", dict(gates=_fake(T, k, dtype=torch.float64)))])
+def test_projection_arguments(match, changed):
+    fn, args = _linear(**changed)
+    _refused(match, fn, **args)
+
+
+@on_host
+@pytest.mark.parametrize("match,device", ELSEWHERE)
+@pytest.mark.parametrize("name", ["w1", "w2", "w3", "w1_scale", "w2_scale", "w3_scale"])
+def test_mlp_weights_elsewhere(match, device, name):
+    t = getattr(_weights(), name)
+    fn, args = _mlp(_weights(**{name: _fake(*t.shape, dtype=t.dtype, device=device)}))
+    _refused(match, fn, **args)
+
+
+@on_host
+@pytest.mark.parametrize("match,weights,changed", [
+    ("do not fit", dict(w2=_fake(E, N + 64, K, dtype=I8)), {}), ("do not fit", dict(w3=_fake(E + 1, N, K, dtype=I8)), {}), ("int8", dict(w1=_fake(E, N, K)), {}),
+    ("float32", dict(w2_scale=_fake(E, K)), {}), ("output columns", dict(w2_scale=_fake(E, N, dtype=F32)), {}), ("hidden size", dict(w1=_fake(E * N, K, dtype=I8)), {}),
+    ("bf16 or fp16", {}, dict(x=_fake(T, K, dtype=F32))), ("do not fit", {}, dict(x=_fake(T, K + 64))), ("do not fit", {}, dict(k=1)), ("do not fit", {}, dict(k=0)),
+    ("cover", {}, dict(expert_offsets=_fake(E - 1, dtype=I32))), ("int32 or int64", {}, dict(sorted_scattered_idxs=_fake(T * k, dtype=F32))),
+    ("gates of", {}, dict(gates=_fake(k, T, 1, dtype=F32)))])
+def test_mlp_arguments(match, weights, changed):
+    fn, args = _mlp(_weights(**weights), **changed)
+    _refused(match, fn, **args)
+
+
+@on_host
+def test_mlp_sizes_and_layouts():
+    d, f = 96, 128
+    w = _weights(w1=_fake(E, f, d, dtype=I8), w2=_fake(E, f, d, dtype=I8), w3=_fake(E, f, d, dtype=I8), w2_scale=_fake(E, d, dtype=F32))
+    fn, args = _mlp(w, x=_fake(T, d))
+    _refused("multiples of 64", fn, **args)
+    with _MODE:
+        turned = torch.empty((E, K, N), dtype=I8, device="cuda:0").transpose(1, 2)
+    fn, args = _mlp(_weights(w3=turned))
+    _refused("contiguous", fn, **args)
+
+
+@on_host
+def test_layer_and_quantiser_arguments():
+    import moe_distributed_training_amd as moe
+    _refused("router weight", moe.moe_layer_forward_int8, _fake(T, K), _fake(E + 1, K), _weights())
+    _refused("share a dtype", moe.moe_layer_forward_int8, _fake(T, K), _fake(E, K, dtype=F32), _weights())
+    _refused("rows, columns", moe.quantize_rows, _fake(T, K, 1))
+    _refused("unsupported dtype", moe.quantize_rows, _fake(T, K, dtype=I8))
+    _refused("experts, inputs, outputs", moe.quantize_expert_weights, _fake(T, K))
+    _refused("unsupported dtype", moe.quantize_expert_weights, _fake(E, K, N, dtype=I8))
+    _refused("GPU only", moe.quantize_rows, torch.zeros(2, 3))
+
+
+def test_a_gradient_needs_every_assignment():
+    import moe_distributed_training_amd as moe
+    if torch.cuda.is_available():
+        pytest.skip("a fake's pointer must not reach a kernel")
+    x = _fake(T, K)
+    with _MODE:
+        x.requires_grad_(True)
+    fn, args = _mlp(x=x, sorted_scattered_idxs=_fake(T, dtype=I32))
+    _refused("one position for each", fn, **args)
+    assert moe.fused_expert_mlp_int8 is fn
+
+
+def test_c_entries_refuse_on_the_host():
+    """Status codes before anything is enqueued (16: non-null stand-ins that are never dereferenced)."""
+    from moe_distributed_training_amd._lib import lib
+    q = lib.moe_quantize_rows
+    assert q(16, 64, 3, 16, 128, 16, 4, 64, None) == -1 and q(16, 64, 0, 16, 120, 16, 4, 64, None) == -1 and q(16, 64, 0, 24, 128, 16, 4, 64, None) == -1
+    assert q(None, 64, 0, 16, 128, 16, 4, 64, None) == -1 and q(None, 64, 0, None, 128, None, 0, 64, None) == 0
+    assert lib.moe_quantize_weights(16, 1, 1, 1, 0, 2, 0, 8, 16, 1, 1, 1, 16, 16, 1 << 20, None) == -1
+    assert lib.moe_quantize_weights(16, 1, 1, 1, 0, 2, 8, 8, 16, 1, 1, 1, 16, 16, 8, None) == -3
+
+    def fwd(x=16, ldx=64, rows=8, dt=0, w=16, st=(8192, 1, 64), y=16, ldy=128, ydt=0, pos=16, E=2, R=16, K=64, N=128, fan=2, xg=0, yg=0, ws=16, n=1 << 30):
+        return lib.moe_linear_int8_fwd(x, ldx, rows, dt, w, *st, 16, y, ldy, ydt, pos, 0, 16, 0, E, R, K, N, fan, xg, yg, ws, n, None)
+    assert fwd(x=None) == -1 and fwd(dt=3) == -1 and fwd(ydt=-1) == -1 and fwd(ldx=63) == -1 and fwd(ldy=127) == -1 and fwd(pos=None) == -1 and fwd(E=0) == -1 and fwd(fan=0) == -1
+    assert fwd(xg=1, rows=15) == -1 and fwd(K=131072, ldx=131072, st=(1 << 25, 1, 131072)) == -2 and fwd(n=64) == -3 and fwd(ws=None) == -3 and fwd(R=0, x=None) == 0
+    # gathered rows whose codes do not fit 32-bit offsets, and a matrix that does not
+    assert fwd(rows=1 << 26, R=16, n=1 << 40) == -2
+    assert fwd(K=65536, ldx=65536, N=70000, ldy=70000, st=(65536 * 70000, 1, 65536), n=1 << 40) == -2
+
+    def bwd(dy=16, ldd=128, dt=0, w=16, st=(8192, 1, 64), dx=16, lddx=64, gates=None, gdt=0, pos=16, E=2, R=16, K=64, N=128, ws=16, n=1 << 30):
+        return lib.moe_linear_int8_bwd(dy, ldd, dt, 0, 2, gates, gdt, w, *st, 16, dx, lddx, dt, 0, pos, 0, 16, 0, E, R, K, N, ws, n, None)
+    assert bwd(dy=None) == -1 and bwd(ldd=127) == -1 and bwd(lddx=63) == -1 and bwd(gates=16, gdt=3) == -1 and bwd(pos=None) == -1 and bwd(N=131072, ldd=131072) == -2 and bwd(n=0) == -3
+
+    def mlp(x=16, dt=0, d=64, f=128, R=16, rows=8, saved=None, sn=0, ws=16, n=1 << 30, w=16):
+        return lib.moe_mlp_int8_fwd(x, d, rows, dt, w, 16, 16, 16, 16, 16, 16, d, 0, 16, 0, 16, 0, 2, R, d, f, 2, 0, saved, sn, ws, n, None)
+    assert mlp(x=None) == -1 and mlp(dt=2) == -2 and mlp(d=96) == -2 and mlp(f=100) == -2 and mlp(w=24) == -2 and mlp(saved=16, sn=8) == -3 and mlp(n=0) == -3 and mlp(R=0) == 0
+    assert lib.moe_mlp_int8_saved_bytes(16, 128) == 2 * (16 * 128 * 3 + 256)       # 24 bits a value, a scale for each 32
+    assert lib.moe_combine_f32(16, 64, 16, 64, 0, None, 0, 0, 4, 64, None) == -1 and lib.moe_combine_f32(None, 64, 16, 64, 0, None, 0, 2, 4, 64, None) == -1
+    assert lib.moe_combine_f32_dgates(16, 64, 16, 63, 0, 16, 0, 2, 4, 64, None) == -1 and lib.moe_combine_f32(None, 64, None, 64, 0, None, 0, 2, 0, 64, None) == 0
+
+
+def test_workspaces_cover_what_the_calls_take():
+    from moe_distributed_training_amd._lib import lib
+    in_place = lib.moe_linear_int8_workspace_bytes(16, 64 * 128, 1, 64, 8, 16, 2, 64, 128)
+    copied = lib.moe_linear_int8_workspace_bytes(16, 60 * 128, 1, 60, 8, 16, 2, 60, 128)
+    assert in_place >= 8 * 128 + 8 * 4 and copied - in_place == 2 * 128 * 64        # codes of 8 rows and scales; both matrices at a pitch of 64
+    assert lib.moe_linear_int8_workspace_bytes(16, 1, 1, 1, 0, 16, 2, 64, 128) == 0
+    for bwd in (0, 1):
+        assert lib.moe_mlp_int8_workspace_bytes(16, 8, 2, 64, 96, bwd) == 0 and lib.moe_mlp_int8_workspace_bytes(16, 8, 2, 64, 128, bwd) > 16 * 128
+
+
+# ---- the oracle itself
+def test_oracle_codes_are_the_nearest_levels():
+    g = torch.Generator().manual_seed(0)
+    v = torch.randn(20, 50, generator=g).double()
+    c, s, edge = oracle.codes(v)
+    levels = torch.arange(-127, 128).double()
+    best = (v.unsqueeze(-1) - s.unsqueeze(-1) * levels).abs().min(-1).values
+    assert torch.allclose((v - c * s).abs(), best, atol=1e-12) and not edge.any() and float(c.abs().max()) == 127
+    tie, _, edge = oracle.codes(torch.tensor([[2.0, 1.0, -1.0, 0.0]]), near=1e-6)    # half the maximum: 63.5
+    assert tie.tolist() == [[127, 64, -64, 0]] and edge.tolist() == [[False, True, True, False]]
+
+
+def test_oracle_gradients_are_those_of_the_dequantised_product():
+    """With rows that are codes already (gradient and input), the straight-through gradient is autograd's of the linear map."""
+    g = torch.Generator().manual_seed(1)
+    T_, K_, N_, E_, k_ = 7, 12, 10, 3, 2
+    sei, ssi, _, gates = oracle.route(T_, E_, k_, 0)
+    w = torch.randint(-127, 128, (E_, K_, N_), generator=g).double()
+    ws = torch.ones(E_, N_).double()
+    x = torch.randint(-126, 127, (T_, K_), generator=g).double()
+    x[:, 0] = 127
+    dout = torch.randint(-126, 127, (T_ * k_, N_), generator=g).double()
+    dout[:, 0] = 127
+    got = oracle.linear(x, w, ws, k_, sei, ssi, None, dout)
+    xr = x.clone().requires_grad_(True)
+    expert = torch.empty(T_ * k_, dtype=torch.int64)
+    expert[ssi] = sei
+    y = torch.einsum("tk,tkn->tn", xr.repeat_interleave(k_, 0), w[expert])
+    y.backward(dout)
+    assert torch.allclose(got["y"], y.detach(), rtol=1e-6) and torch.allclose(got["dx"], xr.grad, rtol=1e-12)
