@@ -5,8 +5,7 @@
 // it comes out (ties are common: half the maximum is 63.5 for every row of a 2-byte type), so the codes are the same on every path and in any
 // precision that a checker takes.  q is guessed with one multiplication by 127 / a and put right from its remainder 127 v - q a: 127 v is held as
 // an fp32 number and its rounding error, and the difference with q a is exact (it is a multiple of half a unit of a's last place and at most a / 2; below a / 254 q
-// is 0).  Gradient rows, products of two or three numbers, are held as an fp32 number and its error from the start.  (In fp64 instead, 8192 x 4096
-// gradient rows took 92 us.)  A row that holds an infinity or a NaN gets the scale NaN and codes 0, so that every product of it is NaN and
+// is 0).  fp32 gradient rows, products of two or three numbers, are held as an fp32 number and its error from the start.  A row that holds an infinity or a NaN gets the scale NaN and codes 0, so that every product of it is NaN and
 // no other row changes; a row of zeros the scale 0.
 //
 // Interims (h, the saved gate and up, dh) travel as 24-bit integers with a scale for each 32 columns of a row: 3 bytes per value, at most 2^-24 of the segment's
@@ -182,9 +181,10 @@ __global__ void __launch_bounds__(1024) quantize_rows_kernel(const MoeQuantizeRo
             }
         }
     };
-    // (the maximum of fp32 products is taken with its error too: left out, it moves borders by 127 * 2^-25 of a step, which would show in an fp32 result and
-    // does not in a 2-byte one)
+    // Gradient rows: in a 2-byte result the few codes that fp32 products round the other way do not show (1 in 10^5, a tenth of the result's own rounding); in an fp32
+    // result each would, so there the values, their maximum and the quotient are taken with their errors.  (With errors everywhere 16384 x 2048 bf16 rows took 44 us.)
     constexpr bool WITH_ERROR = SCALED && std::is_same_v<T, float>;
+    constexpr bool EXACT = !SCALED || WITH_ERROR;
     float keep[KEEP ? KEEP : 1][8], low[KEEP ? KEEP : 1][8];
     std::conditional_t<WITH_ERROR, unsigned long long, uint32_t> top = 0;
     auto look = [&](const float* v, const float* lo) {
@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(1024) quantize_rows_kernel(const MoeQuantizeRo
     auto store = [&](int64_t c0, const float* v, const float* lo) {
         float q[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) q[i] = rc.exact(v[i], lo[i]);
+        for (int i = 0; i < 8; ++i) q[i] = EXACT ? rc.exact(v[i], lo[i]) : rc.nearest(v[i]);
         uint2 w;
         w.x = pack4(q[0], q[1], q[2], q[3]);
         w.y = pack4(q[4], q[5], q[6], q[7]);
