@@ -5,8 +5,8 @@
 // it comes out (ties are common: half the maximum is 63.5 for every row of a 2-byte type), so the codes are the same on every path and in any
 // precision that a checker takes.  q is guessed with one multiplication by 127 / a and put right from its remainder 127 v - q a: 127 v is held as
 // an fp32 number and its rounding error, and the difference with q a is exact (it is a multiple of half a unit of a's last place and at most a / 2; below a / 254 q
-// is 0).  fp32 gradient rows, products of two or three numbers, are held as an fp32 number and its error from the start.  A row that holds an infinity or a NaN gets the scale NaN and codes 0, so that every product of it is NaN and
-// no other row changes; a row of zeros the scale 0.
+// is 0).  Gradient rows, products of two or three numbers, are held as an fp32 number and its error from the start (but for bf16, see below).  A row that holds an
+// infinity or a NaN gets the scale NaN and codes 0, so that every product of it is NaN and no other row changes; a row of zeros the scale 0.
 //
 // Interims (h, the saved gate and up, dh) travel as 24-bit integers with a scale for each 32 columns of a row: 3 bytes per value, at most 2^-24 of the segment's
 // maximum off.  Every value that a rounding on the way carries over a border of the 8-bit codes costs a whole step, so this noise falls with the root of
@@ -181,10 +181,11 @@ __global__ void __launch_bounds__(1024) quantize_rows_kernel(const MoeQuantizeRo
             }
         }
     };
-    // Gradient rows: in a 2-byte result the few codes that fp32 products round the other way do not show (1 in 10^5, a tenth of the result's own rounding); in an fp32
-    // result each would, so there the values, their maximum and the quotient are taken with their errors.  (With errors everywhere 16384 x 2048 bf16 rows took 44 us.)
+    // Gradient rows.  The few codes that fp32 products round the other way (1 in 10^5) add 2 to 5e-4 to a result's error: nothing beside bf16's own rounding (1.7e-3), twice
+    // that of fp16, whose values are taken with their errors; fp32 rows take their maximum with its error too, which moves borders by 127 * 2^-25 of a step.
+    // (16384 x 2048 rows: 44 us with errors, 36 without.)
     constexpr bool WITH_ERROR = SCALED && std::is_same_v<T, float>;
-    constexpr bool EXACT = !SCALED || WITH_ERROR;
+    constexpr bool EXACT = !SCALED || !std::is_same_v<T, __hip_bfloat16>;
     float keep[KEEP ? KEEP : 1][8], low[KEEP ? KEEP : 1][8];
     std::conditional_t<WITH_ERROR, unsigned long long, uint32_t> top = 0;
     auto look = [&](const float* v, const float* lo) {
