@@ -404,7 +404,7 @@ __global__ void __launch_bounds__(NTHREADS, 2) i8_gemm_kernel(const MoeI8Gemm p)
                 uint8_t* to = out + at * MOE_SEG_BYTES;
                 *(u32x4_t*)(to + g * 16) = hi;
                 *(uint2*)(to + 64 + g * 8) = lo;
-                if (g == 0) scales[(wrow0 + m) * SEGS + seg] = !fine ? __uint_as_float(0x7fc00000u) : inv > 0.f ? amax * (1.f / MOE_SEG_LEVELS) * row_scale : 0.f;
+                if (g == 0) scales[(wrow0 + m) * SEGS + seg] = !fine ? __uint_as_float(0x7fc00000u) : (inv > 0.f ? amax * (1.f / MOE_SEG_LEVELS) : 0.f) * row_scale;   // (zeros of a row whose scale is NaN are NaN)
             }
         };
         auto xs = [&](int mb) { return s_xscale[wrow0 + mb * 16 + (lane & 15)]; };

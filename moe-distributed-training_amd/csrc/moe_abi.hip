@@ -1064,7 +1064,7 @@ int moe_quantize_rows(const void* src, int64_t lds, int dtype, int8_t* codes, in
 {
     if (dtype < 0 || dtype > 2 || nrows < 0 || ncols < 0 || ldc < ncols || ldc % 16 != 0) return MOE_ERR_BAD_ARG;
     if (nrows == 0) return MOE_OK;
-    if (!src || !codes || !scale || !aligned16(codes)) return MOE_ERR_BAD_ARG;
+    if (lds < 0 || !src || !codes || !scale || !aligned16(codes)) return MOE_ERR_BAD_ARG;
     if (nrows > 0x7fffffff) return MOE_ERR_UNSUPPORTED;
     MoeQuantizeRows q = {};
     q.src = src; q.lds = lds; q.codes = codes; q.ldc = ldc; q.scale = scale; q.cols = ncols;
@@ -1074,9 +1074,9 @@ int moe_quantize_rows(const void* src, int64_t lds, int dtype, int8_t* codes, in
 int moe_combine_f32(const float* y, int64_t ldy, void* out, int64_t ldo, int dtype, const void* gates, int gates_dtype, int k, int64_t ntok, int64_t ncols, void* stream)
 {
     hipStream_t st = S(stream);
-    if (dtype < 0 || dtype > 2 || k < 1 || ntok < 0 || ncols < 0 || ldy < ncols || ldo < ncols || (gates && (gates_dtype < 0 || gates_dtype > 2))) return MOE_ERR_BAD_ARG;
+    if (dtype < 0 || dtype > 2 || k < 1 || ntok < 0 || ncols < 0 || (gates && (gates_dtype < 0 || gates_dtype > 2))) return MOE_ERR_BAD_ARG;
     if (ntok == 0 || ncols == 0) return MOE_OK;
-    if (!y || !out) return MOE_ERR_BAD_ARG;
+    if (ldy < 0 || (ntok > 1 && ldo < ncols) || !y || !out) return MOE_ERR_BAD_ARG;
     if (ntok > 0x7fffffff) return MOE_ERR_UNSUPPORTED;
     TIMED("rows.combine_f32");
     return moe_launch_combine_f32(y, ldy, out, ldo, dtype, gates, gates_dtype, k, ntok, ncols, st);
@@ -1085,9 +1085,9 @@ int moe_combine_f32(const float* y, int64_t ldy, void* out, int64_t ldo, int dty
 int moe_combine_f32_dgates(const float* y, int64_t ldy, const void* dout, int64_t ldd, int dtype, void* dgates, int gates_dtype, int k, int64_t ntok, int64_t ncols, void* stream)
 {
     hipStream_t st = S(stream);
-    if (dtype < 0 || dtype > 2 || gates_dtype < 0 || gates_dtype > 2 || k < 1 || ntok < 0 || ncols < 0 || ldy < ncols || ldd < ncols) return MOE_ERR_BAD_ARG;
+    if (dtype < 0 || dtype > 2 || gates_dtype < 0 || gates_dtype > 2 || k < 1 || ntok < 0 || ncols < 0) return MOE_ERR_BAD_ARG;
     if (ntok == 0) return MOE_OK;
-    if (!y || !dout || !dgates) return MOE_ERR_BAD_ARG;
+    if (ldy < 0 || ldd < 0 || !y || !dout || !dgates) return MOE_ERR_BAD_ARG;
     if (ntok * k > 0x7fffffff) return MOE_ERR_UNSUPPORTED;
     TIMED("rows.combine_f32_dgates");
     return moe_launch_dgates_f32(y, ldy, dout, ldd, dtype, dgates, gates_dtype, k, ntok, ncols, st);
@@ -1158,8 +1158,9 @@ int moe_linear_int8_fwd(const void* x, int64_t ldx, int64_t x_rows, int dtype, c
                         const float* w_scale, void* y, int64_t ldy, int y_dtype, const void* pos, int pos64, const void* offsets, int off64, int E, int64_t R, int64_t K,
                         int64_t N, int fan_out, int x_grouped, int y_grouped, void* workspace, size_t workspace_bytes, void* stream)
 {
-    if (dtype < 0 || dtype > 2 || y_dtype < 0 || y_dtype > 2 || E < 1 || R < 0 || x_rows < 0 || K < 1 || N < 0 || fan_out < 1 || ldx < K || ldy < N) return MOE_ERR_BAD_ARG;
+    if (dtype < 0 || dtype > 2 || y_dtype < 0 || y_dtype > 2 || E < 1 || R < 0 || x_rows < 0 || K < 1 || N < 0 || fan_out < 1) return MOE_ERR_BAD_ARG;
     if (R == 0 || N == 0) return MOE_OK;
+    if (ldx < 0 || (R > 1 && ldy < N)) return MOE_ERR_BAD_ARG;   // (rows of an input may overlap)
     if (!x || x_rows < 1 || !W || !w_scale || !y || !offsets || ((!x_grouped || !y_grouped) && !pos) || (x_grouped && x_rows < R)) return MOE_ERR_BAD_ARG;
     if (K > MOE_I8_MAX_K || E > 65535 || x_rows > 0x7fffffff) return MOE_ERR_UNSUPPORTED;
     const I8Weights w = i8_weights(W, swe, swk, swn, E, K, N);
@@ -1177,8 +1178,9 @@ int moe_linear_int8_bwd(const void* dy, int64_t lddy, int dtype, int dy_grouped,
                         int64_t swe, int64_t swk, int64_t swn, const float* w_scale, void* dx_rows, int64_t lddx, int dx_dtype, int dx_grouped, const void* pos, int pos64,
                         const void* offsets, int off64, int E, int64_t R, int64_t K, int64_t N, void* workspace, size_t workspace_bytes, void* stream)
 {
-    if (dtype < 0 || dtype > 2 || dx_dtype < 0 || dx_dtype > 2 || E < 1 || R < 0 || K < 0 || N < 1 || dy_fan_out < 1 || lddy < N || lddx < K || (gates && (gates_dtype < 0 || gates_dtype > 2))) return MOE_ERR_BAD_ARG;
+    if (dtype < 0 || dtype > 2 || dx_dtype < 0 || dx_dtype > 2 || E < 1 || R < 0 || K < 0 || N < 1 || dy_fan_out < 1 || (gates && (gates_dtype < 0 || gates_dtype > 2))) return MOE_ERR_BAD_ARG;
     if (R == 0 || K == 0) return MOE_OK;
+    if (lddy < 0 || (R > 1 && lddx < K)) return MOE_ERR_BAD_ARG;
     if (!dy || !W || !w_scale || !dx_rows || !offsets || ((!dy_grouped || !dx_grouped) && !pos)) return MOE_ERR_BAD_ARG;
     if (N > MOE_I8_MAX_K || E > 65535 || R > 0x7fffffff) return MOE_ERR_UNSUPPORTED;
     const I8Weights w = i8_weights(W, swe, swn, swk, E, N, K);   // W^T: the contraction runs over N
@@ -1224,8 +1226,9 @@ int moe_mlp_int8_fwd(const void* x, int64_t ldx, int64_t x_rows, int dtype, cons
                      size_t workspace_bytes, void* stream)
 {
     hipStream_t st = S(stream);
-    if (dtype < 0 || dtype > 2 || y_dtype < 0 || y_dtype > 2 || E < 1 || R < 0 || x_rows < 0 || d < 1 || f < 1 || fan_out < 1 || ldx < d || ldy < d) return MOE_ERR_BAD_ARG;
+    if (dtype < 0 || dtype > 2 || y_dtype < 0 || y_dtype > 2 || E < 1 || R < 0 || x_rows < 0 || d < 1 || f < 1 || fan_out < 1) return MOE_ERR_BAD_ARG;
     if (R == 0) return MOE_OK;
+    if (ldx < 0 || (R > 1 && ldy < d)) return MOE_ERR_BAD_ARG;
     if (!x || x_rows < 1 || !w1 || !s1 || !w3 || !s3 || !w2 || !s2 || !y || !pos || !offsets) return MOE_ERR_BAD_ARG;
     if (dtype == MOE_F32 || !i8_mlp_sizes_ok(d, f) || d > MOE_I8_MAX_K || f > MOE_I8_MAX_K || E > 65535 || x_rows > 0x7fffffff || R > 0x7fffffff) return MOE_ERR_UNSUPPORTED;
     if (!aligned16(w1) || !aligned16(w3) || !aligned16(w2)) return MOE_ERR_UNSUPPORTED;
@@ -1272,8 +1275,9 @@ int moe_mlp_int8_bwd(const void* dy, int64_t lddy, int dtype, int dy_grouped, in
                      void* workspace, size_t workspace_bytes, void* stream)
 {
     hipStream_t st = S(stream);
-    if (dtype < 0 || dtype > 2 || dx_dtype < 0 || dx_dtype > 2 || E < 1 || R < 0 || d < 1 || f < 1 || dy_fan_out < 1 || lddy < d || lddx < d || (gates && (gates_dtype < 0 || gates_dtype > 2 || dy_grouped))) return MOE_ERR_BAD_ARG;
+    if (dtype < 0 || dtype > 2 || dx_dtype < 0 || dx_dtype > 2 || E < 1 || R < 0 || d < 1 || f < 1 || dy_fan_out < 1 || (gates && (gates_dtype < 0 || gates_dtype > 2 || dy_grouped))) return MOE_ERR_BAD_ARG;
     if (R == 0) return MOE_OK;
+    if (lddy < 0 || (R > 1 && lddx < d)) return MOE_ERR_BAD_ARG;
     if (!dy || !w1 || !s1 || !w3 || !s3 || !w2 || !s2 || !saved || !dx_rows || !pos || !offsets) return MOE_ERR_BAD_ARG;
     if (dtype == MOE_F32 || !i8_mlp_sizes_ok(d, f) || d > MOE_I8_MAX_K || 2 * f > MOE_I8_MAX_K || E > 65535 || R > 0x7fffffff) return MOE_ERR_UNSUPPORTED;
     if (!aligned16(w1) || !aligned16(w3) || !aligned16(w2)) return MOE_ERR_UNSUPPORTED;

@@ -61,6 +61,7 @@ void check_codes(const Tensor& q, const Tensor& scale, int64_t E, int64_t N)
 {
     TORCH_CHECK_TYPE(q.scalar_type() == at::kChar, "weight codes are int8, got ", q.scalar_type());
     TORCH_CHECK_TYPE(scale.scalar_type() == at::kFloat, "weight scales are float32, got ", scale.scalar_type());
+    TORCH_CHECK(!(at::GradMode::is_enabled() && scale.requires_grad()), "weights in 8 bits are frozen: their scales take no gradient");
     TORCH_CHECK(scale.dim() == 2 && scale.size(0) == E && scale.size(1) == N, "weight scales of ", scale.sizes(), " are not one for each of ", E, " experts' ",
                 N, " output columns");
 }

@@ -214,6 +214,25 @@ def test_linear_without_rows(dev):
     assert x.grad.shape == x.shape
 
 
+@pytest.mark.parametrize("rows", [1, 37])
+def test_rows_that_are_one_row(dev, rows):
+    """Inputs and gradients whose rows are one row of memory (a stride of 0), as expand and sum().backward() make them."""
+    K, N, E = 128, 96, 3
+    sei, ssi, eo, _ = (t.to(dev) for t in oracle.route(rows, E, 1, 2))
+    w, ws = (t.to(dev) for t in weights(E, K, N, 1, "nk"))
+    one = torch.randn(K, generator=torch.Generator().manual_seed(3)).to(BF16).to(dev)
+    call = lambda x: moe.parallel_linear_int8(x, w, ws, 1, sei, ssi, None, eo)   # noqa: E731
+    a, b = one.expand(rows, K).requires_grad_(True), one.expand(rows, K).contiguous().requires_grad_(True)
+    assert torch.equal(call(a), call(b)) and torch.equal(moe.quantize_rows(a)[0], moe.quantize_rows(b)[0])
+    dout = torch.ones(N, dtype=BF16, device=dev).expand(rows, N)
+    want = torch.autograd.grad(call(b), b, dout.contiguous())[0]
+    assert torch.equal(torch.autograd.grad(call(a), a, dout)[0], want) and torch.equal(torch.autograd.grad(call(b).sum(), b)[0], want)
+    mw = moe.Int8ExpertWeights(*(t.to(dev) for t in mlp_weights(E, K, 64, 0)))
+    mlp = lambda x: moe.fused_expert_mlp_int8(x, mw, 1, ssi, eo)   # noqa: E731
+    assert torch.equal(mlp(a), mlp(b))
+    assert torch.equal(torch.autograd.grad(mlp(a).sum(), a)[0], torch.autograd.grad(mlp(b).sum(), b)[0])
+
+
 def test_a_row_that_is_not_finite_stays_alone(dev):
     T, K, N, E, k = 40, 256, 128, 4, 2
     sei, ssi, eo, _ = oracle.route(T, E, k, 3)
@@ -489,6 +508,58 @@ def test_among_the_tools_of_autograd(dev):
     assert torch.equal(traced(other), call(other))
     with fwad.dual_level(), pytest.raises(RuntimeError, match="(?i)jvp|forward"):
         call(fwad.make_dual(x, torch.randn_like(x)))
+
+
+@pytest.mark.parametrize("gates_dtype", [F32, F16])
+def test_gates_of_another_type(dev, gates_dtype):
+    """Gate weights keep their own type, and so does their gradient: fp32 sums of fp32 rows, rounded once."""
+    T, K, N, E, k = 120, 192, 256, 4, 2
+    sei, ssi, eo, gw = oracle.route(T, E, k, 8)
+    w, ws = weights(E, K, N, 2, "nk")
+    g = torch.Generator().manual_seed(5)
+    x, dout, gw = torch.randn(T, K, generator=g).to(BF16), torch.randn(T, N, generator=g).to(BF16), gw.to(gates_dtype)
+    want = oracle.linear(x, w, ws, k, sei, ssi, gw, dout, near=127 * 5 * 2.0 ** -24)
+    xd, gd = x.to(dev).requires_grad_(True), gw.to(dev).requires_grad_(True)
+    y = moe.parallel_linear_int8(xd, w.to(dev), ws.to(dev), k, sei.to(dev), ssi.to(dev), None, eo.to(dev), gd)
+    y.backward(dout.to(dev))
+    h = half_step(BF16)
+    close(y, want["y"], want["y_terms"] * (F32_STEPS + 2 * k * 2.0 ** -24) * 1.01 + want["y"].abs() * h * 1.01, "y")
+    close(xd.grad, want["dx"], want["dx_slack"] * 1.01 + want["dx_terms"] * (F32_STEPS + k * 2.0 ** -24) * 1.01 + (want["dx"].abs() + want["dx_slack"]) * h * 1.01, "dx")
+    assert gd.grad.dtype == gates_dtype
+    close(gd.grad, want["d_gates"], want["d_gates_terms"] * (F32_STEPS + (N + 1) * 2.0 ** -24) * 1.01 + want["d_gates"].abs() * half_step(gates_dtype) * 1.01, "d_gates")
+
+
+def test_mlp_without_rows(dev):
+    x, w, ssi, eo, gates = setup_mlp(dev, 1)
+    x0, g0 = x[:0].detach().requires_grad_(True), gates[:0].detach().requires_grad_(True)
+    for grouped in (False, True):
+        y = moe.fused_expert_mlp_int8(x0, w, 2, ssi[:0], torch.zeros_like(eo), None if grouped else g0, grouped)
+        y.sum().backward()
+        assert y.shape == (0, x.size(1)) and x0.grad.shape == x0.shape
+    assert g0.grad.shape == g0.shape
+
+
+def test_what_is_not_finite_reaches_its_own_rows_only(dev):
+    """A weight column that is not finite reaches every row of its expert (through h), a token or a gradient row that is not only itself."""
+    x, w, ssi, eo, gates = setup_mlp(dev, 60)
+    dout = torch.randn_like(x)
+    good = mlp_step(x, w, 2, ssi, eo, gates, dout)
+    expert = torch.empty(120, dtype=torch.int64, device=dev)
+    expert[ssi] = torch.repeat_interleave(torch.arange(8, device=dev), torch.diff(eo, prepend=eo.new_zeros(1)))
+    bad_scale = w.w3_scale.clone()
+    bad_scale[3, 100] = float("nan")
+    bad = mlp_step(x, w._replace(w3_scale=bad_scale), 2, ssi, eo, gates, dout)
+    hit = (expert.view(60, 2) == 3).any(1)
+    for i in range(2):
+        assert torch.isnan(bad[i][hit]).all() and torch.equal(bad[i][~hit], good[i][~hit])
+    x2, d2 = x.clone(), dout.clone()
+    x2[7, 3] = float("inf")
+    d2[9] = float("-inf")
+    bad = mlp_step(x2, w, 2, ssi, eo, gates, d2)
+    rows = torch.arange(60, device=dev)
+    assert torch.isnan(bad[0][7]).all() and torch.equal(bad[0][rows != 7], good[0][rows != 7])
+    fine = (rows != 7) & (rows != 9)
+    assert torch.isnan(bad[1][[7, 9]]).all() and torch.equal(bad[1][fine], good[1][fine])
 
 
 # ---------------------------------------------------------------------------------------------------------------

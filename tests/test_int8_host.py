@@ -119,6 +119,16 @@ def test_layer_and_quantiser_arguments():
     _refused("GPU only", moe.quantize_rows, torch.zeros(2, 3))
 
 
+@on_host
+def test_scales_that_want_a_gradient():
+    with _MODE:
+        ws = torch.empty((E, N), dtype=F32, device="cuda:0", requires_grad=True)
+    fn, args = _linear(weight_scales=ws)
+    _refused("frozen", fn, **args)
+    fn, args = _mlp(_weights(w1_scale=ws))
+    _refused("frozen", fn, **args)
+
+
 def test_a_gradient_needs_every_assignment():
     import moe_distributed_training_amd as moe
     if torch.cuda.is_available():
@@ -136,13 +146,13 @@ def test_c_entries_refuse_on_the_host():
     from moe_distributed_training_amd._lib import lib
     q = lib.moe_quantize_rows
     assert q(16, 64, 3, 16, 128, 16, 4, 64, None) == -1 and q(16, 64, 0, 16, 120, 16, 4, 64, None) == -1 and q(16, 64, 0, 24, 128, 16, 4, 64, None) == -1
-    assert q(None, 64, 0, 16, 128, 16, 4, 64, None) == -1 and q(None, 64, 0, None, 128, None, 0, 64, None) == 0
+    assert q(16, -1, 0, 16, 128, 16, 4, 64, None) == -1 and q(None, 64, 0, 16, 128, 16, 4, 64, None) == -1 and q(None, 64, 0, None, 128, None, 0, 64, None) == 0
     assert lib.moe_quantize_weights(16, 1, 1, 1, 0, 2, 0, 8, 16, 1, 1, 1, 16, 16, 1 << 20, None) == -1
     assert lib.moe_quantize_weights(16, 1, 1, 1, 0, 2, 8, 8, 16, 1, 1, 1, 16, 16, 8, None) == -3
 
     def fwd(x=16, ldx=64, rows=8, dt=0, w=16, st=(8192, 1, 64), y=16, ldy=128, ydt=0, pos=16, E=2, R=16, K=64, N=128, fan=2, xg=0, yg=0, ws=16, n=1 << 30):
         return lib.moe_linear_int8_fwd(x, ldx, rows, dt, w, *st, 16, y, ldy, ydt, pos, 0, 16, 0, E, R, K, N, fan, xg, yg, ws, n, None)
-    assert fwd(x=None) == -1 and fwd(dt=3) == -1 and fwd(ydt=-1) == -1 and fwd(ldx=63) == -1 and fwd(ldy=127) == -1 and fwd(pos=None) == -1 and fwd(E=0) == -1 and fwd(fan=0) == -1
+    assert fwd(x=None) == -1 and fwd(dt=3) == -1 and fwd(ydt=-1) == -1 and fwd(ldx=-1) == -1 and fwd(ldy=127) == -1 and fwd(pos=None) == -1 and fwd(E=0) == -1 and fwd(fan=0) == -1
     assert fwd(xg=1, rows=15) == -1 and fwd(K=131072, ldx=131072, st=(1 << 25, 1, 131072)) == -2 and fwd(n=64) == -3 and fwd(ws=None) == -3 and fwd(R=0, x=None) == 0
     # gathered rows whose codes do not fit 32-bit offsets, and a matrix that does not
     assert fwd(rows=1 << 26, R=16, n=1 << 40) == -2
@@ -150,14 +160,14 @@ def test_c_entries_refuse_on_the_host():
 
     def bwd(dy=16, ldd=128, dt=0, w=16, st=(8192, 1, 64), dx=16, lddx=64, gates=None, gdt=0, pos=16, E=2, R=16, K=64, N=128, ws=16, n=1 << 30):
         return lib.moe_linear_int8_bwd(dy, ldd, dt, 0, 2, gates, gdt, w, *st, 16, dx, lddx, dt, 0, pos, 0, 16, 0, E, R, K, N, ws, n, None)
-    assert bwd(dy=None) == -1 and bwd(ldd=127) == -1 and bwd(lddx=63) == -1 and bwd(gates=16, gdt=3) == -1 and bwd(pos=None) == -1 and bwd(N=131072, ldd=131072) == -2 and bwd(n=0) == -3
+    assert bwd(dy=None) == -1 and bwd(ldd=-1) == -1 and bwd(lddx=63) == -1 and bwd(gates=16, gdt=3) == -1 and bwd(pos=None) == -1 and bwd(N=131072, ldd=131072) == -2 and bwd(n=0) == -3
 
     def mlp(x=16, dt=0, d=64, f=128, R=16, rows=8, saved=None, sn=0, ws=16, n=1 << 30, w=16):
         return lib.moe_mlp_int8_fwd(x, d, rows, dt, w, 16, 16, 16, 16, 16, 16, d, 0, 16, 0, 16, 0, 2, R, d, f, 2, 0, saved, sn, ws, n, None)
     assert mlp(x=None) == -1 and mlp(dt=2) == -2 and mlp(d=96) == -2 and mlp(f=100) == -2 and mlp(w=24) == -2 and mlp(saved=16, sn=8) == -3 and mlp(n=0) == -3 and mlp(R=0) == 0
     assert lib.moe_mlp_int8_saved_bytes(16, 128) == 2 * (16 * 128 * 3 + 256)       # 24 bits a value, a scale for each 32
     assert lib.moe_combine_f32(16, 64, 16, 64, 0, None, 0, 0, 4, 64, None) == -1 and lib.moe_combine_f32(None, 64, 16, 64, 0, None, 0, 2, 4, 64, None) == -1
-    assert lib.moe_combine_f32_dgates(16, 64, 16, 63, 0, 16, 0, 2, 4, 64, None) == -1 and lib.moe_combine_f32(None, 64, None, 64, 0, None, 0, 2, 0, 64, None) == 0
+    assert lib.moe_combine_f32_dgates(16, 64, 16, -1, 0, 16, 0, 2, 4, 64, None) == -1 and lib.moe_combine_f32(None, 64, None, 64, 0, None, 0, 2, 0, 64, None) == 0
 
 
 def test_workspaces_cover_what_the_calls_take():
