@@ -17,7 +17,7 @@ for line in text.splitlines():
         name = m.group(1)
         continue
     m = re.search(r"(SGPRs|VGPRs) Spill: (\d+)", line)
-    if m and name and "grouped_gemm_mfma_kernel" in name:
+    if m and name and ("grouped_gemm_mfma_kernel" in name or "i8_gemm_kernel" in name):
         seen += 1
         general = name.endswith("Lb1EEEv13MoeGemmParams")
         if int(m.group(2)) > 0 and (m.group(1) == "VGPRs" or not general):
