@@ -383,12 +383,13 @@ __global__ void __launch_bounds__(NTHREADS, 2) i8_gemm_kernel(const MoeI8Gemm p)
             pair = __builtin_amdgcn_permlane32_swap(top, top, false, false);
             top = max(pair[0], pair[1]);
             const float amax = __uint_as_float(top);
-            const bool fine = top < 0x7f800000u;
-            // (a segment below 2^-100 is zero to the 8-bit codes of any row that is not as small as that)
-            const float inv = fine && amax > 0x1p-100f ? MOE_SEG_LEVELS * __builtin_amdgcn_rcpf(amax) : 0.f;
-            if (__any(!fine))   // (its scale says NaN)
+            const bool fine = top < 0x7f800000u;   // (otherwise its scale says NaN)
+            // (magnitudes from which the steps per unit would leave fp32's range, and zeros, are multiplied by a power of two first)
+            const float by = amax > 0x1p64f ? 0x1p-64f : amax < 0x1p-64f ? 0x1p64f : 1.f;
+            const float inv = fine && amax > 0.f ? MOE_SEG_LEVELS * __builtin_amdgcn_rcpf(amax * by) : 0.f;
+            if (__any(!fine || by != 1.f))
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = fine ? v[i] : 0.f;
+                for (int i = 0; i < 8; ++i) v[i] = fine ? v[i] * by : 0.f;
             int q[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) q[i] = (int)rintf(v[i] * inv);
@@ -404,7 +405,7 @@ __global__ void __launch_bounds__(NTHREADS, 2) i8_gemm_kernel(const MoeI8Gemm p)
                 uint8_t* to = out + at * MOE_SEG_BYTES;
                 *(u32x4_t*)(to + g * 16) = hi;
                 *(uint2*)(to + 64 + g * 8) = lo;
-                if (g == 0) scales[(wrow0 + m) * SEGS + seg] = !fine ? __uint_as_float(0x7fc00000u) : (inv > 0.f ? amax * (1.f / MOE_SEG_LEVELS) : 0.f) * row_scale;   // (zeros of a row whose scale is NaN are NaN)
+                if (g == 0) scales[(wrow0 + m) * SEGS + seg] = fine ? amax * row_scale : __uint_as_float(0x7fc00000u);   // (zeros of a row whose scale is NaN are NaN)
             }
         };
         auto xs = [&](int mb) { return s_xscale[wrow0 + mb * 16 + (lane & 15)]; };

@@ -230,15 +230,15 @@ __global__ void __launch_bounds__(1024) quantize_rows_kernel(const MoeQuantizeRo
     if (threadIdx.x == 0) p.scale[m] = rc.scale;
 }
 
-// Columns c0 .. c0 + 7 of a row of segments, times s.  A value's three bytes go to the upper three of a word, so that one conversion makes it a float (256 times
-// what it is: s carries the rest).
+// Columns c0 .. c0 + 7 of a row of segments, of a segment whose maximum is s (2^-95 or more).  A value's three bytes go to the upper three of a word, so that one
+// conversion makes it a float (256 times what it is: s carries the rest).
 __device__ __forceinline__ void ld8_seg(const uint8_t* row, int64_t c0, float s, float* v)
 {
     const uint8_t* seg = row + c0 / MOE_SEG_COLS * MOE_SEG_BYTES;
     const int c = (int)(c0 % MOE_SEG_COLS);
     const u32x4_t hi = *(const u32x4_t*)(seg + c * 2);
     const uint2 lo = *(const uint2*)(seg + 64 + c);
-    s *= 1.f / 256.f;
+    s *= 1.f / (256.f * MOE_SEG_LEVELS);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const uint32_t l = i < 2 ? lo.x : lo.y;
@@ -247,13 +247,23 @@ __device__ __forceinline__ void ld8_seg(const uint8_t* row, int64_t c0, float s,
     }
 }
 
-// Rows of segments -> codes: the maximum of a row is that of its segments, MOE_SEG_LEVELS times their scales.
+// ... of any maximum: the step of a segment below 2^-95 would be subnormal, so that one is read 2^64 times as large.
+__device__ __forceinline__ void ld8_seg_any(const uint8_t* row, int64_t c0, float s, float* v)
+{
+    const bool tiny = s < 0x1p-90f;
+    ld8_seg(row, c0, tiny ? s * 0x1p64f : s, v);
+    if (tiny)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] *= 0x1p-64f;
+}
+
+// Rows of segments -> codes: the maximum of a row is that of its segments.
 __global__ void __launch_bounds__(1024) requantize_rows_kernel(const uint8_t* src, const float* seg, int64_t cols, int8_t* codes, int64_t ldc, float* scale)
 {
     const int64_t m = blockIdx.x;
     const int64_t nseg = cols / MOE_SEG_COLS;
     uint32_t top = 0;
-    for (int64_t i = threadIdx.x; i < nseg; i += blockDim.x) top = max(top, mag_bits(seg[m * nseg + i] * MOE_SEG_LEVELS));
+    for (int64_t i = threadIdx.x; i < nseg; i += blockDim.x) top = max(top, mag_bits(seg[m * nseg + i]));
     const RowCoder rc(block_max(top));
     for (int64_t c0 = (int64_t)threadIdx.x * 8; c0 < ldc; c0 += (int64_t)blockDim.x * 8) {
         uint2 w = {0u, 0u};
@@ -285,9 +295,9 @@ __global__ void __launch_bounds__(KEEP == 1 ? 256 : 512) swiglu_bwd_codes_kernel
     auto load = [&](int64_t c0, float* a, float* b) {
         float dh[8], g[8], u[8], x1[8], x3[8];
         const int64_t s = m * nseg + c0 / MOE_SEG_COLS;
-        ld8_seg(dh_row, c0, p.dh_seg[s], dh);
-        ld8_seg(gate_row, c0, p.gate_seg[s], g);
-        ld8_seg(up_row, c0, p.up_seg[s], u);
+        ld8_seg_any(dh_row, c0, p.dh_seg[s], dh);
+        ld8_seg_any(gate_row, c0, p.gate_seg[s], g);
+        ld8_seg_any(up_row, c0, p.up_seg[s], u);
         Loader<float>::ld8(c1 + c0, x1);
         Loader<float>::ld8(c3 + c0, x3);
 #pragma unroll

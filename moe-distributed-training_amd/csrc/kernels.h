@@ -213,8 +213,8 @@ int moe_launch_swiglu_bwd(const void* g, const void* u, const void* dh, void* dg
                           hipStream_t stream);
 
 // ---- expert products in 8-bit integers (int8_rows.hip, int8_gemm.hip)
-// interims between two products: segments of 32 columns of a row as 24-bit integers that share a scale, 96 bytes each: the upper 16 bits of the 32
-// values, then their lower 8; [R][N / 32] of them.  The maximum of a segment is MOE_SEG_LEVELS steps, far enough from 2^23 for a reciprocal that is off by its last bit.
+// interims between two products: segments of 32 columns of a row as 24-bit integers that share a scale, the segment's maximum, 96 bytes each: the upper 16 bits of the 32
+// values, then their lower 8; [R][N / 32] of them.  The maximum is MOE_SEG_LEVELS steps, far enough from 2^23 for a reciprocal that is off by its last bit.
 constexpr int MOE_SEG_COLS = 32, MOE_SEG_BYTES = 96;
 constexpr float MOE_SEG_LEVELS = 8388600.f;
 constexpr int MOE_I8_KTILE = 128;       // codes of a row come in whole K tiles, zeros behind the last column

@@ -103,3 +103,80 @@ def mlp(x, w, k, sei, ssi, gates=None, dout=None, grouped_out=False, near=0.0):
         if gates is not None:
             out["d_gates"] = (y.view(T, kk, d) * dout.double().unsqueeze(1)).sum(-1)
     return out
+
+
+STEP = 2.0 ** -24     # relative rounding error of fp32
+
+
+def _segment_max(v):
+    return v.abs().view(v.size(0), -1, 32).amax(2, keepdim=True).expand(-1, -1, 32).reshape(v.shape)
+
+
+def _stored(v, err):
+    """Error of values that are off by err and then kept as 24-bit multiples of a step of their 32-column segment: half a step, and the fp32 roundings of the
+    factor (a reciprocal, off by its last bit), of the product and of the way back."""
+    return err + 8 * STEP * v.abs() + 1.01 * STEP * _segment_max(v)
+
+
+def _codes_of_approximate(v, err):
+    """Codes and scales of rows whose values are off by up to err; which codes an implementation may round the other way, and the relative error of its scales."""
+    c, s, _ = codes(v)
+    top = s * 127
+    top = torch.where(top > 0, top, torch.ones_like(top))
+    worst = err.amax(1, keepdim=True) / top
+    near = 127 * (err + v.abs() * (worst + 4 * STEP)) / top
+    edge = (127 * v / top - c).abs() > 0.5 - near
+    return c, s, edge.double(), worst + 2 * STEP
+
+
+def mlp_bounds(x, w, k, sei, ssi, gates=None, dout=None):
+    """As mlp(), with a bound for every element of y, dx and d_gates before their last rounding: codes that lie so near a border that the roundings of fp32
+    arithmetic and of 24-bit interims may carry them over it count with a whole step, everything else with its roundings.  Codes of x and of the gradient's rows are
+    exact.  The logistic function: exp2 of a rounded product (relative error 2 |g| + 2 steps), one sum, one reciprocal."""
+    w1, s1, w2, s2, w3, s3 = (t.double() for t in w)
+    cx, sx, _ = codes(x)
+    sx = sx.float().double()
+    R, d, f = ssi.numel(), x.size(1), w1.size(1)
+    y, y_slack, dx, dx_slack = (torch.zeros(R, d, dtype=torch.float64) for _ in range(4))
+    flat = None if gates is None else gates.double().reshape(-1)
+    for e in sei.unique().tolist():
+        i = (sei == e).nonzero().squeeze(1)
+        at, t = ssi[i], ssi[i] // k
+        g, u = (cx[t] @ w1[e].t()) * sx[t] * s1[e], (cx[t] @ w3[e].t()) * sx[t] * s3[e]
+        sig = torch.sigmoid(g)
+        slope = sig * torch.sigmoid(-g)
+        sig_err = torch.where(g > 18, torch.exp(-g), slope * (2 * g.abs() + 2) * STEP + 4 * STEP * sig) + 2.0 ** -125
+        ge, ue = 3 * STEP * g.abs(), 3 * STEP * u.abs()
+        h = g * sig * u
+        h_err = u.abs() * (sig + g.abs() * slope) * ge + (g * sig).abs() * ue + (g * u).abs() * sig_err + 3 * STEP * h.abs() + 2.0 ** -148
+        ch, sh, edge, off = _codes_of_approximate(h, _stored(h, h_err))
+        y[at] = (ch @ w2[e]) * sh * s2[e]
+        y_slack[at] = (edge @ w2[e].abs()) * sh * s2[e] + y[at].abs() * (off + 6 * STEP)
+        if dout is None:
+            continue
+        dy = dout.double()[at // gates.size(1)] * flat[at][:, None] if gates is not None else dout.double()[at]
+        cg, sg, _ = codes(dy * s2[e])
+        dh = (cg @ w2[e].t()) * sg
+        ge, ue, de = _stored(g, ge), _stored(u, ue), _stored(dh, 4 * STEP * dh.abs())
+        rest = torch.sigmoid(-g)
+        a, b = dh * u * sig * (1 + g * rest) * s1[e], dh * g * sig * s3[e]
+        p_err = (2 + g.abs()) * slope * ge + sig_err * (1 + g.abs() * (rest + sig)) + 4 * STEP * sig * (1 + g.abs() * rest)
+        a_err = ((u * sig * (1 + g * rest)).abs() * de + (dh * sig * (1 + g * rest)).abs() * ue + (dh * u).abs() * p_err) * s1[e] + 6 * STEP * a.abs()
+        b_err = ((g * sig).abs() * de + dh.abs() * (sig + g.abs() * slope) * ge + (dh * g).abs() * sig_err) * s3[e] + 6 * STEP * b.abs()
+        ca, sa, edge, off = _codes_of_approximate(torch.cat([a, b], 1), torch.cat([a_err, b_err], 1) + 2.0 ** -148)
+        dx[at] = (ca[:, :f] @ w1[e] + ca[:, f:] @ w3[e]) * sa
+        dx_slack[at] = (edge[:, :f] @ w1[e].abs() + edge[:, f:] @ w3[e].abs()) * sa + dx[at].abs() * (off + 4 * STEP)
+    out = {"y": y, "y_slack": y_slack}
+    if gates is not None:
+        T, kk = gates.shape
+        z = gates.double().unsqueeze(-1)
+        terms = (y.view(T, kk, d) * z).abs().sum(1)
+        out["y"], out["y_slack"] = (y.view(T, kk, d) * z).sum(1), (y_slack.view(T, kk, d) * z.abs()).sum(1) + 2 * kk * STEP * terms
+    if dout is not None:
+        out["dx"] = dx.view(-1, k, d).sum(1)
+        out["dx_slack"] = dx_slack.view(-1, k, d).sum(1) + (k * STEP * dx.abs().view(-1, k, d).sum(1) if k > 1 else 0)
+        if gates is not None:
+            dd = dout.double().unsqueeze(1)
+            out["d_gates"] = (y.view(T, kk, d) * dd).sum(-1)
+            out["d_gates_slack"] = (y_slack.view(T, kk, d) * dd.abs()).sum(-1) + (d + 1) * STEP * (y.view(T, kk, d) * dd).abs().sum(-1)
+    return out
