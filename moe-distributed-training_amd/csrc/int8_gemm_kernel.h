@@ -482,6 +482,17 @@ __global__ void __launch_bounds__(NTHREADS, 2) i8_gemm_kernel(const MoeI8Gemm p)
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) column_scales(nb, w[nb]);
         const int64_t ncol0 = n0 + wn * WTN;
+        // Sum times row scale times column scale.  Where the first product could leave fp32's range (rows of 2^71 on) the row scale comes 2^40 times smaller, and what
+        // it comes to is as much larger again: powers of two round nothing.
+        auto values = [&](int mb, int nb, float xs, float* v) {
+            const bool far = xs > 0x1p64f;
+            const float x = far ? xs * 0x1p-40f : xs;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[r] = (float)acc[mb][nb][r] * x * w[nb][r];
+            if (__any(far))
+#pragma unroll
+                for (int r = 0; r < 4; ++r) v[r] = far ? v[r] * 0x1p40f : v[r];
+        };
         if (p.ydtype == MOE_F32) {
             const bool vec = p.y_vec;
 #pragma unroll
@@ -494,8 +505,7 @@ __global__ void __launch_bounds__(NTHREADS, 2) i8_gemm_kernel(const MoeI8Gemm p)
                 for (int nb = 0; nb < NB; ++nb) {
                     const int64_t n = ncol0 + nb * 16 + nq;
                     float v[4];
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) v[r] = (float)acc[mb][nb][r] * xs * w[nb][r];
+                    values(mb, nb, xs, v);
                     if (vec && n < p.N) *(float4*)(y + n) = make_float4(v[0], v[1], v[2], v[3]);
                     else
 #pragma unroll
@@ -513,8 +523,7 @@ __global__ void __launch_bounds__(NTHREADS, 2) i8_gemm_kernel(const MoeI8Gemm p)
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
                 float v[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) v[r] = (float)acc[mb][nb][r] * xs * w[nb][r];
+                values(mb, nb, xs, v);
                 uint2 o;
                 if (f16) { o.x = NumF16::pack2(v[0], v[1]); o.y = NumF16::pack2(v[2], v[3]); }
                 else { o.x = NumBf16::pack2(v[0], v[1]); o.y = NumBf16::pack2(v[2], v[3]); }

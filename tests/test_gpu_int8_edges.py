@@ -1,5 +1,5 @@
-"""Expert products over 8-bit weights at the edges of what their entry points take: magnitudes down to the end of fp32's
-range.  Every result is compared element by element with the definition in 64 bits; what a code next to a border may change is counted there."""
+"""Expert products over 8-bit weights at the edges of what their entry points take: magnitudes from one end of fp32's
+range to the other.  Every result is compared element by element with the definition in 64 bits; what a code next to a border may change is counted there."""
 import pytest
 import torch
 
@@ -36,11 +36,14 @@ def mlp_weights(E, d, f, seed):
 SMALL = [(-56, 0), (-53, -10), (-51, 0), (-45, 30), (-20, -90), (0, -105), (0, 0)]   # powers of two that rows of x and of the gradient are multiplied by
 
 
-@pytest.mark.parametrize("powers", [SMALL])
+LARGE = [(20, 0), (40, 0), (63, -100)]
+
+
+@pytest.mark.parametrize("powers", [SMALL, LARGE])
 @pytest.mark.parametrize("gated", [False, True])
 @pytest.mark.parametrize("d,f,per", [(128, 192, 3), (64, 512, 40)])
 def test_mlp_rows_of_any_magnitude(dev, d, f, per, gated, powers):
-    """h is a product of two projections: rows of 2^-56 give h of about 2^-115, which fp32 and bf16 hold."""
+    """h is a product of two projections: rows of 2^-56 give h of about 2^-115, rows of 2^63 of about 2^126, which fp32 and bf16 hold."""
     T, E, k = per * len(powers), 3, 1
     g = torch.Generator().manual_seed(d + per)
     exps = torch.tensor(powers, dtype=torch.float64).repeat_interleave(per, 0)
@@ -55,3 +58,22 @@ def test_mlp_rows_of_any_magnitude(dev, d, f, per, gated, powers):
     close(y, want["y"], want["y_slack"], BF16, "y")
     dx = torch.autograd.grad(y, xd, dout.to(dev))[0]
     close(dx, want["dx"], want["dx_slack"], BF16, "dx")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("T", [24, 700])
+def test_linear_rows_up_to_the_end_of_the_range(dev, dtype, gated, T):
+    """Results of up to 2^122: the sum of a row of 2^124 times the row's scale alone would leave fp32's range."""
+    K, N, E, k = 512, 192, 3, 2
+    g = torch.Generator().manual_seed(T)
+    power = torch.tensor([0, 60, 72, 100, 115, 122])[torch.arange(T) % 6].double()
+    x = (torch.randn(T, K, generator=g).double().clamp(-3, 3) * 2.0 ** power[:, None]).to(dtype)
+    w = torch.randint(-127, 128, (E, N, K), generator=g, dtype=torch.int8).transpose(1, 2)
+    ws = (torch.rand(E, N, generator=g) + 0.5) * 2.0 ** -16
+    sei, ssi, eo, gw = oracle.route(T, E, k, 3)
+    gw = gw.to(dtype) if gated else None
+    want = oracle.linear(x, w, ws, k, sei, ssi, gw)
+    assert 2.0 ** 114 < float(want["y"].abs().max()) < 2.0 ** 126
+    y = moe.parallel_linear_int8(x.to(dev), w.to(dev), ws.to(dev), k, sei.to(dev), ssi.to(dev), None, eo.to(dev), gw.to(dev) if gated else None)
+    close(y, want["y"], (want["y_terms"] if gated else want["y"].abs()) * (6 + 2 * k) * 2.0 ** -24, dtype, "y")
