@@ -2,11 +2,13 @@
 // weights in an order that the product kernel can read.
 //
 // A row v becomes codes q[c] = rne(127 v[c] / a) with a = max |v| and the scale a / 127: the quotient is rounded as it is, not as some fp32 value of
-// it comes out (ties are common: half the maximum is 63.5 for every row of a 2-byte type), so the codes are the same on every path and in any
-// precision that a checker takes.  q is guessed with one multiplication by 127 / a and put right from its remainder 127 v - q a: 127 v is held as
-// an fp32 number and its rounding error, and the difference with q a is exact (it is a multiple of half a unit of a's last place and at most a / 2; below a / 254 q
-// is 0).  Gradient rows, products of two or three numbers, are held as an fp32 number and its error from the start (but for bf16, see below).  A row that holds an
-// infinity or a NaN gets the scale NaN and codes 0, so that every product of it is NaN and no other row changes; a row of zeros the scale 0.
+// it comes out (ties are common: half the maximum is 63.5 for every row of a 2-byte type).  q is guessed with one multiplication by 127 / a and, next to a border, put right
+// from its remainder 127 v - q a: 127 v is held as an fp32 number and its rounding error, and the difference with q a is exact (it is a multiple of half a unit of a's last
+// place and at most a / 2; below a / 254 q is 0).  Rows of inputs and weights are what they are; rows of gradients, products of two or three numbers, are held as an fp32
+// number and its error (together off by 2^-46 of it) from the start, their maximum too.  (16384 x 2048 bf16 gradient rows: 45 us, against 36 from fp32 products and a rounded 127 / a,
+// which puts 1 code in 10^5, and ties of most maxima, on the other side.)  The MLP's own interims, h and the joint row of dgate and dup, are computed in fp32 and carry its
+// rounding: their codes are of the fp32 values, by one multiplication, and a value within 127 * 2^-20 of a step from a border may go to either side.
+// A row that holds an infinity or a NaN gets the scale NaN and codes 0, so that every product of it is NaN and no other row changes; a row of zeros the scale 0.
 //
 // Interims (h, the saved gate and up, dh) travel as 24-bit integers with a scale for each 32 columns of a row: 3 bytes per value, at most 2^-24 of the segment's
 // maximum off.  Every value that a rounding on the way carries over a border of the 8-bit codes costs a whole step, so this noise falls with the root of
@@ -22,29 +24,34 @@ typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 // Magnitudes are compared as bits: those of an infinity lie above every number's, and NaN's above those.
 constexpr uint32_t NOT_FINITE = 0x7f800000u;
 __device__ __forceinline__ uint32_t mag_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-template <typename U> __device__ __forceinline__ U block_max(U v)
+// (a kernel's second maximum has its own place: the first may still be read)
+template <int PLACE = 0> __device__ __forceinline__ uint32_t block_max(uint32_t v)
 {
-    __shared__ U s_max[16];
+    __shared__ uint32_t s_max[16];
 #pragma unroll
-    for (int m = 32; m > 0; m >>= 1) { const U o = __shfl_xor(v, m); v = v > o ? v : o; }
+    for (int m = 32; m > 0; m >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, m));
     if (blockDim.x == 64) return v;
     if ((threadIdx.x & 63) == 0) s_max[threadIdx.x >> 6] = v;
     __syncthreads();
     v = s_max[0];
-    for (int w = 1; w < (int)(blockDim.x >> 6); ++w) v = v > s_max[w] ? v : s_max[w];
+    for (int w = 1; w < (int)(blockDim.x >> 6); ++w) v = max(v, s_max[w]);
     return v;
 }
-// The order of magnitudes |v + lo| of numbers held with their errors, and the error of the magnitude at a place in that order.
-__device__ __forceinline__ unsigned long long mag_key(float v, float lo)
+// (g + ge) s as the nearest fp32 number and its error.  (Contracted, the sum of the product and its error would hold the error twice.)
+__device__ __forceinline__ void times_with_error(float g, float ge, float s, float* v, float* lo)
+{
+#pragma clang fp contract(off)
+    const float h = g * s, he = fmaf(g, s, -h) + ge * s;
+    *v = h + he;
+    *lo = he - (*v - h);
+}
+// Errors lo of numbers v as those of their magnitudes, in an order that unsigned numbers have, and back.
+__device__ __forceinline__ uint32_t error_key(float v, float lo)
 {
     const uint32_t b = __float_as_uint(v < 0.f ? -lo : lo);
-    return (unsigned long long)mag_bits(v) << 32 | (b >> 31 ? ~b : b | 0x80000000u);
+    return b >> 31 ? ~b : b | 0x80000000u;
 }
-__device__ __forceinline__ float key_error(unsigned long long key)
-{
-    const uint32_t b = (uint32_t)key;
-    return __uint_as_float(b >> 31 ? b & 0x7fffffffu : ~b);
-}
+__device__ __forceinline__ float key_error(uint32_t b) { return __uint_as_float(b >> 31 ? b & 0x7fffffffu : ~b); }
 
 // What turns values of a row into its codes.  f: what the values are multiplied by first, so that 127 v and 127 / a stay inside fp32's range (a value that the
 // factor makes subnormal is far below half a step).
@@ -61,7 +68,12 @@ struct RowCoder {
         if (inv == 0.f) f = 0.f;   // every code 0
         scale = fine ? amax / 127.f : __uint_as_float(0x7fc00000u);
     }
-    // the code of v + lo, lo the rounding error of v
+    // The code of v + lo, lo the rounding error of v.  v times 127 / a is off by five roundings, 127 * 5 * 2^-24 < 4e-5 of a step: only beside a border does more matter.
+    __device__ __forceinline__ float code(float v, float lo) const
+    {
+        const float t = f == 0.f ? 0.f : v * f * inv, q = rintf(t);
+        return fabsf(t - q) > 0.4999f ? exact(v, lo) : q;
+    }
     __device__ __forceinline__ float exact(float v, float lo) const
     {
         v = f == 0.f ? 0.f : v * f;
@@ -174,59 +186,49 @@ __global__ void __launch_bounds__(1024) quantize_rows_kernel(const MoeQuantizeRo
                 const float g = coeff * x[i], ge = fmaf(coeff, x[i], -g);
                 v[i] = g;
                 lo[i] = ge;
-                if (cs) {
-                    v[i] = g * s[i];
-                    lo[i] = fmaf(g, s[i], -v[i]) + ge * s[i];
-                }
+                if (cs) times_with_error(g, ge, s[i], v + i, lo + i);
             }
         }
     };
-    // Gradient rows.  The few codes that fp32 products round the other way (1 in 10^5) add 2 to 5e-4 to a result's error: nothing beside bf16's own rounding (1.7e-3), twice
-    // that of fp16, whose values are taken with their errors; fp32 rows take their maximum with its error too, which moves borders by 127 * 2^-25 of a step.
-    // (16384 x 2048 rows: 44 us with errors, 36 without.)
-    constexpr bool WITH_ERROR = SCALED && std::is_same_v<T, float>;
-    constexpr bool EXACT = !SCALED || !std::is_same_v<T, __hip_bfloat16>;
     float keep[KEEP ? KEEP : 1][8], low[KEEP ? KEEP : 1][8];
-    std::conditional_t<WITH_ERROR, unsigned long long, uint32_t> top = 0;
-    auto look = [&](const float* v, const float* lo) {
+    uint32_t mine = 0;
+    auto each = [&](auto fn) {
+        if constexpr (KEEP > 0) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if constexpr (WITH_ERROR) { const unsigned long long key = mag_key(v[i], lo[i]); top = key > top ? key : top; }
-            else top = max(top, mag_bits(v[i]));
-        }
+            for (int j = 0; j < KEEP; ++j) {
+                const int64_t c0 = ((int64_t)j * nt + threadIdx.x) * 8;
+                if (c0 < p.ldc) fn(j, c0);
+            }
+        } else
+            for (int64_t c0 = (int64_t)threadIdx.x * 8; c0 < p.ldc; c0 += (int64_t)nt * 8) { load(c0, keep[0], low[0]); fn(0, c0); }
     };
-    if constexpr (KEEP > 0) {
+    if constexpr (KEEP > 0) each([&](int j, int64_t c0) { load(c0, keep[j], low[j]); });
+    each([&](int j, int64_t) {
 #pragma unroll
-        for (int j = 0; j < KEEP; ++j) {
-            const int64_t c0 = ((int64_t)j * nt + threadIdx.x) * 8;
-            if (c0 < p.ldc) { load(c0, keep[j], low[j]); look(keep[j], low[j]); }
-        }
-    } else {
-        for (int64_t c0 = (int64_t)threadIdx.x * 8; c0 < p.ldc; c0 += (int64_t)nt * 8) { load(c0, keep[0], low[0]); look(keep[0], low[0]); }
+        for (int i = 0; i < 8; ++i) mine = max(mine, mag_bits(keep[j][i]));
+    });
+    const uint32_t top = block_max(mine);
+    uint32_t top_error = 0;
+    if (SCALED) {
+        if (mine == top)   // (few lanes: those that hold the maximum)
+            each([&](int j, int64_t) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (mag_bits(keep[j][i]) == top) top_error = max(top_error, error_key(keep[j][i], low[j][i]));
+            });
+        top_error = block_max<1>(top_error);
     }
-    top = block_max(top);
-    RowCoder rc(0u);
-    if constexpr (WITH_ERROR) rc = RowCoder((uint32_t)(top >> 32), key_error(top));
-    else rc = RowCoder(top);
+    const RowCoder rc(top, SCALED ? key_error(top_error) : 0.f);
     int8_t* out = p.codes + m * p.ldc;
-    auto store = [&](int64_t c0, const float* v, const float* lo) {
+    each([&](int j, int64_t c0) {
         float q[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) q[i] = EXACT ? rc.exact(v[i], lo[i]) : rc.nearest(v[i]);
+        for (int i = 0; i < 8; ++i) q[i] = rc.code(keep[j][i], low[j][i]);
         uint2 w;
         w.x = pack4(q[0], q[1], q[2], q[3]);
         w.y = pack4(q[4], q[5], q[6], q[7]);
         *(uint2*)(out + c0) = w;
-    };
-    if constexpr (KEEP > 0) {
-#pragma unroll
-        for (int j = 0; j < KEEP; ++j) {
-            const int64_t c0 = ((int64_t)j * nt + threadIdx.x) * 8;
-            if (c0 < p.ldc) store(c0, keep[j], low[j]);
-        }
-    } else {
-        for (int64_t c0 = (int64_t)threadIdx.x * 8; c0 < p.ldc; c0 += (int64_t)nt * 8) { load(c0, keep[0], low[0]); store(c0, keep[0], low[0]); }
-    }
+    });
     if (threadIdx.x == 0) p.scale[m] = rc.scale;
 }
 

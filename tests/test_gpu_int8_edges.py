@@ -1,5 +1,5 @@
 """Expert products over 8-bit weights at the edges of what their entry points take: magnitudes from one end of fp32's
-range to the other.  Every result is compared element by element with the definition in 64 bits; what a code next to a border may change is counted there."""
+range to the other, gradient rows full of ties.  Every result is compared element by element with the definition in 64 bits; what a code next to a border may change is counted there."""
 import pytest
 import torch
 
@@ -77,3 +77,49 @@ def test_linear_rows_up_to_the_end_of_the_range(dev, dtype, gated, T):
     assert 2.0 ** 114 < float(want["y"].abs().max()) < 2.0 ** 126
     y = moe.parallel_linear_int8(x.to(dev), w.to(dev), ws.to(dev), k, sei.to(dev), ssi.to(dev), None, eo.to(dev), gw.to(dev) if gated else None)
     close(y, want["y"], (want["y_terms"] if gated else want["y"].abs()) * (6 + 2 * k) * 2.0 ** -24, dtype, "y")
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# codes of gradient rows
+# ---------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("gated", [False, True])
+def test_gradient_rows_full_of_ties(dev, dtype, gated):
+    """Half of a row's maximum is 63.5 steps: ties go to the even code, whatever the maximum.  Weights that pick single inputs hand the codes out one by one, and a power of
+    two as gate and column scale leaves the quotients as they are."""
+    K = N = 256
+    T = 254
+    tops = torch.arange(129, 256, 2).double()                      # odd: half of it is the other side of a tie in any of the types
+    top = tops.repeat(4)[:T]
+    dout = torch.empty(T, N, dtype=torch.float64)
+    dout[:, 0::4], dout[:, 1::4] = top[:, None] / 2, -top[:, None] / 2
+    dout[:, 2::4], dout[:, 3::4] = top[:, None] / 4, torch.arange(0, 64).double()
+    dout[:, 7] = top
+    dout = dout.to(dtype)
+    assert torch.equal(dout[:, 0].double(), top / 2)
+    w = torch.eye(K, dtype=torch.int8).unsqueeze(0)
+    x = torch.ones(T, K, dtype=dtype, device=dev, requires_grad=True)
+    idx = torch.arange(T, device=dev)
+    gates = torch.full((T, 1), 0.5, dtype=dtype, device=dev) if gated else None
+    y = moe.parallel_linear_int8(x, w.to(dev), torch.full((1, N), 0.25, device=dev), 1, torch.zeros_like(idx), idx, None, None, gates)
+    dx = torch.autograd.grad(y, x, dout.to(dev))[0]
+    c, s, _ = oracle.codes(dout)
+    want = c * s.float().double() * (0.125 if gated else 0.25)
+    close(dx, want, 4 * 2.0 ** -24 * want.abs(), dtype, "dx")
+
+
+@pytest.mark.parametrize("dtype,gates_dtype", [(BF16, BF16), (BF16, F32), (F16, F16), (F16, F32), (F32, F32)])
+def test_gradient_codes_are_those_of_the_exact_products(dev, dtype, gates_dtype):
+    """2^20 products of gradient, gate and column scale: a code that lies 2^-22 of a step or more from a border goes to the nearer side.  (A product is held as an fp32 number and its
+    error, together off by 2^-46 of it.)"""
+    T, K, N, E, k = 1024, 48, 512, 4, 2
+    sei, ssi, eo, gw = oracle.route(T, E, k, 12)
+    g = torch.Generator().manual_seed(6)
+    w = torch.randint(-127, 128, (E, K, N), generator=g, dtype=torch.int8)
+    ws = torch.rand(E, N, generator=g) * 1e-3 + 1e-4
+    x, dout, gw = torch.randn(T, K, generator=g).to(dtype), torch.randn(T, N, generator=g).to(dtype), gw.to(gates_dtype)
+    want = oracle.linear(x, w, ws, k, sei, ssi, gw, dout, near=127 * 2.0 ** -29)
+    xd = x.to(dev).requires_grad_(True)
+    y = moe.parallel_linear_int8(xd, w.to(dev), ws.to(dev), k, sei.to(dev), ssi.to(dev), None, eo.to(dev), gw.to(dev))
+    dx = torch.autograd.grad(y, xd, dout.to(dev))[0]
+    close(dx, want["dx"], want["dx_slack"] + want["dx_terms"] * (6 + k) * 2.0 ** -24, dtype, "dx")
