@@ -222,11 +222,19 @@ class ScatterMoEBlock(nn.Module):
         """Puts 8-bit codes in the place of the expert weights, for serving and for training what lies before and around them:
         w1, w2, w3 become int8 buffers (E, f, d) with fp32 buffers ``w1_scale``, ``w2_scale``, ``w3_scale`` of their output
         columns, and ``forward`` takes the products over them (bf16 or fp16 hidden states, sizes that are multiples of 64).  The
-        router keeps its type.  Not for a block with adapters: its factors are trained against the weights as they are."""
+        router keeps its type.  Not for a block with adapters: its factors are trained against the weights as they are.  A block that
+        the products could not serve is refused and keeps its weights."""
         if self.lora_r > 0:
             raise ValueError("a block with adapters keeps its expert weights: quantize_experts() takes blocks with lora_r = 0")
         if self.is_quantized:
             return self
+        if self.router.dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f"the expert MLP over 8-bit weights takes bf16 or fp16 hidden states, this block's are {self.router.dtype}: "
+                             "convert the block first")
+        d, f = self.hidden_size, self.ffn_hidden_size
+        if d % 64 or f % 64 or max(d, f) >= 2 ** 17 or d * f >= 2 ** (31 if d % 128 or f % 128 else 32) - 16:
+            raise ValueError(f"the expert MLP over 8-bit weights takes sizes that are multiples of 64, below 2^17 and together below 2^32 (2^31 "
+                             f"where one is no multiple of 128), not hidden size {d} and ffn size {f}")
         q = Int8ExpertWeights.quantize(self.w1, self.w2, self.w3, self.ffn_hidden_size, self.hidden_size)
         for name, t in q._asdict().items():
             if hasattr(self, name):
