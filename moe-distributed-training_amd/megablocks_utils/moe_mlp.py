@@ -222,8 +222,9 @@ class ScatterMoEBlock(nn.Module):
         """Puts 8-bit codes in the place of the expert weights, for serving and for training what lies before and around them:
         w1, w2, w3 become int8 buffers (E, f, d) with fp32 buffers ``w1_scale``, ``w2_scale``, ``w3_scale`` of their output
         columns, and ``forward`` takes the products over them (bf16 or fp16 hidden states, sizes that are multiples of 64).  The
-        router keeps its type.  Not for a block with adapters: its factors are trained against the weights as they are.  A block that
-        the products could not serve is refused and keeps its weights."""
+        router keeps its type, and the block from then on: a conversion that would round the scales is refused.  Not for a block with
+        adapters: its factors are trained against the weights as they are.  A block that the products could not serve is refused and
+        keeps its weights."""
         if self.lora_r > 0:
             raise ValueError("a block with adapters keeps its expert weights: quantize_experts() takes blocks with lora_r = 0")
         if self.is_quantized:
@@ -245,6 +246,12 @@ class ScatterMoEBlock(nn.Module):
     @property
     def is_quantized(self) -> bool:
         return self.w1.dtype == torch.int8
+
+    def _apply(self, fn, *args, **kw):
+        # (what ``to``, ``half``, ``cuda`` and the like go through, also those of a module around this one)
+        if self.is_quantized and self.w1_scale.is_floating_point() and fn(self.w1_scale[:0]).dtype != self.w1_scale.dtype:
+            raise TypeError("the scales of a block with experts in 8 bits stay float32: choose the block's type before quantize_experts()")
+        return super()._apply(fn, *args, **kw)
 
     def forward(self, hidden_states: torch.Tensor):
         shape = hidden_states.shape

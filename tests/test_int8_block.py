@@ -1,4 +1,5 @@
-"""A block whose experts are to be held in 8 bits, on the host: what is refused before anything of the block changes."""
+"""A block whose experts are to be held in 8 bits, on the host: what is refused before anything of the block changes,
+and what a conversion leaves as it was."""
 import pytest
 import torch
 
@@ -19,3 +20,38 @@ def test_a_block_that_cannot_be_served_keeps_its_weights(match, kw):
     assert not block.is_quantized and list(dict(block.named_buffers())) == []
     after = dict(block.named_parameters())
     assert list(after) == list(before) and all(after[n] is p and p.dtype == dt for n, (p, dt) in before.items())
+
+
+def stand_in(dtype=BF16, E=2, f=128, d=64):
+    """A block with codes and scales as quantize_experts() leaves them."""
+    block = moe.ScatterMoEBlock(d, f, E, dtype=dtype)
+    g = torch.Generator().manual_seed(0)
+    for n, cols in (("w1", f), ("w2", d), ("w3", f)):
+        delattr(block, n)
+        block.register_buffer(n, torch.randint(-127, 128, (E, f, d), generator=g, dtype=torch.int8))
+        block.register_buffer(n + "_scale", torch.rand(E, cols, generator=g) * 1e-3)
+    assert block.is_quantized
+    return block
+
+
+@pytest.mark.parametrize("convert", [lambda m: m.to(BF16), lambda m: m.half(), lambda m: m.to("cpu", F16), lambda m: m.double(), lambda m: m.bfloat16()])
+@pytest.mark.parametrize("inside", [False, True])
+def test_a_conversion_does_not_round_the_scales(convert, inside):
+    block = stand_in()
+    before = {n: t.clone() for n, t in block.state_dict().items()}
+    with pytest.raises(TypeError, match="float32"):
+        convert(torch.nn.Sequential(block, torch.nn.Linear(4, 4)) if inside else block)
+    assert all(t.dtype == before[n].dtype and torch.equal(t, before[n]) for n, t in block.state_dict().items())
+
+
+def test_moves_and_conversions_that_keep_the_scales():
+    import copy
+    block = stand_in()
+    before = {n: t.clone() for n, t in block.state_dict().items()}
+    other = copy.deepcopy(block).to("cpu").cpu().requires_grad_(False).share_memory()
+    assert all(torch.equal(t, before[n]) and t.dtype == before[n].dtype for n, t in other.state_dict().items())
+    assert block.to("meta").w1_scale.dtype == F32 and block.to_empty(device="cpu").w2_scale.shape == (2, 64)
+    block.load_state_dict(before)
+    assert all(torch.equal(t, before[n]) for n, t in block.state_dict().items())
+    plain = moe.ScatterMoEBlock(64, 128, 2, dtype=F32).to(BF16).half()          # blocks with their weights convert as ever
+    assert plain.w1.dtype == F16
