@@ -182,7 +182,7 @@ struct MlpI8Fn : Function<MlpI8Fn> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& gates_, const I8Mlp& m, const Tensor& ssi, const Tensor& offsets, const MlpCfg& c)
     {
         const Tensor gates = val(gates_);
-        Tensor saved, y = mlp_int8_rows(x, m, c, ssi, offsets, &saved, gates.defined());
+        Tensor saved, y = mlp_int8_rows(x, m, c, ssi, offsets, x.requires_grad() ? &saved : nullptr, gates.defined());   // (only dx reads gate and up again)
         Tensor out = gates.defined() ? combine_rows(y, gates, gates.size(1), gates.size(0), x.scalar_type()) : y;
         ctx->save_for_backward({m.w[0], m.w[1], m.w[2], m.s[0], m.s[1], m.s[2], gates, ssi, offsets, saved, gates.defined() && gates.requires_grad() ? y : Tensor()});
         ctx->saved_data["fan_out"] = c.fan_out;

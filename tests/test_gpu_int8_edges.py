@@ -123,3 +123,25 @@ def test_gradient_codes_are_those_of_the_exact_products(dev, dtype, gates_dtype)
     y = moe.parallel_linear_int8(xd, w.to(dev), ws.to(dev), k, sei.to(dev), ssi.to(dev), None, eo.to(dev), gw.to(dev))
     dx = torch.autograd.grad(y, xd, dout.to(dev))[0]
     close(dx, want["dx"], want["dx_slack"] + want["dx_terms"] * (6 + k) * 2.0 ** -24, dtype, "dx")
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# what a backward pass keeps
+# ---------------------------------------------------------------------------------------------------------------
+def test_gates_alone_keep_no_gate_and_up(dev):
+    """The gradient of the gate weights needs the rows of y and nothing else of the MLP."""
+    T, d, f, E, k = 1024, 64, 4096, 4, 2
+    sei, ssi, eo, gw = oracle.route(T, E, k, 0)
+    w = moe.Int8ExpertWeights(*(t.to(dev) for t in mlp_weights(E, d, f, 1)))
+    g = torch.Generator().manual_seed(1)
+    x, dout, ssi, eo = torch.randn(T, d, generator=g).to(BF16).to(dev), torch.randn(T, d, generator=g).to(BF16).to(dev), ssi.to(dev), eo.to(dev)
+    both = x.clone().requires_grad_(True), gw.to(dev).requires_grad_(True)
+    want = torch.autograd.grad(moe.fused_expert_mlp_int8(both[0], w, k, ssi, eo, both[1]), both[1], dout)[0]
+    alone = gw.to(dev).requires_grad_(True)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    y = moe.fused_expert_mlp_int8(x, w, k, ssi, eo, alone)
+    held = torch.cuda.memory_allocated() - before
+    rows = T * k * d * 4 + T * d * 2                            # y's fp32 rows and the result
+    assert held < rows + (1 << 20), f"{held} bytes are held for the backward pass; gate and up would be {2 * T * k * f * 25 // 8}"
+    assert torch.equal(torch.autograd.grad(y, alone, dout)[0], want)
