@@ -1064,7 +1064,8 @@ int moe_quantize_rows(const void* src, int64_t lds, int dtype, int8_t* codes, in
 {
     if (dtype < 0 || dtype > 2 || nrows < 0 || ncols < 0 || ldc < ncols || ldc % 16 != 0) return MOE_ERR_BAD_ARG;
     if (nrows == 0) return MOE_OK;
-    if (lds < 0 || !src || !codes || !scale || !aligned16(codes)) return MOE_ERR_BAD_ARG;
+    // (rows of no columns have nothing to read, and of pitch 0 nothing but their scales to write)
+    if (lds < 0 || (!src && ncols > 0) || (!codes && ldc > 0) || !scale || !aligned16(codes)) return MOE_ERR_BAD_ARG;
     if (nrows > 0x7fffffff) return MOE_ERR_UNSUPPORTED;
     MoeQuantizeRows q = {};
     q.src = src; q.lds = lds; q.codes = codes; q.ldc = ldc; q.scale = scale; q.cols = ncols;

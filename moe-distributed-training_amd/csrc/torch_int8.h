@@ -30,8 +30,9 @@ variable_list quantize_rows(const Tensor& x_)
     dtype_code(x_);
     const c10::DeviceGuard guard(x_.device());
     const Tensor x = unit_inner(x_.detach());
-    Tensor q = at::empty({x.size(0), code_pitch(x.size(1))}, x.options().dtype(at::kChar)), scale = at::empty({x.size(0)}, x.options().dtype(at::kFloat));
-    check(moe_quantize_rows(ptr(x), x.stride(0), dtype_code(x), (int8_t*)ptr(q), q.stride(0), (float*)ptr(scale), x.size(0), x.size(1), stream_of(x)), "moe_quantize_rows");
+    const int64_t pitch = code_pitch(x.size(1));   // (0 for rows of no columns: the codes' own stride says 1)
+    Tensor q = at::empty({x.size(0), pitch}, x.options().dtype(at::kChar)), scale = at::empty({x.size(0)}, x.options().dtype(at::kFloat));
+    check(moe_quantize_rows(ptr(x), x.stride(0), dtype_code(x), (int8_t*)ptr(q), pitch, (float*)ptr(scale), x.size(0), x.size(1), stream_of(x)), "moe_quantize_rows");
     return {q.narrow(1, 0, x.size(1)), scale};
 }
 

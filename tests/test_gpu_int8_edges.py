@@ -126,7 +126,7 @@ def test_gradient_codes_are_those_of_the_exact_products(dev, dtype, gates_dtype)
 
 
 # ---------------------------------------------------------------------------------------------------------------
-# what a backward pass keeps
+# what a backward pass keeps, rows without columns
 # ---------------------------------------------------------------------------------------------------------------
 def test_gates_alone_keep_no_gate_and_up(dev):
     """The gradient of the gate weights needs the rows of y and nothing else of the MLP."""
@@ -145,3 +145,11 @@ def test_gates_alone_keep_no_gate_and_up(dev):
     rows = T * k * d * 4 + T * d * 2                            # y's fp32 rows and the result
     assert held < rows + (1 << 20), f"{held} bytes are held for the backward pass; gate and up would be {2 * T * k * f * 25 // 8}"
     assert torch.equal(torch.autograd.grad(y, alone, dout)[0], want)
+
+
+@pytest.mark.parametrize("rows", [0, 1, 5])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_rows_of_no_columns(dev, dtype, rows):
+    codes, scales = moe.quantize_rows(torch.empty(rows, 0, dtype=dtype, device=dev))
+    assert codes.shape == (rows, 0) and codes.dtype == torch.int8
+    assert torch.equal(scales.cpu(), torch.zeros(rows))
