@@ -1088,7 +1088,7 @@ int moe_combine_f32_dgates(const float* y, int64_t ldy, const void* dout, int64_
     hipStream_t st = S(stream);
     if (dtype < 0 || dtype > 2 || gates_dtype < 0 || gates_dtype > 2 || k < 1 || ntok < 0 || ncols < 0) return MOE_ERR_BAD_ARG;
     if (ntok == 0) return MOE_OK;
-    if (ldy < 0 || ldd < 0 || !y || !dout || !dgates) return MOE_ERR_BAD_ARG;
+    if (ldy < 0 || ldd < 0 || (ncols > 0 && (!y || !dout)) || !dgates) return MOE_ERR_BAD_ARG;   // (sums of no columns are zeros)
     if (ntok * k > 0x7fffffff) return MOE_ERR_UNSUPPORTED;
     TIMED("rows.combine_f32_dgates");
     return moe_launch_dgates_f32(y, ldy, dout, ldd, dtype, dgates, gates_dtype, k, ntok, ncols, st);

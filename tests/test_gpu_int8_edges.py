@@ -153,3 +153,16 @@ def test_rows_of_no_columns(dev, dtype, rows):
     codes, scales = moe.quantize_rows(torch.empty(rows, 0, dtype=dtype, device=dev))
     assert codes.shape == (rows, 0) and codes.dtype == torch.int8
     assert torch.equal(scales.cpu(), torch.zeros(rows))
+
+
+@pytest.mark.parametrize("gated", [False, True])
+def test_weights_of_no_output_columns(dev, gated):
+    """An empty sum for every gate, and zeros for the input."""
+    T, K, E, k = 6, 64, 3, 2
+    sei, ssi, eo, gw = (t.to(dev) for t in oracle.route(T, E, k, 0))
+    x = torch.ones(T, K, dtype=BF16, device=dev, requires_grad=True)
+    gates = gw.clone().requires_grad_(True) if gated else None
+    y = moe.parallel_linear_int8(x, torch.empty(E, K, 0, dtype=torch.int8, device=dev), torch.empty(E, 0, device=dev), k, sei, ssi, None, eo, gates)
+    assert y.shape == (T if gated else T * k, 0) and y.dtype == BF16
+    got = torch.autograd.grad(y, (x, gates) if gated else (x,), torch.empty_like(y))
+    assert all(torch.equal(g, torch.zeros_like(g)) for g in got)
