@@ -224,6 +224,9 @@ static inline int moe_device_cus()
     return n;
 }
 
+// whether a launch of one-dimensional workgroups can be enqueued: its threads are counted in 32 bits
+static inline bool moe_grid_fits(int64_t blocks, int64_t threads) { return blocks <= 0x7fffffff && blocks * threads < (int64_t)1 << 32; }
+
 static inline int moe_launch_status()
 {
     return hipGetLastError() == hipSuccess ? MOE_OK : MOE_ERR_LAUNCH;

@@ -59,12 +59,16 @@ Plan plan(int cus, int64_t R, int E, int64_t ktiles, int64_t N, bool pair)
 
 bool moe_i8_weights_ok(const void* W, int64_t swe, int64_t ldw) { return (uintptr_t)W % 16 == 0 && swe % 16 == 0 && ldw % 16 == 0; }
 
-// 32-bit byte offsets: gathered rows of X from its start (grouped ones from the tile's first row), one expert's matrix (2 GiB where its last K tile is masked)
+// 32-bit byte offsets: gathered rows of X from its start (grouped ones from the tile's first row), one expert's matrix (2 GiB where its last K tile is masked); and the
+// threads of the grid
 bool moe_i8_gemm_supported(const MoeI8Gemm& p, int64_t R, int64_t x_rows)
 {
-    (void)R;
     const int64_t rows = p.x_grouped ? BM : x_rows, limit = p.K % BK ? (int64_t)1 << 31 : (int64_t)1 << 32;
-    return rows * p.ldx < ((int64_t)1 << 32) && (p.nn ? (p.K - 1) * p.ldw + p.N : (p.N - 1) * p.ldw + p.K) + 16 < limit;
+    if (rows * p.ldx >= ((int64_t)1 << 32) || (p.nn ? (p.K - 1) * p.ldw + p.N : (p.N - 1) * p.ldw + p.K) + 16 >= limit) return false;
+    const bool pair = p.epi == MOE_I8_SWIGLU;
+    const int cus = plan_cus();
+    auto fits = [&](int tile) { return moe_grid_fits(tiles_at_most(tile, R, p.E, p.N, pair) + (256 / tile) * cus + NXCD, 2 * tile); };   // (as plan_grid has it, or a few more)
+    return fits(128) || fits(plan(cus, R, p.E, (p.K + BK - 1) / BK * p.nseg, p.N, pair).tile);
 }
 
 // Where a launch's split tiles meet: `zeros` ints, a counter per workgroup of a round (tiles of 128 have twice those of 256) and, for tiles of 128, the matrix of

@@ -553,7 +553,7 @@ template <bool NN, int EPI, bool KTAIL> int launch_typed(const MoeI8Gemm& p, int
     q.num_cus = WGS_PER_CU * p.num_cus;
     const int cols = EPI == MOE_I8_SWIGLU ? BN / 2 : BN;
     const int64_t grid = plan_grid(R, p.E, (int)((p.N + cols - 1) / cols), q.num_cus);
-    if (grid > 0x7fffffff) return MOE_ERR_UNSUPPORTED;
+    if (!moe_grid_fits(grid, NTHREADS)) return MOE_ERR_UNSUPPORTED;
     hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(NTHREADS), LDS_BYTES, stream, q);
     return moe_launch_status();
 }

@@ -496,11 +496,21 @@ __global__ void zero_u32_kernel(uint32_t* p, int64_t n)
     if (i < n) p[i] = 0;
 }
 
+// threads of a workgroup: pieces of 8 columns, one to four of them a thread
+int quantize_threads(int64_t rows, int64_t ldc)
+{
+    const int64_t pieces = (ldc + 7) / 8;
+    return pieces <= 64 ? 64 : pieces <= 128 ? 128 : pieces <= 256 || (pieces <= 1024 && rows > 256) ? 256 : pieces <= 512 || (pieces <= 2048 && rows > 256) ? 512 : 1024;
+}
+int64_t quantize_blocks(int64_t rows, int64_t zero_n) { return rows + (zero_n + ZERO_PIECE - 1) / ZERO_PIECE; }
+// (few rows: latency is all of it, and more threads have less each)
+int requantize_threads(int64_t rows, int64_t ldc) { return ldc / 8 <= 64 ? 64 : ldc / 8 <= 128 ? 128 : rows > 256 || ldc / 8 <= 256 ? 256 : ldc / 8 <= 512 ? 512 : 1024; }
+int swiglu_bwd_threads(int64_t f) { return f / 8 <= 64 ? 64 : f / 8 <= 128 ? 128 : f / 8 <= 256 ? 256 : 512; }
+
 template <typename T, bool SCALED> int launch_quantize_t(const MoeQuantizeRows& p, int64_t rows, hipStream_t stream)
 {
-    // pieces of 8 columns: one to four of them a thread
-    const int64_t pieces = (p.ldc + 7) / 8, grid = rows + (p.zero_n + ZERO_PIECE - 1) / ZERO_PIECE;
-    const int nt = pieces <= 64 ? 64 : pieces <= 128 ? 128 : pieces <= 256 || (pieces <= 1024 && rows > 256) ? 256 : pieces <= 512 || (pieces <= 2048 && rows > 256) ? 512 : 1024;
+    const int64_t pieces = (p.ldc + 7) / 8, grid = quantize_blocks(rows, p.zero_n);
+    const int nt = quantize_threads(rows, p.ldc);
     const int64_t keep = (pieces + nt - 1) / nt;
     if (keep <= 1) hipLaunchKernelGGL((quantize_rows_kernel<T, SCALED, 1>), dim3((unsigned)grid), dim3(nt), 0, stream, p);
     else if (keep <= 2) hipLaunchKernelGGL((quantize_rows_kernel<T, SCALED, 2>), dim3((unsigned)grid), dim3(nt), 0, stream, p);
@@ -510,6 +520,11 @@ template <typename T, bool SCALED> int launch_quantize_t(const MoeQuantizeRows& 
 }
 
 }  // namespace
+
+bool moe_quantize_rows_supported(int64_t rows, int64_t ldc, int64_t zero_n) { return moe_grid_fits(quantize_blocks(rows, zero_n), quantize_threads(rows, ldc)); }
+bool moe_requantize_rows_supported(int64_t rows, int64_t ldc) { return moe_grid_fits(rows, requantize_threads(rows, ldc)); }
+bool moe_swiglu_bwd_codes_supported(int64_t rows, int64_t f) { return moe_grid_fits(rows, swiglu_bwd_threads(f)); }
+bool moe_pack_codes_supported(int64_t N) { return (N + 63) / 64 <= 65535; }
 
 int moe_launch_quantize_rows(const MoeQuantizeRows& p_, int dtype, int64_t rows, hipStream_t stream)
 {
@@ -527,8 +542,7 @@ int moe_launch_quantize_rows(const MoeQuantizeRows& p_, int dtype, int64_t rows,
 int moe_launch_requantize_rows(const uint8_t* src, const float* seg, int64_t rows, int64_t cols, int8_t* codes, int64_t ldc, float* scale, hipStream_t stream)
 {
     if (rows == 0) return MOE_OK;
-    // (few rows: latency is all of it, and more threads have less each)
-    const int nt = ldc / 8 <= 64 ? 64 : ldc / 8 <= 128 ? 128 : rows > 256 || ldc / 8 <= 256 ? 256 : ldc / 8 <= 512 ? 512 : 1024;
+    const int nt = requantize_threads(rows, ldc);
     hipLaunchKernelGGL(requantize_rows_kernel, dim3((unsigned)rows), dim3(nt), 0, stream, src, seg, cols, codes, ldc, scale);
     return moe_launch_status();
 }
@@ -537,7 +551,7 @@ int moe_launch_swiglu_bwd_codes(const MoeSwigluBwdCodes& p, int64_t rows, hipStr
 {
     if (rows == 0) return MOE_OK;
     const int64_t pieces = p.f / 8;
-    const int nt = pieces <= 64 ? 64 : pieces <= 128 ? 128 : pieces <= 256 ? 256 : 512;
+    const int nt = swiglu_bwd_threads(p.f);
     const int64_t keep = (pieces + nt - 1) / nt;
     if (keep <= 1 && nt <= 256) hipLaunchKernelGGL(swiglu_bwd_codes_kernel<1>, dim3((unsigned)rows), dim3(nt), 0, stream, p);
     else if (keep <= 2) hipLaunchKernelGGL(swiglu_bwd_codes_kernel<2>, dim3((unsigned)rows), dim3(nt), 0, stream, p);
@@ -578,7 +592,8 @@ int moe_launch_combine_f32(const float* y, int64_t ldy, void* out, int64_t ldo, 
     if (ntok == 0 || ncols == 0) return MOE_OK;
     // (few tokens: the columns of one are dealt to several workgroups)
     const int64_t pieces = (ncols + 1023) / 1024;
-    const dim3 grid((unsigned)ntok, (unsigned)(ntok < 1024 ? pieces : (pieces + 3) / 4));
+    const int64_t parts = ntok < 1024 ? pieces : (pieces + 3) / 4;
+    const dim3 grid((unsigned)ntok, (unsigned)(parts < 65535 ? parts : 65535));
     MOE_DISPATCH_DTYPE(dtype, {
         const int vec = ncols % 4 == 0 && ldy % 4 == 0 && ldo % 4 == 0 && (uintptr_t)y % 16 == 0 && (uintptr_t)out % (4 * sizeof(T)) == 0;
         hipLaunchKernelGGL(combine_f32_kernel<T>, grid, dim3(256), 0, stream, y, ldy, (T*)out, ldo, gates, gdtype, k, ncols, vec);

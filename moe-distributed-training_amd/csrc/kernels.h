@@ -251,6 +251,12 @@ int moe_launch_pack_codes(const int8_t* W, int64_t swe, int64_t swk, int64_t swn
 int moe_launch_quantize_weights(const void* W, int64_t swe, int64_t swk, int64_t swn, int dtype, int E, int64_t K, int64_t N, int8_t* codes, int64_t sce,
                                 int64_t sck, int64_t scn, float* scale, uint32_t* top, hipStream_t stream);
 
+// whether launches over so many rows can be enqueued: asked before the first launch of a call
+bool moe_quantize_rows_supported(int64_t rows, int64_t ldc, int64_t zero_n);
+bool moe_requantize_rows_supported(int64_t rows, int64_t ldc);
+bool moe_swiglu_bwd_codes_supported(int64_t rows, int64_t f);
+bool moe_pack_codes_supported(int64_t N);
+
 int moe_launch_combine_f32(const float* y, int64_t ldy, void* out, int64_t ldo, int dtype, const void* gates, int gdtype, int k, int64_t ntok, int64_t ncols, hipStream_t stream);
 int moe_launch_dgates_f32(const float* y, int64_t ldy, const void* dout, int64_t ldd, int dtype, void* dgates, int gdtype, int k, int64_t ntok, int64_t ncols, hipStream_t stream);
 
@@ -282,7 +288,7 @@ constexpr int MOE_I8_MIN_PART = 4;
 int moe_launch_i8_gemm_small(const MoeI8Gemm& p, int64_t R, hipStream_t stream);
 // whether the kernel reads W in this orientation and alignment (otherwise: moe_launch_pack_codes first)
 bool moe_i8_weights_ok(const void* W, int64_t swe, int64_t ldw);
-// whether sizes stay inside the kernel's 32-bit offsets (x_rows: rows of X)
+// whether sizes stay inside the kernel's 32-bit offsets (x_rows: rows of X) and the launch can be enqueued
 bool moe_i8_gemm_supported(const MoeI8Gemm& p, int64_t R, int64_t x_rows);
 struct MoeI8Exchange { int64_t zeros, slots; };   // ints
 MoeI8Exchange moe_i8_exchange(int64_t R, int E, int64_t K, int64_t N, bool pair);   // K: all segments

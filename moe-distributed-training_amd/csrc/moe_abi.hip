@@ -1066,7 +1066,7 @@ int moe_quantize_rows(const void* src, int64_t lds, int dtype, int8_t* codes, in
     if (nrows == 0) return MOE_OK;
     // (rows of no columns have nothing to read, and of pitch 0 nothing but their scales to write)
     if (lds < 0 || (!src && ncols > 0) || (!codes && ldc > 0) || !scale || !aligned16(codes)) return MOE_ERR_BAD_ARG;
-    if (nrows > 0x7fffffff) return MOE_ERR_UNSUPPORTED;
+    if (!moe_quantize_rows_supported(nrows, ldc, 0)) return MOE_ERR_UNSUPPORTED;
     MoeQuantizeRows q = {};
     q.src = src; q.lds = lds; q.codes = codes; q.ldc = ldc; q.scale = scale; q.cols = ncols;
     return moe_launch_quantize_rows(q, dtype, nrows, S(stream));
@@ -1078,7 +1078,7 @@ int moe_combine_f32(const float* y, int64_t ldy, void* out, int64_t ldo, int dty
     if (dtype < 0 || dtype > 2 || k < 1 || ntok < 0 || ncols < 0 || (gates && (gates_dtype < 0 || gates_dtype > 2))) return MOE_ERR_BAD_ARG;
     if (ntok == 0 || ncols == 0) return MOE_OK;
     if (ldy < 0 || (ntok > 1 && ldo < ncols) || !y || !out) return MOE_ERR_BAD_ARG;
-    if (ntok > 0x7fffffff) return MOE_ERR_UNSUPPORTED;
+    if (!moe_grid_fits(ntok, 256)) return MOE_ERR_UNSUPPORTED;
     TIMED("rows.combine_f32");
     return moe_launch_combine_f32(y, ldy, out, ldo, dtype, gates, gates_dtype, k, ntok, ncols, st);
 }
@@ -1089,7 +1089,7 @@ int moe_combine_f32_dgates(const float* y, int64_t ldy, const void* dout, int64_
     if (dtype < 0 || dtype > 2 || gates_dtype < 0 || gates_dtype > 2 || k < 1 || ntok < 0 || ncols < 0) return MOE_ERR_BAD_ARG;
     if (ntok == 0) return MOE_OK;
     if (ldy < 0 || ldd < 0 || (ncols > 0 && (!y || !dout)) || !dgates) return MOE_ERR_BAD_ARG;   // (sums of no columns are zeros)
-    if (ntok * k > 0x7fffffff) return MOE_ERR_UNSUPPORTED;
+    if (ntok > 0x7fffffff || !moe_grid_fits(ntok * k, 256)) return MOE_ERR_UNSUPPORTED;
     TIMED("rows.combine_f32_dgates");
     return moe_launch_dgates_f32(y, ldy, dout, ldd, dtype, dgates, gates_dtype, k, ntok, ncols, st);
 }
@@ -1137,7 +1137,8 @@ int i8_linear(MoeQuantizeRows q, MoeI8Gemm g, int dtype, const I8Weights& w, con
     g.W[0] = copy ? copy : W; g.swe = w.swe; g.ldw = w.ldw; g.nn = w.nn; g.nseg = 1;
     I8Exchange(moe_i8_exchange(R, g.E, g.K, g.N, false)).take(b, q, g);
     g.epi = MOE_I8_STORE;
-    if (!moe_i8_gemm_supported(g, R, code_rows)) return MOE_ERR_UNSUPPORTED;
+    if (!moe_i8_gemm_supported(g, R, code_rows) || !moe_quantize_rows_supported(code_rows, pitch, q.zero_n)) return MOE_ERR_UNSUPPORTED;
+    if (w.copy == 2 && !moe_pack_codes_supported(g.N)) return MOE_ERR_UNSUPPORTED;
     { TIMED("i8_codes"); TRY(moe_launch_quantize_rows(q, dtype, code_rows, st)); }
     if (w.copy) {
         TIMED("i8_weights_copy");
@@ -1263,6 +1264,7 @@ int moe_mlp_int8_fwd(const void* x, int64_t ldx, int64_t x_rows, int dtype, cons
     MoeQuantizeRows q = {};
     q.src = x; q.lds = ldx; q.codes = xq; q.ldc = dp; q.scale = xs; q.cols = d;
     i8_mlp_exchange(R, E, d, f, false).take(b, q, g, g2);
+    if (!moe_quantize_rows_supported(x_rows, dp, q.zero_n) || !moe_requantize_rows_supported(R, fp)) return MOE_ERR_UNSUPPORTED;
     { TIMED("i8_codes_x"); TRY(moe_launch_quantize_rows(q, dtype, x_rows, st)); }
     { TIMED("i8_gemm_gate_up"); TRY(moe_launch_i8_gemm(g, R, st)); }
     { TIMED("i8_codes_h"); TRY(moe_launch_requantize_rows(h.v, h.s, R, f, hq, fp, hs, st)); }
@@ -1311,6 +1313,7 @@ int moe_mlp_int8_bwd(const void* dy, int64_t lddy, int dtype, int dy_grouped, in
     q.src = dy; q.lds = lddy; q.pos = dy_grouped ? nullptr : pos; q.pos64 = pos64; q.fan_out = dy_fan_out; q.coeff = gates; q.coeff_dtype = gates_dtype;
     q.col_scale = s2; q.offsets = offsets; q.off64 = off64; q.E = E; q.codes = gq; q.ldc = dp; q.scale = gs; q.cols = d;
     i8_mlp_exchange(R, E, d, f, true).take(b, q, g, g2);
+    if (!moe_quantize_rows_supported(R, dp, q.zero_n) || !moe_swiglu_bwd_codes_supported(R, f)) return MOE_ERR_UNSUPPORTED;
     const MoeSwigluBwdCodes a = {dh.v, gate.v, up.v, dh.s, gate.s, up.s, s1, s3, offsets, off64, E, aq, fp, as, f};
     { TIMED("i8_codes_dy"); TRY(moe_launch_quantize_rows(q, dtype, R, st)); }
     { TIMED("i8_gemm_dh"); TRY(moe_launch_i8_gemm(g, R, st)); }
