@@ -1,6 +1,8 @@
 // Part of torch_layer.cpp: the expert products over 8-bit weights as autograd functions.  The weights are frozen; gradients of the input and of the gate
 // weights go straight through the rounding to codes.
 
+constexpr int64_t MAX_SUM = 1 << 17;   // products of codes in one sum of 32 bits, fewer than
+
 inline int64_t code_pitch(int64_t cols) { return (cols + 127) / 128 * 128; }
 
 // Rows that are summed per token stay fp32 until then (sums: whether they are).
@@ -156,6 +158,7 @@ Tensor linear_int8(const Tensor& x_, const Tensor& W, const Tensor& scale_, int6
     const Tensor x = unit_inner(x_), scale = scale_.contiguous(), ssi = ssi_.contiguous(), eo = eo_.defined() ? eo_.contiguous() : offsets_from_sorted(sei, W.size(0));
     const Tensor gates = gates_.defined() ? gates_.contiguous() : Tensor();
     const LinearCfg c{0.0, 0.0, k, grouped_in, grouped_out};
+    TORCH_CHECK(!needs_node({&x}) || W.size(2) < MAX_SUM, "the gradient of X is a sum over the ", W.size(2), " output columns: exact for fewer than ", MAX_SUM);
     if (needs_node({&x, &gates})) return LinearI8Fn::apply(x, opt(gates), W, scale, ssi, eo, c);
     Tensor y = linear_int8_rows(x, W, scale, ssi, eo, c, gates.defined());
     return gates.defined() ? combine_rows(y, gates, gates.size(1), gates.size(0), x.scalar_type()) : y;
@@ -258,6 +261,7 @@ Tensor expert_mlp_int8(const Tensor& x_, const Tensor& w1, const Tensor& s1, con
     if (needs_node({&x, &gates})) {
         // rows of dx lie at their positions: each is written once only where the positions are a permutation of all of x's assignments
         TORCH_CHECK(ssi.numel() == x.size(0) * fan_out, "gradients need one position for each of the ", x.size(0) * fan_out, " assignments, got ", ssi.numel());
+        TORCH_CHECK(!needs_node({&x}) || 2 * w1.size(1) < MAX_SUM, "the gradient of x is a sum over twice the ", w1.size(1), " ffn columns: exact for fewer than ", MAX_SUM);
         return MlpI8Fn::apply(x, opt(gates), m, ssi, offsets, c);
     }
     Tensor y = mlp_int8_rows(x, m, c, ssi, offsets, nullptr, gates.defined());

@@ -1,5 +1,16 @@
-"""What the C entries of the 8-bit expert products refuse on the host, at the ends of their sizes (16: non-null stand-ins that are never dereferenced)."""
+"""What the 8-bit expert products refuse on the host, at the ends of their sizes (C entries: 16 are non-null stand-ins that are never dereferenced; tensors are fakes that only
+claim to lie on a GPU)."""
+import warnings
+
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+import moe_distributed_training_amd as moe
 from moe_distributed_training_amd._lib import lib
+
+BF16, F32, I8, I32 = torch.bfloat16, torch.float32, torch.int8, torch.int32
+_MODE = FakeTensorMode(allow_non_fake_inputs=True)
 
 
 def test_rows_of_no_columns_need_their_scales_only():
@@ -33,3 +44,24 @@ def test_more_threads_than_a_grid_counts_are_refused():
     def mlp_bwd(R, f):
         return lib.moe_mlp_int8_bwd(16, 64, 0, 0, 1, None, 0, 16, 16, 16, 16, 16, 16, 16, n, 16, 64, 0, 16, 0, 16, 0, 2, R, 64, f, 16, n, None)
     assert mlp_bwd(1 << 23, 8192) == unsupported                               # codes of dgate and dup, 512 threads
+
+
+def _fake(*shape, dtype=BF16, grad=False):
+    with _MODE:
+        return torch.empty(shape, dtype=dtype, device="cuda:0", requires_grad=grad)
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="a fake's pointer must not reach a kernel")
+def test_a_gradient_that_could_not_be_taken_is_refused_with_the_forward_call():
+    idx = _fake(4, dtype=I32)
+    with warnings.catch_warnings():
+        warnings.simplefilter("ignore")   # (a fake's data pointer)
+        N = 1 << 17
+        args = (_fake(2, 64, N, dtype=I8), _fake(2, N, dtype=F32), 2, idx, idx, None, _fake(2, dtype=I32))
+        with pytest.raises(RuntimeError, match="output columns"):
+            moe.parallel_linear_int8(_fake(2, 64, grad=True), *args)
+        f = 1 << 16
+        codes = [_fake(2, f, 64, dtype=I8) for _ in range(3)]
+        w = moe.Int8ExpertWeights(codes[0], _fake(2, f, dtype=F32), codes[1], _fake(2, 64, dtype=F32), codes[2], _fake(2, f, dtype=F32))
+        with pytest.raises(RuntimeError, match="ffn columns"):
+            moe.fused_expert_mlp_int8(_fake(2, 64, grad=True), w, 2, idx, _fake(2, dtype=I32))
