@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define MOE_HIP_ABI_VERSION 3   /* 3: expert products in 8-bit integers; 2: router weight gradient, static-scratch sort, stage-timer selection, moe_combine with k = 0; fp16 on the matrix cores (dtype argument of moe_mlp_fwd / moe_mlp_bwd) */
+#define MOE_HIP_ABI_VERSION 4   /* 4: moe_int8_debug_tile; 3: expert products in 8-bit integers; 2: router weight gradient, static-scratch sort, stage-timer selection, moe_combine with k = 0; fp16 on the matrix cores (dtype argument of moe_mlp_fwd / moe_mlp_bwd) */
 
 #define MOE_OK 0
 #define MOE_ERR_BAD_ARG (-1)      /* inconsistent sizes / null pointers */
@@ -259,6 +259,9 @@ int moe_mlp_bwd(const void* dy, int64_t lddy, int dy_grouped, int dy_fan_out, co
  *
  * moe_quantize_rows: rows of src -> codes (pitch ldc >= ncols, a multiple of 16, 16-byte aligned; columns from ncols on are written as zeros) and scales. */
 int moe_quantize_rows(const void* src, int64_t lds, int dtype, int8_t* codes, int64_t ldc, float* scale, int64_t nrows, int64_t ncols, void* stream);
+/* The tile size (128 or 256) that a product of R rows of E experts, nseg segments of K inputs and N columns takes on this device (pair != 0: gate and up side by side, half the
+ * columns of each per tile), and in `parts` (host memory, or NULL) how many parts the K range of a tile of the last, partial round may be cut into: the most that fit the round. */
+int moe_int8_debug_tile(int64_t R, int E, int64_t K, int64_t N, int pair, int nseg, int* parts);
 /* moe_combine and moe_combine_dgates of fp32 rows in token order and an output, or dout, of `dtype`: out[t] = sum_j gates[t*k+j] * y[t*k+j] (gates NULL: 1),
  * d_gates[t*k+j] = <y[t*k+j], dout[t]>. */
 int moe_combine_f32(const float* y, int64_t ldy, void* out, int64_t ldo, int dtype, const void* gates, int gates_dtype, int k, int64_t ntok,

@@ -10,7 +10,7 @@ import torch
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libmoe_hip.so")
 
-ABI_VERSION = 3   # MOE_HIP_ABI_VERSION of include/moe_hip.h this binding was written against
+ABI_VERSION = 4   # MOE_HIP_ABI_VERSION of include/moe_hip.h this binding was written against
 MOE_BF16, MOE_F16, MOE_F32 = 0, 1, 2
 _DTYPES = {torch.bfloat16: MOE_BF16, torch.float16: MOE_F16, torch.float32: MOE_F32}
 
@@ -62,6 +62,7 @@ _SIGNATURES = {
     "moe_mlp_saved_bytes": ("z", "li"),
     "moe_mlp_fwd": ("i", "pl" + "ppp" + "pp" + "if" + "pppp" + "l" + "pi" + "pi" + "i" + "lll" + "iii" + "p" + "pzp"),
     "moe_mlp_bwd": ("i", "plii" + "p" + "pl" + "ppp" + "pp" + "pp" + "if" + "ppp" + "pp" + "pli" + "pi" + "pi" + "i" + "lll" + "ii" + "p" + "pzp"),
+    "moe_int8_debug_tile": ("i", "lillii" + "p"),
     "moe_quantize_rows": ("i", "plipl" + "pll" + "p"),
     "moe_quantize_weights_workspace_bytes": ("z", "il"),
     "moe_quantize_weights": ("i", "plll" + "iill" + "plll" + "p" + "pzp"),

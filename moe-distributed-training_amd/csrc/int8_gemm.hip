@@ -84,6 +84,13 @@ MoeI8Exchange moe_i8_exchange(int64_t R, int E, int64_t K, int64_t N, bool pair)
     return {counters(cus), (all < cus ? all : cus) * BM * BN};
 }
 
+int moe_i8_tile(int64_t R, int E, int64_t K, int64_t N, bool pair, int nseg, int* parts)
+{
+    const Plan pl = plan(plan_cus(), R, E, (K + BK - 1) / BK * nseg, N, pair);
+    if (parts) *parts = pl.split;
+    return pl.tile;
+}
+
 int moe_launch_i8_gemm(const MoeI8Gemm& p_, int64_t R, hipStream_t stream)
 {
     if (R == 0 || p_.N == 0) return MOE_OK;

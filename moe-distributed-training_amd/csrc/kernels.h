@@ -292,4 +292,5 @@ bool moe_i8_weights_ok(const void* W, int64_t swe, int64_t ldw);
 bool moe_i8_gemm_supported(const MoeI8Gemm& p, int64_t R, int64_t x_rows);
 struct MoeI8Exchange { int64_t zeros, slots; };   // ints
 MoeI8Exchange moe_i8_exchange(int64_t R, int E, int64_t K, int64_t N, bool pair);   // K: all segments
+int moe_i8_tile(int64_t R, int E, int64_t K, int64_t N, bool pair, int nseg, int* parts);   // the tile size of a launch, and how many K parts its tiles may be cut into
 int moe_launch_i8_gemm(const MoeI8Gemm& p, int64_t R, hipStream_t stream);

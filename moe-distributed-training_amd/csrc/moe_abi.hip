@@ -1060,6 +1060,11 @@ int moe_mlp_bwd(const void* dy, int64_t lddy, int dy_grouped, int dy_fan_out, co
 }
 
 // ---- expert products in 8-bit integers -------------------------------------------------------------------------
+int moe_int8_debug_tile(int64_t R, int E, int64_t K, int64_t N, int pair, int nseg, int* parts)
+{
+    return R < 1 || E < 1 || K < 1 || N < 1 || nseg < 1 ? MOE_ERR_BAD_ARG : moe_i8_tile(R, E, K, N, pair != 0, nseg, parts);
+}
+
 int moe_quantize_rows(const void* src, int64_t lds, int dtype, int8_t* codes, int64_t ldc, float* scale, int64_t nrows, int64_t ncols, void* stream)
 {
     if (dtype < 0 || dtype > 2 || nrows < 0 || ncols < 0 || ldc < ncols || ldc % 16 != 0) return MOE_ERR_BAD_ARG;

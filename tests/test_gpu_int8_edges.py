@@ -126,7 +126,7 @@ def test_gradient_codes_are_those_of_the_exact_products(dev, dtype, gates_dtype)
 
 
 # ---------------------------------------------------------------------------------------------------------------
-# what a backward pass keeps, rows without columns
+# what a backward pass keeps, rows without columns, scales anywhere
 # ---------------------------------------------------------------------------------------------------------------
 def test_gates_alone_keep_no_gate_and_up(dev):
     """The gradient of the gate weights needs the rows of y and nothing else of the MLP."""
@@ -166,3 +166,22 @@ def test_weights_of_no_output_columns(dev, gated):
     assert y.shape == (T if gated else T * k, 0) and y.dtype == BF16
     got = torch.autograd.grad(y, (x, gates) if gated else (x,), torch.empty_like(y))
     assert all(torch.equal(g, torch.zeros_like(g)) for g in got)
+
+
+def test_scales_at_any_address(dev):
+    """Scales that are part of a larger tensor begin at any multiple of 4 bytes."""
+    T, d, f, E, k = 90, 128, 192, 3, 2
+    sei, ssi, eo, gates = (t.to(dev) for t in oracle.route(T, E, k, 0))
+    w = moe.Int8ExpertWeights(*(t.to(dev) for t in mlp_weights(E, d, f, 1)))
+
+    def moved(t, by):
+        big = torch.zeros(t.numel() + by, dtype=t.dtype, device=dev)
+        return big[by:].view(t.shape).copy_(t)
+    odd = w._replace(w1_scale=moved(w.w1_scale, 1), w2_scale=moved(w.w2_scale, 2), w3_scale=moved(w.w3_scale, 3))
+    x = torch.randn(T, d, generator=torch.Generator().manual_seed(1)).to(BF16).to(dev)
+
+    def step(weights):
+        a, b = x.clone().requires_grad_(True), gates.clone().requires_grad_(True)
+        y = moe.fused_expert_mlp_int8(a, weights, k, ssi, eo, b)
+        return [y.detach(), *torch.autograd.grad(y, (a, b), torch.ones_like(y))]
+    assert all(torch.equal(a, b) for a, b in zip(step(odd), step(w)))

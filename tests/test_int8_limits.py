@@ -1,5 +1,6 @@
 """What the 8-bit expert products refuse on the host, at the ends of their sizes (C entries: 16 are non-null stand-ins that are never dereferenced; tensors are fakes that only
 claim to lie on a GPU)."""
+import ctypes
 import warnings
 
 import pytest
@@ -65,3 +66,21 @@ def test_a_gradient_that_could_not_be_taken_is_refused_with_the_forward_call():
         w = moe.Int8ExpertWeights(codes[0], _fake(2, f, dtype=F32), codes[1], _fake(2, 64, dtype=F32), codes[2], _fake(2, f, dtype=F32))
         with pytest.raises(RuntimeError, match="ffn columns"):
             moe.fused_expert_mlp_int8(_fake(2, 64, grad=True), w, 2, idx, _fake(2, dtype=I32))
+
+
+def test_tiles_and_parts_of_known_sizes():
+    """What products take on 256 compute units (which a host without a GPU plans for): gate and up, h W2, dh, and dx over two segments."""
+    def plan(R, E, K, N, pair=0, nseg=1):
+        parts = ctypes.c_int(0)
+        return lib.moe_int8_debug_tile(R, E, K, N, pair, nseg, ctypes.addressof(parts)), parts.value
+
+    def mlp(R, E, d, f):
+        return plan(R, E, d, f, 1), plan(R, E, f, d), plan(R, E, d, f), plan(R, E, f, d, 0, 2)
+    assert plan(8192, 8, 4096, 14336, 1) == (lib.moe_int8_debug_tile(8192, 8, 4096, 14336, 1, 1, None), 2)
+    assert mlp(2, 8, 4096, 14336) == ((128, 1), (128, 4), (128, 1), (128, 4))                  # one token, two experts
+    assert mlp(48, 8, 4096, 14336) == ((128, 1),) * 4                                          # 24 tokens
+    assert mlp(666, 8, 4096, 14336) == ((128, 1),) * 4                                         # 333
+    assert mlp(8192, 8, 4096, 14336) == ((256, 2), (256, 4), (256, 2), (256, 4))               # 4096
+    assert mlp(16384, 64, 2048, 1024) == ((256, 1),) * 4                                       # many narrow experts
+    assert plan(500, 1, 14336, 4096) == (256, 4) and plan(64, 1, 14336, 4096)[0] == 256 and plan(4, 1, 14336, 4096) == (128, 8)
+    assert lib.moe_int8_debug_tile(0, 8, 64, 64, 0, 1, None) == -1 and lib.moe_int8_debug_tile(8, 8, 64, 64, 0, 0, None) == -1
