@@ -24,9 +24,17 @@ int64_t tiles_at_most(int tile, int64_t R, int E, int64_t N, bool pair)
 //   - a chain of K tiles per workgroup, 550 + 1.2 per row of the tile for tiles of 128 (two workgroups per compute unit) and 750 + 1.8 for 256, times the rounds;
 //   - at least the weights at 6 TB/s;
 //   - where tiles are cut, the meeting of the parts: sums by atomics at 80 per ns (128), or slots written and read at 2.5 TB/s behind fences of 8 us (256).
-// Measured (d=4096, f=14336; us, [tile, parts] and the estimate in brackets): h W2 of 4 rows of one expert [128, 8] 19 (20), [128, 1] 61 (68), [256, 8] 29 (26); of 64 rows
-// [128, 8] 43 (46), [256, 8] 40 (33), [128, 1] 71 (76); of 500 [128, 1] 61 (78), [256, 8] 85 (80); 48 rows of 8 experts [128, 1] 83 (87), [256, 4] 92; gate/up of
-// 666 rows of 8 [128, 1] 200 (163), [256, 1] 187.  Where the chip is full anyway (a round of tiles or more) only tiles of 256 are cut, into parts of 16 K tiles at least: those of
+// Measured and, in brackets, estimated (us; f=14336, d=4096), [tile, parts]; * what the rule takes:
+//   h W2, 2 rows of 2 experts   *[128, 4] 24 (23)    [128, 8] 25 (23)   [128, 1] 57 (62)   [256, 8] 33 (28)
+//         4 rows of 1           *[128, 8] 17 (14)    [128, 4] 22 (19)   [128, 1] 56 (62)   [256, 8] 27 (19)
+//         64 rows of 1          *[256, 8] 35 (27)    [128, 4] 37 (34)   [128, 8] 40 (39)   [128, 1] 66 (70)
+//         500 rows of 1         *[256, 4] 64 (68)    [256, 8] 82 (77)   [128, 1] 59 (79): 8 % slower than it could be
+//         48 rows of 8          *[128, 1] 82 (78)    [256, 1] 99 (85)
+//         666 rows of 8         *[128, 1] 97 (78)    [256, 4] 110 (-)   [256, 1] 132 (101)
+//   gate/up, 666 rows of 8      *[128, 1] 212 (157)  [256, 1] 189 (157): both at the weights' time, and the first of equals is taken, here the slower one
+//   gate/up, 16384 rows of 64, 2048 x 1024   *[256, 1] 107 (45)  [128, 1] 141 (45);   their h W2  *[256, 1] 73 (22)  [128, 1] 95 (23)
+// The estimate knows neither what a tile costs before its first K tile nor how ragged the groups are: of many small tiles it says far too little, of both sizes alike.
+// Where the chip is full anyway (a round of tiles or more) only tiles of 256 are cut, into parts of 16 K tiles at least: those of
 // the last round (dX of 8192 rows of 2 experts 903 us uncut, 752 cut; dh, whose K is 32 tiles, 485 uncut, 510 in parts of 4).
 struct Plan { int tile, split; };
 Plan plan(int cus, int64_t R, int E, int64_t ktiles, int64_t N, bool pair)

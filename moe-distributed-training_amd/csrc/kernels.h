@@ -262,7 +262,7 @@ int moe_launch_dgates_f32(const float* y, int64_t ldy, const void* dout, int64_t
 
 // epilogues of the 8-bit grouped product
 #define MOE_I8_STORE 0      // Y = acc * x_scale * w_scale in ydtype
-#define MOE_I8_SEG 1        // the same as segments (grouped rows)
+#define MOE_I8_SEG 1        // acc * x_scale as segments (grouped rows; no column scales)
 #define MOE_I8_SWIGLU 2     // weight pair (gate, up): S[0] = silu(gate) * up and, where given, S[1] = gate, S[2] = up, as segments
 
 struct MoeI8Gemm {
