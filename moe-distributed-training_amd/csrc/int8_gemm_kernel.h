@@ -382,14 +382,16 @@ __global__ void __launch_bounds__(NTHREADS, 2) i8_gemm_kernel(const MoeI8Gemm p)
             top = max(pair[0], pair[1]);
             pair = __builtin_amdgcn_permlane32_swap(top, top, false, false);
             top = max(pair[0], pair[1]);
-            const float amax = __uint_as_float(top);
-            const bool fine = top < 0x7f800000u;   // (otherwise its scale says NaN)
-            // (magnitudes from which the steps per unit would leave fp32's range, and zeros, are multiplied by a power of two first)
-            const float by = amax > 0x1p64f ? 0x1p-64f : amax < 0x1p-64f ? 0x1p64f : 1.f;
-            const float inv = fine && amax > 0.f ? MOE_SEG_LEVELS * __builtin_amdgcn_rcpf(amax * by) : 0.f;
-            if (__any(!fine || by != 1.f))
+            float amax = __uint_as_float(top), inv = MOE_SEG_LEVELS * __builtin_amdgcn_rcpf(amax);
+            if (__any(top - 0x1f800000u > 0x5f800000u - 0x1f800000u)) {   // not 2^-64 .. 2^64
+                // (magnitudes whose steps per unit would leave fp32's range are multiplied by a power of two first; zeros; a segment that is not finite: its scale says NaN)
+                const bool fine = top < 0x7f800000u;
+                const float by = amax > 0x1p64f ? 0x1p-64f : amax < 0x1p-64f ? 0x1p64f : 1.f;
+                inv = fine && amax > 0.f ? MOE_SEG_LEVELS * __builtin_amdgcn_rcpf(amax * by) : 0.f;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[i] = fine ? v[i] * by : 0.f;
+                amax = fine ? amax : __uint_as_float(0x7fc00000u);
+            }
             int q[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) q[i] = (int)rintf(v[i] * inv);
@@ -405,7 +407,7 @@ __global__ void __launch_bounds__(NTHREADS, 2) i8_gemm_kernel(const MoeI8Gemm p)
                 uint8_t* to = out + at * MOE_SEG_BYTES;
                 *(u32x4_t*)(to + g * 16) = hi;
                 *(uint2*)(to + 64 + g * 8) = lo;
-                if (g == 0) scales[(wrow0 + m) * SEGS + seg] = fine ? amax * row_scale : __uint_as_float(0x7fc00000u);   // (zeros of a row whose scale is NaN are NaN)
+                if (g == 0) scales[(wrow0 + m) * SEGS + seg] = amax * row_scale;   // (zeros of a row whose scale is NaN are NaN)
             }
         };
         auto xs = [&](int mb) { return s_xscale[wrow0 + mb * 16 + (lane & 15)]; };
@@ -482,55 +484,64 @@ __global__ void __launch_bounds__(NTHREADS, 2) i8_gemm_kernel(const MoeI8Gemm p)
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) column_scales(nb, w[nb]);
         const int64_t ncol0 = n0 + wn * WTN;
-        // Sum times row scale times column scale.  Where the first product could leave fp32's range (rows of 2^71 on) the row scale comes 2^40 times smaller, and what
-        // it comes to is as much larger again: powers of two round nothing.
-        auto values = [&](int mb, int nb, float xs, float* v) {
-            const bool far = xs > 0x1p64f;
-            const float x = far ? xs * 0x1p-40f : xs;
+        // Sum times row scale times column scale.  FAR: where the first product could leave fp32's range (rows of 2^71 on) the row scale comes 2^40 times smaller, and what
+        // it comes to is as much larger again: powers of two round nothing.  (A copy of its own for waves that have such rows: as a branch or a select around each product
+        // the products of 64 narrow experts took 110 -> 115 us.)
+        auto write = [&](auto far_tag) {
+            constexpr bool FAR = decltype(far_tag)::value;
+            auto values = [&](int mb, int nb, float xs, float* v) {
+                const bool much = FAR && xs > 0x1p64f;
+                const float x = much ? xs * 0x1p-40f : xs;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) v[r] = (float)acc[mb][nb][r] * x * w[nb][r];
-            if (__any(far))
+                for (int r = 0; r < 4; ++r) {
+                    v[r] = (float)acc[mb][nb][r] * x * w[nb][r];
+                    if (FAR) v[r] = much ? v[r] * 0x1p40f : v[r];
+                }
+            };
+            if (p.ydtype == MOE_F32) {
+                const bool vec = p.y_vec;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) v[r] = far ? v[r] * 0x1p40f : v[r];
-        };
-        if (p.ydtype == MOE_F32) {
-            const bool vec = p.y_vec;
+                for (int mb = 0; mb < MB; ++mb) {
+                    const int m = mb * 16 + mrow;
+                    if (mb >= mb_cnt || m >= wrows) continue;
+                    const float xs = s_xscale[wrow0 + m];
+                    float* y = (float*)p.Y + (p.y_grouped ? row0 + wrow0 + m : s_row[wrow0 + m]) * p.ldy;
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) {
+                        const int64_t n = ncol0 + nb * 16 + nq;
+                        float v[4];
+                        values(mb, nb, xs, v);
+                        if (vec && n < p.N) *(float4*)(y + n) = make_float4(v[0], v[1], v[2], v[3]);
+                        else
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                if (n + r < p.N) y[n + r] = v[r];
+                    }
+                }
+                return;
+            }
+            const bool f16 = p.ydtype == MOE_F16;
 #pragma unroll
             for (int mb = 0; mb < MB; ++mb) {
-                const int m = mb * 16 + mrow;
-                if (mb >= mb_cnt || m >= wrows) continue;
-                const float xs = s_xscale[wrow0 + m];
-                float* y = (float*)p.Y + (p.y_grouped ? row0 + wrow0 + m : s_row[wrow0 + m]) * p.ldy;
+                if (mb >= mb_cnt) continue;
+                const float xs = s_xscale[wrow0 + mb * 16 + mrow];
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
-                    const int64_t n = ncol0 + nb * 16 + nq;
                     float v[4];
                     values(mb, nb, xs, v);
-                    if (vec && n < p.N) *(float4*)(y + n) = make_float4(v[0], v[1], v[2], v[3]);
-                    else
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (n + r < p.N) y[n + r] = v[r];
+                    uint2 o;
+                    if (f16) { o.x = NumF16::pack2(v[0], v[1]); o.y = NumF16::pack2(v[2], v[3]); }
+                    else { o.x = NumBf16::pack2(v[0], v[1]); o.y = NumBf16::pack2(v[2], v[3]); }
+                    stage_put(WTN, mb * 16 + mrow, nb * 16 + nq, o);
                 }
             }
-            return;
-        }
-        const bool f16 = p.ydtype == MOE_F16;
+            stage_flush(WTN, (uint16_t*)p.Y, p.ldy, !p.y_grouped, ncol0, p.y_vec);
+        };
+        bool far = false;
 #pragma unroll
-        for (int mb = 0; mb < MB; ++mb) {
-            if (mb >= mb_cnt) continue;
-            const float xs = s_xscale[wrow0 + mb * 16 + mrow];
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-                float v[4];
-                values(mb, nb, xs, v);
-                uint2 o;
-                if (f16) { o.x = NumF16::pack2(v[0], v[1]); o.y = NumF16::pack2(v[2], v[3]); }
-                else { o.x = NumBf16::pack2(v[0], v[1]); o.y = NumBf16::pack2(v[2], v[3]); }
-                stage_put(WTN, mb * 16 + mrow, nb * 16 + nq, o);
-            }
-        }
-        stage_flush(WTN, (uint16_t*)p.Y, p.ldy, !p.y_grouped, ncol0, p.y_vec);
+        for (int i = 0; i < WTM; i += 64) far = far || s_xscale[wrow0 + i + lane] > 0x1p64f;   // (rows behind the wave's own are in the table as well)
+        if (__builtin_expect(__any(far), 0)) write(T_{});
+        else write(F_{});
     }
 }
 

@@ -5,7 +5,7 @@
 // it comes out (ties are common: half the maximum is 63.5 for every row of a 2-byte type).  q is guessed with one multiplication by 127 / a and, next to a border, put right
 // from its remainder 127 v - q a: 127 v is held as an fp32 number and its rounding error, and the difference with q a is exact (it is a multiple of half a unit of a's last
 // place and at most a / 2; below a / 254 q is 0).  Rows of inputs and weights are what they are; rows of gradients, products of two or three numbers, are held as an fp32
-// number and its error (together off by 2^-46 of it) from the start, their maximum too.  (16384 x 2048 bf16 gradient rows: 45 us, against 36 from fp32 products and a rounded 127 / a,
+// number and its error (together off by 2^-46 of it) from the start, their maximum too.  (16384 x 2048 bf16 gradient rows: 39.5 us, against 32 from fp32 products and a rounded 127 / a,
 // which puts 1 code in 10^5, and ties of most maxima, on the other side.)  The MLP's own interims, h and the joint row of dgate and dup, are computed in fp32 and carry its
 // rounding: their codes are of the fp32 values, by one multiplication, and a value within 127 * 2^-20 of a step from a border may go to either side.
 // A row that holds an infinity or a NaN gets the scale NaN and codes 0, so that every product of it is NaN and no other row changes; a row of zeros the scale 0.
@@ -24,17 +24,17 @@ typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 // Magnitudes are compared as bits: those of an infinity lie above every number's, and NaN's above those.
 constexpr uint32_t NOT_FINITE = 0x7f800000u;
 __device__ __forceinline__ uint32_t mag_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-// (a kernel's second maximum has its own place: the first may still be read)
-template <int PLACE = 0> __device__ __forceinline__ uint32_t block_max(uint32_t v)
+// (at most one maximum of each type in a kernel: its place is not used twice)
+template <typename U> __device__ __forceinline__ U block_max(U v)
 {
-    __shared__ uint32_t s_max[16];
+    __shared__ U s_max[16];
 #pragma unroll
-    for (int m = 32; m > 0; m >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, m));
+    for (int m = 32; m > 0; m >>= 1) { const U o = __shfl_xor(v, m); v = v > o ? v : o; }
     if (blockDim.x == 64) return v;
     if ((threadIdx.x & 63) == 0) s_max[threadIdx.x >> 6] = v;
     __syncthreads();
     v = s_max[0];
-    for (int w = 1; w < (int)(blockDim.x >> 6); ++w) v = max(v, s_max[w]);
+    for (int w = 1; w < (int)(blockDim.x >> 6); ++w) v = v > s_max[w] ? v : s_max[w];
     return v;
 }
 // (g + ge) s as the nearest fp32 number and its error.  (Contracted, the sum of the product and its error would hold the error twice.)
@@ -45,7 +45,7 @@ __device__ __forceinline__ void times_with_error(float g, float ge, float s, flo
     *v = h + he;
     *lo = he - (*v - h);
 }
-// Errors lo of numbers v as those of their magnitudes, in an order that unsigned numbers have, and back.
+// Errors lo of nearest fp32 numbers v as those of their magnitudes, in an order that unsigned numbers have, and back.
 __device__ __forceinline__ uint32_t error_key(float v, float lo)
 {
     const uint32_t b = __float_as_uint(v < 0.f ? -lo : lo);
@@ -72,7 +72,7 @@ struct RowCoder {
     __device__ __forceinline__ float code(float v, float lo) const
     {
         const float t = f == 0.f ? 0.f : v * f * inv, q = rintf(t);
-        return fabsf(t - q) > 0.4999f ? exact(v, lo) : q;
+        return fabsf(t - q) > 0.49995f ? exact(v, lo) : q;
     }
     __device__ __forceinline__ float exact(float v, float lo) const
     {
@@ -164,15 +164,16 @@ __global__ void __launch_bounds__(1024) quantize_rows_kernel(const MoeQuantizeRo
     }
     const T* row = (const T*)p.src + src_row * p.lds;
     const int nt = blockDim.x;
-    // eight values and, of products, their rounding errors
+    // eight values and, of products, their errors
     auto load = [&](int64_t c0, float* v, float* lo) {
         const bool whole = c0 + 8 <= p.cols;
-        float x[8], s[8];
-        if (p.vec && whole) Loader<T>::ld8(row + c0, x);
+        float s[8];
+        if (p.vec && whole) Loader<T>::ld8(row + c0, v);
         else
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = c0 + i < p.cols ? Elem<T>::ld(row + c0 + i) : 0.f;
-        if (SCALED && cs) {
+            for (int i = 0; i < 8; ++i) v[i] = c0 + i < p.cols ? Elem<T>::ld(row + c0 + i) : 0.f;
+        if (!SCALED) return;
+        if (cs) {
             if (p.vec_scale && whole) Loader<float>::ld8(cs + c0, s);
             else
 #pragma unroll
@@ -180,50 +181,46 @@ __global__ void __launch_bounds__(1024) quantize_rows_kernel(const MoeQuantizeRo
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            v[i] = x[i];
-            lo[i] = 0.f;
-            if (SCALED) {
-                const float g = coeff * x[i], ge = fmaf(coeff, x[i], -g);
-                v[i] = g;
-                lo[i] = ge;
-                if (cs) times_with_error(g, ge, s[i], v + i, lo + i);
-            }
+            const float x = v[i], g = coeff * x, ge = fmaf(coeff, x, -g);
+            v[i] = g;
+            lo[i] = ge;
+            if (cs) times_with_error(g, ge, s[i], v + i, lo + i);
         }
     };
     float keep[KEEP ? KEEP : 1][8], low[KEEP ? KEEP : 1][8];
-    uint32_t mine = 0;
     auto each = [&](auto fn) {
         if constexpr (KEEP > 0) {
 #pragma unroll
             for (int j = 0; j < KEEP; ++j) {
                 const int64_t c0 = ((int64_t)j * nt + threadIdx.x) * 8;
-                if (c0 < p.ldc) fn(j, c0);
+                if (c0 < p.ldc) fn(keep[j], low[j], c0);
             }
         } else
-            for (int64_t c0 = (int64_t)threadIdx.x * 8; c0 < p.ldc; c0 += (int64_t)nt * 8) { load(c0, keep[0], low[0]); fn(0, c0); }
+            for (int64_t c0 = (int64_t)threadIdx.x * 8; c0 < p.ldc; c0 += (int64_t)nt * 8) { load(c0, keep[0], low[0]); fn(keep[0], low[0], c0); }
     };
-    if constexpr (KEEP > 0) each([&](int j, int64_t c0) { load(c0, keep[j], low[j]); });
-    each([&](int j, int64_t) {
+    if constexpr (KEEP > 0) each([&](float* v, float* lo, int64_t c0) { load(c0, v, lo); });
+    std::conditional_t<SCALED, unsigned long long, uint32_t> top = 0;
+    each([&](const float* v, const float* lo, int64_t) {
+        uint32_t mine = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) mine = max(mine, mag_bits(keep[j][i]));
+        for (int i = 0; i < 8; ++i) mine = max(mine, mag_bits(v[i]));
+        if constexpr (SCALED) {   // (errors count among equal magnitudes only)
+            uint32_t error = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) error = mag_bits(v[i]) == mine ? max(error, error_key(v[i], lo[i])) : error;
+            const unsigned long long key = (unsigned long long)mine << 32 | error;
+            top = key > top ? key : top;
+        } else top = max(top, mine);
     });
-    const uint32_t top = block_max(mine);
-    uint32_t top_error = 0;
-    if (SCALED) {
-        if (mine == top)   // (few lanes: those that hold the maximum)
-            each([&](int j, int64_t) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (mag_bits(keep[j][i]) == top) top_error = max(top_error, error_key(keep[j][i], low[j][i]));
-            });
-        top_error = block_max<1>(top_error);
-    }
-    const RowCoder rc(top, SCALED ? key_error(top_error) : 0.f);
+    top = block_max(top);
+    RowCoder rc(0u);
+    if constexpr (SCALED) rc = RowCoder((uint32_t)(top >> 32), key_error((uint32_t)top));
+    else rc = RowCoder(top);
     int8_t* out = p.codes + m * p.ldc;
-    each([&](int j, int64_t c0) {
+    each([&](const float* v, const float* lo, int64_t c0) {
         float q[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) q[i] = rc.code(keep[j][i], low[j][i]);
+        for (int i = 0; i < 8; ++i) q[i] = rc.code(v[i], SCALED ? lo[i] : 0.f);
         uint2 w;
         w.x = pack4(q[0], q[1], q[2], q[3]);
         w.y = pack4(q[4], q[5], q[6], q[7]);
@@ -232,31 +229,23 @@ __global__ void __launch_bounds__(1024) quantize_rows_kernel(const MoeQuantizeRo
     if (threadIdx.x == 0) p.scale[m] = rc.scale;
 }
 
-// Columns c0 .. c0 + 7 of a row of segments, of a segment whose maximum is s (2^-95 or more).  A value's three bytes go to the upper three of a word, so that one
-// conversion makes it a float (256 times what it is: s carries the rest).
-__device__ __forceinline__ void ld8_seg(const uint8_t* row, int64_t c0, float s, float* v)
+// Columns c0 .. c0 + 7 of a row of segments, of a segment whose maximum is s.  A value's three bytes go to the upper three of a word, so that one conversion makes it a float
+// (256 times what it is).  ANY: also where the step of the segment would be subnormal (s below 2^-95): one product more per value.  (As a branch around those, which keeps
+// the loads of a thread's later pieces behind it, 8192 rows of 14336 columns of gate, up and dh took 303 us instead of 262.)
+template <bool ANY = false> __device__ __forceinline__ void ld8_seg(const uint8_t* row, int64_t c0, float s, float* v)
 {
+    constexpr float STEP = 1.f / (256.f * MOE_SEG_LEVELS);
     const uint8_t* seg = row + c0 / MOE_SEG_COLS * MOE_SEG_BYTES;
     const int c = (int)(c0 % MOE_SEG_COLS);
     const u32x4_t hi = *(const u32x4_t*)(seg + c * 2);
     const uint2 lo = *(const uint2*)(seg + 64 + c);
-    s *= 1.f / (256.f * MOE_SEG_LEVELS);
+    auto value = [&](uint32_t word) { return ANY ? (float)(int)word * STEP * s : (float)(int)word * (STEP * s); };
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const uint32_t l = i < 2 ? lo.x : lo.y;
-        v[2 * i] = (float)(int)__builtin_amdgcn_perm(hi[i], l, i & 1 ? 0x0504020cu : 0x0504000cu) * s;
-        v[2 * i + 1] = (float)(int)__builtin_amdgcn_perm(hi[i], l, i & 1 ? 0x0706030cu : 0x0706010cu) * s;
+        v[2 * i] = value(__builtin_amdgcn_perm(hi[i], l, i & 1 ? 0x0504020cu : 0x0504000cu));
+        v[2 * i + 1] = value(__builtin_amdgcn_perm(hi[i], l, i & 1 ? 0x0706030cu : 0x0706010cu));
     }
-}
-
-// ... of any maximum: the step of a segment below 2^-95 would be subnormal, so that one is read 2^64 times as large.
-__device__ __forceinline__ void ld8_seg_any(const uint8_t* row, int64_t c0, float s, float* v)
-{
-    const bool tiny = s < 0x1p-90f;
-    ld8_seg(row, c0, tiny ? s * 0x1p64f : s, v);
-    if (tiny)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] *= 0x1p-64f;
 }
 
 // Rows of segments -> codes: the maximum of a row is that of its segments.
@@ -297,9 +286,9 @@ __global__ void __launch_bounds__(KEEP == 1 ? 256 : 512) swiglu_bwd_codes_kernel
     auto load = [&](int64_t c0, float* a, float* b) {
         float dh[8], g[8], u[8], x1[8], x3[8];
         const int64_t s = m * nseg + c0 / MOE_SEG_COLS;
-        ld8_seg_any(dh_row, c0, p.dh_seg[s], dh);
-        ld8_seg_any(gate_row, c0, p.gate_seg[s], g);
-        ld8_seg_any(up_row, c0, p.up_seg[s], u);
+        ld8_seg<true>(dh_row, c0, p.dh_seg[s], dh);
+        ld8_seg<true>(gate_row, c0, p.gate_seg[s], g);
+        ld8_seg<true>(up_row, c0, p.up_seg[s], u);
         Loader<float>::ld8(c1 + c0, x1);
         Loader<float>::ld8(c3 + c0, x3);
 #pragma unroll
