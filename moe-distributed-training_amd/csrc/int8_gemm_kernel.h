@@ -430,6 +430,7 @@ __global__ void __launch_bounds__(NTHREADS, 2) i8_gemm_kernel(const MoeI8Gemm p)
             for (int mb = 0; mb < MB; ++mb) {
                 if (mb >= mb_cnt) continue;
                 const float x = xs(mb);
+                // (the hardware's exponential and reciprocal, off by 1 in the last place each: beside the roundings of a, u and the segment)
                 put_segment(mb, [&](int i) {
                     const float a = (float)acc[mb][i / 4][i % 4] * x * wg[i], u = (float)acc[mb][NBH + i / 4][i % 4] * x * wu[i];
                     return a * __builtin_amdgcn_rcpf(1.f + __expf(-a)) * u;

@@ -7,13 +7,14 @@
 // place and at most a / 2; below a / 254 q is 0).  Rows of inputs and weights are what they are; rows of gradients, products of two or three numbers, are held as an fp32
 // number and its error (together off by 2^-46 of it) from the start, their maximum too.  (16384 x 2048 bf16 gradient rows: 39.5 us, against 32 from fp32 products and a rounded 127 / a,
 // which puts 1 code in 10^5, and ties of most maxima, on the other side.)  The MLP's own interims, h and the joint row of dgate and dup, are computed in fp32 and carry its
-// rounding: their codes are of the fp32 values, by one multiplication, and a value within 127 * 2^-20 of a step from a border may go to either side.
+// rounding: their codes are of the fp32 values, by one multiplication, and a value that lies on a border to within that rounding may go to either side (1 to 2 in 10^6 codes of h;
+// half as many where gate, up and h are kept in fp32).
 // A row that holds an infinity or a NaN gets the scale NaN and codes 0, so that every product of it is NaN and no other row changes; a row of zeros the scale 0.
 //
 // Interims (h, the saved gate and up, dh) travel as 24-bit integers with a scale for each 32 columns of a row: 3 bytes per value, at most 2^-24 of the segment's
 // maximum off.  Every value that a rounding on the way carries over a border of the 8-bit codes costs a whole step, so this noise falls with the root of
 // the rounding only: with 16 bits 1 code in 700 changed and the MLP's error against 64 bits was 1.5e-3 of its result's norm (bf16 rows would be off by four
-// times that), with 24 it is that of fp32 arithmetic, at three quarters of an fp32 tensor's bytes.
+// times that), with 24 it is about twice that of fp32 arithmetic, at three quarters of an fp32 tensor's bytes.
 #include "common.h"
 #include "kernels.h"
 
