@@ -97,7 +97,7 @@ def fused_expert_mlp_int8(x, weights: Int8ExpertWeights, k, sorted_scattered_idx
     other arguments and the result as there.  Both projections of a row work on one set of codes of it, the down projection
     on codes of h = silu(gate) * up.  Gradients: of x and ``gates``, straight through the rounding to codes; the gradient
     rows that meet weights are codes as well (dY times the gates and w2's scales; dgate and dup times their scales, one
-    joint row).  Every assignment has to belong to an expert."""
+    joint row); a gradient of x takes f below 2^16.  Every assignment has to belong to an expert."""
     return entry("expert_mlp_int8")(x, weights.w1, weights.w1_scale, weights.w2, weights.w2_scale, weights.w3, weights.w3_scale, k,
                                     sorted_scattered_idxs, expert_offsets, gates, grouped_out)
 
@@ -249,8 +249,8 @@ class ScatterMoEBlock(nn.Module):
 
     def _apply(self, fn, *args, **kw):
         # (what ``to``, ``half``, ``cuda`` and the like go through, also those of a module around this one)
-        if self.is_quantized and self.w1_scale.is_floating_point() and fn(self.w1_scale[:0]).dtype != self.w1_scale.dtype:
-            raise TypeError("the scales of a block with experts in 8 bits stay float32: choose the block's type before quantize_experts()")
+        if self.is_quantized and any(fn(t.detach()[:0]).dtype != t.dtype for t in (self.w1_scale, self.router)):
+            raise TypeError("a block with experts in 8 bits keeps its type, and its scales stay float32: choose the type before quantize_experts()")
         return super()._apply(fn, *args, **kw)
 
     def forward(self, hidden_states: torch.Tensor):

@@ -35,6 +35,6 @@ def parallel_linear_int8(inputs, expert_weights, weight_scales, k, sorted_expert
     """``parallel_linear`` over 8-bit weights: inputs (rows, K) bf16, fp16 or fp32; expert_weights (E, K, N) int8 codes of
     any strides (codes whose rows are not contiguous and 16-byte aligned are copied within the call); weight_scales (E, N)
     fp32; the other arguments as in ``parallel_linear``.  Every assignment has to belong to an expert: rows of the result
-    that no group covers are not written.  Gradients: of ``inputs`` and ``gates``."""
+    that no group covers are not written.  Gradients: of ``inputs`` (fewer than 2^17 output columns) and ``gates``."""
     return entry("linear_int8")(inputs, expert_weights, weight_scales, k, sorted_expert_idxs, sorted_scattered_idxs, expert_offsets, gates,
                                 grouped_in, grouped_out)

@@ -55,3 +55,13 @@ def test_moves_and_conversions_that_keep_the_scales():
     assert all(torch.equal(t, before[n]) for n, t in block.state_dict().items())
     plain = moe.ScatterMoEBlock(64, 128, 2, dtype=F32).to(BF16).half()          # blocks with their weights convert as ever
     assert plain.w1.dtype == F16
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_a_quantised_block_keeps_a_type_that_its_products_take(dtype):
+    """An fp32 router would be served by nothing, and the way back would be refused for the scales' sake."""
+    block = stand_in(dtype)
+    for convert in (lambda m: m.float(), lambda m: m.to(F32)):
+        with pytest.raises(TypeError, match="keeps its type"):
+            convert(block)
+    assert block.router.dtype == dtype and block.router.requires_grad and block.w2_scale.dtype == F32
