@@ -256,7 +256,7 @@ int moe_mlp_bwd(const void* dy, int64_t lddy, int dy_grouped, int dy_fan_out, co
  * infinity or a NaN the scale NaN and codes 0, which makes every product of it NaN.  Rows of inputs, weights and dY (times gates and column scales, as exact products) are
  * taken so; the MLP's h and [dgate s1 | dup s3] are computed in fp32, and a value of theirs that lies on a border to within that rounding may go to either side.  Sums of products are exact (K < 2^17, else MOE_ERR_UNSUPPORTED);
  * their values do not depend on the order or number of launches.  Row counts are limited by what one launch can hold, 2^32 threads of 64 to 1024 per row: more are refused
- * with MOE_ERR_UNSUPPORTED before anything is enqueued.
+ * with MOE_ERR_UNSUPPORTED before anything is enqueued.  Workspaces and `saved` of the products are 16-byte aligned (that of moe_quantize_weights 4-byte), else MOE_ERR_BAD_ARG.
  *
  * moe_quantize_rows: rows of src -> codes (pitch ldc >= ncols, a multiple of 16, 16-byte aligned; columns from ncols on are written as zeros) and scales. */
 int moe_quantize_rows(const void* src, int64_t lds, int dtype, int8_t* codes, int64_t ldc, float* scale, int64_t nrows, int64_t ncols, void* stream);

@@ -1104,7 +1104,7 @@ size_t moe_quantize_weights_workspace_bytes(int E, int64_t N) { return E < 1 || 
 int moe_quantize_weights(const void* W, int64_t swe, int64_t swk, int64_t swn, int dtype, int E, int64_t K, int64_t N, int8_t* codes, int64_t sce,
                          int64_t sck, int64_t scn, float* scale, void* workspace, size_t workspace_bytes, void* stream)
 {
-    if (dtype < 0 || dtype > 2 || E < 1 || K < 1 || N < 1 || !W || !codes || !scale) return MOE_ERR_BAD_ARG;
+    if (dtype < 0 || dtype > 2 || E < 1 || K < 1 || N < 1 || !W || !codes || !scale || (uintptr_t)workspace % 4 != 0) return MOE_ERR_BAD_ARG;
     if (E > 65535 || K > 65535 * (int64_t)16 || N > 65535 * (int64_t)16) return MOE_ERR_UNSUPPORTED;
     if (!workspace || workspace_bytes < moe_quantize_weights_workspace_bytes(E, N)) return MOE_ERR_WORKSPACE;
     return moe_launch_quantize_weights(W, swe, swk, swn, dtype, E, K, N, codes, sce, sck, scn, scale, (uint32_t*)workspace, S(stream));
@@ -1168,7 +1168,7 @@ int moe_linear_int8_fwd(const void* x, int64_t ldx, int64_t x_rows, int dtype, c
     if (dtype < 0 || dtype > 2 || y_dtype < 0 || y_dtype > 2 || E < 1 || R < 0 || x_rows < 0 || K < 1 || N < 0 || fan_out < 1) return MOE_ERR_BAD_ARG;
     if (R == 0 || N == 0) return MOE_OK;
     if (ldx < 0 || (R > 1 && ldy < N)) return MOE_ERR_BAD_ARG;   // (rows of an input may overlap)
-    if (!x || x_rows < 1 || !W || !w_scale || !y || !offsets || ((!x_grouped || !y_grouped) && !pos) || (x_grouped && x_rows < R)) return MOE_ERR_BAD_ARG;
+    if (!x || x_rows < 1 || !W || !w_scale || !y || !offsets || ((!x_grouped || !y_grouped) && !pos) || (x_grouped && x_rows < R) || !aligned16(workspace)) return MOE_ERR_BAD_ARG;
     if (K > MOE_I8_MAX_K || E > 65535 || x_rows > 0x7fffffff) return MOE_ERR_UNSUPPORTED;
     const I8Weights w = i8_weights(W, swe, swk, swn, E, K, N);
     if (!workspace || workspace_bytes < i8_linear_bytes(w, x_rows, R, E, K, N)) return MOE_ERR_WORKSPACE;
@@ -1188,7 +1188,7 @@ int moe_linear_int8_bwd(const void* dy, int64_t lddy, int dtype, int dy_grouped,
     if (dtype < 0 || dtype > 2 || dx_dtype < 0 || dx_dtype > 2 || E < 1 || R < 0 || K < 0 || N < 1 || dy_fan_out < 1 || (gates && (gates_dtype < 0 || gates_dtype > 2))) return MOE_ERR_BAD_ARG;
     if (R == 0 || K == 0) return MOE_OK;
     if (lddy < 0 || (R > 1 && lddx < K)) return MOE_ERR_BAD_ARG;
-    if (!dy || !W || !w_scale || !dx_rows || !offsets || ((!dy_grouped || !dx_grouped) && !pos)) return MOE_ERR_BAD_ARG;
+    if (!dy || !W || !w_scale || !dx_rows || !offsets || ((!dy_grouped || !dx_grouped) && !pos) || !aligned16(workspace)) return MOE_ERR_BAD_ARG;
     if (N > MOE_I8_MAX_K || E > 65535 || R > 0x7fffffff) return MOE_ERR_UNSUPPORTED;
     const I8Weights w = i8_weights(W, swe, swn, swk, E, N, K);   // W^T: the contraction runs over N
     if (!workspace || workspace_bytes < i8_linear_bytes(w, R, R, E, N, K)) return MOE_ERR_WORKSPACE;
@@ -1236,7 +1236,7 @@ int moe_mlp_int8_fwd(const void* x, int64_t ldx, int64_t x_rows, int dtype, cons
     if (dtype < 0 || dtype > 2 || y_dtype < 0 || y_dtype > 2 || E < 1 || R < 0 || x_rows < 0 || d < 1 || f < 1 || fan_out < 1) return MOE_ERR_BAD_ARG;
     if (R == 0) return MOE_OK;
     if (ldx < 0 || (R > 1 && ldy < d)) return MOE_ERR_BAD_ARG;
-    if (!x || x_rows < 1 || !w1 || !s1 || !w3 || !s3 || !w2 || !s2 || !y || !pos || !offsets) return MOE_ERR_BAD_ARG;
+    if (!x || x_rows < 1 || !w1 || !s1 || !w3 || !s3 || !w2 || !s2 || !y || !pos || !offsets || !aligned16(saved) || !aligned16(workspace)) return MOE_ERR_BAD_ARG;
     if (dtype == MOE_F32 || !i8_mlp_sizes_ok(d, f) || d > MOE_I8_MAX_K || f > MOE_I8_MAX_K || E > 65535 || x_rows > 0x7fffffff || R > 0x7fffffff) return MOE_ERR_UNSUPPORTED;
     if (!aligned16(w1) || !aligned16(w3) || !aligned16(w2)) return MOE_ERR_UNSUPPORTED;
     if (saved && saved_bytes < moe_mlp_int8_saved_bytes(R, f)) return MOE_ERR_WORKSPACE;
@@ -1286,7 +1286,7 @@ int moe_mlp_int8_bwd(const void* dy, int64_t lddy, int dtype, int dy_grouped, in
     if (dtype < 0 || dtype > 2 || dx_dtype < 0 || dx_dtype > 2 || E < 1 || R < 0 || d < 1 || f < 1 || dy_fan_out < 1 || (gates && (gates_dtype < 0 || gates_dtype > 2 || dy_grouped))) return MOE_ERR_BAD_ARG;
     if (R == 0) return MOE_OK;
     if (lddy < 0 || (R > 1 && lddx < d)) return MOE_ERR_BAD_ARG;
-    if (!dy || !w1 || !s1 || !w3 || !s3 || !w2 || !s2 || !saved || !dx_rows || !pos || !offsets) return MOE_ERR_BAD_ARG;
+    if (!dy || !w1 || !s1 || !w3 || !s3 || !w2 || !s2 || !saved || !dx_rows || !pos || !offsets || !aligned16(saved) || !aligned16(workspace)) return MOE_ERR_BAD_ARG;
     if (dtype == MOE_F32 || !i8_mlp_sizes_ok(d, f) || d > MOE_I8_MAX_K || 2 * f > MOE_I8_MAX_K || E > 65535 || R > 0x7fffffff) return MOE_ERR_UNSUPPORTED;
     if (!aligned16(w1) || !aligned16(w3) || !aligned16(w2)) return MOE_ERR_UNSUPPORTED;
     if (saved_bytes < moe_mlp_int8_saved_bytes(R, f)) return MOE_ERR_WORKSPACE;

@@ -84,3 +84,16 @@ def test_tiles_and_parts_of_known_sizes():
     assert mlp(16384, 64, 2048, 1024) == ((256, 1),) * 4                                       # many narrow experts
     assert plan(500, 1, 14336, 4096) == (256, 4) and plan(64, 1, 14336, 4096)[0] == 256 and plan(4, 1, 14336, 4096) == (128, 8)
     assert lib.moe_int8_debug_tile(0, 8, 64, 64, 0, 1, None) == -1 and lib.moe_int8_debug_tile(8, 8, 64, 64, 0, 0, None) == -1
+
+
+def test_workspaces_at_odd_addresses_are_refused():
+    """The counters of split tiles are updated by atomics and codes are moved 16 bytes at a time: neither may begin anywhere."""
+    n = 1 << 30
+    for at in (17, 20, 24):
+        assert lib.moe_linear_int8_fwd(16, 64, 8, 0, 16, 8192, 1, 64, 16, 16, 128, 0, 16, 0, 16, 0, 2, 16, 64, 128, 2, 0, 0, at, n, None) == -1
+        assert lib.moe_linear_int8_bwd(16, 128, 0, 0, 2, None, 0, 16, 8192, 1, 64, 16, 16, 64, 0, 0, 16, 0, 16, 0, 2, 16, 64, 128, at, n, None) == -1
+        for saved, ws in ((None, at), (at, 16)):
+            assert lib.moe_mlp_int8_fwd(16, 64, 8, 0, 16, 16, 16, 16, 16, 16, 16, 64, 0, 16, 0, 16, 0, 2, 16, 64, 128, 2, 0, saved, n, ws, n, None) == -1
+        for saved, ws in ((16, at), (at, 16)):
+            assert lib.moe_mlp_int8_bwd(16, 64, 0, 0, 2, None, 0, 16, 16, 16, 16, 16, 16, saved, n, 16, 64, 0, 16, 0, 16, 0, 2, 16, 64, 128, ws, n, None) == -1
+    assert lib.moe_quantize_weights(16, 1, 1, 1, 0, 2, 8, 8, 16, 1, 1, 1, 16, 18, n, None) == -1
