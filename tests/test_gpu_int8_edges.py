@@ -185,3 +185,94 @@ def test_scales_at_any_address(dev):
         y = moe.fused_expert_mlp_int8(a, weights, k, ssi, eo, b)
         return [y.detach(), *torch.autograd.grad(y, (a, b), torch.ones_like(y))]
     assert all(torch.equal(a, b) for a, b in zip(step(odd), step(w)))
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# arguments in other forms
+# ---------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("ssi_type,eo_type", [(torch.int32, torch.int64), (torch.int64, torch.int32)])
+def test_grouped_rows_in_and_a_weighted_sum_out(dev, dtype, ssi_type, eo_type):
+    """A down projection: one grouped row per assignment, and each token's rows weighted and summed; index tensors of different types."""
+    T, K, N, E, k = 150, 192, 224, 5, 2
+    sei, ssi, eo, gw = oracle.route(T, E, k, 1)
+    g = torch.Generator().manual_seed(2)
+    w = torch.randint(-127, 128, (E, K, N), generator=g, dtype=torch.int8)
+    ws = torch.rand(E, N, generator=g) * 1e-3 + 1e-4
+    h, dout, gw = torch.randn(T * k, K, generator=g).to(dtype), torch.randn(T, N, generator=g).to(dtype), gw.to(dtype)
+    want = oracle.linear(h, w, ws, 1, sei, ssi, gw, dout, grouped_in=True, near=127 * 2.0 ** -29)
+    hd, gd = h.to(dev).requires_grad_(True), gw.to(dev).requires_grad_(True)
+    y = moe.parallel_linear_int8(hd, w.to(dev), ws.to(dev), 1, sei.to(dev, ssi_type), ssi.to(dev, ssi_type), None, eo.to(dev, eo_type), gd, grouped_in=True)
+    got = torch.autograd.grad(y, (hd, gd), dout.to(dev))
+    close(y, want["y"], want["y_terms"] * (6 + 2 * k) * 2.0 ** -24, dtype, "y")
+    close(got[0], want["dx_rows"], want["dx_slack"] + want["dx_rows"].abs() * 6 * 2.0 ** -24, dtype, "dx")
+    close(got[1], want["d_gates"], want["d_gates_terms"] * (N + 7) * 2.0 ** -24, dtype, "d_gates")
+
+
+def test_one_matrix_for_all_experts(dev):
+    """Codes expanded over the experts (a stride of 0), with a scale for each."""
+    T, K, N, E = 70, 128, 160, 6
+    sei, ssi, eo, _ = (t.to(dev) for t in oracle.route(T, E, 2, 3))
+    g = torch.Generator().manual_seed(0)
+    w = torch.randint(-127, 128, (1, N, K), generator=g, dtype=torch.int8).to(dev).transpose(1, 2).expand(E, K, N)
+    ws, x = (torch.rand(E, N, generator=g) * 1e-3).to(dev), torch.randn(T, K, generator=g).to(BF16).to(dev)
+    a, b = x.clone().requires_grad_(True), x.clone().requires_grad_(True)
+    ya, yb = (moe.parallel_linear_int8(v, c, ws, 2, sei, ssi, None, eo) for v, c in ((a, w), (b, w.contiguous())))
+    assert torch.equal(ya, yb)
+    assert torch.equal(torch.autograd.grad(ya.sum(), a)[0], torch.autograd.grad(yb.sum(), b)[0])
+
+
+@pytest.mark.parametrize("order", [(0, 1, 2), (0, 2, 1), (1, 0, 2), (1, 2, 0), (2, 0, 1), (2, 1, 0)])
+def test_weights_of_any_order_of_dimensions_become_the_same_codes(dev, order):
+    sizes = (3, 70, 50)
+    w = torch.randn(sizes, generator=torch.Generator().manual_seed(1)).to(BF16).to(dev)
+    back = [order.index(i) for i in range(3)]
+    turned = w.permute(order).contiguous().permute(back)
+    assert turned.shape == w.shape
+    want, got = moe.quantize_expert_weights(w), moe.quantize_expert_weights(turned)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    # every second of a larger tensor's columns and rows
+    big = torch.randn(3, 140, 100, generator=torch.Generator().manual_seed(2)).to(dev)
+    a, b = moe.quantize_expert_weights(big[:, ::2, 1::2]), moe.quantize_expert_weights(big[:, ::2, 1::2].contiguous())
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_without_autograd_and_in_inference_mode(dev):
+    T, d, f, E, k = 40, 128, 192, 3, 2
+    block = moe.ScatterMoEBlock(d, f, E, top_k=k, device=dev).quantize_experts()
+    x = torch.randn(T, d, generator=torch.Generator().manual_seed(0)).to(BF16).to(dev)
+    want = block(x)[0].detach()
+    with torch.no_grad():
+        assert torch.equal(block(x)[0], want)
+    with torch.inference_mode():
+        got = block(x.clone())[0]
+        assert torch.equal(got, want) and got.is_inference()
+        codes, scales = moe.quantize_rows(x)
+        assert torch.equal(codes, moe.quantize_rows(x)[0]) and scales.shape == (T,)
+
+
+def test_graphs_of_one_memory_pool(dev):
+    """Two captured calls whose workspaces may be the same memory, replayed in turn."""
+    T, d, f, E, k = 3, 1024, 4096, 4, 2                          # few rows: parts of tiles meet in the workspace
+    sei, ssi, eo, gates = (t.to(dev) for t in oracle.route(T, E, k, 0))
+    w = moe.Int8ExpertWeights(*(t.to(dev) for t in mlp_weights(E, d, f, 1)))
+    x = torch.randn(T, d, generator=torch.Generator().manual_seed(1)).to(BF16).to(dev)
+    calls = [lambda: moe.fused_expert_mlp_int8(x, w, k, ssi, eo, gates), lambda: moe.fused_expert_mlp_int8(x, w, k, ssi, eo)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for c in calls:
+            c()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs, pool = [], [], None
+    for c in calls:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], pool=pool):
+            outs.append(c())
+        pool = pool or graphs[0].pool()
+    for trial, i in enumerate((0, 1, 1, 0, 0, 1)):
+        x.copy_(torch.randn(x.shape, generator=torch.Generator().manual_seed(trial)).to(BF16))
+        graphs[i].replay()
+        torch.cuda.synchronize()
+        got = outs[i].clone()
+        assert torch.equal(got, calls[i]()), (trial, i)
