@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define MOE_HIP_ABI_VERSION 4   /* 4: moe_int8_debug_tile; 3: expert products in 8-bit integers; 2: router weight gradient, static-scratch sort, stage-timer selection, moe_combine with k = 0; fp16 on the matrix cores (dtype argument of moe_mlp_fwd / moe_mlp_bwd) */
+#define MOE_HIP_ABI_VERSION 5   /* 5: expert products over 4-bit weights, SwiGLU with kept 8-bit inputs; 4: moe_int8_debug_tile; 3: expert products in 8-bit integers; 2: router weight gradient, static-scratch sort, stage-timer selection, moe_combine with k = 0; fp16 on the matrix cores (dtype argument of moe_mlp_fwd / moe_mlp_bwd) */
 
 #define MOE_OK 0
 #define MOE_ERR_BAD_ARG (-1)      /* inconsistent sizes / null pointers */
@@ -303,6 +303,37 @@ int moe_mlp_int8_bwd(const void* dy, int64_t lddy, int dtype, int dy_grouped, in
                      const float* s1, const int8_t* w3, const float* s3, const int8_t* w2, const float* s2, const void* saved, size_t saved_bytes,
                      void* dx_rows, int64_t lddx, int dx_dtype, const void* pos, int pos64, const void* offsets, int off64, int E, int64_t R, int64_t d, int64_t f,
                      void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- expert products over 4-bit weights (no counterpart in the reference) --------------------------------------
+ * A weight is a code of one sign, two exponent and one mantissa bit (0, 0.5, 1, 1.5, 2, 3, 4, 6; bit 3 is the sign) times 2^(s - 127), s the scale byte that it shares with the
+ * 31 others of its group: 32 consecutive inputs of one output column, of an expert's inputs 0.. on.  s = 255 is NaN.  codes (E, N, ceil(K/32) * 16) bytes: byte b of a row holds inputs
+ * 2b (lower half) and 2b + 1; those behind K are zeros.  scales (E, N, ceil(K/32)) bytes.  Strides count bytes; rows of codes start at multiples of 16.
+ *
+ * moe_fp4_quantize_weights: (E,K,N) weights of any strides -> the nearest codes (the even one of two) under the least power of two that leaves the group's largest magnitude at
+ * 7 units or below.  A group of zeros gets the scale 0, one that holds an infinity or a NaN the scale 255 and codes 0. */
+int moe_fp4_quantize_weights(const void* W, int64_t swe, int64_t swk, int64_t swn, int dtype, int E, int64_t K, int64_t N, uint8_t* codes, int64_t sce, int64_t scn,
+                             uint8_t* scales, int64_t sse, int64_t ssn, void* stream);
+/* moe_scatter2scatter without adapters over 4-bit weights: y[out_row] = x[in_row] @ W[e], rows addressed as there; x has x_rows rows.  Weights enter as numbers of
+ * x's type: exact in bf16 and fp32; in fp16 for scales from 104 to 140, beyond which they round (or overflow) as a conversion to fp16 does.
+ * Backward (weights frozen): dy in grouped order, dx_rows[dx_grouped ? m : pos[m]] = dy[m] @ W[e]^T.  Rows that no group covers are not written. */
+size_t moe_linear_fp4_workspace_bytes(int dtype, int64_t R, int E, int64_t K, int64_t N);
+int moe_linear_fp4_fwd(const void* x, int64_t ldx, int64_t x_rows, int dtype, const uint8_t* codes, int64_t sce, int64_t scn, const uint8_t* scales, int64_t sse, int64_t ssn,
+                       void* y, int64_t ldy, int y_dtype, const void* pos, int pos64, const void* offsets, int off64, int E, int64_t R, int64_t K, int64_t N, int fan_out,
+                       int x_grouped, int y_grouped, void* workspace, size_t workspace_bytes, void* stream);
+int moe_linear_fp4_bwd(const void* dy, int64_t lddy, int dtype, const uint8_t* codes, int64_t sce, int64_t scn, const uint8_t* scales, int64_t sse, int64_t ssn, void* dx_rows,
+                       int64_t lddx, int dx_grouped, const void* pos, int pos64, const void* offsets, int off64, int E, int64_t R, int64_t K, int64_t N, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/* ---- SwiGLU that keeps its inputs in 8 bits (no counterpart in the reference) -----------------------------------
+ * h = silu(gate) * up; kept (or NULL: nothing is) are, for the backward pass, codes rne(127 v / a) of blocks of 64 columns of each row of gate and up (the exact quotient, ties to even; a the
+ * block's largest magnitude, the last block of a row may be shorter) and the scales a / 127 (fp32; NaN for a block that holds an infinity or a NaN): moe_swiglu8_kept_bytes, 16-byte
+ * aligned.  Backward, with g, u = codes * scale and s = 1 / (1 + exp(-g)):  dgate = dh u s (1 + g (1 - s)), dup = dh g s.  Rows of any pitch, columns one after the other; fewer than
+ * 2^28 blocks. */
+size_t moe_swiglu8_kept_bytes(int64_t rows, int64_t cols);
+int moe_swiglu8_fwd(const void* gate, int64_t ldg, const void* up, int64_t ldu, void* h, int64_t ldh, void* kept, size_t kept_size, int64_t rows, int64_t cols, int dtype,
+                    void* stream);
+int moe_swiglu8_bwd(const void* kept, size_t kept_size, const void* dh, int64_t lddh, void* dgate, int64_t lddg, void* dup, int64_t lddu, int64_t rows, int64_t cols, int dtype,
+                    void* stream);
 
 #ifdef __cplusplus
 }

@@ -14,10 +14,11 @@ from .scattermoe_utils.kernels.ops import (  # noqa: F401
 from .scattermoe_utils.parallel_linear_lora import ParallelLinearLora, parallel_linear_lora  # noqa: F401
 from .scattermoe_utils.parallel_experts import ParallelLinear, parallel_linear, ParallelExperts  # noqa: F401
 from .scattermoe_utils.parallel_linear_int8 import parallel_linear_int8, quantize_expert_weights  # noqa: F401
+from .scattermoe_utils.parallel_linear_fp4 import parallel_linear_fp4, quantize_expert_weights_fp4  # noqa: F401
 from .megablocks_utils.router import forward_router, route_and_sort  # noqa: F401
 from .megablocks_utils.moe_mlp import (  # noqa: F401
     scattermoe_permute_and_compute, fused_expert_mlp, moe_layer_forward, ScatterMoEBlock,
-    Int8ExpertWeights, fused_expert_mlp_int8, moe_layer_forward_int8,
+    Int8ExpertWeights, fused_expert_mlp_int8, moe_layer_forward_int8, swiglu_8bit,
 )
 
 __all__ = [
@@ -25,5 +26,6 @@ __all__ = [
     "group_bwd_W", "ParallelLinearLora", "parallel_linear_lora", "ParallelLinear", "parallel_linear",
     "ParallelExperts", "forward_router", "route_and_sort", "scattermoe_permute_and_compute", "fused_expert_mlp",
     "moe_layer_forward", "ScatterMoEBlock", "quantize_rows", "quantize_expert_weights", "parallel_linear_int8",
-    "Int8ExpertWeights", "fused_expert_mlp_int8", "moe_layer_forward_int8",
+    "Int8ExpertWeights", "fused_expert_mlp_int8", "moe_layer_forward_int8", "quantize_expert_weights_fp4", "parallel_linear_fp4",
+    "swiglu_8bit",
 ]

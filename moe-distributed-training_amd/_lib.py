@@ -10,7 +10,7 @@ import torch
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libmoe_hip.so")
 
-ABI_VERSION = 4   # MOE_HIP_ABI_VERSION of include/moe_hip.h this binding was written against
+ABI_VERSION = 5   # MOE_HIP_ABI_VERSION of include/moe_hip.h this binding was written against
 MOE_BF16, MOE_F16, MOE_F32 = 0, 1, 2
 _DTYPES = {torch.bfloat16: MOE_BF16, torch.float16: MOE_F16, torch.float32: MOE_F32}
 
@@ -74,6 +74,13 @@ _SIGNATURES = {
     "moe_mlp_int8_saved_bytes": ("z", "ll"),
     "moe_mlp_int8_workspace_bytes": ("z", "llilli"),
     "moe_mlp_int8_fwd": ("i", "plli" + "pppppp" + "pli" + "pi" + "pi" + "i" + "lll" + "ii" + "pz" + "pzp"),
+    "moe_fp4_quantize_weights": ("i", "plll" + "iill" + "pll" + "pll" + "p"),
+    "moe_linear_fp4_workspace_bytes": ("z", "ilill"),
+    "moe_linear_fp4_fwd": ("i", "plli" + "pll" + "pll" + "pli" + "pi" + "pi" + "i" + "lll" + "iii" + "pzp"),
+    "moe_linear_fp4_bwd": ("i", "pli" + "pll" + "pll" + "pli" + "pi" + "pi" + "i" + "lll" + "pzp"),
+    "moe_swiglu8_kept_bytes": ("z", "ll"),
+    "moe_swiglu8_fwd": ("i", "plplpl" + "pz" + "ll" + "i" + "p"),
+    "moe_swiglu8_bwd": ("i", "pzplplpl" + "ll" + "i" + "p"),
     "moe_mlp_int8_bwd": ("i", "pliii" + "pi" + "pppppp" + "pz" + "pli" + "pi" + "pi" + "i" + "lll" + "pzp"),
 }
 

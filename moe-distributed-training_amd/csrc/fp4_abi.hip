@@ -1,0 +1,121 @@
+// C-ABI entries of the expert products over 4-bit weights and of the SwiGLU that keeps its inputs in 8 bits: argument checks and launch sequences.  Declarations and their
+// contracts: include/moe_hip.h.
+#include "../../include/moe_hip.h"
+#include "common.h"
+#include "kernels.h"
+
+namespace {
+
+inline hipStream_t S(void* s) { return (hipStream_t)s; }
+inline size_t al(size_t n) { return (n + 255) & ~(size_t)255; }
+inline bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
+inline int64_t groups_of(int64_t K) { return (K + 31) / 32; }
+inline size_t elem_bytes(int dtype) { return dtype == MOE_F32 ? 4 : 2; }
+#define TRY(call) do { const int rc_ = (call); if (rc_ != MOE_OK) return rc_; } while (0)
+
+// rows of codes that 16-byte loads take, and scales that lie one after the other
+bool weights_ok(const MoeFp4Weights& w) { return w.codes && w.scales && aligned16(w.codes) && w.sce % 16 == 0 && w.scn % 16 == 0; }
+
+struct Kept { size_t codes, scales; };
+Kept kept_sizes(int64_t rows, int64_t cols)
+{
+    const size_t blocks = (size_t)rows * (size_t)((cols + MOE_KEPT_BLOCK - 1) / MOE_KEPT_BLOCK);
+    return {al(blocks * MOE_KEPT_BLOCK), al(blocks * 4)};
+}
+size_t kept_bytes(int64_t rows, int64_t cols) { const Kept k = kept_sizes(rows, cols); return 2 * (k.codes + k.scales); }
+
+int swiglu8_params(MoeSwiglu8& p, uint8_t* kept, int64_t rows, int64_t cols)
+{
+    p.cols = cols;
+    const int64_t row_blocks = (cols + MOE_KEPT_BLOCK - 1) / MOE_KEPT_BLOCK;
+    // (a launch's threads, eight to a block, are counted in 32 bits)
+    if (row_blocks > 0x7fffffff || rows > 0x7fffffff || rows * row_blocks >= (int64_t)1 << 28) return MOE_ERR_UNSUPPORTED;
+    p.row_blocks = (uint32_t)row_blocks;
+    p.nblocks = (uint32_t)(rows * row_blocks);
+    if (kept) {
+        const Kept k = kept_sizes(rows, cols);
+        p.codes[0] = kept; p.codes[1] = kept + k.codes;
+        p.scales[0] = (float*)(kept + 2 * k.codes); p.scales[1] = (float*)(kept + 2 * k.codes + k.scales);
+    }
+    return MOE_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int moe_fp4_quantize_weights(const void* W, int64_t swe, int64_t swk, int64_t swn, int dtype, int E, int64_t K, int64_t N, uint8_t* codes, int64_t sce, int64_t scn, uint8_t* scales,
+                             int64_t sse, int64_t ssn, void* stream)
+{
+    if (dtype < 0 || dtype > 2 || E < 1 || K < 1 || N < 1 || !W || !codes || !scales || !aligned16(codes) || sce % 16 != 0 || scn % 16 != 0 || scn < groups_of(K) * 16) return MOE_ERR_BAD_ARG;
+    return moe_launch_fp4_quantize(W, swe, swk, swn, dtype, E, K, N, codes, sce, scn, scales, sse, ssn, S(stream));
+}
+
+size_t moe_linear_fp4_workspace_bytes(int dtype, int64_t R, int E, int64_t K, int64_t N)
+{
+    if (dtype < 0 || dtype > 2 || R < 1 || E < 1 || K < 1 || N < 1) return 0;
+    const size_t fwd = moe_scatter2scatter_workspace_bytes(R, E, K, N, 0), bwd = moe_scatter2scatter_workspace_bytes(R, E, N, K, 0);
+    return al((size_t)E * (size_t)N * (size_t)K * elem_bytes(dtype)) + (fwd > bwd ? fwd : bwd);   // (of either direction)
+}
+
+int moe_linear_fp4_fwd(const void* x, int64_t ldx, int64_t x_rows, int dtype, const uint8_t* codes, int64_t sce, int64_t scn, const uint8_t* scales, int64_t sse, int64_t ssn, void* y,
+                       int64_t ldy, int y_dtype, const void* pos, int pos64, const void* offsets, int off64, int E, int64_t R, int64_t K, int64_t N, int fan_out, int x_grouped,
+                       int y_grouped, void* workspace, size_t workspace_bytes, void* stream)
+{
+    if (dtype < 0 || dtype > 2 || y_dtype != dtype || E < 1 || R < 0 || x_rows < 0 || K < 1 || N < 0 || fan_out < 1) return MOE_ERR_BAD_ARG;
+    if (R == 0 || N == 0) return MOE_OK;
+    if (ldx < 0 || (R > 1 && ldy < N)) return MOE_ERR_BAD_ARG;   // (rows of an input may overlap)
+    const MoeFp4Weights w = {codes, sce, scn, scales, sse, ssn};
+    if (!x || x_rows < 1 || !weights_ok(w) || !y || !offsets || ((!x_grouped || !y_grouped) && !pos) || (x_grouped && x_rows < R) || !aligned16(workspace)) return MOE_ERR_BAD_ARG;
+    const size_t need = moe_linear_fp4_workspace_bytes(dtype, R, E, K, N), wb = al((size_t)E * (size_t)N * (size_t)K * elem_bytes(dtype));
+    if (!workspace || workspace_bytes < need) return MOE_ERR_WORKSPACE;
+    TRY(moe_launch_fp4_expand(codes, sce, scn, scales, sse, ssn, E, K, N, workspace, dtype, S(stream)));
+    return moe_scatter2scatter(x, ldx, 1, workspace, N * K, 1, K, nullptr, 0, 0, 0, nullptr, 0, 0, 0, 0, 0.f, y, ldy, 1, pos, pos64, offsets, off64, E, R, K, N, fan_out, x_grouped,
+                               y_grouped, dtype, (uint8_t*)workspace + wb, workspace_bytes - wb, stream);
+}
+
+int moe_linear_fp4_bwd(const void* dy, int64_t lddy, int dtype, const uint8_t* codes, int64_t sce, int64_t scn, const uint8_t* scales, int64_t sse, int64_t ssn, void* dx_rows,
+                       int64_t lddx, int dx_grouped, const void* pos, int pos64, const void* offsets, int off64, int E, int64_t R, int64_t K, int64_t N, void* workspace,
+                       size_t workspace_bytes, void* stream)
+{
+    if (dtype < 0 || dtype > 2 || E < 1 || R < 0 || K < 1 || N < 1) return MOE_ERR_BAD_ARG;
+    if (R == 0) return MOE_OK;
+    const MoeFp4Weights w = {codes, sce, scn, scales, sse, ssn};
+    if (lddy < 0 || (R > 1 && lddx < K) || !dy || !weights_ok(w) || !dx_rows || !offsets || (!dx_grouped && !pos) || !aligned16(workspace)) return MOE_ERR_BAD_ARG;
+    const size_t need = moe_linear_fp4_workspace_bytes(dtype, R, E, K, N), wb = al((size_t)E * (size_t)N * (size_t)K * elem_bytes(dtype));
+    if (!workspace || workspace_bytes < need) return MOE_ERR_WORKSPACE;
+    TRY(moe_launch_fp4_expand(codes, sce, scn, scales, sse, ssn, E, K, N, workspace, dtype, S(stream)));
+    return moe_scatter2scatter(dy, lddy, 1, workspace, N * K, K, 1, nullptr, 0, 0, 0, nullptr, 0, 0, 0, 0, 0.f, dx_rows, lddx, 1, pos, pos64, offsets, off64, E, R, N, K, 1, 1,
+                               dx_grouped, dtype, (uint8_t*)workspace + wb, workspace_bytes - wb, stream);
+}
+
+size_t moe_swiglu8_kept_bytes(int64_t rows, int64_t cols) { return rows < 1 || cols < 1 ? 0 : kept_bytes(rows, cols); }
+
+int moe_swiglu8_fwd(const void* gate, int64_t ldg, const void* up, int64_t ldu, void* h, int64_t ldh, void* kept, size_t kept_size, int64_t rows, int64_t cols, int dtype, void* stream)
+{
+    if (dtype < 0 || dtype > 2 || rows < 0 || cols < 0) return MOE_ERR_BAD_ARG;
+    if (rows == 0 || cols == 0) return MOE_OK;
+    if (!gate || !up || !h || ldg < 0 || ldu < 0 || (rows > 1 && ldh < cols) || !aligned16(kept)) return MOE_ERR_BAD_ARG;
+    if (kept && kept_size < kept_bytes(rows, cols)) return MOE_ERR_WORKSPACE;
+    MoeSwiglu8 p = {};
+    p.gate = gate; p.up = up; p.h = h; p.ldg = ldg; p.ldu = ldu; p.ldh = ldh;
+    TRY(swiglu8_params(p, (uint8_t*)kept, rows, cols));
+    const bool vec = cols % 8 == 0 && ldg % 8 == 0 && ldu % 8 == 0 && ldh % 8 == 0 && aligned16(gate) && aligned16(up) && aligned16(h);
+    return moe_launch_swiglu8(p, dtype, vec, false, S(stream));
+}
+
+int moe_swiglu8_bwd(const void* kept, size_t kept_size, const void* dh, int64_t lddh, void* dgate, int64_t lddg, void* dup, int64_t lddu, int64_t rows, int64_t cols, int dtype,
+                    void* stream)
+{
+    if (dtype < 0 || dtype > 2 || rows < 0 || cols < 0) return MOE_ERR_BAD_ARG;
+    if (rows == 0 || cols == 0) return MOE_OK;
+    if (!kept || !dh || !dgate || !dup || lddh < 0 || (rows > 1 && (lddg < cols || lddu < cols)) || !aligned16(kept)) return MOE_ERR_BAD_ARG;
+    if (kept_size < kept_bytes(rows, cols)) return MOE_ERR_WORKSPACE;
+    MoeSwiglu8 p = {};
+    p.dh = dh; p.dgate = dgate; p.dup = dup; p.ldg = lddg; p.ldu = lddu; p.ldh = lddh;
+    TRY(swiglu8_params(p, (uint8_t*)kept, rows, cols));
+    const bool vec = cols % 8 == 0 && lddh % 8 == 0 && lddg % 8 == 0 && lddu % 8 == 0 && aligned16(dh) && aligned16(dgate) && aligned16(dup);
+    return moe_launch_swiglu8(p, dtype, vec, true, S(stream));
+}
+
+}  // extern "C"

@@ -294,3 +294,27 @@ struct MoeI8Exchange { int64_t zeros, slots; };   // ints
 MoeI8Exchange moe_i8_exchange(int64_t R, int E, int64_t K, int64_t N, bool pair);   // K: all segments
 int moe_i8_tile(int64_t R, int E, int64_t K, int64_t N, bool pair, int nseg, int* parts);   // the tile size of a launch, and how many K parts its tiles may be cut into
 int moe_launch_i8_gemm(const MoeI8Gemm& p, int64_t R, hipStream_t stream);
+
+// ---- expert products over 4-bit weights (fp4.h) ----------------------------------------------------------------
+struct MoeFp4Weights {                  // codes (E, N, ceil(K/32) * 16 bytes), rows 16-byte aligned, and scales (E, N, ceil(K/32))
+    const uint8_t* codes; int64_t sce, scn;
+    const uint8_t* scales; int64_t sse, ssn;
+};
+int moe_launch_fp4_quantize(const void* W, int64_t swe, int64_t swk, int64_t swn, int dtype, int E, int64_t K, int64_t N, uint8_t* codes, int64_t sce, int64_t scn, uint8_t* scales,
+                            int64_t sse, int64_t ssn, hipStream_t stream);
+int moe_launch_fp4_expand(const uint8_t* codes, int64_t sce, int64_t scn, const uint8_t* scales, int64_t sse, int64_t ssn, int E, int64_t K, int64_t N, void* out, int dtype,
+                          hipStream_t stream);
+
+// ---- SwiGLU that keeps its inputs in 8 bits (swiglu8.hip) ------------------------------------------------------
+constexpr int MOE_KEPT_BLOCK = 64;      // columns that share a scale
+struct MoeSwiglu8 {
+    const void *gate, *up, *dh;
+    void *h, *dgate, *dup;
+    int64_t ldg, ldu, ldh;              // of gate and dgate, up and dup, h and dh
+    uint8_t* codes[2];                  // of gate and up: [rows][row_blocks][64]; null: nothing is kept
+    float* scales[2];                   // [rows][row_blocks]
+    int64_t cols;
+    uint32_t row_blocks, nblocks;       // blocks of a row, of all rows
+};
+// vec: columns and row pitches multiples of 8, addresses of 16 bytes
+int moe_launch_swiglu8(const MoeSwiglu8& p, int dtype, bool vec, bool backward, hipStream_t stream);

@@ -1,0 +1,177 @@
+// Part of torch_layer.cpp: the expert products over 4-bit weights and the SwiGLU that keeps its inputs in 8 bits as autograd functions.
+
+constexpr int64_t FP4_GROUP = 32, FP4_GROUP_BYTES = 16;
+inline int64_t fp4_groups(int64_t K) { return (K + FP4_GROUP - 1) / FP4_GROUP; }
+
+// (E, K, N) weights -> codes (E, N, groups * 16) and scales (E, N, groups), both uint8
+variable_list quantize_weights_fp4(const Tensor& w_)
+{
+    require_gpu({&w_});
+    TORCH_CHECK(w_.dim() == 3, "quantize_expert_weights_fp4 takes (experts, inputs, outputs), got ", w_.sizes());
+    const Tensor w = w_.detach();
+    const int64_t E = w.size(0), K = w.size(1), N = w.size(2), G = fp4_groups(K);
+    const int dt = dtype_code(w);
+    const c10::DeviceGuard guard(w.device());
+    Tensor codes = at::empty({E, N, G * FP4_GROUP_BYTES}, w.options().dtype(at::kByte)), scales = at::empty({E, N, G}, w.options().dtype(at::kByte));
+    if (w.numel() == 0) return {codes, scales};
+    check(moe_fp4_quantize_weights(ptr(w), w.stride(0), w.stride(1), w.stride(2), dt, (int)E, K, N, (uint8_t*)ptr(codes), codes.stride(0), codes.stride(1), (uint8_t*)ptr(scales),
+                                   scales.stride(0), scales.stride(1), stream_of(w)), "moe_fp4_quantize_weights");
+    return {codes, scales};
+}
+
+// codes and scales of (E, N, K) weights
+struct Fp4W {
+    Tensor codes, scales;
+    const uint8_t* c() const { return (const uint8_t*)ptr(codes); }
+    const uint8_t* s() const { return (const uint8_t*)ptr(scales); }
+};
+
+void check_fp4(const Tensor& codes, const Tensor& scales, int64_t K)
+{
+    TORCH_CHECK_TYPE(codes.scalar_type() == at::kByte, "4-bit weight codes are uint8, two to a byte, got ", codes.scalar_type());
+    TORCH_CHECK_TYPE(scales.scalar_type() == at::kByte, "scales of 4-bit weights are uint8 exponents, got ", scales.scalar_type());
+    TORCH_CHECK(codes.dim() == 3 && scales.dim() == 3, "4-bit weights are (experts, outputs, bytes) with scales (experts, outputs, groups), got ", codes.sizes(), " and ", scales.sizes());
+    TORCH_CHECK(scales.size(0) == codes.size(0) && scales.size(1) == codes.size(1) && scales.size(2) == fp4_groups(K) && codes.size(2) == scales.size(2) * FP4_GROUP_BYTES,
+                "codes of ", codes.sizes(), " with scales of ", scales.sizes(), " are not 4-bit weights of ", K, " inputs");
+}
+
+// as the kernels read them: rows of codes in 16-byte pieces, a row's scales one after the other
+Fp4W take_fp4(const Tensor& codes, const Tensor& scales)
+{
+    const bool ok = codes.stride(2) == 1 && codes.stride(0) % 16 == 0 && codes.stride(1) % 16 == 0 && (uintptr_t)codes.data_ptr() % 16 == 0;
+    Tensor c = ok ? codes : codes.contiguous();
+    if ((uintptr_t)c.data_ptr() % 16 != 0) c = c.clone();   // (contiguous already, at an address that 16-byte loads do not take)
+    return {c, scales.stride(2) == 1 ? scales : scales.contiguous()};
+}
+
+Tensor linear_fp4_rows(const Tensor& x, const Fp4W& w, const Tensor& ssi, const Tensor& eo, const LinearCfg& c, bool sums)
+{
+    const int64_t R = ssi.size(0), E = w.codes.size(0), K = x.size(1), N = w.codes.size(1);
+    (void)sums;
+    Tensor y = at::empty({R, N}, x.options());
+    if (R == 0 || N == 0) return y;
+    Tensor ws = bytes_on(x, moe_linear_fp4_workspace_bytes(dtype_code(x), R, (int)E, K, N));
+    check(moe_linear_fp4_fwd(ptr(x), x.stride(0), x.size(0), dtype_code(x), w.c(), w.codes.stride(0), w.codes.stride(1), w.s(), w.scales.stride(0), w.scales.stride(1), ptr(y), y.stride(0),
+                             dtype_code(y), ptr(ssi), is64(ssi), ptr(eo), is64(eo), (int)E, R, K, N, (int)c.k, c.grouped_in, c.grouped_out, ptr(ws), (size_t)ws.numel(), stream_of(x)),
+          "moe_linear_fp4_fwd");
+    return y;
+}
+
+struct LinearFp4Fn : Function<LinearFp4Fn> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& gates_, const Tensor& codes, const Tensor& scales, const Tensor& ssi, const Tensor& eo, const LinearCfg& c)
+    {
+        const Tensor gates = val(gates_);
+        Tensor y = linear_fp4_rows(x, take_fp4(codes, scales), ssi, eo, c, gates.defined()), y_rows;
+        if (gates.defined()) {
+            y_rows = y;
+            y = combine(y_rows, gates, nullptr, gates.size(1), gates.size(0));
+        }
+        ctx->save_for_backward({codes, scales, gates, ssi, eo, gates.defined() && gates.requires_grad() ? y_rows : Tensor()});
+        ctx->saved_data["K"] = x.size(1);
+        ctx->saved_data["k"] = c.k;
+        ctx->saved_data["flags"] = (int64_t)(c.grouped_in | (c.grouped_out << 1));
+        return y;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list g)
+    {
+        const auto sv = ctx->get_saved_variables();
+        const Tensor& gates = sv[2];
+        const c10::DeviceGuard guard(sv[0].device());
+        const Fp4W w = take_fp4(sv[0], sv[1]);
+        const Tensor ssi = sv[3].contiguous(), eo = sv[4].contiguous();   // (a saved-tensor hook may hand back other strides)
+        const int64_t k = ctx->saved_data["k"].toInt(), flags = ctx->saved_data["flags"].toInt(), K = ctx->saved_data["K"].toInt(), E = w.codes.size(0), N = w.codes.size(1), R = ssi.size(0);
+        const bool grouped_in = flags & 1, grouped_out = flags & 2;
+        const Tensor dout = g[0].contiguous();
+        Tensor dx, d_gates;
+        int64_t gate_fan = 1;
+        if (gates.defined()) {
+            gate_fan = gates.size(1);
+            if (ctx->needs_input_grad(1)) d_gates = combine_dgates(sv[5].contiguous(), dout, gate_fan, gates.scalar_type(), nullptr);
+        }
+        if (ctx->needs_input_grad(0)) {
+            dx = at::empty({R, K}, dout.options());
+            if (R > 0 && N > 0) {
+                const Tensor dy = grouped_out ? dout : group_rows(dout, ptr(ssi), is64(ssi), R, gate_fan, flat_gates(gates));
+                Tensor ws = bytes_on(dout, moe_linear_fp4_workspace_bytes(dtype_code(dout), R, (int)E, K, N));
+                check(moe_linear_fp4_bwd(ptr(dy), dy.stride(0), dtype_code(dy), w.c(), w.codes.stride(0), w.codes.stride(1), w.s(), w.scales.stride(0), w.scales.stride(1), ptr(dx),
+                                         dx.stride(0), grouped_in, ptr(ssi), is64(ssi), ptr(eo), is64(eo), (int)E, R, K, N, ptr(ws), (size_t)ws.numel(), stream_of(dout)),
+                      "moe_linear_fp4_bwd");
+            } else dx.zero_();
+            if (k != 1) dx = combine(dx, Tensor(), nullptr, k, R / k);
+        }
+        return {dx, d_gates, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+Tensor linear_fp4(const Tensor& x_, const Tensor& codes, const Tensor& scales, int64_t k, const Tensor& sei, const Tensor& ssi_, const OptTensor& eo_in, const OptTensor& gates_in,
+                  bool grouped_in, bool grouped_out)
+{
+    const Tensor eo_ = val(eo_in), gates_ = val(gates_in);
+    require_gpu({&x_, &codes, &scales, &sei, &ssi_, &eo_, &gates_});
+    MOE_ASSERT(x_.dim() == 2, "X has to be (rows, inputs).");
+    TORCH_CHECK(x_.size(1) >= 1, "rows of ", x_.sizes(), " hold nothing to multiply");
+    check_fp4(codes, scales, x_.size(1));
+    TORCH_CHECK(codes.size(0) >= 1, "expert weights of ", codes.sizes(), " hold nothing to multiply by");
+    MOE_ASSERT(ssi_.dim() == 1 && sei.dim() == 1 && ssi_.size(0) == sei.size(0), "sorted_scattered_idxs and sorted_expert_idxs differ in length");
+    MOE_ASSERT(k >= 1 && ssi_.size(0) == x_.size(0) * k, "the number of assignments is not rows of X times k");
+    MOE_ASSERT(!grouped_in || k == 1, "grouped rows of X are one for each assignment: k is 1 with them");
+    MOE_ASSERT(!grouped_out || !gates_.defined(), "gates combine rows in token order: not with a grouped output");
+    dtype_code(x_);
+    is64(ssi_);
+    is64(sei);
+    if (eo_.defined()) { check_offsets(eo_, codes.size(0)); is64(eo_); }
+    check_gates(gates_, ssi_.size(0));
+    if (gates_.defined()) dtype_code(gates_);
+    const c10::DeviceGuard guard(x_.device());
+    const Tensor x = unit_inner(x_), ssi = ssi_.contiguous(), eo = eo_.defined() ? eo_.contiguous() : offsets_from_sorted(sei, codes.size(0));
+    const Tensor gates = gates_.defined() ? gates_.contiguous() : Tensor();
+    const LinearCfg c{0.0, 0.0, k, grouped_in, grouped_out};
+    if (needs_node({&x, &gates})) return LinearFp4Fn::apply(x, opt(gates), codes, scales, ssi, eo, c);
+    Tensor y = linear_fp4_rows(x, take_fp4(codes, scales), ssi, eo, c, gates.defined());
+    return gates.defined() ? combine(y, gates, nullptr, gates.size(1), gates.size(0)) : y;
+}
+
+// ---- SwiGLU with its inputs kept in 8 bits
+Tensor swiglu8_forward(const Tensor& gate, const Tensor& up, at::IntArrayRef sizes, Tensor* kept)
+{
+    const int64_t rows = gate.size(0), cols = gate.size(1);
+    Tensor h = at::empty(sizes, gate.options());
+    if (kept) *kept = bytes_on(gate, moe_swiglu8_kept_bytes(rows, cols));
+    check(moe_swiglu8_fwd(ptr(gate), gate.stride(0), ptr(up), up.stride(0), ptr(h), cols, kept ? ptr(*kept) : nullptr, kept ? (size_t)kept->numel() : 0, rows, cols, dtype_code(gate),
+                          stream_of(gate)), "moe_swiglu8_fwd");
+    return h;
+}
+
+// rows of any pitch whose columns lie one after the other
+Tensor as_rows(const Tensor& t) { return unit_inner(t.dim() == 2 ? t : t.reshape({t.numel() / (t.size(-1) ? t.size(-1) : 1), t.size(-1)})); }
+
+struct Swiglu8Fn : Function<Swiglu8Fn> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& gate, const Tensor& up)
+    {
+        Tensor kept, h = swiglu8_forward(as_rows(gate), as_rows(up), gate.sizes(), &kept);
+        ctx->save_for_backward({kept});
+        ctx->saved_data["sizes"] = gate.sizes().vec();
+        return h;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list g)
+    {
+        const Tensor kept = ctx->get_saved_variables()[0].contiguous();
+        const c10::DeviceGuard guard(kept.device());
+        const auto sizes = ctx->saved_data["sizes"].toIntVector();
+        const Tensor dh = as_rows(g[0]);
+        const int64_t rows = dh.size(0), cols = dh.size(1);
+        Tensor dg = at::empty(sizes, dh.options()), du = at::empty(sizes, dh.options());
+        check(moe_swiglu8_bwd(ptr(kept), (size_t)kept.numel(), ptr(dh), dh.stride(0), ptr(dg), cols, ptr(du), cols, rows, cols, dtype_code(dh), stream_of(dh)), "moe_swiglu8_bwd");
+        return {dg, du};
+    }
+};
+
+Tensor swiglu_8bit(const Tensor& gate, const Tensor& up)
+{
+    require_gpu({&gate, &up});
+    TORCH_CHECK(gate.dim() >= 1 && gate.sizes() == up.sizes(), "gate of ", gate.sizes(), " and up of ", up.sizes(), " differ in shape");
+    MOE_ASSERT(gate.scalar_type() == up.scalar_type(), "gate and up must share a dtype");
+    dtype_code(gate);
+    const c10::DeviceGuard guard(gate.device());
+    return needs_node({&gate, &up}) ? Swiglu8Fn::apply(gate, up) : swiglu8_forward(as_rows(gate), as_rows(up), gate.sizes(), nullptr);
+}

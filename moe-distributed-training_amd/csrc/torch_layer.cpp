@@ -835,6 +835,11 @@ variable_list layer(const Tensor& x, const Tensor& wg, const Tensor& w1_, const 
 // ---------------------------------------------------------------------------------------------------------------
 #include "torch_int8.h"
 
+// ---------------------------------------------------------------------------------------------------------------
+// ... over 4-bit weights, and the activation that keeps 8 bits
+// ---------------------------------------------------------------------------------------------------------------
+#include "torch_fp4.h"
+
 }  // namespace
 
 // Called from Python without the interpreter lock.  The wrapper carries a Python exception that is raised below (a saved-tensor
@@ -852,6 +857,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
     m.def("linear_int8", torch::wrap_pybind_function_no_gil(linear_int8));
     m.def("expert_mlp_int8", torch::wrap_pybind_function_no_gil(expert_mlp_int8));
     m.def("layer_int8", torch::wrap_pybind_function_no_gil(layer_int8));
+    m.def("quantize_weights_fp4", torch::wrap_pybind_function_no_gil(quantize_weights_fp4));
+    m.def("linear_fp4", torch::wrap_pybind_function_no_gil(linear_fp4));
+    m.def("swiglu_8bit", torch::wrap_pybind_function_no_gil(swiglu_8bit));
 }
 
 // The same functions as dispatcher operators, for torch.jit.trace: a trace records operators, and of the functions above it
@@ -884,4 +892,10 @@ TORCH_LIBRARY(moe_hip, m)
     });
     m.def("layer_int8", [](const Tensor& x, const Tensor& wg, const Tensor& w1, const Tensor& s1, const Tensor& w2, const Tensor& s2, const Tensor& w3,
                            const Tensor& s3, int64_t k, bool normalize) { return layer_int8(x, wg, w1, s1, w2, s2, w3, s3, k, normalize); });
+    m.def("quantize_weights_fp4", [](const Tensor& w) { return quantize_weights_fp4(w); });
+    m.def("linear_fp4", [](const Tensor& x, const Tensor& codes, const Tensor& scales, int64_t k, const Tensor& sei, const Tensor& ssi, const OptTensor& eo,
+                           const OptTensor& gates, bool grouped_in, bool grouped_out) {
+        return linear_fp4(x, codes, scales, k, sei, ssi, eo, gates, grouped_in, grouped_out);
+    });
+    m.def("swiglu_8bit", [](const Tensor& gate, const Tensor& up) { return swiglu_8bit(gate, up); });
 }

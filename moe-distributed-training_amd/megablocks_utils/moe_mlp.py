@@ -102,6 +102,14 @@ def fused_expert_mlp_int8(x, weights: Int8ExpertWeights, k, sorted_scattered_idx
                                     sorted_scattered_idxs, expert_offsets, gates, grouped_out)
 
 
+def swiglu_8bit(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
+    """``silu(gate) * up`` of bf16, fp16 or fp32 tensors of one shape (any strides), keeping for the backward pass 8-bit codes of gate and up
+    in place of the tensors: blocks of 64 columns with a scale each, 1.0625 bytes per value.  The result is that of the inputs as they
+    are; the gradients are the formula's at the values that the codes stand for (off by at most 1/254 of their block's largest
+    magnitude).  A block that holds an infinity or a NaN has NaN gradients."""
+    return entry("swiglu_8bit")(gate, up)
+
+
 def scattermoe_permute_and_compute(x, w1, w2, w3, ffn_hidden_size, hidden_size, top_k, bin_ids, indices, num_experts,
                                    lora_pointers=None, moe_expert_model_parallelism=True, expert_offsets=None,
                                    lora_views: Optional[LoraViews] = None, lora_alpha: float = 1.0):

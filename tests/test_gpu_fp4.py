@@ -1,0 +1,205 @@
+"""Expert products over 4-bit weights against their definition in 64 bits.
+
+The weights are what their codes say, so a projection's result is off by its last rounding (half a step of its type) and by the roundings of a
+32-bit sum: at most (terms + 8) * 2^-24 of the sum of the terms' magnitudes, whatever their order."""
+import pytest
+import torch
+
+import moe_distributed_training_amd as moe
+from oracle import fp4_oracle as oracle
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+ROWS = 1.0   # rows of one assignment are rounded to the type before they are summed per token
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def close(got, want, slack, what):
+    got = got.detach().double().cpu()
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    assert not torch.isnan(got).any(), f"{what}: NaN"
+    over = (got - want).abs() - slack
+    assert float(over.max()) <= 0, f"{what}: {float(over.max()):.3g} past its bound at {torch.nonzero(over == over.max())[0].tolist()}"
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# weights into codes
+# ---------------------------------------------------------------------------------------------------------------
+def check_codes(w, dev):
+    codes, scales = moe.quantize_expert_weights_fp4(w.to(dev))
+    c, s = oracle.quantize(w)
+    assert codes.dtype == torch.uint8 and scales.dtype == torch.uint8
+    assert torch.equal(scales.cpu(), s), "scales differ"
+    assert torch.equal(codes.cpu(), c), "codes differ"
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("E,K,N", [(1, 1, 1), (2, 31, 3), (3, 32, 64), (2, 33, 5), (4, 129, 70), (1, 1000, 24)])
+def test_weights_become_the_nearest_codes(dev, dtype, E, K, N):
+    g = torch.Generator().manual_seed(K * 3 + N)
+    w = (torch.randn(E, K, N, generator=g) * torch.exp(torch.randn(E, 1, N, generator=g))).to(dtype)
+    check_codes(w, dev)
+    check_codes(w.transpose(1, 2).contiguous().transpose(1, 2), dev)          # contiguous along the inputs
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_weights_at_borders_and_ends_of_their_type(dev, dtype):
+    fi = torch.finfo(dtype)
+    K = 64
+    w = torch.zeros(1, K, 16, dtype=torch.float64)
+    quarter = torch.arange(-32, 32).double() / 4                              # every border between codes, and their neighbours
+    w[0, :, 0] = quarter
+    w[0, :, 1] = quarter * 7 / 8                                              # largest magnitude 7 units: still this power
+    w[0, :, 2] = quarter * 2.0 ** -6
+    w[0, 5, 3] = fi.max
+    w[0, :, 4] = fi.max * quarter / 8
+    w[0, 40, 5] = fi.tiny
+    w[0, :, 6] = quarter * fi.tiny * (4 if dtype == F16 else 64)
+    w[0, 3, 7], w[0, 4, 7] = float("inf"), 1.0
+    w[0, 33, 8] = float("nan")
+    w[0, 63, 9], w[0, 1, 9] = float("-inf"), -2.0
+    w[0, :, 10] = -quarter
+    w[0, 31, 11], w[0, 32, 11] = 7.0, 7.03125                                 # one group each: 7 units, and just above
+    check_codes(w.to(dtype), dev)
+
+
+def test_weights_of_nothing(dev):
+    c, s = moe.quantize_expert_weights_fp4(torch.empty(2, 64, 0, device=dev))
+    assert c.shape == (2, 0, 32) and s.shape == (2, 0, 2)
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# one projection
+# ---------------------------------------------------------------------------------------------------------------
+def make(T, K, N, E, k, dtype, seed=0, absent=()):
+    g = torch.Generator().manual_seed(seed * 101 + T + K + N)
+    x = (torch.randn(T, K, generator=g) * torch.exp(0.4 * torch.randn(T, 1, generator=g))).to(dtype)
+    codes, scales = oracle.quantize(torch.randn(E, K, N, generator=g) * 0.02)
+    return x, codes, scales, oracle.route(T, E, k, seed + 5, absent), g
+
+
+def check_linear(dev, T, K, N, E, k, dtype, gates=True, train=True, grouped_in=False, grouped_out=False, absent=(), index=torch.int64, move=lambda t: t, seed=0):
+    x, codes, scales, (sei, ssi, offs, gw), g = make(T, K, N, E, k, dtype, seed, absent)
+    gw = gw.to(dtype) if gates else None
+    dout = torch.randn(T if gates else T * k, N, generator=g).to(dtype) if train else None
+    want = oracle.linear(x, oracle.weights(codes, scales, K), k, sei, ssi, gw, dout, grouped_in, grouped_out)
+    xd = move(x.to(dev)).requires_grad_(train)
+    gd = gw.to(dev).requires_grad_(train) if gates else None
+    y = moe.parallel_linear_fp4(xd, move(codes.to(dev)), move(scales.to(dev)), k, sei.to(dev, index), ssi.to(dev, index), None, offs.to(dev, index), gd, grouped_in, grouped_out)
+    assert y.dtype == dtype
+    u, a = half_step(dtype), 2.0 ** -24
+    rows = ROWS * u if gates else 0.0
+    close(y, want["y"], (u * want["y"].abs() + (rows + 4 * a) * want["y_sums"]) * (1 + 4 * u) + (K + 8) * a * want["y_terms"], "y")
+    if not train:
+        return
+    grads = torch.autograd.grad(y, [xd, gd] if gates else [xd], dout.to(dev))
+    rows = ROWS * u * ((k > 1) * want["dx_sums"] + gates * want["dx_terms"])
+    close(grads[0], want["dx"], (u * want["dx"].abs() + rows + 4 * a * want["dx_sums"]) * (1 + 4 * u) + (N + 8) * a * want["dx_terms"], "dx")
+    if gates:
+        close(grads[1], want["d_gates"], (u * want["d_gates"].abs() + ROWS * u * want["d_gates_sums"]) * (1 + 4 * u) + ((N + 8) + (K + 8)) * a * want["d_gates_terms"], "d_gates")
+
+
+SIZES = [  # T, K, N, E, k
+    (1, 64, 64, 8, 2), (1, 32, 16, 1, 1), (3, 1, 5, 2, 1), (7, 31, 33, 3, 2), (16, 128, 256, 4, 2), (33, 256, 64, 4, 1), (5, 1000, 72, 8, 2), (50, 1000, 136, 8, 2),
+    (130, 192, 320, 2, 2), (64, 2048, 48, 16, 4), (300, 264, 200, 5, 3), (600, 512, 520, 3, 2), (40, 136, 1000, 2, 1),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("T,K,N,E,k", SIZES)
+def test_projection(dev, dtype, T, K, N, E, k):
+    check_linear(dev, T, K, N, E, k, dtype)
+    check_linear(dev, T, K, N, E, k, dtype, gates=False)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("grouped_in,grouped_out", [(True, False), (False, True), (True, True)])
+def test_grouped_rows(dev, dtype, grouped_in, grouped_out):
+    check_linear(dev, 150, 256, 192, 4, 1, dtype, gates=False, grouped_in=grouped_in, grouped_out=grouped_out)
+    check_linear(dev, 9, 96, 40, 4, 1, dtype, gates=False, grouped_in=grouped_in, grouped_out=grouped_out)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_experts_without_rows_and_int32_indices(dev, dtype):
+    check_linear(dev, 40, 128, 96, 9, 2, dtype, absent=(0, 3, 8), index=torch.int32)
+    check_linear(dev, 2, 128, 96, 100, 1, dtype, absent=tuple(range(60)))
+
+
+def _strided(t):
+    """The same values in memory where no row is contiguous and nothing is aligned."""
+    buf = torch.empty(tuple(s + 1 for s in t.shape[:-1]) + (2 * t.shape[-1] + 1,), dtype=t.dtype, device=t.device)
+    view = buf[tuple(slice(1, None) for _ in t.shape[:-1]) + (slice(1, None, 2),)]
+    return view.copy_(t)
+
+
+def _offset(t):
+    """The same values in rows of an odd pitch, at an odd address."""
+    buf = torch.empty(t.shape[:-1] + (t.shape[-1] + 3,), dtype=t.dtype, device=t.device)
+    return buf[..., 3:].copy_(t)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("move", [_strided, _offset])
+def test_strides(dev, dtype, move):
+    check_linear(dev, 5, 256, 72, 4, 2, dtype, move=lambda t: move(t.detach()))
+    check_linear(dev, 90, 200, 136, 4, 2, dtype, move=lambda t: move(t.detach()))
+
+
+def test_scales_at_the_ends(dev):
+    """The least and largest powers of two: bf16 holds every such weight; a scale of 255 makes the rows of its group's expert NaN and nothing else."""
+    x, codes, scales, (sei, ssi, offs, _), g = make(20, 96, 64, 3, 1, BF16)
+    scales[0, 5, :] = 0
+    scales[1, 7, 1] = 240
+    args = (sei.to(dev), ssi.to(dev), None, offs.to(dev))
+    want = oracle.linear(x, oracle.weights(codes, scales, 96), 1, sei, ssi)
+    y = moe.parallel_linear_fp4(x.to(dev), codes.to(dev), scales.to(dev), 1, *args)
+    close(y, want["y"], half_step(BF16) * want["y"].abs() + 104 * 2.0 ** -24 * want["y_terms"] + 2.0 ** -133, "y")
+    scales[2, 9, 2] = 255
+    y2 = moe.parallel_linear_fp4(x.to(dev), codes.to(dev), scales.to(dev), 1, *args)
+    hit = torch.zeros(20, 64, dtype=torch.bool)
+    hit[ssi[sei == 2], 9] = True
+    assert torch.equal(torch.isnan(y2).cpu(), hit)
+    assert torch.equal(y2.cpu()[~hit], y.cpu()[~hit])
+
+
+def test_infinities_stay_in_their_rows(dev):
+    x, codes, scales, (sei, ssi, offs, _), g = make(70, 160, 96, 3, 2, BF16)
+    args = (codes.to(dev), scales.to(dev), 2, sei.to(dev), ssi.to(dev), None, offs.to(dev))
+    clean = moe.parallel_linear_fp4(x.to(dev), *args).cpu()
+    x[11, 3], x[40, 159] = float("inf"), float("nan")
+    y = moe.parallel_linear_fp4(x.to(dev), *args).cpu()
+    rows = torch.ones(140, dtype=torch.bool)
+    rows[22:24] = rows[80:82] = False
+    assert torch.equal(y[rows], clean[rows]) and not torch.isfinite(y[~rows]).all()
+
+
+def test_empty_batches(dev):
+    codes, scales = (t.to(dev) for t in oracle.quantize(torch.randn(3, 64, 32)))
+    z = torch.zeros(0, dtype=torch.int64, device=dev)
+    x = torch.empty(0, 64, dtype=BF16, device=dev, requires_grad=True)
+    y = moe.parallel_linear_fp4(x, codes, scales, 2, z, z, None, torch.zeros(3, dtype=torch.int64, device=dev))
+    assert y.shape == (0, 32)
+    assert torch.autograd.grad(y.sum(), x)[0].shape == (0, 64)
+
+
+def test_rows_behind_the_last_group_are_left_as_they_were(dev):
+    """Offsets that end before the rows do: what no group covers is not read and not written (C entry, output of the caller's own)."""
+    from moe_distributed_training_amd import _lib
+    for T in (6, 80):
+        x, codes, scales, (sei, ssi, offs, _), g = make(T, 128, 64, 2, 1, BF16)
+        offs = offs.clone()
+        offs[1] -= 2
+        xd, cd, sd, pd, od = x.to(dev), codes.to(dev), scales.to(dev), ssi.to(dev), offs.to(dev)
+        y = torch.full((T, 64), 7.0, dtype=BF16, device=dev)
+        n = _lib.lib.moe_linear_fp4_workspace_bytes(0, T, 2, 128, 64)
+        ws = torch.empty(max(n, 256), dtype=torch.uint8, device=dev)
+        _lib.check(_lib.lib.moe_linear_fp4_fwd(xd.data_ptr(), 128, T, 0, cd.data_ptr(), cd.stride(0), cd.stride(1), sd.data_ptr(), sd.stride(0), sd.stride(1), y.data_ptr(), 64, 0,
+                                               pd.data_ptr(), 1, od.data_ptr(), 1, 2, T, 128, 64, 1, 0, 0, ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream), "fwd")
+        assert bool((y[ssi[-2:].to(dev)] == 7.0).all())
+        want = oracle.linear(x, oracle.weights(codes, scales, 128), 1, sei, ssi)
+        at = ssi[:-2]
+        close(y.cpu()[at], want["y"][at], half_step(BF16) * want["y"][at].abs() + 136 * 2.0 ** -24 * want["y_terms"][at], "y")
