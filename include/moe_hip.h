@@ -316,7 +316,8 @@ int moe_fp4_quantize_weights(const void* W, int64_t swe, int64_t swk, int64_t sw
 /* moe_scatter2scatter without adapters over 4-bit weights: y[out_row] = x[in_row] @ W[e], rows addressed as there; x has x_rows rows.  Weights enter as numbers of
  * x's type: exact in bf16 and fp32; in fp16 for scales from 104 to 140, beyond which they round (or overflow) as a conversion to fp16 does.
  * Backward (weights frozen): dy in grouped order, dx_rows[dx_grouped ? m : pos[m]] = dy[m] @ W[e]^T.  Rows that no group covers are not written. */
-size_t moe_linear_fp4_workspace_bytes(int dtype, int64_t R, int E, int64_t K, int64_t N);
+size_t moe_linear_fp4_workspace_bytes(const void* x, int64_t ldx, int64_t x_rows, int x_grouped, int dtype, int64_t R, int E, int64_t K, int64_t N);
+size_t moe_linear_fp4_bwd_workspace_bytes(int dtype, int64_t R, int E, int64_t K, int64_t N);
 int moe_linear_fp4_fwd(const void* x, int64_t ldx, int64_t x_rows, int dtype, const uint8_t* codes, int64_t sce, int64_t scn, const uint8_t* scales, int64_t sse, int64_t ssn,
                        void* y, int64_t ldy, int y_dtype, const void* pos, int pos64, const void* offsets, int off64, int E, int64_t R, int64_t K, int64_t N, int fan_out,
                        int x_grouped, int y_grouped, void* workspace, size_t workspace_bytes, void* stream);

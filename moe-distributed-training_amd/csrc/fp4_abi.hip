@@ -16,6 +16,15 @@ inline size_t elem_bytes(int dtype) { return dtype == MOE_F32 ? 4 : 2; }
 // rows of codes that 16-byte loads take, and scales that lie one after the other
 bool weights_ok(const MoeFp4Weights& w) { return w.codes && w.scales && aligned16(w.codes) && w.sce % 16 == 0 && w.scn % 16 == 0; }
 
+// rows that 16-byte loads take as they are; otherwise they are packed
+bool rows_ok(const void* x, int64_t ldx, int64_t x_rows, int64_t K, int x_grouped)
+{
+    return aligned16(x) && ldx % 8 == 0 && K % 8 == 0 && ((x_grouped ? 128 : x_rows) * ldx + K) * 2 < MOE_FP4_RANGE;
+}
+int64_t packed_cols(int64_t K) { return (K + 7) / 8 * 8; }
+size_t packed_bytes(int64_t R, int64_t K) { return al((size_t)R * (size_t)packed_cols(K) * 2); }
+size_t expanded_bytes(int E, int64_t K, int64_t N, int dtype) { return al((size_t)E * (size_t)N * (size_t)K * elem_bytes(dtype)); }
+
 struct Kept { size_t codes, scales; };
 Kept kept_sizes(int64_t rows, int64_t cols)
 {
@@ -51,27 +60,48 @@ int moe_fp4_quantize_weights(const void* W, int64_t swe, int64_t swk, int64_t sw
     return moe_launch_fp4_quantize(W, swe, swk, swn, dtype, E, K, N, codes, sce, scn, scales, sse, ssn, S(stream));
 }
 
-size_t moe_linear_fp4_workspace_bytes(int dtype, int64_t R, int E, int64_t K, int64_t N)
+size_t moe_linear_fp4_workspace_bytes(const void* x, int64_t ldx, int64_t x_rows, int x_grouped, int dtype, int64_t R, int E, int64_t K, int64_t N)
 {
     if (dtype < 0 || dtype > 2 || R < 1 || E < 1 || K < 1 || N < 1) return 0;
-    const size_t fwd = moe_scatter2scatter_workspace_bytes(R, E, K, N, 0), bwd = moe_scatter2scatter_workspace_bytes(R, E, N, K, 0);
-    return al((size_t)E * (size_t)N * (size_t)K * elem_bytes(dtype)) + (fwd > bwd ? fwd : bwd);   // (of either direction)
+    if (dtype != MOE_F32) return rows_ok(x, ldx, x_rows, K, x_grouped) ? 0 : packed_bytes(R, K);
+    return expanded_bytes(E, K, N, dtype) + moe_scatter2scatter_workspace_bytes(R, E, K, N, 0);
 }
 
 int moe_linear_fp4_fwd(const void* x, int64_t ldx, int64_t x_rows, int dtype, const uint8_t* codes, int64_t sce, int64_t scn, const uint8_t* scales, int64_t sse, int64_t ssn, void* y,
                        int64_t ldy, int y_dtype, const void* pos, int pos64, const void* offsets, int off64, int E, int64_t R, int64_t K, int64_t N, int fan_out, int x_grouped,
                        int y_grouped, void* workspace, size_t workspace_bytes, void* stream)
 {
-    if (dtype < 0 || dtype > 2 || y_dtype != dtype || E < 1 || R < 0 || x_rows < 0 || K < 1 || N < 0 || fan_out < 1) return MOE_ERR_BAD_ARG;
+    if (dtype < 0 || dtype > 2 || y_dtype < 0 || y_dtype > 2 || E < 1 || R < 0 || x_rows < 0 || K < 1 || N < 0 || fan_out < 1) return MOE_ERR_BAD_ARG;
     if (R == 0 || N == 0) return MOE_OK;
     if (ldx < 0 || (R > 1 && ldy < N)) return MOE_ERR_BAD_ARG;   // (rows of an input may overlap)
     const MoeFp4Weights w = {codes, sce, scn, scales, sse, ssn};
     if (!x || x_rows < 1 || !weights_ok(w) || !y || !offsets || ((!x_grouped || !y_grouped) && !pos) || (x_grouped && x_rows < R) || !aligned16(workspace)) return MOE_ERR_BAD_ARG;
-    const size_t need = moe_linear_fp4_workspace_bytes(dtype, R, E, K, N), wb = al((size_t)E * (size_t)N * (size_t)K * elem_bytes(dtype));
-    if (!workspace || workspace_bytes < need) return MOE_ERR_WORKSPACE;
-    TRY(moe_launch_fp4_expand(codes, sce, scn, scales, sse, ssn, E, K, N, workspace, dtype, S(stream)));
-    return moe_scatter2scatter(x, ldx, 1, workspace, N * K, 1, K, nullptr, 0, 0, 0, nullptr, 0, 0, 0, 0, 0.f, y, ldy, 1, pos, pos64, offsets, off64, E, R, K, N, fan_out, x_grouped,
-                               y_grouped, dtype, (uint8_t*)workspace + wb, workspace_bytes - wb, stream);
+    const size_t need = moe_linear_fp4_workspace_bytes(x, ldx, x_rows, x_grouped, dtype, R, E, K, N);
+    if (need && (!workspace || workspace_bytes < need)) return MOE_ERR_WORKSPACE;
+    if (K > 0x3fffffff || E > 65535) return MOE_ERR_UNSUPPORTED;
+    if (dtype != MOE_F32 && (N * scn >= MOE_FP4_RANGE || N * ssn >= MOE_FP4_RANGE || packed_cols(K) * 256 >= MOE_FP4_RANGE)) return MOE_ERR_UNSUPPORTED;
+    if (dtype == MOE_F32) {
+        if (y_dtype != MOE_F32) return MOE_ERR_UNSUPPORTED;
+        const size_t wb = expanded_bytes(E, K, N, dtype);
+        TRY(moe_launch_fp4_expand(codes, sce, scn, scales, sse, ssn, E, K, N, workspace, dtype, S(stream)));
+        return moe_scatter2scatter(x, ldx, 1, workspace, N * K, 1, K, nullptr, 0, 0, 0, nullptr, 0, 0, 0, 0, 0.f, y, ldy, 1, pos, pos64, offsets, off64, E, R, K, N, fan_out, x_grouped,
+                                   y_grouped, dtype, (uint8_t*)workspace + wb, workspace_bytes - wb, stream);
+    }
+    MoeFp4Gemm g = {};
+    g.X = x; g.ldx = ldx; g.w = w; g.Y = y; g.ldy = ldy; g.ydtype = y_dtype; g.pos = pos; g.pos64 = pos64; g.offsets = offsets; g.off64 = off64;
+    g.E = E; g.K = (int)K; g.N = N; g.fan_out = fan_out; g.x_grouped = x_grouped; g.y_grouped = y_grouped; g.f16 = dtype == MOE_F16;
+    if (need) {   // rows in the order of the product, padded
+        const int64_t ld = packed_cols(K);
+        TRY(moe_launch_fp4_pack_rows(x, ldx, x_grouped ? nullptr : pos, pos64, fan_out, offsets, off64, E, R, K, workspace, ld, S(stream)));
+        g.X = workspace; g.ldx = ld; g.K = (int)ld; g.x_grouped = 1;
+    }
+    return moe_launch_fp4_gemm(g, R, S(stream));
+}
+
+size_t moe_linear_fp4_bwd_workspace_bytes(int dtype, int64_t R, int E, int64_t K, int64_t N)
+{
+    if (dtype < 0 || dtype > 2 || R < 1 || E < 1 || K < 1 || N < 1) return 0;
+    return expanded_bytes(E, K, N, dtype) + moe_scatter2scatter_workspace_bytes(R, E, N, K, 0);
 }
 
 int moe_linear_fp4_bwd(const void* dy, int64_t lddy, int dtype, const uint8_t* codes, int64_t sce, int64_t scn, const uint8_t* scales, int64_t sse, int64_t ssn, void* dx_rows,
@@ -82,7 +112,7 @@ int moe_linear_fp4_bwd(const void* dy, int64_t lddy, int dtype, const uint8_t* c
     if (R == 0) return MOE_OK;
     const MoeFp4Weights w = {codes, sce, scn, scales, sse, ssn};
     if (lddy < 0 || (R > 1 && lddx < K) || !dy || !weights_ok(w) || !dx_rows || !offsets || (!dx_grouped && !pos) || !aligned16(workspace)) return MOE_ERR_BAD_ARG;
-    const size_t need = moe_linear_fp4_workspace_bytes(dtype, R, E, K, N), wb = al((size_t)E * (size_t)N * (size_t)K * elem_bytes(dtype));
+    const size_t need = moe_linear_fp4_bwd_workspace_bytes(dtype, R, E, K, N), wb = expanded_bytes(E, K, N, dtype);
     if (!workspace || workspace_bytes < need) return MOE_ERR_WORKSPACE;
     TRY(moe_launch_fp4_expand(codes, sce, scn, scales, sse, ssn, E, K, N, workspace, dtype, S(stream)));
     return moe_scatter2scatter(dy, lddy, 1, workspace, N * K, K, 1, nullptr, 0, 0, 0, nullptr, 0, 0, 0, 0, 0.f, dx_rows, lddx, 1, pos, pos64, offsets, off64, E, R, N, K, 1, 1,

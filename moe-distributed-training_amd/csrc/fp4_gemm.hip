@@ -1,0 +1,139 @@
+// Grouped product of 16-bit rows with 4-bit weights (fp4.h) over ragged expert groups:
+//
+//   Y[out_row(m)][n] = sum_k X[in_row(m)][k] W[e(m)][n][k]
+//
+// Few rows per expert: fp4_few_rows_kernel, which streams the codes (few_rows.h).
+#include "few_rows.h"
+#include "kernels.h"
+
+namespace {
+
+// four consecutive values of a row
+__device__ __forceinline__ void store4(void* Y, int64_t at, int dtype, f32x4_t v, int live, bool vec)
+{
+    if (dtype == MOE_F32) {
+        float* y = (float*)Y + at;
+        if (vec && live == 4) { *(float4*)y = make_float4(v[0], v[1], v[2], v[3]); return; }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < live) y[i] = v[i];
+        return;
+    }
+    uint16_t* y = (uint16_t*)Y + at;
+    uint2 o;
+    if (dtype == MOE_BF16) { o.x = NumBf16::pack2(v[0], v[1]); o.y = NumBf16::pack2(v[2], v[3]); }
+    else { o.x = NumF16::pack2(v[0], v[1]); o.y = NumF16::pack2(v[2], v[3]); }
+    if (vec && live == 4) { *(uint2*)y = o; return; }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (i < live) y[i] = (uint16_t)((i < 2 ? o.x : o.y) >> (16 * (i & 1)));
+}
+
+// A workgroup: one row tile of 16 MB rows, 16 NB columns; its waves share the contraction and add up their sums in LDS, in wave order.
+template <class Num, int MB, int NB>
+__global__ void __launch_bounds__(512) fp4_few_rows_kernel(const MoeFp4Gemm p)
+{
+    typedef few::Fp4Cols<Num, NB> W;
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const int i = lane & 15, q = lane >> 4;
+    const uint32_t ncb = (uint32_t)p.col_blocks, tile = blockIdx.x / ncb, cb = blockIdx.x - tile * ncb;
+    RowTile t;
+    if (!find_row_tile(p.offsets, p.off64, p.E, 16 * MB, tile, &t)) return;
+    const int64_t row0 = uniform_i64(t.row0);
+    const int nrows = __builtin_amdgcn_readfirstlane((int)(t.row1 - t.row0)), e = __builtin_amdgcn_readfirstlane(t.expert);
+    W w;
+    w.two = false;
+    w.codes[0] = few::buffer(p.w.codes + e * p.w.sce);
+    w.scales[0] = few::buffer(p.w.scales + e * p.w.sse);
+    w.left = p.G - q;
+    // column i of the wave's block nb is 16 (i >> 2) + 4 nb + (i & 3) with NB = 4: a lane then holds 16 consecutive columns of its row
+    const int64_t n0 = (int64_t)cb * (16 * NB);
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+        int64_t n = n0 + (i >> 2) * (4 * NB) + 4 * nb + (i & 3);
+        if (n >= p.N) n = p.N - 1;
+        w.c[nb] = (uint32_t)(n * p.w.scn) + q * FP4_GROUP_BYTES;
+        w.s[nb] = (uint32_t)(n * p.w.ssn) + q;
+    }
+    few::Rows<MB> rows;
+    rows.K = p.K;
+    const int64_t base = p.x_grouped ? row0 : 0;
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) {
+        const int r = mb * 16 + i;
+        rows.x[mb] = few::buffer((const uint16_t*)p.X + base * p.ldx);
+        rows.a[mb] = few::RANGE;
+        if (r < nrows) {
+            const int64_t m = row0 + r;
+            rows.a[mb] = (uint32_t)(((p.x_grouped ? m : load_idx(p.pos, m, p.pos64) / p.fan_out) - base) * p.ldx + W::input(0, q)) * 2;
+        }
+    }
+    f32x4_t acc[MB][NB];
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) acc[mb][nb] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+    const int chunks = (p.K + few::CHUNK - 1) / few::CHUNK;
+    few::stream<W, MB, false, MB == 1 ? 4 : 2>(acc, w, rows, chunks * wave / waves, chunks * (wave + 1) / waves);
+    f32x4_t* red = (f32x4_t*)smem;   // [wave][MB * NB][64]
+    if (waves > 1) {
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) red[(wave * (MB * NB) + mb * NB + nb) * 64 + lane] = acc[mb][nb];
+        __syncthreads();
+    }
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) {
+        const int r = mb * 16 + i;
+        const int64_t m = row0 + (r < nrows ? r : 0);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            const int unit = mb * NB + nb;
+            if (unit % waves != wave) continue;
+            f32x4_t v = acc[mb][nb];
+            if (waves > 1) {
+                v = red[unit * 64 + lane];
+                for (int x = 1; x < waves; ++x) v += red[(x * (MB * NB) + unit) * 64 + lane];
+            }
+            const int64_t n = n0 + q * (4 * NB) + 4 * nb;
+            if (r >= nrows || n >= p.N) continue;
+            const int64_t out = p.y_grouped ? m : load_idx(p.pos, m, p.pos64);
+            store4(p.Y, out * p.ldy + n, p.ydtype, v, p.N - n < 4 ? (int)(p.N - n) : 4, p.y_vec);
+        }
+    }
+}
+
+template <class Num, int MB, int NB> int launch_few_typed(MoeFp4Gemm p, int64_t R, int waves, hipStream_t stream)
+{
+    p.col_blocks = (p.N + 16 * NB - 1) / (16 * NB);
+    const int64_t most = R / (16 * MB) + p.E, tiles = most < R ? most : R;   // (a tile holds a row at least)
+    if (!moe_grid_fits(tiles * p.col_blocks, waves * 64)) return MOE_ERR_UNSUPPORTED;
+    const size_t lds = waves > 1 ? (size_t)waves * MB * NB * 64 * 16 : 0;
+    hipLaunchKernelGGL((fp4_few_rows_kernel<Num, MB, NB>), dim3((unsigned)(tiles * p.col_blocks)), dim3(waves * 64), lds, stream, p);
+    return moe_launch_status();
+}
+
+template <class Num> int launch_few(const MoeFp4Gemm& p, int64_t R, hipStream_t stream)
+{
+    const int MB = R <= 16 * (int64_t)p.E ? 1 : 2;
+    const int64_t tiles = R / (16 * MB) + p.E < R ? R / (16 * MB) + p.E : R;
+    const int chunks = (p.K + few::CHUNK - 1) / few::CHUNK, cus = moe_device_cus();
+    // waves that share a contraction: as many as it has pairs of chunks, until the chip has twelve waves per compute unit
+    const bool narrow = tiles * ((p.N + 63) / 64) < cus;   // few column blocks: blocks of 16 columns give every compute unit one
+    const int64_t groups = tiles * (narrow ? (p.N + 15) / 16 : (p.N + 63) / 64);
+    int waves = 1;
+    while (waves < 8 && groups * waves < 12 * (int64_t)cus && chunks >= 2 * waves) waves *= 2;
+    if (MB == 1) return narrow ? launch_few_typed<Num, 1, 1>(p, R, waves, stream) : launch_few_typed<Num, 1, 4>(p, R, waves, stream);
+    return narrow ? launch_few_typed<Num, 2, 1>(p, R, waves, stream) : launch_few_typed<Num, 2, 4>(p, R, waves, stream);
+}
+
+}  // namespace
+
+int moe_launch_fp4_gemm(MoeFp4Gemm p, int64_t R, hipStream_t stream)
+{
+    p.G = (int)((p.K + FP4_GROUP - 1) / FP4_GROUP);
+    p.y_vec = p.ldy % 4 == 0 && (uintptr_t)p.Y % 16 == 0;
+    return p.f16 ? launch_few<NumF16>(p, R, stream) : launch_few<NumBf16>(p, R, stream);
+}

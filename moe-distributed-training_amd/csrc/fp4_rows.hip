@@ -77,7 +77,26 @@ __global__ void __launch_bounds__(256) fp4_expand_kernel(const uint8_t* codes, i
     }
 }
 
+// Rows that 16-byte loads do not take, in the order of the product and padded to whole pieces.  (Rows behind the last group are left alone: their positions may be anything.)
+__global__ void __launch_bounds__(256) fp4_pack_rows_kernel(const uint16_t* X, int64_t ldx, const void* pos, int pos64, int fan_out, const void* offsets, int off64, int E, int64_t K,
+                                                            uint16_t* out, int64_t ldo)
+{
+    const int64_t m = blockIdx.x;
+    if (m >= load_idx(offsets, E - 1, off64)) return;
+    const uint16_t* x = X + (pos ? load_idx(pos, m, pos64) / fan_out : m) * ldx;
+    for (int64_t c = threadIdx.x; c < ldo; c += 256) out[m * ldo + c] = c < K ? x[c] : (uint16_t)0;
+}
+
 }  // namespace
+
+int moe_launch_fp4_pack_rows(const void* X, int64_t ldx, const void* pos, int pos64, int fan_out, const void* offsets, int off64, int E, int64_t R, int64_t K, void* out, int64_t ldo,
+                             hipStream_t stream)
+{
+    if (!moe_grid_fits(R, 256)) return MOE_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL(fp4_pack_rows_kernel, dim3((unsigned)R), dim3(256), 0, stream, (const uint16_t*)X, ldx, pos, pos64, fan_out, offsets, off64, E, K, (uint16_t*)out,
+                       ldo);
+    return moe_launch_status();
+}
 
 int moe_launch_fp4_quantize(const void* W, int64_t swe, int64_t swk, int64_t swn, int dtype, int E, int64_t K, int64_t N, uint8_t* codes, int64_t sce, int64_t scn, uint8_t* scales,
                             int64_t sse, int64_t ssn, hipStream_t stream)

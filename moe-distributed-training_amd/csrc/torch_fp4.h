@@ -47,10 +47,9 @@ Fp4W take_fp4(const Tensor& codes, const Tensor& scales)
 Tensor linear_fp4_rows(const Tensor& x, const Fp4W& w, const Tensor& ssi, const Tensor& eo, const LinearCfg& c, bool sums)
 {
     const int64_t R = ssi.size(0), E = w.codes.size(0), K = x.size(1), N = w.codes.size(1);
-    (void)sums;
-    Tensor y = at::empty({R, N}, x.options());
+    Tensor y = at::empty({R, N}, x.options().dtype(rows_type(x.scalar_type(), sums)));
     if (R == 0 || N == 0) return y;
-    Tensor ws = bytes_on(x, moe_linear_fp4_workspace_bytes(dtype_code(x), R, (int)E, K, N));
+    Tensor ws = bytes_on(x, moe_linear_fp4_workspace_bytes(ptr(x), x.stride(0), x.size(0), c.grouped_in, dtype_code(x), R, (int)E, K, N));
     check(moe_linear_fp4_fwd(ptr(x), x.stride(0), x.size(0), dtype_code(x), w.c(), w.codes.stride(0), w.codes.stride(1), w.s(), w.scales.stride(0), w.scales.stride(1), ptr(y), y.stride(0),
                              dtype_code(y), ptr(ssi), is64(ssi), ptr(eo), is64(eo), (int)E, R, K, N, (int)c.k, c.grouped_in, c.grouped_out, ptr(ws), (size_t)ws.numel(), stream_of(x)),
           "moe_linear_fp4_fwd");
@@ -64,7 +63,7 @@ struct LinearFp4Fn : Function<LinearFp4Fn> {
         Tensor y = linear_fp4_rows(x, take_fp4(codes, scales), ssi, eo, c, gates.defined()), y_rows;
         if (gates.defined()) {
             y_rows = y;
-            y = combine(y_rows, gates, nullptr, gates.size(1), gates.size(0));
+            y = combine_rows(y_rows, gates, gates.size(1), gates.size(0), x.scalar_type());
         }
         ctx->save_for_backward({codes, scales, gates, ssi, eo, gates.defined() && gates.requires_grad() ? y_rows : Tensor()});
         ctx->saved_data["K"] = x.size(1);
@@ -86,13 +85,13 @@ struct LinearFp4Fn : Function<LinearFp4Fn> {
         int64_t gate_fan = 1;
         if (gates.defined()) {
             gate_fan = gates.size(1);
-            if (ctx->needs_input_grad(1)) d_gates = combine_dgates(sv[5].contiguous(), dout, gate_fan, gates.scalar_type(), nullptr);
+            if (ctx->needs_input_grad(1)) d_gates = combine_rows_dgates(sv[5].contiguous(), dout, gate_fan, gates.scalar_type());
         }
         if (ctx->needs_input_grad(0)) {
             dx = at::empty({R, K}, dout.options());
             if (R > 0 && N > 0) {
                 const Tensor dy = grouped_out ? dout : group_rows(dout, ptr(ssi), is64(ssi), R, gate_fan, flat_gates(gates));
-                Tensor ws = bytes_on(dout, moe_linear_fp4_workspace_bytes(dtype_code(dout), R, (int)E, K, N));
+                Tensor ws = bytes_on(dout, moe_linear_fp4_bwd_workspace_bytes(dtype_code(dout), R, (int)E, K, N));
                 check(moe_linear_fp4_bwd(ptr(dy), dy.stride(0), dtype_code(dy), w.c(), w.codes.stride(0), w.codes.stride(1), w.s(), w.scales.stride(0), w.scales.stride(1), ptr(dx),
                                          dx.stride(0), grouped_in, ptr(ssi), is64(ssi), ptr(eo), is64(eo), (int)E, R, K, N, ptr(ws), (size_t)ws.numel(), stream_of(dout)),
                       "moe_linear_fp4_bwd");
@@ -128,7 +127,7 @@ Tensor linear_fp4(const Tensor& x_, const Tensor& codes, const Tensor& scales, i
     const LinearCfg c{0.0, 0.0, k, grouped_in, grouped_out};
     if (needs_node({&x, &gates})) return LinearFp4Fn::apply(x, opt(gates), codes, scales, ssi, eo, c);
     Tensor y = linear_fp4_rows(x, take_fp4(codes, scales), ssi, eo, c, gates.defined());
-    return gates.defined() ? combine(y, gates, nullptr, gates.size(1), gates.size(0)) : y;
+    return gates.defined() ? combine_rows(y, gates, gates.size(1), gates.size(0), x.scalar_type()) : y;
 }
 
 // ---- SwiGLU with its inputs kept in 8 bits
