@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define MOE_HIP_ABI_VERSION 5   /* 5: expert products over 4-bit weights, SwiGLU with kept 8-bit inputs; 4: moe_int8_debug_tile; 3: expert products in 8-bit integers; 2: router weight gradient, static-scratch sort, stage-timer selection, moe_combine with k = 0; fp16 on the matrix cores (dtype argument of moe_mlp_fwd / moe_mlp_bwd) */
+#define MOE_HIP_ABI_VERSION 5   /* 5: expert products over 4-bit weights, SwiGLU with kept 8-bit inputs, the layer for a few tokens; 4: moe_int8_debug_tile; 3: expert products in 8-bit integers; 2: router weight gradient, static-scratch sort, stage-timer selection, moe_combine with k = 0; fp16 on the matrix cores (dtype argument of moe_mlp_fwd / moe_mlp_bwd) */
 
 #define MOE_OK 0
 #define MOE_ERR_BAD_ARG (-1)      /* inconsistent sizes / null pointers */
@@ -335,6 +335,18 @@ int moe_swiglu8_fwd(const void* gate, int64_t ldg, const void* up, int64_t ldu, 
                     void* stream);
 int moe_swiglu8_bwd(const void* kept, size_t kept_size, const void* dh, int64_t lddh, void* dgate, int64_t lddg, void* dup, int64_t lddu, int64_t rows, int64_t cols, int dtype,
                     void* stream);
+
+/* ---- the whole layer for a few tokens, two launches (no counterpart in the reference) ---------------------------
+ * Router, softmax, top-k (ties to the lower expert; normalize: weights divided by their sum), gate and up projection, SwiGLU, down projection and weighted sum of at most 16 tokens, 256
+ * experts, 16 experts per token; bf16 or fp16 x and router weight wg (E, d); d and f multiples of 64.  out (T, d) of x's type, weights (T, k) fp32, indices (T, k).  Rows of x and wg start at
+ * multiples of 16 bytes, out's at multiples of 8.  Expert weights: w1, w3, w2 (E, f, d) of x's type, contiguous; or codes and scales of 4-bit weights (above), contiguous: c1, c3 (E, f, d), c2
+ * (E, d, f).  Every expert's matrix below 2 GiB. */
+size_t moe_decode_layer_workspace_bytes(int64_t T, int E, int64_t d, int64_t f, int k, int bits);
+int moe_decode_layer(const void* x, int64_t ldx, const void* wg, int64_t ldwg, int dtype, const void* w1, const void* w3, const void* w2, void* out, int64_t ldo, float* weights,
+                     int32_t* indices, int64_t T, int E, int64_t d, int64_t f, int k, int normalize, void* workspace, size_t workspace_bytes, void* stream);
+int moe_decode_layer_fp4(const void* x, int64_t ldx, const void* wg, int64_t ldwg, int dtype, const uint8_t* c1, const uint8_t* s1, const uint8_t* c3, const uint8_t* s3,
+                         const uint8_t* c2, const uint8_t* s2, void* out, int64_t ldo, float* weights, int32_t* indices, int64_t T, int E, int64_t d, int64_t f, int k, int normalize,
+                         void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -19,6 +19,7 @@ from .megablocks_utils.router import forward_router, route_and_sort  # noqa: F40
 from .megablocks_utils.moe_mlp import (  # noqa: F401
     scattermoe_permute_and_compute, fused_expert_mlp, moe_layer_forward, ScatterMoEBlock,
     Int8ExpertWeights, fused_expert_mlp_int8, moe_layer_forward_int8, swiglu_8bit,
+    Fp4ExpertWeights, fused_expert_mlp_fp4, moe_layer_forward_fp4, moe_layer_decode,
 )
 
 __all__ = [
@@ -27,5 +28,5 @@ __all__ = [
     "ParallelExperts", "forward_router", "route_and_sort", "scattermoe_permute_and_compute", "fused_expert_mlp",
     "moe_layer_forward", "ScatterMoEBlock", "quantize_rows", "quantize_expert_weights", "parallel_linear_int8",
     "Int8ExpertWeights", "fused_expert_mlp_int8", "moe_layer_forward_int8", "quantize_expert_weights_fp4", "parallel_linear_fp4",
-    "swiglu_8bit",
+    "swiglu_8bit", "Fp4ExpertWeights", "fused_expert_mlp_fp4", "moe_layer_forward_fp4", "moe_layer_decode",
 ]

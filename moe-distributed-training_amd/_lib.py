@@ -82,6 +82,9 @@ _SIGNATURES = {
     "moe_swiglu8_kept_bytes": ("z", "ll"),
     "moe_swiglu8_fwd": ("i", "plplpl" + "pz" + "ll" + "i" + "p"),
     "moe_swiglu8_bwd": ("i", "pzplplpl" + "ll" + "i" + "p"),
+    "moe_decode_layer_workspace_bytes": ("z", "lillii"),
+    "moe_decode_layer": ("i", "plpli" + "ppp" + "plpp" + "lilli" + "i" + "pzp"),
+    "moe_decode_layer_fp4": ("i", "plpli" + "pppppp" + "plpp" + "lilli" + "i" + "pzp"),
     "moe_mlp_int8_bwd": ("i", "pliii" + "pi" + "pppppp" + "pz" + "pli" + "pi" + "pi" + "i" + "lll" + "pzp"),
 }
 

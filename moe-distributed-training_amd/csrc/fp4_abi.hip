@@ -49,6 +49,24 @@ int swiglu8_params(MoeSwiglu8& p, uint8_t* kept, int64_t rows, int64_t cols)
     return MOE_OK;
 }
 
+constexpr int64_t MAX_WIDTH = 1 << 20;   // hidden and ffn size of the layer for a few tokens
+
+// what both entry points of the layer for a few tokens share
+int decode_params(MoeDecode& p, const void* x, int64_t ldx, const void* wg, int64_t ldwg, int dtype, void* out, int64_t ldo, float* weights, int32_t* indices, int64_t T, int E,
+                  int64_t d, int64_t f, int k, int normalize, void* workspace, size_t workspace_bytes, int bits)
+{
+    if (dtype < 0 || dtype > 2 || T < 0 || E < 1 || d < 64 || f < 64 || d % 64 != 0 || f % 64 != 0 || k < 1 || k > E) return MOE_ERR_BAD_ARG;
+    if (dtype == MOE_F32 || T > MOE_DECODE_TOKENS || E > MOE_DECODE_EXPERTS || k > MOE_DECODE_TOPK || d > MAX_WIDTH || f > MAX_WIDTH) return MOE_ERR_UNSUPPORTED;
+    if (T == 0) return MOE_OK;
+    if (!x || !wg || !out || !weights || !indices || ldx < 0 || ldwg < 0 || (T > 1 && ldo < d)) return MOE_ERR_BAD_ARG;
+    if (!aligned16(x) || !aligned16(wg) || ldx % 8 != 0 || ldwg % 8 != 0 || (uintptr_t)out % 8 != 0 || ldo % 4 != 0 || !aligned16(workspace)) return MOE_ERR_BAD_ARG;
+    if ((T * ldx + d) * 2 >= MOE_FP4_RANGE || (E * ldwg + d) * 2 >= MOE_FP4_RANGE) return MOE_ERR_UNSUPPORTED;
+    if (!workspace || workspace_bytes < moe_decode_bytes((int)T, E, (int)d, (int)f, k, bits == 4)) return MOE_ERR_WORKSPACE;
+    p.x = x; p.ldx = ldx; p.wg = wg; p.ldwg = ldwg; p.out = out; p.ldo = ldo; p.weights = weights; p.indices = indices;
+    p.T = (int)T; p.E = E; p.d = (int)d; p.f = (int)f; p.k = k; p.normalize = normalize;
+    return MOE_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -146,6 +164,40 @@ int moe_swiglu8_bwd(const void* kept, size_t kept_size, const void* dh, int64_t 
     TRY(swiglu8_params(p, (uint8_t*)kept, rows, cols));
     const bool vec = cols % 8 == 0 && lddh % 8 == 0 && lddg % 8 == 0 && lddu % 8 == 0 && aligned16(dh) && aligned16(dgate) && aligned16(dup);
     return moe_launch_swiglu8(p, dtype, vec, true, S(stream));
+}
+
+size_t moe_decode_layer_workspace_bytes(int64_t T, int E, int64_t d, int64_t f, int k, int bits)
+{
+    if (T < 1 || T > MOE_DECODE_TOKENS || E < 1 || E > MOE_DECODE_EXPERTS || d < 64 || f < 64 || d > MAX_WIDTH || f > MAX_WIDTH || k < 1 || k > E || k > MOE_DECODE_TOPK) return 0;
+    return moe_decode_bytes((int)T, E, (int)d, (int)f, k, bits == 4);
+}
+
+int moe_decode_layer(const void* x, int64_t ldx, const void* wg, int64_t ldwg, int dtype, const void* w1, const void* w3, const void* w2, void* out, int64_t ldo, float* weights,
+                     int32_t* indices, int64_t T, int E, int64_t d, int64_t f, int k, int normalize, void* workspace, size_t workspace_bytes, void* stream)
+{
+    MoeDecode p = {};
+    TRY(decode_params(p, x, ldx, wg, ldwg, dtype, out, ldo, weights, indices, T, E, d, f, k, normalize, workspace, workspace_bytes, 16));
+    if (T == 0) return MOE_OK;
+    if (!w1 || !w3 || !w2 || !aligned16(w1) || !aligned16(w3) || !aligned16(w2)) return MOE_ERR_BAD_ARG;
+    if (d * f * 2 >= MOE_FP4_RANGE) return MOE_ERR_UNSUPPORTED;
+    p.w1 = w1; p.w3 = w3; p.w2 = w2;
+    return moe_launch_decode(p, false, dtype == MOE_F16, workspace, S(stream));
+}
+
+int moe_decode_layer_fp4(const void* x, int64_t ldx, const void* wg, int64_t ldwg, int dtype, const uint8_t* c1, const uint8_t* s1, const uint8_t* c3, const uint8_t* s3,
+                         const uint8_t* c2, const uint8_t* s2, void* out, int64_t ldo, float* weights, int32_t* indices, int64_t T, int E, int64_t d, int64_t f, int k, int normalize,
+                         void* workspace, size_t workspace_bytes, void* stream)
+{
+    MoeDecode p = {};
+    TRY(decode_params(p, x, ldx, wg, ldwg, dtype, out, ldo, weights, indices, T, E, d, f, k, normalize, workspace, workspace_bytes, 4));
+    if (T == 0) return MOE_OK;
+    if (d * f >= MOE_FP4_RANGE) return MOE_ERR_UNSUPPORTED;
+    auto take = [](const uint8_t* c, const uint8_t* s, int64_t rows, int64_t inner) { return MoeFp4Weights{c, rows * (inner / 2), inner / 2, s, rows * (inner / 32), inner / 32}; };
+    p.f1 = take(c1, s1, f, d);
+    p.f3 = take(c3, s3, f, d);
+    p.f2 = take(c2, s2, d, f);
+    if (!weights_ok(p.f1) || !weights_ok(p.f3) || !weights_ok(p.f2)) return MOE_ERR_BAD_ARG;
+    return moe_launch_decode(p, true, dtype == MOE_F16, workspace, S(stream));
 }
 
 }  // extern "C"

@@ -335,3 +335,20 @@ struct MoeSwiglu8 {
 };
 // vec: columns and row pitches multiples of 8, addresses of 16 bytes
 int moe_launch_swiglu8(const MoeSwiglu8& p, int dtype, bool vec, bool backward, hipStream_t stream);
+
+// ---- the layer for a few tokens (decode_layer.hip) -------------------------------------------------------------
+constexpr int MOE_DECODE_TOKENS = 16, MOE_DECODE_TOPK = 16, MOE_DECODE_EXPERTS = 256;   // at most
+struct MoeDecode {
+    const void* x; int64_t ldx;         // 16-bit rows at multiples of 16 bytes
+    const void* wg; int64_t ldwg;
+    const void *w1, *w3, *w2;           // 16-bit weights (E, f, d) contiguous, or
+    MoeFp4Weights f1, f3, f2;           // 4-bit weights (E, f, d), (E, f, d), (E, d, f)
+    void* out; int64_t ldo;
+    float* weights; int32_t* indices;   // (T, k)
+    int T, E, d, f, k, normalize;
+    // set by the launcher
+    uint16_t* h; int64_t h_lo;          // (T k, f); what the rounding lost lies h_lo elements further
+    float* slots; int* counters; int counters_n, parts;
+};
+size_t moe_decode_bytes(int T, int E, int d, int f, int k, bool fp4);
+int moe_launch_decode(MoeDecode p, bool fp4, bool f16, void* workspace, hipStream_t stream);

@@ -174,3 +174,151 @@ Tensor swiglu_8bit(const Tensor& gate, const Tensor& up)
     const c10::DeviceGuard guard(gate.device());
     return needs_node({&gate, &up}) ? Swiglu8Fn::apply(gate, up) : swiglu8_forward(as_rows(gate), as_rows(up), gate.sizes(), nullptr);
 }
+
+// ---- expert MLP and layer: codes and scales in the order w1, w2, w3; w1 and w3 (E, f, d), w2 (E, d, f)
+struct Fp4Mlp { Tensor w[3], s[3]; int64_t E, d, f; };
+
+Fp4Mlp take_mlp_fp4(const Tensor& w1, const Tensor& s1, const Tensor& w2, const Tensor& s2, const Tensor& w3, const Tensor& s3, int64_t d)
+{
+    check_fp4(w1, s1, d);
+    const int64_t E = w1.size(0), f = w1.size(1);
+    check_fp4(w3, s3, d);
+    check_fp4(w2, s2, f);
+    TORCH_CHECK(w3.size(0) == E && w3.size(1) == f && w2.size(0) == E && w2.size(1) == d, "4-bit expert weights of ", w1.sizes(), ", ", w2.sizes(), " and ", w3.sizes(), " do not fit ", E,
+                " experts of ", f, " x ", d);
+    TORCH_CHECK(E >= 1 && f >= 1, "expert weights of ", w1.sizes(), " hold nothing to multiply by");
+    return {{w1, w2, w3}, {s1, s2, s3}, E, d, f};
+}
+
+struct DecodeOut { Tensor out, weights, indices; };
+DecodeOut decode_outputs(const Tensor& x, int64_t k)
+{
+    const int64_t T = x.size(0);
+    return {at::empty({T, x.size(1)}, x.options()), at::empty({T, k}, x.options().dtype(at::kFloat)), at::empty({T, k}, x.options().dtype(at::kInt))};
+}
+
+// rows at multiples of 16 bytes
+Tensor aligned_rows(const Tensor& t)
+{
+    const Tensor u = unit_inner(t);
+    return (uintptr_t)u.data_ptr() % 16 == 0 && (u.size(0) < 2 || u.stride(0) % 8 == 0) ? u : u.clone(at::MemoryFormat::Contiguous);
+}
+
+// what the two launches for a few tokens take
+bool decode_takes(int64_t T, int64_t E, int64_t d, int64_t f, int64_t k)
+{
+    return T <= 16 && E <= 256 && k <= 16 && d % 64 == 0 && f % 64 == 0 && d <= (1 << 20) && f <= (1 << 20) && d * f < (int64_t)1 << 30;
+}
+
+void check_layer_input(const Tensor& x, const Tensor& wg, int64_t E, int64_t k)
+{
+    TORCH_CHECK(x.dim() == 2, "the layer takes (tokens, hidden size), got ", x.sizes());
+    TORCH_CHECK(wg.dim() == 2 && wg.size(0) == E && wg.size(1) == x.size(1), "router weight of ", wg.sizes(), " does not fit ", E, " experts of rows of ", x.sizes());
+    MOE_ASSERT(wg.scalar_type() == x.scalar_type(), "router weight and X must share a dtype");
+    MOE_ASSERT(k >= 1 && k <= E, "top_k must be between 1 and the number of experts");
+}
+
+variable_list layer_decode(const Tensor& x_, const Tensor& wg_, const Tensor& w1_, const Tensor& w2_, const Tensor& w3_, int64_t k, bool normalize)
+{
+    require_gpu({&x_, &wg_, &w1_, &w2_, &w3_});
+    TORCH_CHECK(w1_.dim() == 3, "expert weights are (experts, ffn size, hidden size), got ", w1_.sizes());
+    const int64_t E = w1_.size(0), f = w1_.size(1), d = w1_.size(2), T = x_.dim() ? x_.size(0) : 0;
+    check_layer_input(x_, wg_, E, k);
+    for (const Tensor* w : {&w1_, &w2_, &w3_}) {
+        TORCH_CHECK(w->dim() == 3, "expert weights are (experts, ffn size, hidden size), got ", w->sizes());
+        check_expert_weight(*w, E, f, d);
+        MOE_ASSERT(w->scalar_type() == x_.scalar_type(), "X and W must share a dtype");
+    }
+    TORCH_CHECK_TYPE(x_.scalar_type() == at::kBFloat16 || x_.scalar_type() == at::kHalf, "moe_layer_decode takes bf16 or fp16, got ", x_.scalar_type(), "; use moe_layer_forward for others");
+    TORCH_CHECK(!needs_node({&x_, &wg_, &w1_, &w2_, &w3_}), "moe_layer_decode takes no gradients: call it under torch.no_grad(), or use moe_layer_forward");
+    TORCH_CHECK(d >= 64 && f >= 64 && decode_takes(T, E, d, f, k), "moe_layer_decode takes up to 16 tokens, 256 experts and 16 experts per token, hidden and ffn sizes that are multiples of 64, and matrices below 2 GiB; got ", T,
+                " tokens, ", E, " experts of ", f, " x ", d, ", top ", k, "; use moe_layer_forward for others");
+    const c10::DeviceGuard guard(x_.device());
+    const Tensor x = aligned_rows(x_), wg = aligned_rows(wg_);
+    auto whole = [](const Tensor& w) { return w.is_contiguous() && (uintptr_t)w.data_ptr() % 16 == 0 ? w : w.clone(at::MemoryFormat::Contiguous); };
+    const Tensor w1 = whole(w1_), w2 = whole(w2_), w3 = whole(w3_);
+    DecodeOut o = decode_outputs(x, k);
+    if (T == 0) return {o.out, o.weights, o.indices};
+    Tensor ws = bytes_on(x, moe_decode_layer_workspace_bytes(T, (int)E, d, f, (int)k, 16));
+    check(moe_decode_layer(ptr(x), x.stride(0), ptr(wg), wg.stride(0), dtype_code(x), ptr(w1), ptr(w3), ptr(w2), ptr(o.out), o.out.stride(0), (float*)ptr(o.weights),
+                           (int32_t*)ptr(o.indices), T, (int)E, d, f, (int)k, normalize, ptr(ws), (size_t)ws.numel(), stream_of(x)), "moe_decode_layer");
+    return {o.out, o.weights, o.indices};
+}
+
+// Few tokens without gradients: two launches.
+DecodeOut layer_decode_fp4(const Tensor& x_, const Tensor& wg_, const Fp4Mlp& m, int64_t k, bool normalize)
+{
+    const Tensor x = aligned_rows(x_), wg = aligned_rows(wg_);
+    const int64_t T = x.size(0);
+    DecodeOut o = decode_outputs(x, k);
+    Tensor w[3], s[3];
+    for (int i = 0; i < 3; ++i) {
+        w[i] = m.w[i].is_contiguous() && (uintptr_t)m.w[i].data_ptr() % 16 == 0 ? m.w[i] : m.w[i].clone(at::MemoryFormat::Contiguous);
+        s[i] = m.s[i].contiguous();
+    }
+    auto b = [](const Tensor& t) { return (const uint8_t*)ptr(t); };
+    Tensor ws = bytes_on(x, moe_decode_layer_workspace_bytes(T, (int)m.E, m.d, m.f, (int)k, 4));
+    check(moe_decode_layer_fp4(ptr(x), x.stride(0), ptr(wg), wg.stride(0), dtype_code(x), b(w[0]), b(s[0]), b(w[2]), b(s[2]), b(w[1]), b(s[1]), ptr(o.out), o.out.stride(0),
+                               (float*)ptr(o.weights), (int32_t*)ptr(o.indices), T, (int)m.E, m.d, m.f, (int)k, normalize, ptr(ws), (size_t)ws.numel(), stream_of(x)),
+          "moe_decode_layer_fp4");
+    return o;
+}
+
+// the three projections as autograd nodes of their own; keep8: gate and up are kept in 8 bits
+Tensor mlp_fp4(const Tensor& x, const Fp4Mlp& m, int64_t fan_out, const Tensor& ssi, const Tensor& offsets, const Tensor& gates, bool grouped_out, bool keep8)
+{
+    auto proj = [&](const Tensor& in, int i, const Tensor& g, int64_t k, bool gin, bool gout) {
+        const LinearCfg c{0.0, 0.0, k, gin, gout};
+        const Tensor xr = unit_inner(in);
+        if (needs_node({&xr, &g})) return LinearFp4Fn::apply(xr, opt(g), m.w[i], m.s[i], ssi, offsets, c);
+        Tensor y = linear_fp4_rows(xr, take_fp4(m.w[i], m.s[i]), ssi, offsets, c, g.defined());
+        return g.defined() ? combine_rows(y, g, g.size(1), g.size(0), xr.scalar_type()) : y;
+    };
+    const Tensor gate = proj(x, 0, Tensor(), fan_out, false, true), up = proj(x, 2, Tensor(), fan_out, false, true);
+    return proj(keep8 ? swiglu_8bit(gate, up) : swiglu(gate, up), 1, gates, 1, true, grouped_out);
+}
+
+Tensor expert_mlp_fp4(const Tensor& x, const Tensor& w1, const Tensor& s1, const Tensor& w2, const Tensor& s2, const Tensor& w3, const Tensor& s3, int64_t fan_out, const Tensor& ssi_,
+                      const Tensor& offsets_, const OptTensor& gates_in, bool grouped_out, bool keep8)
+{
+    const Tensor gates_ = val(gates_in);
+    require_gpu({&x, &w1, &s1, &w2, &s2, &w3, &s3, &ssi_, &offsets_, &gates_});
+    TORCH_CHECK(x.dim() == 2 && x.size(1) >= 1, "the expert MLP takes (rows, hidden size), got ", x.sizes());
+    const c10::DeviceGuard guard(x.device());
+    const Fp4Mlp m = take_mlp_fp4(w1, s1, w2, s2, w3, s3, x.size(1));
+    dtype_code(x);
+    check_gates(gates_, ssi_.numel());
+    if (gates_.defined()) dtype_code(gates_);
+    check_offsets(offsets_, m.E);
+    is64(ssi_);
+    is64(offsets_);
+    TORCH_CHECK(fan_out >= 1 && ssi_.numel() == x.size(0) * fan_out, "positions of ", ssi_.sizes(), " do not fit ", x.size(0), " rows with a fan-out of ", fan_out);
+    const Tensor ssi = ssi_.contiguous(), offsets = offsets_.contiguous(), gates = gates_.defined() ? gates_.contiguous() : Tensor();
+    return mlp_fp4(x, m, fan_out, ssi, offsets, gates, grouped_out && !gates.defined(), keep8);
+}
+
+// router -> experts over 4-bit weights -> weighted sum; returns as layer()
+variable_list layer_fp4(const Tensor& x, const Tensor& wg, const Tensor& w1, const Tensor& s1, const Tensor& w2, const Tensor& s2, const Tensor& w3, const Tensor& s3, int64_t k,
+                        bool normalize, bool keep8)
+{
+    require_gpu({&x, &wg, &w1, &s1, &w2, &s2, &w3, &s3});
+    TORCH_CHECK(x.dim() == 2 && x.size(1) >= 1, "the layer takes (tokens, hidden size), got ", x.sizes());
+    const Fp4Mlp m = take_mlp_fp4(w1, s1, w2, s2, w3, s3, x.size(1));
+    check_layer_input(x, wg, m.E, k);
+    dtype_code(x);
+    const c10::DeviceGuard guard(x.device());
+    const bool node = needs_node({&x, &wg});
+    if (!node && x.size(0) > 0 && x.scalar_type() != at::kFloat && decode_takes(x.size(0), m.E, m.d, m.f, k)) {
+        const DecodeOut o = layer_decode_fp4(x, wg, m, k, normalize);
+        return {o.out, o.weights, o.indices};
+    }
+    RouterOut rt;
+    Sorted so;
+    if (node) {
+        const variable_list r = router(x, wg, k, normalize);
+        rt = {r[0], r[1], r[2]};
+        so = sort_assignments(rt.indices, m.E);
+    } else router_and_sort(unit_inner(x), unit_inner(wg), k, normalize, rt, so);
+    const Tensor out = mlp_fp4(x, m, k, so.ints.narrow(0, so.R, so.R), so.ints.narrow(0, 3 * so.R, m.E), rt.weights, false, keep8);
+    return {out, rt.weights, rt.indices};
+}

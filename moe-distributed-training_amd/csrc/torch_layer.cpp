@@ -860,6 +860,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
     m.def("quantize_weights_fp4", torch::wrap_pybind_function_no_gil(quantize_weights_fp4));
     m.def("linear_fp4", torch::wrap_pybind_function_no_gil(linear_fp4));
     m.def("swiglu_8bit", torch::wrap_pybind_function_no_gil(swiglu_8bit));
+    m.def("layer_decode", torch::wrap_pybind_function_no_gil(layer_decode));
+    m.def("expert_mlp_fp4", torch::wrap_pybind_function_no_gil(expert_mlp_fp4));
+    m.def("layer_fp4", torch::wrap_pybind_function_no_gil(layer_fp4));
 }
 
 // The same functions as dispatcher operators, for torch.jit.trace: a trace records operators, and of the functions above it
@@ -898,4 +901,13 @@ TORCH_LIBRARY(moe_hip, m)
         return linear_fp4(x, codes, scales, k, sei, ssi, eo, gates, grouped_in, grouped_out);
     });
     m.def("swiglu_8bit", [](const Tensor& gate, const Tensor& up) { return swiglu_8bit(gate, up); });
+    m.def("layer_decode", [](const Tensor& x, const Tensor& wg, const Tensor& w1, const Tensor& w2, const Tensor& w3, int64_t k, bool normalize) {
+        return layer_decode(x, wg, w1, w2, w3, k, normalize);
+    });
+    m.def("expert_mlp_fp4", [](const Tensor& x, const Tensor& w1, const Tensor& s1, const Tensor& w2, const Tensor& s2, const Tensor& w3, const Tensor& s3, int64_t fan_out,
+                               const Tensor& ssi, const Tensor& offsets, const OptTensor& gates, bool grouped_out, bool keep8) {
+        return expert_mlp_fp4(x, w1, s1, w2, s2, w3, s3, fan_out, ssi, offsets, gates, grouped_out, keep8);
+    });
+    m.def("layer_fp4", [](const Tensor& x, const Tensor& wg, const Tensor& w1, const Tensor& s1, const Tensor& w2, const Tensor& s2, const Tensor& w3, const Tensor& s3, int64_t k,
+                          bool normalize, bool keep8) { return layer_fp4(x, wg, w1, s1, w2, s2, w3, s3, k, normalize, keep8); });
 }

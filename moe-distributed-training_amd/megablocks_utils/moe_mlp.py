@@ -17,6 +17,7 @@ import torch.nn as nn
 from .._lib import entry, native, require_gpu
 from ..scattermoe_utils.kernels import ops
 from ..scattermoe_utils.parallel_experts import parallel_linear
+from ..scattermoe_utils.parallel_linear_fp4 import quantize_expert_weights_fp4
 from ..scattermoe_utils.parallel_linear_int8 import quantize_expert_weights
 from ..scattermoe_utils.parallel_linear_lora import parallel_linear_lora
 
@@ -110,6 +111,38 @@ def swiglu_8bit(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
     return entry("swiglu_8bit")(gate, up)
 
 
+class Fp4ExpertWeights(NamedTuple):
+    """Expert weights in 4 bits (``quantize_expert_weights_fp4``): codes and scales, uint8, of w1 and w3 (E, f, d / 2) and (E, f, d / 32),
+    and of w2 turned round, (E, d, f / 2) and (E, d, f / 32): every output's inputs lie side by side."""
+    w1: torch.Tensor
+    w1_scale: torch.Tensor
+    w2: torch.Tensor
+    w2_scale: torch.Tensor
+    w3: torch.Tensor
+    w3_scale: torch.Tensor
+
+    @classmethod
+    def quantize(cls, w1, w2, w3, ffn_hidden_size=None, hidden_size=None):
+        """From bf16 / fp16 / fp32 weights (E, f, d), or in storage (E*f, d) with both sizes given."""
+        out = []
+        for name, w in (("w1", w1), ("w2", w2), ("w3", w3)):
+            w = resolve_dtensor(w)
+            if w.dim() == 2:
+                w = w.view(-1, ffn_hidden_size, hidden_size)
+            out += quantize_expert_weights_fp4(w if name == "w2" else w.transpose(1, 2))
+        return cls(*out)
+
+
+def fused_expert_mlp_fp4(x, weights: Fp4ExpertWeights, k, sorted_scattered_idxs, expert_offsets, gates: Optional[torch.Tensor] = None,
+                         grouped_out: bool = False, keep_8bit: bool = False):
+    """``fused_expert_mlp`` over 4-bit weights (frozen; no adapters): x (rows, d) bf16, fp16 or fp32, the other arguments and the result as
+    there, one position for each of the rows' k assignments.  Gradients: of x and ``gates``.  ``keep_8bit``: the backward pass keeps
+    gate and up as 8-bit codes (``swiglu_8bit``), 2.1 bytes per ffn value and assignment in place of 4 (fp32: 8).  Every assignment has to
+    belong to an expert."""
+    return entry("expert_mlp_fp4")(x, weights.w1, weights.w1_scale, weights.w2, weights.w2_scale, weights.w3, weights.w3_scale, k,
+                                   sorted_scattered_idxs, expert_offsets, gates, grouped_out, keep_8bit)
+
+
 def scattermoe_permute_and_compute(x, w1, w2, w3, ffn_hidden_size, hidden_size, top_k, bin_ids, indices, num_experts,
                                    lora_pointers=None, moe_expert_model_parallelism=True, expert_offsets=None,
                                    lora_views: Optional[LoraViews] = None, lora_alpha: float = 1.0):
@@ -182,6 +215,24 @@ def moe_layer_forward_int8(x, wg, weights: Int8ExpertWeights, top_k=2, normalize
         return _empty_layer(x, wg, weights, top_k)
     return entry("layer_int8")(x, wg, weights.w1, weights.w1_scale, weights.w2, weights.w2_scale, weights.w3, weights.w3_scale, top_k,
                                bool(normalize))
+
+
+def moe_layer_forward_fp4(x, wg, weights: Fp4ExpertWeights, top_k=2, normalize: bool = True, keep_8bit: bool = False):
+    """``moe_layer_forward`` over 4-bit expert weights: x (T, d) bf16, fp16 or fp32 -> (out (T, d), expert_weights (T, k) fp32,
+    expert_indices (T, k) int32).  Up to 16 bf16 or fp16 tokens of at most 256 experts and 16 per token, d and f multiples of 64, without
+    gradients run as two launches.  Gradients: of x and the router weight wg; ``keep_8bit`` as in ``fused_expert_mlp_fp4``."""
+    if x.size(0) == 0:
+        return _empty_layer(x, wg, weights, top_k)
+    return entry("layer_fp4")(x, wg, weights.w1, weights.w1_scale, weights.w2, weights.w2_scale, weights.w3, weights.w3_scale, top_k,
+                              bool(normalize), bool(keep_8bit))
+
+
+def moe_layer_decode(x, wg, w1, w2, w3, top_k=2, normalize: bool = True):
+    """``moe_layer_forward`` for the tokens of a generation step, in two launches and without gradients: x (T, d), T up to 16, wg (E, d) and
+    w1, w2, w3 (E, f, d), all bf16 or all fp16, E up to 256, top_k up to 16, d and f multiples of 64 -> (out (T, d), expert_weights (T, k) fp32,
+    expert_indices (T, k) int32).  The weights of a chosen expert are read once, however many tokens chose it; the result differs from
+    ``moe_layer_forward``'s by roundings (the interim of the two projections keeps 16 more bits here)."""
+    return entry("layer_decode")(x, wg, w1, w2, w3, top_k, bool(normalize))
 
 
 class ScatterMoEBlock(nn.Module):

@@ -1,0 +1,213 @@
+"""The layer for a few tokens, over 16-bit and 4-bit weights, against its definition in 64 bits.
+
+What an output element may be off by: its own last rounding; the roundings of 32-bit sums over d and f (in units of the sums of their terms' magnitudes, those of gate and up
+carried through SwiGLU and the down projection); the two numbers of the type that h travels as (bf16: 2^-17 of it, fp16: 2^-23, or half a subnormal step); the hardware exponential's and
+the weights' few 2^-24."""
+import pytest
+import torch
+
+import moe_distributed_training_amd as moe
+from oracle import fp4_oracle as oracle
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16 = torch.bfloat16, torch.float16
+
+
+def make(T, d, f, E, k, dtype, bits, seed=0):
+    g = torch.Generator().manual_seed(seed * 31 + T + d + f + E)
+    x = (torch.randn(T, d, generator=g) * torch.exp(0.4 * torch.randn(T, 1, generator=g))).to(dtype)
+    wg = (torch.randn(E, d, generator=g) * 0.05).to(dtype)
+    w = [torch.randn(E, f, d, generator=g) * 0.05 for _ in range(3)]
+    if bits == 16:
+        w = [t.to(dtype) for t in w]
+        return x, wg, w, (w[0].double(), w[2].double(), w[1].double().transpose(1, 2))
+    q = [oracle.quantize(w[0].transpose(1, 2)), oracle.quantize(w[1]), oracle.quantize(w[2].transpose(1, 2))]
+    return x, wg, q, (oracle.weights(*q[0], d), oracle.weights(*q[2], d), oracle.weights(*q[1], f))
+
+
+def run(dev, x, wg, w, k, normalize=True, bits=16):
+    with torch.no_grad():
+        if bits == 16:
+            return moe.moe_layer_decode(x.to(dev), wg.to(dev), *(t.to(dev) for t in w), k, normalize)
+        weights = moe.Fp4ExpertWeights(*(t.to(dev) for q in w for t in q))
+        return moe.moe_layer_forward_fp4(x.to(dev), wg.to(dev), weights, k, normalize)
+
+
+def slack_of(out, terms, back, w2_sum, d, f, dtype):
+    a = 2.0 ** -24
+    h = 2.0 ** -17 if dtype == BF16 else 2.0 ** -22
+    return (torch.finfo(dtype).eps / 2 * out.abs() + (d + 24) * a * back + ((f + 64) * a + h) * terms + 2.0 ** -24 * w2_sum * (dtype == F16)) * 1.01
+
+
+def check(dev, T, d, f, E, k, dtype, bits, normalize=True, seed=0):
+    x, wg, w, (w1, w3, w2) = make(T, d, f, E, k, dtype, bits, seed)
+    want, weights, idx, terms, back = oracle.layer(x, wg, w1, w3, w2, k, normalize)
+    out, ew, ei = run(dev, x, wg, w, k, normalize, bits)
+    assert out.dtype == dtype and out.shape == (T, d) and ew.dtype == torch.float32 and ei.dtype == torch.int32
+    assert torch.equal(ei.cpu().long(), idx), "choices differ"
+    # logits are off by (d + 8) 2^-24 of their terms, weights by twice that
+    lt = (x.double().abs() @ wg.double().abs().t()).amax()
+    assert float(((ew.double().cpu() - weights) / weights).abs().max()) <= 2 * ((d + 8) * lt + 16) * 2.0 ** -24
+    w2_sum = sum((w2[idx[:, j]].abs().sum(-1) * weights[:, j, None]) for j in range(k))
+    over = (out.double().cpu() - want).abs() - slack_of(want, terms + 0, back, w2_sum, d, f, dtype) - 2 * ((d + 8) * lt + 16) * 2.0 ** -24 * terms
+    assert float(over.max()) <= 0, f"{float(over.max()):.3g} past its bound at {torch.nonzero(over == over.max())[0].tolist()}"
+    return out, ew, ei
+
+
+SIZES = [  # T, d, f, E, k
+    (1, 64, 64, 1, 1), (1, 128, 64, 8, 2), (2, 64, 192, 4, 2), (3, 256, 512, 8, 2), (16, 128, 128, 2, 1), (7, 192, 320, 16, 4), (16, 256, 64, 64, 8), (5, 320, 128, 96, 3),
+    (16, 64, 64, 256, 16), (13, 1024, 256, 8, 2), (9, 448, 960, 3, 3), (4, 2176, 1088, 4, 2), (16, 64, 64, 1, 1),
+]
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("T,d,f,E,k", SIZES)
+def test_layer(dev, T, d, f, E, k, dtype, bits):
+    check(dev, T, d, f, E, k, dtype, bits)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_weights_that_are_not_normalised(dev, bits):
+    check(dev, 6, 128, 192, 8, 3, BF16, bits, normalize=False)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_every_number_of_tokens(dev, bits):
+    for T in range(1, 17):
+        check(dev, T, 192, 128, 5, 2, BF16, bits, seed=T)
+
+
+def test_more_than_sixteen_tokens_and_fp32_over_4_bits(dev):
+    """What the two launches do not take runs on the layer's other kernels: the interims are rounded to the type there."""
+    for T, dtype, d in ((17, BF16, 128), (40, F16, 192), (5, torch.float32, 96)):
+        x, wg, w, (w1, w3, w2) = make(T, d, 128, 4, 2, dtype, 4)
+        want, weights, idx, terms, back = oracle.layer(x, wg, w1, w3, w2, 2)
+        out, _, ei = run(dev, x, wg, w, 2, bits=4)
+        assert torch.equal(ei.cpu().long(), idx)
+        u = torch.finfo(dtype).eps / 2
+        # gate, up and h are rounded once each: three half steps of |silu'| <= 1.1 gate up
+        assert float(((out.double().cpu() - want).abs() - (u * want.abs() + 3.3 * u * (terms + back) + 300 * 2.0 ** -24 * (terms + back))).max()) <= 0
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_ties_go_to_the_lower_expert(dev, bits):
+    x, wg, w, _ = make(5, 128, 64, 8, 3, BF16, bits)
+    wg[5] = wg[2]
+    wg[7] = wg[2]
+    wg[2] *= 1
+    x[0] = 0                                              # every logit 0
+    _, ew, ei = run(dev, x, wg, w, 3, bits=bits)
+    _, _, idx = oracle.router(x, wg, 3)
+    assert torch.equal(ei.cpu().long(), idx)
+    assert ei[0].tolist() == [0, 1, 2] and torch.allclose(ew[0].cpu(), torch.full((3,), 1 / 3))
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_what_is_not_finite_stays_with_its_token(dev, bits):
+    T, d, f, E, k = 6, 128, 192, 4, 2
+    x, wg, w, _ = make(T, d, f, E, k, BF16, bits)
+    clean = run(dev, x, wg, w, k, bits=bits)
+    x2 = x.clone()
+    x2[2, 5] = float("nan")
+    x2[4, 9] = float("inf")
+    out, ew, ei = run(dev, x2, wg, w, k, bits=bits)
+    assert int(ei.min()) >= 0 and int(ei.max()) < E
+    keep = [0, 1, 3, 5]
+    for a, b in zip((out, ew, ei), clean):
+        assert torch.equal(a[keep], b[keep])
+    assert torch.isnan(out[2]).all() and not torch.isfinite(out[4]).any()
+    # ... and an expert's weights with those that chose it
+    chosen = (clean[2] == 1).any(-1).cpu()
+    if bits == 16:
+        w[1][1, 3, 7], w[0][1, 8, 2] = float("inf"), float("nan")
+    else:
+        w[1][1][1, 7, 0], w[0][1][1, 8, 0] = 255, 255
+    out, ew, ei = run(dev, x, wg, w, k, bits=bits)
+    assert torch.equal(ew, clean[1]) and torch.equal(ei, clean[2])
+    assert bool(chosen.any()) and not bool(chosen.all())
+    assert torch.equal(out[~chosen], clean[0][~chosen])
+    assert not torch.isfinite(out[chosen]).all()
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_repeats_itself_and_in_a_graph(dev, bits):
+    T, d, f, E, k = 9, 256, 448, 8, 2
+    x, wg, w, _ = make(T, d, f, E, k, BF16, bits)
+    xs = [(x + i).to(dev) for i in range(4)]
+    wgd = wg.to(dev)
+    wd = [t.to(dev) for t in w] if bits == 16 else moe.Fp4ExpertWeights(*(t.to(dev) for q in w for t in q))
+    call = (lambda v: moe.moe_layer_decode(v, wgd, *wd, k)) if bits == 16 else (lambda v: moe.moe_layer_forward_fp4(v, wgd, wd, k))
+    with torch.no_grad():
+        eager = [call(v) for v in xs]
+        for v, e in zip(xs, eager):
+            for _ in range(5):
+                assert all(torch.equal(a, b) for a, b in zip(call(v), e))
+        buf = xs[0].clone()
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            call(buf)
+        torch.cuda.current_stream().wait_stream(s)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = call(buf)
+        for n in range(8):
+            buf.copy_(xs[n % 4])
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, eager[n % 4])), n
+            call(xs[(n + 1) % 4])
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_two_calls_at_once(dev, bits):
+    T, d, f, E, k = 4, 512, 1024, 8, 2
+    x, wg, w, _ = make(T, d, f, E, k, BF16, bits)
+    xd = [(x * (i + 1)).to(dev) for i in range(2)]
+    wgd = wg.to(dev)
+    wd = [t.to(dev) for t in w] if bits == 16 else moe.Fp4ExpertWeights(*(t.to(dev) for q in w for t in q))
+    call = (lambda v: moe.moe_layer_decode(v, wgd, *wd, k)) if bits == 16 else (lambda v: moe.moe_layer_forward_fp4(v, wgd, wd, k))
+    with torch.no_grad():
+        want = [call(v) for v in xd]
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        torch.cuda.synchronize()
+        got = [[], []]
+        for _ in range(20):
+            for i, s in enumerate(streams):
+                with torch.cuda.stream(s):
+                    got[i].append(call(xd[i]))
+        torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(a, b) for r in got[i] for a, b in zip(r, want[i]))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_strides_and_unaligned_inputs(dev, dtype):
+    T, d, f, E, k = 5, 128, 192, 4, 2
+    x, wg, w, _ = make(T, d, f, E, k, dtype, 16)
+    want = run(dev, x, wg, w, k)
+    with torch.no_grad():
+        odd = lambda t: torch.cat((t[..., :3], t), -1)[..., 3:]
+        turned = lambda t: t.transpose(0, 1).contiguous().transpose(0, 1)
+        for move in (odd, turned):
+            got = moe.moe_layer_decode(move(x.to(dev)), move(wg.to(dev)), *(move(t.to(dev)) for t in w), k)
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_agrees_with_the_layer(dev):
+    """moe_layer_forward rounds its interims to the type; both lie within a few half steps of each other."""
+    x, wg, w, _ = make(8, 256, 512, 8, 2, BF16, 16)
+    out, ew, ei = run(dev, x, wg, w, 2)
+    with torch.no_grad():
+        o2, w2, i2 = moe.moe_layer_forward(x.to(dev), wg.to(dev), *(t.to(dev) for t in w), 2)
+    assert torch.equal(ei, i2) and torch.allclose(ew, w2, rtol=1e-5)
+    assert float((out.float() - o2.float()).norm() / o2.float().norm()) < 4 * 2.0 ** -8
+
+
+def test_empty(dev):
+    x, wg, w, _ = make(1, 64, 64, 2, 1, BF16, 16)
+    with torch.no_grad():
+        out, ew, ei = moe.moe_layer_decode(x[:0].to(dev), wg.to(dev), *(t.to(dev) for t in w), 1)
+    assert out.shape == (0, 64) and ew.shape == (0, 1) and ei.shape == (0, 1)
