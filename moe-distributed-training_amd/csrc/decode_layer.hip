@@ -23,30 +23,25 @@ constexpr int TOK = MOE_DECODE_TOKENS, MAXK = MOE_DECODE_TOPK, MAXE = MOE_DECODE
 struct Chosen {
     int idx[TOK][MAXK];
     float weight[TOK][MAXK];
-    int used[MAXE];          // whether a token chose the expert
-    int active[MAXE];        // those experts, in order
-    int nactive;
+    uint32_t used[MAXE / 32];   // bits of the experts that a token chose
+    int active[MAXE];           // those experts, in order
 };
 
-// the chosen experts in order, from idx; all threads
-__device__ __forceinline__ void list_active(Chosen& c, int T, int E, int k)
+// the chosen experts in order, from their bits; all threads, behind a barrier
+__device__ __forceinline__ int list_active(Chosen& c)
 {
-    for (int e = threadIdx.x; e < E; e += THREADS) c.used[e] = 0;
-    __syncthreads();
-    for (int x = threadIdx.x; x < T * k; x += THREADS) c.used[c.idx[x / k][x % k]] = 1;   // (several threads may write the same 1)
-    __syncthreads();
-    if (threadIdx.x < 64) {
-        int n = 0;
-        for (int base = 0; base < E; base += 64) {
-            const int e = base + threadIdx.x;
-            const bool on = e < E && c.used[e];
-            const unsigned long long m = __ballot(on);
-            if (on) c.active[n + __popcll(m & ((1ull << threadIdx.x) - 1))] = e;
-            n += __popcll(m);
-        }
-        if (threadIdx.x == 0) c.nactive = n;
+    static_assert(THREADS >= MAXE, "a thread per expert");
+    const int e = threadIdx.x;
+    int n = 0, before = 0;
+#pragma unroll
+    for (int w = 0; w < MAXE / 32; ++w) {
+        const uint32_t bits = c.used[w];
+        before += __popc(e >> 5 > w ? bits : e >> 5 == w ? bits & ((1u << (e & 31)) - 1) : 0u);
+        n += __popc(bits);
     }
+    if (e < MAXE && c.used[e >> 5] >> (e & 31) & 1) c.active[before] = e;
     __syncthreads();
+    return __builtin_amdgcn_readfirstlane(n);
 }
 
 // which of token t's choices is expert e: -1 if none
@@ -57,122 +52,265 @@ __device__ __forceinline__ int choice_of(const Chosen& c, int t, int e, int k)
     return at;
 }
 
-// numbers in an order that unsigned integers have (NaN, of either sign, before all others)
+// numbers in an order that positive integers have (NaN, of either sign, before all others)
 __device__ __forceinline__ uint32_t order_of(float v)
 {
-    if (v != v) return 0;
+    if (v != v) return 1;
     const uint32_t b = __float_as_uint(v);
     return b >> 31 ? ~b : b | 0x80000000u;
 }
 
-// Logits, softmax and choices of all tokens, in LDS (scratch: WAVES * 1 KiB of sums and TOK * MAXE logits).
-template <class Num> __device__ __forceinline__ void route(const MoeDecode& p, Chosen& c, float* red, float* logits)
+// the largest value of the wave's lanes, in every lane: within rows of 16 lanes and from row to row without LDS
+__device__ __forceinline__ uint32_t wave_max(uint32_t v)
 {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, q = lane >> 4;
-    const int chunks = (p.d + few::CHUNK - 1) / few::CHUNK;
-    typedef few::Cols16<Num, 1> W;
-    few::Rows<1> rows;
-    rows.K = p.d;
-    rows.x[0] = few::buffer(p.x);
-    rows.a[0] = i < p.T ? (uint32_t)(i * p.ldx + 8 * q) * 2 : few::RANGE;
-    W w;
-    w.w[0] = w.w[1] = few::buffer(p.wg);
-    w.left = p.d - 8 * q;
-    for (int eb = 0; eb < p.E; eb += 16) {
-        const int e = eb + i < p.E ? eb + i : p.E - 1;
-        w.c[0] = (uint32_t)(e * p.ldwg + 8 * q) * 2;
-        f32x4_t acc[1][1] = {{(f32x4_t){0.f, 0.f, 0.f, 0.f}}};
-        few::stream<W, 1, false, 4>(acc, w, rows, chunks * wave / WAVES, chunks * (wave + 1) / WAVES);
-        *(f32x4_t*)(red + (wave * 64 + lane) * 4) = acc[0][0];
-        __syncthreads();
-        if (threadIdx.x < 256) {   // expert eb + x of token t
-            const int t = threadIdx.x & 15, x = threadIdx.x >> 4;
-            double sum = 0;   // (choices between experts are values next to a border)
-            for (int v = 0; v < WAVES; ++v) sum += (double)red[(v * 64 + (x >> 2) * 16 + t) * 4 + (x & 3)];
-            if (eb + x < p.E) logits[t * MAXE + eb + x] = (float)sum;
-        }
-        __syncthreads();
-    }
-    // a wave per token: softmax over its experts, then the largest one after the other
+    auto with = [&](auto ctrl, auto rows) {
+        const uint32_t o = __builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, decltype(rows)::value, 0xf, true);
+        v = o > v ? o : v;
+    };
+    with(std::integral_constant<int, DPP_ROW_SHR + 1>{}, std::integral_constant<int, 0xf>{});
+    with(std::integral_constant<int, DPP_ROW_SHR + 2>{}, std::integral_constant<int, 0xf>{});
+    with(std::integral_constant<int, DPP_ROW_SHR + 4>{}, std::integral_constant<int, 0xf>{});
+    with(std::integral_constant<int, DPP_ROW_SHR + 8>{}, std::integral_constant<int, 0xf>{});
+    with(std::integral_constant<int, DPP_ROW_BCAST15>{}, std::integral_constant<int, 0xa>{});
+    with(std::integral_constant<int, DPP_ROW_BCAST31>{}, std::integral_constant<int, 0xc>{});
+    return __builtin_amdgcn_readlane(v, 63);
+}
+__device__ __forceinline__ float wave_sum(float v)
+{
+    auto with = [&](auto ctrl, auto rows) {
+        v += __uint_as_float(__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), decltype(ctrl)::value, decltype(rows)::value, 0xf, true));
+    };
+    with(std::integral_constant<int, DPP_ROW_SHR + 1>{}, std::integral_constant<int, 0xf>{});
+    with(std::integral_constant<int, DPP_ROW_SHR + 2>{}, std::integral_constant<int, 0xf>{});
+    with(std::integral_constant<int, DPP_ROW_SHR + 4>{}, std::integral_constant<int, 0xf>{});
+    with(std::integral_constant<int, DPP_ROW_SHR + 8>{}, std::integral_constant<int, 0xf>{});
+    with(std::integral_constant<int, DPP_ROW_BCAST15>{}, std::integral_constant<int, 0xa>{});
+    with(std::integral_constant<int, DPP_ROW_BCAST31>{}, std::integral_constant<int, 0xc>{});
+    return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), 63));
+}
+
+// Softmax and choices of all tokens from their logits: a wave per token.
+__device__ __forceinline__ void choose(const MoeDecode& p, Chosen& c, const float* logits)
+{
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    constexpr int PER = MAXE / 64;
+    const int per = (p.E + 63) / 64;
     for (int t = wave; t < p.T; t += WAVES) {
-        constexpr int PER = MAXE / 64;
-        float v[PER], top = -__builtin_inff();
-        unsigned long long key[PER];
-        bool nan = false;
+        float v[PER];
+        uint32_t key[PER], top = 0;
+        for (int r = 0; r < PER; ++r) { v[r] = 0.f; key[r] = 0; }
+        // (the key of a taken or absent expert is 0)
 #pragma unroll
-        for (int r = 0; r < PER; ++r) {
-            const int e = r * 64 + lane;
-            v[r] = e < p.E ? logits[t * MAXE + e] : -__builtin_inff();
-            top = fmaxf(top, v[r]);
-            nan = nan || v[r] != v[r];
-            // (ties to the lower expert; an expert's key is never 0, that of a taken or absent one is)
-            key[r] = e < p.E ? (unsigned long long)order_of(v[r]) << 32 | (0xffffffffu - e) : 0;
-        }
+        for (int r = 0; r < PER; ++r)
+            if (r < per && r * 64 + lane < p.E) {
+                v[r] = logits[t * MAXE + r * 64 + lane];
+                key[r] = order_of(v[r]);
+                top = key[r] > top ? key[r] : top;
+            }
         float sum = 0.f;
-        for (int m = 32; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor(top, m));
+        const uint32_t most = wave_max(top);
+        const float shift = __uint_as_float(most >> 31 ? most & 0x7fffffffu : ~most);   // the largest logit
 #pragma unroll
-        for (int r = 0; r < PER; ++r) {
-            v[r] = r * 64 + lane < p.E ? expf(v[r] - top) : 0.f;
-            sum += v[r];
-        }
-        for (int m = 32; m > 0; m >>= 1) sum += __shfl_xor(sum, m);
-        if (__any(nan)) sum = __builtin_nanf("");
-        float chosen[MAXK], total = 0.f;
+        for (int r = 0; r < PER; ++r)
+            if (r < per && r * 64 + lane < p.E) {
+                v[r] = expf(v[r] - shift);
+                sum += v[r];
+            }
+        sum = wave_sum(sum);
+        float total = 0.f;
+        float chosen = 0.f;   // lane j keeps the weight of choice j
+        int choice = 0;
         for (int j = 0; j < p.k; ++j) {
-            unsigned long long best = 0;
+            uint32_t best = 0;
 #pragma unroll
             for (int r = 0; r < PER; ++r) best = key[r] > best ? key[r] : best;
-            for (int m = 32; m > 0; m >>= 1) {
-                const unsigned long long o = __shfl_xor(best, m);
-                best = o > best ? o : best;
-            }
-            const int e = (int)(0xffffffffu - (uint32_t)best);
-            float mine = 0.f;
+            best = wave_max(best);
+            int e = 0;
+            float s = 0.f;
+            bool found = false;
 #pragma unroll
             for (int r = 0; r < PER; ++r)
-                if (r * 64 + lane == e) { mine = v[r]; key[r] = 0; }
-            chosen[j] = __shfl(mine, e & 63) / sum;
-            total += chosen[j];
-            if (lane == 0) c.idx[t][j] = e;
+                if (r < per && !found) {   // ties: the lower expert
+                    const unsigned long long hit = __ballot(key[r] == best);
+                    if (hit != 0) {
+                        const int l = __ffsll(hit) - 1;
+                        e = r * 64 + l;
+                        s = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v[r]), l)) / sum;
+                        if (lane == l) key[r] = 0;
+                        found = true;
+                    }
+                }
+            total += s;
+            if (lane == j) { chosen = s; choice = e; }
         }
-        for (int j = 0; j < p.k; ++j)
-            if (lane == 0) c.weight[t][j] = p.normalize ? chosen[j] / total : chosen[j];
+        if (lane < p.k) {
+            c.idx[t][lane] = choice;
+            c.weight[t][lane] = p.normalize ? chosen / total : chosen;
+            atomicOr(&c.used[choice >> 5], 1u << (choice & 31));
+        }
     }
     __syncthreads();
 }
 
-template <class W> __device__ __forceinline__ void gate_up_columns(const MoeDecode& p, W& w, int e, int n, int i, int q)
+// Logits of all tokens for experts of a block of 16 each, from the waves' sums red[wave][64][4]: a block of `blocks` from eb on is shared by `split` waves.
+__device__ __forceinline__ void sum_logits(const MoeDecode& p, const float* red, float* logits, int eb, int blocks, int split)
 {
-    if constexpr (std::is_same<W, few::Fp4Cols<typename W::Num, 2>>::value) {
-        w.two = true;
-        w.left = p.d / FP4_GROUP - q;
+    for (int x = threadIdx.x; x < blocks * 256; x += THREADS) {
+        const int t = x & 15, y = x >> 4 & 15, b = x >> 8, e = (eb + b) * 16 + y;
+        double sum = 0;   // (choices between experts are values next to a border)
+        for (int v = 0; v < split; ++v) sum += (double)red[((b * split + v) * 64 + (y >> 2) * 16 + t) * 4 + (y & 3)];
+        if (e < p.E) logits[t * MAXE + e] = (float)sum;
+    }
+}
+
+// rows of x
+__device__ __forceinline__ few::Rows<1> token_rows(const MoeDecode& p, const void* x, int64_t ldx, int K)
+{
+    const int lane = threadIdx.x & 63;
+    few::Rows<1> r;
+    r.x[0] = few::buffer(x);
+    r.left = K - 8 * (lane & 15);
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            const MoeFp4Weights& f = m ? p.f3 : p.f1;
-            w.codes[m] = few::buffer(f.codes + e * f.sce);
-            w.scales[m] = few::buffer(f.scales + e * f.sse);
-            w.c[m] = (uint32_t)((n + i) * f.scn) + q * FP4_GROUP_BYTES;
-            w.s[m] = (uint32_t)((n + i) * f.ssn) + q;
+    for (int j = 0; j < 4; ++j) {
+        const int t = 4 * j + (lane >> 4);
+        r.a[0][j] = t < p.T ? (uint32_t)(t * ldx + 8 * (lane & 15)) * 2 : few::RANGE;
+    }
+    return r;
+}
+
+// Logits, softmax and choices where x is not kept
+template <class Num> __device__ __forceinline__ void route(const MoeDecode& p, Chosen& c, float* red, float* logits, uint8_t* scratch)
+{
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int chunks = (p.d + few::CHUNK - 1) / few::CHUNK;
+    typedef few::Cols16<Num, 1> W;
+    const few::Rows<1> rows = token_rows(p, p.x, p.ldx, p.d);
+    W w;
+    w.w[0] = w.w[1] = few::buffer(p.wg);
+    w.left = p.d - 8 * few::quad_piece(lane);
+    for (int eb = 0; eb * 16 < p.E; ++eb) {
+        const int x = eb * 16 + (lane >> 2), e = x < p.E ? x : p.E - 1;
+        w.c[0] = (uint32_t)(e * p.ldwg + 8 * few::quad_piece(lane)) * 2;
+        f32x4_t acc[1][1] = {{(f32x4_t){0.f, 0.f, 0.f, 0.f}}};
+        few::stream<W, 1, false, 4, 4>(acc, w, rows, chunks * wave / WAVES, chunks * (wave + 1) / WAVES, scratch);
+        *(f32x4_t*)(red + (wave * 64 + lane) * 4) = acc[0][0];
+        __syncthreads();
+        sum_logits(p, red, logits, eb, 1, WAVES);
+        __syncthreads();
+    }
+    choose(p, c, logits);
+}
+
+// ... and where it is, in the order of W's pieces: the waves of a group of `split` share a block's inputs, groups take different blocks, and the router's rows of the next block are on
+// their way while one is summed.  (Loaded as rows of x are: 16 experts x 256 bytes.)
+template <class W> __device__ __forceinline__ void route_kept(const MoeDecode& p, Chosen& c, float* red, float* logits, const few::Rows<1>::Stage (&xs)[4], uint8_t* scratch)
+{
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, q = lane >> 4;
+    const int group = wave / p.split, groups = WAVES / p.split, c0 = (wave & (p.split - 1)) * 4, nblocks = (p.E + 15) / 16;
+    few::Rows<1>::Stage f[2][4];
+    auto fetch = [&](int to, int eb) {
+        few::Rows<1> r;
+        r.x[0] = few::buffer(p.wg);
+        r.left = p.d - 8 * i;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int e = eb * 16 + 4 * j + q;
+            r.a[0][j] = e < p.E ? (uint32_t)(e * p.ldwg + 8 * i) * 2 : few::RANGE;
         }
+#pragma unroll
+        for (int d = 0; d < 4; ++d) r.load(f[to][d], c0 + d);
+    };
+    auto block = [&](int from, int eb0) {   // blocks eb0 .. eb0 + groups - 1
+        f32x4_t acc = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            few::Rows<1>().template ready<W>(f[from][d], scratch);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc = W::Num::mfma(__builtin_bit_cast(bf16x8_t, f[from][d].f[0][j]), __builtin_bit_cast(bf16x8_t, xs[d].f[0][j]), acc);
+        }
+        *(f32x4_t*)(red + (wave * 64 + lane) * 4) = acc;
+        __syncthreads();
+        sum_logits(p, red, logits, eb0, groups, p.split);
+        __syncthreads();
+    };
+    fetch(0, group);
+    if (groups < nblocks) fetch(1, groups + group);
+    for (int eb0 = 0; eb0 < nblocks; eb0 += 2 * groups) {
+        block(0, eb0);
+        if (eb0 + 2 * groups < nblocks) fetch(0, eb0 + 2 * groups + group);
+        if (eb0 + groups < nblocks) block(1, eb0 + groups);
+        if (eb0 + 3 * groups < nblocks) fetch(1, eb0 + 3 * groups + group);
+    }
+    choose(p, c, logits);
+}
+
+// One job's columns [n, n + 16) of both projections of expert e.
+template <class W> __device__ __forceinline__ void gate_up_columns(const MoeDecode& p, W& w, int e, int n)
+{
+    const int lane = threadIdx.x & 63;
+    if constexpr (!std::is_same<W, few::Cols16<typename W::Num, 2>>::value) {
+        w.columns(0, p.f1, e, p.d, [&](int, int c) { return (int64_t)n + c; });
+        w.columns(1, p.f3, e, p.d, [&](int, int c) { return (int64_t)n + c; });
     } else {
-        w.left = p.d - 8 * q;
+        w.left = p.d - 8 * few::quad_piece(lane);
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
             w.w[m] = few::buffer((const uint16_t*)(m ? p.w3 : p.w1) + (int64_t)e * p.f * p.d);
-            w.c[m] = (uint32_t)((int64_t)(n + i) * p.d + 8 * q) * 2;
+            w.c[m] = (uint32_t)((int64_t)(n + (lane >> 2)) * p.d + 8 * few::quad_piece(lane)) * 2;
         }
     }
 }
 
-template <class Num, bool FP4>
-__global__ void __launch_bounds__(THREADS) gate_up_kernel(const MoeDecode p)
+// silu(gate) * up of four columns of a token, as two numbers of the type
+template <class Num> __device__ __forceinline__ void store_h(const MoeDecode& p, int row, int n, f32x4_t g, f32x4_t u)
 {
-    typedef typename std::conditional<FP4, few::Fp4Cols<Num, 2>, few::Cols16<Num, 2>>::type W;
+    float hi[4], lo[4];
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+        const float h = g[v] / (1.f + __expf(-g[v])) * u[v];
+        hi[v] = Num::to_f32(Num::from_f32(h));
+        lo[v] = fabsf(hi[v]) < __builtin_inff() ? h - hi[v] : 0.f;
+    }
+    uint16_t* h = p.h + ((int64_t)row * p.f + n);
+    *(uint2*)h = make_uint2(Num::pack2(hi[0], hi[1]), Num::pack2(hi[2], hi[3]));
+    *(uint2*)(h + p.h_lo) = make_uint2(Num::pack2(lo[0], lo[1]), Num::pack2(lo[2], lo[3]));
+}
+
+// KEPT (hidden sizes up to 4096): p.split waves share a job's contraction, four chunks each, so that every job meets a wave with the same chunks of x: they stay in registers, and the
+// ring holds exactly one job: while chunk d of a job is multiplied, chunk d of the next one is requested into its place.  With 8 / p.split jobs at a time.
+// Otherwise all eight waves share a job, chunk by chunk through few::stream.
+// a wave's scratch: its rows of x and its weights, or the router's
+template <class W, bool KEPT> constexpr int gate_up_scratch()
+{
+    constexpr int router = few::Cols16<typename W::Num, 1>::SCRATCH;
+    return few::Rows<1>::SCRATCH + (KEPT ? 0 : W::SCRATCH > router ? W::SCRATCH : router);
+}
+
+template <class Num, int BITS, bool KEPT, bool QUADS>
+__global__ void __launch_bounds__(THREADS, 2) gate_up_kernel(const MoeDecode p)
+{
+    constexpr bool FP4 = BITS == 4;
+    typedef typename std::conditional<FP4, typename std::conditional<QUADS, few::Fp4Quads<Num, 2, true>, few::Fp4Cols<Num, 2, true>>::type, few::Cols16<Num, 2>>::type W;
+    static_assert(!KEPT || QUADS || !FP4, "whole chunks");
+    constexpr int SCRATCH = gate_up_scratch<W, KEPT>();
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];   // every wave's scratch
+    constexpr int AHEAD = FP4 ? 2 : 1;   // jobs in the ring: 128 or 256 KiB on their way per compute unit
     __shared__ Chosen c;
     __shared__ __attribute__((aligned(16))) float red[2][WAVES][2][64][4];   // sums of two jobs; before them the router's
     __shared__ float logits[TOK * MAXE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, q = lane >> 4;
-    route<Num>(p, c, &red[0][0][0][0][0], logits);
+    if (threadIdx.x < MAXE / 32) c.used[threadIdx.x] = 0;   // (the router's barriers lie in between)
+    uint8_t* scratch = smem + wave * SCRATCH;
+    const few::Rows<1> rows = token_rows(p, p.x, p.ldx, p.d);
+    few::Rows<1>::Stage xs[4];
+    const int member = KEPT ? wave & (p.split - 1) : 0, c0 = member * 4;
+    if constexpr (KEPT) {
+#pragma unroll
+        for (int d = 0; d < 4; ++d) rows.load(xs[d], c0 + d);
+#pragma unroll
+        for (int d = 0; d < 4; ++d) rows.template ready<W>(xs[d], scratch);
+        route_kept<W>(p, c, &red[0][0][0][0][0], logits, xs, scratch);
+    } else route<Num>(p, c, &red[0][0][0][0][0], logits, scratch);
     if (blockIdx.x == 0) {
         for (int x = threadIdx.x; x < p.T * p.k; x += THREADS) {
             p.indices[x] = c.idx[x / p.k][x % p.k];
@@ -180,39 +318,122 @@ __global__ void __launch_bounds__(THREADS) gate_up_kernel(const MoeDecode p)
         }
         for (int x = threadIdx.x; x < p.counters_n; x += THREADS) p.counters[x] = 0;   // of launch 2
     }
-    list_active(c, p.T, p.E, p.k);
-    const int ncb = p.f / 16, jobs = c.nactive * ncb, chunks = (p.d + few::CHUNK - 1) / few::CHUNK;
-    few::Rows<1> rows;
-    rows.K = p.d;
-    rows.x[0] = few::buffer(p.x);
-    rows.a[0] = i < p.T ? (uint32_t)(i * p.ldx + W::input(0, q)) * 2 : few::RANGE;
-    int turn = 0;
-    for (int job = blockIdx.x; job < jobs; job += gridDim.x, ++turn) {
-        const int e = __builtin_amdgcn_readfirstlane(c.active[job / ncb]), n = __builtin_amdgcn_readfirstlane(job % ncb) * 16;
+    const int ncb = p.f / 16, jobs = list_active(c) * ncb;
+    auto place = [&](int job, int* e, int* n) {
+        *e = __builtin_amdgcn_readfirstlane(c.active[job / ncb]);
+        *n = __builtin_amdgcn_readfirstlane(job % ncb) * 16;
+    };
+    if constexpr (KEPT) {
+        const int split = p.split, at_once = WAVES / split;
+        const int step = gridDim.x * at_once, first = blockIdx.x * at_once + wave / split;
+        const int rounds = (jobs - (int)blockIdx.x * at_once + step - 1) / step;   // of this workgroup, the same for all of its waves
         W w;
-        gate_up_columns(p, w, e, n, i, q);
-        f32x4_t acc[1][2] = {{(f32x4_t){0.f, 0.f, 0.f, 0.f}, (f32x4_t){0.f, 0.f, 0.f, 0.f}}};
-        few::stream<W, 1, false, FP4 ? 4 : 2>(acc, w, rows, chunks * wave / WAVES, chunks * (wave + 1) / WAVES);
-        float (*r)[2][64][4] = red[turn & 1];   // (the other one may still be read)
-        *(f32x4_t*)r[wave][0][lane] = acc[0][0];
-        *(f32x4_t*)r[wave][1][lane] = acc[0][1];
-        __syncthreads();
-        if (wave == (turn & (WAVES - 1)) && i < p.T) {
-            const int j = choice_of(c, i, e, p.k);
-            if (j >= 0) {
-                f32x4_t g = (f32x4_t){0.f, 0.f, 0.f, 0.f}, u = g;
+        bool some = false;
+        constexpr int UNITS = 4 / W::UNIT;
+        typename W::Stage ring[AHEAD][UNITS];
+        fp4_u32x4_t scales[AHEAD][2];   // of the four chunks, 16 bytes: lane l brings those of column l
+        auto turn_to = [&](int job, fp4_u32x4_t (&to)[2]) {   // where a job's weights lie; there may be none
+            int e = 0, n = 0;
+            some = job < jobs;
+            if (some) place(job, &e, &n);
+            gate_up_columns(p, w, e, n);
+            if constexpr (FP4) {
+                const bool mine = some && lane < 16 && (c0 + 4) * few::CHUNK <= p.d;
 #pragma unroll
-                for (int v = 0; v < WAVES; ++v) { g += *(const f32x4_t*)r[v][0][lane]; u += *(const f32x4_t*)r[v][1][lane]; }
-                float hi[4], lo[4];
+                for (int m = 0; m < 2; ++m) to[m] = few::load16(w.scales[m], mine ? w.s[m] : few::RANGE, c0 * 4);
+            } else if (!some) w.left = 0;
+        };
+        auto fetch = [&](typename W::Stage& to, int u) {
+            if constexpr (FP4) {
+                const bool in = some && (c0 + 2 * u) * few::CHUNK < p.d;
 #pragma unroll
-                for (int v = 0; v < 4; ++v) {
-                    const float h = g[v] / (1.f + __expf(-g[v])) * u[v];
-                    hi[v] = Num::to_f32(Num::from_f32(h));
-                    lo[v] = fabsf(hi[v]) < __builtin_inff() ? h - hi[v] : 0.f;
+                for (int m = 0; m < 2; ++m)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) to.c[m][h] = few::load16_streamed(w.codes[m], in ? w.c[m][h] : few::RANGE, (c0 / 2 + u) * 128);
+            } else w.load(to, c0 + u);
+        };
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) {
+            turn_to(a < rounds ? first + a * step : jobs, scales[a]);
+#pragma unroll
+            for (int u = 0; u < UNITS; ++u) fetch(ring[a][u], u);
+        }
+        for (int r0 = 0; r0 < rounds; r0 += AHEAD)
+#pragma unroll
+            for (int a = 0; a < AHEAD; ++a) {
+                const int r = r0 + a;
+                if (AHEAD > 1 && r >= rounds) break;
+                const int job = first + r * step;
+                fp4_u32x4_t now[2];   // scales of column lane & 15: byte q of word d
+                if constexpr (FP4) {
+#pragma unroll
+                    for (int m = 0; m < 2; ++m)
+                        if (lane < 16) *(fp4_u32x4_t*)(scratch + (m * 16 + lane) * 16) = scales[a][m];
+#pragma unroll
+                    for (int m = 0; m < 2; ++m) now[m] = *(const fp4_u32x4_t*)(scratch + (m * 16 + i) * 16);
                 }
-                uint16_t* h = p.h + ((int64_t)(i * p.k + j) * p.f + n + 4 * q);
-                *(uint2*)h = make_uint2(Num::pack2(hi[0], hi[1]), Num::pack2(hi[2], hi[3]));
-                *(uint2*)(h + p.h_lo) = make_uint2(Num::pack2(lo[0], lo[1]), Num::pack2(lo[2], lo[3]));
+                turn_to(r + AHEAD < rounds ? job + AHEAD * step : jobs, scales[a]);
+                f32x4_t acc[2] = {(f32x4_t){0.f, 0.f, 0.f, 0.f}, (f32x4_t){0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+                for (int v = 0; v < UNITS; ++v) {
+                    if constexpr (FP4) {
+#pragma unroll
+                        for (int m = 0; m < 2; ++m) few::from_lines(ring[a][v].c[m], scratch + m * 2048);
+                    } else w.ready(ring[a][v], scratch);
+#pragma unroll
+                    for (int cc = 0; cc < W::UNIT; ++cc)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+#pragma unroll
+                            for (int m = 0; m < 2; ++m) {
+                                const int d = v * W::UNIT + cc;
+                                bf16x8_t f;
+                                if constexpr (FP4) f = fp4_expand8<Num>(ring[a][v].c[m][cc][j], fp4_scale(now[m][d] >> (8 * q) & 0xff));
+                                else f = W::frag(ring[a][v], cc, m, j);
+                                acc[m] = Num::mfma(f, __builtin_bit_cast(bf16x8_t, xs[d].f[0][j]), acc[m]);
+                            }
+                    __builtin_amdgcn_sched_barrier(0);   // (as in few::stream)
+                    fetch(ring[a][v], v);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                float (*s)[2][64][4] = red[r & 1];   // (the other one may still be read)
+                *(f32x4_t*)s[wave][0][lane] = acc[0];
+                *(f32x4_t*)s[wave][1][lane] = acc[1];
+                __syncthreads();
+                if (member == (r & (split - 1)) && job < jobs && i < p.T) {
+                    int e, n;
+                    place(job, &e, &n);
+                    const int j = choice_of(c, i, e, p.k);
+                    if (j >= 0) {
+                        f32x4_t g = (f32x4_t){0.f, 0.f, 0.f, 0.f}, u = g;
+                        for (int v = wave - member; v < wave - member + split; ++v) { g += *(const f32x4_t*)s[v][0][lane]; u += *(const f32x4_t*)s[v][1][lane]; }
+                        store_h<Num>(p, i * p.k + j, n + 4 * q, g, u);
+                    }
+                }
+            }
+    } else {
+        constexpr int UNIT = W::UNIT * few::CHUNK;
+        const int units = (p.d + UNIT - 1) / UNIT;
+        int turn = 0;
+        for (int job = blockIdx.x; job < jobs; job += gridDim.x, ++turn) {
+            int e, n;
+            place(job, &e, &n);
+            W w;
+            gate_up_columns(p, w, e, n);
+            f32x4_t acc[1][2] = {{(f32x4_t){0.f, 0.f, 0.f, 0.f}, (f32x4_t){0.f, 0.f, 0.f, 0.f}}};
+            few::stream<W, 1, false, 2, 2>(acc, w, rows, units * wave / WAVES, units * (wave + 1) / WAVES, scratch);
+            float (*s)[2][64][4] = red[turn & 1];
+            *(f32x4_t*)s[wave][0][lane] = acc[0][0];
+            *(f32x4_t*)s[wave][1][lane] = acc[0][1];
+            __syncthreads();
+            if (wave == (turn & (WAVES - 1)) && i < p.T) {
+                const int j = choice_of(c, i, e, p.k);
+                if (j >= 0) {
+                    f32x4_t g = (f32x4_t){0.f, 0.f, 0.f, 0.f}, u = g;
+#pragma unroll
+                    for (int v = 0; v < WAVES; ++v) { g += *(const f32x4_t*)s[v][0][lane]; u += *(const f32x4_t*)s[v][1][lane]; }
+                    store_h<Num>(p, i * p.k + j, n + 4 * q, g, u);
+                }
             }
         }
     }
@@ -224,9 +445,12 @@ __global__ void __launch_bounds__(THREADS) gate_up_kernel(const MoeDecode p)
 // ends up with 8 consecutive columns of four tokens.
 constexpr int DOWN_PARTS_MAX = 64;
 
-template <class Num, bool FP4>
+template <class Num, int BITS, bool QUADS>
 __global__ void __launch_bounds__(THREADS) down_kernel(const MoeDecode p)
 {
+    constexpr bool FP4 = BITS == 4;
+    typedef typename std::conditional<QUADS, few::Fp4Quads<Num, 4, false>, few::Fp4Cols<Num, 4, false>>::type W;
+    constexpr int SCRATCH = W::SCRATCH + few::Rows<2>::SCRATCH;   // of a wave, with 4-bit weights
     constexpr int UNITS = 4, PER = FP4 ? 4 : 8;   // floats of a lane and unit: unit nb holds 4 columns of one token, unit r 8 columns of one
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     __shared__ Chosen c;
@@ -234,15 +458,22 @@ __global__ void __launch_bounds__(THREADS) down_kernel(const MoeDecode p)
     float* red = (float*)smem;   // [wave][unit][64][PER]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, q = lane >> 4;
     const int tile = blockIdx.x / p.parts, part = blockIdx.x - tile * p.parts;
-    for (int x = threadIdx.x; x < p.T * p.k; x += THREADS) {
-        c.idx[x / p.k][x % p.k] = p.indices[x];
+    static_assert(THREADS >= TOK * MAXK, "a thread per choice");
+    const int x = threadIdx.x;
+    const int choice = x < p.T * p.k ? p.indices[x] : 0;
+    if (x < MAXE / 32) c.used[x] = 0;
+    __syncthreads();
+    if (x < p.T * p.k) {
+        c.idx[x / p.k][x % p.k] = choice;
         c.weight[x / p.k][x % p.k] = p.weights[x];
+        atomicOr(&c.used[choice >> 5], 1u << (choice & 31));
     }
     __syncthreads();
-    list_active(c, p.T, p.E, p.k);
+    const int nactive = list_active(c);
     // this wave's share of the contraction: steps of the chosen experts one after the other
-    const int steps = FP4 ? (p.f + few::CHUNK - 1) / few::CHUNK : p.f / 32;
-    const int64_t total = (int64_t)c.nactive * steps;
+    constexpr int STEP = FP4 ? W::UNIT * few::CHUNK : 32;
+    const int steps = (p.f + STEP - 1) / STEP;
+    const int64_t total = (int64_t)nactive * steps;
     const int shares = p.parts * WAVES, share = part * WAVES + wave;
     int64_t at = total * share / shares;
     const int64_t end = total * (share + 1) / shares;
@@ -257,28 +488,22 @@ __global__ void __launch_bounds__(THREADS) down_kernel(const MoeDecode p)
         const int e = __builtin_amdgcn_readfirstlane(c.active[a]);
         at += s1 - s0;
         const int j = i < p.T ? choice_of(c, i, e, p.k) : -1;
-        few::Rows<2> rows;
-        rows.K = p.f;
-        rows.x[0] = few::buffer(p.h);
-        rows.x[1] = few::buffer(p.h + p.h_lo);
         if constexpr (FP4) {
-            typedef few::Fp4Cols<Num, 4> W;
             W w;
-            w.two = false;
-            w.left = p.f / FP4_GROUP - q;
-            w.codes[0] = few::buffer(p.f2.codes + e * p.f2.sce);
-            w.scales[0] = few::buffer(p.f2.scales + e * p.f2.sse);
+            w.columns(0, p.f2, e, p.f, [&](int nb, int c) { return (int64_t)tile * 64 + (c >> 2) * 16 + 4 * nb + (c & 3); });   // (d is a multiple of 64)
+            few::Rows<2> rows;
+            rows.x[0] = few::buffer(p.h);
+            rows.x[1] = few::buffer(p.h + p.h_lo);
+            rows.left = p.f - 8 * i;
 #pragma unroll
-            for (int nb = 0; nb < 4; ++nb) {
-                const int n = tile * 64 + (i >> 2) * 16 + 4 * nb + (i & 3);   // (d is a multiple of 64)
-                w.c[nb] = (uint32_t)(n * p.f2.scn) + q * FP4_GROUP_BYTES;
-                w.s[nb] = (uint32_t)(n * p.f2.ssn) + q;
+            for (int y = 0; y < 4; ++y) {
+                const int t = 4 * y + q, jt = t < p.T ? choice_of(c, t, e, p.k) : -1;
+                rows.a[0][y] = rows.a[1][y] = jt >= 0 ? (uint32_t)((t * p.k + jt) * p.f + 8 * i) * 2 : few::RANGE;
             }
-            rows.a[0] = rows.a[1] = j >= 0 ? (uint32_t)((i * p.k + j) * p.f + W::input(0, q)) * 2 : few::RANGE;
             f32x4_t acc[1][4];
 #pragma unroll
             for (int nb = 0; nb < 4; ++nb) acc[0][nb] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-            few::stream<W, 2, true, 2>(acc, w, rows, s0, s1);
+            few::stream<W, 2, true, 2, 2>(acc, w, rows, s0, s1, smem + wave * SCRATCH);
             const float g = j >= 0 ? c.weight[i][j] : 0.f;
 #pragma unroll
             for (int u = 0; u < UNITS; ++u)
@@ -289,6 +514,7 @@ __global__ void __launch_bounds__(THREADS) down_kernel(const MoeDecode p)
             const int n = tile * 128 + 8 * i;
             const uint32_t col = n < p.d ? (uint32_t)(n + 8 * q * p.d) * 2 : few::RANGE;
             const uint32_t row = j >= 0 ? (uint32_t)((i * p.k + j) * p.f + 8 * q) * 2 : few::RANGE;
+            const few::Buffer hb[2] = {few::buffer(p.h), few::buffer(p.h + p.h_lo)};
             f32x4_t acc[8];
 #pragma unroll
             for (int b = 0; b < 8; ++b) acc[b] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
@@ -299,7 +525,8 @@ __global__ void __launch_bounds__(THREADS) down_kernel(const MoeDecode p)
 #pragma unroll
                 for (int r = 0; r < 8; ++r) ws[dst][r] = few::load16_streamed(w, col, (uint32_t)(s * 32 + r) * (uint32_t)p.d * 2);
 #pragma unroll
-                for (int m = 0; m < 2; ++m) as[dst][m] = few::load16(rows.x[m], row, (uint32_t)s * 64);
+                for (int m = 0; m < 2; ++m) as[dst][m] = __builtin_bit_cast(bf16x8_t, few::load16(hb[m], row, (uint32_t)s * 64));
+                __builtin_amdgcn_sched_barrier(0);
             };
             auto multiply = [&](int src) {
 #pragma unroll
@@ -312,6 +539,7 @@ __global__ void __launch_bounds__(THREADS) down_kernel(const MoeDecode p)
                     acc[b] = Num::mfma(as[src][0], wf, acc[b]);
                     acc[b] = Num::mfma(as[src][1], wf, acc[b]);
                 }
+                __builtin_amdgcn_sched_barrier(0);   // (as in few::stream)
             };
             int s = s0;
             if (s1 - s0 >= DEPTH) {
@@ -341,6 +569,7 @@ __global__ void __launch_bounds__(THREADS) down_kernel(const MoeDecode p)
         }
     }
     // ---- the waves' sums, in wave order
+    __syncthreads();   // (they take the place of the operands)
 #pragma unroll
     for (int u = 0; u < UNITS; ++u)
 #pragma unroll
@@ -391,16 +620,26 @@ __global__ void __launch_bounds__(THREADS) down_kernel(const MoeDecode p)
     for (int v = 0; v < PER; v += 4) *(uint2*)(o + v) = make_uint2(Num::pack2(sum[v], sum[v + 1]), Num::pack2(sum[v + 2], sum[v + 3]));
 }
 
-struct Plan { int grid1, tiles, parts; size_t h_bytes, counter_bytes, slot_bytes; };
+inline int64_t chunks_of(int64_t n) { return (n + few::CHUNK - 1) / few::CHUNK; }
+
+struct Plan { int grid1, split, tiles, parts; size_t h_bytes, counter_bytes, slot_bytes; };
 Plan plan(int T, int E, int d, int f, int k, bool fp4)
 {
     Plan r = {};
     const int cus = moe_device_cus();
     const int64_t jobs = (int64_t)(E < T * k ? E : T * k) * (f / 16);
-    r.grid1 = (int)(jobs < 2 * cus ? jobs : 2 * cus);
+    // split: 0 where a wave cannot keep its part of x (gate_up_kernel)
+    const int chunks = (d + few::CHUNK - 1) / few::CHUNK;
+    r.split = 0;
+    if (chunks <= 4 * WAVES && (!fp4 || d % (4 * few::CHUNK) == 0))
+        for (r.split = 1; r.split * 4 < chunks;) r.split *= 2;
+    const int64_t at_once = r.split ? WAVES / r.split : 1, groups = (jobs + at_once - 1) / at_once;
+    r.grid1 = (int)(groups < cus ? groups : cus);
     r.tiles = fp4 ? d / 64 : (d + 127) / 128;
+    // parts of launch 2: until every compute unit has one, as long as its waves have two steps each
+    const int64_t steps = (int64_t)(E < T * k ? E : T * k) * (fp4 ? chunks_of(f) : f / 32);
     r.parts = 1;
-    while (r.parts < DOWN_PARTS_MAX && r.tiles * r.parts < cus) r.parts *= 2;
+    while (r.parts < DOWN_PARTS_MAX && r.tiles * r.parts < cus && steps >= r.parts * 2 * WAVES * 2) r.parts *= 2;
     auto al = [](size_t n) { return (n + 255) & ~(size_t)255; };
     r.h_bytes = al((size_t)T * k * f * 2);
     r.counter_bytes = al((size_t)r.tiles * 4);
@@ -408,12 +647,30 @@ Plan plan(int T, int E, int d, int f, int k, bool fp4)
     return r;
 }
 
-template <class Num, bool FP4> int launch_typed(const MoeDecode& p, const Plan& pl, hipStream_t stream)
+template <class Num, int BITS> int launch_typed(const MoeDecode& p, const Plan& pl, hipStream_t stream)
 {
-    constexpr size_t lds = (size_t)WAVES * 4 * 64 * (FP4 ? 4 : 8) * 4;
-    hipLaunchKernelGGL((gate_up_kernel<Num, FP4>), dim3((unsigned)pl.grid1), dim3(THREADS), 0, stream, p);
-    hipLaunchKernelGGL((down_kernel<Num, FP4>), dim3((unsigned)(pl.tiles * pl.parts)), dim3(THREADS), lds, stream, p);
-    return moe_launch_status();
+    constexpr bool FP4 = BITS == 4;
+    auto go = [&](auto kern, int grid, size_t lds, std::atomic<bool>* attr_set) {
+        const int dev = moe_current_device();
+        if (!attr_set[dev]) {
+            if (hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess) return MOE_ERR_LAUNCH;
+            attr_set[dev] = true;
+        }
+        hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(THREADS), lds, stream, p);
+        return moe_launch_status();
+    };
+    static std::atomic<bool> set1[3][MOE_MAX_DEVICES], set2[2][MOE_MAX_DEVICES];
+    typedef few::Fp4Quads<Num, 2, true> Q2;
+    typedef few::Fp4Quads<Num, 4, false> Q4;
+    constexpr size_t rows2 = few::Rows<2>::SCRATCH, sums = (size_t)4 * 64 * (FP4 ? 4 : 8) * 4;
+    int rc;
+    if (p.split) rc = go(gate_up_kernel<Num, BITS, true, true>, pl.grid1, WAVES * gate_up_scratch<Q2, true>(), set1[0]);
+    else if (FP4 && p.d % (2 * few::CHUNK)) rc = go(gate_up_kernel<Num, BITS, false, false>, pl.grid1, WAVES * gate_up_scratch<few::Fp4Cols<Num, 2, true>, false>(), set1[1]);
+    else rc = go(gate_up_kernel<Num, BITS, false, true>, pl.grid1, WAVES * (FP4 ? gate_up_scratch<Q2, false>() : gate_up_scratch<few::Cols16<Num, 2>, false>()), set1[2]);
+    if (rc != MOE_OK) return rc;
+    if (FP4 && p.f % (2 * few::CHUNK)) return go(down_kernel<Num, BITS, false>, pl.tiles * pl.parts, WAVES * (rows2 > sums ? rows2 : sums), set2[0]);
+    constexpr size_t operands = FP4 ? Q4::SCRATCH + rows2 : 0;
+    return go(down_kernel<Num, BITS, true>, pl.tiles * pl.parts, WAVES * (operands > sums ? operands : sums), set2[1]);
 }
 
 }  // namespace
@@ -432,6 +689,7 @@ int moe_launch_decode(MoeDecode p, bool fp4, bool f16, void* workspace, hipStrea
     p.counters = (int*)(b + 2 * pl.h_bytes); p.counters_n = pl.tiles;
     p.slots = (float*)(b + 2 * pl.h_bytes + pl.counter_bytes);
     p.parts = pl.parts;
-    if (f16) return fp4 ? launch_typed<NumF16, true>(p, pl, stream) : launch_typed<NumF16, false>(p, pl, stream);
-    return fp4 ? launch_typed<NumBf16, true>(p, pl, stream) : launch_typed<NumBf16, false>(p, pl, stream);
+    p.split = pl.split;
+    if (f16) return fp4 ? launch_typed<NumF16, 4>(p, pl, stream) : launch_typed<NumF16, 16>(p, pl, stream);
+    return fp4 ? launch_typed<NumBf16, 4>(p, pl, stream) : launch_typed<NumBf16, 16>(p, pl, stream);
 }

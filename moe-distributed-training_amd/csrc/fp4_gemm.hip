@@ -30,10 +30,10 @@ __device__ __forceinline__ void store4(void* Y, int64_t at, int dtype, f32x4_t v
 }
 
 // A workgroup: one row tile of 16 MB rows, 16 NB columns; its waves share the contraction and add up their sums in LDS, in wave order.
-template <class Num, int MB, int NB>
+template <class Num, int MB, int NB, bool QUADS>
 __global__ void __launch_bounds__(512) fp4_few_rows_kernel(const MoeFp4Gemm p)
 {
-    typedef few::Fp4Cols<Num, NB> W;
+    typedef typename std::conditional<QUADS, few::Fp4Quads<Num, NB, false>, few::Fp4Cols<Num, NB, false>>::type W;
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const int i = lane & 15, q = lane >> 4;
@@ -43,30 +43,26 @@ __global__ void __launch_bounds__(512) fp4_few_rows_kernel(const MoeFp4Gemm p)
     const int64_t row0 = uniform_i64(t.row0);
     const int nrows = __builtin_amdgcn_readfirstlane((int)(t.row1 - t.row0)), e = __builtin_amdgcn_readfirstlane(t.expert);
     W w;
-    w.two = false;
-    w.codes[0] = few::buffer(p.w.codes + e * p.w.sce);
-    w.scales[0] = few::buffer(p.w.scales + e * p.w.sse);
-    w.left = p.G - q;
     // column i of the wave's block nb is 16 (i >> 2) + 4 nb + (i & 3) with NB = 4: a lane then holds 16 consecutive columns of its row
     const int64_t n0 = (int64_t)cb * (16 * NB);
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-        int64_t n = n0 + (i >> 2) * (4 * NB) + 4 * nb + (i & 3);
-        if (n >= p.N) n = p.N - 1;
-        w.c[nb] = (uint32_t)(n * p.w.scn) + q * FP4_GROUP_BYTES;
-        w.s[nb] = (uint32_t)(n * p.w.ssn) + q;
-    }
+    w.columns(0, p.w, e, p.K, [&](int nb, int c) {
+        const int64_t n = n0 + (c >> 2) * (4 * NB) + 4 * nb + (c & 3);
+        return n < p.N ? n : p.N - 1;
+    });
     few::Rows<MB> rows;
-    rows.K = p.K;
+    rows.left = p.K - 8 * i;
     const int64_t base = p.x_grouped ? row0 : 0;
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) {
-        const int r = mb * 16 + i;
         rows.x[mb] = few::buffer((const uint16_t*)p.X + base * p.ldx);
-        rows.a[mb] = few::RANGE;
-        if (r < nrows) {
-            const int64_t m = row0 + r;
-            rows.a[mb] = (uint32_t)(((p.x_grouped ? m : load_idx(p.pos, m, p.pos64) / p.fan_out) - base) * p.ldx + W::input(0, q)) * 2;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int r = mb * 16 + 4 * j + q;
+            rows.a[mb][j] = few::RANGE;
+            if (r < nrows) {
+                const int64_t m = row0 + r;
+                rows.a[mb][j] = (uint32_t)(((p.x_grouped ? m : load_idx(p.pos, m, p.pos64) / p.fan_out) - base) * p.ldx + 8 * i) * 2;
+            }
         }
     }
     f32x4_t acc[MB][NB];
@@ -74,10 +70,13 @@ __global__ void __launch_bounds__(512) fp4_few_rows_kernel(const MoeFp4Gemm p)
     for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) acc[mb][nb] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-    const int chunks = (p.K + few::CHUNK - 1) / few::CHUNK;
-    few::stream<W, MB, false, MB == 1 ? 4 : 2>(acc, w, rows, chunks * wave / waves, chunks * (wave + 1) / waves);
-    f32x4_t* red = (f32x4_t*)smem;   // [wave][MB * NB][64]
+    constexpr int UNIT = W::UNIT * few::CHUNK, SCRATCH = W::SCRATCH + few::Rows<MB>::SCRATCH;
+    const int units = (p.K + UNIT - 1) / UNIT;
+    few::stream<W, MB, false, 2, 2>(acc, w, rows, units * wave / waves, units * (wave + 1) / waves, smem + wave * SCRATCH);
+    f32x4_t* red = (f32x4_t*)smem;   // [wave][MB * NB][64], in place of the operands
+    static_assert(MB * NB * 1024 <= SCRATCH, "the sums fit where the operands were");
     if (waves > 1) {
+        __syncthreads();
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
@@ -110,9 +109,20 @@ template <class Num, int MB, int NB> int launch_few_typed(MoeFp4Gemm p, int64_t 
     p.col_blocks = (p.N + 16 * NB - 1) / (16 * NB);
     const int64_t most = R / (16 * MB) + p.E, tiles = most < R ? most : R;   // (a tile holds a row at least)
     if (!moe_grid_fits(tiles * p.col_blocks, waves * 64)) return MOE_ERR_UNSUPPORTED;
-    const size_t lds = waves > 1 ? (size_t)waves * MB * NB * 64 * 16 : 0;
-    hipLaunchKernelGGL((fp4_few_rows_kernel<Num, MB, NB>), dim3((unsigned)(tiles * p.col_blocks)), dim3(waves * 64), lds, stream, p);
-    return moe_launch_status();
+    auto go = [&](auto quads) {
+        constexpr bool Q = decltype(quads)::value;
+        const size_t lds = (size_t)waves * (few::Rows<MB>::SCRATCH + (Q ? few::Fp4Quads<Num, NB, false>::SCRATCH : 0));
+        auto kern = fp4_few_rows_kernel<Num, MB, NB, Q>;
+        static std::atomic<bool> attr_set[MOE_MAX_DEVICES];
+        const int dev = moe_current_device();
+        if (!attr_set[dev]) {
+            if (hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != hipSuccess) return MOE_ERR_LAUNCH;
+            attr_set[dev] = true;
+        }
+        hipLaunchKernelGGL(kern, dim3((unsigned)(tiles * p.col_blocks)), dim3(waves * 64), lds, stream, p);
+        return moe_launch_status();
+    };
+    return p.quads ? go(std::true_type{}) : go(std::false_type{});
 }
 
 template <class Num> int launch_few(const MoeFp4Gemm& p, int64_t R, hipStream_t stream)
@@ -133,7 +143,8 @@ template <class Num> int launch_few(const MoeFp4Gemm& p, int64_t R, hipStream_t 
 
 int moe_launch_fp4_gemm(MoeFp4Gemm p, int64_t R, hipStream_t stream)
 {
-    p.G = (int)((p.K + FP4_GROUP - 1) / FP4_GROUP);
+    // (columns of other sizes, and scales at odd addresses, are loaded group by group)
+    p.quads = p.K % (2 * few::CHUNK) == 0 && p.w.ssn % 4 == 0 && p.w.sse % 4 == 0 && (uintptr_t)p.w.scales % 4 == 0;
     p.y_vec = p.ldy % 4 == 0 && (uintptr_t)p.Y % 16 == 0;
     return p.f16 ? launch_few<NumF16>(p, R, stream) : launch_few<NumBf16>(p, R, stream);
 }

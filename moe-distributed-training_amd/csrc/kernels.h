@@ -308,7 +308,7 @@ struct MoeFp4Gemm {
     int E, K; int64_t N;
     int fan_out, x_grouped, y_grouped, f16;
     // set by the launcher
-    int G;                              // groups of a column
+    int quads;                          // weights can be loaded side by side (few_rows.h)
     int64_t col_blocks;
     int y_vec;                          // Y takes stores of four values
 };
@@ -348,7 +348,7 @@ struct MoeDecode {
     int T, E, d, f, k, normalize;
     // set by the launcher
     uint16_t* h; int64_t h_lo;          // (T k, f); what the rounding lost lies h_lo elements further
-    float* slots; int* counters; int counters_n, parts;
+    float* slots; int* counters; int counters_n, parts, split;
 };
 size_t moe_decode_bytes(int T, int E, int d, int f, int k, bool fp4);
 int moe_launch_decode(MoeDecode p, bool fp4, bool f16, void* workspace, hipStream_t stream);
