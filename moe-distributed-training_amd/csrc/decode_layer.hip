@@ -12,6 +12,7 @@
 // many tokens chose its expert; rows of other tokens are computed in launch 1 and not stored, and are absent from launch 2.
 // h travels as two numbers of the activations' type, h and what its rounding lost (16 bits more), whose products are added: the result then carries one rounding, its own.
 #include "few_rows.h"
+#include "gemm_tiles.h"
 #include "kernels.h"
 
 namespace {
@@ -152,13 +153,13 @@ __device__ __forceinline__ void choose(const MoeDecode& p, Chosen& c, const floa
     __syncthreads();
 }
 
-// Logits of all tokens for experts of a block of 16 each, from the waves' sums red[wave][64][4]: a block of `blocks` from eb on is shared by `split` waves.
-__device__ __forceinline__ void sum_logits(const MoeDecode& p, const float* red, float* logits, int eb, int blocks, int split)
+// Logits of all tokens for experts of a block of 16 each, from the waves' sums [64][4], `stride` apart: each of `blocks` blocks from eb on is shared by `split` waves.
+__device__ __forceinline__ void sum_logits(const MoeDecode& p, const float* red, int stride, float* logits, int eb, int blocks, int split)
 {
     for (int x = threadIdx.x; x < blocks * 256; x += THREADS) {
         const int t = x & 15, y = x >> 4 & 15, b = x >> 8, e = (eb + b) * 16 + y;
         double sum = 0;   // (choices between experts are values next to a border)
-        for (int v = 0; v < split; ++v) sum += (double)red[((b * split + v) * 64 + (y >> 2) * 16 + t) * 4 + (y & 3)];
+        for (int v = 0; v < split; ++v) sum += (double)red[(b * split + v) * stride + ((y >> 2) * 16 + t) * 4 + (y & 3)];
         if (e < p.E) logits[t * MAXE + e] = (float)sum;
     }
 }
@@ -195,7 +196,7 @@ template <class Num> __device__ __forceinline__ void route(const MoeDecode& p, C
         few::stream<W, 1, false, 4, 4>(acc, w, rows, chunks * wave / WAVES, chunks * (wave + 1) / WAVES, scratch);
         *(f32x4_t*)(red + (wave * 64 + lane) * 4) = acc[0][0];
         __syncthreads();
-        sum_logits(p, red, logits, eb, 1, WAVES);
+        sum_logits(p, red, 256, logits, eb, 1, WAVES);
         __syncthreads();
     }
     choose(p, c, logits);
@@ -203,7 +204,7 @@ template <class Num> __device__ __forceinline__ void route(const MoeDecode& p, C
 
 // ... and where it is, in the order of W's pieces: the waves of a group of `split` share a block's inputs, groups take different blocks, and the router's rows of the next block are on
 // their way while one is summed.  (Loaded as rows of x are: 16 experts x 256 bytes.)
-template <class W> __device__ __forceinline__ void route_kept(const MoeDecode& p, Chosen& c, float* red, float* logits, const few::Rows<1>::Stage (&xs)[4], uint8_t* scratch)
+template <class W> __device__ __forceinline__ void route_kept(const MoeDecode& p, Chosen& c, float* red, int stride, float* logits, const few::Rows<1>::Stage (&xs)[4], uint8_t* scratch)
 {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, q = lane >> 4;
     const int group = wave / p.split, groups = WAVES / p.split, c0 = (wave & (p.split - 1)) * 4, nblocks = (p.E + 15) / 16;
@@ -228,9 +229,9 @@ template <class W> __device__ __forceinline__ void route_kept(const MoeDecode& p
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc = W::Num::mfma(__builtin_bit_cast(bf16x8_t, f[from][d].f[0][j]), __builtin_bit_cast(bf16x8_t, xs[d].f[0][j]), acc);
         }
-        *(f32x4_t*)(red + (wave * 64 + lane) * 4) = acc;
+        *(f32x4_t*)(red + wave * stride + lane * 4) = acc;
         __syncthreads();
-        sum_logits(p, red, logits, eb0, groups, p.split);
+        sum_logits(p, red, stride, logits, eb0, groups, p.split);
         __syncthreads();
     };
     fetch(0, group);
@@ -276,9 +277,34 @@ template <class Num> __device__ __forceinline__ void store_h(const MoeDecode& p,
     *(uint2*)(h + p.h_lo) = make_uint2(Num::pack2(lo[0], lo[1]), Num::pack2(lo[2], lo[3]));
 }
 
-// KEPT (hidden sizes up to 4096): p.split waves share a job's contraction, four chunks each, so that every job meets a wave with the same chunks of x: they stay in registers, and the
-// ring holds exactly one job: while chunk d of a job is multiplied, chunk d of the next one is requested into its place.  With 8 / p.split jobs at a time.
-// Otherwise all eight waves share a job, chunk by chunk through few::stream.
+// A job's sums [wave][gate, up][64][4] of `split` waves, in wave order; h of the tokens that chose its expert.
+template <class Num, class P> __device__ __forceinline__ void finish_job(const MoeDecode& p, const Chosen& c, const P& place, int job, const float* sums, int split)
+{
+    const int lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
+    if (i >= p.T) return;
+    int e, n;
+    place(job, &e, &n);
+    const int j = choice_of(c, i, e, p.k);
+    if (j < 0) return;
+    f32x4_t g = (f32x4_t){0.f, 0.f, 0.f, 0.f}, u = g;
+    for (int v = 0; v < split; ++v) { g += *(const f32x4_t*)(sums + (v * 128 + lane) * 4); u += *(const f32x4_t*)(sums + (v * 128 + 64 + lane) * 4); }
+    store_h<Num>(p, i * p.k + j, n + 4 * q, g, u);
+}
+
+// what launch 1 leaves for the caller and for launch 2; all threads of the first workgroup
+__device__ __forceinline__ void store_choices(const MoeDecode& p, const Chosen& c)
+{
+    if (blockIdx.x != 0) return;
+    for (int x = threadIdx.x; x < p.T * p.k; x += THREADS) {
+        p.indices[x] = c.idx[x / p.k][x % p.k];
+        p.weights[x] = c.weight[x / p.k][x % p.k];
+    }
+    for (int x = threadIdx.x; x < p.counters_n; x += THREADS) p.counters[x] = 0;
+}
+
+// Launch 1, hidden sizes up to 4096 (KEPT): p.split waves share a job's contraction, four chunks each, so that every job meets a wave with the same chunks of x: they stay in registers,
+// with 8 / p.split jobs at a time.  The ring holds exactly one job (256 KiB of a compute unit): while a chunk of a job is multiplied, that of the next one is on its way into its place.
+// Otherwise all eight waves share a job, through few::stream.
 // a wave's scratch: its rows of x and its weights, or the router's
 template <class W, bool KEPT> constexpr int gate_up_scratch()
 {
@@ -291,10 +317,9 @@ __global__ void __launch_bounds__(THREADS, 2) gate_up_kernel(const MoeDecode p)
 {
     constexpr bool FP4 = BITS == 4;
     typedef typename std::conditional<FP4, typename std::conditional<QUADS, few::Fp4Quads<Num, 2, true>, few::Fp4Cols<Num, 2, true>>::type, few::Cols16<Num, 2>>::type W;
-    static_assert(!KEPT || QUADS || !FP4, "whole chunks");
+    static_assert(!KEPT || !FP4, "4-bit weights: gate_up_fp4_kernel");
     constexpr int SCRATCH = gate_up_scratch<W, KEPT>();
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];   // every wave's scratch
-    constexpr int AHEAD = FP4 ? 2 : 1;   // jobs in the ring: 128 or 256 KiB on their way per compute unit
     __shared__ Chosen c;
     __shared__ __attribute__((aligned(16))) float red[2][WAVES][2][64][4];   // sums of two jobs; before them the router's
     __shared__ float logits[TOK * MAXE];
@@ -309,15 +334,9 @@ __global__ void __launch_bounds__(THREADS, 2) gate_up_kernel(const MoeDecode p)
         for (int d = 0; d < 4; ++d) rows.load(xs[d], c0 + d);
 #pragma unroll
         for (int d = 0; d < 4; ++d) rows.template ready<W>(xs[d], scratch);
-        route_kept<W>(p, c, &red[0][0][0][0][0], logits, xs, scratch);
+        route_kept<W>(p, c, &red[0][0][0][0][0], 256, logits, xs, scratch);
     } else route<Num>(p, c, &red[0][0][0][0][0], logits, scratch);
-    if (blockIdx.x == 0) {
-        for (int x = threadIdx.x; x < p.T * p.k; x += THREADS) {
-            p.indices[x] = c.idx[x / p.k][x % p.k];
-            p.weights[x] = c.weight[x / p.k][x % p.k];
-        }
-        for (int x = threadIdx.x; x < p.counters_n; x += THREADS) p.counters[x] = 0;   // of launch 2
-    }
+    store_choices(p, c);
     const int ncb = p.f / 16, jobs = list_active(c) * ncb;
     auto place = [&](int job, int* e, int* n) {
         *e = __builtin_amdgcn_readfirstlane(c.active[job / ncb]);
@@ -328,89 +347,37 @@ __global__ void __launch_bounds__(THREADS, 2) gate_up_kernel(const MoeDecode p)
         const int step = gridDim.x * at_once, first = blockIdx.x * at_once + wave / split;
         const int rounds = (jobs - (int)blockIdx.x * at_once + step - 1) / step;   // of this workgroup, the same for all of its waves
         W w;
-        bool some = false;
-        constexpr int UNITS = 4 / W::UNIT;
-        typename W::Stage ring[AHEAD][UNITS];
-        fp4_u32x4_t scales[AHEAD][2];   // of the four chunks, 16 bytes: lane l brings those of column l
-        auto turn_to = [&](int job, fp4_u32x4_t (&to)[2]) {   // where a job's weights lie; there may be none
+        typename W::Stage ring[4];
+        auto turn_to = [&](int job) {   // where a job's weights lie; there may be none
             int e = 0, n = 0;
-            some = job < jobs;
-            if (some) place(job, &e, &n);
+            if (job < jobs) place(job, &e, &n);
             gate_up_columns(p, w, e, n);
-            if constexpr (FP4) {
-                const bool mine = some && lane < 16 && (c0 + 4) * few::CHUNK <= p.d;
-#pragma unroll
-                for (int m = 0; m < 2; ++m) to[m] = few::load16(w.scales[m], mine ? w.s[m] : few::RANGE, c0 * 4);
-            } else if (!some) w.left = 0;
+            if (job >= jobs) w.left = 0;
         };
-        auto fetch = [&](typename W::Stage& to, int u) {
-            if constexpr (FP4) {
-                const bool in = some && (c0 + 2 * u) * few::CHUNK < p.d;
+        turn_to(rounds > 0 ? first : jobs);
 #pragma unroll
-                for (int m = 0; m < 2; ++m)
+        for (int d = 0; d < 4; ++d) w.load(ring[d], c0 + d);
+        for (int r = 0; r < rounds; ++r) {
+            const int job = first + r * step;
+            turn_to(r + 1 < rounds ? job + step : jobs);
+            f32x4_t acc[2] = {(f32x4_t){0.f, 0.f, 0.f, 0.f}, (f32x4_t){0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) to.c[m][h] = few::load16_streamed(w.codes[m], in ? w.c[m][h] : few::RANGE, (c0 / 2 + u) * 128);
-            } else w.load(to, c0 + u);
-        };
+            for (int d = 0; d < 4; ++d) {
+                w.ready(ring[d], scratch);
 #pragma unroll
-        for (int a = 0; a < AHEAD; ++a) {
-            turn_to(a < rounds ? first + a * step : jobs, scales[a]);
+                for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int u = 0; u < UNITS; ++u) fetch(ring[a][u], u);
-        }
-        for (int r0 = 0; r0 < rounds; r0 += AHEAD)
-#pragma unroll
-            for (int a = 0; a < AHEAD; ++a) {
-                const int r = r0 + a;
-                if (AHEAD > 1 && r >= rounds) break;
-                const int job = first + r * step;
-                fp4_u32x4_t now[2];   // scales of column lane & 15: byte q of word d
-                if constexpr (FP4) {
-#pragma unroll
-                    for (int m = 0; m < 2; ++m)
-                        if (lane < 16) *(fp4_u32x4_t*)(scratch + (m * 16 + lane) * 16) = scales[a][m];
-#pragma unroll
-                    for (int m = 0; m < 2; ++m) now[m] = *(const fp4_u32x4_t*)(scratch + (m * 16 + i) * 16);
-                }
-                turn_to(r + AHEAD < rounds ? job + AHEAD * step : jobs, scales[a]);
-                f32x4_t acc[2] = {(f32x4_t){0.f, 0.f, 0.f, 0.f}, (f32x4_t){0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-                for (int v = 0; v < UNITS; ++v) {
-                    if constexpr (FP4) {
-#pragma unroll
-                        for (int m = 0; m < 2; ++m) few::from_lines(ring[a][v].c[m], scratch + m * 2048);
-                    } else w.ready(ring[a][v], scratch);
-#pragma unroll
-                    for (int cc = 0; cc < W::UNIT; ++cc)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-#pragma unroll
-                            for (int m = 0; m < 2; ++m) {
-                                const int d = v * W::UNIT + cc;
-                                bf16x8_t f;
-                                if constexpr (FP4) f = fp4_expand8<Num>(ring[a][v].c[m][cc][j], fp4_scale(now[m][d] >> (8 * q) & 0xff));
-                                else f = W::frag(ring[a][v], cc, m, j);
-                                acc[m] = Num::mfma(f, __builtin_bit_cast(bf16x8_t, xs[d].f[0][j]), acc[m]);
-                            }
-                    __builtin_amdgcn_sched_barrier(0);   // (as in few::stream)
-                    fetch(ring[a][v], v);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-                float (*s)[2][64][4] = red[r & 1];   // (the other one may still be read)
-                *(f32x4_t*)s[wave][0][lane] = acc[0];
-                *(f32x4_t*)s[wave][1][lane] = acc[1];
-                __syncthreads();
-                if (member == (r & (split - 1)) && job < jobs && i < p.T) {
-                    int e, n;
-                    place(job, &e, &n);
-                    const int j = choice_of(c, i, e, p.k);
-                    if (j >= 0) {
-                        f32x4_t g = (f32x4_t){0.f, 0.f, 0.f, 0.f}, u = g;
-                        for (int v = wave - member; v < wave - member + split; ++v) { g += *(const f32x4_t*)s[v][0][lane]; u += *(const f32x4_t*)s[v][1][lane]; }
-                        store_h<Num>(p, i * p.k + j, n + 4 * q, g, u);
-                    }
-                }
+                    for (int m = 0; m < 2; ++m) acc[m] = Num::mfma(W::frag(ring[d], 0, m, j), __builtin_bit_cast(bf16x8_t, xs[d].f[0][j]), acc[m]);
+                __builtin_amdgcn_sched_barrier(0);   // (as in few::stream)
+                w.load(ring[d], c0 + d);
+                __builtin_amdgcn_sched_barrier(0);
             }
+            float (*s)[2][64][4] = red[r & 1];   // (the other one may still be read)
+            *(f32x4_t*)s[wave][0][lane] = acc[0];
+            *(f32x4_t*)s[wave][1][lane] = acc[1];
+            __syncthreads();
+            if (member == (r & (split - 1)) && job < jobs) finish_job<Num>(p, c, place, job, &s[wave - member][0][0][0], split);
+        }
     } else {
         constexpr int UNIT = W::UNIT * few::CHUNK;
         const int units = (p.d + UNIT - 1) / UNIT;
@@ -426,17 +393,122 @@ __global__ void __launch_bounds__(THREADS, 2) gate_up_kernel(const MoeDecode p)
             *(f32x4_t*)s[wave][0][lane] = acc[0][0];
             *(f32x4_t*)s[wave][1][lane] = acc[0][1];
             __syncthreads();
-            if (wave == (turn & (WAVES - 1)) && i < p.T) {
-                const int j = choice_of(c, i, e, p.k);
-                if (j >= 0) {
-                    f32x4_t g = (f32x4_t){0.f, 0.f, 0.f, 0.f}, u = g;
-#pragma unroll
-                    for (int v = 0; v < WAVES; ++v) { g += *(const f32x4_t*)s[v][0][lane]; u += *(const f32x4_t*)s[v][1][lane]; }
-                    store_h<Num>(p, i * p.k + j, n + 4 * q, g, u);
-                }
-            }
+            if (wave == (turn & (WAVES - 1))) finish_job<Num>(p, c, place, job, &s[0][0][0][0], WAVES);
         }
     }
+}
+
+// Launch 1 over 4-bit weights, hidden sizes up to 4096 that are multiples of 512: as KEPT above, but codes go straight into LDS, a ring of four units (256 inputs of 16 columns of both
+// projections, 4 KiB) per wave, two jobs: a job is only 64 KiB of a compute unit, and with one of them in registers the loop waited for memory (4 us a job).  Requests are counted by
+// hand: a job is the scales of gate and up and two units of four loads; scales and a unit are awaited with what was requested behind them still on its way.
+constexpr int FP4_UNIT_LDS = 4096, FP4_SCALES_LDS = 512, FP4_WAVE_LDS = 4 * FP4_UNIT_LDS + 2 * FP4_SCALES_LDS, FP4_LDS = WAVES * FP4_WAVE_LDS + WAVES * 2 * 1024;
+
+template <int N> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+
+template <class Num>
+__global__ void __launch_bounds__(THREADS, 2) gate_up_fp4_kernel(const MoeDecode p)
+{
+    typedef few::Fp4Quads<Num, 2, true> W;
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];   // every wave's ring and scales, and the sums of a job [wave][gate, up][64][4]
+    __shared__ Chosen c;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, q = lane >> 4;
+    float* red = (float*)(smem + WAVES * FP4_WAVE_LDS);
+    uint8_t* area = smem + wave * FP4_WAVE_LDS;
+    if (threadIdx.x < MAXE / 32) c.used[threadIdx.x] = 0;   // (the router's barriers lie in between)
+    const int split = p.split, member = wave & (split - 1), c0 = member * 4;
+    const few::Rows<1> rows = token_rows(p, p.x, p.ldx, p.d);
+    few::Rows<1>::Stage xs[4];
+#pragma unroll
+    for (int d = 0; d < 4; ++d) rows.load(xs[d], c0 + d);
+#pragma unroll
+    for (int d = 0; d < 4; ++d) rows.template ready<W>(xs[d], area);
+    // (the router's sums lie behind every wave's scratch, its logits where a job's sums will be)
+    static_assert(TOK * MAXE * 4 <= WAVES * 2 * 1024 && few::Rows<1>::SCRATCH + 1024 <= FP4_WAVE_LDS, "");
+    route_kept<W>(p, c, (float*)(smem + few::Rows<1>::SCRATCH), FP4_WAVE_LDS / 4, red, xs, area);
+    store_choices(p, c);
+    const int ncb = p.f / 16, jobs = list_active(c) * ncb;
+    auto place = [&](int job, int* e, int* n) {
+        *e = __builtin_amdgcn_readfirstlane(c.active[job / ncb]);
+        *n = __builtin_amdgcn_readfirstlane(job % ncb) * 16;
+    };
+    const int at_once = WAVES / split, step = gridDim.x * at_once, first = blockIdx.x * at_once + wave / split;
+    const int rounds = (jobs - (int)blockIdx.x * at_once + step - 1) / step;   // of this workgroup, the same for all of its waves
+    // where a job's weights lie (there may be none: requests outside the buffer's range)
+    i32x4_t codes[2], scales[2];
+    uint32_t col[2], scale_at = few::RANGE;   // of the two halves of a block's columns, from the job's first one
+    const uint32_t area_u = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)LDS_PTR(area));
+    auto turn_to = [&](int job) {
+        const bool some = job < jobs && c0 * few::CHUNK < p.d;
+        int e = 0, n = 0;
+        if (job < jobs) place(job, &e, &n);
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            const MoeFp4Weights& f = m ? p.f3 : p.f1;
+            codes[m] = make_buffer(f.codes + e * f.sce + n * f.scn, few::RANGE);
+            scales[m] = make_buffer(f.scales + e * f.sse + n * f.ssn, few::RANGE);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) col[h] = some ? (uint32_t)((8 * h + (lane >> 3)) * p.f1.scn) + few::line_piece(lane, h) * 16 : few::RANGE;   // (w1 and w3 have the same pitch)
+        scale_at = some ? (uint32_t)(lane * p.f1.ssn) : few::RANGE;
+    };
+    auto fetch_scales = [&](int slot) {
+        if (lane < 16)
+#pragma unroll
+            for (int m = 0; m < 2; ++m) load_to_lds_16(scales[m], scale_at, c0 * 4, area_u + 4 * FP4_UNIT_LDS + slot * FP4_SCALES_LDS + m * 256);
+    };
+    auto fetch = [&](int slot, int u) {
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) load_to_lds_16<true>(codes[m], col[h], (c0 / 2 + u) * 128, area_u + (slot * 2 + u) * FP4_UNIT_LDS + m * 2048 + h * 1024);
+    };
+    constexpr int UNIT_LOADS = 4, JOB_LOADS = 2 + 2 * UNIT_LOADS;
+#pragma unroll 1
+    for (int r = 0; r < 2; ++r) {
+        turn_to(r < rounds ? first + r * step : jobs);
+        fetch_scales(r);
+        fetch(r, 0);
+        fetch(r, 1);
+    }
+#pragma unroll 1
+    for (int r = 0; r < rounds; ++r) {
+        const int job = first + r * step, slot = r & 1;
+        turn_to(r + 2 < rounds ? job + 2 * step : jobs);
+        f32x4_t acc[2] = {(f32x4_t){0.f, 0.f, 0.f, 0.f}, (f32x4_t){0.f, 0.f, 0.f, 0.f}};
+        fp4_u32x4_t now[2];   // scales of column i: byte q of word d
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            if (u == 0) {
+                wait_loads<UNIT_LOADS + JOB_LOADS>();
+#pragma unroll
+                for (int m = 0; m < 2; ++m) now[m] = *(const fp4_u32x4_t*)(area + 4 * FP4_UNIT_LDS + slot * FP4_SCALES_LDS + m * 256 + i * 16);
+            } else wait_loads<JOB_LOADS + 2 + UNIT_LOADS>();
+            fp4_u32x4_t f[2][2];
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int cc = 0; cc < 2; ++cc) f[m][cc] = *(const fp4_u32x4_t*)(area + (slot * 2 + u) * FP4_UNIT_LDS + m * 2048 + i * 128 + ((cc * 4 + q) ^ ((i >> 1) & 7)) * 16);
+#pragma unroll
+            for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int m = 0; m < 2; ++m)
+                        acc[m] = Num::mfma(fp4_expand8<Num>(f[m][cc][j], fp4_scale(now[m][2 * u + cc] >> (8 * q) & 0xff)), __builtin_bit_cast(bf16x8_t, xs[2 * u + cc].f[0][j]), acc[m]);
+            // every read of this unit's place has come back: the job after the next goes there
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
+            if (u == 0) fetch_scales(slot);
+            fetch(slot, u);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        __syncthreads();   // the sums of the job before have been read
+        *(f32x4_t*)(red + (wave * 128 + lane) * 4) = acc[0];
+        *(f32x4_t*)(red + (wave * 128 + 64 + lane) * 4) = acc[1];
+        __syncthreads();
+        if (member == (r & (split - 1)) && job < jobs) finish_job<Num>(p, c, place, job, red + (wave - member) * 512, split);
+    }
+    wait_loads<0>();   // (nothing lands in LDS that is no longer this workgroup's)
 }
 
 // ---- launch 2
@@ -664,9 +736,14 @@ template <class Num, int BITS> int launch_typed(const MoeDecode& p, const Plan& 
     typedef few::Fp4Quads<Num, 4, false> Q4;
     constexpr size_t rows2 = few::Rows<2>::SCRATCH, sums = (size_t)4 * 64 * (FP4 ? 4 : 8) * 4;
     int rc;
-    if (p.split) rc = go(gate_up_kernel<Num, BITS, true, true>, pl.grid1, WAVES * gate_up_scratch<Q2, true>(), set1[0]);
-    else if (FP4 && p.d % (2 * few::CHUNK)) rc = go(gate_up_kernel<Num, BITS, false, false>, pl.grid1, WAVES * gate_up_scratch<few::Fp4Cols<Num, 2, true>, false>(), set1[1]);
-    else rc = go(gate_up_kernel<Num, BITS, false, true>, pl.grid1, WAVES * (FP4 ? gate_up_scratch<Q2, false>() : gate_up_scratch<few::Cols16<Num, 2>, false>()), set1[2]);
+    if constexpr (FP4) {
+        if (p.split) rc = go(gate_up_fp4_kernel<Num>, pl.grid1, FP4_LDS, set1[0]);
+        else if (p.d % (2 * few::CHUNK)) rc = go(gate_up_kernel<Num, 4, false, false>, pl.grid1, WAVES * gate_up_scratch<few::Fp4Cols<Num, 2, true>, false>(), set1[1]);
+        else rc = go(gate_up_kernel<Num, 4, false, true>, pl.grid1, WAVES * gate_up_scratch<Q2, false>(), set1[2]);
+    } else {
+        if (p.split) rc = go(gate_up_kernel<Num, 16, true, true>, pl.grid1, WAVES * gate_up_scratch<few::Cols16<Num, 2>, true>(), set1[0]);
+        else rc = go(gate_up_kernel<Num, 16, false, true>, pl.grid1, WAVES * gate_up_scratch<few::Cols16<Num, 2>, false>(), set1[1]);
+    }
     if (rc != MOE_OK) return rc;
     if (FP4 && p.f % (2 * few::CHUNK)) return go(down_kernel<Num, BITS, false>, pl.tiles * pl.parts, WAVES * (rows2 > sums ? rows2 : sums), set2[0]);
     constexpr size_t operands = FP4 ? Q4::SCRATCH + rows2 : 0;
