@@ -16,14 +16,43 @@ inline size_t elem_bytes(int dtype) { return dtype == MOE_F32 ? 4 : 2; }
 // rows of codes that 16-byte loads take, and scales that lie one after the other
 bool weights_ok(const MoeFp4Weights& w) { return w.codes && w.scales && aligned16(w.codes) && w.sce % 16 == 0 && w.scn % 16 == 0; }
 
-// rows that 16-byte loads take as they are; otherwise they are packed
-bool rows_ok(const void* x, int64_t ldx, int64_t x_rows, int64_t K, int x_grouped)
+// rows that 16-byte loads take as they are, within their offsets; otherwise they are packed in the order of the product
+bool rows_ok(const void* x, int64_t ldx, int64_t x_rows, int64_t cols, int x_grouped)
 {
-    return aligned16(x) && ldx % 8 == 0 && K % 8 == 0 && ((x_grouped ? 128 : x_rows) * ldx + K) * 2 < MOE_FP4_RANGE;
+    return aligned16(x) && ldx % 8 == 0 && cols % 8 == 0 && ((x_grouped ? 128 : x_rows) * ldx + cols) * 2 < MOE_FP4_RANGE;
 }
-int64_t packed_cols(int64_t K) { return (K + 7) / 8 * 8; }
-size_t packed_bytes(int64_t R, int64_t K) { return al((size_t)R * (size_t)packed_cols(K) * 2); }
+int64_t packed_cols(int64_t n) { return (n + 7) / 8 * 8; }
+// scales that 4-byte loads take as they are; otherwise rows of whole fours are made of them
+bool scales_ok(const uint8_t* scales, int64_t sse, int64_t ssn, int64_t G) { return (uintptr_t)scales % 4 == 0 && sse % 4 == 0 && ssn % 4 == 0 && G % 4 == 0; }
+int64_t packed_groups(int64_t G) { return (G + 3) / 4 * 4; }
 size_t expanded_bytes(int E, int64_t K, int64_t N, int dtype) { return al((size_t)E * (size_t)N * (size_t)K * elem_bytes(dtype)); }
+
+// What a 16-bit product copies into its workspace before it starts: rows (len columns) and scales.
+struct Fp4Copies {
+    size_t rows, scales;
+    Fp4Copies(const void* x, int64_t ldx, int64_t x_rows, int x_grouped, const uint8_t* s, int64_t sse, int64_t ssn, int64_t R, int E, int64_t K, int64_t N, int64_t len)
+        : rows(rows_ok(x, ldx, x_rows, len, x_grouped) ? 0 : al((size_t)R * (size_t)packed_cols(len) * 2)),
+          scales(scales_ok(s, sse, ssn, groups_of(K)) ? 0 : al((size_t)E * (size_t)N * (size_t)packed_groups(groups_of(K)))) {}
+    // makes them, and has g read them; len becomes whole pieces of rows
+    int make(MoeFp4Gemm& g, int64_t R, int64_t len, uint8_t* ws, hipStream_t st) const
+    {
+        if (rows) {
+            const int64_t ld = packed_cols(len);
+            TRY(moe_launch_fp4_pack_rows(g.X, g.ldx, g.x_grouped ? nullptr : g.pos, g.pos64, g.fan_out, g.offsets, g.off64, g.E, R, len, ws, ld, st));
+            g.X = ws; g.ldx = ld; g.x_grouped = 1;
+        }
+        if (scales) {
+            const int64_t G = groups_of(g.K), ld = packed_groups(G);
+            TRY(moe_launch_fp4_pack_scales(g.w.scales, g.w.sse, g.w.ssn, g.E, g.N, G, ws + rows, ld, st));
+            g.w.scales = ws + rows; g.w.ssn = ld; g.w.sse = g.N * ld;
+        }
+        return MOE_OK;
+    }
+};
+bool fp4_sizes_ok(int64_t K, int64_t N, int E, int64_t scn, int64_t ssn)
+{
+    return K <= 0x3fffff && E <= 65535 && N * scn < MOE_FP4_RANGE && N * ssn < MOE_FP4_RANGE && N * packed_groups(groups_of(K)) < MOE_FP4_RANGE && packed_cols(N) * 256 < MOE_FP4_RANGE;
+}
 
 struct Kept { size_t codes, scales; };
 Kept kept_sizes(int64_t rows, int64_t cols)
@@ -78,11 +107,13 @@ int moe_fp4_quantize_weights(const void* W, int64_t swe, int64_t swk, int64_t sw
     return moe_launch_fp4_quantize(W, swe, swk, swn, dtype, E, K, N, codes, sce, scn, scales, sse, ssn, S(stream));
 }
 
-size_t moe_linear_fp4_workspace_bytes(const void* x, int64_t ldx, int64_t x_rows, int x_grouped, int dtype, int64_t R, int E, int64_t K, int64_t N)
+size_t moe_linear_fp4_workspace_bytes(const void* x, int64_t ldx, int64_t x_rows, int x_grouped, int dtype, const uint8_t* scales, int64_t sse, int64_t ssn, int64_t R, int E, int64_t K,
+                                      int64_t N)
 {
     if (dtype < 0 || dtype > 2 || R < 1 || E < 1 || K < 1 || N < 1) return 0;
-    if (dtype != MOE_F32) return rows_ok(x, ldx, x_rows, K, x_grouped) ? 0 : packed_bytes(R, K);
-    return expanded_bytes(E, K, N, dtype) + moe_scatter2scatter_workspace_bytes(R, E, K, N, 0);
+    if (dtype == MOE_F32) return expanded_bytes(E, K, N, dtype) + moe_scatter2scatter_workspace_bytes(R, E, K, N, 0);
+    const Fp4Copies c(x, ldx, x_rows, x_grouped, scales, sse, ssn, R, E, K, N, K);
+    return c.rows + c.scales;
 }
 
 int moe_linear_fp4_fwd(const void* x, int64_t ldx, int64_t x_rows, int dtype, const uint8_t* codes, int64_t sce, int64_t scn, const uint8_t* scales, int64_t sse, int64_t ssn, void* y,
@@ -94,10 +125,8 @@ int moe_linear_fp4_fwd(const void* x, int64_t ldx, int64_t x_rows, int dtype, co
     if (ldx < 0 || (R > 1 && ldy < N)) return MOE_ERR_BAD_ARG;   // (rows of an input may overlap)
     const MoeFp4Weights w = {codes, sce, scn, scales, sse, ssn};
     if (!x || x_rows < 1 || !weights_ok(w) || !y || !offsets || ((!x_grouped || !y_grouped) && !pos) || (x_grouped && x_rows < R) || !aligned16(workspace)) return MOE_ERR_BAD_ARG;
-    const size_t need = moe_linear_fp4_workspace_bytes(x, ldx, x_rows, x_grouped, dtype, R, E, K, N);
+    const size_t need = moe_linear_fp4_workspace_bytes(x, ldx, x_rows, x_grouped, dtype, scales, sse, ssn, R, E, K, N);
     if (need && (!workspace || workspace_bytes < need)) return MOE_ERR_WORKSPACE;
-    if (K > 0x3fffffff || E > 65535) return MOE_ERR_UNSUPPORTED;
-    if (dtype != MOE_F32 && (N * scn >= MOE_FP4_RANGE || N * ssn >= MOE_FP4_RANGE || packed_cols(K) * 256 >= MOE_FP4_RANGE)) return MOE_ERR_UNSUPPORTED;
     if (dtype == MOE_F32) {
         if (y_dtype != MOE_F32) return MOE_ERR_UNSUPPORTED;
         const size_t wb = expanded_bytes(E, K, N, dtype);
@@ -105,36 +134,60 @@ int moe_linear_fp4_fwd(const void* x, int64_t ldx, int64_t x_rows, int dtype, co
         return moe_scatter2scatter(x, ldx, 1, workspace, N * K, 1, K, nullptr, 0, 0, 0, nullptr, 0, 0, 0, 0, 0.f, y, ldy, 1, pos, pos64, offsets, off64, E, R, K, N, fan_out, x_grouped,
                                    y_grouped, dtype, (uint8_t*)workspace + wb, workspace_bytes - wb, stream);
     }
+    if (!fp4_sizes_ok(K, N, E, scn, ssn)) return MOE_ERR_UNSUPPORTED;
     MoeFp4Gemm g = {};
     g.X = x; g.ldx = ldx; g.w = w; g.Y = y; g.ldy = ldy; g.ydtype = y_dtype; g.pos = pos; g.pos64 = pos64; g.offsets = offsets; g.off64 = off64;
     g.E = E; g.K = (int)K; g.N = N; g.fan_out = fan_out; g.x_grouped = x_grouped; g.y_grouped = y_grouped; g.f16 = dtype == MOE_F16;
-    if (need) {   // rows in the order of the product, padded
-        const int64_t ld = packed_cols(K);
-        TRY(moe_launch_fp4_pack_rows(x, ldx, x_grouped ? nullptr : pos, pos64, fan_out, offsets, off64, E, R, K, workspace, ld, S(stream)));
-        g.X = workspace; g.ldx = ld; g.K = (int)ld; g.x_grouped = 1;
-    }
-    return moe_launch_fp4_gemm(g, R, S(stream));
+    const Fp4Copies c(x, ldx, x_rows, x_grouped, scales, sse, ssn, R, E, K, N, K);
+    TRY(c.make(g, R, K, (uint8_t*)workspace, S(stream)));
+    if (c.rows) g.K = (int)packed_cols(K);   // (the same groups of weights; the rows have zeros there)
+    return R <= 16 * (int64_t)E ? moe_launch_fp4_few_rows(g, R, S(stream)) : moe_launch_fp4_tiles(g, R, false, S(stream));
 }
 
-size_t moe_linear_fp4_bwd_workspace_bytes(int dtype, int64_t R, int E, int64_t K, int64_t N)
+size_t moe_linear_fp4_bwd_workspace_bytes(const void* dy, int64_t lddy, int64_t dy_rows, int dy_grouped, int weighted, int dtype, const uint8_t* scales, int64_t sse, int64_t ssn, int64_t R,
+                                          int E, int64_t K, int64_t N)
 {
     if (dtype < 0 || dtype > 2 || R < 1 || E < 1 || K < 1 || N < 1) return 0;
-    return expanded_bytes(E, K, N, dtype) + moe_scatter2scatter_workspace_bytes(R, E, N, K, 0);
+    if (dtype == MOE_F32)
+        return expanded_bytes(E, K, N, dtype) + (dy_grouped && !weighted ? 0 : al((size_t)R * (size_t)N * 4)) + moe_scatter2scatter_workspace_bytes(R, E, N, K, 0);
+    const Fp4Copies c(dy, lddy, dy_rows, dy_grouped, scales, sse, ssn, R, E, K, N, N);
+    return c.rows + c.scales;
 }
 
-int moe_linear_fp4_bwd(const void* dy, int64_t lddy, int dtype, const uint8_t* codes, int64_t sce, int64_t scn, const uint8_t* scales, int64_t sse, int64_t ssn, void* dx_rows,
-                       int64_t lddx, int dx_grouped, const void* pos, int pos64, const void* offsets, int off64, int E, int64_t R, int64_t K, int64_t N, void* workspace,
-                       size_t workspace_bytes, void* stream)
+int moe_linear_fp4_bwd(const void* dy, int64_t lddy, int64_t dy_rows, int dtype, int dy_grouped, int dy_fan_out, const void* gates, int gates_dtype, const uint8_t* codes, int64_t sce,
+                       int64_t scn, const uint8_t* scales, int64_t sse, int64_t ssn, void* dx_rows, int64_t lddx, int dx_dtype, int dx_grouped, const void* pos, int pos64, const void* offsets,
+                       int off64, int E, int64_t R, int64_t K, int64_t N, void* workspace, size_t workspace_bytes, void* stream)
 {
-    if (dtype < 0 || dtype > 2 || E < 1 || R < 0 || K < 1 || N < 1) return MOE_ERR_BAD_ARG;
+    if (dtype < 0 || dtype > 2 || dx_dtype < 0 || dx_dtype > 2 || E < 1 || R < 0 || dy_rows < 0 || K < 1 || N < 1 || dy_fan_out < 1 || (gates && (gates_dtype < 0 || gates_dtype > 2 || dy_grouped))) return MOE_ERR_BAD_ARG;
     if (R == 0) return MOE_OK;
     const MoeFp4Weights w = {codes, sce, scn, scales, sse, ssn};
-    if (lddy < 0 || (R > 1 && lddx < K) || !dy || !weights_ok(w) || !dx_rows || !offsets || (!dx_grouped && !pos) || !aligned16(workspace)) return MOE_ERR_BAD_ARG;
-    const size_t need = moe_linear_fp4_bwd_workspace_bytes(dtype, R, E, K, N), wb = expanded_bytes(E, K, N, dtype);
-    if (!workspace || workspace_bytes < need) return MOE_ERR_WORKSPACE;
-    TRY(moe_launch_fp4_expand(codes, sce, scn, scales, sse, ssn, E, K, N, workspace, dtype, S(stream)));
-    return moe_scatter2scatter(dy, lddy, 1, workspace, N * K, K, 1, nullptr, 0, 0, 0, nullptr, 0, 0, 0, 0, 0.f, dx_rows, lddx, 1, pos, pos64, offsets, off64, E, R, N, K, 1, 1,
-                               dx_grouped, dtype, (uint8_t*)workspace + wb, workspace_bytes - wb, stream);
+    if (lddy < 0 || (R > 1 && lddx < K) || !dy || dy_rows < 1 || !weights_ok(w) || !dx_rows || !offsets || ((!dy_grouped || !dx_grouped) && !pos) || (dy_grouped && dy_rows < R) ||
+        !aligned16(workspace)) return MOE_ERR_BAD_ARG;
+    const size_t need = moe_linear_fp4_bwd_workspace_bytes(dy, lddy, dy_rows, dy_grouped, gates != nullptr, dtype, scales, sse, ssn, R, E, K, N);
+    if (need && (!workspace || workspace_bytes < need)) return MOE_ERR_WORKSPACE;
+    if (dtype == MOE_F32) {
+        if (dx_dtype != MOE_F32) return MOE_ERR_UNSUPPORTED;
+        size_t used = expanded_bytes(E, K, N, dtype);
+        TRY(moe_launch_fp4_expand(codes, sce, scn, scales, sse, ssn, E, K, N, workspace, dtype, S(stream)));
+        const void* rows = dy;
+        int64_t ld = lddy;
+        if (!dy_grouped) {
+            rows = (uint8_t*)workspace + used;
+            ld = N;
+            used += al((size_t)R * (size_t)N * 4);
+            TRY(moe_group_rows(dy, lddy, (void*)rows, N, pos, pos64, dy_fan_out, gates, gates_dtype, R, N, dtype, stream));
+        }
+        return moe_scatter2scatter(rows, ld, 1, workspace, N * K, K, 1, nullptr, 0, 0, 0, nullptr, 0, 0, 0, 0, 0.f, dx_rows, lddx, 1, pos, pos64, offsets, off64, E, R, N, K, 1, 1,
+                                   dx_grouped, dtype, (uint8_t*)workspace + used, workspace_bytes - used, stream);
+    }
+    if (!fp4_sizes_ok(K, N, E, scn, ssn)) return MOE_ERR_UNSUPPORTED;
+    MoeFp4Gemm g = {};
+    g.X = dy; g.ldx = lddy; g.w = w; g.Y = dx_rows; g.ldy = lddx; g.ydtype = dx_dtype; g.pos = pos; g.pos64 = pos64; g.offsets = offsets; g.off64 = off64;
+    g.E = E; g.K = (int)K; g.N = N; g.fan_out = dy_fan_out; g.x_grouped = dy_grouped; g.y_grouped = dx_grouped; g.f16 = dtype == MOE_F16;
+    g.gates = gates; g.gates_dtype = gates_dtype;
+    const Fp4Copies c(dy, lddy, dy_rows, dy_grouped, scales, sse, ssn, R, E, K, N, N);
+    TRY(c.make(g, R, N, (uint8_t*)workspace, S(stream)));
+    return moe_launch_fp4_tiles(g, R, true, S(stream));
 }
 
 size_t moe_swiglu8_kept_bytes(int64_t rows, int64_t cols) { return rows < 1 || cols < 1 ? 0 : kept_bytes(rows, cols); }

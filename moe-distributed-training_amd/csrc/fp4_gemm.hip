@@ -1,8 +1,6 @@
-// Grouped product of 16-bit rows with 4-bit weights (fp4.h) over ragged expert groups:
+// Grouped product of 16-bit rows with 4-bit weights (fp4.h) over ragged expert groups, few rows per expert: the codes are streamed (few_rows.h).
 //
 //   Y[out_row(m)][n] = sum_k X[in_row(m)][k] W[e(m)][n][k]
-//
-// Few rows per expert: fp4_few_rows_kernel, which streams the codes (few_rows.h).
 #include "few_rows.h"
 #include "kernels.h"
 
@@ -29,10 +27,11 @@ __device__ __forceinline__ void store4(void* Y, int64_t at, int dtype, f32x4_t v
         if (i < live) y[i] = (uint16_t)((i < 2 ? o.x : o.y) >> (16 * (i & 1)));
 }
 
-// A workgroup: one row tile of 16 MB rows, 16 NB columns; its waves share the contraction and add up their sums in LDS, in wave order.
-template <class Num, int MB, int NB, bool QUADS>
+// A workgroup: one row tile of 16 rows, 16 NB columns; its waves share the contraction and add up their sums in LDS, in wave order.
+template <class Num, int NB, bool QUADS>
 __global__ void __launch_bounds__(512) fp4_few_rows_kernel(const MoeFp4Gemm p)
 {
+    constexpr int MB = 1;
     typedef typename std::conditional<QUADS, few::Fp4Quads<Num, NB, false>, few::Fp4Cols<Num, NB, false>>::type W;
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
@@ -104,15 +103,14 @@ __global__ void __launch_bounds__(512) fp4_few_rows_kernel(const MoeFp4Gemm p)
     }
 }
 
-template <class Num, int MB, int NB> int launch_few_typed(MoeFp4Gemm p, int64_t R, int waves, hipStream_t stream)
+template <class Num, int NB> int launch_few_typed(MoeFp4Gemm p, int64_t tiles, int waves, hipStream_t stream)
 {
     p.col_blocks = (p.N + 16 * NB - 1) / (16 * NB);
-    const int64_t most = R / (16 * MB) + p.E, tiles = most < R ? most : R;   // (a tile holds a row at least)
     if (!moe_grid_fits(tiles * p.col_blocks, waves * 64)) return MOE_ERR_UNSUPPORTED;
     auto go = [&](auto quads) {
         constexpr bool Q = decltype(quads)::value;
-        const size_t lds = (size_t)waves * (few::Rows<MB>::SCRATCH + (Q ? few::Fp4Quads<Num, NB, false>::SCRATCH : 0));
-        auto kern = fp4_few_rows_kernel<Num, MB, NB, Q>;
+        const size_t lds = (size_t)waves * (few::Rows<1>::SCRATCH + (Q ? few::Fp4Quads<Num, NB, false>::SCRATCH : 0));
+        auto kern = fp4_few_rows_kernel<Num, NB, Q>;
         static std::atomic<bool> attr_set[MOE_MAX_DEVICES];
         const int dev = moe_current_device();
         if (!attr_set[dev]) {
@@ -127,24 +125,21 @@ template <class Num, int MB, int NB> int launch_few_typed(MoeFp4Gemm p, int64_t 
 
 template <class Num> int launch_few(const MoeFp4Gemm& p, int64_t R, hipStream_t stream)
 {
-    const int MB = R <= 16 * (int64_t)p.E ? 1 : 2;
-    const int64_t tiles = R / (16 * MB) + p.E < R ? R / (16 * MB) + p.E : R;
+    const int64_t most = R / 16 + p.E, tiles = most < R ? most : R;   // (a tile holds a row at least)
     const int chunks = (p.K + few::CHUNK - 1) / few::CHUNK, cus = moe_device_cus();
     // waves that share a contraction: as many as it has pairs of chunks, until the chip has twelve waves per compute unit
     const bool narrow = tiles * ((p.N + 63) / 64) < cus;   // few column blocks: blocks of 16 columns give every compute unit one
     const int64_t groups = tiles * (narrow ? (p.N + 15) / 16 : (p.N + 63) / 64);
     int waves = 1;
     while (waves < 8 && groups * waves < 12 * (int64_t)cus && chunks >= 2 * waves) waves *= 2;
-    if (MB == 1) return narrow ? launch_few_typed<Num, 1, 1>(p, R, waves, stream) : launch_few_typed<Num, 1, 4>(p, R, waves, stream);
-    return narrow ? launch_few_typed<Num, 2, 1>(p, R, waves, stream) : launch_few_typed<Num, 2, 4>(p, R, waves, stream);
+    return narrow ? launch_few_typed<Num, 1>(p, tiles, waves, stream) : launch_few_typed<Num, 4>(p, tiles, waves, stream);
 }
 
 }  // namespace
 
-int moe_launch_fp4_gemm(MoeFp4Gemm p, int64_t R, hipStream_t stream)
+int moe_launch_fp4_few_rows(MoeFp4Gemm p, int64_t R, hipStream_t stream)
 {
-    // (columns of other sizes, and scales at odd addresses, are loaded group by group)
-    p.quads = p.K % (2 * few::CHUNK) == 0 && p.w.ssn % 4 == 0 && p.w.sse % 4 == 0 && (uintptr_t)p.w.scales % 4 == 0;
+    p.quads = p.K % (2 * few::CHUNK) == 0;   // (columns of other sizes are loaded group by group)
     p.y_vec = p.ldy % 4 == 0 && (uintptr_t)p.Y % 16 == 0;
     return p.f16 ? launch_few<NumF16>(p, R, stream) : launch_few<NumBf16>(p, R, stream);
 }

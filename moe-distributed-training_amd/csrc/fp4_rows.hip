@@ -87,7 +87,24 @@ __global__ void __launch_bounds__(256) fp4_pack_rows_kernel(const uint16_t* X, i
     for (int64_t c = threadIdx.x; c < ldo; c += 256) out[m * ldo + c] = c < K ? x[c] : (uint16_t)0;
 }
 
+// Scales that 4-byte loads do not take, in rows of whole fours.
+__global__ void __launch_bounds__(256) fp4_pack_scales_kernel(const uint8_t* scales, int64_t sse, int64_t ssn, int64_t N, int64_t G, uint8_t* out, int64_t ldo, int64_t total)
+{
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= total) return;
+    const int64_t row = i / ldo, g = i - row * ldo, e = row / N, n = row - e * N;
+    out[i] = g < G ? scales[e * sse + n * ssn + g] : (uint8_t)0;
+}
+
 }  // namespace
+
+int moe_launch_fp4_pack_scales(const uint8_t* scales, int64_t sse, int64_t ssn, int E, int64_t N, int64_t G, uint8_t* out, int64_t ldo, hipStream_t stream)
+{
+    const int64_t total = E * N * ldo;
+    if (!moe_grid_fits((total + 255) / 256, 256)) return MOE_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL(fp4_pack_scales_kernel, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, stream, scales, sse, ssn, N, G, out, ldo, total);
+    return moe_launch_status();
+}
 
 int moe_launch_fp4_pack_rows(const void* X, int64_t ldx, const void* pos, int pos64, int fan_out, const void* offsets, int off64, int E, int64_t R, int64_t K, void* out, int64_t ldo,
                              hipStream_t stream)

@@ -307,13 +307,19 @@ struct MoeFp4Gemm {
     const void* pos; int pos64; const void* offsets; int off64;
     int E, K; int64_t N;
     int fan_out, x_grouped, y_grouped, f16;
+    const void* gates; int gates_dtype; // backward: weights of the rows at their flat positions, or null
     // set by the launcher
     int quads;                          // weights can be loaded side by side (few_rows.h)
+    int num_cus;                        // workgroups of a round of the tile plan
     int64_t col_blocks;
     int y_vec;                          // Y takes stores of four values
 };
 constexpr int64_t MOE_FP4_RANGE = (int64_t)1 << 31;   // bytes of one expert's codes, and of gathered rows, that 32-bit offsets reach
-int moe_launch_fp4_gemm(MoeFp4Gemm p, int64_t R, hipStream_t stream);
+// (scales of either start at multiples of 4 bytes, in rows of whole fours)
+int moe_launch_fp4_few_rows(MoeFp4Gemm p, int64_t R, hipStream_t stream);
+int moe_launch_fp4_tiles(MoeFp4Gemm p, int64_t R, bool backward, hipStream_t stream);
+// scales (E, N, G) of any strides into rows of ldo, zeros behind G
+int moe_launch_fp4_pack_scales(const uint8_t* scales, int64_t sse, int64_t ssn, int E, int64_t N, int64_t G, uint8_t* out, int64_t ldo, hipStream_t stream);
 // rows of X (row m of the order: m, or pos[m] / fan_out), K of ld columns of a 16-bit type, into rows one after the other of pitch ldo, zeros behind K
 int moe_launch_fp4_pack_rows(const void* X, int64_t ldx, const void* pos, int pos64, int fan_out, const void* offsets, int off64, int E, int64_t R, int64_t K, void* out, int64_t ldo,
                              hipStream_t stream);

@@ -49,7 +49,7 @@ Tensor linear_fp4_rows(const Tensor& x, const Fp4W& w, const Tensor& ssi, const 
     const int64_t R = ssi.size(0), E = w.codes.size(0), K = x.size(1), N = w.codes.size(1);
     Tensor y = at::empty({R, N}, x.options().dtype(rows_type(x.scalar_type(), sums)));
     if (R == 0 || N == 0) return y;
-    Tensor ws = bytes_on(x, moe_linear_fp4_workspace_bytes(ptr(x), x.stride(0), x.size(0), c.grouped_in, dtype_code(x), R, (int)E, K, N));
+    Tensor ws = bytes_on(x, moe_linear_fp4_workspace_bytes(ptr(x), x.stride(0), x.size(0), c.grouped_in, dtype_code(x), w.s(), w.scales.stride(0), w.scales.stride(1), R, (int)E, K, N));
     check(moe_linear_fp4_fwd(ptr(x), x.stride(0), x.size(0), dtype_code(x), w.c(), w.codes.stride(0), w.codes.stride(1), w.s(), w.scales.stride(0), w.scales.stride(1), ptr(y), y.stride(0),
                              dtype_code(y), ptr(ssi), is64(ssi), ptr(eo), is64(eo), (int)E, R, K, N, (int)c.k, c.grouped_in, c.grouped_out, ptr(ws), (size_t)ws.numel(), stream_of(x)),
           "moe_linear_fp4_fwd");
@@ -88,15 +88,16 @@ struct LinearFp4Fn : Function<LinearFp4Fn> {
             if (ctx->needs_input_grad(1)) d_gates = combine_rows_dgates(sv[5].contiguous(), dout, gate_fan, gates.scalar_type());
         }
         if (ctx->needs_input_grad(0)) {
-            dx = at::empty({R, K}, dout.options());
+            dx = at::empty({R, K}, dout.options().dtype(rows_type(dout.scalar_type(), k != 1)));
             if (R > 0 && N > 0) {
-                const Tensor dy = grouped_out ? dout : group_rows(dout, ptr(ssi), is64(ssi), R, gate_fan, flat_gates(gates));
-                Tensor ws = bytes_on(dout, moe_linear_fp4_bwd_workspace_bytes(dtype_code(dout), R, (int)E, K, N));
-                check(moe_linear_fp4_bwd(ptr(dy), dy.stride(0), dtype_code(dy), w.c(), w.codes.stride(0), w.codes.stride(1), w.s(), w.scales.stride(0), w.scales.stride(1), ptr(dx),
-                                         dx.stride(0), grouped_in, ptr(ssi), is64(ssi), ptr(eo), is64(eo), (int)E, R, K, N, ptr(ws), (size_t)ws.numel(), stream_of(dout)),
-                      "moe_linear_fp4_bwd");
+                const Tensor coeff = flat_gates(gates);
+                Tensor ws = bytes_on(dout, moe_linear_fp4_bwd_workspace_bytes(ptr(dout), dout.stride(0), dout.size(0), grouped_out, coeff.defined(), dtype_code(dout), w.s(),
+                                                                              w.scales.stride(0), w.scales.stride(1), R, (int)E, K, N));
+                check(moe_linear_fp4_bwd(ptr(dout), dout.stride(0), dout.size(0), dtype_code(dout), grouped_out, (int)gate_fan, ptr(coeff), coeff.defined() ? dtype_code(coeff) : 0, w.c(),
+                                         w.codes.stride(0), w.codes.stride(1), w.s(), w.scales.stride(0), w.scales.stride(1), ptr(dx), dx.stride(0), dtype_code(dx), grouped_in, ptr(ssi),
+                                         is64(ssi), ptr(eo), is64(eo), (int)E, R, K, N, ptr(ws), (size_t)ws.numel(), stream_of(dout)), "moe_linear_fp4_bwd");
             } else dx.zero_();
-            if (k != 1) dx = combine(dx, Tensor(), nullptr, k, R / k);
+            if (k != 1) dx = combine_rows(dx, Tensor(), k, R / k, dout.scalar_type());
         }
         return {dx, d_gates, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
     }
