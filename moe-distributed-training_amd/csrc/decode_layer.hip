@@ -517,12 +517,13 @@ __global__ void __launch_bounds__(THREADS, 2) gate_up_fp4_kernel(const MoeDecode
 // ends up with 8 consecutive columns of four tokens.
 constexpr int DOWN_PARTS_MAX = 64;
 
-template <class Num, int BITS, bool QUADS>
+// HALVES (up to 8 tokens): rows 8 on of the operand are what the rounding of h lost, so that one product takes both numbers; otherwise two products.
+template <class Num, int BITS, bool QUADS, bool HALVES>
 __global__ void __launch_bounds__(THREADS) down_kernel(const MoeDecode p)
 {
     constexpr bool FP4 = BITS == 4;
     typedef typename std::conditional<QUADS, few::Fp4Quads<Num, 4, false>, few::Fp4Cols<Num, 4, false>>::type W;
-    constexpr int SCRATCH = W::SCRATCH + few::Rows<2>::SCRATCH;   // of a wave, with 4-bit weights
+    constexpr int NA = HALVES ? 1 : 2, SCRATCH = W::SCRATCH + few::Rows<NA>::SCRATCH;   // of a wave, with 4-bit weights
     constexpr int UNITS = 4, PER = FP4 ? 4 : 8;   // floats of a lane and unit: unit nb holds 4 columns of one token, unit r 8 columns of one
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     __shared__ Chosen c;
@@ -549,6 +550,9 @@ __global__ void __launch_bounds__(THREADS) down_kernel(const MoeDecode p)
     const int shares = p.parts * WAVES, share = part * WAVES + wave;
     int64_t at = total * share / shares;
     const int64_t end = total * (share + 1) / shares;
+    // the token that row r of the operand belongs to, and where its numbers lie
+    auto token = [&](int r) { return HALVES ? r & 7 : r; };
+    auto row_of = [&](int r, int j) { return (uint32_t)((token(r) * p.k + j) * p.f + (HALVES && r >= 8 ? (int)p.h_lo : 0)) * 2; };
     float out[UNITS][PER];
 #pragma unroll
     for (int u = 0; u < UNITS; ++u)
@@ -559,24 +563,25 @@ __global__ void __launch_bounds__(THREADS) down_kernel(const MoeDecode p)
         const int s1 = __builtin_amdgcn_readfirstlane(end - at < steps - s0 ? s0 + (int)(end - at) : steps);
         const int e = __builtin_amdgcn_readfirstlane(c.active[a]);
         at += s1 - s0;
-        const int j = i < p.T ? choice_of(c, i, e, p.k) : -1;
+        const int j = token(i) < p.T ? choice_of(c, token(i), e, p.k) : -1;
         if constexpr (FP4) {
             W w;
             w.columns(0, p.f2, e, p.f, [&](int nb, int c) { return (int64_t)tile * 64 + (c >> 2) * 16 + 4 * nb + (c & 3); });   // (d is a multiple of 64)
-            few::Rows<2> rows;
-            rows.x[0] = few::buffer(p.h);
-            rows.x[1] = few::buffer(p.h + p.h_lo);
+            few::Rows<NA> rows;
+#pragma unroll
+            for (int m = 0; m < NA; ++m) rows.x[m] = few::buffer(p.h + m * p.h_lo);
             rows.left = p.f - 8 * i;
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
-                const int t = 4 * y + q, jt = t < p.T ? choice_of(c, t, e, p.k) : -1;
-                rows.a[0][y] = rows.a[1][y] = jt >= 0 ? (uint32_t)((t * p.k + jt) * p.f + 8 * i) * 2 : few::RANGE;
+                const int r = 4 * y + q, jt = token(r) < p.T ? choice_of(c, token(r), e, p.k) : -1;
+#pragma unroll
+                for (int m = 0; m < NA; ++m) rows.a[m][y] = jt >= 0 ? row_of(r, jt) + 16 * i : few::RANGE;
             }
             f32x4_t acc[1][4];
 #pragma unroll
             for (int nb = 0; nb < 4; ++nb) acc[0][nb] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-            few::stream<W, 2, true, 2, 2>(acc, w, rows, s0, s1, smem + wave * SCRATCH);
-            const float g = j >= 0 ? c.weight[i][j] : 0.f;
+            few::stream<W, NA, true, HALVES ? 3 : 2, HALVES && W::UNIT == 1 ? 3 : 2>(acc, w, rows, s0, s1, smem + wave * SCRATCH);
+            const float g = j >= 0 ? c.weight[token(i)][j] : 0.f;
 #pragma unroll
             for (int u = 0; u < UNITS; ++u)
 #pragma unroll
@@ -585,19 +590,19 @@ __global__ void __launch_bounds__(THREADS) down_kernel(const MoeDecode p)
             const few::Buffer w = few::buffer((const uint16_t*)p.w2 + (int64_t)e * p.f * p.d);
             const int n = tile * 128 + 8 * i;
             const uint32_t col = n < p.d ? (uint32_t)(n + 8 * q * p.d) * 2 : few::RANGE;
-            const uint32_t row = j >= 0 ? (uint32_t)((i * p.k + j) * p.f + 8 * q) * 2 : few::RANGE;
+            const uint32_t row = j >= 0 ? row_of(i, j) + 16 * q : few::RANGE;
             const few::Buffer hb[2] = {few::buffer(p.h), few::buffer(p.h + p.h_lo)};
             f32x4_t acc[8];
 #pragma unroll
             for (int b = 0; b < 8; ++b) acc[b] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-            constexpr int DEPTH = 2;
+            constexpr int DEPTH = HALVES ? 3 : 2;
             fp4_u32x4_t ws[DEPTH][8];
-            bf16x8_t as[DEPTH][2];
+            bf16x8_t as[DEPTH][NA];
             auto fetch = [&](int dst, int s) {
 #pragma unroll
                 for (int r = 0; r < 8; ++r) ws[dst][r] = few::load16_streamed(w, col, (uint32_t)(s * 32 + r) * (uint32_t)p.d * 2);
 #pragma unroll
-                for (int m = 0; m < 2; ++m) as[dst][m] = __builtin_bit_cast(bf16x8_t, few::load16(hb[m], row, (uint32_t)s * 64));
+                for (int m = 0; m < NA; ++m) as[dst][m] = __builtin_bit_cast(bf16x8_t, few::load16(hb[m], row, (uint32_t)s * 64));
                 __builtin_amdgcn_sched_barrier(0);
             };
             auto multiply = [&](int src) {
@@ -608,38 +613,40 @@ __global__ void __launch_bounds__(THREADS) down_kernel(const MoeDecode p)
                     for (int r = 0; r < 4; ++r)
                         f[r] = __builtin_amdgcn_perm(ws[src][2 * r + 1][b / 2], ws[src][2 * r][b / 2], b & 1 ? 0x07060302u : 0x05040100u);
                     const bf16x8_t wf = __builtin_bit_cast(bf16x8_t, f);
-                    acc[b] = Num::mfma(as[src][0], wf, acc[b]);
-                    acc[b] = Num::mfma(as[src][1], wf, acc[b]);
+#pragma unroll
+                    for (int m = 0; m < NA; ++m) acc[b] = Num::mfma(as[src][m], wf, acc[b]);
                 }
                 __builtin_amdgcn_sched_barrier(0);   // (as in few::stream)
             };
+#pragma unroll
+            for (int x = 0; x < DEPTH; ++x)
+                if (s0 + x < s1) fetch(x, s0 + x);
             int s = s0;
-            if (s1 - s0 >= DEPTH) {
+            for (; s + 2 * DEPTH <= s1; s += DEPTH)
 #pragma unroll
-                for (int x = 0; x < DEPTH; ++x) fetch(x, s + x);
-                for (; s + 2 * DEPTH <= s1; s += DEPTH)
+                for (int x = 0; x < DEPTH; ++x) { multiply(x); fetch(x, s + DEPTH + x); }
+            for (; s < s1; s += DEPTH)
 #pragma unroll
-                    for (int x = 0; x < DEPTH; ++x) { multiply(x); fetch(x, s + DEPTH + x); }
-                const int more = s1 - s - DEPTH;
-#pragma unroll
-                for (int x = 0; x < DEPTH; ++x) { multiply(x); if (x < more) fetch(x, s + DEPTH + x); }
-#pragma unroll
-                for (int x = 0; x < DEPTH - 1; ++x)
-                    if (x < more) multiply(x);
-            } else {
-                fetch(0, s);
-                multiply(0);
-            }
-            // acc[b][r] is column 8 i + b of token 4 q + r
+                for (int x = 0; x < DEPTH; ++x) {
+                    if (s + x >= s1) break;
+                    multiply(x);
+                    if (s + x + DEPTH < s1) fetch(x, s + x + DEPTH);
+                }
+            // acc[b][r] is column 8 i + b of row 4 q + r
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int t = 4 * q + r, jr = t < p.T ? choice_of(c, t, e, p.k) : -1;
+                const int t = token(4 * q + r), jr = t < p.T ? choice_of(c, t, e, p.k) : -1;
                 const float g = jr >= 0 ? c.weight[t][jr] : 0.f;
 #pragma unroll
                 for (int b = 0; b < 8; ++b) out[r][b] = jr >= 0 ? out[r][b] + g * acc[b][r] : out[r][b];
             }
         }
     }
+    if constexpr (HALVES)   // both numbers' products
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u)
+#pragma unroll
+            for (int v = 0; v < PER; ++v) out[u][v] += __shfl_xor(out[u][v], FP4 ? 8 : 32);
     // ---- the waves' sums, in wave order
     __syncthreads();   // (they take the place of the operands)
 #pragma unroll
@@ -731,7 +738,7 @@ template <class Num, int BITS> int launch_typed(const MoeDecode& p, const Plan& 
         hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(THREADS), lds, stream, p);
         return moe_launch_status();
     };
-    static std::atomic<bool> set1[3][MOE_MAX_DEVICES], set2[2][MOE_MAX_DEVICES];
+    static std::atomic<bool> set1[3][MOE_MAX_DEVICES], set2[4][MOE_MAX_DEVICES];
     typedef few::Fp4Quads<Num, 2, true> Q2;
     typedef few::Fp4Quads<Num, 4, false> Q4;
     constexpr size_t rows2 = few::Rows<2>::SCRATCH, sums = (size_t)4 * 64 * (FP4 ? 4 : 8) * 4;
@@ -745,9 +752,12 @@ template <class Num, int BITS> int launch_typed(const MoeDecode& p, const Plan& 
         else rc = go(gate_up_kernel<Num, 16, false, true>, pl.grid1, WAVES * gate_up_scratch<few::Cols16<Num, 2>, false>(), set1[1]);
     }
     if (rc != MOE_OK) return rc;
-    if (FP4 && p.f % (2 * few::CHUNK)) return go(down_kernel<Num, BITS, false>, pl.tiles * pl.parts, WAVES * (rows2 > sums ? rows2 : sums), set2[0]);
     constexpr size_t operands = FP4 ? Q4::SCRATCH + rows2 : 0;
-    return go(down_kernel<Num, BITS, true>, pl.tiles * pl.parts, WAVES * (operands > sums ? operands : sums), set2[1]);
+    const bool halves = p.T <= 8, odd = FP4 && p.f % (2 * few::CHUNK);
+    const size_t lds = WAVES * (odd ? (rows2 > sums ? rows2 : sums) : operands > sums ? operands : sums);
+    if constexpr (FP4)
+        if (odd) return halves ? go(down_kernel<Num, BITS, false, true>, pl.tiles * pl.parts, lds, set2[0]) : go(down_kernel<Num, BITS, false, false>, pl.tiles * pl.parts, lds, set2[1]);
+    return halves ? go(down_kernel<Num, BITS, true, true>, pl.tiles * pl.parts, lds, set2[2]) : go(down_kernel<Num, BITS, true, false>, pl.tiles * pl.parts, lds, set2[3]);
 }
 
 }  // namespace
