@@ -710,7 +710,8 @@ Plan plan(int T, int E, int d, int f, int k, bool fp4)
     // split: 0 where a wave cannot keep its part of x (gate_up_kernel)
     const int chunks = (d + few::CHUNK - 1) / few::CHUNK;
     r.split = 0;
-    if (chunks <= 4 * WAVES && (!fp4 || d % (4 * few::CHUNK) == 0))
+    // (nor where there is at most one job per compute unit: nothing to keep x for, and a ring of whole jobs costs more than it hides: d = 256, f = 512, 3 tokens 13.3 us)
+    if (jobs > cus && chunks <= 4 * WAVES && (!fp4 || d % (4 * few::CHUNK) == 0))
         for (r.split = 1; r.split * 4 < chunks;) r.split *= 2;
     const int64_t at_once = r.split ? WAVES / r.split : 1, groups = (jobs + at_once - 1) / at_once;
     r.grid1 = (int)(groups < cus ? groups : cus);
