@@ -145,14 +145,15 @@ def fused_expert_mlp_fp4(x, weights: Fp4ExpertWeights, k, sorted_scattered_idxs,
 
 def scattermoe_permute_and_compute(x, w1, w2, w3, ffn_hidden_size, hidden_size, top_k, bin_ids, indices, num_experts,
                                    lora_pointers=None, moe_expert_model_parallelism=True, expert_offsets=None,
-                                   lora_views: Optional[LoraViews] = None, lora_alpha: float = 1.0):
+                                   lora_views: Optional[LoraViews] = None, lora_alpha: float = 1.0, keep_8bit: bool = False):
     """Functional form of the reference caller (config_utils.py:99-185).
 
     x (rows, hidden); w1, w2, w3 storage (E*ffn, hidden); ``bin_ids`` / ``indices`` = sorted expert ids and sorted
     flat positions; ``lora_pointers[name] = (A.weight, B.weight, r, alpha, hidden, ffn)`` as peft_utils.py:127-132
     (or ``lora_views`` / ``lora_alpha``: the six factor views already in (E, K, r) / (E, r, N) form).
     Expert-parallel mode treats x as pre-dispatched rows (fan-out 1) and scatters the output back to ``indices``;
-    otherwise the fan-out is top_k and the output stays in grouped order (the caller's ops.scatter combines it)."""
+    otherwise the fan-out is top_k and the output stays in grouped order (the caller's ops.scatter combines it).  ``keep_8bit``: through the
+    three projections, gate and up kept for the backward pass as 8-bit codes (``swiglu_8bit``)."""
     with torch.no_grad():
         if expert_offsets is None:
             expert_offsets = ops.expert_offsets_from_sorted(bin_ids, num_experts)
@@ -169,7 +170,7 @@ def scattermoe_permute_and_compute(x, w1, w2, w3, ffn_hidden_size, hidden_size, 
         lora = LoraViews(v["a1"], v["b1"], v["a3"], v["b3"], v["a2"], v["b2"])
     elif lora_views is not None:
         lora, alpha = lora_views, lora_alpha
-    if native.mlp_fast_path(x, W["w1"], W["w2"], W["w3"], [] if lora is None else list(lora)):
+    if not keep_8bit and native.mlp_fast_path(x, W["w1"], W["w2"], W["w3"], [] if lora is None else list(lora)):
         return fused_expert_mlp(x, W["w1"], W["w2"], W["w3"], fan, indices, expert_offsets, lora, alpha, None, grouped_out)
     # generic route: the reference's three calls (:127-166)
     def proj(inp, name, kk, gin, gout):
@@ -181,7 +182,7 @@ def scattermoe_permute_and_compute(x, w1, w2, w3, ffn_hidden_size, hidden_size, 
                                     gin, gout)
     h1 = proj(x, "w1", fan, False, True)
     h3 = proj(x, "w3", fan, False, True)
-    h = entry("swiglu")(h1, h3)
+    h = swiglu_8bit(h1, h3) if keep_8bit else entry("swiglu")(h1, h3)
     return proj(h, "w2", 1, True, grouped_out)
 
 
@@ -247,6 +248,7 @@ class ScatterMoEBlock(nn.Module):
                  dtype=torch.bfloat16, device=None, bias=False, return_bias=False):
         super().__init__()
         self.return_bias = return_bias
+        self.keep_8bit = False
         self.bias = nn.Parameter(torch.zeros(hidden_size, dtype=dtype, device=device)) if bias else None
         self.hidden_size, self.ffn_hidden_size = hidden_size, ffn_hidden_size
         self.num_experts, self.top_k, self.lora_r, self.lora_alpha = num_experts, top_k, lora_r, lora_alpha
@@ -277,40 +279,79 @@ class ScatterMoEBlock(nn.Module):
             v["a" + n[1]], v["b" + n[1]] = a, b
         return LoraViews(v["a1"], v["b1"], v["a3"], v["b3"], v["a2"], v["b2"])
 
-    def quantize_experts(self) -> "ScatterMoEBlock":
-        """Puts 8-bit codes in the place of the expert weights, for serving and for training what lies before and around them:
-        w1, w2, w3 become int8 buffers (E, f, d) with fp32 buffers ``w1_scale``, ``w2_scale``, ``w3_scale`` of their output
-        columns, and ``forward`` takes the products over them (bf16 or fp16 hidden states, sizes that are multiples of 64).  The
-        router keeps its type, and the block from then on: a conversion that would round the scales is refused.  Not for a block with
-        adapters: its factors are trained against the weights as they are.  A block that the products could not serve is refused and
-        keeps its weights."""
+    def quantize_experts(self, bits: int = 8, keep_8bit: bool = False) -> "ScatterMoEBlock":
+        """Puts codes in the place of the expert weights, for serving and for training what lies before and around them.
+
+        ``bits`` 8: w1, w2, w3 become int8 buffers (E, f, d) with fp32 buffers ``w1_scale``, ``w2_scale``, ``w3_scale`` of their output
+        columns, and ``forward`` takes the products over them (bf16 or fp16 hidden states, sizes that are multiples of 64).  The router
+        keeps its type, and the block from then on: a conversion that would round the scales is refused.
+        ``bits`` 4: uint8 buffers of ``Fp4ExpertWeights``; a batch of up to 16 tokens without gradients runs as two launches;
+        ``keep_8bit`` as in ``fused_expert_mlp_fp4``.
+
+        Not for a block with adapters: its factors are trained against the weights as they are.  A block that the products could not
+        serve is refused and keeps its weights."""
+        if bits not in (4, 8):
+            raise ValueError(f"expert weights are held in 8 or 4 bits, not {bits}")
+        if keep_8bit and bits != 4:
+            raise ValueError("keep_8bit goes with experts in 4 bits: the products over 8-bit weights keep interims of their own")
         if self.lora_r > 0:
             raise ValueError("a block with adapters keeps its expert weights: quantize_experts() takes blocks with lora_r = 0")
         if self.is_quantized:
+            if bits != self.expert_bits:
+                raise ValueError(f"the experts are held in {self.expert_bits} bits already; their weights are gone")
+            self.keep_8bit = bool(keep_8bit)
             return self
-        if self.router.dtype not in (torch.bfloat16, torch.float16):
-            raise ValueError(f"the expert MLP over 8-bit weights takes bf16 or fp16 hidden states, this block's are {self.router.dtype}: "
-                             "convert the block first")
         d, f = self.hidden_size, self.ffn_hidden_size
-        if d % 64 or f % 64 or max(d, f) >= 2 ** 17 or d * f >= 2 ** (31 if d % 128 or f % 128 else 32) - 16:
-            raise ValueError(f"the expert MLP over 8-bit weights takes sizes that are multiples of 64, below 2^17 and together below 2^32 (2^31 "
-                             f"where one is no multiple of 128), not hidden size {d} and ffn size {f}")
-        q = Int8ExpertWeights.quantize(self.w1, self.w2, self.w3, self.ffn_hidden_size, self.hidden_size)
+        if bits == 4:
+            if self.router.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+                raise ValueError(f"the expert MLP over 4-bit weights takes bf16, fp16 or fp32 hidden states, this block's are {self.router.dtype}")
+            if max(d, f) > 2 ** 20 or d * f >= 2 ** 31:
+                raise ValueError(f"the expert MLP over 4-bit weights takes sizes up to 2^20, together below 2^31, not hidden size {d} and ffn size {f}")
+            q = Fp4ExpertWeights.quantize(self.w1, self.w2, self.w3, f, d)
+        else:
+            if self.router.dtype not in (torch.bfloat16, torch.float16):
+                raise ValueError(f"the expert MLP over 8-bit weights takes bf16 or fp16 hidden states, this block's are {self.router.dtype}: "
+                                 "convert the block first")
+            if d % 64 or f % 64 or max(d, f) >= 2 ** 17 or d * f >= 2 ** (31 if d % 128 or f % 128 else 32) - 16:
+                raise ValueError(f"the expert MLP over 8-bit weights takes sizes that are multiples of 64, below 2^17 and together below 2^32 (2^31 "
+                                 f"where one is no multiple of 128), not hidden size {d} and ffn size {f}")
+            q = Int8ExpertWeights.quantize(self.w1, self.w2, self.w3, f, d)
         for name, t in q._asdict().items():
             if hasattr(self, name):
                 delattr(self, name)
             self.register_buffer(name, t)
+        self.keep_8bit = bool(keep_8bit)
         return self
 
     @property
+    def expert_bits(self) -> int:
+        """Bits of an expert weight: 4 or 8 after ``quantize_experts``, otherwise those of its type."""
+        return {torch.uint8: 4, torch.int8: 8}.get(self.w1.dtype) or torch.finfo(self.w1.dtype).bits
+
+    @property
     def is_quantized(self) -> bool:
-        return self.w1.dtype == torch.int8
+        return self.w1.dtype in (torch.int8, torch.uint8)
 
     def _apply(self, fn, *args, **kw):
-        # (what ``to``, ``half``, ``cuda`` and the like go through, also those of a module around this one)
-        if self.is_quantized and any(fn(t.detach()[:0]).dtype != t.dtype for t in (self.w1_scale, self.router)):
+        # (what ``to``, ``half``, ``cuda`` and the like go through, also those of a module around this one; 4-bit weights have no type to lose)
+        if self.w1.dtype == torch.int8 and any(fn(t.detach()[:0]).dtype != t.dtype for t in (self.w1_scale, self.router)):
             raise TypeError("a block with experts in 8 bits keeps its type, and its scales stay float32: choose the type before quantize_experts()")
         return super()._apply(fn, *args, **kw)
+
+    def _weights(self, kind):
+        return kind(*(getattr(self, n) for n in kind._fields))
+
+    def decode(self, hidden_states: torch.Tensor):
+        """``forward`` for the tokens of a generation step, without gradients: up to 16 of them through ``moe_layer_decode`` (two launches;
+        a block without adapters, bf16 or fp16 weights or weights in 4 bits).  Returns as ``forward`` does."""
+        if self.lora_r > 0:
+            raise ValueError("decode() takes blocks without adapters (lora_r = 0): use forward()")
+        with torch.no_grad():
+            if self.is_quantized:
+                return self.forward(hidden_states)
+            x = hidden_states.reshape(-1, hidden_states.shape[-1])
+            w = [resolve_dtensor(t).view(self.num_experts, self.ffn_hidden_size, self.hidden_size) for t in (self.w1, self.w2, self.w3)]
+            return self._returned(moe_layer_decode(x, resolve_dtensor(self.router), *w, self.top_k)[0].view(hidden_states.shape))
 
     def forward(self, hidden_states: torch.Tensor):
         shape = hidden_states.shape
@@ -319,13 +360,16 @@ class ScatterMoEBlock(nn.Module):
         lora = []
         if self.lora_r > 0:   # the factors in their storage, in the order a1, b1, a3, b3, a2, b2 (w2's are swapped, see lora_views)
             lora = [resolve_dtensor(t) for t in (self.lora_A_w1, self.lora_B_w1, self.lora_A_w3, self.lora_B_w3, self.lora_B_w2, self.lora_A_w2)]
-        if self.is_quantized:
-            out = moe_layer_forward_int8(x, resolve_dtensor(self.router), Int8ExpertWeights(*(getattr(self, n) for n in Int8ExpertWeights._fields)),
-                                         self.top_k)[0]
+        if self.expert_bits == 8:
+            out = moe_layer_forward_int8(x, resolve_dtensor(self.router), self._weights(Int8ExpertWeights), self.top_k)[0]
+        elif self.expert_bits == 4:
+            out = moe_layer_forward_fp4(x, resolve_dtensor(self.router), self._weights(Fp4ExpertWeights), self.top_k, keep_8bit=self.keep_8bit)[0]
         else:
             out = _layer(x, resolve_dtensor(self.router), resolve_dtensor(self.w1), resolve_dtensor(self.w2), resolve_dtensor(self.w3), E, f,
                          self.top_k, lora, self.lora_alpha, True, True)[0]
-        out = out.view(shape)
+        return self._returned(out.view(shape))
+
+    def _returned(self, out):
         if self.bias is not None:
             if self.return_bias:
                 return out, self.bias
