@@ -263,7 +263,8 @@ int moe_decode_layer_fp4(const void* x, int64_t ldx, const void* wg, int64_t ldw
     p.f1 = take(c1, s1, f, d);
     p.f3 = take(c3, s3, f, d);
     p.f2 = take(c2, s2, d, f);
-    if (!weights_ok(p.f1) || !weights_ok(p.f3) || !weights_ok(p.f2)) return MOE_ERR_BAD_ARG;
+    for (const MoeFp4Weights* w : {&p.f1, &p.f3, &p.f2})
+        if (!weights_ok(*w) || !aligned16(w->scales)) return MOE_ERR_BAD_ARG;
     return moe_launch_decode(p, true, dtype == MOE_F16, workspace, S(stream));
 }
 

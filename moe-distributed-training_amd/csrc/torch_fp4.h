@@ -39,9 +39,8 @@ void check_fp4(const Tensor& codes, const Tensor& scales, int64_t K)
 Fp4W take_fp4(const Tensor& codes, const Tensor& scales)
 {
     const bool ok = codes.stride(2) == 1 && codes.stride(0) % 16 == 0 && codes.stride(1) % 16 == 0 && (uintptr_t)codes.data_ptr() % 16 == 0;
-    Tensor c = ok ? codes : codes.contiguous();
-    if ((uintptr_t)c.data_ptr() % 16 != 0) c = c.clone();   // (contiguous already, at an address that 16-byte loads do not take)
-    return {c, scales.stride(2) == 1 ? scales : scales.contiguous()};
+    // (a copy also where contiguous() would see nothing to do: an odd address, or an odd pitch of a single row)
+    return {ok ? codes : codes.clone(at::MemoryFormat::Contiguous), scales.stride(2) == 1 ? scales : scales.contiguous()};
 }
 
 Tensor linear_fp4_rows(const Tensor& x, const Fp4W& w, const Tensor& ssi, const Tensor& eo, const LinearCfg& c, bool sums)
@@ -198,12 +197,16 @@ DecodeOut decode_outputs(const Tensor& x, int64_t k)
     return {at::empty({T, x.size(1)}, x.options()), at::empty({T, k}, x.options().dtype(at::kFloat)), at::empty({T, k}, x.options().dtype(at::kInt))};
 }
 
-// rows at multiples of 16 bytes
+// rows at multiples of 16 bytes, within 32-bit offsets
 Tensor aligned_rows(const Tensor& t)
 {
     const Tensor u = unit_inner(t);
-    return (uintptr_t)u.data_ptr() % 16 == 0 && (u.size(0) < 2 || u.stride(0) % 8 == 0) ? u : u.clone(at::MemoryFormat::Contiguous);
+    const bool ok = (uintptr_t)u.data_ptr() % 16 == 0 && u.stride(0) % 8 == 0 && u.size(0) * u.stride(0) + u.size(1) < (int64_t)1 << 30;
+    return ok ? u : u.clone(at::MemoryFormat::Contiguous);
 }
+
+// all of it in order, from a multiple of 16 bytes on
+Tensor whole(const Tensor& t) { return t.is_contiguous() && (uintptr_t)t.data_ptr() % 16 == 0 ? t : t.clone(at::MemoryFormat::Contiguous); }
 
 // what the two launches for a few tokens take
 bool decode_takes(int64_t T, int64_t E, int64_t d, int64_t f, int64_t k)
@@ -236,7 +239,6 @@ variable_list layer_decode(const Tensor& x_, const Tensor& wg_, const Tensor& w1
                 " tokens, ", E, " experts of ", f, " x ", d, ", top ", k, "; use moe_layer_forward for others");
     const c10::DeviceGuard guard(x_.device());
     const Tensor x = aligned_rows(x_), wg = aligned_rows(wg_);
-    auto whole = [](const Tensor& w) { return w.is_contiguous() && (uintptr_t)w.data_ptr() % 16 == 0 ? w : w.clone(at::MemoryFormat::Contiguous); };
     const Tensor w1 = whole(w1_), w2 = whole(w2_), w3 = whole(w3_);
     DecodeOut o = decode_outputs(x, k);
     if (T == 0) return {o.out, o.weights, o.indices};
@@ -253,10 +255,7 @@ DecodeOut layer_decode_fp4(const Tensor& x_, const Tensor& wg_, const Fp4Mlp& m,
     const int64_t T = x.size(0);
     DecodeOut o = decode_outputs(x, k);
     Tensor w[3], s[3];
-    for (int i = 0; i < 3; ++i) {
-        w[i] = m.w[i].is_contiguous() && (uintptr_t)m.w[i].data_ptr() % 16 == 0 ? m.w[i] : m.w[i].clone(at::MemoryFormat::Contiguous);
-        s[i] = m.s[i].contiguous();
-    }
+    for (int i = 0; i < 3; ++i) { w[i] = whole(m.w[i]); s[i] = whole(m.s[i]); }
     auto b = [](const Tensor& t) { return (const uint8_t*)ptr(t); };
     Tensor ws = bytes_on(x, moe_decode_layer_workspace_bytes(T, (int)m.E, m.d, m.f, (int)k, 4));
     check(moe_decode_layer_fp4(ptr(x), x.stride(0), ptr(wg), wg.stride(0), dtype_code(x), b(w[0]), b(s[0]), b(w[2]), b(s[2]), b(w[1]), b(s[1]), ptr(o.out), o.out.stride(0),

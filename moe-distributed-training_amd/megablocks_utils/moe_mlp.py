@@ -360,9 +360,9 @@ class ScatterMoEBlock(nn.Module):
         lora = []
         if self.lora_r > 0:   # the factors in their storage, in the order a1, b1, a3, b3, a2, b2 (w2's are swapped, see lora_views)
             lora = [resolve_dtensor(t) for t in (self.lora_A_w1, self.lora_B_w1, self.lora_A_w3, self.lora_B_w3, self.lora_B_w2, self.lora_A_w2)]
-        if self.expert_bits == 8:
+        if self.w1.dtype == torch.int8:
             out = moe_layer_forward_int8(x, resolve_dtensor(self.router), self._weights(Int8ExpertWeights), self.top_k)[0]
-        elif self.expert_bits == 4:
+        elif self.w1.dtype == torch.uint8:
             out = moe_layer_forward_fp4(x, resolve_dtensor(self.router), self._weights(Fp4ExpertWeights), self.top_k, keep_8bit=self.keep_8bit)[0]
         else:
             out = _layer(x, resolve_dtensor(self.router), resolve_dtensor(self.w1), resolve_dtensor(self.w2), resolve_dtensor(self.w3), E, f,
