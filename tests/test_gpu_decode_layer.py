@@ -211,3 +211,102 @@ def test_empty(dev):
     with torch.no_grad():
         out, ew, ei = moe.moe_layer_decode(x[:0].to(dev), wg.to(dev), *(t.to(dev) for t in w), 1)
     assert out.shape == (0, 64) and ew.shape == (0, 1) and ei.shape == (0, 1)
+
+
+def make_codes(T, d, f, E, seed=0):
+    """Any codes and scales: what a quantisation gives is a part of them."""
+    g = torch.Generator().manual_seed(seed * 31 + T + d + f + E)
+    x = torch.randn(T, d, generator=g).to(BF16)
+    wg = (torch.randn(E, d, generator=g) * 0.05).to(BF16)
+    q = [(torch.randint(0, 256, (E, n, m // 2), generator=g, dtype=torch.uint8), torch.randint(117, 123, (E, n, m // 32), generator=g, dtype=torch.uint8)) for n, m in ((f, d), (d, f), (f, d))]
+    return x, wg, q
+
+
+KEPT = [  # more blocks of 16 ffn columns than the card has compute units, hidden sizes up to 4096 and above
+    (3, 512, 1024, 8, 2), (16, 1024, 1024, 8, 2), (5, 1536, 2048, 4, 3), (2, 4096, 1536, 4, 2), (16, 2048, 512, 32, 4), (6, 576, 1216, 6, 3), (9, 128, 2112, 4, 2), (8, 64, 4160, 2, 1),
+    (2, 4160, 1088, 4, 2), (1, 8192, 2112, 2, 2), (12, 256, 960, 20, 8),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("T,d,f,E,k", KEPT)
+def test_layer_of_many_blocks(dev, T, d, f, E, k, dtype):
+    check(dev, T, d, f, E, k, dtype, 16)
+
+
+@pytest.mark.parametrize("T,d,f,E,k", KEPT)
+def test_layer_of_many_blocks_in_4_bits(dev, T, d, f, E, k):
+    x, wg, q = make_codes(T, d, f, E)
+    w1, w2, w3 = (oracle.weights(*t, n) for t, n in zip(q, (d, f, d)))
+    want, weights, idx, terms, back = oracle.layer(x, wg, w1, w3, w2, k)
+    out, ew, ei = run(dev, x, wg, q, k, bits=4)
+    assert torch.equal(ei.cpu().long(), idx)
+    lt = 2 * ((d + 8) * (x.double().abs() @ wg.double().abs().t()).amax() + 16) * 2.0 ** -24
+    assert float(((ew.double().cpu() - weights) / weights).abs().max()) <= lt
+    over = (out.double().cpu() - want).abs() - slack_of(want, terms, back, 0.0, d, f, BF16) - lt * terms
+    assert float(over.max()) <= 0
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_many_blocks_repeat_and_keep_what_is_not_finite(dev, bits):
+    """The same bits from call to call, and from a token alone to the same token beside others that hold NaN."""
+    T, d, f, E, k = 10, 512, 1536, 6, 2
+    x, wg, q = make_codes(T, d, f, E)
+    w = q if bits == 4 else [(0.05 * torch.randn(E, f, d, generator=torch.Generator().manual_seed(i))).to(BF16) for i in range(3)]
+    want = run(dev, x, wg, w, k, bits=bits)
+    for _ in range(5):
+        assert all(torch.equal(a, b) for a, b in zip(run(dev, x, wg, w, k, bits=bits), want))
+    bad = x.clone()
+    bad[3], bad[7, 100] = float("nan"), float("-inf")
+    out, ew, ei = run(dev, bad, wg, w, k, bits=bits)
+    keep = [0, 1, 2, 4, 5, 6, 8, 9]
+    assert torch.equal(out[keep], want[0][keep]) and torch.equal(ei[keep], want[2][keep]) and int(ei.min()) >= 0 and int(ei.max()) < E
+
+
+def test_codes_and_scales_at_odd_addresses(dev):
+    T, d, f, E, k = 4, 512, 1024, 8, 2
+    x, wg, q = make_codes(T, d, f, E)
+    want = run(dev, x, wg, q, k, bits=4)
+
+    def odd(t):
+        buf = torch.empty(t.numel() + 16, dtype=t.dtype, device=dev)
+        at = 3 if buf.data_ptr() % 16 == 0 else 0
+        return buf[at:at + t.numel()].view(t.shape).copy_(t)
+    with torch.no_grad():
+        for pick in (lambda i: True, lambda i: i % 2 == 0, lambda i: i % 2 == 1):
+            w = moe.Fp4ExpertWeights(*(odd(t) if pick(i) else t.to(dev) for i, t in enumerate(t for p in q for t in p)))
+            got = moe.moe_layer_forward_fp4(x.to(dev), wg.to(dev), w, k)
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+        # one row of a pitch that 16-byte loads do not take, and every token the same row
+        one = torch.empty(1, d + 3, dtype=BF16, device=dev)[:, :d].copy_(x[:1])
+        assert torch.equal(moe.moe_layer_forward_fp4(one, wg.to(dev), moe.Fp4ExpertWeights(*(t.to(dev) for p in q for t in p)), k)[0], run(dev, x[:1], wg, q, k, bits=4)[0])
+        same = moe.moe_layer_forward_fp4(x[:1].to(dev).expand(5, d), wg.to(dev), moe.Fp4ExpertWeights(*(t.to(dev) for p in q for t in p)), k)[0]
+        assert torch.equal(same, run(dev, x[:1].repeat(5, 1), wg, q, k, bits=4)[0])
+
+
+def test_graphs_that_share_a_memory_pool(dev):
+    """Two captured layers whose workspaces may be the same memory, replayed in turn between eager calls."""
+    T, d, f, E, k = 5, 512, 1024, 8, 2
+    x, wg, q = make_codes(T, d, f, E)
+    xd, wgd, w4 = x.to(dev), wg.to(dev), moe.Fp4ExpertWeights(*(t.to(dev) for p in q for t in p))
+    w16 = [(0.05 * torch.randn(E, f, d, generator=torch.Generator().manual_seed(i))).to(BF16).to(dev) for i in range(3)]
+    calls = [lambda: moe.moe_layer_forward_fp4(xd, wgd, w4, k)[0], lambda: moe.moe_layer_decode(xd, wgd, *w16, k)[0]]
+    with torch.no_grad():
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for c in calls:
+                c()
+        torch.cuda.current_stream().wait_stream(side)
+        graphs, outs, pool = [], [], None
+        for c in calls:
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1], pool=pool):
+                outs.append(c())
+            pool = pool or graphs[0].pool()
+        for trial, i in enumerate((0, 1, 1, 0, 0, 1)):
+            xd.copy_(torch.randn(x.shape, generator=torch.Generator().manual_seed(trial)).to(BF16))
+            graphs[i].replay()
+            torch.cuda.synchronize()
+            got = outs[i].clone()
+            assert torch.equal(got, calls[i]()), (trial, i)

@@ -200,3 +200,126 @@ def test_rows_behind_the_last_group_are_left_as_they_were(dev):
         want = oracle.linear(x, oracle.weights(codes, scales, 128), 1, sei, ssi)
         at = ssi[:-2]
         close(y.cpu()[at], want["y"][at], half_step(BF16) * want["y"][at].abs() + 136 * 2.0 ** -24 * want["y_terms"][at], "y")
+
+
+LARGER = [  # whole lines of codes (multiples of 256 inputs), narrow and wide, few rows and tiles, up to several rounds of tiles
+    (24, 1024, 640, 3, 2), (9, 4096, 200, 2, 1), (1, 2560, 1408, 8, 2), (700, 512, 1032, 8, 2), (260, 768, 2056, 1, 1), (2000, 256, 264, 3, 2), (129, 520, 5000, 2, 1), (64, 8192, 24, 2, 2),
+    (333, 1368, 1000, 6, 2), (17, 96, 4104, 40, 4),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("T,K,N,E,k", LARGER)
+def test_larger_projections(dev, dtype, T, K, N, E, k):
+    check_linear(dev, T, K, N, E, k, dtype)
+
+
+@pytest.mark.parametrize("T", [1, 15, 16, 17, 31, 33, 63, 65, 96, 127, 128, 129, 200, 257])
+def test_groups_of_every_filling(dev, T):
+    """All rows in one of three experts, and rows spread over them."""
+    check_linear(dev, T, 320, 272, 3, 1, BF16, absent=(0, 2), seed=T)
+    check_linear(dev, T, 512, 136, 3, 2, BF16, gates=False, seed=T)
+
+
+def test_single_columns_and_groups_with_odd_strides(dev):
+    """Sizes of one, whose strides say nothing."""
+    x, codes, scales, (sei, ssi, offs, _), g = make(6, 32, 1, 1, 1, BF16)
+    want = oracle.linear(x, oracle.weights(codes, scales, 32), 1, sei, ssi)
+    args = (1, sei.to(dev), ssi.to(dev), None, offs.to(dev))
+    c = torch.empty(1, 1, 16, dtype=torch.uint8, device=dev).copy_(codes).as_strided((1, 1, 16), (5, 7, 1))
+    s = scales.to(dev).as_strided((1, 1, 1), (3, 5, 9))
+    close(moe.parallel_linear_fp4(x.to(dev), c, s, *args), want["y"], half_step(BF16) * want["y"].abs() + 40 * 2.0 ** -24 * want["y_terms"], "y")
+    # one expert's weights for all, and one row for all
+    x2, codes2, scales2, (sei, ssi, offs, _), g = make(20, 64, 48, 3, 1, BF16)
+    cd, sd = (t[:1].to(dev).expand(3, *t.shape[1:]) for t in (codes2, scales2))
+    xe = x2[:1].to(dev).expand(20, 64).requires_grad_(True)
+    y = moe.parallel_linear_fp4(xe, cd, sd, 1, sei.to(dev), ssi.to(dev), None, offs.to(dev))
+    w = oracle.weights(codes2[:1], scales2[:1], 64)[0]
+    want = (x2[:1].double() @ w.t()).expand(20, 48)
+    close(y, want, half_step(BF16) * want.abs() + 72 * 2.0 ** -24 * (x2[:1].double().abs() @ w.abs().t()), "y")
+    dx, = torch.autograd.grad(y, xe, torch.ones((), dtype=BF16, device=dev).expand(20, 48))   # a gradient of no strides
+    want = w.sum(0).expand(20, 64)
+    close(dx, want, half_step(BF16) * want.abs() + 56 * 2.0 ** -24 * w.abs().sum(0), "dx")
+
+
+def device_inputs(dev, T=40, K=256, N=192, E=4, k=2, dtype=BF16):
+    x, codes, scales, (sei, ssi, offs, gw), g = make(T, K, N, E, k, dtype)
+    return x.to(dev), gw.to(dev, dtype), (codes.to(dev), scales.to(dev), k, sei.to(dev), ssi.to(dev), None, offs.to(dev))
+
+
+def test_backward_runs_again_for_either_input_and_through_hooks(dev):
+    x, gw, args = device_inputs(dev)
+    a, b = x.requires_grad_(True), gw.requires_grad_(True)
+    y = moe.parallel_linear_fp4(a, *args, b)
+    dout = torch.randn_like(y)
+    want = torch.autograd.grad(y, (a, b), dout, retain_graph=True)
+    assert all(torch.equal(u, v) for u, v in zip(torch.autograd.grad(y, (a, b), dout), want))
+    for i, (u, v) in enumerate(((a, b.detach()), (a.detach(), b))):
+        assert torch.equal(torch.autograd.grad(moe.parallel_linear_fp4(u, *args, v), (a, b)[i], dout)[0], want[i])
+    # what is saved may come back with other strides, at another address
+    pack = lambda t: t.cpu()
+    unpack = lambda t: torch.stack((t, t), -1).to(dev)[..., 0]
+    with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+        y = moe.parallel_linear_fp4(a, *args, b)
+    assert all(torch.equal(u, v) for u, v in zip(torch.autograd.grad(y, (a, b), dout), want))
+    # codes that change between the passes are noticed
+    args = (args[0].clone(), *args[1:])
+    y = moe.parallel_linear_fp4(a, *args, b)
+    args[0].zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        torch.autograd.grad(y, a, dout)
+
+
+@pytest.mark.parametrize("T,dtype", [(3, BF16), (40, F16), (300, BF16), (20, F32)])
+def test_a_training_step_in_a_graph(dev, T, dtype):
+    x, gw, args = device_inputs(dev, T=T, K=264, N=200, dtype=dtype)
+    leaves = [x.requires_grad_(True), gw.requires_grad_(True)]
+    dout = torch.randn(T, 200, generator=torch.Generator().manual_seed(1)).to(dev, dtype)
+
+    def step():
+        for t in leaves:
+            t.grad = None
+        y = moe.parallel_linear_fp4(x, *args, gw)
+        y.backward(dout)
+        return y.detach()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = step()
+    captured = [y] + [t.grad for t in leaves]
+    for trial in range(4):
+        with torch.no_grad():
+            x.copy_(torch.randn(x.shape, generator=torch.Generator().manual_seed(trial)).to(dtype))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in captured]
+        want = [step()] + [t.grad for t in leaves]
+        assert all(torch.equal(u, v) for u, v in zip(got, want)), trial
+
+
+def test_two_streams_at_once(dev):
+    sets = [device_inputs(dev, T=T, K=K) for T, K in ((5, 512), (300, 256), (40, 264), (1, 1024))]
+    want = [moe.parallel_linear_fp4(x, *a, g) for x, g, a in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(3):
+        got = []
+        for s, (x, g, a) in zip(streams, sets):
+            with torch.cuda.stream(s):
+                got.append(moe.parallel_linear_fp4(x, *a, g))
+        torch.cuda.synchronize()
+        assert all(torch.equal(u, v) for u, v in zip(got, want))
+
+
+def test_without_autograd_traced_and_in_inference_mode(dev):
+    x, gw, args = device_inputs(dev, T=7)
+    want = moe.parallel_linear_fp4(x, *args, gw)
+    with torch.inference_mode():
+        assert torch.equal(moe.parallel_linear_fp4(x.clone(), *args, gw), want)
+    traced = torch.jit.trace(lambda v: moe.parallel_linear_fp4(v, *args, gw), (x,), check_trace=False)
+    assert torch.equal(traced(x * 1), want)

@@ -144,3 +144,62 @@ def test_what_is_kept_is_small(dev):
     held = torch.cuda.memory_allocated() - before - y.numel() * 2
     assert held <= 2 * rows * cols * 1.0625 + 4096
     assert _lib.lib.moe_swiglu8_kept_bytes(rows, cols) <= 2 * rows * cols * 1.0625 + 1024
+
+
+def test_backward_again_alone_and_through_hooks(dev):
+    gate, up, dh = (t.to(dev) for t in draw(40, 200, BF16, 5))
+    a, b = gate.requires_grad_(True), up.requires_grad_(True)
+    y = moe.swiglu_8bit(a, b)
+    want = torch.autograd.grad(y, (a, b), dh, retain_graph=True)
+    assert all(torch.equal(u, v) for u, v in zip(torch.autograd.grad(y, (a, b), dh), want))
+    for i, (u, v) in enumerate(((a, b.detach()), (a.detach(), b))):
+        assert torch.equal(torch.autograd.grad(moe.swiglu_8bit(u, v), (a, b)[i], dh)[0], want[i])
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: torch.stack((t, t), -1).to(dev)[..., 0]):
+        y = moe.swiglu_8bit(a, b)
+    assert all(torch.equal(u, v) for u, v in zip(torch.autograd.grad(y, (a, b), dh), want))
+    # one tensor twice, and a gradient without strides
+    y = moe.swiglu_8bit(a, a)
+    ga, = torch.autograd.grad(y, a, torch.ones((), dtype=BF16, device=dev).expand(40, 200))
+    one = torch.autograd.grad(moe.swiglu_8bit(a, gate.detach().clone().requires_grad_(True)), a, torch.ones_like(y))[0]
+    two = torch.autograd.grad(moe.swiglu_8bit(a.detach(), a), a, torch.ones_like(y))[0]
+    assert torch.equal(ga, one + two)
+
+
+def test_steps_in_graphs_between_eager_ones_and_on_two_streams(dev):
+    sets = [[t.to(dev) for t in draw(*s, BF16, 7)] for s in ((300, 512), (33, 200))]
+    leaves = [[t.requires_grad_(True) for t in s[:2]] for s in sets]
+
+    def step(i):
+        for t in leaves[i]:
+            t.grad = None
+        moe.swiglu_8bit(*leaves[i]).backward(sets[i][2])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for i in (0, 1, 0, 1):
+            step(i)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, grads, pool = [], [], None
+    for i in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], pool=pool):
+            step(i)
+        pool = pool or graphs[0].pool()
+        grads.append([t.grad for t in leaves[i]])
+    for trial, i in enumerate((0, 1, 1, 0, 0)):
+        with torch.no_grad():
+            leaves[i][0].copy_(torch.randn(leaves[i][0].shape, generator=torch.Generator().manual_seed(trial)).to(BF16))
+        graphs[i].replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in grads[i]]
+        step(i)
+        assert all(torch.equal(u, t.grad) for u, t in zip(got, leaves[i])), trial
+    want = [[t.grad.clone() for t in leaves[i]] for i in range(2) if step(i) is None]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for i, s in enumerate(streams):
+        with torch.cuda.stream(s):
+            got.append(torch.autograd.grad(moe.swiglu_8bit(*leaves[i]), leaves[i], sets[i][2]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(u, v) for g, w in zip(got, want) for u, v in zip(g, w))
