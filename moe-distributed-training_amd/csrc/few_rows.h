@@ -92,7 +92,7 @@ __device__ __forceinline__ void from_lines(fp4_u32x4_t (&v)[2], uint8_t* scratch
 // ... loaded side by side: units of 256 inputs, scales in 8-byte pieces.  NB 1, 2 or 4: lane l brings the eight scales of column l of a matrix's blocks.
 template <class Num_, int NB_, bool TWO> struct Fp4Quads {
     typedef Num_ Num;
-    static constexpr int NB = NB_, UNIT = 2, SCRATCH = NB * 2048 + NB * 128, MATS = TWO ? 2 : 1, EACH = 16 * NB / MATS;
+    static constexpr int NB = NB_, UNIT = 2, SCRATCH = 2048 + NB * 128, MATS = TWO ? 2 : 1, EACH = 16 * NB / MATS;
     Buffer codes[2], scales[2];
     uint32_t c[NB][2], s[MATS];
     struct Stage { fp4_u32x4_t c[NB][2]; uint32_t s[NB][2]; };
@@ -126,8 +126,8 @@ template <class Num_, int NB_, bool TWO> struct Fp4Quads {
     {
         const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) from_lines(t.c[nb], scratch + nb * 2048);
-        uint2* sc = (uint2*)(scratch + NB * 2048);
+        for (int nb = 0; nb < NB; ++nb) from_lines(t.c[nb], scratch);   // (the same 2 KiB for every block: a wave's accesses to LDS happen in order)
+        uint2* sc = (uint2*)(scratch + 2048);
 #pragma unroll
         for (int m = 0; m < MATS; ++m)
             if (lane < EACH) sc[m * EACH + lane] = make_uint2(t.s[m][0], t.s[m][1]);

@@ -125,13 +125,15 @@ template <class Num, int NB> int launch_few_typed(MoeFp4Gemm p, int64_t tiles, i
 
 template <class Num> int launch_few(const MoeFp4Gemm& p, int64_t R, hipStream_t stream)
 {
-    const int64_t most = R / 16 + p.E, tiles = most < R ? most : R;   // (a tile holds a row at least)
+    const int64_t most = R / 16 + p.E, tiles = most < R ? most : R, used = p.E < R ? p.E : R;   // (a tile holds a row at least)
     const int chunks = (p.K + few::CHUNK - 1) / few::CHUNK, cus = moe_device_cus();
-    // waves that share a contraction: as many as it has pairs of chunks, until the chip has twelve waves per compute unit
     const bool narrow = tiles * ((p.N + 63) / 64) < cus;   // few column blocks: blocks of 16 columns give every compute unit one
-    const int64_t groups = tiles * (narrow ? (p.N + 15) / 16 : (p.N + 63) / 64);
+    // Waves that share a contraction: as many as the chip holds at once (by their registers, below; tiles as many as evenly spread rows fill, half of them partly), two chunks each at least.  One
+    // token of 4096 x 14336, 448 workgroups: 1 / 2 / 4 / 8 waves 25 / 19 / 15 / 20 us, the last in two rounds; 16 of one expert each 50 / 54 / 52 / 70; 666 rows of 1000 x 1368 17.2 / 17.2 / 19.9 / 27.
+    const int64_t expected = R / 16 + used / 2, groups = (expected > used ? expected : used) * (narrow ? (p.N + 15) / 16 : (p.N + 63) / 64);
+    const int64_t resident = (int64_t)cus * (narrow ? (p.quads ? 16 : 20) : p.quads ? 8 : 12);
     int waves = 1;
-    while (waves < 8 && groups * waves < 12 * (int64_t)cus && chunks >= 2 * waves) waves *= 2;
+    while (waves < 8 && groups * waves * 2 <= resident && chunks >= 2 * waves) waves *= 2;
     return narrow ? launch_few_typed<Num, 1>(p, tiles, waves, stream) : launch_few_typed<Num, 4>(p, tiles, waves, stream);
 }
 
