@@ -204,7 +204,8 @@ template <class Num> __device__ __forceinline__ void route(const MoeDecode& p, C
 
 // ... and where it is, in the order of W's pieces: the waves of a group of `split` share a block's inputs, groups take different blocks, and the router's rows of the next block are on
 // their way while one is summed.  (Loaded as rows of x are: 16 experts x 256 bytes.)
-template <class W> __device__ __forceinline__ void route_kept(const MoeDecode& p, Chosen& c, float* red, int stride, float* logits, const few::Rows<1>::Stage (&xs)[4], uint8_t* scratch)
+// xs: this wave's chunks of x, loaded on entry and in the operand's order on return.
+template <class W> __device__ __forceinline__ void route_kept(const MoeDecode& p, Chosen& c, float* red, int stride, float* logits, few::Rows<1>::Stage (&xs)[4], uint8_t* scratch)
 {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, q = lane >> 4;
     const int group = wave / p.split, groups = WAVES / p.split, c0 = (wave & (p.split - 1)) * 4, nblocks = (p.E + 15) / 16;
@@ -236,6 +237,9 @@ template <class W> __device__ __forceinline__ void route_kept(const MoeDecode& p
     };
     fetch(0, group);
     if (groups < nblocks) fetch(1, groups + group);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int d = 0; d < 4; ++d) few::Rows<1>().template ready<W>(xs[d], scratch);
     for (int eb0 = 0; eb0 < nblocks; eb0 += 2 * groups) {
         block(0, eb0);
         if (eb0 + 2 * groups < nblocks) fetch(0, eb0 + 2 * groups + group);
@@ -332,8 +336,6 @@ __global__ void __launch_bounds__(THREADS, 2) gate_up_kernel(const MoeDecode p)
     if constexpr (KEPT) {
 #pragma unroll
         for (int d = 0; d < 4; ++d) rows.load(xs[d], c0 + d);
-#pragma unroll
-        for (int d = 0; d < 4; ++d) rows.template ready<W>(xs[d], scratch);
         route_kept<W>(p, c, &red[0][0][0][0][0], 256, logits, xs, scratch);
     } else route<Num>(p, c, &red[0][0][0][0][0], logits, scratch);
     store_choices(p, c);
@@ -420,8 +422,6 @@ __global__ void __launch_bounds__(THREADS, 2) gate_up_fp4_kernel(const MoeDecode
     few::Rows<1>::Stage xs[4];
 #pragma unroll
     for (int d = 0; d < 4; ++d) rows.load(xs[d], c0 + d);
-#pragma unroll
-    for (int d = 0; d < 4; ++d) rows.template ready<W>(xs[d], area);
     // (the router's sums lie behind every wave's scratch, its logits where a job's sums will be)
     static_assert(TOK * MAXE * 4 <= WAVES * 2 * 1024 && few::Rows<1>::SCRATCH + 1024 <= FP4_WAVE_LDS, "");
     route_kept<W>(p, c, (float*)(smem + few::Rows<1>::SCRATCH), FP4_WAVE_LDS / 4, red, xs, area);
@@ -530,7 +530,9 @@ __global__ void __launch_bounds__(THREADS) down_kernel(const MoeDecode p)
     __shared__ int arrival;
     float* red = (float*)smem;   // [wave][unit][64][PER]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, q = lane >> 4;
-    const int tile = blockIdx.x / p.parts, part = blockIdx.x - tile * p.parts;
+    // (tiles side by side, so that an XCD has every row of a few tiles: with a few rows of every tile each, columns 256 bytes apart in rows of 8 KiB came out of its L2 at two speeds, 34 and 49 us of
+    // one token's 53 of 4096 x 14336 in 16 bits; now 34 to 41)
+    const int tiles = gridDim.x / p.parts, part = blockIdx.x / tiles, tile = blockIdx.x - part * tiles;
     static_assert(THREADS >= TOK * MAXK, "a thread per choice");
     const int x = threadIdx.x;
     const int choice = x < p.T * p.k ? p.indices[x] : 0;
@@ -684,13 +686,20 @@ __global__ void __launch_bounds__(THREADS) down_kernel(const MoeDecode p)
         if (live) {
 #pragma unroll
             for (int v = 0; v < PER; ++v) sum[v] = 0.f;
-            for (int x = 0; x < p.parts; ++x)
+            // (eight parts' sums are requested together: one after the other they cost a trip to memory each, 3 us with four parts)
+            constexpr int BATCH = 8;
+            for (int x0 = 0; x0 < p.parts; x0 += BATCH) {
+                f32x4_t s[BATCH][PER / 4];
 #pragma unroll
-                for (int v = 0; v < PER; v += 4) {
-                    const f32x4_t s = __builtin_bit_cast(f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(slots, slot(x) + 4 * v, 0, DEVICE_SCOPE));
+                for (int b = 0; b < BATCH; ++b)
 #pragma unroll
-                    for (int y = 0; y < 4; ++y) sum[v + y] += s[y];
-                }
+                    for (int v = 0; v < PER / 4; ++v)
+                        s[b][v] = __builtin_bit_cast(f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(slots, x0 + b < p.parts ? slot(x0 + b) + 16 * v : few::RANGE, 0, DEVICE_SCOPE));
+#pragma unroll
+                for (int b = 0; b < BATCH; ++b)
+#pragma unroll
+                    for (int v = 0; v < PER; ++v) sum[v] += s[b][v / 4][v % 4];
+            }
         }
     }
     if (!live) return;
@@ -716,10 +725,12 @@ Plan plan(int T, int E, int d, int f, int k, bool fp4)
     const int64_t at_once = r.split ? WAVES / r.split : 1, groups = (jobs + at_once - 1) / at_once;
     r.grid1 = (int)(groups < cus ? groups : cus);
     r.tiles = fp4 ? d / 64 : (d + 127) / 128;
-    // parts of launch 2: until every compute unit has one, as long as its waves have two steps each
+    // parts of launch 2, one workgroup per compute unit at a time: as few as come near the least time in rounds, as long as their waves have two steps each
     const int64_t steps = (int64_t)(E < T * k ? E : T * k) * (fp4 ? chunks_of(f) : f / 32);
+    auto time = [&](int parts) { return (double)((r.tiles * (int64_t)parts + cus - 1) / cus) / parts; };
     r.parts = 1;
-    while (r.parts < DOWN_PARTS_MAX && r.tiles * r.parts < cus && steps >= r.parts * 2 * WAVES * 2) r.parts *= 2;
+    for (int parts = 2; parts <= DOWN_PARTS_MAX && steps >= (int64_t)parts * 2 * WAVES; ++parts)
+        if (time(parts) < 0.9 * time(r.parts)) r.parts = parts;
     auto al = [](size_t n) { return (n + 255) & ~(size_t)255; };
     r.h_bytes = al((size_t)T * k * f * 2);
     r.counter_bytes = al((size_t)r.tiles * 4);
