@@ -316,13 +316,13 @@ int moe_fp4_quantize_weights(const void* W, int64_t swe, int64_t swk, int64_t sw
 /* moe_scatter2scatter without adapters over 4-bit weights: y[out_row] = x[in_row] @ W[e], rows addressed as there; x has x_rows rows, of `dtype`, y of y_dtype (fp32 x: fp32).  Weights
  * enter as numbers of x's type: exact in bf16 and fp32; in fp16 for scales from 104 to 140, beyond which they round (or overflow) as a conversion to fp16 does.
  * Backward (weights frozen): row m of the order is dY's row m (dy_grouped) or pos[m] / dy_fan_out of dy_rows;  dx_rows[dx_grouped ? m : pos[m]] = c dY[row] @ W[e]^T, c = gates[pos[m]]
- * (`gates` NULL: 1; not with dy_grouped; `weighted` of the query: whether there are any).  Rows that no group covers are not written.  One expert's codes, and 128 rows, below 2 GiB. */
+ * (`gates` NULL: 1; not with dy_grouped).  Rows that no group covers are not written.  16-bit rows: one expert's codes, and 128 rows, below 2 GiB. */
 size_t moe_linear_fp4_workspace_bytes(const void* x, int64_t ldx, int64_t x_rows, int x_grouped, int dtype, const uint8_t* scales, int64_t sse, int64_t ssn, int64_t R, int E,
                                       int64_t K, int64_t N);
 int moe_linear_fp4_fwd(const void* x, int64_t ldx, int64_t x_rows, int dtype, const uint8_t* codes, int64_t sce, int64_t scn, const uint8_t* scales, int64_t sse, int64_t ssn,
                        void* y, int64_t ldy, int y_dtype, const void* pos, int pos64, const void* offsets, int off64, int E, int64_t R, int64_t K, int64_t N, int fan_out,
                        int x_grouped, int y_grouped, void* workspace, size_t workspace_bytes, void* stream);
-size_t moe_linear_fp4_bwd_workspace_bytes(const void* dy, int64_t lddy, int64_t dy_rows, int dy_grouped, int weighted, int dtype, const uint8_t* scales, int64_t sse, int64_t ssn,
+size_t moe_linear_fp4_bwd_workspace_bytes(const void* dy, int64_t lddy, int64_t dy_rows, int dy_grouped, int dtype, const uint8_t* scales, int64_t sse, int64_t ssn,
                                           int64_t R, int E, int64_t K, int64_t N);
 int moe_linear_fp4_bwd(const void* dy, int64_t lddy, int64_t dy_rows, int dtype, int dy_grouped, int dy_fan_out, const void* gates, int gates_dtype, const uint8_t* codes,
                        int64_t sce, int64_t scn, const uint8_t* scales, int64_t sse, int64_t ssn, void* dx_rows, int64_t lddx, int dx_dtype, int dx_grouped, const void* pos, int pos64,

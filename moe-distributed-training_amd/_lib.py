@@ -76,7 +76,7 @@ _SIGNATURES = {
     "moe_mlp_int8_fwd": ("i", "plli" + "pppppp" + "pli" + "pi" + "pi" + "i" + "lll" + "ii" + "pz" + "pzp"),
     "moe_fp4_quantize_weights": ("i", "plll" + "iill" + "pll" + "pll" + "p"),
     "moe_linear_fp4_workspace_bytes": ("z", "plli" + "i" + "pll" + "lill"),
-    "moe_linear_fp4_bwd_workspace_bytes": ("z", "plli" + "ii" + "pll" + "lill"),
+    "moe_linear_fp4_bwd_workspace_bytes": ("z", "plli" + "i" + "pll" + "lill"),
     "moe_linear_fp4_fwd": ("i", "plli" + "pll" + "pll" + "pli" + "pi" + "pi" + "i" + "lll" + "iii" + "pzp"),
     "moe_linear_fp4_bwd": ("i", "plliii" + "pi" + "pll" + "pll" + "plii" + "pi" + "pi" + "i" + "lll" + "pzp"),
     "moe_swiglu8_kept_bytes": ("z", "ll"),

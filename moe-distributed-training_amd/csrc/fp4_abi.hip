@@ -10,7 +10,6 @@ inline hipStream_t S(void* s) { return (hipStream_t)s; }
 inline size_t al(size_t n) { return (n + 255) & ~(size_t)255; }
 inline bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
 inline int64_t groups_of(int64_t K) { return (K + 31) / 32; }
-inline size_t elem_bytes(int dtype) { return dtype == MOE_F32 ? 4 : 2; }
 #define TRY(call) do { const int rc_ = (call); if (rc_ != MOE_OK) return rc_; } while (0)
 
 // rows of codes that 16-byte loads take, and scales that lie one after the other
@@ -25,7 +24,6 @@ int64_t packed_cols(int64_t n) { return (n + 7) / 8 * 8; }
 // scales that 4-byte loads take as they are; otherwise rows of whole fours are made of them
 bool scales_ok(const uint8_t* scales, int64_t sse, int64_t ssn, int64_t G) { return (uintptr_t)scales % 4 == 0 && sse % 4 == 0 && ssn % 4 == 0 && G % 4 == 0; }
 int64_t packed_groups(int64_t G) { return (G + 3) / 4 * 4; }
-size_t expanded_bytes(int E, int64_t K, int64_t N, int dtype) { return al((size_t)E * (size_t)N * (size_t)K * elem_bytes(dtype)); }
 
 // What a 16-bit product copies into its workspace before it starts: rows (len columns) and scales.
 struct Fp4Copies {
@@ -124,8 +122,7 @@ int moe_fp4_quantize_weights(const void* W, int64_t swe, int64_t swk, int64_t sw
 size_t moe_linear_fp4_workspace_bytes(const void* x, int64_t ldx, int64_t x_rows, int x_grouped, int dtype, const uint8_t* scales, int64_t sse, int64_t ssn, int64_t R, int E, int64_t K,
                                       int64_t N)
 {
-    if (dtype < 0 || dtype > 2 || R < 1 || E < 1 || K < 1 || N < 1) return 0;
-    if (dtype == MOE_F32) return expanded_bytes(E, K, N, dtype) + moe_scatter2scatter_workspace_bytes(R, E, K, N, 0);
+    if (dtype < 0 || dtype > 2 || dtype == MOE_F32 || R < 1 || E < 1 || K < 1 || N < 1) return 0;
     const Fp4Copies c(x, ldx, x_rows, x_grouped, scales, sse, ssn, R, E, K, N, K);
     return c.rows + c.scales;
 }
@@ -141,29 +138,21 @@ int moe_linear_fp4_fwd(const void* x, int64_t ldx, int64_t x_rows, int dtype, co
     if (!x || x_rows < 1 || !weights_ok(w) || !y || !offsets || ((!x_grouped || !y_grouped) && !pos) || (x_grouped && x_rows < R) || !aligned16(workspace)) return MOE_ERR_BAD_ARG;
     const size_t need = moe_linear_fp4_workspace_bytes(x, ldx, x_rows, x_grouped, dtype, scales, sse, ssn, R, E, K, N);
     if (need && (!workspace || workspace_bytes < need)) return MOE_ERR_WORKSPACE;
-    if (dtype == MOE_F32) {
-        if (y_dtype != MOE_F32) return MOE_ERR_UNSUPPORTED;
-        const size_t wb = expanded_bytes(E, K, N, dtype);
-        TRY(moe_launch_fp4_expand(codes, sce, scn, scales, sse, ssn, E, K, N, workspace, dtype, S(stream)));
-        return moe_scatter2scatter(x, ldx, 1, workspace, N * K, 1, K, nullptr, 0, 0, 0, nullptr, 0, 0, 0, 0, 0.f, y, ldy, 1, pos, pos64, offsets, off64, E, R, K, N, fan_out, x_grouped,
-                                   y_grouped, dtype, (uint8_t*)workspace + wb, workspace_bytes - wb, stream);
-    }
-    if (!fp4_sizes_ok(K, N, E, scn, ssn)) return MOE_ERR_UNSUPPORTED;
+    if (dtype == MOE_F32 ? y_dtype != MOE_F32 || K > 0x3fffffff : !fp4_sizes_ok(K, N, E, scn, ssn)) return MOE_ERR_UNSUPPORTED;
     MoeFp4Gemm g = {};
     g.X = x; g.ldx = ldx; g.w = w; g.Y = y; g.ldy = ldy; g.ydtype = y_dtype; g.pos = pos; g.pos64 = pos64; g.offsets = offsets; g.off64 = off64;
     g.E = E; g.K = (int)K; g.N = N; g.fan_out = fan_out; g.x_grouped = x_grouped; g.y_grouped = y_grouped; g.f16 = dtype == MOE_F16;
+    if (dtype == MOE_F32) return moe_launch_fp4_f32(g, R, false, S(stream));
     const Fp4Copies c(x, ldx, x_rows, x_grouped, scales, sse, ssn, R, E, K, N, K);
     TRY(c.make(g, R, K, (uint8_t*)workspace, S(stream)));
     if (c.rows) g.K = (int)packed_cols(K);   // (the same groups of weights; the rows have zeros there)
     return fp4_few_rows(R, E, g.K, N) ? moe_launch_fp4_few_rows(g, R, S(stream)) : moe_launch_fp4_tiles(g, R, false, S(stream));
 }
 
-size_t moe_linear_fp4_bwd_workspace_bytes(const void* dy, int64_t lddy, int64_t dy_rows, int dy_grouped, int weighted, int dtype, const uint8_t* scales, int64_t sse, int64_t ssn, int64_t R,
+size_t moe_linear_fp4_bwd_workspace_bytes(const void* dy, int64_t lddy, int64_t dy_rows, int dy_grouped, int dtype, const uint8_t* scales, int64_t sse, int64_t ssn, int64_t R,
                                           int E, int64_t K, int64_t N)
 {
-    if (dtype < 0 || dtype > 2 || R < 1 || E < 1 || K < 1 || N < 1) return 0;
-    if (dtype == MOE_F32)
-        return expanded_bytes(E, K, N, dtype) + (dy_grouped && !weighted ? 0 : al((size_t)R * (size_t)N * 4)) + moe_scatter2scatter_workspace_bytes(R, E, N, K, 0);
+    if (dtype < 0 || dtype > 2 || dtype == MOE_F32 || R < 1 || E < 1 || K < 1 || N < 1) return 0;
     const Fp4Copies c(dy, lddy, dy_rows, dy_grouped, scales, sse, ssn, R, E, K, N, N);
     return c.rows + c.scales;
 }
@@ -177,28 +166,14 @@ int moe_linear_fp4_bwd(const void* dy, int64_t lddy, int64_t dy_rows, int dtype,
     const MoeFp4Weights w = {codes, sce, scn, scales, sse, ssn};
     if (lddy < 0 || (R > 1 && lddx < K) || !dy || dy_rows < 1 || !weights_ok(w) || !dx_rows || !offsets || ((!dy_grouped || !dx_grouped) && !pos) || (dy_grouped && dy_rows < R) ||
         !aligned16(workspace)) return MOE_ERR_BAD_ARG;
-    const size_t need = moe_linear_fp4_bwd_workspace_bytes(dy, lddy, dy_rows, dy_grouped, gates != nullptr, dtype, scales, sse, ssn, R, E, K, N);
+    const size_t need = moe_linear_fp4_bwd_workspace_bytes(dy, lddy, dy_rows, dy_grouped, dtype, scales, sse, ssn, R, E, K, N);
     if (need && (!workspace || workspace_bytes < need)) return MOE_ERR_WORKSPACE;
-    if (dtype == MOE_F32) {
-        if (dx_dtype != MOE_F32) return MOE_ERR_UNSUPPORTED;
-        size_t used = expanded_bytes(E, K, N, dtype);
-        TRY(moe_launch_fp4_expand(codes, sce, scn, scales, sse, ssn, E, K, N, workspace, dtype, S(stream)));
-        const void* rows = dy;
-        int64_t ld = lddy;
-        if (!dy_grouped) {
-            rows = (uint8_t*)workspace + used;
-            ld = N;
-            used += al((size_t)R * (size_t)N * 4);
-            TRY(moe_group_rows(dy, lddy, (void*)rows, N, pos, pos64, dy_fan_out, gates, gates_dtype, R, N, dtype, stream));
-        }
-        return moe_scatter2scatter(rows, ld, 1, workspace, N * K, K, 1, nullptr, 0, 0, 0, nullptr, 0, 0, 0, 0, 0.f, dx_rows, lddx, 1, pos, pos64, offsets, off64, E, R, N, K, 1, 1,
-                                   dx_grouped, dtype, (uint8_t*)workspace + used, workspace_bytes - used, stream);
-    }
-    if (!fp4_sizes_ok(K, N, E, scn, ssn)) return MOE_ERR_UNSUPPORTED;
+    if (dtype == MOE_F32 ? dx_dtype != MOE_F32 || K > 0x3fffffff : !fp4_sizes_ok(K, N, E, scn, ssn)) return MOE_ERR_UNSUPPORTED;
     MoeFp4Gemm g = {};
     g.X = dy; g.ldx = lddy; g.w = w; g.Y = dx_rows; g.ldy = lddx; g.ydtype = dx_dtype; g.pos = pos; g.pos64 = pos64; g.offsets = offsets; g.off64 = off64;
     g.E = E; g.K = (int)K; g.N = N; g.fan_out = dy_fan_out; g.x_grouped = dy_grouped; g.y_grouped = dx_grouped; g.f16 = dtype == MOE_F16;
     g.gates = gates; g.gates_dtype = gates_dtype;
+    if (dtype == MOE_F32) return moe_launch_fp4_f32(g, R, true, S(stream));
     const Fp4Copies c(dy, lddy, dy_rows, dy_grouped, scales, sse, ssn, R, E, K, N, N);
     TRY(c.make(g, R, N, (uint8_t*)workspace, S(stream)));
     return moe_launch_fp4_tiles(g, R, true, S(stream));

@@ -1,5 +1,4 @@
-// Weights of 16 or 32 bits into 4-bit codes with a scale per 32 inputs, and back (fp4.h).  Done once per weight, or, by products that the matrix cores do not take in
-// 4 bits (fp32), once per call.
+// Weights of 16 or 32 bits into 4-bit codes with a scale per 32 inputs (fp4.h), once per weight; and copies of rows and scales that the 16-bit products do not take as they lie.
 #include "fp4.h"
 #include "kernels.h"
 
@@ -52,31 +51,6 @@ __global__ void __launch_bounds__(256) fp4_quantize_kernel(const T* W, int64_t s
     scales[e * sse + n * ssn + g] = fine ? (uint8_t)(p + 127) : 255;
 }
 
-// codes -> (E, N, K) weights of T, rows of K one after the other; a thread per group
-template <typename T>
-__global__ void __launch_bounds__(256) fp4_expand_kernel(const uint8_t* codes, int64_t sce, int64_t scn, const uint8_t* scales, int64_t sse, int64_t ssn, int64_t K, int64_t N,
-                                                         int64_t G, int64_t total, T* out)
-{
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= total) return;
-    const int64_t e = i / (N * G), j = i - e * N * G, n = j / G, g = j % G;
-    const fp4_u32x4_t c = *(const fp4_u32x4_t*)(codes + e * sce + n * scn + g * FP4_GROUP_BYTES);
-    const float s = fp4_scale(scales[e * sse + n * ssn + g]);
-    T* to = out + (e * N + n) * K + g * FP4_GROUP;
-    const int live = K - g * FP4_GROUP < FP4_GROUP ? (int)(K - g * FP4_GROUP) : FP4_GROUP;
-    auto put = [&](int k, float2 v) {
-        if (k < live) Elem<T>::st(to + k, v.x);
-        if (k + 1 < live) Elem<T>::st(to + k + 1, v.y);
-    };
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        put(8 * w, fp4_pair_f32<0>(c[w], s));
-        put(8 * w + 2, fp4_pair_f32<1>(c[w], s));
-        put(8 * w + 4, fp4_pair_f32<2>(c[w], s));
-        put(8 * w + 6, fp4_pair_f32<3>(c[w], s));
-    }
-}
-
 // Rows that 16-byte loads do not take, in the order of the product and padded to whole pieces.  (Rows behind the last group are left alone: their positions may be anything.)
 __global__ void __launch_bounds__(256) fp4_pack_rows_kernel(const uint16_t* X, int64_t ldx, const void* pos, int pos64, int fan_out, const void* offsets, int off64, int E, int64_t K,
                                                             uint16_t* out, int64_t ldo)
@@ -122,15 +96,5 @@ int moe_launch_fp4_quantize(const void* W, int64_t swe, int64_t swk, int64_t swn
     if (!moe_grid_fits((total + 255) / 256, 256)) return MOE_ERR_UNSUPPORTED;
     MOE_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL((fp4_quantize_kernel<T>), dim3((unsigned)((total + 255) / 256)), dim3(256), 0, stream, (const T*)W, swe, swk, swn, K, N, G, total,
                                                  swn < swk, codes, sce, scn, scales, sse, ssn));
-    return moe_launch_status();
-}
-
-int moe_launch_fp4_expand(const uint8_t* codes, int64_t sce, int64_t scn, const uint8_t* scales, int64_t sse, int64_t ssn, int E, int64_t K, int64_t N, void* out, int dtype,
-                          hipStream_t stream)
-{
-    const int64_t G = (K + FP4_GROUP - 1) / FP4_GROUP, total = E * N * G;
-    if (!moe_grid_fits((total + 255) / 256, 256)) return MOE_ERR_UNSUPPORTED;
-    MOE_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL((fp4_expand_kernel<T>), dim3((unsigned)((total + 255) / 256)), dim3(256), 0, stream, codes, sce, scn, scales, sse, ssn, K, N, G, total,
-                                                 (T*)out));
     return moe_launch_status();
 }

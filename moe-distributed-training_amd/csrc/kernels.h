@@ -301,7 +301,7 @@ struct MoeFp4Weights {                  // codes (E, N, ceil(K/32) * 16 bytes), 
     const uint8_t* scales; int64_t sse, ssn;
 };
 struct MoeFp4Gemm {
-    const void* X; int64_t ldx;         // 16-bit rows of K values, a multiple of 8, at multiples of 16 bytes
+    const void* X; int64_t ldx;         // rows of K values (16 bits: a multiple of 8, at multiples of 16 bytes)
     MoeFp4Weights w;
     void* Y; int64_t ldy; int ydtype;
     const void* pos; int pos64; const void* offsets; int off64;
@@ -312,12 +312,13 @@ struct MoeFp4Gemm {
     int quads;                          // weights can be loaded side by side (few_rows.h)
     int num_cus;                        // workgroups of a round of the tile plan
     int64_t col_blocks;
-    int y_vec;                          // Y takes stores of four values
+    int x_vec, y_vec;                   // X takes loads, Y stores of four values
 };
 constexpr int64_t MOE_FP4_RANGE = (int64_t)1 << 31;   // bytes of one expert's codes, and of gathered rows, that 32-bit offsets reach
 // (scales of either start at multiples of 4 bytes, in rows of whole fours)
 int moe_launch_fp4_few_rows(MoeFp4Gemm p, int64_t R, hipStream_t stream);
 int moe_launch_fp4_tiles(MoeFp4Gemm p, int64_t R, bool backward, hipStream_t stream);
+int moe_launch_fp4_f32(MoeFp4Gemm p, int64_t R, bool backward, hipStream_t stream);
 // scales (E, N, G) of any strides into rows of ldo, zeros behind G
 int moe_launch_fp4_pack_scales(const uint8_t* scales, int64_t sse, int64_t ssn, int E, int64_t N, int64_t G, uint8_t* out, int64_t ldo, hipStream_t stream);
 // rows of X (row m of the order: m, or pos[m] / fan_out), K of ld columns of a 16-bit type, into rows one after the other of pitch ldo, zeros behind K
@@ -325,8 +326,6 @@ int moe_launch_fp4_pack_rows(const void* X, int64_t ldx, const void* pos, int po
                              hipStream_t stream);
 int moe_launch_fp4_quantize(const void* W, int64_t swe, int64_t swk, int64_t swn, int dtype, int E, int64_t K, int64_t N, uint8_t* codes, int64_t sce, int64_t scn, uint8_t* scales,
                             int64_t sse, int64_t ssn, hipStream_t stream);
-int moe_launch_fp4_expand(const uint8_t* codes, int64_t sce, int64_t scn, const uint8_t* scales, int64_t sse, int64_t ssn, int E, int64_t K, int64_t N, void* out, int dtype,
-                          hipStream_t stream);
 
 // ---- SwiGLU that keeps its inputs in 8 bits (swiglu8.hip) ------------------------------------------------------
 constexpr int MOE_KEPT_BLOCK = 64;      // columns that share a scale

@@ -90,7 +90,7 @@ struct LinearFp4Fn : Function<LinearFp4Fn> {
             dx = at::empty({R, K}, dout.options().dtype(rows_type(dout.scalar_type(), k != 1)));
             if (R > 0 && N > 0) {
                 const Tensor coeff = flat_gates(gates);
-                Tensor ws = bytes_on(dout, moe_linear_fp4_bwd_workspace_bytes(ptr(dout), dout.stride(0), dout.size(0), grouped_out, coeff.defined(), dtype_code(dout), w.s(),
+                Tensor ws = bytes_on(dout, moe_linear_fp4_bwd_workspace_bytes(ptr(dout), dout.stride(0), dout.size(0), grouped_out, dtype_code(dout), w.s(),
                                                                               w.scales.stride(0), w.scales.stride(1), R, (int)E, K, N));
                 check(moe_linear_fp4_bwd(ptr(dout), dout.stride(0), dout.size(0), dtype_code(dout), grouped_out, (int)gate_fan, ptr(coeff), coeff.defined() ? dtype_code(coeff) : 0, w.c(),
                                          w.codes.stride(0), w.codes.stride(1), w.s(), w.scales.stride(0), w.scales.stride(1), ptr(dx), dx.stride(0), dtype_code(dx), grouped_in, ptr(ssi),

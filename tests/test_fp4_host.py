@@ -164,6 +164,7 @@ def test_c_entries_refuse_on_the_host():
     assert fwd(R=0, x=None) == 0 and fwd(N=0, y=None) == 0
     # scales of two groups and no multiple of four are copied into rows of four: 2 experts x 128 columns x 4; nothing where both lie well
     assert lib.moe_linear_fp4_workspace_bytes(16, 64, 8, 0, 0, 16, 256, 2, 16, 2, 64, 128) == 1024 and lib.moe_linear_fp4_workspace_bytes(16, 128, 8, 0, 0, 16, 512, 4, 16, 2, 128, 128) == 0
+    assert lib.moe_linear_fp4_workspace_bytes(18, 65, 8, 0, 2, 17, 255, 2, 16, 2, 65, 128) == 0                            # fp32 takes everything as it lies
     assert fwd(n=1023) == SPACE and fwd(ws=None) == SPACE
     assert lib.moe_linear_fp4_workspace_bytes(16, 65, 8, 0, 0, 16, 512, 4, 16, 2, 128, 128) == 16 * 128 * 2 and lib.moe_linear_fp4_workspace_bytes(18, 128, 8, 0, 0, 16, 512, 4, 16, 2, 128, 128) == 16 * 128 * 2
     assert lib.moe_linear_fp4_workspace_bytes(16, 64, 8, 0, 5, 16, 256, 2, 16, 2, 64, 128) == 0 and lib.moe_linear_fp4_workspace_bytes(16, 64, 8, 0, 0, 16, 256, 2, 0, 2, 64, 128) == 0
@@ -174,8 +175,8 @@ def test_c_entries_refuse_on_the_host():
     assert all(v == BAD for v in (bwd(dy=None), bwd(ldd=-1), bwd(rows=0), bwd(dt=3), bwd(dxt=3), bwd(gates=16, gdt=3), bwd(gates=16, dg=1, rows=16), bwd(c=24), bwd(scn=8), bwd(s=None),
                                   bwd(dx=None), bwd(ldx=63), bwd(pos=None), bwd(off=None), bwd(E=0), bwd(K=0), bwd(N=0), bwd(fan=0), bwd(dg=1, rows=15), bwd(ws=8)))
     assert bwd(R=0, dy=None) == 0 and bwd(n=1023) == SPACE and bwd(ws=None) == SPACE and bwd(dt=2, dxt=0) == UNSUP
-    assert lib.moe_linear_fp4_bwd_workspace_bytes(16, 128, 8, 0, 0, 0, 16, 512, 4, 16, 2, 128, 128) == 0
-    assert lib.moe_linear_fp4_bwd_workspace_bytes(16, 130, 8, 0, 0, 0, 16, 512, 4, 16, 2, 128, 130) == 16 * 136 * 2
+    assert lib.moe_linear_fp4_bwd_workspace_bytes(16, 128, 8, 0, 0, 16, 512, 4, 16, 2, 128, 128) == 0
+    assert lib.moe_linear_fp4_bwd_workspace_bytes(16, 130, 8, 0, 0, 16, 512, 4, 16, 2, 128, 130) == 16 * 136 * 2
 
     kept = lib.moe_swiglu8_kept_bytes(3, 65)
     assert kept == 2 * (512 + 256) and lib.moe_swiglu8_kept_bytes(0, 65) == 0 and lib.moe_swiglu8_kept_bytes(3, -1) == 0   # three rows of two blocks of 64 codes, a scale each; pieces of 256

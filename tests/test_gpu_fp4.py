@@ -323,3 +323,22 @@ def test_without_autograd_traced_and_in_inference_mode(dev):
         assert torch.equal(moe.parallel_linear_fp4(x.clone(), *args, gw), want)
     traced = torch.jit.trace(lambda v: moe.parallel_linear_fp4(v, *args, gw), (x,), check_trace=False)
     assert torch.equal(traced(x * 1), want)
+
+
+@pytest.mark.parametrize("T,K,N,E,k", [(24, 1024, 640, 3, 2), (300, 1000, 136, 8, 2), (1, 2560, 200, 4, 2), (200, 72, 1032, 2, 1), (65, 33, 67, 1, 1), (700, 264, 130, 3, 2)])
+def test_larger_projections_in_fp32(dev, T, K, N, E, k):
+    check_linear(dev, T, K, N, E, k, F32)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_codes_behind_the_last_input_meet_nothing(dev, dtype):
+    """Any codes there, under scales that make them infinite in a product that read them."""
+    x, codes, scales, (sei, ssi, offs, _), g = make(9, 40, 24, 2, 1, dtype)
+    args = (1, sei.to(dev), ssi.to(dev), None, offs.to(dev))
+    want = moe.parallel_linear_fp4(x.to(dev), codes.to(dev), scales.to(dev), *args)
+    codes[..., 20:] = 0x7f
+    assert torch.equal(moe.parallel_linear_fp4(x.to(dev), codes.to(dev), scales.to(dev), *args), want)
+    if dtype == F32:
+        codes[..., 16:20], scales[..., 1] = 0, 254
+        got = moe.parallel_linear_fp4(x.to(dev), codes.to(dev), scales.to(dev), *args)
+        assert bool(torch.isfinite(got).all())
