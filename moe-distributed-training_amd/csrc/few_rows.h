@@ -9,8 +9,8 @@
 // Operands do not come from memory in that order: the memory pipeline takes four neighbouring lanes at a time, and neighbours here belong to different columns, so a 1 KiB load of 16 columns
 // x 64 bytes occupies it for 65 cycles, against 21 where four neighbours read one column's 64 bytes, 18 for eight columns x 128 bytes, and 17 for whole kilobytes (and for nothing at all).  And a
 // 64-byte piece is half a cache line: the other half, asked for a chunk later, came from memory a second time (W2 of eight experts, 249 MB: 432 MB fetched, 106 us for 16 tokens).  So lanes load
-// whole lines side by side, and an operand passes through a piece of LDS of its wave's own (no barrier) on its way into the matrix instructions.  Where a shape does not allow it (inputs that
-// are no multiple of 256, or scales that 4-byte loads do not take), 4-bit weights are loaded in the operand's order.
+// whole lines side by side, and an operand passes through a piece of LDS of its wave's own (no barrier) on its way into the matrix instructions.  Where a shape does not allow it (groups
+// of inputs that are no multiple of eight), 4-bit weights are loaded in the operand's order.
 //
 // All loads are buffer loads at 32-bit offsets; what does not exist (rows, inputs behind the last) is asked for at an offset past the buffer's range, which returns zeros without
 // moving a byte, so that no load stands behind a branch and the waits count exactly.

@@ -128,9 +128,9 @@ template <class Num> int launch_few(const MoeFp4Gemm& p, int64_t R, hipStream_t 
     const int64_t most = R / 16 + p.E, tiles = most < R ? most : R, used = p.E < R ? p.E : R;   // (a tile holds a row at least)
     const int chunks = (p.K + few::CHUNK - 1) / few::CHUNK, cus = moe_device_cus();
     const bool narrow = tiles * ((p.N + 63) / 64) < cus;   // few column blocks: blocks of 16 columns give every compute unit one
-    // Waves that share a contraction: as many as the chip holds at once (by their registers, below; tiles as many as evenly spread rows fill, half of them partly), two chunks each at least.  One
-    // token of 4096 x 14336, 448 workgroups: 1 / 2 / 4 / 8 waves 25 / 19 / 15 / 20 us, the last in two rounds; 16 of one expert each 50 / 54 / 52 / 70; 666 rows of 1000 x 1368 17.2 / 17.2 / 19.9 / 27.
-    const int64_t expected = R / 16 + used / 2, groups = (expected > used ? expected : used) * (narrow ? (p.N + 15) / 16 : (p.N + 63) / 64);
+    // Waves that share a contraction: as many as the chip holds at once (by their registers, below; tiles as many as spread rows fill: evenly, or with half a tile more for each expert), two chunks each at least.  One
+    // token of 4096 x 14336, 448 workgroups: 1 / 2 / 4 / 8 waves 25 / 19 / 15 / 20 us, the last in two rounds; 16 of one expert each 50 / 54 / 52 / 70; 666 rows of 1000 x 1368 12.6 / 14.9 / 16.4 / 27.
+    const int64_t even = used * ((R + 16 * used - 1) / (16 * used)), uneven = R / 16 + used / 2, groups = (even > uneven ? even : uneven) * (narrow ? (p.N + 15) / 16 : (p.N + 63) / 64);
     const int64_t resident = (int64_t)cus * (narrow ? (p.quads ? 16 : 20) : p.quads ? 8 : 12);
     int waves = 1;
     while (waves < 8 && groups * waves * 2 <= resident && chunks >= 2 * waves) waves *= 2;
@@ -141,7 +141,7 @@ template <class Num> int launch_few(const MoeFp4Gemm& p, int64_t R, hipStream_t 
 
 int moe_launch_fp4_few_rows(MoeFp4Gemm p, int64_t R, hipStream_t stream)
 {
-    p.quads = p.K % (2 * few::CHUNK) == 0;   // (columns of other sizes are loaded group by group)
+    p.quads = (p.K + FP4_GROUP - 1) / FP4_GROUP % 8 == 0;   // whole lines of codes and scales; columns of other sizes are loaded group by group (666 rows of 1000 x 1368: 17.2 us, 12.6 in lines)
     p.y_vec = p.ldy % 4 == 0 && (uintptr_t)p.Y % 16 == 0;
     return p.f16 ? launch_few<NumF16>(p, R, stream) : launch_few<NumBf16>(p, R, stream);
 }

@@ -204,7 +204,7 @@ def test_rows_behind_the_last_group_are_left_as_they_were(dev):
 
 LARGER = [  # whole lines of codes (multiples of 256 inputs), narrow and wide, few rows and tiles, up to several rounds of tiles
     (24, 1024, 640, 3, 2), (9, 4096, 200, 2, 1), (1, 2560, 1408, 8, 2), (700, 512, 1032, 8, 2), (260, 768, 2056, 1, 1), (2000, 256, 264, 3, 2), (129, 520, 5000, 2, 1), (64, 8192, 24, 2, 2),
-    (333, 1368, 1000, 6, 2), (17, 96, 4104, 40, 4),
+    (333, 1368, 1000, 6, 2), (17, 96, 4104, 40, 4), (12, 1017, 40, 3, 2), (40, 250, 48, 2, 1), (20, 1000, 1368, 3, 2),
 ]
 
 
