@@ -193,7 +193,7 @@ template <class Num> __device__ __forceinline__ void route(const MoeDecode& p, C
         const int x = eb * 16 + (lane >> 2), e = x < p.E ? x : p.E - 1;
         w.c[0] = (uint32_t)(e * p.ldwg + 8 * few::quad_piece(lane)) * 2;
         f32x4_t acc[1][1] = {{(f32x4_t){0.f, 0.f, 0.f, 0.f}}};
-        few::stream<W, 1, false, 4, 4>(acc, w, rows, chunks * wave / WAVES, chunks * (wave + 1) / WAVES, scratch);
+        few::stream<W, 1, false, 4, 4>(acc, w, rows, wave, (chunks - wave + WAVES - 1) / WAVES, WAVES, scratch);
         *(f32x4_t*)(red + (wave * 64 + lane) * 4) = acc[0][0];
         __syncthreads();
         sum_logits(p, red, 256, logits, eb, 1, WAVES);
@@ -390,7 +390,7 @@ __global__ void __launch_bounds__(THREADS, 2) gate_up_kernel(const MoeDecode p)
             W w;
             gate_up_columns(p, w, e, n);
             f32x4_t acc[1][2] = {{(f32x4_t){0.f, 0.f, 0.f, 0.f}, (f32x4_t){0.f, 0.f, 0.f, 0.f}}};
-            few::stream<W, 1, false, 2, 2>(acc, w, rows, units * wave / WAVES, units * (wave + 1) / WAVES, scratch);
+            few::stream<W, 1, false, 2, 2>(acc, w, rows, wave, (units - wave + WAVES - 1) / WAVES, WAVES, scratch);
             float (*s)[2][64][4] = red[turn & 1];
             *(f32x4_t*)s[wave][0][lane] = acc[0][0];
             *(f32x4_t*)s[wave][1][lane] = acc[0][1];
@@ -549,7 +549,9 @@ __global__ void __launch_bounds__(THREADS) down_kernel(const MoeDecode p)
     constexpr int STEP = FP4 ? W::UNIT * few::CHUNK : 32;
     const int steps = (p.f + STEP - 1) / STEP;
     const int64_t total = (int64_t)nactive * steps;
-    const int shares = p.parts * WAVES, share = part * WAVES + wave;
+    // (the waves of a part take every eighth step, side by side in memory; where an expert has few, ranges of their own)
+    const bool side_by_side = FP4 && steps >= 2 * WAVES;
+    const int shares = side_by_side ? p.parts : p.parts * WAVES, share = side_by_side ? part : part * WAVES + wave;
     int64_t at = total * share / shares;
     const int64_t end = total * (share + 1) / shares;
     // the token that row r of the operand belongs to, and where its numbers lie
@@ -582,7 +584,8 @@ __global__ void __launch_bounds__(THREADS) down_kernel(const MoeDecode p)
             f32x4_t acc[1][4];
 #pragma unroll
             for (int nb = 0; nb < 4; ++nb) acc[0][nb] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-            few::stream<W, NA, true, HALVES ? 3 : 2, HALVES && W::UNIT == 1 ? 3 : 2>(acc, w, rows, s0, s1, smem + wave * SCRATCH);
+            const int step = side_by_side ? WAVES : 1, first = side_by_side ? s0 + wave : s0;
+            few::stream<W, NA, true, HALVES ? 3 : 2, HALVES && W::UNIT == 1 ? 3 : 2>(acc, w, rows, first, (s1 - first + step - 1) / step, step, smem + wave * SCRATCH);
             const float g = j >= 0 ? c.weight[token(i)][j] : 0.f;
 #pragma unroll
             for (int u = 0; u < UNITS; ++u)

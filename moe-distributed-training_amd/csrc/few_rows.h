@@ -198,18 +198,18 @@ template <int NA> struct Rows {
     }
 };
 
-// acc[m][nb] += rows m times columns nb over units [u0, u1) of W::UNIT chunks, DEPTH of them requested ahead, and the rows of AHEAD chunks (SUM: all row operands into acc[0]).  u0 and u1
-// are the same in every lane; scratch is the wave's own W::SCRATCH + Rows::SCRATCH bytes.
+// acc[m][nb] += rows m times columns nb over `count` units of W::UNIT chunks, `first` and every `step`th from there on, DEPTH of them requested ahead, and the rows of AHEAD chunks (SUM: all
+// row operands into acc[0]).  These numbers are the same in every lane; scratch is the wave's own W::SCRATCH + Rows::SCRATCH bytes.
 template <class W, int NA, bool SUM, int DEPTH, int AHEAD>
-__device__ __forceinline__ void stream(f32x4_t (&acc)[SUM ? 1 : NA][W::NB], const W& w, const Rows<NA>& rows, int u0, int u1, uint8_t* scratch)
+__device__ __forceinline__ void stream(f32x4_t (&acc)[SUM ? 1 : NA][W::NB], const W& w, const Rows<NA>& rows, int first, int count, int step, uint8_t* scratch)
 {
     constexpr int UNIT = W::UNIT;
     static_assert(DEPTH * UNIT % AHEAD == 0, "a chunk's place in the ring of rows is known when the loop is compiled");
     typename W::Stage ws[DEPTH];
     typename Rows<NA>::Stage as[AHEAD];
     // (the scheduler would gather the requests of a round behind its products: each stays where it is written)
-    auto fetch = [&](int d, int u) { w.load(ws[d], u); __builtin_amdgcn_sched_barrier(0); };
-    auto fetch_rows = [&](int a, int c) { rows.load(as[a], c); __builtin_amdgcn_sched_barrier(0); };
+    auto fetch = [&](int d, int u) { w.load(ws[d], first + u * step); __builtin_amdgcn_sched_barrier(0); };
+    auto fetch_rows = [&](int a, int c) { rows.load(as[a], (first + c / UNIT * step) * UNIT + c % UNIT); __builtin_amdgcn_sched_barrier(0); };
     auto multiply = [&](int d, int cc) {
         auto& x = as[(d * UNIT + cc) % AHEAD];
         if (cc == 0) w.ready(ws[d], scratch);
@@ -224,32 +224,32 @@ __device__ __forceinline__ void stream(f32x4_t (&acc)[SUM ? 1 : NA][W::NB], cons
             }
         __builtin_amdgcn_sched_barrier(0);
     };
-    const int last = u1 * UNIT;   // chunks from here on are not this wave's
+    const int last = count * UNIT;   // chunks from here on are not this wave's
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d)
-        if (u0 + d < u1) fetch(d, u0 + d);
+        if (d < count) fetch(d, d);
 #pragma unroll
     for (int a = 0; a < AHEAD; ++a)
-        if (u0 * UNIT + a < last) fetch_rows(a, u0 * UNIT + a);
-    int u = u0;
-    for (; u + 2 * DEPTH <= u1; u += DEPTH)
+        if (a < last) fetch_rows(a, a);
+    int u = 0;
+    for (; u + 2 * DEPTH <= count; u += DEPTH)
 #pragma unroll
         for (int d = 0; d < DEPTH; ++d) {
 #pragma unroll
             for (int cc = 0; cc < UNIT; ++cc) { multiply(d, cc); fetch_rows((d * UNIT + cc) % AHEAD, (u + d) * UNIT + cc + AHEAD); }
             fetch(d, u + DEPTH + d);
         }
-    for (; u < u1; u += DEPTH)
+    for (; u < count; u += DEPTH)
 #pragma unroll
         for (int d = 0; d < DEPTH; ++d) {
-            if (u + d >= u1) break;
+            if (u + d >= count) break;
 #pragma unroll
             for (int cc = 0; cc < UNIT; ++cc) {
                 multiply(d, cc);
                 const int c = (u + d) * UNIT + cc + AHEAD;
                 if (c < last) fetch_rows((d * UNIT + cc) % AHEAD, c);
             }
-            if (u + d + DEPTH < u1) fetch(d, u + d + DEPTH);
+            if (u + d + DEPTH < count) fetch(d, u + d + DEPTH);
         }
 }
 

@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(512) fp4_few_rows_kernel(const MoeFp4Gemm p)
         for (int nb = 0; nb < NB; ++nb) acc[mb][nb] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
     constexpr int UNIT = W::UNIT * few::CHUNK, SCRATCH = W::SCRATCH + few::Rows<MB>::SCRATCH;
     const int units = (p.K + UNIT - 1) / UNIT;
-    few::stream<W, MB, false, 2, 2>(acc, w, rows, units * wave / waves, units * (wave + 1) / waves, smem + wave * SCRATCH);
+    few::stream<W, MB, false, 2, 2>(acc, w, rows, wave, (units - wave + waves - 1) / waves, waves, smem + wave * SCRATCH);
     f32x4_t* red = (f32x4_t*)smem;   // [wave][MB * NB][64], in place of the operands
     static_assert(MB * NB * 1024 <= SCRATCH, "the sums fit where the operands were");
     if (waves > 1) {
