@@ -24,6 +24,11 @@ constexpr int B_STAGE = 16384;                       // forward: 256 columns x 6
 constexpr int S_STAGE = 1024;                        // scales: forward 256 columns x 4, backward 64 rows x 8
 constexpr int B_OFF = 2 * A_STAGE, S_OFF = B_OFF + 2 * B_STAGE, LDS_BYTES = S_OFF + 2 * S_STAGE;
 
+// Which places of its eight a row's pieces are dealt to: place = piece ^ turn(row).  A 16-byte read of LDS takes lanes 0 .. 3, 12 .. 15 with 20 .. 27 and the like at a time, rows of one piece
+// with those of the next lane group's: turn() gives {0, 1, 6, 7} and {2, 3, 4, 5} halves of their own, which neighbours one (backward) or two (forward) pieces apart keep.  (turn = row >> 1:
+// every forward read in two passes, 17 % of a compute unit's cycles.)
+__device__ __forceinline__ int turn(int row) { const int x = (row >> 1) & 7; return x ^ ((x & 2) << 1); }
+
 // four bytes per lane, global -> LDS at lds_addr + 4 * lane (load_to_lds_16 otherwise)
 __device__ __forceinline__ void load_to_lds_4(i32x4_t rsrc, uint32_t lane_off, uint32_t uniform_off, uint32_t lds_addr)
 {
@@ -71,16 +76,16 @@ __global__ void __launch_bounds__(THREADS, 2) fp4_tile_kernel(const MoeFp4Gemm p
     const int e = item.expert, nrows = (int)(item.row1 - item.row0), nblocks = (nrows + 15) / 16;
     const int64_t row0 = item.row0, n0 = (int64_t)item.nt * BN;
 
-    // ---- where this lane's pieces of the images come from.  X: rows of 128 bytes, 16-byte piece c of row r at place c ^ ((r >> 1) & 7); instruction j of wave w fills rows (4 j + w) * 8 ..
+    // ---- where this lane's pieces of the images come from.  X: rows of 128 bytes, 16-byte piece c of row r at place c ^ turn(r); instruction j of wave w fills rows (4 j + w) * 8 ..
     const int64_t base = p.x_grouped ? row0 : 0;
     uint32_t a_off[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const int r = (4 * j + wave) * 8 + (lane >> 3);
         const int64_t m = row0 + (r < nrows ? r : nrows - 1);   // rows past the tile re-read its last one
-        a_off[j] = (uint32_t)(((p.x_grouped ? m : load_idx(p.pos, m, p.pos64) / p.fan_out) - base) * p.ldx) * 2 + ((lane & 7) ^ ((r >> 1) & 7)) * 16;
+        a_off[j] = (uint32_t)(((p.x_grouped ? m : load_idx(p.pos, m, p.pos64) / p.fan_out) - base) * p.ldx) * 2 + ((lane & 7) ^ turn(r)) * 16;
     }
-    const int a_k = ((lane & 7) ^ ((4 * wave + (lane >> 4)) & 7)) * 8;   // this lane's first input within a stage (the same for every j)
+    const int a_k = ((lane & 7) ^ turn(8 * wave + (lane >> 3))) * 8;   // this lane's first input within a stage (the same for every j)
     const i32x4_t a_buf = make_buffer((const uint16_t*)p.X + base * p.ldx, RANGE);
     const i32x4_t b_buf = make_buffer(p.w.codes + e * p.w.sce, RANGE), s_buf = make_buffer(p.w.scales + e * p.w.sse, RANGE);
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)LDS_PTR(smem));
@@ -187,7 +192,7 @@ __global__ void __launch_bounds__(THREADS, 2) fp4_tile_kernel(const MoeFp4Gemm p
                 const int chunk = BWD ? 4 * j + q : 2 * q + j;
 #pragma unroll
                 for (int mb = 0; mb < NBLK; ++mb) {
-                    const bf16x8_t a = *(const bf16x8_t*)(a_lds + (mb * 16 + i) * 128 + (chunk ^ ((i >> 1) & 7)) * 16);
+                    const bf16x8_t a = *(const bf16x8_t*)(a_lds + (mb * 16 + i) * 128 + (chunk ^ turn(i)) * 16);
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb) acc[mb][nb] = Num::mfma(b[nb], a, acc[mb][nb]);
                 }
