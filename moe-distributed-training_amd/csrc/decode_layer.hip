@@ -10,6 +10,8 @@
 //
 // Both are bound by the weights of the chosen experts, each byte read once (few_rows.h).  All tokens of the batch are rows of the matrix operand, so a weight is read once however
 // many tokens chose its expert; rows of other tokens are computed in launch 1 and not stored, and are absent from launch 2.
+// Measured (launch 1 + launch 2, 4096 x 14336, 8 experts, top-2): one token in 16 bits 84 + 49 us (5.6 and 4.8 TB/s), in 4 bits 30 + 22.5; sixteen tokens in 4 bits 87 + 65 (5.7 and 3.9; their rows of h, read by
+// every tile, cost 10).  Of launch 1 the router takes 6 us (10 with 64 experts), of launch 2 the meeting of the parts 4.
 // h travels as two numbers of the activations' type, h and what its rounding lost (16 bits more), whose products are added: the result then carries one rounding, its own.
 #include "few_rows.h"
 #include "gemm_tiles.h"

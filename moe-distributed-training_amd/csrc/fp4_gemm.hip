@@ -1,6 +1,9 @@
 // Grouped product of 16-bit rows with 4-bit weights (fp4.h) over ragged expert groups, few rows per expert: the codes are streamed (few_rows.h).
 //
 //   Y[out_row(m)][n] = sum_k X[in_row(m)][k] W[e(m)][n][k]
+//
+// Bound by the codes (17 bytes per 32 weights) of the experts that hold a row: two rows of 4096 x 14336 15.2 us = 4.1 TB/s, of which 3 us are the launch, the look-up of the tile and its rows and the sum
+// over waves; sixteen rows of eight experts 50 us = 5.0 TB/s.
 #include "few_rows.h"
 #include "kernels.h"
 
