@@ -1,4 +1,4 @@
-// Grouped product of 16-bit rows with 4-bit weights (fp4.h) on the matrix cores, both directions, tiles of 128 rows x 256 columns:
+// Grouped product of 16-bit rows with 4-bit weights (fp4.h) on the matrix cores, both directions, tiles of 128 (or 112, or 96) rows x 256 columns:
 //
 //   forward:   Y[out_row(m)][n]  = sum_k X[in_row(m)][k] W[e(m)][n][k]
 //   backward:  Y[out_row(m)][k] = c[m] sum_n X[in_row(m)][n] W[e(m)][n][k]      (X: gradient rows, c: their gate weights or 1)
@@ -11,7 +11,7 @@
 //   halves per pair of rows make four operands of it.
 // Measured: 8192 rows of 8 experts x 4096 x 14336 forward 770 to 830 us by card = 1.16 to 1.25 PFLOP/s (matrix cores busy in 64 % of the cycles at 1.96 GHz; the library's dense product of 8192^3
 // runs at 1.27 to 1.32), 3000 rows of
-// 4096 x 4096 forward 126 us, backward 133 us: 416 tiles on 512 places, so compute units hold two or one of them.
+// 4096 x 4096 forward 120 us, backward 125 us: 416 and 512 tiles on 512 places, so compute units hold two or one of them.
 // Columns are dealt to the matrix instructions so that a lane ends up with 16 consecutive ones of a row.  Sums, gate weights and the rows that the caller sums further are fp32.
 #include "fp4.h"
 #include "gemm_tiles.h"
@@ -65,7 +65,7 @@ __device__ __forceinline__ void store16(void* Y, int64_t at, int dtype, const fl
             if (i < live) y[i] = (uint16_t)(o[i / 2] >> (16 * (i & 1)));
 }
 
-template <class Num, bool BWD>
+template <class Num, bool BWD, int ROWS>
 __global__ void __launch_bounds__(THREADS, 2) fp4_tile_kernel(const MoeFp4Gemm p)
 {
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(THREADS, 2) fp4_tile_kernel(const MoeFp4Gemm p
     const int len = BWD ? (int)p.N : p.K;                       // of the contraction
     const int G = (p.K + FP4_GROUP - 1) / FP4_GROUP;
     const int ntiles_n = (int)((cols + BN - 1) / BN), ktiles = (len + BK - 1) / BK;
-    const WorkItem item = decode_work_item<BM, 1>(p.offsets, p.off64, p.E, ntiles_n, ktiles, 1, p.num_cus);
+    const WorkItem item = decode_work_item<ROWS, 1>(p.offsets, p.off64, p.E, ntiles_n, ktiles, 1, p.num_cus);
     if (!item.valid) return;
     const int e = item.expert, nrows = (int)(item.row1 - item.row0), nblocks = (nrows + 15) / 16;
     const int64_t row0 = item.row0, n0 = (int64_t)item.nt * BN;
@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(THREADS, 2) fp4_tile_kernel(const MoeFp4Gemm p
             }
         }
     };
-    if (nblocks > 6) mainloop(std::integral_constant<int, 8>{});
+    if (ROWS > 96 && nblocks > 6) mainloop(std::integral_constant<int, ROWS == 112 ? 7 : 8>{});
     else if (nblocks > 4) mainloop(std::integral_constant<int, 6>{});
     else if (nblocks > 2) mainloop(std::integral_constant<int, 4>{});
     else mainloop(std::integral_constant<int, 2>{});
@@ -227,10 +227,10 @@ __global__ void __launch_bounds__(THREADS, 2) fp4_tile_kernel(const MoeFp4Gemm p
     }
 }
 
-template <class Num, bool BWD> int launch_typed(MoeFp4Gemm p, int64_t R, hipStream_t stream)
+template <class Num, bool BWD, int ROWS> int launch_rows(MoeFp4Gemm p, int64_t R, hipStream_t stream)
 {
     static std::atomic<bool> attr_set[MOE_MAX_DEVICES];
-    auto kern = fp4_tile_kernel<Num, BWD>;
+    auto kern = fp4_tile_kernel<Num, BWD, ROWS>;
     const int dev = moe_current_device();
     if (!attr_set[dev]) {
         if (hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, LDS_BYTES) != hipSuccess) return MOE_ERR_LAUNCH;
@@ -239,10 +239,27 @@ template <class Num, bool BWD> int launch_typed(MoeFp4Gemm p, int64_t R, hipStre
     p.num_cus = WGS_PER_CU * moe_device_cus();
     const int64_t cols = BWD ? p.K : p.N, ntiles = (cols + BN - 1) / BN;
     // an upper bound on the tiles (a tile holds a row at least), and a round for the last, partial one; surplus workgroups leave at once
-    const int64_t most = R / BM + p.E, grid = ((most < R ? most : R) * ntiles + p.num_cus + NXCD - 1) / NXCD * NXCD;
+    const int64_t most = R / ROWS + p.E, grid = ((most < R ? most : R) * ntiles + p.num_cus + NXCD - 1) / NXCD * NXCD;
     if (!moe_grid_fits(grid, THREADS)) return MOE_ERR_UNSUPPORTED;
     hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(THREADS), LDS_BYTES, stream, p);
     return moe_launch_status();
+}
+
+template <class Num, bool BWD> int launch_typed(const MoeFp4Gemm& p, int64_t R, hipStream_t stream)
+{
+    // Rows of a tile: by the tiles that fall to a compute unit and their rows, half a tile more for each expert than its rows fill.  A launch of a few tiles per compute unit gains by smaller ones that
+    // come out even; backward 112 rows too (forward their odd number of blocks cost what they gained).  128 rows / the choice, us, 8 experts, forward and backward: 2000 rows of 4096 x 4096 97 / 84 and 104 /
+    // 94, 3000 120 / 120 and 129 / 125, 4000 155 / 138 and 176 / 152, 8192 270 / 264 and 278 / 259; 4096 of 2048 x 2048 52 / 44 and 57 / 50; 800 of 4096 x 4096 64 / 57 and 79 / 69.  (96 rows where 128 are chosen:
+    // 3000 rows 140 and 160.)
+    const int64_t used = p.E < R ? p.E : R, ntiles = ((BWD ? p.K : p.N) + BN - 1) / BN, rows = (R + used - 1) / used, cus = moe_device_cus();
+    auto time = [&](int bm) {
+        const double tiles = (double)R / bm + 0.5 * used;
+        return ceil((tiles > used ? tiles : used) * ntiles / cus) * (rows < bm ? (rows + 31) / 32 * 32 : bm);
+    };
+    if (time(96) < 0.95 * time(128) && (!BWD || time(96) <= time(112))) return launch_rows<Num, BWD, 96>(p, R, stream);
+    if constexpr (BWD)
+        if (time(112) < 0.95 * time(128)) return launch_rows<Num, BWD, 112>(p, R, stream);
+    return launch_rows<Num, BWD, 128>(p, R, stream);
 }
 
 }  // namespace

@@ -342,3 +342,8 @@ def test_codes_behind_the_last_input_meet_nothing(dev, dtype):
         codes[..., 16:20], scales[..., 1] = 0, 254
         got = moe.parallel_linear_fp4(x.to(dev), codes.to(dev), scales.to(dev), *args)
         assert bool(torch.isfinite(got).all())
+
+
+@pytest.mark.parametrize("T,K,N,E,k", [(2000, 128, 1536, 2, 1), (1600, 96, 2560, 2, 2), (2500, 1536, 136, 4, 2), (1000, 2816, 72, 2, 1), (1900, 264, 1032, 3, 2), (1500, 2048, 72, 4, 2)])
+def test_launches_of_tiles_of_every_height(dev, T, K, N, E, k):
+    check_linear(dev, T, K, N, E, k, BF16)
