@@ -347,3 +347,24 @@ def test_codes_behind_the_last_input_meet_nothing(dev, dtype):
 @pytest.mark.parametrize("T,K,N,E,k", [(2000, 128, 1536, 2, 1), (1600, 96, 2560, 2, 2), (2500, 1536, 136, 4, 2), (1000, 2816, 72, 2, 1), (1900, 264, 1032, 3, 2), (1500, 2048, 72, 4, 2)])
 def test_launches_of_tiles_of_every_height(dev, T, K, N, E, k):
     check_linear(dev, T, K, N, E, k, BF16)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_rows_beyond_32_bit_offsets(dev, dtype):
+    """Rows of more than 2 GiB together: both directions give what they give for the halves."""
+    T, K, N = 540000, 2112, 16
+    codes, scales = (t.to(dev) for t in oracle.quantize(torch.randn(2, K, N, generator=torch.Generator().manual_seed(0))))
+    x = torch.randn(T, K, device=dev, dtype=dtype)
+    dout = torch.randn(T, N, device=dev, dtype=dtype)
+
+    def both(x, dout):
+        n = x.size(0)
+        ssi = torch.cat((torch.arange(0, n, 2, device=dev), torch.arange(1, n, 2, device=dev)))
+        sei, offs = torch.arange(2, device=dev).repeat_interleave(n // 2), torch.tensor([n // 2, n], device=dev)
+        v = x.detach().requires_grad_(True)
+        y = moe.parallel_linear_fp4(v, codes, scales, 1, sei, ssi, None, offs)
+        return y.detach(), torch.autograd.grad(y, v, dout)[0]
+    whole, h = both(x, dout), T // 2
+    for part in (slice(0, h), slice(h, T)):
+        for a, b in zip(whole, both(x[part], dout[part])):
+            assert torch.equal(a[part], b)

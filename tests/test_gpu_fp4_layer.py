@@ -277,3 +277,20 @@ def test_trained_around_4_bit_experts_then_serving_tokens(dev):
             few = block.decode(h[rows])[0]
             # the layer for many tokens rounds gate, up and h to the type, a half step each, this one does not
             assert float((few.float() - many[rows].float()).norm() / many[rows].float().norm()) <= 4 * 2.0 ** -8
+
+
+def test_decode_of_blocks_in_8_bits_and_with_a_bias(dev):
+    x = torch.randn(5, 128, generator=torch.Generator().manual_seed(1)).to(BF16).to(dev)
+    for bits in (8, 4, 16):
+        torch.manual_seed(0)
+        block = moe.ScatterMoEBlock(128, 192, 4, device=dev, bias=True, return_bias=True)
+        if bits != 16:
+            block.quantize_experts(bits=bits)
+        with torch.no_grad():
+            out, bias = block.decode(x)
+            want, _ = block(x)
+        assert bias is block.bias and out.shape == x.shape
+        if bits != 16:
+            assert torch.equal(out, want)
+        assert float((out.float() - want.float()).norm() / want.float().norm()) <= 4 * 2.0 ** -8
+        assert block.decode(x[:0])[0].shape == (0, 128)

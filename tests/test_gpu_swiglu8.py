@@ -203,3 +203,16 @@ def test_steps_in_graphs_between_eager_ones_and_on_two_streams(dev):
             got.append(torch.autograd.grad(moe.swiglu_8bit(*leaves[i]), leaves[i], sets[i][2]))
     torch.cuda.synchronize()
     assert all(torch.equal(u, v) for g, w in zip(got, want) for u, v in zip(g, w))
+
+
+def test_more_values_than_32_bits_count(dev):
+    rows, cols = 160000, 14336
+    gate, up, dh = (torch.empty(rows, cols, dtype=BF16, device=dev).normal_() for _ in range(3))
+    a, b = gate.requires_grad_(True), up.requires_grad_(True)
+    y = moe.swiglu_8bit(a, b)
+    ga, gb = torch.autograd.grad(y, (a, b), dh)
+    for part in (slice(0, 9), slice(149795, 149805), slice(rows - 9, rows)):   # (2^31 lies in row 149796)
+        u, v = (t[part].detach().clone().requires_grad_(True) for t in (gate, up))
+        z = moe.swiglu_8bit(u, v)
+        assert torch.equal(y[part], z)
+        assert all(torch.equal(p, q) for p, q in zip((ga[part], gb[part]), torch.autograd.grad(z, (u, v), dh[part])))
