@@ -52,18 +52,19 @@ bool fp4_sizes_ok(int64_t K, int64_t N, int E, int64_t scn, int64_t ssn)
     return K <= 0x3fffff && E <= 65535 && N * scn < MOE_FP4_RANGE && N * ssn < MOE_FP4_RANGE && N * packed_groups(groups_of(K)) < MOE_FP4_RANGE && packed_cols(N) * 256 < MOE_FP4_RANGE;
 }
 
-// Which of the two kernels a forward product takes, by their estimated times (us; the host knows the groups' sizes on average only).  Few rows: every 16 rows of an expert stream its codes, at 4.6
-// TB/s.  Tiles: rounds of two workgroups per compute unit, 0.55 us per 64 inputs and up to as much again for the rows, and the codes once.  Measured (8 experts, rows per expert: few rows / tiles):
-//   4096 x 14336   16: 58 / 60     24: 109 / 63    64: 199 / 77         4096 x 4096   16: 19 / 40    32: 31 / 42    48: 56 / 49    64: 62 / 51
-//   14336 x 4096   16: 60 / 134    32: 107 / 138   48: 190 / 173        1000 x 1368   16: 6.9 / 11.4    64: 12.8 / 16.3    128: 22.1 / 23.5         2048 x 512   128: 15 / 39
+// Which of the two kernels a forward product takes, by their estimated times (us; the host knows the groups' sizes on average only).  Few rows: every 16 rows of an expert, begun ones too, stream its
+// codes, at 4.6 TB/s.  Tiles: rounds of two workgroups per compute unit, 0.55 us per 64 inputs and up to as much again for the rows, and the codes once.  Measured (8 experts, rows per expert, give or
+// take three: few rows / tiles):
+//   4096 x 14336   8: 53 / 67    16: 82 / 67    24: 107 / 67       4096 x 4096   16: 24 / 40    32: 38 / 45    48: 48 / 47    64: 69 / 54       2048 x 2816   16: 11 / 19    64: 23 / 29
+//   14336 x 4096   16: 81 / 134    32: 138 / 171    48: 172 / 174    64: 251 / 194       1000 x 1368   16: 6.8 / 11.3    64: 9.4 / 17.5    128: 13.9 / 18.9       2048 x 512   256: 20 / 31
 bool fp4_few_rows(int64_t R, int E, int64_t K, int64_t N)
 {
     const int64_t used = E < R ? E : R;                    // groups that hold a row, at most
     const double rows = (double)R / used, codes = (double)used * N * groups_of(K) * 17 / 4.6e6;
-    const double few = 4 + codes * (rows > 16 ? rows / 16 : 1);
+    const double few = 4 + codes * (rows > 8 ? rows / 16 + 0.5 : 1);
     const int64_t tiles = (R / 128 + used) * ((N + 255) / 256), slots = 2 * (int64_t)moe_device_cus();
     const double tiled = 3 + (double)((tiles + slots - 1) / slots) * ((K + 63) / 64) * (0.55 + 0.5 * (rows < 128 ? rows / 128 : 1));
-    return few <= (tiled > codes + 3 ? tiled : codes + 3) || rows <= 16;
+    return few <= (tiled > codes + 3 ? tiled : codes + 3) || rows <= 8;
 }
 
 struct Kept { size_t codes, scales; };
