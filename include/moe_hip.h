@@ -340,7 +340,7 @@ int moe_swiglu8_bwd(const void* kept, size_t kept_size, const void* dh, int64_t 
                     void* stream);
 
 /* ---- the whole layer for a few tokens, two launches (no counterpart in the reference) ---------------------------
- * Router, softmax, top-k (ties to the lower expert; normalize: weights divided by their sum), gate and up projection, SwiGLU, down projection and weighted sum of at most 16 tokens, 256
+ * Router, softmax, top-k (by the fp32 scores, as moe_router_topk ranks: ties to the lower expert, NaN scores last and in expert order; normalize: weights divided by their sum), gate and up projection, SwiGLU, down projection and weighted sum of at most 16 tokens, 256
  * experts, 16 experts per token; bf16 or fp16 x and router weight wg (E, d); d and f multiples of 64.  out (T, d) of x's type, weights (T, k) fp32, indices (T, k).  Rows of x and wg start at
  * multiples of 16 bytes, out's at multiples of 8.  Expert weights: w1, w3, w2 (E, f, d) of x's type, contiguous; or codes and scales of 4-bit weights (above), contiguous: c1, c3 (E, f, d), c2
  * (E, d, f).  Every expert's matrix below 2 GiB. */

@@ -1,6 +1,6 @@
 // The whole MoE layer for the few tokens of a generation step (16 at most) in two launches:
 //
-//   logits = x Wg^T;  s = softmax(logits);  the k largest (ties to the lower expert), w_j = s_j / sum s  (or s_j);
+//   logits = x Wg^T;  s = softmax(logits), fp32;  the k largest s (ties to the lower expert), w_j = s_j / sum s  (or s_j);
 //   h_j = silu(x W1_j^T) * (x W3_j^T);      out = sum_j w_j (h_j W2_j^T)
 //
 // Launch 1 (gate_up_kernel): every workgroup computes the router for itself -- the router's weight stays in L2, and a launch of its own would cost more -- and then
@@ -78,22 +78,18 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v)
     with(std::integral_constant<int, DPP_ROW_BCAST31>{}, std::integral_constant<int, 0xc>{});
     return __builtin_amdgcn_readlane(v, 63);
 }
-__device__ __forceinline__ float wave_sum(float v)
+
+// a wave's own writes to LDS, read by its other lanes
+__device__ __forceinline__ void own_lds_done()
 {
-    auto with = [&](auto ctrl, auto rows) {
-        v += __uint_as_float(__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), decltype(ctrl)::value, decltype(rows)::value, 0xf, true));
-    };
-    with(std::integral_constant<int, DPP_ROW_SHR + 1>{}, std::integral_constant<int, 0xf>{});
-    with(std::integral_constant<int, DPP_ROW_SHR + 2>{}, std::integral_constant<int, 0xf>{});
-    with(std::integral_constant<int, DPP_ROW_SHR + 4>{}, std::integral_constant<int, 0xf>{});
-    with(std::integral_constant<int, DPP_ROW_SHR + 8>{}, std::integral_constant<int, 0xf>{});
-    with(std::integral_constant<int, DPP_ROW_BCAST15>{}, std::integral_constant<int, 0xa>{});
-    with(std::integral_constant<int, DPP_ROW_BCAST31>{}, std::integral_constant<int, 0xc>{});
-    return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), 63));
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 }
 
-// Softmax and choices of all tokens from their logits: a wave per token.
-__device__ __forceinline__ void choose(const MoeDecode& p, Chosen& c, const float* logits)
+// Softmax and choices of all tokens from their logits, which make room for the exponentials: a wave per token.  Experts are ranked by their fp32 scores, as the router of the other paths ranks them (softmax_topk_token of routing.hip, with
+// the exponentials added in expert order there too, so that equal logits get the same bits): scores that underflow or round to the same number are ties, and NaN scores lose to every number and
+// are taken in expert order.
+__device__ __forceinline__ void choose(const MoeDecode& p, Chosen& c, float* logits)
 {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     constexpr int PER = MAXE / 64;
@@ -102,24 +98,36 @@ __device__ __forceinline__ void choose(const MoeDecode& p, Chosen& c, const floa
         float v[PER];
         uint32_t key[PER], top = 0;
         for (int r = 0; r < PER; ++r) { v[r] = 0.f; key[r] = 0; }
-        // (the key of a taken or absent expert is 0)
 #pragma unroll
         for (int r = 0; r < PER; ++r)
             if (r < per && r * 64 + lane < p.E) {
                 v[r] = logits[t * MAXE + r * 64 + lane];
-                key[r] = order_of(v[r]);
-                top = key[r] > top ? key[r] : top;
+                const uint32_t o = order_of(v[r]);
+                top = o > top ? o : top;
             }
         float sum = 0.f;
         const uint32_t most = wave_max(top);
         const float shift = __uint_as_float(most >> 31 ? most & 0x7fffffffu : ~most);   // the largest logit
 #pragma unroll
         for (int r = 0; r < PER; ++r)
-            if (r < per && r * 64 + lane < p.E) {
-                v[r] = expf(v[r] - shift);
-                sum += v[r];
+            if (r < per) {
+                v[r] = r * 64 + lane < p.E ? expf(v[r] - shift) : 0.f;
+                logits[t * MAXE + r * 64 + lane] = v[r];
             }
-        sum = wave_sum(sum);
+        own_lds_done();
+        // (every lane adds all of them, from LDS: with moves between lanes 64 experts took 2 us more, 256 experts and 16 tokens 17)
+#pragma unroll 4
+        for (int e = 0; e < p.E; e += 4) {
+            const f32x4_t x = *(const f32x4_t*)(logits + t * MAXE + e);
+            sum += x[0]; sum += x[1]; sum += x[2]; sum += x[3];
+        }
+        // (the key of a taken or absent expert is 0, of a NaN score 1)
+#pragma unroll
+        for (int r = 0; r < PER; ++r)
+            if (r < per && r * 64 + lane < p.E) {
+                v[r] /= sum;
+                key[r] = v[r] >= 0.f ? __float_as_uint(v[r]) + 2 : 1;
+            }
         float total = 0.f;
         float chosen = 0.f;   // lane j keeps the weight of choice j
         int choice = 0;
@@ -138,7 +146,7 @@ __device__ __forceinline__ void choose(const MoeDecode& p, Chosen& c, const floa
                     if (hit != 0) {
                         const int l = __ffsll(hit) - 1;
                         e = r * 64 + l;
-                        s = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v[r]), l)) / sum;
+                        s = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v[r]), l));
                         if (lane == l) key[r] = 0;
                         found = true;
                     }
@@ -328,7 +336,7 @@ __global__ void __launch_bounds__(THREADS, 2) gate_up_kernel(const MoeDecode p)
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];   // every wave's scratch
     __shared__ Chosen c;
     __shared__ __attribute__((aligned(16))) float red[2][WAVES][2][64][4];   // sums of two jobs; before them the router's
-    __shared__ float logits[TOK * MAXE];
+    __shared__ __attribute__((aligned(16))) float logits[TOK * MAXE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, q = lane >> 4;
     if (threadIdx.x < MAXE / 32) c.used[threadIdx.x] = 0;   // (the router's barriers lie in between)
     uint8_t* scratch = smem + wave * SCRATCH;

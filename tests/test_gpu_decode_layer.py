@@ -310,3 +310,81 @@ def test_graphs_that_share_a_memory_pool(dev):
             torch.cuda.synchronize()
             got = outs[i].clone()
             assert torch.equal(got, calls[i]()), (trial, i)
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# the router of the few-token layer beside the framework's own
+# ---------------------------------------------------------------------------------------------------------------
+def route_both(dev, x, wg, k, f, normalize=True, bits=4):
+    """(weights, indices) of the few-token layer, and of the router that every other path takes."""
+    E, d = wg.shape
+    if bits == 16:
+        w = [torch.zeros(E, f, d, dtype=x.dtype) for _ in range(3)]
+    else:
+        w = [(torch.zeros(E, n, m // 2, dtype=torch.uint8), torch.full((E, n, m // 32), 120, dtype=torch.uint8)) for n, m in ((f, d), (d, f), (f, d))]
+    few = run(dev, x, wg, w, k, normalize, bits)
+    return few[1:], moe.megablocks_utils.router.router_forward(x.to(dev), wg.to(dev), k, normalize)[2:]
+
+
+def with_logits(logits, d, dtype, rest=None):
+    """x (T, d) and wg (E, d) whose logits are the given ones (numbers of the type), plus `rest` where given: sums of one or two exact products."""
+    T, E = logits.shape
+    x, wg = torch.zeros(T, d, dtype=dtype), torch.zeros(E, d, dtype=dtype)
+    at = torch.arange(T)
+    x[at, at] = 1
+    wg[:, :T] = logits.t().to(dtype)
+    assert torch.equal(wg[:, :T].double(), logits.t().double())
+    if rest is not None:
+        x[at, T + at] = 1
+        wg[:, T:2 * T] = rest.t().to(dtype)
+        assert torch.equal(wg[:, T:2 * T].double(), rest.t().double())
+    return x, wg
+
+
+@pytest.mark.parametrize("E,k,d,f", [(8, 4, 128, 64), (8, 8, 1024, 1088), (24, 6, 512, 1088), (64, 8, 192, 64), (200, 16, 4160, 64)])
+@pytest.mark.parametrize("normalize", [True, False])
+def test_scores_that_underflow_are_ties(dev, E, k, d, f, normalize):
+    """Experts are ranked by their fp32 scores: exp(-110) and less is 0 in fp32 (the least subnormal number is e^-103.3), so all but the first ones tie, and ties go to the lower
+    expert."""
+    g = torch.Generator().manual_seed(E)
+    T = 7
+    logits = -110.0 - torch.randint(0, 16, (T, E), generator=g).double()
+    best = [torch.randperm(E, generator=g)[:n % 3 + 1].tolist() for n in range(T)]
+    for t, b in enumerate(best):
+        for j, e in enumerate(b):
+            logits[t, e] = 8.0 - j
+    x, wg = with_logits(logits, d, BF16)
+    (ew, ei), (rw, ri) = route_both(dev, x, wg, k, f, normalize)
+    for t, b in enumerate(best):
+        assert ei[t].tolist() == (b + [e for e in range(E) if e not in b])[:k], t
+        assert not ew[t, len(b):].any()
+    assert torch.equal(ei, ri) and torch.equal(ew, rw)
+
+
+@pytest.mark.parametrize("E,k", [(8, 3), (16, 16), (64, 8)])
+def test_logits_that_round_to_one_score(dev, E, k):
+    """Neighbouring fp32 numbers below -1: their exponentials are spaced more widely than they are apart."""
+    g = torch.Generator().manual_seed(E)
+    T = 9
+    rest = torch.stack([torch.randperm(E, generator=g) for _ in range(T)]).double() * 2.0 ** -24
+    base = torch.full((T, E), -1.0).double()
+    base[torch.arange(T), torch.randint(0, E, (T,), generator=g)] = torch.arange(T).double() / 4
+    x, wg = with_logits(base, 128, BF16, rest)
+    (ew, ei), (rw, ri) = route_both(dev, x, wg, k, 64)
+    assert torch.equal(ei, ri) and torch.equal(ew, rw)
+
+
+@pytest.mark.parametrize("E,k", [(4, 2), (12, 5), (64, 8)])
+def test_tokens_without_finite_scores_take_experts_in_order(dev, E, k):
+    """A NaN among the logits, or an infinite one: every score of the token is NaN, which loses to no other, and its experts are the first ones; as in every other path."""
+    T, d = 6, 128
+    g = torch.Generator().manual_seed(E)
+    x, wg = with_logits(torch.randint(-8, 9, (T, E), generator=g).double(), d, BF16)
+    x[1, 100], wg[E - 1, 100] = 2.0 ** 100, 2.0 ** 100      # one logit overflows to infinity
+    x[2, 101], wg[2, 101] = -2.0 ** 100, 2.0 ** 100         # one is minus infinity: a score of 0
+    x[3, 102] = float("nan")
+    (ew, ei), (rw, ri) = route_both(dev, x, wg, k, 64)
+    for t in (1, 3):
+        assert ei[t].tolist() == list(range(k)) and torch.isnan(ew[t]).all()
+    assert torch.isfinite(ew[2]).all() and 2 not in ei[2].tolist()
+    assert torch.equal(ei, ri) and torch.equal(torch.nan_to_num(ew, 7.0), torch.nan_to_num(rw, 7.0))
