@@ -198,10 +198,20 @@ template <int NA> struct Rows {
     }
 };
 
+// a step's 32 products are summed by the instruction, the steps in fp32 or, where a sum decides between experts, in 64 bits
+struct Wide { double v[4]; };
+template <class Num> __device__ __forceinline__ void add_products(f32x4_t& a, bf16x8_t w, bf16x8_t x) { a = Num::mfma(w, x, a); }
+template <class Num> __device__ __forceinline__ void add_products(Wide& a, bf16x8_t w, bf16x8_t x)
+{
+    const f32x4_t p = Num::mfma(w, x, (f32x4_t){0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+    for (int r = 0; r < 4; ++r) a.v[r] += (double)p[r];
+}
+
 // acc[m][nb] += rows m times columns nb over `count` units of W::UNIT chunks, `first` and every `step`th from there on, DEPTH of them requested ahead, and the rows of AHEAD chunks (SUM: all
 // row operands into acc[0]).  These numbers are the same in every lane; scratch is the wave's own W::SCRATCH + Rows::SCRATCH bytes.
-template <class W, int NA, bool SUM, int DEPTH, int AHEAD>
-__device__ __forceinline__ void stream(f32x4_t (&acc)[SUM ? 1 : NA][W::NB], const W& w, const Rows<NA>& rows, int first, int count, int step, uint8_t* scratch)
+template <class W, int NA, bool SUM, int DEPTH, int AHEAD, class Acc>
+__device__ __forceinline__ void stream(Acc (&acc)[SUM ? 1 : NA][W::NB], const W& w, const Rows<NA>& rows, int first, int count, int step, uint8_t* scratch)
 {
     constexpr int UNIT = W::UNIT;
     static_assert(DEPTH * UNIT % AHEAD == 0, "a chunk's place in the ring of rows is known when the loop is compiled");
@@ -220,7 +230,7 @@ __device__ __forceinline__ void stream(f32x4_t (&acc)[SUM ? 1 : NA][W::NB], cons
             for (int nb = 0; nb < W::NB; ++nb) {
                 const bf16x8_t f = W::frag(ws[d], cc, nb, j);
 #pragma unroll
-                for (int m = 0; m < NA; ++m) acc[SUM ? 0 : m][nb] = W::Num::mfma(f, __builtin_bit_cast(bf16x8_t, x.f[m][j]), acc[SUM ? 0 : m][nb]);
+                for (int m = 0; m < NA; ++m) add_products<typename W::Num>(acc[SUM ? 0 : m][nb], f, __builtin_bit_cast(bf16x8_t, x.f[m][j]));
             }
         __builtin_amdgcn_sched_barrier(0);
     };

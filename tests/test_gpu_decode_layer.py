@@ -388,3 +388,28 @@ def test_tokens_without_finite_scores_take_experts_in_order(dev, E, k):
         assert ei[t].tolist() == list(range(k)) and torch.isnan(ew[t]).all()
     assert torch.isfinite(ew[2]).all() and 2 not in ei[2].tolist()
     assert torch.equal(ei, ri) and torch.equal(torch.nan_to_num(ew, 7.0), torch.nan_to_num(rw, 7.0))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("d,f,at", [(1024, 384, (0, 1, 2, 3)), (1024, 64, (0, 1, 2, 3)), (4096, 384, (12, 13, 14, 15)), (4224, 128, (0, 8, 16, 24))])
+def test_large_terms_that_cancel_do_not_hide_the_others(dev, d, f, at, bits, dtype):
+    """Logits are 2^16 r 2^-25 + 2^16 - 2^16 over 16 experts: 256 terms r 2^-17 between two that cancel, in chunks of 128 inputs of one wave's share.  A sum of 32 terms is exact in fp32 (and lost in a
+    fp32 sum that already holds 2^16: at most 15 * 2^-12 < half of its last place, 2^-8)."""
+    E, k, T = 16, 8, 3
+    g = torch.Generator().manual_seed(d + f)
+    ranks = torch.randperm(E, generator=g)
+    x, wg = torch.zeros(T, d, dtype=dtype), torch.zeros(E, d, dtype=dtype)
+    for t in range(T):
+        x[t, at[0] * 128 + 5], x[t, at[3] * 128 + 77] = 256, -256
+        x[t, at[1] * 128:at[1] * 128 + 128] = x[t, at[2] * 128:at[2] * 128 + 128] = 1
+    wg[:, at[0] * 128 + 5] = wg[:, at[3] * 128 + 77] = 256
+    for c in at[1:3]:
+        wg[:, c * 128:c * 128 + 128] = (ranks.double() * 2.0 ** -17).to(dtype)[:, None]
+    _, weights, idx = oracle.router(x, wg, k)
+    assert torch.equal(idx[0], ranks.argsort(descending=True)[:k])
+    (ew, ei), (rw, ri) = route_both(dev, x, wg, k, f, bits=bits)
+    assert torch.equal(ri.cpu().long(), idx)
+    assert torch.equal(ei.cpu().long(), idx)
+    # logits are exact; an exponential within 2^-23, a sum and two quotients on top
+    assert float(((ew.double().cpu() - weights) / weights).abs().max()) <= 24 * 2.0 ** -24
