@@ -79,13 +79,6 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v)
     return __builtin_amdgcn_readlane(v, 63);
 }
 
-// a wave's own writes to LDS, read by its other lanes
-__device__ __forceinline__ void own_lds_done()
-{
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
-
 // Softmax and choices of all tokens from their logits, which make room for the exponentials: a wave per token.  Experts are ranked by their fp32 scores, as the router of the other paths ranks them (softmax_topk_token of routing.hip, with
 // the exponentials added in expert order there too, so that equal logits get the same bits): scores that underflow or round to the same number are ties, and NaN scores lose to every number and
 // are taken in expert order.
@@ -114,7 +107,7 @@ __device__ __forceinline__ void choose(const MoeDecode& p, Chosen& c, float* log
                 v[r] = r * 64 + lane < p.E ? expf(v[r] - shift) : 0.f;
                 logits[t * MAXE + r * 64 + lane] = v[r];
             }
-        own_lds_done();
+        few::in_order();
         // (every lane adds all of them, from LDS: with moves between lanes 64 experts took 2 us more, 256 experts and 16 tokens 17)
 #pragma unroll 4
         for (int e = 0; e < p.E; e += 4) {

@@ -29,13 +29,23 @@ constexpr int STREAMED = 2;                  // non-temporal: nobody else reads 
 __device__ __forceinline__ fp4_u32x4_t load16(Buffer b, uint32_t lane_off, uint32_t off) { return __builtin_bit_cast(fp4_u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(b, lane_off, off, 0)); }
 __device__ __forceinline__ fp4_u32x4_t load16_streamed(Buffer b, uint32_t lane_off, uint32_t off) { return __builtin_bit_cast(fp4_u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(b, lane_off, off, STREAMED)); }
 
+// The lanes of a wave pass operands to each other through LDS of the wave's own.  The hardware takes a wave's accesses to LDS in order; this tells the compiler to leave them in that order, around every
+// exchange (lanes write what others read, and write again where others have read).  It costs no instruction.
+__device__ __forceinline__ void in_order()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // A block of 16 columns x 64 bytes, loaded with lane l at column l >> 2, piece quad_piece(l) of 16 bytes, as the operand's lane (i, g) holds it: through 1 KiB of LDS.  (The pieces'
 // places depend on the column so that 16 columns meet all banks once.)
 __device__ __forceinline__ int quad_piece(int lane) { return (lane & 3) ^ (lane >> 4); }
 __device__ __forceinline__ fp4_u32x4_t from_quads(fp4_u32x4_t v, uint8_t* scratch)
 {
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+    in_order();
     *(fp4_u32x4_t*)(scratch + lane * 16) = v;
+    in_order();
     return *(const fp4_u32x4_t*)(scratch + i * 64 + (g ^ (i >> 2)) * 16);
 }
 
@@ -83,8 +93,10 @@ __device__ __forceinline__ int line_piece(int lane, int h) { return (lane & 7) ^
 __device__ __forceinline__ void from_lines(fp4_u32x4_t (&v)[2], uint8_t* scratch)
 {
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+    in_order();
 #pragma unroll
     for (int h = 0; h < 2; ++h) *(fp4_u32x4_t*)(scratch + (h * 64 + lane) * 16) = v[h];
+    in_order();
 #pragma unroll
     for (int cc = 0; cc < 2; ++cc) v[cc] = *(const fp4_u32x4_t*)(scratch + i * 128 + ((cc * 4 + g) ^ ((i >> 1) & 7)) * 16);
 }
@@ -128,9 +140,11 @@ template <class Num_, int NB_, bool TWO> struct Fp4Quads {
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) from_lines(t.c[nb], scratch);   // (the same 2 KiB for every block: a wave's accesses to LDS happen in order)
         uint2* sc = (uint2*)(scratch + 2048);
+        in_order();
 #pragma unroll
         for (int m = 0; m < MATS; ++m)
             if (lane < EACH) sc[m * EACH + lane] = make_uint2(t.s[m][0], t.s[m][1]);
+        in_order();
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
             const uint2 v = sc[nb * 16 + i];
@@ -187,11 +201,13 @@ template <int NA> struct Rows {
     template <class W> __device__ __forceinline__ void ready(Stage& t, uint8_t* scratch) const
     {
         const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+        in_order();
 #pragma unroll
         for (int m = 0; m < NA; ++m) {
             uint8_t* s = scratch + m * 4096;
 #pragma unroll
             for (int j = 0; j < 4; ++j) *(fp4_u32x4_t*)(s + (4 * j + g) * 256 + (i ^ (4 * j + g)) * 16) = t.f[m][j];
+            in_order();
 #pragma unroll
             for (int j = 0; j < 4; ++j) t.f[m][j] = *(const fp4_u32x4_t*)(s + i * 256 + (W::piece(j, g) ^ i) * 16);
         }
