@@ -413,3 +413,20 @@ def test_large_terms_that_cancel_do_not_hide_the_others(dev, d, f, at, bits, dty
     assert torch.equal(ei.cpu().long(), idx)
     # logits are exact; an exponential within 2^-23, a sum and two quotients on top
     assert float(((ew.double().cpu() - weights) / weights).abs().max()) <= 24 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("T,d,f,E,k", KEPT + [(8, 2048, 1024, 64, 8), (1, 512, 4160, 2, 1), (11, 3584, 1536, 4, 2)])
+def test_layer_of_many_blocks_in_4_bits_of_either_type(dev, T, d, f, E, k, dtype):
+    """Scales 117 to 122 are exact in both types."""
+    x, wg, q = make_codes(T, d, f, E)
+    x, wg = x.to(dtype), wg.to(dtype)
+    w1, w2, w3 = (oracle.weights(*t, n) for t, n in zip(q, (d, f, d)))
+    want, weights, idx, terms, back = oracle.layer(x, wg, w1, w3, w2, k)
+    out, ew, ei = run(dev, x, wg, q, k, bits=4)
+    assert out.dtype == dtype and torch.equal(ei.cpu().long(), idx)
+    lt = 2 * ((d + 8) * (x.double().abs() @ wg.double().abs().t()).amax() + 16) * 2.0 ** -24
+    assert float(((ew.double().cpu() - weights) / weights).abs().max()) <= lt
+    w2_sum = sum((w2[idx[:, j]].abs().sum(-1) * weights[:, j, None]) for j in range(k))
+    over = (out.double().cpu() - want).abs() - slack_of(want, terms, back, w2_sum, d, f, dtype) - lt * terms
+    assert float(over.max()) <= 0

@@ -368,3 +368,62 @@ def test_rows_beyond_32_bit_offsets(dev, dtype):
     for part in (slice(0, h), slice(h, T)):
         for a, b in zip(whole, both(x[part], dout[part])):
             assert torch.equal(a[part], b)
+
+
+# Tiles of 128, 96, 112 (backward) rows over more than a whole round of the card's places (two per compute unit): tiles of the whole rounds and of the last, partial one are dealt differently
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("T,K,N,E,k", [(4096, 264, 3800, 8, 2), (4100, 3800, 264, 8, 2), (6000, 72, 2816, 5, 2), (4096, 4096, 72, 8, 2)])
+def test_several_rounds_of_tiles(dev, dtype, T, K, N, E, k):
+    check_linear(dev, T, K, N, E, k, dtype)
+
+
+@pytest.mark.parametrize("T,K,N,E,k", [(2000, 128, 1536, 2, 1), (1900, 264, 1032, 3, 2), (1500, 2048, 72, 4, 2), (2500, 1536, 136, 4, 2)])
+def test_launches_of_tiles_of_every_height_in_fp16(dev, T, K, N, E, k):
+    check_linear(dev, T, K, N, E, k, F16)
+
+
+def every_weight():
+    """Every code under every scale: codes (16, 256) and what they stand for."""
+    c, s = torch.arange(16).repeat(256, 1).t().contiguous(), torch.arange(256).repeat(16, 1)
+    return c, s, oracle.LEVELS[c & 7] * torch.where(c >= 8, -1.0, 1.0).double() * torch.where(s == 255, torch.full(s.shape, float("nan")).double(), torch.pow(torch.tensor(2.0).double(), s.double() - 127))
+
+
+def same_weights(got, want):
+    """Equal numbers; NaN where NaN is wanted."""
+    got, want = got.double().cpu(), want.double()
+    return torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(torch.nan_to_num(got, 0.0, 1e300, -1e300), torch.nan_to_num(want, 0.0, 1e300, -1e300))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("T", [1, 40, 300])
+def test_every_code_under_every_scale(dev, dtype, T):
+    """Experts of one input and 4096 outputs: the result of a row of 1 is the weights as numbers of the type, rounded as a conversion of the weight rounds.  fp16: exact for scales from 104 to 140."""
+    c, s, w = every_weight()
+    codes = torch.zeros(1, 4096, 16, dtype=torch.uint8)
+    codes[0, :, 0] = c.flatten().to(torch.uint8)
+    i = torch.arange(T, device=dev)
+    y = moe.parallel_linear_fp4(torch.ones(T, 1, dtype=dtype, device=dev), codes.to(dev), s.flatten().view(1, 4096, 1).to(torch.uint8).to(dev), 1, torch.zeros_like(i), i, None,
+                                torch.tensor([T], device=dev))
+    want = w.flatten().to(dtype)
+    exact = (s.flatten() >= 104) & (s.flatten() <= 140)
+    assert torch.equal(want.double()[exact], w.flatten()[exact])
+    for row in (0, T - 1):
+        bad = (y[row].cpu() != want) & ~(torch.isnan(y[row].cpu()) & torch.isnan(want))
+        assert same_weights(y[row], want), [(int(a), int(b), float(p), float(q)) for a, b, p, q in zip(c.flatten()[bad][:8], s.flatten()[bad][:8], y[row].cpu()[bad][:8], want[bad][:8])]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_every_code_under_every_scale_backward(dev, dtype):
+    """Experts of one output: the gradient of a row is that output's weights, 32 of a scale (codes 0 to 15 twice)."""
+    c, s, w = every_weight()
+    both = c.t().repeat(1, 2)                                   # (256 groups, 32 inputs)
+    codes = (both[:, 0::2] + 16 * both[:, 1::2]).to(torch.uint8).view(1, 1, 256 * 16)
+    x = torch.zeros(9, 256 * 32, dtype=dtype, device=dev, requires_grad=True)
+    i = torch.arange(9, device=dev)
+    y = moe.parallel_linear_fp4(x, codes.to(dev), torch.arange(256).view(1, 1, 256).to(torch.uint8).to(dev), 1, torch.zeros_like(i), i, None, torch.tensor([9], device=dev))
+    dx, = torch.autograd.grad(y, x, torch.ones(9, 1, dtype=dtype, device=dev))
+    want = w.t().repeat(1, 2).flatten().to(dtype)
+    for row in (0, 8):
+        bad = (dx[row].cpu() != want) & ~(torch.isnan(dx[row].cpu()) & torch.isnan(want))
+        assert same_weights(dx[row], want), [(int(a), int(b), float(p), float(q)) for a, b, p, q in zip(both.flatten()[bad][:8], torch.arange(256).repeat_interleave(32)[bad][:8],
+                                                                                                         dx[row].cpu()[bad][:8], want[bad][:8])]
