@@ -11,8 +11,10 @@
 // Both are bound by the weights of the chosen experts, each byte read once (few_rows.h).  All tokens of the batch are rows of the matrix operand, so a weight is read once however
 // many tokens chose its expert; rows of other tokens are computed in launch 1 and not stored, and are absent from launch 2.
 // Measured (launch 1 + launch 2, 4096 x 14336, 8 experts, top-2): one token in 16 bits 84 + 49 us (5.6 and 4.8 TB/s), in 4 bits 30 + 22.5; sixteen tokens in 4 bits 87 + 65 (5.7 and 3.9; their rows of h, read by
-// every tile, cost 10).  Of launch 1 the router takes 6 us (10 with 64 experts), of launch 2 the meeting of the parts 4.
-// h travels as two numbers of the activations' type, h and what its rounding lost (16 bits more), whose products are added: the result then carries one rounding, its own.
+// every tile, cost 10).  Of launch 1 the router takes 6 us (11 with 64 experts), of launch 2 the meeting of the parts 4.
+// h travels as two numbers of the activations' type, h and what its rounding lost, whose products are added: h to 2^-17 of itself in bf16; in fp16 to 2^-23, or to 2^-25 where that is more (half the
+// subnormal step), and infinite beyond 65504.  Besides that the result carries one rounding, its own.  (A third number would be half as many products and
+// bytes of rows again; for the lack of it 10 of a bf16 result's 4096 values round the other way, at the same error.)
 #include "few_rows.h"
 #include "gemm_tiles.h"
 #include "kernels.h"

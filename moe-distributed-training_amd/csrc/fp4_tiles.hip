@@ -9,9 +9,8 @@
 //   Forward, codes run along the contraction: a lane reads 8 bytes of its column (16 inputs of one scale) per 64 steps; its inputs are 16 g + 8 j .. + 7, and so are those of the row operand.
 //   Backward, the contraction runs over n, so a lane's 8 weights lie in 8 rows with a scale each: it reads two bytes of each (four columns), converts, and two moves of 16-bit
 //   halves per pair of rows make four operands of it.
-// Measured: 8192 rows of 8 experts x 4096 x 14336 forward 770 to 830 us by card = 1.16 to 1.25 PFLOP/s (matrix cores busy in 64 % of the cycles at 1.96 GHz; the library's dense product of 8192^3
-// runs at 1.27 to 1.32), 3000 rows of
-// 4096 x 4096 forward 120 us, backward 125 us: 416 and 512 tiles on 512 places, so compute units hold two or one of them.
+// Measured: 8192 rows of 8 experts x 4096 x 14336 forward 770 to 830 us by card = 1.16 to 1.25 PFLOP/s (matrix cores busy in 64 % of the cycles at 1.96 GHz; the library's dense product of
+// these sizes runs at 1.52), 3000 rows of 4096 x 4096 forward 120 us, backward 125 us: 416 and 512 tiles on 512 places, so compute units hold two or one of them.
 // Columns are dealt to the matrix instructions so that a lane ends up with 16 consecutive ones of a row.  Sums, gate weights and the rows that the caller sums further are fp32.
 #include "fp4.h"
 #include "gemm_tiles.h"

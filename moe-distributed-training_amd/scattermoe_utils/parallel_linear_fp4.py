@@ -30,7 +30,7 @@ def parallel_linear_fp4(inputs, expert_codes, weight_scales, k, sorted_expert_id
                         expert_offsets, gates=None, grouped_in=False, grouped_out=False):
     """``parallel_linear`` over 4-bit weights: inputs (rows, K) bf16, fp16 or fp32; expert_codes and weight_scales as
     ``quantize_expert_weights_fp4`` returns them, of any strides (codes whose rows are not contiguous and 16-byte aligned are copied
-    within the call); the other arguments as in ``parallel_linear``.  With fp16 inputs the weights are numbers of fp16: scales from 104
+    within the call, and with 16-bit inputs the scales where ceil(K / 32) or a stride is no multiple of 4); the other arguments as in ``parallel_linear``.  With fp16 inputs the weights are numbers of fp16: scales from 104
     to 140 are exact, beyond them weights round, or overflow to infinity.  Every assignment has to belong to an expert: rows of the
     result that no group covers are not written.  Gradients: of ``inputs`` and ``gates``."""
     return entry("linear_fp4")(inputs, expert_codes, weight_scales, k, sorted_expert_idxs, sorted_scattered_idxs, expert_offsets, gates, grouped_in,
