@@ -307,7 +307,8 @@ int moe_mlp_int8_bwd(const void* dy, int64_t lddy, int dtype, int dy_grouped, in
 /* ---- expert products over 4-bit weights (no counterpart in the reference) --------------------------------------
  * A weight is a code of one sign, two exponent and one mantissa bit (0, 0.5, 1, 1.5, 2, 3, 4, 6; bit 3 is the sign) times 2^(s - 127), s the scale byte that it shares with the
  * 31 others of its group: 32 consecutive inputs of one output column, of an expert's inputs 0.. on.  s = 255 is NaN.  codes (E, N, ceil(K/32) * 16) bytes: byte b of a row holds inputs
- * 2b (lower half) and 2b + 1; those behind K are zeros.  scales (E, N, ceil(K/32)) bytes.  Strides count bytes; rows of codes start at multiples of 16.
+ * 2b (lower half) and 2b + 1; those behind K are zeros.  scales (E, N, ceil(K/32)) bytes.  Strides count bytes and are
+ * not negative; rows of codes start at multiples of 16.
  *
  * moe_fp4_quantize_weights: (E,K,N) weights of any strides -> the nearest codes (the even one of two) under the least power of two that leaves the group's largest magnitude at
  * 7 units or below.  A group of zeros gets the scale 0, one that holds an infinity or a NaN the scale 255 and codes 0. */

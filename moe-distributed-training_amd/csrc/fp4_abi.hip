@@ -12,8 +12,11 @@ inline bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
 inline int64_t groups_of(int64_t K) { return (K + 31) / 32; }
 #define TRY(call) do { const int rc_ = (call); if (rc_ != MOE_OK) return rc_; } while (0)
 
-// rows of codes that 16-byte loads take, and scales that lie one after the other
-bool weights_ok(const MoeFp4Weights& w) { return w.codes && w.scales && aligned16(w.codes) && w.sce % 16 == 0 && w.scn % 16 == 0; }
+// rows of codes that 16-byte loads take, and scales that lie one after the other; offsets are unsigned
+bool weights_ok(const MoeFp4Weights& w)
+{
+    return w.codes && w.scales && aligned16(w.codes) && w.sce >= 0 && w.scn >= 0 && w.sse >= 0 && w.ssn >= 0 && w.sce % 16 == 0 && w.scn % 16 == 0;
+}
 
 // rows that 16-byte loads take as they are, within their offsets; otherwise they are packed in the order of the product
 bool rows_ok(const void* x, int64_t ldx, int64_t x_rows, int64_t cols, int x_grouped)

@@ -206,6 +206,15 @@ def test_c_entries_refuse_on_the_host():
     assert q(0, 4, 64, 128, 2, 16) == 0 and q(17, 4, 64, 128, 2, 16) == 0 and q(4, 4, 64, 128, 5, 16) == 0 and q(4, 257, 64, 128, 2, 4) == 0
 
 
+def test_c_entries_refuse_strides_below_zero():
+    """Offsets into an expert's codes and scales are unsigned: a negative pitch of 16-bit products would read zeros (stand-ins as above)."""
+    from moe_distributed_training_amd._lib import lib
+    for dt in (0, 1, 2):
+        for sce, scn, sse, ssn in ((-4096, 32, 256, 4), (4096, -32, 256, 4), (4096, 32, -256, 4), (4096, 32, 256, -4)):
+            assert lib.moe_linear_fp4_fwd(16, 64, 8, dt, 16, sce, scn, 16, sse, ssn, 16, 128, dt, 16, 0, 16, 0, 2, 16, 64, 128, 2, 0, 0, 256, 1 << 40, None) == -1
+            assert lib.moe_linear_fp4_bwd(16, 128, 8, dt, 0, 2, None, 0, 16, sce, scn, 16, sse, ssn, 16, 64, dt, 0, 16, 0, 16, 0, 2, 16, 64, 128, 256, 1 << 40, None) == -1
+
+
 def test_block_refusals_on_the_host():
     block = moe.ScatterMoEBlock(64, 128, 2, dtype=BF16)
     for match, kw in (("8 or 4 bits", dict(bits=2)), ("goes with experts in 4 bits", dict(keep_8bit=True)), ("goes with experts in 4 bits", dict(bits=8, keep_8bit=True))):
