@@ -427,3 +427,14 @@ def test_every_code_under_every_scale_backward(dev, dtype):
         bad = (dx[row].cpu() != want) & ~(torch.isnan(dx[row].cpu()) & torch.isnan(want))
         assert same_weights(dx[row], want), [(int(a), int(b), float(p), float(q)) for a, b, p, q in zip(both.flatten()[bad][:8], torch.arange(256).repeat_interleave(32)[bad][:8],
                                                                                                          dx[row].cpu()[bad][:8], want[bad][:8])]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_weights_of_no_output_columns(dev, dtype):
+    """Sums of nothing: empty rows, and gradients of zeros."""
+    x, _, _, (sei, ssi, offs, gw), _ = make(6, 64, 32, 3, 2, dtype)
+    xd, gd = x.to(dev).requires_grad_(True), gw.to(dev, dtype).requires_grad_(True)
+    y = moe.parallel_linear_fp4(xd, torch.empty(3, 0, 32, dtype=torch.uint8, device=dev), torch.empty(3, 0, 2, dtype=torch.uint8, device=dev), 2, sei.to(dev), ssi.to(dev), None, offs.to(dev), gd)
+    assert y.shape == (6, 0)
+    dx, dg = torch.autograd.grad(y.sum(), (xd, gd))
+    assert dx.shape == (6, 64) and dg.shape == (6, 2) and not dx.any() and not dg.any()
